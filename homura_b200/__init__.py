@@ -41,6 +41,7 @@ class DType(enum.IntEnum):
     U8 = 7
     Q4_K = 8
     Q6_K = 9
+    MXFP4 = 10
 
 
 class HomuraError(RuntimeError):
@@ -157,6 +158,19 @@ SIGNATURES = {
     "hm_gqa_write": (_i32, [_vp, _i32, _i32, _i32, _i32, _i32, _i32, _vp, _vp, C.c_float, C.c_float, C.c_float, _i32, _vp, _i32, C.c_float, _vp, _vp, _i32, _vp, _i32, _i32, _vp, _vp, _vp, _vp]),
     "hm_gqa_attn_paged": (_i32, [_vp, _vp, _vp, _i32, _vp, _i32, _i32, _vp, _vp, _i32, _i32, _i32, _i32, _i32, _vp, _i32, _i32, _vp, _vp]),
     "hm_post_norm_route": (_i32, [_vp, _vp, _vp, _i32, _i32, _vp, C.c_float, C.c_float, _vp, _vp, _i32, _i32, _i32, _vp, _vp, _vp, _vp]),
+    "hm_image_bytes": (C.c_size_t, [_i32, _i32, _i32]),
+    "hm_image_pack": (_i32, [_vp, _i32, _i32, _i32, C.c_size_t, _i32, _i32, _vp, _vp]),
+    "hm_image_unpack": (_i32, [_vp, _i32, _i32, _i32, _vp, _i32, C.c_size_t, _vp]),
+    "hm_image_from_blocks": (_i32, [_vp, _i32, _i32, _vp, _vp]),
+    "hm_gemm_image": (_i32, [_vp, _vp, _i32, _i32, _i32, _i32, _vp, _i32, C.c_size_t, _vp]),
+    "hm_gemv_mx4": (_i32, [_vp, _i32, C.c_size_t, _vp, _i32, _i32, _i32, _vp, _i32, C.c_size_t, _vp]),
+    "hm_expert_plan_ints": (C.c_size_t, [_i32, _i32]),
+    "hm_expert_plan_rows": (_i32, [_i32, _i32]),
+    "hm_expert_plan": (_i32, [_vp, _i32, _i32, _vp, _vp]),
+    "hm_expert_pack": (_i32, [_vp, _i32, _i32, C.c_size_t, _i32, _vp, _i32, _i32, _i32, _i32, _vp, _vp]),
+    "hm_expert_gemm": (_i32, [_vp, _vp, _i32, _vp, _i32, _i32, _i32, _i32, _vp, _i32, C.c_size_t, _vp]),
+    "hm_expert_gemv": (_i32, [_vp, _i32, C.c_size_t, _vp, _vp, _i32, _i32, _i32, _i32, _i32, _vp, _i32, C.c_size_t, _vp]),
+    "hm_expert_sum": (_i32, [_vp, _i32, _vp, _vp, _i32, _i32, _i32, _i32, _vp, _vp, _i32, _vp]),
     "hm_argmax": (_i32, [_vp, _i32, _i32, _vp, _vp]),
     "hm_dev_alloc": (_i32, [C.c_size_t, C.POINTER(_vp)]),
     "hm_dev_free": (_i32, [_vp]),
@@ -706,6 +720,212 @@ def qknorm_rope(x, cos_rows, sin_rows, norm_w=None, eps: float = 1e-6) -> np.nda
     nw = None if norm_w is None else np.ascontiguousarray(norm_w, dtype=np.float32)
     _check(lib.hm_qknorm_rope(_ptr(x), rows, heads, hd, _ptr(nw), eps, _ptr(c), _ptr(s), None))
     return x
+
+
+# ---- operand images (4-bit microscaled floats, bf16) and products grouped by expert ------------------
+#
+# Host mode: numpy arrays in, numpy arrays out; bf16 rows are uint16 bit patterns.  Device mode (asynchronous): x=(addr, rows), the other
+# arguments integer device addresses, sizes and types given; rows may be `ld` elements apart.
+
+
+def _rows_in(x):
+    """(contiguous [rows, K] array, its DType) of f32 rows or bf16 bits."""
+    x = np.atleast_2d(np.asarray(x))
+    bits = x.dtype == np.uint16
+    return np.ascontiguousarray(x, dtype=np.uint16 if bits else np.float32), DType.BF16 if bits else DType.F32
+
+
+def _rows_out(shape, dtype) -> np.ndarray:
+    return np.zeros(shape, np.uint16 if dtype == DType.BF16 else np.float32)
+
+
+def image_bytes(dtype: DType, rows: int, K: int) -> int:
+    """Bytes of an image of `rows` rows of K values (DType.MXFP4 or DType.BF16)."""
+    return int(load_library().hm_image_bytes(int(dtype), rows, K))
+
+
+def expert_plan_ints(pairs: int, experts: int) -> int:
+    """int32 words of a plan (expert_plan)."""
+    return int(load_library().hm_expert_plan_ints(pairs, experts))
+
+
+def expert_plan_rows(pairs: int, experts: int) -> int:
+    """Rows of an image that is packed with a plan."""
+    return int(load_library().hm_expert_plan_rows(pairs, experts))
+
+
+def _image_out(dtype, rows, K) -> np.ndarray:
+    n = image_bytes(dtype, rows, K)
+    if n == 0:
+        raise HomuraError(HM_ERR_INVALID, "an image has rows, values, and the type MXFP4 or BF16")
+    buf = np.zeros(n + 16, np.uint8)
+    at = -buf.ctypes.data % 16
+    return buf[at : at + n]
+
+
+def _image_in(image) -> np.ndarray:
+    image = np.ascontiguousarray(image, dtype=np.uint8)
+    if image.ctypes.data % 16:
+        buf = np.empty(image.size + 16, np.uint8)
+        at = -buf.ctypes.data % 16
+        buf[at : at + image.size] = image.reshape(-1)
+        image = buf[at : at + image.size]
+    return image
+
+
+def _fits(image, count, dtype, rows, K, what):
+    if image.size != count * image_bytes(dtype, rows, K) or image.size == 0:
+        raise HomuraError(HM_ERR_INVALID, f"{what} does not match its sizes")
+
+
+def image_pack(x, dtype: DType, K: Optional[int] = None, x_dtype=DType.F32, ldx: Optional[int] = None, glu: bool = False, plan=None, pairs: int = 0, experts: int = 0, top: int = 1, image=None, stream=None):
+    """Rows -> image; glu: rows of 2 K values, silu(first K) * last K.  With a plan the rows go where it puts their pairs
+    (pair p is row p // top of x), else each to its own place."""
+    lib = load_library()
+    host = not isinstance(x, tuple)
+    if host:
+        xa, x_dtype = _rows_in(x)
+        rows, ldx = xa.shape
+        K = ldx // 2 if glu else ldx
+        if plan is not None:
+            plan, pairs = np.ascontiguousarray(plan, dtype=np.int32), rows * top
+            if plan.size != expert_plan_ints(pairs, experts):
+                raise HomuraError(HM_ERR_INVALID, "the plan does not match the pairs and experts")
+        image = _image_out(dtype, rows if plan is None else expert_plan_rows(pairs, experts), K)
+    else:
+        xa, rows = x
+        ldx = ldx or (2 * K if glu else K)
+        if plan is not None and rows * top != pairs:
+            raise HomuraError(HM_ERR_INVALID, "a plan's pairs are top times the rows")
+    if plan is None:
+        _check(lib.hm_image_pack(_ptr(xa), int(x_dtype), rows, K, ldx, int(glu), int(dtype), _ptr(image), _ptr(stream)))
+    else:
+        _check(lib.hm_expert_pack(_ptr(xa), int(x_dtype), K, ldx, int(glu), _ptr(plan), pairs, experts, top, int(dtype), _ptr(image), _ptr(stream)))
+    return image if host else None
+
+
+def image_unpack(image, dtype: DType, K: int, rows: Optional[int] = None, out=None, out_dtype: DType = DType.F32, ldo: Optional[int] = None, stream=None):
+    """The values [rows, K] an image stands for.  Device mode: image=(addr, rows)."""
+    lib = load_library()
+    if isinstance(image, tuple):
+        (ia, rows) = image
+        _check(lib.hm_image_unpack(_ptr(ia), int(dtype), rows, K, _ptr(out), int(out_dtype), ldo or K, _ptr(stream)))
+        return None
+    im = _image_in(image)
+    _fits(im, 1, dtype, rows, K, "the image")
+    o = _rows_out((rows, K), out_dtype)
+    _check(lib.hm_image_unpack(_ptr(im), int(dtype), rows, K, _ptr(o), int(out_dtype), K, None))
+    return o
+
+
+def image_from_blocks(blocks, K: int, image=None, stream=None):
+    """GGUF blocks [rows, K / 32, 17] of 4-bit microscaled floats -> MXFP4 image.  Device mode: blocks=(addr, rows)."""
+    lib = load_library()
+    if isinstance(blocks, tuple):
+        (ba, rows) = blocks
+        _check(lib.hm_image_from_blocks(_ptr(ba), rows, K, _ptr(image), _ptr(stream)))
+        return None
+    b = np.ascontiguousarray(blocks, dtype=np.uint8)
+    rows = b.size // (17 * max(K // 32, 1))
+    im = _image_out(DType.MXFP4, rows, K)
+    _check(lib.hm_image_from_blocks(_ptr(b), rows, K, _ptr(im), None))
+    return im
+
+
+def gemm_image(x_image, w_image, N: int, dtype: DType, K: int, M: Optional[int] = None, y=None, y_dtype: DType = DType.F32, ldy: Optional[int] = None, stream=None):
+    """y [M, N] = x @ W^T from two images of one type.  Device mode: x_image=(addr, M)."""
+    lib = load_library()
+    if isinstance(x_image, tuple):
+        (xa, M) = x_image
+        _check(lib.hm_gemm_image(_ptr(xa), _ptr(w_image), int(dtype), M, K, N, _ptr(y), int(y_dtype), ldy or N, _ptr(stream)))
+        return None
+    xi, wi = _image_in(x_image), _image_in(w_image)
+    _fits(xi, 1, dtype, M, K, "x_image")
+    _fits(wi, 1, dtype, N, K, "w_image")
+    o = _rows_out((M, N), y_dtype)
+    _check(lib.hm_gemm_image(_ptr(xi), _ptr(wi), int(dtype), M, K, N, _ptr(o), int(y_dtype), N, None))
+    return o
+
+
+def gemv_mx4(x, w_image, N: int, K: Optional[int] = None, x_dtype=DType.F32, ldx: Optional[int] = None, y=None, y_dtype: DType = DType.F32, ldy: Optional[int] = None, stream=None):
+    """y [M, N] = x @ W^T for up to eight rows as they are and an MXFP4 image of the weights."""
+    lib = load_library()
+    if isinstance(x, tuple):
+        (xa, M) = x
+        _check(lib.hm_gemv_mx4(_ptr(xa), int(x_dtype), ldx or K, _ptr(w_image), M, K, N, _ptr(y), int(y_dtype), ldy or N, _ptr(stream)))
+        return None
+    xa, x_dtype = _rows_in(x)
+    M, K = xa.shape
+    wi = _image_in(w_image)
+    _fits(wi, 1, DType.MXFP4, N, K, "w_image")
+    o = _rows_out((M, N), y_dtype)
+    _check(lib.hm_gemv_mx4(_ptr(xa), int(x_dtype), K, _ptr(wi), M, K, N, _ptr(o), int(y_dtype), N, None))
+    return o
+
+
+def expert_plan(ids, experts: int, plan=None, stream=None):
+    """Groups pairs by their experts ids (outside [0, experts): none).  Device mode: ids=(addr, pairs).  Host mode returns the plan's
+    int32 words: first block [experts + 1], count [experts], place [pairs], row [expert_plan_rows]."""
+    lib = load_library()
+    if isinstance(ids, tuple):
+        (ia, pairs) = ids
+        _check(lib.hm_expert_plan(_ptr(ia), pairs, experts, _ptr(plan), _ptr(stream)))
+        return None
+    ia = np.ascontiguousarray(ids, dtype=np.int32)
+    out = np.empty(max(expert_plan_ints(ia.size, experts), 1), np.int32)
+    _check(lib.hm_expert_plan(_ptr(ia), ia.size, experts, _ptr(out), None))
+    return out
+
+
+def expert_gemm(x_image, w_images, plan, N: int, dtype: DType, pairs: int, experts: int, K: int, y=None, y_dtype: DType = DType.F32, ldy: Optional[int] = None, stream=None):
+    """y [pairs, N]: each pair's row of the grouped image times its expert's weights (images back to back).  Rows of pairs without an
+    expert stay as they are (host mode: those of y, else zero)."""
+    lib = load_library()
+    if not isinstance(x_image, np.ndarray):
+        _check(lib.hm_expert_gemm(_ptr(x_image), _ptr(w_images), int(dtype), _ptr(plan), pairs, experts, K, N, _ptr(y), int(y_dtype), ldy or N, _ptr(stream)))
+        return None
+    xi, wi, p = _image_in(x_image), _image_in(w_images), np.ascontiguousarray(plan, dtype=np.int32)
+    _fits(xi, 1, dtype, expert_plan_rows(pairs, experts), K, "x_image")
+    _fits(wi, experts, dtype, N, K, "w_images")
+    o = _rows_out((pairs, N), y_dtype) if y is None else np.ascontiguousarray(y)
+    _check(lib.hm_expert_gemm(_ptr(xi), _ptr(wi), int(dtype), _ptr(p), pairs, experts, K, N, _ptr(o), int(y_dtype), N, None))
+    return o
+
+
+def expert_gemv(x, w_images, ids, N: int, top: int, experts: int, K: Optional[int] = None, x_dtype=DType.F32, ldx: Optional[int] = None, y=None, y_dtype: DType = DType.F32, ldy: Optional[int] = None, stream=None):
+    """y [pairs, N]: row p // top of x, as it is, times the MXFP4 image of expert ids[p]; for few pairs."""
+    lib = load_library()
+    if isinstance(x, tuple):
+        (xa, rows) = x
+        _check(lib.hm_expert_gemv(_ptr(xa), int(x_dtype), ldx or K, _ptr(w_images), _ptr(ids), rows * top, top, experts, K, N, _ptr(y), int(y_dtype), ldy or N, _ptr(stream)))
+        return None
+    xa, x_dtype = _rows_in(x)
+    rows, K = xa.shape
+    wi, ia = _image_in(w_images), np.ascontiguousarray(ids, dtype=np.int32)
+    _fits(wi, experts, DType.MXFP4, N, K, "w_images")
+    if ia.size != rows * top:
+        raise HomuraError(HM_ERR_INVALID, "ids are top times the rows")
+    o = _rows_out((rows * top, N), y_dtype) if y is None else np.ascontiguousarray(y)
+    _check(lib.hm_expert_gemv(_ptr(xa), int(x_dtype), K, _ptr(wi), _ptr(ia), rows * top, top, experts, K, N, _ptr(o), int(y_dtype), N, None))
+    return o
+
+
+def expert_sum(rows, ids, weights, top: int, experts: int, width: Optional[int] = None, rows_dtype=DType.F32, resid=None, y=None, y_dtype: DType = DType.F32, stream=None):
+    """y [tokens, width] = resid + sum over a token's choices with an expert of weights * rows.  Device mode: rows=(addr, tokens)."""
+    lib = load_library()
+    if isinstance(rows, tuple):
+        (ra, tokens) = rows
+        _check(lib.hm_expert_sum(_ptr(ra), int(rows_dtype), _ptr(ids), _ptr(weights), tokens, top, experts, width, _ptr(resid), _ptr(y), int(y_dtype), _ptr(stream)))
+        return None
+    ra, rows_dtype = _rows_in(rows)
+    tokens, width = ra.shape[0] // top, ra.shape[1]
+    ia, w = np.ascontiguousarray(ids, dtype=np.int32), np.ascontiguousarray(weights, dtype=np.float32)
+    r = None if resid is None else np.ascontiguousarray(resid, dtype=np.float32)
+    if ia.size != ra.shape[0] or w.size != ia.size or ia.size != tokens * top or (r is not None and r.shape != (tokens, width)):
+        raise HomuraError(HM_ERR_INVALID, "ids, weights and resid do not match the rows")
+    o = _rows_out((tokens, width), y_dtype)
+    _check(lib.hm_expert_sum(_ptr(ra), int(rows_dtype), _ptr(ia), _ptr(w), tokens, top, experts, width, _ptr(r), _ptr(o), int(y_dtype), None))
+    return o
 
 
 def argmax(logits) -> np.ndarray:

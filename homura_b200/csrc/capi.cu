@@ -1,8 +1,10 @@
 // extern "C" surface declared in include/homura_b200.h.
 #include <algorithm>
+#include <climits>
 #include <cmath>
 #include <cstdlib>
 #include <cstring>
+#include <initializer_list>
 #include <map>
 #include <memory>
 #include <mutex>
@@ -12,6 +14,7 @@
 #include "engine.h"
 #include "gemm_tc.h"
 #include "gqa_attn.h"
+#include "image.h"
 #include "moe.h"
 #include "kquant.h"
 #include "latent_attn.h"
@@ -191,6 +194,28 @@ bool have_device() {
     }
     return n > 0;
 }
+
+// Device memory of another GPU than the current one among these pointers (host pointers and null do not count).
+bool on_other_device(std::initializer_list<const void*> ptrs) {
+    int dev = 0;
+    if (cudaGetDevice(&dev) != cudaSuccess) return false;
+    for (const void* p : ptrs) {
+        cudaPointerAttributes at;
+        if (!p) continue;
+        if (cudaPointerGetAttributes(&at, p) != cudaSuccess) {
+            cudaGetLastError();
+            continue;
+        }
+        if (at.type == cudaMemoryTypeDevice && at.device != dev) return true;
+    }
+    return false;
+}
+bool misaligned(const void* p, size_t n) { return ((uintptr_t)p & (n - 1)) != 0; }
+bool is_image_dtype(int d) { return d == HM_MXFP4 || d == HM_BF16; }
+bool is_row_dtype(int d) { return d == HM_F32 || d == HM_BF16; }
+size_t row_bytes(int dtype) { return dtype == HM_BF16 ? 2 : 4; }
+// Bytes of rows of `width` elements, ld apart.
+size_t span_bytes(int rows, int width, size_t ld, int dtype) { return rows < 1 ? 0 : ((size_t)(rows - 1) * ld + width) * row_bytes(dtype); }
 
 #define NEED_DEVICE()                                                                             \
     do {                                                                                          \
@@ -1175,6 +1200,250 @@ int hm_post_norm_route(const float* y, const float* identity, float* x, int M, i
     }
     if (!a.y || !a.x || !a.w || (identity && !a.identity) || (router && (!a.router || !a.correction || !a.out.ids || !a.out.weights || !a.out.identity))) return sg.finish(cudaErrorMemoryAllocation);
     return sg.finish(launch_post_norm(a, sm_count_of_current_device(), st, false));
+}
+
+size_t hm_image_bytes(int dtype, int rows, int K) { return rows < 1 || K < 1 || !is_image_dtype(dtype) ? 0 : img_bytes(dtype == HM_MXFP4, rows, K); }
+
+int hm_image_pack(const void* x, int x_dtype, int rows, int K, size_t ldx, int glu, int dtype, void* image, void* stream) {
+    const int width = glu ? 2 : 1;
+    if (!x || !image || rows < 0 || K < 1 || K > INT_MAX / 4 || ldx < (size_t)K * width) return gfail(HM_ERR_INVALID, "hm_image_pack: bad arguments (ldx >= K, 2 K with glu)");
+    if (!is_row_dtype(x_dtype) || !is_image_dtype(dtype)) return gfail(HM_ERR_UNSUPPORTED, "hm_image_pack: rows are HM_F32 or HM_BF16, images HM_MXFP4 or HM_BF16");
+    if (misaligned(x, row_bytes(x_dtype)) || misaligned(image, 16)) return gfail(HM_ERR_INVALID, "hm_image_pack: misaligned pointer (images start on 16-byte boundaries)");
+    if (rows == 0) return HM_OK;
+    NEED_DEVICE();
+    if (on_other_device({x, image})) return gfail(HM_ERR_INVALID, "hm_image_pack: memory of another device than the current one");
+    cudaStream_t st = (cudaStream_t)stream;
+    Staging sg(st);
+    const bool mx = dtype == HM_MXFP4;
+    PackArgs a{};
+    a.x = sg.in((const uint8_t*)x, span_bytes(rows, K * width, ldx, x_dtype));
+    a.bf16 = x_dtype == HM_BF16;
+    a.glu = glu != 0;
+    a.ldx = ldx;
+    a.rows = rows;
+    a.K = K;
+    a.image = sg.out((unsigned char*)image, img_bytes(mx, rows, K), true);
+    if (!a.x || !a.image) return sg.finish(cudaErrorMemoryAllocation);
+    return sg.finish(launch_image_pack(a, mx, st));
+}
+
+int hm_image_unpack(const void* image, int dtype, int rows, int K, void* out, int out_dtype, size_t ldo, void* stream) {
+    if (!image || !out || rows < 0 || K < 1 || K > INT_MAX / 4 || ldo < (size_t)K) return gfail(HM_ERR_INVALID, "hm_image_unpack: bad arguments (ldo >= K)");
+    if (!is_row_dtype(out_dtype) || !is_image_dtype(dtype)) return gfail(HM_ERR_UNSUPPORTED, "hm_image_unpack: rows are HM_F32 or HM_BF16, images HM_MXFP4 or HM_BF16");
+    if (misaligned(out, row_bytes(out_dtype)) || misaligned(image, 16)) return gfail(HM_ERR_INVALID, "hm_image_unpack: misaligned pointer (images start on 16-byte boundaries)");
+    if (rows == 0) return HM_OK;
+    NEED_DEVICE();
+    if (on_other_device({image, out})) return gfail(HM_ERR_INVALID, "hm_image_unpack: memory of another device than the current one");
+    cudaStream_t st = (cudaStream_t)stream;
+    Staging sg(st);
+    const bool mx = dtype == HM_MXFP4;
+    const unsigned char* im = sg.in((const unsigned char*)image, img_bytes(mx, rows, K));
+    uint8_t* o = sg.out((uint8_t*)out, span_bytes(rows, K, ldo, out_dtype), true);
+    if (!im || !o) return sg.finish(cudaErrorMemoryAllocation);
+    return sg.finish(launch_image_unpack(im, mx, rows, K, o, out_dtype == HM_BF16, ldo, st));
+}
+
+int hm_image_from_blocks(const void* blocks, int rows, int K, void* image, void* stream) {
+    if (!blocks || !image || rows < 0 || K < 32 || K % 32 != 0) return gfail(HM_ERR_INVALID, "hm_image_from_blocks: bad arguments (K a multiple of 32)");
+    if (misaligned(image, 16)) return gfail(HM_ERR_INVALID, "hm_image_from_blocks: images start on 16-byte boundaries");
+    if (rows == 0) return HM_OK;
+    NEED_DEVICE();
+    if (on_other_device({blocks, image})) return gfail(HM_ERR_INVALID, "hm_image_from_blocks: memory of another device than the current one");
+    cudaStream_t st = (cudaStream_t)stream;
+    Staging sg(st);
+    const uint8_t* b = sg.in((const uint8_t*)blocks, (size_t)rows * (K / 32) * 17);
+    unsigned char* im = sg.out((unsigned char*)image, img_bytes(true, rows, K), true);
+    if (!b || !im) return sg.finish(cudaErrorMemoryAllocation);
+    return sg.finish(launch_image_blocks(b, rows, K, im, st));
+}
+
+// What the entry points of products have in common: status of the launch, and of a wait that ran out where the call synchronised.
+static int finish_product(Staging& sg, cudaError_t launched, const char* timeout) {
+    const bool synced = sg.staged();
+    const int rc = sg.finish(launched);
+    if (rc != HM_OK) return rc;
+    if (synced && take_wait_err()) return gfail(HM_ERR_TIMEOUT, timeout);
+    return HM_OK;
+}
+
+int hm_gemm_image(const void* x_image, const void* w_image, int dtype, int M, int K, int N, void* y, int y_dtype, size_t ldy, void* stream) {
+    if (!x_image || !w_image || !y || M < 0 || K < 1 || K > INT_MAX / 4 || N < 1 || N > INT_MAX - 128 || ldy < (size_t)N) return gfail(HM_ERR_INVALID, "hm_gemm_image: bad arguments (ldy >= N)");
+    if (!is_row_dtype(y_dtype) || !is_image_dtype(dtype)) return gfail(HM_ERR_UNSUPPORTED, "hm_gemm_image: y is HM_F32 or HM_BF16, images HM_MXFP4 or HM_BF16");
+    if (misaligned(x_image, 16) || misaligned(w_image, 16) || misaligned(y, row_bytes(y_dtype))) return gfail(HM_ERR_INVALID, "hm_gemm_image: misaligned pointer (images start on 16-byte boundaries)");
+    if (M == 0) return HM_OK;
+    NEED_DEVICE();
+    if (on_other_device({x_image, w_image, y})) return gfail(HM_ERR_INVALID, "hm_gemm_image: memory of another device than the current one");
+    cudaStream_t st = (cudaStream_t)stream;
+    Staging sg(st);
+    const bool mx = dtype == HM_MXFP4;
+    ImageGemmArgs a{};
+    a.x = sg.in((const unsigned char*)x_image, img_bytes(mx, M, K));
+    a.w = sg.in((const unsigned char*)w_image, img_bytes(mx, N, K));
+    a.M = M;
+    a.N = N;
+    a.K = K;
+    a.y = sg.out((uint8_t*)y, span_bytes(M, N, ldy, y_dtype), true);
+    a.ldy = ldy;
+    a.bf16 = y_dtype == HM_BF16;
+    if (!a.x || !a.w || !a.y) return sg.finish(cudaErrorMemoryAllocation);
+    if (!sg.ok(get_wait_err(&a.err_flag))) return sg.finish(cudaSuccess);
+    return finish_product(sg, launch_image_gemm(a, mx, sm_count_of_current_device(), st), "hm_gemm_image: a bounded device-side wait ran out");
+}
+
+int hm_gemv_mx4(const void* x, int x_dtype, size_t ldx, const void* w_image, int M, int K, int N, void* y, int y_dtype, size_t ldy, void* stream) {
+    if (!x || !w_image || !y || M < 0 || M > 8 || K < 1 || N < 1 || N > INT_MAX - 128 || ldx < (size_t)K || ldy < (size_t)N) return gfail(HM_ERR_INVALID, "hm_gemv_mx4: bad arguments (M <= 8, ldx >= K, ldy >= N)");
+    if (!is_row_dtype(x_dtype) || !is_row_dtype(y_dtype) || K > MX_GEMV_K) return gfail(HM_ERR_UNSUPPORTED, "hm_gemv_mx4: x and y are HM_F32 or HM_BF16, K at most 32768");
+    if (misaligned(x, row_bytes(x_dtype)) || misaligned(w_image, 16) || misaligned(y, row_bytes(y_dtype))) return gfail(HM_ERR_INVALID, "hm_gemv_mx4: misaligned pointer (images start on 16-byte boundaries)");
+    if (M == 0) return HM_OK;
+    NEED_DEVICE();
+    if (on_other_device({x, w_image, y})) return gfail(HM_ERR_INVALID, "hm_gemv_mx4: memory of another device than the current one");
+    cudaStream_t st = (cudaStream_t)stream;
+    Staging sg(st);
+    MxGemvArgs a{};
+    a.x = sg.in((const uint8_t*)x, span_bytes(M, K, ldx, x_dtype));
+    a.bf16 = x_dtype == HM_BF16;
+    a.ldx = ldx;
+    a.M = M;
+    a.w = sg.in((const unsigned char*)w_image, img_bytes(true, N, K));
+    a.N = N;
+    a.K = K;
+    a.y = sg.out((uint8_t*)y, span_bytes(M, N, ldy, y_dtype), true);
+    a.ldy = ldy;
+    a.y_bf16 = y_dtype == HM_BF16;
+    if (!a.x || !a.w || !a.y) return sg.finish(cudaErrorMemoryAllocation);
+    if (!sg.ok(get_wait_err(&a.err_flag))) return sg.finish(cudaSuccess);
+    return finish_product(sg, launch_mx4_gemv(a, sm_count_of_current_device(), st), "hm_gemv_mx4: a bounded device-side wait ran out");
+}
+
+static bool bad_groups(int pairs, int experts) { return pairs < 0 || pairs > (1 << 28) || experts < 1 || experts > PLAN_EXPERTS; }
+size_t hm_expert_plan_ints(int pairs, int experts) { return bad_groups(pairs, experts) ? 0 : plan_ints(pairs, experts); }
+int hm_expert_plan_rows(int pairs, int experts) { return bad_groups(pairs, experts) ? 0 : plan_blocks(pairs, experts) * IMG_ROWS; }
+
+int hm_expert_plan(const int32_t* ids, int pairs, int experts, int32_t* plan, void* stream) {
+    if (!plan || (!ids && pairs > 0) || bad_groups(pairs, experts)) return gfail(HM_ERR_INVALID, "hm_expert_plan: bad arguments (experts <= 1024, pairs <= 2^28)");
+    if (misaligned(ids, 4) || misaligned(plan, 4)) return gfail(HM_ERR_INVALID, "hm_expert_plan: misaligned pointer");
+    NEED_DEVICE();
+    if (on_other_device({ids, plan})) return gfail(HM_ERR_INVALID, "hm_expert_plan: memory of another device than the current one");
+    cudaStream_t st = (cudaStream_t)stream;
+    Staging sg(st);
+    const int32_t* id = sg.in(ids, (size_t)pairs);
+    int32_t* p = sg.out(plan, plan_ints(pairs, experts));
+    if ((pairs > 0 && !id) || !p) return sg.finish(cudaErrorMemoryAllocation);
+    return sg.finish(launch_plan(id, plan_at(p, pairs, experts), st));
+}
+
+int hm_expert_pack(const void* x, int x_dtype, int K, size_t ldx, int glu, const int32_t* plan, int pairs, int experts, int top, int dtype, void* image, void* stream) {
+    const int width = glu ? 2 : 1;
+    if (!x || !plan || !image || K < 1 || K > INT_MAX / 4 || ldx < (size_t)K * width || bad_groups(pairs, experts) || top < 1 || pairs % top != 0)
+        return gfail(HM_ERR_INVALID, "hm_expert_pack: bad arguments (ldx >= K, 2 K with glu; pairs a multiple of top; experts <= 1024)");
+    if (!is_row_dtype(x_dtype) || !is_image_dtype(dtype)) return gfail(HM_ERR_UNSUPPORTED, "hm_expert_pack: rows are HM_F32 or HM_BF16, images HM_MXFP4 or HM_BF16");
+    if (misaligned(x, row_bytes(x_dtype)) || misaligned(plan, 4) || misaligned(image, 16)) return gfail(HM_ERR_INVALID, "hm_expert_pack: misaligned pointer (images start on 16-byte boundaries)");
+    if (pairs == 0) return HM_OK;
+    NEED_DEVICE();
+    if (on_other_device({x, plan, image})) return gfail(HM_ERR_INVALID, "hm_expert_pack: memory of another device than the current one");
+    cudaStream_t st = (cudaStream_t)stream;
+    Staging sg(st);
+    const bool mx = dtype == HM_MXFP4;
+    const Plan p = plan_at(const_cast<int32_t*>(sg.in(plan, plan_ints(pairs, experts))), pairs, experts);
+    PackArgs a{};
+    a.x = sg.in((const uint8_t*)x, span_bytes(pairs / top, K * width, ldx, x_dtype));
+    a.bf16 = x_dtype == HM_BF16;
+    a.glu = glu != 0;
+    a.ldx = ldx;
+    a.rows = p.rows;
+    a.K = K;
+    a.src = p.row;
+    a.div = top;
+    a.src_rows = pairs / top;
+    a.image = sg.out((unsigned char*)image, img_bytes(mx, p.rows, K), true);
+    if (!p.first || !a.x || !a.image) return sg.finish(cudaErrorMemoryAllocation);
+    return sg.finish(launch_image_pack(a, mx, st));
+}
+
+int hm_expert_gemm(const void* x_image, const void* w_images, int dtype, const int32_t* plan, int pairs, int experts, int K, int N, void* y, int y_dtype, size_t ldy, void* stream) {
+    if (!x_image || !w_images || !plan || !y || bad_groups(pairs, experts) || K < 1 || K > INT_MAX / 4 || N < 1 || N > INT_MAX - 128 || ldy < (size_t)N) return gfail(HM_ERR_INVALID, "hm_expert_gemm: bad arguments (ldy >= N, experts <= 1024)");
+    if (!is_row_dtype(y_dtype) || !is_image_dtype(dtype)) return gfail(HM_ERR_UNSUPPORTED, "hm_expert_gemm: y is HM_F32 or HM_BF16, images HM_MXFP4 or HM_BF16");
+    if (misaligned(x_image, 16) || misaligned(w_images, 16) || misaligned(plan, 4) || misaligned(y, row_bytes(y_dtype))) return gfail(HM_ERR_INVALID, "hm_expert_gemm: misaligned pointer (images start on 16-byte boundaries)");
+    if (pairs == 0) return HM_OK;
+    NEED_DEVICE();
+    if (on_other_device({x_image, w_images, plan, y})) return gfail(HM_ERR_INVALID, "hm_expert_gemm: memory of another device than the current one");
+    cudaStream_t st = (cudaStream_t)stream;
+    Staging sg(st);
+    const bool mx = dtype == HM_MXFP4;
+    const Plan p = plan_at(const_cast<int32_t*>(sg.in(plan, plan_ints(pairs, experts))), pairs, experts);
+    ImageGemmArgs a{};
+    a.w_stride = img_bytes(mx, N, K);
+    a.x = sg.in((const unsigned char*)x_image, img_bytes(mx, p.rows, K));
+    a.w = sg.in((const unsigned char*)w_images, a.w_stride * experts);
+    a.N = N;
+    a.K = K;
+    a.y = sg.out((uint8_t*)y, span_bytes(pairs, N, ldy, y_dtype), true);
+    a.ldy = ldy;
+    a.bf16 = y_dtype == HM_BF16;
+    a.first = p.first;
+    a.count = p.count;
+    a.row = p.row;
+    a.experts = experts;
+    a.pairs = pairs;
+    if (!p.first || !a.x || !a.w || !a.y) return sg.finish(cudaErrorMemoryAllocation);
+    if (!sg.ok(get_wait_err(&a.err_flag))) return sg.finish(cudaSuccess);
+    return finish_product(sg, launch_image_gemm(a, mx, sm_count_of_current_device(), st), "hm_expert_gemm: a bounded device-side wait ran out");
+}
+
+int hm_expert_gemv(const void* x, int x_dtype, size_t ldx, const void* w_images, const int32_t* ids, int pairs, int top, int experts, int K, int N, void* y, int y_dtype, size_t ldy, void* stream) {
+    if (!x || !w_images || !ids || !y || bad_groups(pairs, experts) || pairs > 65535 || top < 1 || pairs % top != 0 || K < 1 || N < 1 || N > INT_MAX - 128 || ldx < (size_t)K || ldy < (size_t)N)
+        return gfail(HM_ERR_INVALID, "hm_expert_gemv: bad arguments (pairs <= 65535 and a multiple of top, ldx >= K, ldy >= N, experts <= 1024)");
+    if (!is_row_dtype(x_dtype) || !is_row_dtype(y_dtype) || K > MX_GEMV_K) return gfail(HM_ERR_UNSUPPORTED, "hm_expert_gemv: x and y are HM_F32 or HM_BF16, K at most 32768");
+    if (misaligned(x, row_bytes(x_dtype)) || misaligned(w_images, 16) || misaligned(ids, 4) || misaligned(y, row_bytes(y_dtype))) return gfail(HM_ERR_INVALID, "hm_expert_gemv: misaligned pointer (images start on 16-byte boundaries)");
+    if (pairs == 0) return HM_OK;
+    NEED_DEVICE();
+    if (on_other_device({x, w_images, ids, y})) return gfail(HM_ERR_INVALID, "hm_expert_gemv: memory of another device than the current one");
+    cudaStream_t st = (cudaStream_t)stream;
+    Staging sg(st);
+    MxGemvArgs a{};
+    a.w_stride = img_bytes(true, N, K);
+    a.x = sg.in((const uint8_t*)x, span_bytes(pairs / top, K, ldx, x_dtype));
+    a.bf16 = x_dtype == HM_BF16;
+    a.ldx = ldx;
+    a.M = 1;
+    a.w = sg.in((const unsigned char*)w_images, a.w_stride * experts);
+    a.N = N;
+    a.K = K;
+    a.y = sg.out((uint8_t*)y, span_bytes(pairs, N, ldy, y_dtype), true);
+    a.ldy = ldy;
+    a.y_bf16 = y_dtype == HM_BF16;
+    a.ids = sg.in(ids, (size_t)pairs);
+    a.pairs = pairs;
+    a.top = top;
+    a.experts = experts;
+    if (!a.x || !a.w || !a.y || !a.ids) return sg.finish(cudaErrorMemoryAllocation);
+    if (!sg.ok(get_wait_err(&a.err_flag))) return sg.finish(cudaSuccess);
+    return finish_product(sg, launch_mx4_gemv(a, sm_count_of_current_device(), st), "hm_expert_gemv: a bounded device-side wait ran out");
+}
+
+int hm_expert_sum(const void* rows, int rows_dtype, const int32_t* ids, const float* weights, int tokens, int top, int experts, int W, const float* resid, void* y, int y_dtype, void* stream) {
+    if (!rows || !ids || !weights || !y || tokens < 0 || top < 1 || W < 1 || (long long)tokens * top > (1 << 28) || experts < 1) return gfail(HM_ERR_INVALID, "hm_expert_sum: bad arguments");
+    if (!is_row_dtype(rows_dtype) || !is_row_dtype(y_dtype)) return gfail(HM_ERR_UNSUPPORTED, "hm_expert_sum: rows and y are HM_F32 or HM_BF16");
+    if (misaligned(rows, row_bytes(rows_dtype)) || misaligned(ids, 4) || misaligned(weights, 4) || misaligned(resid, 4) || misaligned(y, row_bytes(y_dtype))) return gfail(HM_ERR_INVALID, "hm_expert_sum: misaligned pointer");
+    if (tokens == 0) return HM_OK;
+    NEED_DEVICE();
+    if (on_other_device({rows, ids, weights, resid, y})) return gfail(HM_ERR_INVALID, "hm_expert_sum: memory of another device than the current one");
+    cudaStream_t st = (cudaStream_t)stream;
+    Staging sg(st);
+    SumArgs a{};
+    a.rows = sg.in((const uint8_t*)rows, (size_t)tokens * top * W * row_bytes(rows_dtype));
+    a.rows_bf16 = rows_dtype == HM_BF16;
+    a.ids = sg.in(ids, (size_t)tokens * top);
+    a.weights = sg.in(weights, (size_t)tokens * top);
+    a.resid = sg.in(resid, (size_t)tokens * W);
+    a.tokens = tokens;
+    a.top = top;
+    a.experts = experts;
+    a.W = W;
+    a.y = sg.out((uint8_t*)y, (size_t)tokens * W * row_bytes(y_dtype));
+    a.y_bf16 = y_dtype == HM_BF16;
+    if (!a.rows || !a.ids || !a.weights || (resid && !a.resid) || !a.y) return sg.finish(cudaErrorMemoryAllocation);
+    return sg.finish(launch_expert_sum(a, st));
 }
 
 int hm_argmax(const float* logits, int rows, int n, uint32_t* out, void* stream) {

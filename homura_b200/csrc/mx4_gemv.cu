@@ -1,0 +1,269 @@
+// Few rows times 4-bit weights: y[m][n] = sum_k x[m][k] w[n][k], x f32 or bf16 as they are, w the image of image.h, f32 sums.
+//
+// Bound by the weights' 17/32 bytes each, if a weight costs few enough instructions: the codes go to f16 by conversion (exactly) and are multiplied
+// on mma.sync m16n8k16, whose eight columns are the rows of x; a block of 32 values is two MMAs into accumulators of their own, which the block's
+// scale then joins to the sum in f32.  x enters as f16: 2^s x with its largest value in [2^7, 2^8), as one term (bf16) or as a sum of two (f32: 2^-22 of a value
+// and 2^-32 of the row's largest), so that a launch of up to eight bf16 or four f32 rows has one MMA column block, eight f32 rows have two.
+//
+//   * a CTA = 128 features (a tile of the image) x its k-blocks; a producer warp copies tiles of 17 KB into a ring, eight warps multiply: four groups of 32
+//     features, two halves of a k-block.  The k order of an MMA is free as long as both operands agree: lane t of a group of four takes values
+//     8 t .. 8 t + 7 of a block, one word of codes.
+//   * tiles that are fewer than the SMs share their k-blocks among the CTAs of a cluster, summed in rank order through distributed shared memory; otherwise
+//     a CTA walks several tiles and converts x once.
+#include <algorithm>
+
+#include "image.h"
+#include "launch_attrs.h"
+#include "mbarrier.cuh"
+
+namespace hm {
+namespace {
+
+constexpr int MMA_WARPS = 8, THREADS = 32 + MMA_WARPS * 32;
+constexpr int MAX_SLOTS = 8, MAX_SPLIT = 8;
+constexpr int PART_LD = 9;  // floats of a feature's partial sums (eight rows), odd: free of bank conflicts
+
+struct Shared {
+    uint64_t full[MAX_SLOTS], empty[MAX_SLOTS];
+    volatile int abort_flag;
+    uint32_t top[8];        // largest finite value of a row, as bits
+};
+
+__device__ __forceinline__ void mma_f16(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
+    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};" : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3]) : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+__device__ __forceinline__ uint32_t f16x2_rn(float lo, float hi) {
+    uint32_t r;
+    asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
+    return r;
+}
+
+// Elements of a column of x in shared memory: the k-blocks of a CTA and half a line, so that neighbouring columns lie in different banks.
+__host__ __device__ inline int x_ld(int kb_per) { return kb_per * MX_K + 32; }
+inline size_t smem_bytes(int slots, int kb_per, int cols) { return 1024 + (size_t)slots * MX_TILE + (size_t)cols * x_ld(kb_per) * 2 + 2 * IMG_ROWS * PART_LD * 4; }
+
+// NB: blocks of eight columns; TERMS: f16 terms of x.  Column of row m, term i: m + 8 i where the rows fill a block, else TERMS m + i.
+template <int NB, int TERMS>
+__global__ void __launch_bounds__(THREADS, 2) mx4_gemv_kernel(const MxGemvArgs a) {
+    extern __shared__ __align__(1024) unsigned char dsm[];
+    __shared__ Shared sh;
+    unsigned char* ring = dsm + ((1024u - (s32(dsm) & 1023u)) & 1023u);
+    const int ldx = x_ld(a.kb_per);
+    uint16_t* xs = reinterpret_cast<uint16_t*>(ring + (size_t)a.slots * MX_TILE);
+    const int cols = a.M * TERMS;
+    float* part = reinterpret_cast<float*>(xs + (size_t)cols * ldx);  // [2 halves][128 features][PART_LD]
+    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+    int expert = 0, xrow0 = 0;
+    if (a.ids) {
+        expert = __ldg(a.ids + blockIdx.y);
+        if (expert < 0 || expert >= a.experts) return;  // the whole cluster
+        xrow0 = blockIdx.y / a.top;
+    }
+    const int rank = blockIdx.x % a.split, step = gridDim.x / a.split;
+    const int kb0 = rank * a.kb_per, kb1 = min(a.kblocks, kb0 + a.kb_per), nkb = kb1 - kb0;
+    if (tid == 0) {
+        for (int s = 0; s < a.slots; ++s) { mb_init(&sh.full[s], 1); mb_init(&sh.empty[s], MMA_WARPS); }
+        sh.abort_flag = 0;
+        asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    }
+    if (tid < 8) sh.top[tid] = 0;
+    __syncthreads();
+    uint32_t issued = 0;
+    if (warp == MMA_WARPS) {
+        if (lane == 0) {
+            const unsigned char* w = a.w + expert * a.w_stride;
+            bool ok = true;
+            for (int t = blockIdx.x / a.split; t < a.tiles && ok; t += step)
+                for (int kb = kb0; kb < kb1; ++kb, ++issued) {
+                    const uint32_t s = issued % a.slots;
+                    if (issued >= (uint32_t)a.slots) ok = mb_wait(&sh.empty[s], ((issued / a.slots) & 1u) ^ 1u, a.err_flag, &sh.abort_flag);
+                    if (!ok) break;
+                    mb_expect_tx(&sh.full[s], MX_TILE);
+                    bulk_copy(ring + (size_t)s * MX_TILE, w + ((size_t)t * a.kblocks + kb) * MX_TILE, MX_TILE, &sh.full[s]);
+                }
+        }
+    } else {
+        // x: its largest finite value per row, then f16 terms
+        constexpr int XT = MMA_WARPS * 32;
+        const int k0 = kb0 * MX_K, kn = min(a.K - k0, nkb * MX_K);
+        const char* x = static_cast<const char*>(a.x);
+        auto at = [&](int m, int k) {
+            const size_t i = (size_t)(xrow0 + m) * a.ldx + k0 + k;
+            return a.bf16 ? bf16_bits_to_f32(__ldg(reinterpret_cast<const uint16_t*>(x) + i)) : __ldg(reinterpret_cast<const float*>(x) + i);
+        };
+        for (int m = 0; m < a.M; ++m) {
+            uint32_t top = 0;
+            for (int k = tid; k < kn; k += XT) {
+                const uint32_t b = __float_as_uint(at(m, k)) & 0x7FFFFFFFu;
+                if (b < 0x7F800000u) top = max(top, b);
+            }
+            top = __reduce_max_sync(0xffffffffu, top);
+            if (lane == 0) atomicMax(&sh.top[m], top);
+        }
+        asm volatile("bar.sync 1, 256;" ::: "memory");
+        for (int m = 0; m < a.M; ++m) {
+            const int e = min(max(134 - (int)(sh.top[m] >> 23), -126), 126);  // 2^e brings the largest value into [2^7, 2^8)
+            const float up = __uint_as_float((uint32_t)(e + 127) << 23);
+            for (int k = 2 * tid; k < nkb * MX_K; k += 2 * XT) {
+                const float u = k < kn ? at(m, k) * up : 0.f, v = k + 1 < kn ? at(m, k + 1) * up : 0.f;
+                const uint32_t h = f16x2_rn(u, v);
+                const int c = NB == 2 ? m : TERMS * m;
+                *reinterpret_cast<uint32_t*>(xs + (size_t)c * ldx + k) = h;
+                if (TERMS == 2) {
+                    // what the first term leaves; nothing of an infinity
+                    const float ru = u - f16_bits_to_f32((uint16_t)h), rv = v - f16_bits_to_f32((uint16_t)(h >> 16));
+                    const float fu = fabsf(u) < __int_as_float(0x7F800000) ? ru : 0.f, fv = fabsf(v) < __int_as_float(0x7F800000) ? rv : 0.f;
+                    *reinterpret_cast<uint32_t*>(xs + (size_t)(NB == 2 ? a.M + m : c + 1) * ldx + k) = f16x2_rn(fu, fv);
+                }
+            }
+        }
+        asm volatile("bar.sync 1, 256;" ::: "memory");
+    }
+    __syncwarp();
+    const int fg = warp & 3, kh = (warp >> 2) & 1, g = lane >> 2, tl = lane & 3;
+    uint32_t used = 0;
+    for (int t = blockIdx.x / a.split; t < a.tiles; t += step) {
+        if (warp < MMA_WARPS) {
+            float sum[2][NB][4];
+#pragma unroll
+            for (int i = 0; i < 2; ++i)
+#pragma unroll
+                for (int b = 0; b < NB; ++b)
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) sum[i][b][e] = 0.f;
+            for (int kb = 0; kb < nkb; ++kb, ++used) {
+                const uint32_t s = used % a.slots;
+                if (!__all_sync(0xffffffffu, mb_wait(&sh.full[s], (used / a.slots) & 1u, a.err_flag, &sh.abort_flag))) continue;
+                const unsigned char* tile = ring + (size_t)s * MX_TILE;
+                const uint32_t* sc = reinterpret_cast<const uint32_t*>(tile + kh * 512 + fg * 4);
+                uint32_t scales[4];  // of features g, g + 8, g + 16, g + 24 of the group: a byte per block of this half
+#pragma unroll
+                for (int i = 0; i < 4; ++i) scales[i] = sc[(g + 8 * i) * 4];
+                const unsigned char* codes = tile + MX_SCALES + (fg * 32 + g) * 128 + tl * 4;
+#pragma unroll
+                for (int j = 0; j < 4; ++j) {
+                    uint4 xv[NB];
+#pragma unroll
+                    for (int b = 0; b < NB; ++b) {
+                        const int col = NB == 2 ? b * a.M + min(g, a.M - 1) : min(g, cols - 1);  // columns that do not exist repeat the last
+                        xv[b] = *reinterpret_cast<const uint4*>(xs + (size_t)col * ldx + kb * MX_K + (kh * 4 + j) * 32 + tl * 8);
+                    }
+#pragma unroll
+                    for (int i = 0; i < 2; ++i) {  // features 16 i + g and 16 i + g + 8
+                        uint32_t lo[4], hi[4];
+                        const int piece = ((kh * 4 + j) ^ g) << 4;
+                        mx_halves(*reinterpret_cast<const uint32_t*>(codes + i * 16 * 128 + piece), lo);
+                        mx_halves(*reinterpret_cast<const uint32_t*>(codes + (i * 16 + 8) * 128 + piece), hi);
+                        const float s0 = mx_scale(scales[2 * i] >> (8 * j) & 255u), s1 = mx_scale(scales[2 * i + 1] >> (8 * j) & 255u);
+#pragma unroll
+                        for (int b = 0; b < NB; ++b) {
+                            float d[4] = {0.f, 0.f, 0.f, 0.f};
+                            mma_f16(d, lo[0], hi[0], lo[1], hi[1], xv[b].x, xv[b].y);
+                            mma_f16(d, lo[2], hi[2], lo[3], hi[3], xv[b].z, xv[b].w);
+                            sum[i][b][0] = fmaf(s0, d[0], sum[i][b][0]);
+                            sum[i][b][1] = fmaf(s0, d[1], sum[i][b][1]);
+                            sum[i][b][2] = fmaf(s1, d[2], sum[i][b][2]);
+                            sum[i][b][3] = fmaf(s1, d[3], sum[i][b][3]);
+                        }
+                    }
+                }
+                __syncwarp();
+                if (lane == 0) mb_arrive(&sh.empty[s]);
+            }
+            // terms of a row come together: in neighbouring columns of a lane, or in the same column of two blocks
+            float* p = part + (size_t)kh * IMG_ROWS * PART_LD;
+#pragma unroll
+            for (int i = 0; i < 2; ++i)
+#pragma unroll
+                for (int h = 0; h < 2; ++h) {
+                    float* q = p + (fg * 32 + i * 16 + h * 8 + g) * PART_LD;
+                    if (NB == 2) {
+                        q[2 * tl] = sum[i][0][2 * h] + sum[i][NB - 1][2 * h];
+                        q[2 * tl + 1] = sum[i][0][2 * h + 1] + sum[i][NB - 1][2 * h + 1];
+                    } else if (TERMS == 2) {
+                        q[tl] = sum[i][0][2 * h] + sum[i][0][2 * h + 1];
+                    } else {
+                        q[2 * tl] = sum[i][0][2 * h];
+                        q[2 * tl + 1] = sum[i][0][2 * h + 1];
+                    }
+                }
+            if (a.split == 1) asm volatile("bar.sync 1, 256;" ::: "memory");
+        }
+        if (a.split > 1) cluster_sync_all();  // one tile per cluster
+        // thread: a feature and every second row
+        const int f = tid & 127, n = t * IMG_ROWS + f;
+        if (warp < MMA_WARPS && n < a.N) {
+            for (int m = tid >> 7; m < a.M; m += 2) {
+                // The CTAs of a cluster scale their own part of a row: each brings its sum back before they are added.
+                float v = 0.f;
+                if (a.split == 1) {
+                    const int e = min(max(134 - (int)(sh.top[m] >> 23), -126), 126);
+                    v = (part[f * PART_LD + m] + part[(IMG_ROWS + f) * PART_LD + m]) * __uint_as_float((uint32_t)(127 - e) << 23);
+                } else if (m % a.split == rank) {
+                    for (int r = 0; r < a.split; ++r) {
+                        const int e = min(max(134 - (int)(__float_as_uint(ld_dsmem_f32(dsmem_addr(&sh.top[m], r))) >> 23), -126), 126);
+                        v += (ld_dsmem_f32(dsmem_addr(part + f * PART_LD + m, r)) + ld_dsmem_f32(dsmem_addr(part + (IMG_ROWS + f) * PART_LD + m, r))) * __uint_as_float((uint32_t)(127 - e) << 23);
+                    }
+                } else
+                    continue;
+                const size_t row = a.ids ? blockIdx.y : m;
+                if (a.y_bf16) static_cast<uint16_t*>(a.y)[row * a.ldy + n] = (uint16_t)bf16x2_rne(v, 0.f);
+                else static_cast<float*>(a.y)[row * a.ldy + n] = v;
+            }
+        }
+        if (a.split > 1) {
+            cluster_sync_all();  // nobody ends while others read its sums
+            break;
+        }
+        if (warp < MMA_WARPS) asm volatile("bar.sync 1, 256;" ::: "memory");  // the next tile's sums take the same place
+    }
+    if (warp == MMA_WARPS && lane == 0 && sh.abort_flag) mb_land_ring(sh.full, issued, (uint32_t)a.slots);
+}
+
+template <int NB, int TERMS>
+cudaError_t launch(MxGemvArgs& a, int sm_count, cudaStream_t st) {
+    constexpr size_t HALF = 112 * 1024, MOST = 225 * 1024;  // two CTAs of up to HALF share an SM
+    const int cols = a.M * TERMS, rows = a.ids ? a.pairs : 1;
+    a.split = 1;
+    // Few tiles share their k-blocks among the CTAs of a cluster; so do rows too long for the shared memory of one.
+    const long long ctas = (long long)a.tiles * rows;
+    if (ctas * 2 <= 2 * sm_count) a.split = (int)std::min<long long>({2 * sm_count / ctas, (long long)MAX_SPLIT, (long long)a.kblocks});
+    a.kb_per = (a.kblocks + a.split - 1) / a.split;
+    while (a.split < MAX_SPLIT && smem_bytes(3, a.kb_per, cols) > MOST) {
+        ++a.split;
+        a.kb_per = (a.kblocks + a.split - 1) / a.split;
+    }
+    a.split = (a.kblocks + a.kb_per - 1) / a.kb_per;
+    a.slots = MAX_SLOTS;
+    if (a.split > 1) a.slots = std::min(a.slots, a.kb_per);
+    const size_t limit = smem_bytes(3, a.kb_per, cols) <= HALF ? HALF : MOST;
+    while (a.slots > 1 && smem_bytes(a.slots, a.kb_per, cols) > limit) --a.slots;
+    const size_t smem = smem_bytes(a.slots, a.kb_per, cols);
+    cudaError_t e = ensure_dyn_smem(mx4_gemv_kernel<NB, TERMS>, smem);
+    if (e != cudaSuccess) return e;
+    cudaLaunchConfig_t cfg{};
+    const int per_sm = smem <= HALF ? 2 : 1;
+    cfg.gridDim = dim3(a.split > 1 || a.ids ? (unsigned)a.tiles * a.split : (unsigned)std::min(a.tiles, per_sm * sm_count), rows);
+    cfg.blockDim = dim3(THREADS);
+    cfg.dynamicSmemBytes = smem;
+    cfg.stream = st;
+    cudaLaunchAttribute at[1];
+    if (a.split > 1) {
+        at[0].id = cudaLaunchAttributeClusterDimension;
+        at[0].val.clusterDim = {(unsigned)a.split, 1, 1};
+        cfg.attrs = at;
+        cfg.numAttrs = 1;
+    }
+    return cudaLaunchKernelEx(&cfg, mx4_gemv_kernel<NB, TERMS>, a);
+}
+
+}  // namespace
+
+cudaError_t launch_mx4_gemv(MxGemvArgs a, int sm_count, cudaStream_t st) {
+    a.kblocks = img_kblocks(true, a.K);
+    a.tiles = (a.N + IMG_ROWS - 1) / IMG_ROWS;
+    if (a.bf16) return launch<1, 1>(a, sm_count, st);
+    return a.M <= 4 ? launch<1, 2>(a, sm_count, st) : launch<2, 2>(a, sm_count, st);
+}
+
+}  // namespace hm

@@ -43,7 +43,8 @@ enum hm_status {
 };
 
 /* DType subset on this path: src/dtype.rs:8-26 (+ Q4_0, which Homura has no DType for). */
-enum hm_dtype { HM_F32 = 0, HM_BF16 = 1, HM_F16 = 2, HM_Q8_0 = 3, HM_Q4_0 = 4, HM_I64 = 5, HM_I32 = 6, HM_U8 = 7, HM_Q4_K = 8, HM_Q6_K = 9 };
+enum hm_dtype { HM_F32 = 0, HM_BF16 = 1, HM_F16 = 2, HM_Q8_0 = 3, HM_Q4_0 = 4, HM_I64 = 5, HM_I32 = 6, HM_U8 = 7, HM_Q4_K = 8, HM_Q6_K = 9,
+                HM_MXFP4 = 10 /* 4-bit microscaled floats: the standalone entry points of images only */ };
 
 /* Weight layouts accepted by the standalone projection kernels. */
 enum hm_layout {
@@ -329,6 +330,47 @@ HM_API int hm_gqa_attn_paged(const float* q, const void* k_pages, const void* v_
  * id_weight [M] the sum of the chosen identity experts' scores. */
 HM_API int hm_post_norm_route(const float* y, const float* identity, float* x, int M, int W, const float* w, float mult, float eps, const uint16_t* router, const float* correction, int experts, int identities, int top, int32_t* ids,
                               float* weights, float* id_weight, void* stream);
+/* ---- operand images: 4-bit microscaled floats and bf16, products, products grouped by expert ---------------------
+ * An image holds rows the way the tensor cores take them, of dtype
+ *   HM_MXFP4  blocks of 32 values along a row: an e8m0 scale 2^e, e = max(floor(log2 max|x|) - 2, -127), and e2m1 codes of x / 2^e (0, 0.5, 1,
+ *             1.5, 2, 3, 4, 6) to nearest, ties to the even code, saturated at 6.  A block with an infinity or a NaN is NaN as a whole.  The last
+ *             block of a row may be short.  17 / 32 bytes per value.
+ *   HM_BF16   bf16, rounded to nearest even: the tiles of hm_pack_bf16_tc, for rows that are rows.
+ * Weights are rows too: one per output feature.  Rows of x, y and of weights to be packed are row-major with `ld` elements from row to row.
+ * Images start on 16-byte boundaries; device pointers belong to the current device (HM_ERR_INVALID otherwise).  With device pointers only, every call is
+ * asynchronous on `stream`, keeps nothing between calls and may run beside others and be captured; make one call on each device before the first
+ * capture.  No counterpart in the reference. */
+HM_API size_t hm_image_bytes(int dtype, int rows, int K);
+/* x [rows, K] (HM_F32 or HM_BF16) -> image; glu != 0: x [rows, 2 K], the image takes silu(first K) * last K, computed in f32. */
+HM_API int hm_image_pack(const void* x, int x_dtype, int rows, int K, size_t ldx, int glu, int dtype, void* image, void* stream);
+/* The values an image stands for; out [rows, K] HM_F32 or HM_BF16 (rounded). */
+HM_API int hm_image_unpack(const void* image, int dtype, int rows, int K, void* out, int out_dtype, size_t ldo, void* stream);
+/* GGUF blocks [rows, K / 32] of 17 bytes (scale byte e + 127; 16 bytes with the codes of values i, low, and i + 16, high) -> HM_MXFP4 image.  K a
+ * multiple of 32. */
+HM_API int hm_image_from_blocks(const void* blocks, int rows, int K, void* image, void* stream);
+/* y [M, N] = x @ W^T from two images of the same dtype; f32 sums; y HM_F32 or HM_BF16 (rounded once). */
+HM_API int hm_gemm_image(const void* x_image, const void* w_image, int dtype, int M, int K, int N, void* y, int y_dtype, size_t ldy, void* stream);
+/* The same for 1 <= M <= 8 rows x that stay as they are (HM_F32 to 2^-22 of a value and 2^-32 of its row's largest, HM_BF16) and an HM_MXFP4
+ * image of weights; K <= 32768. */
+HM_API int hm_gemv_mx4(const void* x, int x_dtype, size_t ldx, const void* w_image, int M, int K, int N, void* y, int y_dtype, size_t ldy, void* stream);
+/* Products grouped by expert.  A pair is a (token, choice) with the expert ids[pair]; ids outside [0, experts) (-1 of hm_post_norm_route) have none.
+ * The images of the experts' weights stand back to back, hm_image_bytes(dtype, N, K) each.  experts <= 1024.
+ * hm_expert_plan groups the pairs, in their order, into image rows that start at a multiple of 128 for every expert.  plan: int32 words
+ *   first [experts + 1] blocks of 128 image rows in front of an expert | count [experts] | place [pairs] image row or -1 | row [hm_expert_plan_rows] pair or -1 */
+HM_API size_t hm_expert_plan_ints(int pairs, int experts);
+HM_API int hm_expert_plan_rows(int pairs, int experts);
+HM_API int hm_expert_plan(const int32_t* ids, int pairs, int experts, int32_t* plan, void* stream);
+/* hm_image_pack into grouped rows: pair p is row p / top of x [pairs / top, K] (top 1: x has a row per pair); image: hm_expert_plan_rows rows, of which
+ * those that no pair has are left as they are. */
+HM_API int hm_expert_pack(const void* x, int x_dtype, int K, size_t ldx, int glu, const int32_t* plan, int pairs, int experts, int top, int dtype, void* image, void* stream);
+/* y [pairs, N]: row p of y = its row of the image @ W[ids[p]]^T; rows of pairs without an expert are left as they are. */
+HM_API int hm_expert_gemm(const void* x_image, const void* w_images, int dtype, const int32_t* plan, int pairs, int experts, int K, int N, void* y, int y_dtype, size_t ldy, void* stream);
+/* The same without a plan for few pairs: x [pairs / top, K] as it is (see hm_gemv_mx4), HM_MXFP4 images; pairs <= 65535. */
+HM_API int hm_expert_gemv(const void* x, int x_dtype, size_t ldx, const void* w_images, const int32_t* ids, int pairs, int top, int experts, int K, int N, void* y, int y_dtype, size_t ldy, void* stream);
+/* y [tokens, W] = resid (f32, or NULL) + sum over the choices j with an expert of weights[t, j] * rows[t * top + j] (HM_F32 or HM_BF16), in their order; y may be
+ * resid. */
+HM_API int hm_expert_sum(const void* rows, int rows_dtype, const int32_t* ids, const float* weights, int tokens, int top, int experts, int W, const float* resid, void* y, int y_dtype, void* stream);
+
 /* argmax with ties to the highest index (src/generate.rs:457-468): logits [rows, n]. */
 HM_API int hm_argmax(const float* logits, int rows, int n, uint32_t* out, void* stream);
 
