@@ -210,6 +210,7 @@ bool on_other_device(std::initializer_list<const void*> ptrs) {
     }
     return false;
 }
+constexpr size_t MAX_LD = 1 << 30;  // elements from row to row of a product
 bool misaligned(const void* p, size_t n) { return ((uintptr_t)p & (n - 1)) != 0; }
 bool is_image_dtype(int d) { return d == HM_MXFP4 || d == HM_BF16; }
 bool is_row_dtype(int d) { return d == HM_F32 || d == HM_BF16; }
@@ -1267,7 +1268,7 @@ static int finish_product(Staging& sg, cudaError_t launched, const char* timeout
 }
 
 int hm_gemm_image(const void* x_image, const void* w_image, int dtype, int M, int K, int N, void* y, int y_dtype, size_t ldy, void* stream) {
-    if (!x_image || !w_image || !y || M < 0 || K < 1 || K > INT_MAX / 4 || N < 1 || N > INT_MAX - 128 || ldy < (size_t)N) return gfail(HM_ERR_INVALID, "hm_gemm_image: bad arguments (ldy >= N)");
+    if (!x_image || !w_image || !y || M < 0 || K < 1 || K > INT_MAX / 4 || N < 1 || N > INT_MAX - 128 || ldy < (size_t)N || ldy > MAX_LD) return gfail(HM_ERR_INVALID, "hm_gemm_image: bad arguments (N <= ldy <= 2^30)");
     if (!is_row_dtype(y_dtype) || !is_image_dtype(dtype)) return gfail(HM_ERR_UNSUPPORTED, "hm_gemm_image: y is HM_F32 or HM_BF16, images HM_MXFP4 or HM_BF16");
     if (misaligned(x_image, 16) || misaligned(w_image, 16) || misaligned(y, row_bytes(y_dtype))) return gfail(HM_ERR_INVALID, "hm_gemm_image: misaligned pointer (images start on 16-byte boundaries)");
     if (M == 0) return HM_OK;
@@ -1361,7 +1362,7 @@ int hm_expert_pack(const void* x, int x_dtype, int K, size_t ldx, int glu, const
 }
 
 int hm_expert_gemm(const void* x_image, const void* w_images, int dtype, const int32_t* plan, int pairs, int experts, int K, int N, void* y, int y_dtype, size_t ldy, void* stream) {
-    if (!x_image || !w_images || !plan || !y || bad_groups(pairs, experts) || K < 1 || K > INT_MAX / 4 || N < 1 || N > INT_MAX - 128 || ldy < (size_t)N) return gfail(HM_ERR_INVALID, "hm_expert_gemm: bad arguments (ldy >= N, experts <= 1024)");
+    if (!x_image || !w_images || !plan || !y || bad_groups(pairs, experts) || K < 1 || K > INT_MAX / 4 || N < 1 || N > INT_MAX - 128 || ldy < (size_t)N || ldy > MAX_LD) return gfail(HM_ERR_INVALID, "hm_expert_gemm: bad arguments (N <= ldy <= 2^30, experts <= 1024)");
     if (!is_row_dtype(y_dtype) || !is_image_dtype(dtype)) return gfail(HM_ERR_UNSUPPORTED, "hm_expert_gemm: y is HM_F32 or HM_BF16, images HM_MXFP4 or HM_BF16");
     if (misaligned(x_image, 16) || misaligned(w_images, 16) || misaligned(plan, 4) || misaligned(y, row_bytes(y_dtype))) return gfail(HM_ERR_INVALID, "hm_expert_gemm: misaligned pointer (images start on 16-byte boundaries)");
     if (pairs == 0) return HM_OK;

@@ -22,45 +22,106 @@ namespace {
 
 constexpr int TN = 192;                      // rows of a unit at most
 constexpr int CHUNK = 8;                     // k-blocks per accumulator
-constexpr int SLOTS = 5;
+constexpr int SLOTS = 4;
 constexpr int EPI_WARPS = 8, THREADS = 64 + EPI_WARPS * 32;
 constexpr int A_SLOT = MX_TILE;              // scales (bf16: unused), 128 features
 constexpr int B_SLOT = 2 * MX_SCALES + TN * 128;
 constexpr int SLOT = A_SLOT + B_SLOT;
-constexpr size_t SMEM = (size_t)SLOTS * SLOT + 1024;
+constexpr int STAGE_LD = IMG_ROWS * 2 + 16;      // bytes of a staged row of 128 bf16: eight of them begin in different banks
+constexpr int STAGE_HALF = 32 * STAGE_LD;        // ... and 16 rows of 128 f32
+constexpr size_t SMEM = (size_t)SLOTS * SLOT + 4 * STAGE_HALF + 1024;
 constexpr int SF_COLS = 24, SF_BASE = 2 * TN;
 constexpr int MAX_SPLIT = 16;
 static_assert(SF_BASE + SLOTS * SF_COLS <= 512, "tensor memory");
 static_assert(TN * IMG_ROWS * 4 <= SLOTS * SLOT, "partial tile");
 
-__device__ __forceinline__ uint64_t desc_sw128(uint32_t smem_addr) {
-    return (uint64_t)((smem_addr >> 4) & 0x3FFF) | (uint64_t)1 << 16 | (uint64_t)(1024 >> 4) << 32 | (uint64_t)1 << 46 | (uint64_t)2 << 61;
+// The warps that copy and multiply stay converged: every lane runs their loops and one, elected in place, issues.  Addresses and
+// descriptors then live in uniform registers; issued from a branch of lane 0 a k-block cost 1300 clocks whatever its MMAs took.
+//
+// Shared-memory descriptors, upper word: rows of 128 bytes in groups of eight, 128-byte swizzle; and 32 rows of 16 bytes, eight rows of 128 bytes in a row.
+constexpr uint32_t DESC_TILE = (1024 >> 4) | 1u << 14 | 2u << 29, DESC_SCALES = (128 >> 4) | 1u << 14;
+__device__ __forceinline__ uint32_t desc_lo(uint32_t smem_addr) { return ((smem_addr >> 4) & 0x3FFF) | 1u << 16; }
+// A k-block: four MMAs of 32 bytes per row, whose end arrives at `done`.  more: adds to the accumulator (0: the first MMA replaces it).
+__device__ __forceinline__ void step_bf16(uint32_t d, uint32_t a, uint32_t b, uint32_t idesc, uint32_t more, uint64_t* done) {
+    asm volatile("{ .reg .pred p, e;\n .reg .b64 x0, x1, x2, x3, y0, y1, y2, y3;\n .reg .b32 t;\n"
+                 "setp.ne.b32 p, %4, 0;\n"
+                 "mov.b64 x0, {%1, %5};\n mov.b64 y0, {%2, %5};\n"
+                 "add.u32 t, %1, 2;\n mov.b64 x1, {t, %5};\n add.u32 t, %2, 2;\n mov.b64 y1, {t, %5};\n"
+                 "add.u32 t, %1, 4;\n mov.b64 x2, {t, %5};\n add.u32 t, %2, 4;\n mov.b64 y2, {t, %5};\n"
+                 "add.u32 t, %1, 6;\n mov.b64 x3, {t, %5};\n add.u32 t, %2, 6;\n mov.b64 y3, {t, %5};\n"
+                 "elect.sync _|e, 0xffffffff;\n"
+                 "@e tcgen05.mma.cta_group::1.kind::f16 [%0], x0, y0, %3, p;\n"
+                 "@e tcgen05.mma.cta_group::1.kind::f16 [%0], x1, y1, %3, 1;\n"
+                 "@e tcgen05.mma.cta_group::1.kind::f16 [%0], x2, y2, %3, 1;\n"
+                 "@e tcgen05.mma.cta_group::1.kind::f16 [%0], x3, y3, %3, 1;\n"
+                 "@e tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%6]; }" ::"r"(d), "r"(a), "r"(b), "r"(idesc), "r"(more), "n"(DESC_TILE), "r"(s32(done)) : "memory");
 }
-// 32 rows of 16 bytes, eight rows of 128 bytes in a row, no swizzle
-__device__ __forceinline__ uint64_t desc_scales(uint32_t smem_addr) { return (uint64_t)((smem_addr >> 4) & 0x3FFF) | (uint64_t)1 << 16 | (uint64_t)(128 >> 4) << 32 | (uint64_t)1 << 46; }
-__device__ __forceinline__ void mma_f16(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t acc) {
-    asm volatile("{ .reg .pred p; setp.ne.b32 p, %4, 0;\n"
-                 "tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p; }" ::"r"(d), "l"(a), "l"(b), "r"(idesc), "r"(acc) : "memory");
-}
-__device__ __forceinline__ void mma_mxf4(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t sa, uint32_t sb, uint32_t acc) {
-    asm volatile("{ .reg .pred p; setp.ne.b32 p, %6, 0;\n"
-                 "tcgen05.mma.cta_group::1.kind::mxf4.block_scale.scale_vec::2X [%0], %1, %2, %3, [%4], [%5], p; }" ::"r"(d), "l"(a), "l"(b), "r"(idesc), "r"(sa), "r"(sb), "r"(acc) : "memory");
-}
-__device__ __forceinline__ void copy_scales(uint32_t taddr, uint32_t smem_addr) {
-    asm volatile("tcgen05.cp.cta_group::1.32x128b.warpx4 [%0], %1;" ::"r"(taddr), "l"(desc_scales(smem_addr)) : "memory");
+// The same on 4-bit codes.  The scales of a block of 128 rows are two times 512 bytes, one for either half of the 256 values, which go to four columns each for
+// all four warps' lanes: features sa -> fa, fa + 4; rows sb -> fb, fb + 8, and of a second block (two) fb + 4, fb + 12.  An MMA of 64 values takes two of a
+// column's four bytes (hi: the idesc of the upper two); the unit's rows begin at column fb + off.
+__device__ __forceinline__ void step_mx(uint32_t d, uint32_t sa, uint32_t a, uint32_t sb, uint32_t b, uint32_t idesc, uint32_t fa, uint32_t off, uint32_t two, uint32_t more, uint64_t* done) {
+    asm volatile("{ .reg .pred p, q, e;\n .reg .b64 x0, x1, x2, x3, y0, y1, y2, y3, s0, s1, s2, s3, s4, s5;\n .reg .b32 t, hi, f4, f8, f12, f16, f20, b0, b1;\n"
+                 "setp.ne.b32 p, %9, 0;\n setp.ne.b32 q, %8, 0;\n"
+                 "mov.b64 s0, {%1, %12};\n add.u32 t, %1, 32;\n mov.b64 s1, {t, %12};\n"
+                 "mov.b64 s2, {%3, %12};\n add.u32 t, %3, 32;\n mov.b64 s3, {t, %12};\n"
+                 "add.u32 t, %3, 64;\n mov.b64 s4, {t, %12};\n add.u32 t, %3, 96;\n mov.b64 s5, {t, %12};\n"
+                 "add.u32 f4, %6, 4;\n add.u32 f8, %6, 8;\n add.u32 f12, %6, 12;\n add.u32 f16, %6, 16;\n add.u32 f20, %6, 20;\n"
+                 "add.u32 b0, f8, %7;\n add.u32 b1, f16, %7;\n or.b32 hi, %5, %13;\n"
+                 "mov.b64 x0, {%2, %11};\n mov.b64 y0, {%4, %11};\n"
+                 "add.u32 t, %2, 2;\n mov.b64 x1, {t, %11};\n add.u32 t, %4, 2;\n mov.b64 y1, {t, %11};\n"
+                 "add.u32 t, %2, 4;\n mov.b64 x2, {t, %11};\n add.u32 t, %4, 4;\n mov.b64 y2, {t, %11};\n"
+                 "add.u32 t, %2, 6;\n mov.b64 x3, {t, %11};\n add.u32 t, %4, 6;\n mov.b64 y3, {t, %11};\n"
+                 "elect.sync _|e, 0xffffffff;\n and.pred q, q, e;\n"
+                 "@e tcgen05.cp.cta_group::1.32x128b.warpx4 [%6], s0;\n"
+                 "@e tcgen05.cp.cta_group::1.32x128b.warpx4 [f4], s1;\n"
+                 "@e tcgen05.cp.cta_group::1.32x128b.warpx4 [f8], s2;\n"
+                 "@e tcgen05.cp.cta_group::1.32x128b.warpx4 [f16], s3;\n"
+                 "@q tcgen05.cp.cta_group::1.32x128b.warpx4 [f12], s4;\n"
+                 "@q tcgen05.cp.cta_group::1.32x128b.warpx4 [f20], s5;\n"
+                 "@e tcgen05.mma.cta_group::1.kind::mxf4.block_scale.scale_vec::2X [%0], x0, y0, %5, [%6], [b0], p;\n"
+                 "@e tcgen05.mma.cta_group::1.kind::mxf4.block_scale.scale_vec::2X [%0], x1, y1, hi, [%6], [b0], 1;\n"
+                 "@e tcgen05.mma.cta_group::1.kind::mxf4.block_scale.scale_vec::2X [%0], x2, y2, %5, [f4], [b1], 1;\n"
+                 "@e tcgen05.mma.cta_group::1.kind::mxf4.block_scale.scale_vec::2X [%0], x3, y3, hi, [f4], [b1], 1;\n"
+                 "@e tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%10]; }" ::"r"(d), "r"(sa), "r"(a), "r"(sb), "r"(b), "r"(idesc), "r"(fa), "r"(off), "r"(two), "r"(more), "r"(s32(done)), "n"(DESC_TILE),
+                 "n"(DESC_SCALES), "n"(2u << 4 | 2u << 29)
+                 : "memory");
 }
 __device__ __forceinline__ void mma_commit(uint64_t* bar) {
-    asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(s32(bar)) : "memory");
+    asm volatile("{ .reg .pred e;\n elect.sync _|e, 0xffffffff;\n @e tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0]; }" ::"r"(s32(bar)) : "memory");
 }
-__device__ __forceinline__ void tmem_ld16(uint32_t (&r)[16], uint32_t addr) {
-    asm volatile("tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%16];"
-                 : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
-                 : "r"(addr));
+__device__ __forceinline__ void expect_tx(uint64_t* b, uint32_t bytes) {
+    asm volatile("{ .reg .pred e;\n .reg .b64 st;\n elect.sync _|e, 0xffffffff;\n @e mbarrier.arrive.expect_tx.shared::cta.b64 st, [%0], %1; }" ::"r"(s32(b)), "r"(bytes) : "memory");
+}
+__device__ __forceinline__ void load(void* dst, const void* src, uint32_t bytes, uint64_t* bar) {
+    asm volatile("{ .reg .pred e;\n elect.sync _|e, 0xffffffff;\n @e cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3]; }" ::"r"(s32(dst)), "l"(src), "r"(bytes), "r"(s32(bar)) : "memory");
+}
+// 32 features (the warp's lanes of the tensor memory) x 32 rows: a lane has one feature of all rows, or, BF16, the fragments that stmatrix takes: of eight
+// rows and eight features lane 4 f + r has feature f, rows 2 r and 2 r + 1.
+template <bool BF16>
+__device__ __forceinline__ int value_row(int lane, int j) { return BF16 ? (j >> 2 & 3) * 8 + (lane & 3) * 2 + (j & 1) : j; }
+template <bool BF16>
+__device__ __forceinline__ int value_feature(int lane, int j) { return BF16 ? (j >> 4) * 16 + (j >> 1 & 1) * 8 + (lane >> 2) : lane; }
+template <bool BF16>
+__device__ __forceinline__ void tmem_read(float (&r)[32], uint32_t addr) {
+    if (BF16) {
+#pragma unroll
+        for (int h = 0; h < 32; h += 16)
+            asm volatile("tcgen05.ld.sync.aligned.16x256b.x4.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%16];"
+                         : "=f"(r[h]), "=f"(r[h + 1]), "=f"(r[h + 2]), "=f"(r[h + 3]), "=f"(r[h + 4]), "=f"(r[h + 5]), "=f"(r[h + 6]), "=f"(r[h + 7]), "=f"(r[h + 8]), "=f"(r[h + 9]), "=f"(r[h + 10]), "=f"(r[h + 11]),
+                           "=f"(r[h + 12]), "=f"(r[h + 13]), "=f"(r[h + 14]), "=f"(r[h + 15])
+                         : "r"(addr + ((uint32_t)h << 16)));
+    } else {
+        asm volatile("tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31}, [%32];"
+                     : "=f"(r[0]), "=f"(r[1]), "=f"(r[2]), "=f"(r[3]), "=f"(r[4]), "=f"(r[5]), "=f"(r[6]), "=f"(r[7]), "=f"(r[8]), "=f"(r[9]), "=f"(r[10]), "=f"(r[11]), "=f"(r[12]), "=f"(r[13]), "=f"(r[14]), "=f"(r[15]),
+                       "=f"(r[16]), "=f"(r[17]), "=f"(r[18]), "=f"(r[19]), "=f"(r[20]), "=f"(r[21]), "=f"(r[22]), "=f"(r[23]), "=f"(r[24]), "=f"(r[25]), "=f"(r[26]), "=f"(r[27]), "=f"(r[28]), "=f"(r[29]), "=f"(r[30]), "=f"(r[31])
+                     : "r"(addr));
+    }
 }
 // Names the registers, so that no use of them moves in front of the wait.
-__device__ __forceinline__ void tmem_wait(uint32_t (&r)[16]) {
+__device__ __forceinline__ void tmem_wait(float (&r)[32]) {
     asm volatile("tcgen05.wait::ld.sync.aligned;"
-                 : "+r"(r[0]), "+r"(r[1]), "+r"(r[2]), "+r"(r[3]), "+r"(r[4]), "+r"(r[5]), "+r"(r[6]), "+r"(r[7]), "+r"(r[8]), "+r"(r[9]), "+r"(r[10]), "+r"(r[11]), "+r"(r[12]), "+r"(r[13]), "+r"(r[14]), "+r"(r[15])
+                 : "+f"(r[0]), "+f"(r[1]), "+f"(r[2]), "+f"(r[3]), "+f"(r[4]), "+f"(r[5]), "+f"(r[6]), "+f"(r[7]), "+f"(r[8]), "+f"(r[9]), "+f"(r[10]), "+f"(r[11]), "+f"(r[12]), "+f"(r[13]), "+f"(r[14]), "+f"(r[15]),
+                   "+f"(r[16]), "+f"(r[17]), "+f"(r[18]), "+f"(r[19]), "+f"(r[20]), "+f"(r[21]), "+f"(r[22]), "+f"(r[23]), "+f"(r[24]), "+f"(r[25]), "+f"(r[26]), "+f"(r[27]), "+f"(r[28]), "+f"(r[29]), "+f"(r[30]), "+f"(r[31])
                  :: "memory");
 }
 
@@ -69,6 +130,7 @@ struct Shared {
     uint32_t tmem;
     volatile int abort_flag;
     int units;
+    int rows[2][TN];  // places of a unit's rows in y, -1: none; units alternate
 };
 
 struct Unit {
@@ -88,8 +150,8 @@ __device__ __forceinline__ Unit unit_at(const ImageGemmArgs& a, const int* ufirs
         }
         r.expert = lo;
         u -= ufirst[lo];
-        rows = __ldg(a.count + lo);
-        base = __ldg(a.first + lo) * IMG_ROWS;
+        rows = __shfl_sync(0xffffffffu, __ldg(a.count + lo), 0);  // the same in all lanes: uniform for the compiler too
+        base = __shfl_sync(0xffffffffu, __ldg(a.first + lo), 0) * IMG_ROWS;
     }
     const int per = (rows + TN - 1) / TN, t = u % per;
     r.tile = u / per;
@@ -102,23 +164,60 @@ __device__ __forceinline__ void store1(const ImageGemmArgs& a, int row, int f, f
     if (a.bf16) static_cast<uint16_t*>(a.y)[(size_t)row * a.ldy + f] = (uint16_t)bf16x2_rne(v, 0.f);
     else static_cast<float*>(a.y)[(size_t)row * a.ldy + f] = v;
 }
-// A warp's 32 features (lane: one) of two rows (-1: none).  bf16: neighbouring lanes swap, so that each stores two features of one row.
-__device__ __forceinline__ void store2(const ImageGemmArgs& a, int r0, int r1, int f, int lane, float v0, float v1) {
-    if (!a.bf16 || !a.wide) {
-        if (f < a.N && r0 >= 0) store1(a, r0, f, v0);
-        if (f < a.N && r1 >= 0) store1(a, r1, f, v1);
-        return;
+// An epilogue warp has 32 features (lane: one) of 32 rows; the four warps of a half bring the rows of 128 features together in shared memory (two buffers in turn,
+// one barrier each) and store them as whole lines, 16 bytes per lane.  Stored from the registers, 4 bytes per lane and a place in y for each, the same tile took
+// three times as long; as bulk copies of one row each, twice.
+struct Stage {
+    unsigned char* buf;  // [2][STAGE_HALF]
+    uint32_t used;       // buffers so far
+    int bar;             // named barrier of the half's warps
+};
+template <typename T, int ROWS, int LD>
+__device__ __forceinline__ void stage_out(const ImageGemmArgs& a, Stage& st, const unsigned char* buf, const int* rows, int n0, int et) {
+    constexpr int PER = 16 / sizeof(T), PIECES = IMG_ROWS / PER;  // values of a piece, pieces of a row
+    asm volatile("bar.sync %0, 128;" ::"r"(st.bar) : "memory");
+    const int nf = min(IMG_ROWS, a.N - n0);
+#pragma unroll
+    for (int i = 0; i < ROWS * PIECES / 128; ++i) {
+        const int piece = i * 128 + et, row = rows[piece / PIECES], c = piece % PIECES * PER;
+        if (row < 0 || c >= nf) continue;
+        const uint4 v = *reinterpret_cast<const uint4*>(buf + piece / PIECES * LD + piece % PIECES * 16);
+        T* y = static_cast<T*>(a.y) + (size_t)row * a.ldy + n0 + c;
+        if (a.wide && c + PER <= nf) *reinterpret_cast<uint4*>(y) = v;
+        else {
+            const uint32_t w[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+            for (int e = 0; e < PER; ++e)
+                if (c + e < nf) y[e] = sizeof(T) == 2 ? (T)(w[e / 2] >> (16 * (e & 1))) : (T)w[e % 4];
+        }
     }
-    const float got = __shfl_xor_sync(0xffffffffu, lane & 1 ? v0 : v1, 1);
-    const int row = lane & 1 ? r1 : r0, g = f & ~1;
-    if (row < 0 || g >= a.N) return;
-    const uint32_t w = lane & 1 ? bf16x2_rne(got, v1) : bf16x2_rne(v0, got);
-    uint16_t* y = static_cast<uint16_t*>(a.y) + (size_t)row * a.ldy + g;
-    if (g + 1 < a.N) *reinterpret_cast<uint32_t*>(y) = w;
-    else *y = (uint16_t)w;
+}
+template <bool BF16>
+__device__ __forceinline__ void emit(const ImageGemmArgs& a, Stage& st, const int* rows, int n0, int et, const float (&v)[32]) {
+    if (BF16) {
+        unsigned char* buf = st.buf + (st.used++ & 1u) * STAGE_HALF;
+        const int lane = et & 31;
+        // eight rows by 32 features at a time: thread 8 g + i names row i of the features' group g
+        const uint32_t at = s32(buf) + (lane & 7) * STAGE_LD + (et & 96) * 2 + (lane >> 3) * 16;
+#pragma unroll
+        for (int j = 0; j < 4; ++j)
+            asm volatile("stmatrix.sync.aligned.m8n8.x4.trans.shared.b16 [%0], {%1, %2, %3, %4};" ::"r"(at + j * 8 * STAGE_LD), "r"(bf16x2_rne(v[4 * j], v[4 * j + 1])), "r"(bf16x2_rne(v[4 * j + 2], v[4 * j + 3])),
+                         "r"(bf16x2_rne(v[16 + 4 * j], v[16 + 4 * j + 1])), "r"(bf16x2_rne(v[16 + 4 * j + 2], v[16 + 4 * j + 3]))
+                         : "memory");
+        stage_out<uint16_t, 32, STAGE_LD>(a, st, buf, rows, n0, et);
+    } else {
+#pragma unroll
+        for (int h = 0; h < 32; h += 16) {
+            unsigned char* buf = st.buf + (st.used++ & 1u) * STAGE_HALF;
+            float* d = reinterpret_cast<float*>(buf) + et;
+#pragma unroll
+            for (int j = 0; j < 16; ++j) d[j * IMG_ROWS] = v[h + j];
+            stage_out<uint32_t, 16, IMG_ROWS * 4>(a, st, buf, rows + h, n0, et);
+        }
+    }
 }
 
-template <bool MX>
+template <bool MX, bool BF16>
 __global__ void __launch_bounds__(THREADS, 1) image_gemm_kernel(const ImageGemmArgs a) {
     extern __shared__ __align__(1024) unsigned char dsm[];
     __shared__ Shared sh;
@@ -156,111 +255,117 @@ __global__ void __launch_bounds__(THREADS, 1) image_gemm_kernel(const ImageGemmA
     asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
     __syncthreads();
     asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-    const uint32_t tmem = sh.tmem;
-    const int units = sh.units;
+    const uint32_t tmem = __shfl_sync(0xffffffffu, sh.tmem, 0), ring_at = __shfl_sync(0xffffffffu, s32(ring), 0);
+    const int units = __shfl_sync(0xffffffffu, sh.units, 0);
     const int rank = blockIdx.x % a.split, step = gridDim.x / a.split, u0 = blockIdx.x / a.split;
     const int kb0 = rank * a.kb_per, kb1 = min(a.kblocks, kb0 + a.kb_per);
     constexpr int TILE = MX ? MX_TILE : IMG_CODES;
 
     uint32_t issued = 0;
     if (warp == 0) {
-        if (lane == 0) {
-            bool ok = true;
-            for (int u = u0; u < units && ok; u += step) {
-                const Unit t = unit_at(a, ufirst, u);
-                const unsigned char* w = a.w + t.expert * a.w_stride + (size_t)t.tile * a.kblocks * TILE;
-                const unsigned char* x = a.x + (size_t)(t.row0 / IMG_ROWS) * a.kblocks * TILE;
-                const size_t x_next = (size_t)a.kblocks * TILE;
-                const int off = t.row0 % IMG_ROWS, n0 = min(t.n, IMG_ROWS - off), n1 = t.n - n0;  // rows in the first and in the second block
-                const uint32_t b0 = (uint32_t)(n0 + 7) / 8 * 1024, b1 = (uint32_t)(n1 + 7) / 8 * 1024;
-                const uint32_t bytes = (uint32_t)TILE + b0 + b1 + (MX ? (n1 > 0 ? 2u : 1u) * MX_SCALES : 0u);
-                for (int kb = kb0; kb < kb1; ++kb, ++issued) {
-                    const uint32_t s = issued % SLOTS;
-                    if (issued >= SLOTS) ok = mb_wait(&sh.empty[s], ((issued / SLOTS) & 1u) ^ 1u, a.err_flag, &sh.abort_flag);
-                    if (!ok) break;
-                    unsigned char *sa = ring + (size_t)s * SLOT, *sb = sa + A_SLOT;
-                    const unsigned char *wk = w + (size_t)kb * TILE, *xk = x + (size_t)kb * TILE;
-                    mb_expect_tx(&sh.full[s], bytes);
-                    bulk_copy(sa + (MX ? 0 : MX_SCALES), wk, TILE, &sh.full[s]);
-                    if (MX) {
-                        bulk_copy(sb, xk, MX_SCALES, &sh.full[s]);
-                        if (n1 > 0) bulk_copy(sb + MX_SCALES, xk + x_next, MX_SCALES, &sh.full[s]);
-                        xk += MX_SCALES;
-                    }
-                    bulk_copy(sb + 2 * MX_SCALES, xk + off * 128, b0, &sh.full[s]);
-                    if (n1 > 0) bulk_copy(sb + 2 * MX_SCALES + n0 * 128, xk + x_next, b1, &sh.full[s]);
+        bool ok = true;
+        for (int u = u0; u < units && ok; u += step) {
+            const Unit t = unit_at(a, ufirst, u);
+            const int off = t.row0 % IMG_ROWS, n0 = min(t.n, IMG_ROWS - off), n1 = t.n - n0;  // rows in the first and in the second block
+            const uint32_t b0 = (uint32_t)(n0 + 7) / 8 * 1024, b1 = (uint32_t)(n1 + 7) / 8 * 1024;
+            const uint32_t bytes = (uint32_t)TILE + b0 + b1 + (MX ? (n1 > 0 ? 2u : 1u) * MX_SCALES : 0u);
+            const unsigned char* w = a.w + t.expert * a.w_stride + ((size_t)t.tile * a.kblocks + kb0) * TILE;
+            const unsigned char* x = a.x + ((size_t)(t.row0 / IMG_ROWS) * a.kblocks + kb0) * TILE;
+            const size_t x_next = (size_t)a.kblocks * TILE;
+            for (int kb = kb0; kb < kb1; ++kb, ++issued, w += TILE, x += TILE) {
+                const uint32_t s = issued % SLOTS;
+                if (issued >= SLOTS) ok = mb_wait(&sh.empty[s], ((issued / SLOTS) & 1u) ^ 1u, a.err_flag, &sh.abort_flag);
+                ok = __all_sync(0xffffffffu, ok);
+                if (!ok) break;
+                unsigned char *sa = ring + (size_t)s * SLOT, *sb = sa + A_SLOT;
+                expect_tx(&sh.full[s], bytes);
+                load(sa + (MX ? 0 : MX_SCALES), w, TILE, &sh.full[s]);
+                if (MX) {
+                    load(sb, x, MX_SCALES, &sh.full[s]);
+                    if (n1 > 0) load(sb + MX_SCALES, x + x_next, MX_SCALES, &sh.full[s]);
                 }
+                const unsigned char* xk = x + (MX ? MX_SCALES : 0);
+                load(sb + 2 * MX_SCALES, xk + off * 128, b0, &sh.full[s]);
+                if (n1 > 0) load(sb + 2 * MX_SCALES + n0 * 128, xk + x_next, b1, &sh.full[s]);
             }
         }
     } else if (warp == 1) {
-        if (lane == 0) {
-            uint32_t i = 0, ci = 0;
-            bool ok = true;
-            for (int u = u0; u < units && ok; u += step) {
-                const Unit t = unit_at(a, ufirst, u);
-                const uint32_t n = (uint32_t)(t.n + 15) & ~15u, sf_off = (uint32_t)(t.row0 % IMG_ROWS) / 32;
-                // D f32, both operands K-major, M 128, N n; bf16, or e2m1 with e8m0 scales
-                const uint32_t idesc = MX ? 1u << 7 | 1u << 10 | (n >> 3) << 17 | 1u << 23 | (128u >> 4) << 24 : 1u << 4 | 1u << 7 | 1u << 10 | (n >> 3) << 17 | (128u >> 4) << 24;
-                for (int kc = kb0; kc < kb1 && ok; kc += CHUNK, ++ci) {
-                    const uint32_t buf = ci & 1u, d = tmem + buf * TN;
-                    if (ci >= 2) ok = mb_wait(&sh.aempty[buf], ((ci >> 1) & 1u) ^ 1u, a.err_flag, &sh.abort_flag);
-                    uint32_t more = 0;
-                    for (int kb = kc; kb < min(kb1, kc + CHUNK) && ok; ++kb, ++i) {
-                        const uint32_t s = i % SLOTS;
-                        ok = mb_wait(&sh.full[s], (i / SLOTS) & 1u, a.err_flag, &sh.abort_flag);
-                        if (!ok) break;
-                        asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-                        const uint32_t sa = s32(ring + (size_t)s * SLOT), sb = sa + A_SLOT, wa = sa + MX_SCALES, xa = sb + 2 * MX_SCALES;
-                        if (MX) {
-                            const uint32_t fa = tmem + SF_BASE + s * SF_COLS, fb = fa + 8;
-#pragma unroll
-                            for (uint32_t h = 0; h < 2; ++h) {
-                                copy_scales(fa + 4 * h, sa + 512 * h);
-                                copy_scales(fb + 8 * h, sb + 512 * h);
-                                copy_scales(fb + 8 * h + 4, sb + MX_SCALES + 512 * h);  // (not loaded where the unit ends in its first block: then nobody reads it)
-                            }
-#pragma unroll
-                            for (uint32_t j = 0; j < 4; ++j) {
-                                const uint32_t id = (j & 1) * 2;
-                                mma_mxf4(d, desc_sw128(wa + j * 32), desc_sw128(xa + j * 32), idesc | id << 4 | id << 29, fa + 4 * (j >> 1), fb + 8 * (j >> 1) + sf_off, more);
-                                more = 1;
-                            }
-                        } else {
-#pragma unroll
-                            for (uint32_t j = 0; j < 4; ++j) {
-                                mma_f16(d, desc_sw128(wa + j * 32), desc_sw128(xa + j * 32), idesc, more);
-                                more = 1;
-                            }
-                        }
-                        mma_commit(&sh.empty[s]);
-                    }
-                    if (ok) mma_commit(&sh.afull[buf]);
+        // No wait's result decides anything here: where one has run out, the others return at once and the MMAs read what is there, whose
+        // results nobody uses.
+        uint32_t i = 0, ci = 0;
+        for (int u = u0; u < units; u += step) {
+            const Unit t = unit_at(a, ufirst, u);
+            const uint32_t off = (uint32_t)t.row0 % IMG_ROWS, n = ((uint32_t)t.n + 15) & ~15u, two = t.n + off > IMG_ROWS;
+            // D f32, both operands K-major, M 128, N n; bf16, or e2m1 with e8m0 scales
+            const uint32_t idesc = MX ? 1u << 7 | 1u << 10 | (n >> 3) << 17 | 1u << 23 | (128u >> 4) << 24 : 1u << 4 | 1u << 7 | 1u << 10 | (n >> 3) << 17 | (128u >> 4) << 24;
+            for (int kc = kb0; kc < kb1; kc += CHUNK, ++ci) {
+                const uint32_t buf = ci & 1u, d = tmem + buf * TN;
+                if (ci >= 2) mb_wait(&sh.aempty[buf], ((ci >> 1) & 1u) ^ 1u, a.err_flag, &sh.abort_flag);
+                const int ke = min(kb1, kc + CHUNK);
+                for (int kb = kc; kb < ke; ++kb, ++i) {
+                    const uint32_t s = i % SLOTS;
+                    mb_wait(&sh.full[s], (i / SLOTS) & 1u, a.err_flag, &sh.abort_flag);
+                    asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+                    const uint32_t sa = desc_lo(ring_at + s * SLOT), wa = sa + (MX_SCALES >> 4), sb = sa + (A_SLOT >> 4), xa = sb + (2 * MX_SCALES >> 4);
+                    if (MX) step_mx(d, sa, wa, sb, xa, idesc, tmem + SF_BASE + s * SF_COLS, off / 32, two, kb > kc, &sh.empty[s]);
+                    else step_bf16(d, wa, xa, idesc, kb > kc, &sh.empty[s]);
                 }
+                mma_commit(&sh.afull[buf]);
             }
         }
     } else {
-        const int quarter = warp & 3, half = (warp - 2) >> 2;  // a warp reads its own quarter of the TMEM lanes; chunks of 16 rows alternate
-        const uint32_t tbase = tmem + ((uint32_t)(quarter * 32) << 16);
-        uint32_t ci = 0;
-        float acc[TN / 2];
-        for (int u = u0; u < units; u += step) {
+        const int quarter = warp & 3, half = (warp - 2) >> 2;  // a warp reads its own quarter of the TMEM lanes; chunks of 32 rows alternate
+        const uint32_t tbase = tmem + ((uint32_t)(quarter * 32) << 16) + half * 32;
+        const int et = tid - 64, qt = quarter * 32 + lane;
+        uint32_t ci = 0, ui = 0;
+        Stage st{ring + (size_t)SLOTS * SLOT + half * 2 * STAGE_HALF, 0, 2 + half};
+        const bool whole = kb1 - kb0 <= CHUNK && a.split == 1;  // one accumulator per unit
+        for (int u = u0; u < units; u += step, ++ui) {
             const Unit t = unit_at(a, ufirst, u);
-            const int f = t.tile * IMG_ROWS + quarter * 32 + lane;
+            const int n0 = t.tile * IMG_ROWS, *rows = sh.rows[ui & 1] + half * 32;
+            // (nobody reads the entries of the unit before the last: its readers have met at the barrier of the last one)
+            if (et < TN) sh.rows[ui & 1][et] = et < t.n ? (a.row ? __ldg(a.row + t.row0 + et) : t.row0 + et) : -1;
+            asm volatile("bar.sync 1, 256;" ::: "memory");
+            if (whole) {  // small code: the loops of the other warps stay in the instruction cache
+                const uint32_t buf = ci & 1u;
+                const bool ok = __all_sync(0xffffffffu, mb_wait(&sh.afull[buf], (ci >> 1) & 1u, a.err_flag, &sh.abort_flag));
+                ++ci;
+                asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+                float v[32];
+                if (half * 32 < t.n) tmem_read<BF16>(v, tbase + buf * TN);
+#pragma unroll 1
+                for (int col = 0; col + half * 32 < t.n; col += 64) {
+                    float now[32];
+                    tmem_wait(v);
 #pragma unroll
-            for (int j = 0; j < TN / 2; ++j) acc[j] = 0.f;
+                    for (int j = 0; j < 32; ++j) now[j] = v[j];
+                    if (col + 64 + half * 32 < t.n) tmem_read<BF16>(v, tbase + buf * TN + col + 64);  // the next rows, while these leave
+                    else {
+                        asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+                        if (ok && lane == 0) mb_arrive(&sh.aempty[buf]);
+                    }
+                    emit<BF16>(a, st, rows + col, n0, qt, now);
+                }
+                if (half * 32 >= t.n && ok && lane == 0) mb_arrive(&sh.aempty[buf]);
+                continue;
+            }
+            float acc[TN / 64][32];
+#pragma unroll
+            for (int c = 0; c < TN / 64; ++c)
+#pragma unroll
+                for (int j = 0; j < 32; ++j) acc[c][j] = 0.f;
             for (int kc = kb0; kc < kb1; kc += CHUNK, ++ci) {
                 const uint32_t buf = ci & 1u;
                 if (!__all_sync(0xffffffffu, mb_wait(&sh.afull[buf], (ci >> 1) & 1u, a.err_flag, &sh.abort_flag))) continue;
                 asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
 #pragma unroll
-                for (int c = 0; c < TN / 32; ++c) {
-                    const int col = (2 * c + half) * 16;
-                    if (col < t.n) {
-                        uint32_t r[16];
-                        tmem_ld16(r, tbase + buf * TN + col);
-                        tmem_wait(r);
+                for (int c = 0; c < TN / 64; ++c) {
+                    if (c * 64 + half * 32 < t.n) {
+                        float v[32];
+                        tmem_read<BF16>(v, tbase + buf * TN + c * 64);
+                        tmem_wait(v);
 #pragma unroll
-                        for (int j = 0; j < 16; ++j) acc[c * 16 + j] += __uint_as_float(r[j]);
+                        for (int j = 0; j < 32; ++j) acc[c][j] += v[j];
                     }
                 }
                 asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
@@ -270,32 +375,24 @@ __global__ void __launch_bounds__(THREADS, 1) image_gemm_kernel(const ImageGemmA
             if (a.split > 1) {  // one unit per cluster: the ring is read, the partial tile [rows][128 features] takes its place
                 float* part = reinterpret_cast<float*>(ring);
 #pragma unroll
-                for (int c = 0; c < TN / 32; ++c)
+                for (int c = 0; c < TN / 64; ++c)
 #pragma unroll
-                    for (int j = 0; j < 16; ++j) {
-                        const int col = (2 * c + half) * 16 + j;
-                        if (col < t.n) part[col * IMG_ROWS + quarter * 32 + lane] = acc[c * 16 + j];
+                    for (int j = 0; j < 32; ++j) {
+                        const int col = c * 64 + half * 32 + value_row<BF16>(lane, j);
+                        if (col < t.n) part[col * IMG_ROWS + quarter * 32 + value_feature<BF16>(lane, j)] = acc[c][j];
                     }
                 break;
             }
 #pragma unroll
-            for (int c = 0; c < TN / 32; ++c) {
-                const int col = (2 * c + half) * 16;
-                if (col < t.n) {
-                    int row = -1;  // where row col + lane of the unit goes
-                    if (lane < 16 && col + lane < t.n) row = a.row ? __ldg(a.row + t.row0 + col + lane) : t.row0 + col + lane;
-#pragma unroll
-                    for (int j = 0; j < 16; j += 2)
-                        store2(a, __shfl_sync(0xffffffffu, row, j), __shfl_sync(0xffffffffu, row, j + 1), f, lane, acc[c * 16 + j], acc[c * 16 + j + 1]);
-                }
-            }
+            for (int c = 0; c < TN / 64; ++c)
+                if (c * 64 + half * 32 < t.n) emit<BF16>(a, st, rows + c * 64, n0, qt, acc[c]);
         }
     }
     asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
     __syncthreads();
     if (sh.abort_flag) {  // a wait ran out: the copies and MMAs in flight end before the CTA does and its accumulators are freed
-        if (tid == 0) mb_land_ring(sh.full, issued, SLOTS);
-        else if (tid == 32) {
+        if (warp == 0) mb_land_ring(sh.full, issued, SLOTS);
+        else if (warp == 1) {
             mma_commit(&sh.done);
             mb_land(&sh.done, 0);
         }
@@ -328,8 +425,9 @@ __global__ void __launch_bounds__(THREADS, 1) image_gemm_kernel(const ImageGemmA
 cudaError_t launch_image_gemm(ImageGemmArgs a, bool mx, int sm_count, cudaStream_t st) {
     a.kblocks = img_kblocks(mx, a.K);
     a.tiles = (a.N + IMG_ROWS - 1) / IMG_ROWS;
-    a.wide = a.ldy % 2 == 0 && (uintptr_t)a.y % 4 == 0;
-    const void* fn = mx ? reinterpret_cast<const void*>(image_gemm_kernel<true>) : reinterpret_cast<const void*>(image_gemm_kernel<false>);
+    a.wide = a.ldy * (a.bf16 ? 2 : 4) % 16 == 0 && (uintptr_t)a.y % 16 == 0;
+    void (*const kernels[2][2])(ImageGemmArgs) = {{image_gemm_kernel<false, false>, image_gemm_kernel<false, true>}, {image_gemm_kernel<true, false>, image_gemm_kernel<true, true>}};
+    void (*const fn)(ImageGemmArgs) = kernels[mx][a.bf16 != 0];
     cudaError_t e = ensure_dyn_smem(fn, SMEM);
     if (e != cudaSuccess) return e;
     long long units;
@@ -357,7 +455,7 @@ cudaError_t launch_image_gemm(ImageGemmArgs a, bool mx, int sm_count, cudaStream
         cfg.attrs = at;
         cfg.numAttrs = 1;
     }
-    return mx ? cudaLaunchKernelEx(&cfg, image_gemm_kernel<true>, a) : cudaLaunchKernelEx(&cfg, image_gemm_kernel<false>, a);
+    return cudaLaunchKernelEx(&cfg, fn, a);
 }
 
 }  // namespace hm
