@@ -55,7 +55,7 @@ class Staging {
     }
     template <typename T>
     const T* in(const T* p, size_t count) {
-        if (!p || is_device_ptr(p)) return p;
+        if (!p || is_device(p)) return p;
         void* d = nullptr;
         if (!ok(cudaMalloc(&d, std::max<size_t>(count * sizeof(T), 16)))) return nullptr;
         owned_.push_back(d);
@@ -64,7 +64,7 @@ class Staging {
     }
     template <typename T>
     T* out(T* p, size_t count, bool copy_in = false) {
-        if (!p || is_device_ptr(p)) return p;
+        if (!p || is_device(p)) return p;
         void* d = nullptr;
         if (!ok(cudaMalloc(&d, std::max<size_t>(count * sizeof(T), 16)))) return nullptr;
         owned_.push_back(d);
@@ -80,6 +80,8 @@ class Staging {
         return d;
     }
     bool staged() const { return !owned_.empty(); }
+    // Whether a pointer was memory of another GPU than the current one.
+    bool elsewhere() const { return elsewhere_; }
     bool ok(cudaError_t e) {
         if (e != cudaSuccess && err_ == cudaSuccess) err_ = e;
         return e == cudaSuccess;
@@ -100,6 +102,20 @@ class Staging {
         void* dev;
         size_t bytes;
     };
+    bool is_device(const void* p) {
+        cudaPointerAttributes at;
+        if (cudaPointerGetAttributes(&at, p) != cudaSuccess) {
+            cudaGetLastError();
+            return false;
+        }
+        if (at.type == cudaMemoryTypeDevice) {
+            if (device_ < 0 && cudaGetDevice(&device_) != cudaSuccess) device_ = at.device;
+            elsewhere_ |= at.device != device_;
+        }
+        return at.type == cudaMemoryTypeDevice || at.type == cudaMemoryTypeManaged;
+    }
+    int device_ = -1;
+    bool elsewhere_ = false;
     cudaStream_t st_;
     std::vector<void*> owned_;
     std::vector<Out> outs_;
@@ -195,22 +211,8 @@ bool have_device() {
     return n > 0;
 }
 
-// Device memory of another GPU than the current one among these pointers (host pointers and null do not count).
-bool on_other_device(std::initializer_list<const void*> ptrs) {
-    int dev = 0;
-    if (cudaGetDevice(&dev) != cudaSuccess) return false;
-    for (const void* p : ptrs) {
-        cudaPointerAttributes at;
-        if (!p) continue;
-        if (cudaPointerGetAttributes(&at, p) != cudaSuccess) {
-            cudaGetLastError();
-            continue;
-        }
-        if (at.type == cudaMemoryTypeDevice && at.device != dev) return true;
-    }
-    return false;
-}
 constexpr size_t MAX_LD = 1 << 30;  // elements from row to row of a product
+constexpr int MAX_K = 1 << 23;      // values of an image's row
 bool misaligned(const void* p, size_t n) { return ((uintptr_t)p & (n - 1)) != 0; }
 bool is_image_dtype(int d) { return d == HM_MXFP4 || d == HM_BF16; }
 bool is_row_dtype(int d) { return d == HM_F32 || d == HM_BF16; }
@@ -1207,12 +1209,11 @@ size_t hm_image_bytes(int dtype, int rows, int K) { return rows < 1 || K < 1 || 
 
 int hm_image_pack(const void* x, int x_dtype, int rows, int K, size_t ldx, int glu, int dtype, void* image, void* stream) {
     const int width = glu ? 2 : 1;
-    if (!x || !image || rows < 0 || K < 1 || K > INT_MAX / 4 || ldx < (size_t)K * width) return gfail(HM_ERR_INVALID, "hm_image_pack: bad arguments (ldx >= K, 2 K with glu)");
+    if (!x || !image || rows < 0 || K < 1 || K > MAX_K || ldx < (size_t)K * width) return gfail(HM_ERR_INVALID, "hm_image_pack: bad arguments (ldx >= K, 2 K with glu)");
     if (!is_row_dtype(x_dtype) || !is_image_dtype(dtype)) return gfail(HM_ERR_UNSUPPORTED, "hm_image_pack: rows are HM_F32 or HM_BF16, images HM_MXFP4 or HM_BF16");
     if (misaligned(x, row_bytes(x_dtype)) || misaligned(image, 16)) return gfail(HM_ERR_INVALID, "hm_image_pack: misaligned pointer (images start on 16-byte boundaries)");
     if (rows == 0) return HM_OK;
     NEED_DEVICE();
-    if (on_other_device({x, image})) return gfail(HM_ERR_INVALID, "hm_image_pack: memory of another device than the current one");
     cudaStream_t st = (cudaStream_t)stream;
     Staging sg(st);
     const bool mx = dtype == HM_MXFP4;
@@ -1225,22 +1226,23 @@ int hm_image_pack(const void* x, int x_dtype, int rows, int K, size_t ldx, int g
     a.K = K;
     a.image = sg.out((unsigned char*)image, img_bytes(mx, rows, K), true);
     if (!a.x || !a.image) return sg.finish(cudaErrorMemoryAllocation);
+    if (sg.elsewhere()) return gfail(HM_ERR_INVALID, "hm_image_pack: memory of another device than the current one");
     return sg.finish(launch_image_pack(a, mx, st));
 }
 
 int hm_image_unpack(const void* image, int dtype, int rows, int K, void* out, int out_dtype, size_t ldo, void* stream) {
-    if (!image || !out || rows < 0 || K < 1 || K > INT_MAX / 4 || ldo < (size_t)K) return gfail(HM_ERR_INVALID, "hm_image_unpack: bad arguments (ldo >= K)");
+    if (!image || !out || rows < 0 || K < 1 || K > MAX_K || ldo < (size_t)K) return gfail(HM_ERR_INVALID, "hm_image_unpack: bad arguments (ldo >= K)");
     if (!is_row_dtype(out_dtype) || !is_image_dtype(dtype)) return gfail(HM_ERR_UNSUPPORTED, "hm_image_unpack: rows are HM_F32 or HM_BF16, images HM_MXFP4 or HM_BF16");
     if (misaligned(out, row_bytes(out_dtype)) || misaligned(image, 16)) return gfail(HM_ERR_INVALID, "hm_image_unpack: misaligned pointer (images start on 16-byte boundaries)");
     if (rows == 0) return HM_OK;
     NEED_DEVICE();
-    if (on_other_device({image, out})) return gfail(HM_ERR_INVALID, "hm_image_unpack: memory of another device than the current one");
     cudaStream_t st = (cudaStream_t)stream;
     Staging sg(st);
     const bool mx = dtype == HM_MXFP4;
     const unsigned char* im = sg.in((const unsigned char*)image, img_bytes(mx, rows, K));
     uint8_t* o = sg.out((uint8_t*)out, span_bytes(rows, K, ldo, out_dtype), true);
     if (!im || !o) return sg.finish(cudaErrorMemoryAllocation);
+    if (sg.elsewhere()) return gfail(HM_ERR_INVALID, "hm_image_unpack: memory of another device than the current one");
     return sg.finish(launch_image_unpack(im, mx, rows, K, o, out_dtype == HM_BF16, ldo, st));
 }
 
@@ -1249,12 +1251,12 @@ int hm_image_from_blocks(const void* blocks, int rows, int K, void* image, void*
     if (misaligned(image, 16)) return gfail(HM_ERR_INVALID, "hm_image_from_blocks: images start on 16-byte boundaries");
     if (rows == 0) return HM_OK;
     NEED_DEVICE();
-    if (on_other_device({blocks, image})) return gfail(HM_ERR_INVALID, "hm_image_from_blocks: memory of another device than the current one");
     cudaStream_t st = (cudaStream_t)stream;
     Staging sg(st);
     const uint8_t* b = sg.in((const uint8_t*)blocks, (size_t)rows * (K / 32) * 17);
     unsigned char* im = sg.out((unsigned char*)image, img_bytes(true, rows, K), true);
     if (!b || !im) return sg.finish(cudaErrorMemoryAllocation);
+    if (sg.elsewhere()) return gfail(HM_ERR_INVALID, "hm_image_from_blocks: memory of another device than the current one");
     return sg.finish(launch_image_blocks(b, rows, K, im, st));
 }
 
@@ -1268,12 +1270,11 @@ static int finish_product(Staging& sg, cudaError_t launched, const char* timeout
 }
 
 int hm_gemm_image(const void* x_image, const void* w_image, int dtype, int M, int K, int N, void* y, int y_dtype, size_t ldy, void* stream) {
-    if (!x_image || !w_image || !y || M < 0 || K < 1 || K > INT_MAX / 4 || N < 1 || N > INT_MAX - 128 || ldy < (size_t)N || ldy > MAX_LD) return gfail(HM_ERR_INVALID, "hm_gemm_image: bad arguments (N <= ldy <= 2^30)");
+    if (!x_image || !w_image || !y || M < 0 || K < 1 || K > MAX_K || N < 1 || N > INT_MAX - 128 || ldy < (size_t)N || ldy > MAX_LD) return gfail(HM_ERR_INVALID, "hm_gemm_image: bad arguments (N <= ldy <= 2^30)");
     if (!is_row_dtype(y_dtype) || !is_image_dtype(dtype)) return gfail(HM_ERR_UNSUPPORTED, "hm_gemm_image: y is HM_F32 or HM_BF16, images HM_MXFP4 or HM_BF16");
     if (misaligned(x_image, 16) || misaligned(w_image, 16) || misaligned(y, row_bytes(y_dtype))) return gfail(HM_ERR_INVALID, "hm_gemm_image: misaligned pointer (images start on 16-byte boundaries)");
     if (M == 0) return HM_OK;
     NEED_DEVICE();
-    if (on_other_device({x_image, w_image, y})) return gfail(HM_ERR_INVALID, "hm_gemm_image: memory of another device than the current one");
     cudaStream_t st = (cudaStream_t)stream;
     Staging sg(st);
     const bool mx = dtype == HM_MXFP4;
@@ -1287,6 +1288,7 @@ int hm_gemm_image(const void* x_image, const void* w_image, int dtype, int M, in
     a.ldy = ldy;
     a.bf16 = y_dtype == HM_BF16;
     if (!a.x || !a.w || !a.y) return sg.finish(cudaErrorMemoryAllocation);
+    if (sg.elsewhere()) return gfail(HM_ERR_INVALID, "hm_gemm_image: memory of another device than the current one");
     if (!sg.ok(get_wait_err(&a.err_flag))) return sg.finish(cudaSuccess);
     return finish_product(sg, launch_image_gemm(a, mx, sm_count_of_current_device(), st), "hm_gemm_image: a bounded device-side wait ran out");
 }
@@ -1297,7 +1299,6 @@ int hm_gemv_mx4(const void* x, int x_dtype, size_t ldx, const void* w_image, int
     if (misaligned(x, row_bytes(x_dtype)) || misaligned(w_image, 16) || misaligned(y, row_bytes(y_dtype))) return gfail(HM_ERR_INVALID, "hm_gemv_mx4: misaligned pointer (images start on 16-byte boundaries)");
     if (M == 0) return HM_OK;
     NEED_DEVICE();
-    if (on_other_device({x, w_image, y})) return gfail(HM_ERR_INVALID, "hm_gemv_mx4: memory of another device than the current one");
     cudaStream_t st = (cudaStream_t)stream;
     Staging sg(st);
     MxGemvArgs a{};
@@ -1312,6 +1313,7 @@ int hm_gemv_mx4(const void* x, int x_dtype, size_t ldx, const void* w_image, int
     a.ldy = ldy;
     a.y_bf16 = y_dtype == HM_BF16;
     if (!a.x || !a.w || !a.y) return sg.finish(cudaErrorMemoryAllocation);
+    if (sg.elsewhere()) return gfail(HM_ERR_INVALID, "hm_gemv_mx4: memory of another device than the current one");
     if (!sg.ok(get_wait_err(&a.err_flag))) return sg.finish(cudaSuccess);
     return finish_product(sg, launch_mx4_gemv(a, sm_count_of_current_device(), st), "hm_gemv_mx4: a bounded device-side wait ran out");
 }
@@ -1324,24 +1326,23 @@ int hm_expert_plan(const int32_t* ids, int pairs, int experts, int32_t* plan, vo
     if (!plan || (!ids && pairs > 0) || bad_groups(pairs, experts)) return gfail(HM_ERR_INVALID, "hm_expert_plan: bad arguments (experts <= 1024, pairs <= 2^28)");
     if (misaligned(ids, 4) || misaligned(plan, 4)) return gfail(HM_ERR_INVALID, "hm_expert_plan: misaligned pointer");
     NEED_DEVICE();
-    if (on_other_device({ids, plan})) return gfail(HM_ERR_INVALID, "hm_expert_plan: memory of another device than the current one");
     cudaStream_t st = (cudaStream_t)stream;
     Staging sg(st);
     const int32_t* id = sg.in(ids, (size_t)pairs);
     int32_t* p = sg.out(plan, plan_ints(pairs, experts));
     if ((pairs > 0 && !id) || !p) return sg.finish(cudaErrorMemoryAllocation);
+    if (sg.elsewhere()) return gfail(HM_ERR_INVALID, "hm_expert_plan: memory of another device than the current one");
     return sg.finish(launch_plan(id, plan_at(p, pairs, experts), st));
 }
 
 int hm_expert_pack(const void* x, int x_dtype, int K, size_t ldx, int glu, const int32_t* plan, int pairs, int experts, int top, int dtype, void* image, void* stream) {
     const int width = glu ? 2 : 1;
-    if (!x || !plan || !image || K < 1 || K > INT_MAX / 4 || ldx < (size_t)K * width || bad_groups(pairs, experts) || top < 1 || pairs % top != 0)
+    if (!x || !plan || !image || K < 1 || K > MAX_K || ldx < (size_t)K * width || bad_groups(pairs, experts) || top < 1 || pairs % top != 0)
         return gfail(HM_ERR_INVALID, "hm_expert_pack: bad arguments (ldx >= K, 2 K with glu; pairs a multiple of top; experts <= 1024)");
     if (!is_row_dtype(x_dtype) || !is_image_dtype(dtype)) return gfail(HM_ERR_UNSUPPORTED, "hm_expert_pack: rows are HM_F32 or HM_BF16, images HM_MXFP4 or HM_BF16");
     if (misaligned(x, row_bytes(x_dtype)) || misaligned(plan, 4) || misaligned(image, 16)) return gfail(HM_ERR_INVALID, "hm_expert_pack: misaligned pointer (images start on 16-byte boundaries)");
     if (pairs == 0) return HM_OK;
     NEED_DEVICE();
-    if (on_other_device({x, plan, image})) return gfail(HM_ERR_INVALID, "hm_expert_pack: memory of another device than the current one");
     cudaStream_t st = (cudaStream_t)stream;
     Staging sg(st);
     const bool mx = dtype == HM_MXFP4;
@@ -1358,16 +1359,16 @@ int hm_expert_pack(const void* x, int x_dtype, int K, size_t ldx, int glu, const
     a.src_rows = pairs / top;
     a.image = sg.out((unsigned char*)image, img_bytes(mx, p.rows, K), true);
     if (!p.first || !a.x || !a.image) return sg.finish(cudaErrorMemoryAllocation);
+    if (sg.elsewhere()) return gfail(HM_ERR_INVALID, "hm_expert_pack: memory of another device than the current one");
     return sg.finish(launch_image_pack(a, mx, st));
 }
 
 int hm_expert_gemm(const void* x_image, const void* w_images, int dtype, const int32_t* plan, int pairs, int experts, int K, int N, void* y, int y_dtype, size_t ldy, void* stream) {
-    if (!x_image || !w_images || !plan || !y || bad_groups(pairs, experts) || K < 1 || K > INT_MAX / 4 || N < 1 || N > INT_MAX - 128 || ldy < (size_t)N || ldy > MAX_LD) return gfail(HM_ERR_INVALID, "hm_expert_gemm: bad arguments (N <= ldy <= 2^30, experts <= 1024)");
+    if (!x_image || !w_images || !plan || !y || bad_groups(pairs, experts) || K < 1 || K > MAX_K || N < 1 || N > INT_MAX - 128 || ldy < (size_t)N || ldy > MAX_LD) return gfail(HM_ERR_INVALID, "hm_expert_gemm: bad arguments (N <= ldy <= 2^30, experts <= 1024)");
     if (!is_row_dtype(y_dtype) || !is_image_dtype(dtype)) return gfail(HM_ERR_UNSUPPORTED, "hm_expert_gemm: y is HM_F32 or HM_BF16, images HM_MXFP4 or HM_BF16");
     if (misaligned(x_image, 16) || misaligned(w_images, 16) || misaligned(plan, 4) || misaligned(y, row_bytes(y_dtype))) return gfail(HM_ERR_INVALID, "hm_expert_gemm: misaligned pointer (images start on 16-byte boundaries)");
     if (pairs == 0) return HM_OK;
     NEED_DEVICE();
-    if (on_other_device({x_image, w_images, plan, y})) return gfail(HM_ERR_INVALID, "hm_expert_gemm: memory of another device than the current one");
     cudaStream_t st = (cudaStream_t)stream;
     Staging sg(st);
     const bool mx = dtype == HM_MXFP4;
@@ -1387,6 +1388,7 @@ int hm_expert_gemm(const void* x_image, const void* w_images, int dtype, const i
     a.experts = experts;
     a.pairs = pairs;
     if (!p.first || !a.x || !a.w || !a.y) return sg.finish(cudaErrorMemoryAllocation);
+    if (sg.elsewhere()) return gfail(HM_ERR_INVALID, "hm_expert_gemm: memory of another device than the current one");
     if (!sg.ok(get_wait_err(&a.err_flag))) return sg.finish(cudaSuccess);
     return finish_product(sg, launch_image_gemm(a, mx, sm_count_of_current_device(), st), "hm_expert_gemm: a bounded device-side wait ran out");
 }
@@ -1398,7 +1400,6 @@ int hm_expert_gemv(const void* x, int x_dtype, size_t ldx, const void* w_images,
     if (misaligned(x, row_bytes(x_dtype)) || misaligned(w_images, 16) || misaligned(ids, 4) || misaligned(y, row_bytes(y_dtype))) return gfail(HM_ERR_INVALID, "hm_expert_gemv: misaligned pointer (images start on 16-byte boundaries)");
     if (pairs == 0) return HM_OK;
     NEED_DEVICE();
-    if (on_other_device({x, w_images, ids, y})) return gfail(HM_ERR_INVALID, "hm_expert_gemv: memory of another device than the current one");
     cudaStream_t st = (cudaStream_t)stream;
     Staging sg(st);
     MxGemvArgs a{};
@@ -1418,6 +1419,7 @@ int hm_expert_gemv(const void* x, int x_dtype, size_t ldx, const void* w_images,
     a.top = top;
     a.experts = experts;
     if (!a.x || !a.w || !a.y || !a.ids) return sg.finish(cudaErrorMemoryAllocation);
+    if (sg.elsewhere()) return gfail(HM_ERR_INVALID, "hm_expert_gemv: memory of another device than the current one");
     if (!sg.ok(get_wait_err(&a.err_flag))) return sg.finish(cudaSuccess);
     return finish_product(sg, launch_mx4_gemv(a, sm_count_of_current_device(), st), "hm_expert_gemv: a bounded device-side wait ran out");
 }
@@ -1428,7 +1430,6 @@ int hm_expert_sum(const void* rows, int rows_dtype, const int32_t* ids, const fl
     if (misaligned(rows, row_bytes(rows_dtype)) || misaligned(ids, 4) || misaligned(weights, 4) || misaligned(resid, 4) || misaligned(y, row_bytes(y_dtype))) return gfail(HM_ERR_INVALID, "hm_expert_sum: misaligned pointer");
     if (tokens == 0) return HM_OK;
     NEED_DEVICE();
-    if (on_other_device({rows, ids, weights, resid, y})) return gfail(HM_ERR_INVALID, "hm_expert_sum: memory of another device than the current one");
     cudaStream_t st = (cudaStream_t)stream;
     Staging sg(st);
     SumArgs a{};
@@ -1444,6 +1445,7 @@ int hm_expert_sum(const void* rows, int rows_dtype, const int32_t* ids, const fl
     a.y = sg.out((uint8_t*)y, (size_t)tokens * W * row_bytes(y_dtype));
     a.y_bf16 = y_dtype == HM_BF16;
     if (!a.rows || !a.ids || !a.weights || (resid && !a.resid) || !a.y) return sg.finish(cudaErrorMemoryAllocation);
+    if (sg.elsewhere()) return gfail(HM_ERR_INVALID, "hm_expert_sum: memory of another device than the current one");
     return sg.finish(launch_expert_sum(a, st));
 }
 

@@ -1,7 +1,7 @@
 // Rows into operand images and back, the plan that groups rows by expert, and the weighted sum of the experts' results.
 //
-//   pack_kernel     a warp per row and k-block (128 bytes of the image: one line): a lane has 4 bytes of codes (eight values) or 4 bytes of bf16 (two).
-//                   Bound by the bytes of x: each warp asks for PACK_UNITS units before it works on the first.
+//   pack_kernel     a warp per row and up to four k-blocks (128 bytes of the image each: one line): a lane has 4 bytes of codes (eight values) or 4
+//                   bytes of bf16 (two).  Bound by the bytes of x.
 //   unpack_kernel   the way back
 //   blocks_kernel   GGUF blocks into the image
 //   plan_kernel     stable counting sort of the pairs by expert: a CTA per expert reads all ids (they stay in the L2), so that neither order nor
@@ -10,46 +10,16 @@
 #include "image.h"
 
 #include <algorithm>
+#include <type_traits>
 
 namespace hm {
 namespace {
 
 constexpr int THREADS = 256, WARPS = THREADS / 32;
-constexpr int PACK_UNITS = 4;
 
 __device__ __forceinline__ float load1(const void* x, int bf16, size_t i) { return bf16 ? bf16_bits_to_f32(__ldg(static_cast<const uint16_t*>(x) + i)) : __ldg(static_cast<const float*>(x) + i); }
 
-// Eight values from element i on (16-byte aligned), or fewer: n exist, the others are zero.
-template <bool BF16>
-__device__ __forceinline__ void load8(const void* x, size_t i, int n, bool aligned, float (&v)[8]) {
-    if (aligned && n >= 8) {
-        if (BF16) {
-            const uint4 u = __ldg(reinterpret_cast<const uint4*>(static_cast<const uint16_t*>(x) + i));
-            const uint32_t w[4] = {u.x, u.y, u.z, u.w};
-#pragma unroll
-            for (int e = 0; e < 4; ++e) {
-                v[2 * e] = bf16_lo(w[e]);
-                v[2 * e + 1] = bf16_hi(w[e]);
-            }
-        } else {
-            const float4 a = __ldg(reinterpret_cast<const float4*>(static_cast<const float*>(x) + i)), b = __ldg(reinterpret_cast<const float4*>(static_cast<const float*>(x) + i) + 1);
-            v[0] = a.x, v[1] = a.y, v[2] = a.z, v[3] = a.w, v[4] = b.x, v[5] = b.y, v[6] = b.z, v[7] = b.w;
-        }
-    } else {
-#pragma unroll
-        for (int e = 0; e < 8; ++e) v[e] = e < n ? load1(x, BF16, i + e) : 0.f;
-    }
-}
 __device__ __forceinline__ float gated(float g, float u) { return g / (1.0f + expf(-g)) * u; }
-
-// Row of x that image row r comes from; -1: none.
-__device__ __forceinline__ long long source_row(const PackArgs& a, int r) {
-    if (!a.src) return r;
-    const int s = __ldg(a.src + r);
-    if (s < 0) return -1;
-    const int q = s / a.div;
-    return q < a.src_rows ? q : -1;
-}
 
 // Block of 32 values over four lanes (eight each): e = floor(log2 max) - 2, at least -127, as byte e + 127; codes x 2^-e to nearest even, saturated at 6.
 // The largest exponent field is 255 where a value is infinite or no number: the whole block is then no number.
@@ -71,90 +41,87 @@ __device__ __forceinline__ void store_mx(unsigned char* tile, int r, int lane, f
     if ((lane & 15) == 0) *reinterpret_cast<uint32_t*>(tile + mx_scale_at(r, piece)) = w;
 }
 
-template <bool MX, bool BF16, bool GLU>
-__global__ void __launch_bounds__(THREADS) pack_kernel(const PackArgs a, int kblocks, long long units) {
-    const int lane = threadIdx.x & 31;
-    const long long u0 = ((long long)blockIdx.x * WARPS + (threadIdx.x >> 5)) * PACK_UNITS;
-    // values of a lane: eight codes; two bf16, of which four units make the same eight loads
-    constexpr int V = MX ? 8 : 2;
-    const size_t es = BF16 ? 2 : 4;
-    const bool aligned = MX ? ((uintptr_t)a.x & 15) == 0 && (a.ldx * es & 15) == 0 && (!GLU || (a.K * es & 15) == 0)
-                            : ((uintptr_t)a.x & (2 * es - 1)) == 0 && (a.ldx & 1) == 0 && (!GLU || (a.K & 1) == 0);
-    float v[PACK_UNITS][V], g[GLU ? PACK_UNITS : 1][V];
-    long long from[PACK_UNITS];
-    int row[PACK_UNITS], kb[PACK_UNITS];
-#pragma unroll
-    for (int i = 0; i < PACK_UNITS; ++i) {
-        const long long u = u0 + i;
-        row[i] = u < units ? (int)(u / kblocks) : 0;
-        kb[i] = u < units ? (int)(u - (long long)row[i] * kblocks) : 0;
-        from[i] = u < units ? source_row(a, row[i]) : -1;
+// CTA: eight rows (x), a warp each; U k-blocks of a row per warp (y).  Everything a warp loads is asked for before it works on the first.
+template <bool MX, bool BF16, bool GLU, int U>
+__global__ void __launch_bounds__(THREADS) pack_kernel(const PackArgs a, int kblocks) {
+    constexpr int V = MX ? 8 : 2;  // values of a lane and k-block
+    using Word = typename Words<V * (BF16 ? 2 : 4)>::type;
+    constexpr int NW = V * (BF16 ? 2 : 4) / sizeof(Word);
+    pdl_launch_dependents();
+    pdl_wait();
+    const int lane = threadIdx.x & 31, row = blockIdx.x * WARPS + (threadIdx.x >> 5), kb0 = blockIdx.y * U;
+    if (row >= a.rows) return;
+    long long from = row;
+    if (a.src) {
+        const int s = __ldg(a.src + row);
+        if (s < 0) return;
+        from = a.div == 1 ? s : s / a.div;
+        if (from >= a.src_rows) return;
     }
+    const size_t es = BF16 ? 2 : 4;
+    const char* x = static_cast<const char*>(a.x) + from * a.ldx * es;
+    const int r = row % IMG_ROWS, k0 = kb0 * (MX ? MX_K : BF_K) + lane * V;
+    unsigned char* tile = a.image + ((size_t)(row / IMG_ROWS) * kblocks + kb0) * (MX ? MX_TILE : IMG_CODES);
+    const bool aligned = ((uintptr_t)x & (sizeof(Word) - 1)) == 0 && (!GLU || (a.K * es & (sizeof(Word) - 1)) == 0);
+    Word w[U][NW], g[GLU ? U : 1][NW];
 #pragma unroll
-    for (int i = 0; i < PACK_UNITS; ++i) {
-        if (from[i] < 0) continue;
-        const int k = kb[i] * (MX ? MX_K : BF_K) + lane * V, n = max(0, a.K - k);
-        const size_t at = (size_t)from[i] * a.ldx + k;
-        if constexpr (MX) {
-            load8<BF16>(a.x, at, n, aligned, v[i]);
-            if constexpr (GLU) load8<BF16>(a.x, at + a.K, n, aligned, g[i]);
+    for (int i = 0; i < U; ++i) {
+        const int k = k0 + i * (MX ? MX_K : BF_K);
+        if (aligned && k + V <= a.K) {
+#pragma unroll
+            for (int e = 0; e < NW; ++e) {
+                w[i][e] = __ldg(reinterpret_cast<const Word*>(x + k * es) + e);
+                if (GLU) g[GLU ? i : 0][e] = __ldg(reinterpret_cast<const Word*>(x + ((size_t)a.K + k) * es) + e);
+            }
         } else {
-            auto load2 = [&](size_t p, float (&d)[V]) {
-                if (aligned && n >= 2) {
-                    if (BF16) {
-                        const uint32_t w = __ldg(reinterpret_cast<const uint32_t*>(static_cast<const uint16_t*>(a.x) + p));
-                        d[0] = bf16_lo(w), d[1] = bf16_hi(w);
-                    } else {
-                        const float2 w = __ldg(reinterpret_cast<const float2*>(static_cast<const float*>(a.x) + p));
-                        d[0] = w.x, d[1] = w.y;
-                    }
-                } else {
-                    d[0] = n > 0 ? load1(a.x, BF16, p) : 0.f;
-                    d[1] = n > 1 ? load1(a.x, BF16, p + 1) : 0.f;
-                }
-            };
-            load2(at, v[i]);
-            if constexpr (GLU) load2(at + a.K, g[i]);
+            load_ragged<V, BF16>(x, k, a.K, w[i]);
+            if (GLU) load_ragged<V, BF16>(x + (size_t)a.K * es, k, a.K, g[GLU ? i : 0]);
         }
     }
 #pragma unroll
-    for (int i = 0; i < PACK_UNITS; ++i) {
-        if (from[i] < 0) continue;  // the same for the whole warp
-        if constexpr (GLU)
+    for (int i = 0; i < U; ++i) {
+        if (kb0 + i >= kblocks) return;
+        float v[V];
+        widen<V, BF16>(w[i], v);
+        if constexpr (GLU) {
+            float u[V];
+            widen<V, BF16>(g[i], u);
 #pragma unroll
-            for (int e = 0; e < V; ++e) v[i][e] = gated(v[i][e], g[i][e]);
-        unsigned char* tile = a.image + ((size_t)(row[i] / IMG_ROWS) * kblocks + kb[i]) * (MX ? MX_TILE : IMG_CODES);
-        const int r = row[i] % IMG_ROWS;
+            for (int e = 0; e < V; ++e) v[e] = gated(v[e], u[e]);
+        }
         if constexpr (MX)
-            store_mx(tile, r, lane, v[i]);
+            store_mx(tile + (size_t)i * MX_TILE, r, lane, v);
         else
-            *reinterpret_cast<uint32_t*>(tile + r * 128 + (((lane >> 2) ^ (r & 7)) << 4) + (lane & 3) * 4) = bf16x2_rne(v[i][0], v[i][1]);
+            *reinterpret_cast<uint32_t*>(tile + (size_t)i * IMG_CODES + r * 128 + (((lane >> 2) ^ (r & 7)) << 4) + (lane & 3) * 4) = bf16x2_rne(v[0], v[1]);
     }
 }
 
-template <bool MX, bool BF16>
-__global__ void __launch_bounds__(THREADS) unpack_kernel(const unsigned char* image, int K, int kblocks, long long units, void* out, size_t ld) {
-    const int lane = threadIdx.x & 31;
-    const long long u0 = ((long long)blockIdx.x * WARPS + (threadIdx.x >> 5)) * PACK_UNITS;
+template <bool MX, bool BF16, int U>
+__global__ void __launch_bounds__(THREADS) unpack_kernel(const unsigned char* image, int rows, int K, int kblocks, void* out, size_t ld) {
     constexpr int V = MX ? 8 : 2;
+    using Word = typename Words<V * (BF16 ? 2 : 4)>::type;
+    constexpr int NW = V * (BF16 ? 2 : 4) / sizeof(Word);
+    pdl_launch_dependents();
+    pdl_wait();
+    const int lane = threadIdx.x & 31, row = blockIdx.x * WARPS + (threadIdx.x >> 5), kb0 = blockIdx.y * U;
+    if (row >= rows) return;
     const size_t es = BF16 ? 2 : 4;
-    const bool aligned = ((uintptr_t)out & (V * es >= 16 ? 15 : V * es - 1)) == 0 && (ld * es & (V * es >= 16 ? 15 : V * es - 1)) == 0;
-    uint32_t w[PACK_UNITS], s[PACK_UNITS];
+    char* y = static_cast<char*>(out) + (size_t)row * ld * es;
+    const bool aligned = ((uintptr_t)y & (sizeof(Word) - 1)) == 0;
+    const int r = row % IMG_ROWS, piece = lane >> 2, k0 = kb0 * (MX ? MX_K : BF_K) + lane * V;
+    const unsigned char* tile = image + ((size_t)(row / IMG_ROWS) * kblocks + kb0) * (MX ? MX_TILE : IMG_CODES);
+    uint32_t w[U], s[U];
 #pragma unroll
-    for (int i = 0; i < PACK_UNITS; ++i) {
-        const long long u = u0 + i;
-        if (u >= units) continue;
-        const int row = (int)(u / kblocks), kb = (int)(u - (long long)row * kblocks), r = row % IMG_ROWS, piece = lane >> 2;
-        const unsigned char* tile = image + ((size_t)(row / IMG_ROWS) * kblocks + kb) * (MX ? MX_TILE : IMG_CODES);
-        w[i] = __ldg(reinterpret_cast<const uint32_t*>(tile + (MX ? MX_SCALES : 0) + r * 128 + ((piece ^ (r & 7)) << 4) + (lane & 3) * 4));
-        if (MX) s[i] = __ldg(tile + mx_scale_at(r, piece));
-    }
+    for (int i = 0; i < U; ++i)
+        if (kb0 + i < kblocks) {
+            const unsigned char* t = tile + (size_t)i * (MX ? MX_TILE : IMG_CODES);
+            w[i] = __ldg(reinterpret_cast<const uint32_t*>(t + (MX ? MX_SCALES : 0) + r * 128 + ((piece ^ (r & 7)) << 4) + (lane & 3) * 4));
+            if (MX) s[i] = __ldg(t + mx_scale_at(r, piece));
+        }
 #pragma unroll
-    for (int i = 0; i < PACK_UNITS; ++i) {
-        const long long u = u0 + i;
-        if (u >= units) continue;
-        const int row = (int)(u / kblocks), kb = (int)(u - (long long)row * kblocks);
-        const int k = kb * (MX ? MX_K : BF_K) + lane * V, n = K - k;
+    for (int i = 0; i < U; ++i) {
+        if (kb0 + i >= kblocks) return;
+        const int k = k0 + i * (MX ? MX_K : BF_K), n = K - k;
         float v[V];
         if constexpr (MX) {
             uint32_t h[4];
@@ -169,28 +136,26 @@ __global__ void __launch_bounds__(THREADS) unpack_kernel(const unsigned char* im
             v[0] = bf16_lo(w[i]);
             v[1] = bf16_hi(w[i]);
         }
-        const size_t at = (size_t)row * ld + k;
-        if (aligned && n >= V) {
-            if constexpr (BF16) {
-                uint32_t p[V / 2];
+        uint32_t p[V * (BF16 ? 2 : 4) / 4];
 #pragma unroll
-                for (int e = 0; e < V / 2; ++e) p[e] = bf16x2_rne(v[2 * e], v[2 * e + 1]);
-                if constexpr (MX) *reinterpret_cast<uint4*>(static_cast<uint16_t*>(out) + at) = make_uint4(p[0], p[1], p[2], p[3]);
-                else *reinterpret_cast<uint32_t*>(static_cast<uint16_t*>(out) + at) = p[0];
-            } else {
-                float* o = static_cast<float*>(out) + at;
-                if constexpr (MX) {
-                    reinterpret_cast<float4*>(o)[0] = make_float4(v[0], v[1], v[2], v[3]);
-                    reinterpret_cast<float4*>(o)[1] = make_float4(v[4], v[5], v[6], v[7]);
-                } else
-                    *reinterpret_cast<float2*>(o) = make_float2(v[0], v[1]);
+        for (int e = 0; e < V; ++e) {
+            if (!BF16) p[e] = __float_as_uint(v[e]);
+            else if ((e & 1) == 0) p[e / 2] = bf16x2_rne(v[e], v[e + 1]);
+        }
+        if (aligned && n >= V) {
+#pragma unroll
+            for (int e = 0; e < NW; ++e) {
+                Word o;
+#pragma unroll
+                for (int q = 0; q < (int)sizeof(Word) / 4; ++q) reinterpret_cast<uint32_t*>(&o)[q] = p[e * (sizeof(Word) / 4) + q];
+                reinterpret_cast<Word*>(y + k * es)[e] = o;
             }
         } else {
 #pragma unroll
             for (int e = 0; e < V; ++e)
                 if (e < n) {
-                    if (BF16) static_cast<uint16_t*>(out)[at + e] = (uint16_t)bf16x2_rne(v[e], 0.f);
-                    else static_cast<float*>(out)[at + e] = v[e];
+                    if (BF16) reinterpret_cast<uint16_t*>(y)[k + e] = (uint16_t)(p[e / 2] >> (16 * (e & 1)));
+                    else reinterpret_cast<uint32_t*>(y)[k + e] = p[e];
                 }
         }
     }
@@ -198,6 +163,8 @@ __global__ void __launch_bounds__(THREADS) unpack_kernel(const unsigned char* im
 
 // A warp per row and k-block of 256 values: eight blocks of 17 bytes; four lanes share a block, each with eight values.
 __global__ void __launch_bounds__(THREADS) blocks_kernel(const uint8_t* blocks, int K, int kblocks, long long units, unsigned char* image) {
+    pdl_launch_dependents();
+    pdl_wait();
     const int lane = threadIdx.x & 31;
     const long long u = (long long)blockIdx.x * WARPS + (threadIdx.x >> 5);
     if (u >= units) return;
@@ -217,59 +184,79 @@ __global__ void __launch_bounds__(THREADS) blocks_kernel(const uint8_t* blocks, 
     if (q == 0) tile[mx_scale_at(r, piece)] = (unsigned char)s;
 }
 
-// CTA e: the expert's rows.  A thread looks at a run of consecutive ids, so that prefix sums over the threads keep the pairs' order.
-constexpr int PLAN_THREADS = 512;
-__global__ void __launch_bounds__(PLAN_THREADS) plan_kernel(const int32_t* __restrict__ ids, const Plan p) {
-    __shared__ int hist[PLAN_EXPERTS], warp_sums[PLAN_THREADS / 32], first_s[2];
+// CTA e: the expert's rows.  Counts of all experts, in copies per lane so that neither a bank nor an address is hit twice by a warp; then a thread looks at
+// eight consecutive ids at a time, so that prefix sums over the threads keep the pairs' order.
+constexpr int PLAN_THREADS = 512, PLAN_IDS = 8;
+inline int plan_copies(int experts) { return experts <= 256 ? 32 : 8; }
+__global__ void __launch_bounds__(PLAN_THREADS) plan_kernel(const int32_t* __restrict__ ids, const Plan p, int copies) {
+    extern __shared__ int hist[];  // [experts][copies], then the sums in the first copy
+    __shared__ int warp_sums[PLAN_THREADS / 32], first_s[2];
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, e = blockIdx.x;
-    for (int i = tid; i < p.experts; i += PLAN_THREADS) hist[i] = 0;
+    pdl_launch_dependents();
+    for (int i = tid; i < p.experts * copies; i += PLAN_THREADS) hist[i] = 0;
     __syncthreads();
+    pdl_wait();
     for (int i = tid; i < p.pairs; i += PLAN_THREADS) {
         const int id = __ldg(ids + i);
-        if (id >= 0 && id < p.experts) atomicAdd(&hist[id], 1);  // counts: the same in any order
+        if (id >= 0 && id < p.experts) atomicAdd(&hist[id * copies + (lane & (copies - 1))], 1);  // counts: the same in any order
         else if (e == 0) p.place[i] = -1;
     }
     __syncthreads();
+    for (int i = tid; i < p.experts; i += PLAN_THREADS) {
+        int n = 0;
+        for (int c = 0; c < copies; ++c) n += hist[i * copies + ((c + i) & (copies - 1))];
+        hist[i * copies] = n;
+    }
+    __syncthreads();
+    const int n = hist[e * copies];
     if (warp == 0) {  // blocks in front of the expert, and of all experts
         int before = 0, all = 0;
         for (int i = lane; i < p.experts; i += 32) {
-            const int b = (hist[i] + IMG_ROWS - 1) / IMG_ROWS;
+            const int b = (hist[i * copies] + IMG_ROWS - 1) / IMG_ROWS;
             all += b;
             if (i < e) before += b;
         }
-#pragma unroll
-        for (int o = 16; o > 0; o >>= 1) {
-            before += __shfl_xor_sync(0xffffffffu, before, o);
-            all += __shfl_xor_sync(0xffffffffu, all, o);
-        }
+        before = __reduce_add_sync(0xffffffffu, before);
+        all = __reduce_add_sync(0xffffffffu, all);
         if (lane == 0) {
             first_s[0] = before;
             first_s[1] = all;
             p.first[e] = before;
-            p.count[e] = hist[e];
+            p.count[e] = n;
             if (e == 0) p.first[p.experts] = all;
         }
     }
     __syncthreads();
-    const int row0 = first_s[0] * IMG_ROWS, n = hist[e];
+    const int row0 = first_s[0] * IMG_ROWS;
     int base = 0;
-    for (int c0 = 0; c0 < p.pairs && base < n; c0 += PLAN_THREADS) {
-        const int i = c0 + tid;
-        const bool mine = i < p.pairs && __ldg(ids + i) == e;
-        const uint32_t votes = __ballot_sync(0xffffffffu, mine);
-        if (lane == 0) warp_sums[warp] = __popc(votes);
+    for (int c0 = 0; c0 < p.pairs && base < n; c0 += PLAN_THREADS * PLAN_IDS) {
+        const int i0 = c0 + tid * PLAN_IDS;
+        int id[PLAN_IDS], mine = 0;
+#pragma unroll
+        for (int k = 0; k < PLAN_IDS; ++k) {
+            id[k] = i0 + k < p.pairs ? __ldg(ids + i0 + k) : -1;
+            mine += id[k] == e;
+        }
+        int inc = mine;
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) {
+            const int t = __shfl_up_sync(0xffffffffu, inc, o);
+            if (lane >= o) inc += t;
+        }
+        if (lane == 31) warp_sums[warp] = inc;
         __syncthreads();
-        int at = base;
+        int r = row0 + base + inc - mine;
 #pragma unroll
         for (int w = 0; w < PLAN_THREADS / 32; ++w) {
-            if (w < warp) at += warp_sums[w];
+            if (w < warp) r += warp_sums[w];
             base += warp_sums[w];
         }
-        if (mine) {
-            const int r = row0 + at + __popc(votes & ((1u << lane) - 1u));
-            p.place[i] = r;
-            p.row[r] = i;
-        }
+#pragma unroll
+        for (int k = 0; k < PLAN_IDS; ++k)
+            if (id[k] == e) {
+                p.place[i0 + k] = r;
+                p.row[r++] = i0 + k;
+            }
         __syncthreads();
     }
     // rows behind the expert's last, and behind the last expert's
@@ -279,6 +266,8 @@ __global__ void __launch_bounds__(PLAN_THREADS) plan_kernel(const int32_t* __res
 
 template <bool RB, bool YB>
 __global__ void __launch_bounds__(THREADS) sum_kernel(const SumArgs a, int v4) {
+    pdl_launch_dependents();
+    pdl_wait();
     const int t = blockIdx.y;
     const int per = v4 ? 4 : 1;
     const int i = (blockIdx.x * THREADS + threadIdx.x) * per;
@@ -327,33 +316,34 @@ inline cudaError_t grid_of(long long units, int per, unsigned* g) {
 
 }  // namespace
 
+// k-blocks of a warp: four, or what short rows have.
+static int pack_units(int kblocks) { return kblocks >= 3 ? 4 : kblocks; }
+
 cudaError_t launch_image_pack(const PackArgs& a, bool mx, cudaStream_t st) {
-    const int kblocks = img_kblocks(mx, a.K);
-    const long long units = (long long)a.rows * kblocks;
-    unsigned g;
-    if (const cudaError_t e = grid_of(units, WARPS * PACK_UNITS, &g)) return e;
-#define PACK(MX, B, G) pack_kernel<MX, B, G><<<g, THREADS, 0, st>>>(a, kblocks, units)
-    if (mx) {
-        if (a.bf16) a.glu ? PACK(true, true, true) : PACK(true, true, false);
-        else a.glu ? PACK(true, false, true) : PACK(true, false, false);
-    } else {
-        if (a.bf16) a.glu ? PACK(false, true, true) : PACK(false, true, false);
-        else a.glu ? PACK(false, false, true) : PACK(false, false, false);
-    }
-#undef PACK
-    return cudaGetLastError();
+    const int kblocks = img_kblocks(mx, a.K), U = pack_units(kblocks);
+    const dim3 g((a.rows + WARPS - 1) / WARPS, (kblocks + U - 1) / U);
+    if (g.y > 65535) return cudaErrorInvalidValue;
+    auto launch = [&](auto MX, auto B, auto G) {
+        if (U == 1) return launch_after(pack_kernel<MX.value, B.value, G.value, 1>, g, THREADS, 0, 1, st, a, kblocks);
+        if (U == 2) return launch_after(pack_kernel<MX.value, B.value, G.value, 2>, g, THREADS, 0, 1, st, a, kblocks);
+        return launch_after(pack_kernel<MX.value, B.value, G.value, 4>, g, THREADS, 0, 1, st, a, kblocks);
+    };
+    auto with = [&](auto MX, auto B) { return a.glu ? launch(MX, B, std::true_type{}) : launch(MX, B, std::false_type{}); };
+    if (mx) return a.bf16 ? with(std::true_type{}, std::true_type{}) : with(std::true_type{}, std::false_type{});
+    return a.bf16 ? with(std::false_type{}, std::true_type{}) : with(std::false_type{}, std::false_type{});
 }
 
 cudaError_t launch_image_unpack(const unsigned char* image, bool mx, int rows, int K, void* out, bool bf16, size_t ld, cudaStream_t st) {
-    const int kblocks = img_kblocks(mx, K);
-    const long long units = (long long)rows * kblocks;
-    unsigned g;
-    if (const cudaError_t e = grid_of(units, WARPS * PACK_UNITS, &g)) return e;
-#define UNPACK(MX, B) unpack_kernel<MX, B><<<g, THREADS, 0, st>>>(image, K, kblocks, units, out, ld)
-    if (mx) bf16 ? UNPACK(true, true) : UNPACK(true, false);
-    else bf16 ? UNPACK(false, true) : UNPACK(false, false);
-#undef UNPACK
-    return cudaGetLastError();
+    const int kblocks = img_kblocks(mx, K), U = pack_units(kblocks);
+    const dim3 g((rows + WARPS - 1) / WARPS, (kblocks + U - 1) / U);
+    if (g.y > 65535) return cudaErrorInvalidValue;
+    auto with = [&](auto MX, auto B) {
+        if (U == 1) return launch_after(unpack_kernel<MX.value, B.value, 1>, g, THREADS, 0, 1, st, image, rows, K, kblocks, out, ld);
+        if (U == 2) return launch_after(unpack_kernel<MX.value, B.value, 2>, g, THREADS, 0, 1, st, image, rows, K, kblocks, out, ld);
+        return launch_after(unpack_kernel<MX.value, B.value, 4>, g, THREADS, 0, 1, st, image, rows, K, kblocks, out, ld);
+    };
+    if (mx) return bf16 ? with(std::true_type{}, std::true_type{}) : with(std::true_type{}, std::false_type{});
+    return bf16 ? with(std::false_type{}, std::true_type{}) : with(std::false_type{}, std::false_type{});
 }
 
 cudaError_t launch_image_blocks(const uint8_t* blocks, int rows, int K, unsigned char* image, cudaStream_t st) {
@@ -361,13 +351,12 @@ cudaError_t launch_image_blocks(const uint8_t* blocks, int rows, int K, unsigned
     const long long units = (long long)rows * kblocks;
     unsigned g;
     if (const cudaError_t e = grid_of(units, WARPS, &g)) return e;
-    blocks_kernel<<<g, THREADS, 0, st>>>(blocks, K, kblocks, units, image);
-    return cudaGetLastError();
+    return launch_after(blocks_kernel, dim3(g), THREADS, 0, 1, st, blocks, K, kblocks, units, image);
 }
 
 cudaError_t launch_plan(const int32_t* ids, const Plan& p, cudaStream_t st) {
-    plan_kernel<<<p.experts, PLAN_THREADS, 0, st>>>(ids, p);
-    return cudaGetLastError();
+    const int copies = plan_copies(p.experts);
+    return launch_after(plan_kernel, dim3(p.experts), PLAN_THREADS, (size_t)p.experts * copies * 4, 1, st, ids, p, copies);
 }
 
 cudaError_t launch_expert_sum(const SumArgs& a, cudaStream_t st) {
@@ -387,9 +376,8 @@ cudaError_t launch_expert_sum(const SumArgs& a, cudaStream_t st) {
         return launch_expert_sum(c, st);
     }
     const dim3 g((a.W / (v4 ? 4 : 1) + THREADS - 1) / THREADS, a.tokens);
-    if (a.rows_bf16) a.y_bf16 ? sum_kernel<true, true><<<g, THREADS, 0, st>>>(a, v4) : sum_kernel<true, false><<<g, THREADS, 0, st>>>(a, v4);
-    else a.y_bf16 ? sum_kernel<false, true><<<g, THREADS, 0, st>>>(a, v4) : sum_kernel<false, false><<<g, THREADS, 0, st>>>(a, v4);
-    return cudaGetLastError();
+    void (*const kernels[2][2])(SumArgs, int) = {{sum_kernel<false, false>, sum_kernel<false, true>}, {sum_kernel<true, false>, sum_kernel<true, true>}};
+    return launch_after(kernels[a.rows_bf16 != 0][a.y_bf16 != 0], g, THREADS, 0, 1, st, a, v4);
 }
 
 }  // namespace hm

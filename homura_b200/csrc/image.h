@@ -102,6 +102,24 @@ struct MxGemvArgs {
 constexpr int MX_GEMV_K = 32768;  // widest row
 cudaError_t launch_mx4_gemv(MxGemvArgs a, int sm_count, cudaStream_t st);
 
+// Launch that may begin while the kernel in front of it ends (each of these kernels waits for that before it touches memory).
+template <typename... P, typename... A>
+inline cudaError_t launch_after(void (*k)(P...), dim3 grid, int threads, size_t smem, int cluster, cudaStream_t st, A... args) {
+    cudaLaunchConfig_t cfg{};
+    cfg.gridDim = grid;
+    cfg.blockDim = dim3(threads);
+    cfg.dynamicSmemBytes = smem;
+    cfg.stream = st;
+    cudaLaunchAttribute at[2];
+    at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    at[0].val.programmaticStreamSerializationAllowed = 1;
+    at[1].id = cudaLaunchAttributeClusterDimension;
+    at[1].val.clusterDim = {(unsigned)cluster, 1, 1};
+    cfg.attrs = at;
+    cfg.numAttrs = cluster > 1 ? 2 : 1;
+    return cudaLaunchKernelEx(&cfg, k, args...);
+}
+
 // ---- codes and scales ---------------------------------------------------------------------------
 #ifdef __CUDACC__
 // Eight values of [-8, 8] (or beyond: they saturate) to the nearest codes, ties to even; v[0] in the lowest four bits.
@@ -116,6 +134,29 @@ __device__ __forceinline__ uint32_t mx_codes(const float (&v)[8]) {
         : "=r"(r)
         : "f"(v[0]), "f"(v[1]), "f"(v[2]), "f"(v[3]), "f"(v[4]), "f"(v[5]), "f"(v[6]), "f"(v[7]));
     return r;
+}
+// What a lane loads at once: up to 16 bytes.
+template <int BYTES> struct Words { using type = uint4; };
+template <> struct Words<8> { using type = uint2; };
+template <> struct Words<4> { using type = uint32_t; };
+// V values from element k of a row of n on; those beyond are zero.
+template <int V, bool BF16, typename Word>
+__device__ __forceinline__ void load_ragged(const char* x, int k, int n, Word* w) {
+    uint32_t* o = reinterpret_cast<uint32_t*>(w);
+#pragma unroll
+    for (int e = 0; e < V; ++e) {
+        if (BF16) {
+            const uint32_t b = k + e < n ? __ldg(reinterpret_cast<const uint16_t*>(x) + k + e) : 0u;
+            o[e / 2] = e & 1 ? o[e / 2] | b << 16 : b;
+        } else
+            o[e] = k + e < n ? __ldg(reinterpret_cast<const uint32_t*>(x) + k + e) : 0u;
+    }
+}
+template <int V, bool BF16, typename Word>
+__device__ __forceinline__ void widen(const Word* w, float (&v)[V]) {
+    const uint32_t* o = reinterpret_cast<const uint32_t*>(w);
+#pragma unroll
+    for (int e = 0; e < V; ++e) v[e] = BF16 ? (e & 1 ? bf16_hi(o[e / 2]) : bf16_lo(o[e / 2])) : __uint_as_float(o[e]);
 }
 // Eight codes as four words of two f16.
 __device__ __forceinline__ void mx_halves(uint32_t codes, uint32_t (&h)[4]) {

@@ -224,6 +224,7 @@ __global__ void __launch_bounds__(THREADS, 1) image_gemm_kernel(const ImageGemmA
     __shared__ int ufirst[PLAN_EXPERTS];
     unsigned char* ring = dsm + ((1024u - (s32(dsm) & 1023u)) & 1023u);  // swizzle atoms need 1024-byte alignment
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+    pdl_launch_dependents();
     if (tid == 0) {
         for (int s = 0; s < SLOTS; ++s) { mb_init(&sh.full[s], 1); mb_init(&sh.empty[s], 1); }
         for (int s = 0; s < 2; ++s) { mb_init(&sh.afull[s], 1); mb_init(&sh.aempty[s], EPI_WARPS); }
@@ -236,6 +237,7 @@ __global__ void __launch_bounds__(THREADS, 1) image_gemm_kernel(const ImageGemmA
         asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], 512;" ::"r"(s32(&sh.tmem)) : "memory");
         asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
     }
+    pdl_wait();
     if (warp == 2 && a.first) {  // first unit of every expert
         int sum = 0;
         for (int i0 = 0; i0 < a.experts; i0 += 32) {
@@ -443,19 +445,7 @@ cudaError_t launch_image_gemm(ImageGemmArgs a, bool mx, int sm_count, cudaStream
     if (a.split > 8 && (e = ensure_nonportable_clusters(fn)) != cudaSuccess) return e;
     a.kb_per = (a.kblocks + a.split - 1) / a.split;
     a.split = (a.kblocks + a.kb_per - 1) / a.kb_per;
-    cudaLaunchConfig_t cfg{};
-    cfg.gridDim = dim3(a.split > 1 ? (unsigned)units * a.split : (unsigned)std::min<long long>(units, sm_count));
-    cfg.blockDim = dim3(THREADS);
-    cfg.dynamicSmemBytes = SMEM;
-    cfg.stream = st;
-    cudaLaunchAttribute at[1];
-    if (a.split > 1) {
-        at[0].id = cudaLaunchAttributeClusterDimension;
-        at[0].val.clusterDim = {(unsigned)a.split, 1, 1};
-        cfg.attrs = at;
-        cfg.numAttrs = 1;
-    }
-    return cudaLaunchKernelEx(&cfg, fn, a);
+    return launch_after(fn, dim3(a.split > 1 ? (unsigned)units * a.split : (unsigned)std::min<long long>(units, sm_count)), THREADS, SMEM, a.split, st, a);
 }
 
 }  // namespace hm

@@ -29,8 +29,15 @@ struct Shared {
     uint32_t top[8];        // largest finite value of a row, as bits
 };
 
-__device__ __forceinline__ void mma_f16(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
-    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};" : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3]) : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+__device__ __forceinline__ void mma_f16(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1, const float (&c)[4]) {
+    asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%10,%11,%12,%13};"
+        : "=f"(d[0]), "=f"(d[1]), "=f"(d[2]), "=f"(d[3])
+        : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1), "f"(c[0]), "f"(c[1]), "f"(c[2]), "f"(c[3]));
+}
+// 2^(byte j of w - 127); 255 counts as infinite here.
+__device__ __forceinline__ float scale_of(uint32_t w, int j) {
+    const uint32_t s = (j == 3 ? w >> 1 : w << (23 - 8 * j)) & 0x7F800000u;
+    return __uint_as_float(max(s, 0x00400000u));
 }
 __device__ __forceinline__ uint32_t f16x2_rn(float lo, float hi) {
     uint32_t r;
@@ -38,9 +45,13 @@ __device__ __forceinline__ uint32_t f16x2_rn(float lo, float hi) {
     return r;
 }
 
+// 2^e brings a row's largest value into [2^7, 2^8).
+__device__ __forceinline__ int row_exponent(uint32_t top) { return min(max(134 - (int)(top >> 23), -126), 126); }
+__device__ __forceinline__ float row_factor(uint32_t top) { return __uint_as_float((uint32_t)(127 - row_exponent(top)) << 23); }
+
 // Elements of a column of x in shared memory: the k-blocks of a CTA and half a line, so that neighbouring columns lie in different banks.
 __host__ __device__ inline int x_ld(int kb_per) { return kb_per * MX_K + 32; }
-inline size_t smem_bytes(int slots, int kb_per, int cols) { return 1024 + (size_t)slots * MX_TILE + (size_t)cols * x_ld(kb_per) * 2 + 2 * IMG_ROWS * PART_LD * 4; }
+inline size_t smem_bytes(int slots, int kb_per, int cols) { return 1024 + (size_t)slots * MX_TILE + (size_t)cols * x_ld(kb_per) * 2 + 4 * IMG_ROWS * PART_LD * 4; }
 
 // NB: blocks of eight columns; TERMS: f16 terms of x.  Column of row m, term i: m + 8 i where the rows fill a block, else TERMS m + i.
 template <int NB, int TERMS>
@@ -51,8 +62,10 @@ __global__ void __launch_bounds__(THREADS, 2) mx4_gemv_kernel(const MxGemvArgs a
     const int ldx = x_ld(a.kb_per);
     uint16_t* xs = reinterpret_cast<uint16_t*>(ring + (size_t)a.slots * MX_TILE);
     const int cols = a.M * TERMS;
-    float* part = reinterpret_cast<float*>(xs + (size_t)cols * ldx);  // [2 halves][128 features][PART_LD]
+    float* parts = reinterpret_cast<float*>(xs + (size_t)cols * ldx);  // [tiles in turn: 2][2 halves][128 features][PART_LD]
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+    pdl_launch_dependents();
+    pdl_wait();
     int expert = 0, xrow0 = 0;
     if (a.ids) {
         expert = __ldg(a.ids + blockIdx.y);
@@ -83,38 +96,72 @@ __global__ void __launch_bounds__(THREADS, 2) mx4_gemv_kernel(const MxGemvArgs a
                 }
         }
     } else {
-        // x: its largest finite value per row, then f16 terms
-        constexpr int XT = MMA_WARPS * 32;
-        const int k0 = kb0 * MX_K, kn = min(a.K - k0, nkb * MX_K);
-        const char* x = static_cast<const char*>(a.x);
-        auto at = [&](int m, int k) {
-            const size_t i = (size_t)(xrow0 + m) * a.ldx + k0 + k;
-            return a.bf16 ? bf16_bits_to_f32(__ldg(reinterpret_cast<const uint16_t*>(x) + i)) : __ldg(reinterpret_cast<const float*>(x) + i);
-        };
-        for (int m = 0; m < a.M; ++m) {
-            uint32_t top = 0;
-            for (int k = tid; k < kn; k += XT) {
-                const uint32_t b = __float_as_uint(at(m, k)) & 0x7FFFFFFFu;
-                if (b < 0x7F800000u) top = max(top, b);
+        // x: its largest finite value per row, then f16 terms.  An item is eight values of a row, 32 items of one row to a warp; up to XU items of a thread
+        // are loaded once.
+        constexpr int XT = MMA_WARPS * 32, XU = 6;
+        constexpr bool B = TERMS == 1;
+        constexpr int NW = B ? 1 : 2;
+        const int k0 = kb0 * MX_K, items = a.M * nkb * 32;
+        const size_t es = B ? 2 : 4;
+        const char* x = static_cast<const char*>(a.x) + (xrow0 * a.ldx + k0) * es;
+        const bool aligned = ((uintptr_t)x & 15) == 0 && (a.ldx * es & 15) == 0;
+        uint4 w[XU][NW];
+        auto fetch = [&](int it0) {
+#pragma unroll
+            for (int u = 0; u < XU; ++u) {
+                const int it = it0 + u * XT;
+                if (it >= items) continue;
+                const int m = (it >> 5) / nkb, k = (it - m * nkb * 32) * 8;
+                const char* row = x + m * a.ldx * es;
+                if (aligned && k0 + k + 8 <= a.K) {
+#pragma unroll
+                    for (int e = 0; e < NW; ++e) w[u][e] = __ldg(reinterpret_cast<const uint4*>(row + k * es) + e);
+                } else
+                    load_ragged<8, B>(row, k, a.K - k0, w[u]);
             }
-            top = __reduce_max_sync(0xffffffffu, top);
-            if (lane == 0) atomicMax(&sh.top[m], top);
+        };
+        for (int it0 = tid; it0 < items; it0 += XU * XT) {
+            fetch(it0);
+#pragma unroll
+            for (int u = 0; u < XU; ++u) {
+                const int it = it0 + u * XT;
+                if (it >= items) continue;  // the same for the whole warp
+                float v[8];
+                widen<8, B>(w[u], v);
+                uint32_t top = 0;
+#pragma unroll
+                for (int e = 0; e < 8; ++e) {
+                    const uint32_t b = __float_as_uint(v[e]) & 0x7FFFFFFFu;
+                    if (b < 0x7F800000u) top = max(top, b);
+                }
+                top = __reduce_max_sync(0xffffffffu, top);
+                if (lane == 0) atomicMax(&sh.top[(it >> 5) / nkb], top);
+            }
         }
         asm volatile("bar.sync 1, 256;" ::: "memory");
-        for (int m = 0; m < a.M; ++m) {
-            const int e = min(max(134 - (int)(sh.top[m] >> 23), -126), 126);  // 2^e brings the largest value into [2^7, 2^8)
-            const float up = __uint_as_float((uint32_t)(e + 127) << 23);
-            for (int k = 2 * tid; k < nkb * MX_K; k += 2 * XT) {
-                const float u = k < kn ? at(m, k) * up : 0.f, v = k + 1 < kn ? at(m, k + 1) * up : 0.f;
-                const uint32_t h = f16x2_rn(u, v);
-                const int c = NB == 2 ? m : TERMS * m;
-                *reinterpret_cast<uint32_t*>(xs + (size_t)c * ldx + k) = h;
-                if (TERMS == 2) {
-                    // what the first term leaves; nothing of an infinity
-                    const float ru = u - f16_bits_to_f32((uint16_t)h), rv = v - f16_bits_to_f32((uint16_t)(h >> 16));
-                    const float fu = fabsf(u) < __int_as_float(0x7F800000) ? ru : 0.f, fv = fabsf(v) < __int_as_float(0x7F800000) ? rv : 0.f;
-                    *reinterpret_cast<uint32_t*>(xs + (size_t)(NB == 2 ? a.M + m : c + 1) * ldx + k) = f16x2_rn(fu, fv);
+        for (int it0 = tid; it0 < items; it0 += XU * XT) {
+            if (items > XU * XT) fetch(it0);
+#pragma unroll
+            for (int u = 0; u < XU; ++u) {
+                const int it = it0 + u * XT;
+                if (it >= items) continue;
+                const int m = (it >> 5) / nkb, k = (it - m * nkb * 32) * 8;
+                const float up = __uint_as_float((uint32_t)(row_exponent(sh.top[m]) + 127) << 23);
+                float v[8];
+                widen<8, B>(w[u], v);
+                uint32_t h[4], l[4];
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    const float p = v[2 * e] * up, q = v[2 * e + 1] * up;
+                    h[e] = f16x2_rn(p, q);
+                    if (TERMS == 2) {  // what the first term leaves; nothing of an infinity
+                        const float rp = p - f16_bits_to_f32((uint16_t)h[e]), rq = q - f16_bits_to_f32((uint16_t)(h[e] >> 16));
+                        l[e] = f16x2_rn(fabsf(p) < __int_as_float(0x7F800000) ? rp : 0.f, fabsf(q) < __int_as_float(0x7F800000) ? rq : 0.f);
+                    }
                 }
+                const int c = NB == 2 ? m : TERMS * m;
+                *reinterpret_cast<uint4*>(xs + (size_t)c * ldx + k) = make_uint4(h[0], h[1], h[2], h[3]);
+                if (TERMS == 2) *reinterpret_cast<uint4*>(xs + (size_t)(NB == 2 ? a.M + m : c + 1) * ldx + k) = make_uint4(l[0], l[1], l[2], l[3]);
             }
         }
         asm volatile("bar.sync 1, 256;" ::: "memory");
@@ -122,7 +169,8 @@ __global__ void __launch_bounds__(THREADS, 2) mx4_gemv_kernel(const MxGemvArgs a
     __syncwarp();
     const int fg = warp & 3, kh = (warp >> 2) & 1, g = lane >> 2, tl = lane & 3;
     uint32_t used = 0;
-    for (int t = blockIdx.x / a.split; t < a.tiles; t += step) {
+    for (int t = blockIdx.x / a.split, turn = 0; t < a.tiles; t += step, turn ^= 1) {
+        float* part = parts + (size_t)turn * 2 * IMG_ROWS * PART_LD;
         if (warp < MMA_WARPS) {
             float sum[2][NB][4];
 #pragma unroll
@@ -138,7 +186,12 @@ __global__ void __launch_bounds__(THREADS, 2) mx4_gemv_kernel(const MxGemvArgs a
                 const uint32_t* sc = reinterpret_cast<const uint32_t*>(tile + kh * 512 + fg * 4);
                 uint32_t scales[4];  // of features g, g + 8, g + 16, g + 24 of the group: a byte per block of this half
 #pragma unroll
-                for (int i = 0; i < 4; ++i) scales[i] = sc[(g + 8 * i) * 4];
+                for (int i = 0; i < 4; ++i) {
+                    scales[i] = sc[(g + 8 * i) * 4];
+                    if (__vcmpeq4(scales[i], 0xFFFFFFFFu))  // a block that is no number
+#pragma unroll
+                        for (int b = 0; b < NB; ++b) sum[i >> 1][b][2 * (i & 1)] = sum[i >> 1][b][2 * (i & 1) + 1] = __int_as_float(0x7FC00000);
+                }
                 const unsigned char* codes = tile + MX_SCALES + (fg * 32 + g) * 128 + tl * 4;
 #pragma unroll
                 for (int j = 0; j < 4; ++j) {
@@ -154,12 +207,13 @@ __global__ void __launch_bounds__(THREADS, 2) mx4_gemv_kernel(const MxGemvArgs a
                         const int piece = ((kh * 4 + j) ^ g) << 4;
                         mx_halves(*reinterpret_cast<const uint32_t*>(codes + i * 16 * 128 + piece), lo);
                         mx_halves(*reinterpret_cast<const uint32_t*>(codes + (i * 16 + 8) * 128 + piece), hi);
-                        const float s0 = mx_scale(scales[2 * i] >> (8 * j) & 255u), s1 = mx_scale(scales[2 * i + 1] >> (8 * j) & 255u);
+                        const float s0 = scale_of(scales[2 * i], j), s1 = scale_of(scales[2 * i + 1], j);
 #pragma unroll
                         for (int b = 0; b < NB; ++b) {
-                            float d[4] = {0.f, 0.f, 0.f, 0.f};
-                            mma_f16(d, lo[0], hi[0], lo[1], hi[1], xv[b].x, xv[b].y);
-                            mma_f16(d, lo[2], hi[2], lo[3], hi[3], xv[b].z, xv[b].w);
+                            const float zero[4] = {0.f, 0.f, 0.f, 0.f};
+                            float c[4], d[4];
+                            mma_f16(c, lo[0], hi[0], lo[1], hi[1], xv[b].x, xv[b].y, zero);
+                            mma_f16(d, lo[2], hi[2], lo[3], hi[3], xv[b].z, xv[b].w, c);
                             sum[i][b][0] = fmaf(s0, d[0], sum[i][b][0]);
                             sum[i][b][1] = fmaf(s0, d[1], sum[i][b][1]);
                             sum[i][b][2] = fmaf(s1, d[2], sum[i][b][2]);
@@ -197,13 +251,10 @@ __global__ void __launch_bounds__(THREADS, 2) mx4_gemv_kernel(const MxGemvArgs a
                 // The CTAs of a cluster scale their own part of a row: each brings its sum back before they are added.
                 float v = 0.f;
                 if (a.split == 1) {
-                    const int e = min(max(134 - (int)(sh.top[m] >> 23), -126), 126);
-                    v = (part[f * PART_LD + m] + part[(IMG_ROWS + f) * PART_LD + m]) * __uint_as_float((uint32_t)(127 - e) << 23);
+                    v = (part[f * PART_LD + m] + part[(IMG_ROWS + f) * PART_LD + m]) * row_factor(sh.top[m]);
                 } else if (m % a.split == rank) {
-                    for (int r = 0; r < a.split; ++r) {
-                        const int e = min(max(134 - (int)(__float_as_uint(ld_dsmem_f32(dsmem_addr(&sh.top[m], r))) >> 23), -126), 126);
-                        v += (ld_dsmem_f32(dsmem_addr(part + f * PART_LD + m, r)) + ld_dsmem_f32(dsmem_addr(part + (IMG_ROWS + f) * PART_LD + m, r))) * __uint_as_float((uint32_t)(127 - e) << 23);
-                    }
+                    for (int r = 0; r < a.split; ++r)
+                        v += (ld_dsmem_f32(dsmem_addr(part + f * PART_LD + m, r)) + ld_dsmem_f32(dsmem_addr(part + (IMG_ROWS + f) * PART_LD + m, r))) * row_factor(__float_as_uint(ld_dsmem_f32(dsmem_addr(&sh.top[m], r))));
                 } else
                     continue;
                 const size_t row = a.ids ? blockIdx.y : m;
@@ -215,7 +266,6 @@ __global__ void __launch_bounds__(THREADS, 2) mx4_gemv_kernel(const MxGemvArgs a
             cluster_sync_all();  // nobody ends while others read its sums
             break;
         }
-        if (warp < MMA_WARPS) asm volatile("bar.sync 1, 256;" ::: "memory");  // the next tile's sums take the same place
     }
     if (warp == MMA_WARPS && lane == 0 && sh.abort_flag) mb_land_ring(sh.full, issued, (uint32_t)a.slots);
 }
@@ -241,20 +291,9 @@ cudaError_t launch(MxGemvArgs& a, int sm_count, cudaStream_t st) {
     const size_t smem = smem_bytes(a.slots, a.kb_per, cols);
     cudaError_t e = ensure_dyn_smem(mx4_gemv_kernel<NB, TERMS>, smem);
     if (e != cudaSuccess) return e;
-    cudaLaunchConfig_t cfg{};
     const int per_sm = smem <= HALF ? 2 : 1;
-    cfg.gridDim = dim3(a.split > 1 || a.ids ? (unsigned)a.tiles * a.split : (unsigned)std::min(a.tiles, per_sm * sm_count), rows);
-    cfg.blockDim = dim3(THREADS);
-    cfg.dynamicSmemBytes = smem;
-    cfg.stream = st;
-    cudaLaunchAttribute at[1];
-    if (a.split > 1) {
-        at[0].id = cudaLaunchAttributeClusterDimension;
-        at[0].val.clusterDim = {(unsigned)a.split, 1, 1};
-        cfg.attrs = at;
-        cfg.numAttrs = 1;
-    }
-    return cudaLaunchKernelEx(&cfg, mx4_gemv_kernel<NB, TERMS>, a);
+    const dim3 grid(a.split > 1 || a.ids ? (unsigned)a.tiles * a.split : (unsigned)std::min(a.tiles, per_sm * sm_count), rows);
+    return launch_after(mx4_gemv_kernel<NB, TERMS>, grid, THREADS, smem, a.split, st, a);
 }
 
 }  // namespace

@@ -334,7 +334,7 @@ HM_API int hm_post_norm_route(const float* y, const float* identity, float* x, i
  * An image holds rows the way the tensor cores take them, of dtype
  *   HM_MXFP4  blocks of 32 values along a row: an e8m0 scale 2^e, e = max(floor(log2 max|x|) - 2, -127), and e2m1 codes of x / 2^e (0, 0.5, 1,
  *             1.5, 2, 3, 4, 6) to nearest, ties to the even code, saturated at 6.  A block with an infinity or a NaN is NaN as a whole.  The last
- *             block of a row may be short.  17 / 32 bytes per value.
+ *             block of a row may be short.  17 / 32 bytes per value.  K <= 2^23.
  *   HM_BF16   bf16, rounded to nearest even: the tiles of hm_pack_bf16_tc, for rows that are rows.
  * Weights are rows too: one per output feature.  Rows of x, y and of weights to be packed are row-major with `ld` elements from row to row.
  * Images start on 16-byte boundaries; device pointers belong to the current device (HM_ERR_INVALID otherwise).  With device pointers only, every call is
