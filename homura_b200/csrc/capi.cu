@@ -1222,7 +1222,7 @@ int hm_image_pack(const void* x, int x_dtype, int rows, int K, size_t ldx, int g
     a.bf16 = x_dtype == HM_BF16;
     a.glu = glu != 0;
     a.ldx = ldx;
-    a.rows = rows;
+    a.rows = a.image_rows = rows;
     a.K = K;
     a.image = sg.out((unsigned char*)image, img_bytes(mx, rows, K), true);
     if (!a.x || !a.image) return sg.finish(cudaErrorMemoryAllocation);
@@ -1352,11 +1352,11 @@ int hm_expert_pack(const void* x, int x_dtype, int K, size_t ldx, int glu, const
     a.bf16 = x_dtype == HM_BF16;
     a.glu = glu != 0;
     a.ldx = ldx;
-    a.rows = p.rows;
+    a.rows = pairs / top;
     a.K = K;
-    a.src = p.row;
-    a.div = top;
-    a.src_rows = pairs / top;
+    a.place = p.place;
+    a.top = top;
+    a.image_rows = p.rows;
     a.image = sg.out((unsigned char*)image, img_bytes(mx, p.rows, K), true);
     if (!p.first || !a.x || !a.image) return sg.finish(cudaErrorMemoryAllocation);
     if (sg.elsewhere()) return gfail(HM_ERR_INVALID, "hm_expert_pack: memory of another device than the current one");
@@ -1387,6 +1387,7 @@ int hm_expert_gemm(const void* x_image, const void* w_images, int dtype, const i
     a.row = p.row;
     a.experts = experts;
     a.pairs = pairs;
+    a.rows = p.rows;
     if (!p.first || !a.x || !a.w || !a.y) return sg.finish(cudaErrorMemoryAllocation);
     if (sg.elsewhere()) return gfail(HM_ERR_INVALID, "hm_expert_gemm: memory of another device than the current one");
     if (!sg.ok(get_wait_err(&a.err_flag))) return sg.finish(cudaSuccess);

@@ -19,30 +19,29 @@ constexpr int THREADS = 256, WARPS = THREADS / 32;
 
 __device__ __forceinline__ float load1(const void* x, int bf16, size_t i) { return bf16 ? bf16_bits_to_f32(__ldg(static_cast<const uint16_t*>(x) + i)) : __ldg(static_cast<const float*>(x) + i); }
 
-__device__ __forceinline__ float gated(float g, float u) { return g / (1.0f + expf(-g)) * u; }
+__device__ __forceinline__ float gated(float g, float u) { return __fdividef(g, 1.0f + expf(-g)) * u; }  // the quotient to 2 ulp
 
-// Block of 32 values over four lanes (eight each): e = floor(log2 max) - 2, at least -127, as byte e + 127; codes x 2^-e to nearest even, saturated at 6.
+// Eight codes of a lane, and the scales of its four blocks (the same in sixteen lanes).  Block of 32 values over four lanes (eight each): e = floor(log2 max) - 2, at least -127, as byte e + 127; codes x 2^-e to nearest even, saturated at 6.
 // The largest exponent field is 255 where a value is infinite or no number: the whole block is then no number.
-__device__ __forceinline__ void store_mx(unsigned char* tile, int r, int lane, float (&v)[8]) {
-    uint32_t top = 0;
+__device__ __forceinline__ uint32_t mx_block(int lane, float (&v)[8], uint32_t& scales) {
+    float most = 0.f;  // keeps a NaN
 #pragma unroll
-    for (int e = 0; e < 8; ++e) top = max(top, __float_as_uint(v[e]) & 0x7FFFFFFFu);
+    for (int e = 0; e < 8; ++e) asm("max.NaN.f32 %0, %0, %1;" : "+f"(most) : "f"(fabsf(v[e])));
+    uint32_t top = __float_as_uint(most) & 0x7FFFFFFFu;
     top = max(top, __shfl_xor_sync(0xffffffffu, top, 1));
     top = max(top, __shfl_xor_sync(0xffffffffu, top, 2));
     const uint32_t field = top >> 23, s = field == 255u ? 255u : field > 2u ? field - 2u : 0u;
     const float up = __uint_as_float((254u - s) << 23);
 #pragma unroll
     for (int e = 0; e < 8; ++e) v[e] = field == 255u ? 0.f : v[e] * up;
-    const int piece = lane >> 2;
-    *reinterpret_cast<uint32_t*>(tile + MX_SCALES + r * 128 + ((piece ^ (r & 7)) << 4) + (lane & 3) * 4) = mx_codes(v);
-    uint32_t w = s << (8 * (piece & 3));
-    w |= __shfl_xor_sync(0xffffffffu, w, 4);
-    w |= __shfl_xor_sync(0xffffffffu, w, 8);
-    if ((lane & 15) == 0) *reinterpret_cast<uint32_t*>(tile + mx_scale_at(r, piece)) = w;
+    scales = s << (8 * (lane >> 2 & 3));
+    scales |= __shfl_xor_sync(0xffffffffu, scales, 4);
+    scales |= __shfl_xor_sync(0xffffffffu, scales, 8);
+    return mx_codes(v);
 }
 
-// CTA: eight rows (x), a warp each; U k-blocks of a row per warp (y).  Everything a warp loads is asked for before it works on the first.
-template <bool MX, bool BF16, bool GLU, int U>
+// CTA: eight rows of x, a warp each (grid x); U k-blocks of a row per warp (grid y).  With a plan a row is read and rounded once for all its pairs.  Everything a warp loads is asked for before it works on the first.
+template <bool MX, bool BF16, bool GLU, bool PLAN, int U>
 __global__ void __launch_bounds__(THREADS) pack_kernel(const PackArgs a, int kblocks) {
     constexpr int V = MX ? 8 : 2;  // values of a lane and k-block
     using Word = typename Words<V * (BF16 ? 2 : 4)>::type;
@@ -51,18 +50,13 @@ __global__ void __launch_bounds__(THREADS) pack_kernel(const PackArgs a, int kbl
     pdl_wait();
     const int lane = threadIdx.x & 31, row = blockIdx.x * WARPS + (threadIdx.x >> 5), kb0 = blockIdx.y * U;
     if (row >= a.rows) return;
-    long long from = row;
-    if (a.src) {
-        const int s = __ldg(a.src + row);
-        if (s < 0) return;
-        from = a.div == 1 ? s : s / a.div;
-        if (from >= a.src_rows) return;
-    }
     const size_t es = BF16 ? 2 : 4;
-    const char* x = static_cast<const char*>(a.x) + from * a.ldx * es;
-    const int r = row % IMG_ROWS, k0 = kb0 * (MX ? MX_K : BF_K) + lane * V;
-    unsigned char* tile = a.image + ((size_t)(row / IMG_ROWS) * kblocks + kb0) * (MX ? MX_TILE : IMG_CODES);
+    const char* x = static_cast<const char*>(a.x) + (size_t)row * a.ldx * es;
+    const int k0 = kb0 * (MX ? MX_K : BF_K) + lane * V;
     const bool aligned = ((uintptr_t)x & (sizeof(Word) - 1)) == 0 && (!GLU || (a.K * es & (sizeof(Word) - 1)) == 0);
+    const int copies = PLAN ? a.top : 1;
+    int place = row;  // lane c: where copy c of the row goes
+    if (PLAN) place = lane < copies ? __ldg(a.place + (size_t)row * a.top + lane) : -1;
     Word w[U][NW], g[GLU ? U : 1][NW];
 #pragma unroll
     for (int i = 0; i < U; ++i) {
@@ -89,10 +83,20 @@ __global__ void __launch_bounds__(THREADS) pack_kernel(const PackArgs a, int kbl
 #pragma unroll
             for (int e = 0; e < V; ++e) v[e] = gated(v[e], u[e]);
         }
-        if constexpr (MX)
-            store_mx(tile + (size_t)i * MX_TILE, r, lane, v);
-        else
-            *reinterpret_cast<uint32_t*>(tile + (size_t)i * IMG_CODES + r * 128 + (((lane >> 2) ^ (r & 7)) << 4) + (lane & 3) * 4) = bf16x2_rne(v[0], v[1]);
+        uint32_t codes, scales = 0;
+        if constexpr (MX) codes = mx_block(lane, v, scales);
+        else codes = bf16x2_rne(v[0], v[1]);
+        // to the row's own place, or to those of its pairs
+        if (PLAN && copies > 32 && i) place = __ldg(a.place + (size_t)row * a.top + lane);
+        for (int c = 0; c < copies; ++c) {
+            if (PLAN && c && (c & 31) == 0) place = c + lane < copies ? __ldg(a.place + (size_t)row * a.top + c + lane) : -1;
+            const int to = PLAN ? __shfl_sync(0xffffffffu, place, c & 31) : row;
+            if (PLAN && (to < 0 || to >= a.image_rows)) continue;
+            const int r = to % IMG_ROWS;
+            unsigned char* tile = a.image + ((size_t)(to / IMG_ROWS) * kblocks + kb0 + i) * (MX ? MX_TILE : IMG_CODES);
+            *reinterpret_cast<uint32_t*>(tile + (MX ? MX_SCALES : 0) + r * 128 + (((lane >> 2) ^ (r & 7)) << 4) + (lane & 3) * 4) = codes;
+            if (MX && (lane & 15) == 0) *reinterpret_cast<uint32_t*>(tile + mx_scale_at(r, lane >> 2)) = scales;
+        }
     }
 }
 
@@ -142,7 +146,16 @@ __global__ void __launch_bounds__(THREADS) unpack_kernel(const unsigned char* im
             if (!BF16) p[e] = __float_as_uint(v[e]);
             else if ((e & 1) == 0) p[e / 2] = bf16x2_rne(v[e], v[e + 1]);
         }
-        if (aligned && n >= V) {
+        if (MX && !BF16 && aligned && __all_sync(0xffffffffu, n >= V)) {
+            // lanes in pairs swap halves, so that a store fills whole sectors of 32 bytes
+            const bool odd = lane & 1;
+            uint32_t q[4];
+#pragma unroll
+            for (int e = 0; e < 4; ++e) q[e] = __shfl_xor_sync(0xffffffffu, odd ? p[e] : p[4 % V + e], 1);
+            char* o = y + (k - (odd ? V : 0)) * es + (odd ? 16 : 0);
+            *reinterpret_cast<uint4*>(o) = odd ? make_uint4(q[0], q[1], q[2], q[3]) : make_uint4(p[0], p[1], p[2 % V], p[3 % V]);
+            *reinterpret_cast<uint4*>(o + 32) = odd ? make_uint4(p[4 % V], p[5 % V], p[6 % V], p[7 % V]) : make_uint4(q[0], q[1], q[2], q[3]);
+        } else if (aligned && n >= V) {
 #pragma unroll
             for (int e = 0; e < NW; ++e) {
                 Word o;
@@ -184,9 +197,9 @@ __global__ void __launch_bounds__(THREADS) blocks_kernel(const uint8_t* blocks, 
     if (q == 0) tile[mx_scale_at(r, piece)] = (unsigned char)s;
 }
 
-// CTA e: the expert's rows.  Counts of all experts, in copies per lane so that neither a bank nor an address is hit twice by a warp; then a thread looks at
-// eight consecutive ids at a time, so that prefix sums over the threads keep the pairs' order.
-constexpr int PLAN_THREADS = 512, PLAN_IDS = 8;
+// CTA e: the expert's rows.  A thread looks at PLAN_IDS consecutive ids of a round, so that prefix sums over the threads keep the pairs' order; one round (16384
+// pairs) stays in registers between the two passes.  First the counts of all experts, in copies per lane so that neither a bank nor an address is hit twice by a warp.
+constexpr int PLAN_THREADS = 512, PLAN_IDS = 32;
 inline int plan_copies(int experts) { return experts <= 256 ? 32 : 8; }
 __global__ void __launch_bounds__(PLAN_THREADS) plan_kernel(const int32_t* __restrict__ ids, const Plan p, int copies) {
     extern __shared__ int hist[];  // [experts][copies], then the sums in the first copy
@@ -196,10 +209,34 @@ __global__ void __launch_bounds__(PLAN_THREADS) plan_kernel(const int32_t* __res
     for (int i = tid; i < p.experts * copies; i += PLAN_THREADS) hist[i] = 0;
     __syncthreads();
     pdl_wait();
-    for (int i = tid; i < p.pairs; i += PLAN_THREADS) {
-        const int id = __ldg(ids + i);
-        if (id >= 0 && id < p.experts) atomicAdd(&hist[id * copies + (lane & (copies - 1))], 1);  // counts: the same in any order
-        else if (e == 0) p.place[i] = -1;
+    int id[PLAN_IDS];
+    const int per = min(PLAN_IDS, max((p.pairs + PLAN_THREADS - 1) / PLAN_THREADS, 1));  // ids of a thread and round
+    const int ids_of = (per + 3) & ~3;  // what a thread holds: whole fours
+    const bool aligned = ((uintptr_t)ids & 15) == 0 && (per & 3) == 0;
+    auto fetch = [&](int c0) {
+        const int i0 = c0 + tid * per;
+#pragma unroll
+        for (int k = 0; k < PLAN_IDS; k += 4) {
+            if (k >= per) break;
+            if (aligned && k < per && i0 + k + 4 <= p.pairs) {
+                const int4 v = __ldg(reinterpret_cast<const int4*>(ids + i0 + k));
+                id[k] = v.x, id[k + 1] = v.y, id[k + 2] = v.z, id[k + 3] = v.w;
+            } else {
+#pragma unroll
+                for (int j = k; j < k + 4; ++j) id[j] = j < per && i0 + j < p.pairs ? __ldg(ids + i0 + j) : -1;
+            }
+        }
+        return i0;
+    };
+    const int round = PLAN_THREADS * per;
+    for (int c0 = 0; c0 < p.pairs; c0 += round) {
+        const int i0 = fetch(c0);
+#pragma unroll
+        for (int k = 0; k < PLAN_IDS; ++k) {
+            if (k >= ids_of) break;
+            if (id[k] >= 0 && id[k] < p.experts) atomicAdd(&hist[id[k] * copies + (lane & (copies - 1))], 1);  // counts: the same in any order
+            else if (e == 0 && k < per && i0 + k < p.pairs) p.place[i0 + k] = -1;
+        }
     }
     __syncthreads();
     for (int i = tid; i < p.experts; i += PLAN_THREADS) {
@@ -229,12 +266,13 @@ __global__ void __launch_bounds__(PLAN_THREADS) plan_kernel(const int32_t* __res
     __syncthreads();
     const int row0 = first_s[0] * IMG_ROWS;
     int base = 0;
-    for (int c0 = 0; c0 < p.pairs && base < n; c0 += PLAN_THREADS * PLAN_IDS) {
-        const int i0 = c0 + tid * PLAN_IDS;
-        int id[PLAN_IDS], mine = 0;
+    for (int c0 = 0; c0 < p.pairs && base < n; c0 += round) {
+        if (p.pairs > round) fetch(c0);
+        const int i0 = c0 + tid * per;
+        int mine = 0;
 #pragma unroll
         for (int k = 0; k < PLAN_IDS; ++k) {
-            id[k] = i0 + k < p.pairs ? __ldg(ids + i0 + k) : -1;
+            if (k >= ids_of) break;
             mine += id[k] == e;
         }
         int inc = mine;
@@ -252,11 +290,13 @@ __global__ void __launch_bounds__(PLAN_THREADS) plan_kernel(const int32_t* __res
             base += warp_sums[w];
         }
 #pragma unroll
-        for (int k = 0; k < PLAN_IDS; ++k)
+        for (int k = 0; k < PLAN_IDS; ++k) {
+            if (k >= ids_of) break;
             if (id[k] == e) {
                 p.place[i0 + k] = r;
                 p.row[r++] = i0 + k;
             }
+        }
         __syncthreads();
     }
     // rows behind the expert's last, and behind the last expert's
@@ -274,24 +314,32 @@ __global__ void __launch_bounds__(THREADS) sum_kernel(const SumArgs a, int v4) {
     if (i >= a.W) return;
     float s[4] = {0.f, 0.f, 0.f, 0.f};
     const size_t at = (size_t)t * a.W + i;
-    for (int j = 0; j < a.top; ++j) {
-        const int id = __ldg(a.ids + (size_t)t * a.top + j);
-        if (id < 0 || id >= a.experts) continue;
-        const float w = __ldg(a.weights + (size_t)t * a.top + j);
-        const size_t p = ((size_t)t * a.top + j) * a.W + i;
-        if (v4) {
-            float v[4];
-            if (RB) {
-                const uint2 u = __ldg(reinterpret_cast<const uint2*>(static_cast<const uint16_t*>(a.rows) + p));
-                v[0] = bf16_lo(u.x), v[1] = bf16_hi(u.x), v[2] = bf16_lo(u.y), v[3] = bf16_hi(u.y);
-            } else {
-                const float4 u = __ldg(reinterpret_cast<const float4*>(static_cast<const float*>(a.rows) + p));
-                v[0] = u.x, v[1] = u.y, v[2] = u.z, v[3] = u.w;
-            }
+    for (int j0 = 0; j0 < a.top; j0 += 4) {  // four rows are asked for at a time
+        float w[4], v[4][4];
+        bool on[4];
 #pragma unroll
-            for (int c = 0; c < 4; ++c) s[c] = fmaf(w, v[c], s[c]);
-        } else
-            s[0] = fmaf(w, load1(a.rows, RB, p), s[0]);
+        for (int q = 0; q < 4; ++q) {
+            const size_t j = (size_t)t * a.top + j0 + q;
+            const int id = j0 + q < a.top ? __ldg(a.ids + j) : -1;
+            on[q] = id >= 0 && id < a.experts;
+            if (!on[q]) continue;
+            w[q] = __ldg(a.weights + j);
+            const size_t p = j * a.W + i;
+            if (v4 && RB) {
+                const uint2 u = __ldg(reinterpret_cast<const uint2*>(static_cast<const uint16_t*>(a.rows) + p));
+                v[q][0] = bf16_lo(u.x), v[q][1] = bf16_hi(u.x), v[q][2] = bf16_lo(u.y), v[q][3] = bf16_hi(u.y);
+            } else if (v4) {
+                const float4 u = __ldg(reinterpret_cast<const float4*>(static_cast<const float*>(a.rows) + p));
+                v[q][0] = u.x, v[q][1] = u.y, v[q][2] = u.z, v[q][3] = u.w;
+            } else
+                v[q][0] = load1(a.rows, RB, p);
+        }
+#pragma unroll
+        for (int q = 0; q < 4; ++q)
+            if (on[q])
+#pragma unroll
+                for (int c = 0; c < 4; ++c)
+                    if (c < per) s[c] = fmaf(w[q], v[q][c], s[c]);
     }
     if (a.resid) {
         const float* x = static_cast<const float*>(a.resid) + at;
@@ -316,31 +364,32 @@ inline cudaError_t grid_of(long long units, int per, unsigned* g) {
 
 }  // namespace
 
-// k-blocks of a warp: four, or what short rows have.
-static int pack_units(int kblocks) { return kblocks >= 3 ? 4 : kblocks; }
+// k-blocks of a warp: three, or one where that gives too few warps (two rounds of 148 SMs with 64 warps each).
+static int pack_units(long long rows, int kblocks) { return kblocks < 3 || rows * kblocks < 2 * 148 * 64 ? 1 : 3; }
 
 cudaError_t launch_image_pack(const PackArgs& a, bool mx, cudaStream_t st) {
-    const int kblocks = img_kblocks(mx, a.K), U = pack_units(kblocks);
+    const int kblocks = img_kblocks(mx, a.K), U = pack_units(a.rows, kblocks);
     const dim3 g((a.rows + WARPS - 1) / WARPS, (kblocks + U - 1) / U);
     if (g.y > 65535) return cudaErrorInvalidValue;
-    auto launch = [&](auto MX, auto B, auto G) {
-        if (U == 1) return launch_after(pack_kernel<MX.value, B.value, G.value, 1>, g, THREADS, 0, 1, st, a, kblocks);
-        if (U == 2) return launch_after(pack_kernel<MX.value, B.value, G.value, 2>, g, THREADS, 0, 1, st, a, kblocks);
-        return launch_after(pack_kernel<MX.value, B.value, G.value, 4>, g, THREADS, 0, 1, st, a, kblocks);
+    auto launch = [&](auto MX, auto B, auto G, auto P) {
+        if (U == 1) return launch_after(pack_kernel<MX.value, B.value, G.value, P.value, 1>, g, THREADS, 0, 1, st, a, kblocks);
+        return launch_after(pack_kernel<MX.value, B.value, G.value, P.value, 3>, g, THREADS, 0, 1, st, a, kblocks);
     };
-    auto with = [&](auto MX, auto B) { return a.glu ? launch(MX, B, std::true_type{}) : launch(MX, B, std::false_type{}); };
-    if (mx) return a.bf16 ? with(std::true_type{}, std::true_type{}) : with(std::true_type{}, std::false_type{});
-    return a.bf16 ? with(std::false_type{}, std::true_type{}) : with(std::false_type{}, std::false_type{});
+    const std::true_type yes;
+    const std::false_type no;
+    auto with_glu = [&](auto MX, auto B, auto G) { return a.place ? launch(MX, B, G, yes) : launch(MX, B, G, no); };
+    auto with = [&](auto MX, auto B) { return a.glu ? with_glu(MX, B, yes) : with_glu(MX, B, no); };
+    if (mx) return a.bf16 ? with(yes, yes) : with(yes, no);
+    return a.bf16 ? with(no, yes) : with(no, no);
 }
 
 cudaError_t launch_image_unpack(const unsigned char* image, bool mx, int rows, int K, void* out, bool bf16, size_t ld, cudaStream_t st) {
-    const int kblocks = img_kblocks(mx, K), U = pack_units(kblocks);
+    const int kblocks = img_kblocks(mx, K), U = pack_units(rows, kblocks);
     const dim3 g((rows + WARPS - 1) / WARPS, (kblocks + U - 1) / U);
     if (g.y > 65535) return cudaErrorInvalidValue;
     auto with = [&](auto MX, auto B) {
         if (U == 1) return launch_after(unpack_kernel<MX.value, B.value, 1>, g, THREADS, 0, 1, st, image, rows, K, kblocks, out, ld);
-        if (U == 2) return launch_after(unpack_kernel<MX.value, B.value, 2>, g, THREADS, 0, 1, st, image, rows, K, kblocks, out, ld);
-        return launch_after(unpack_kernel<MX.value, B.value, 4>, g, THREADS, 0, 1, st, image, rows, K, kblocks, out, ld);
+        return launch_after(unpack_kernel<MX.value, B.value, 3>, g, THREADS, 0, 1, st, image, rows, K, kblocks, out, ld);
     };
     if (mx) return bf16 ? with(std::true_type{}, std::true_type{}) : with(std::true_type{}, std::false_type{});
     return bf16 ? with(std::false_type{}, std::true_type{}) : with(std::false_type{}, std::false_type{});

@@ -46,9 +46,9 @@ struct PackArgs {
     const void* x;        // rows of K values, or of 2 K with glu: silu(first K) * last K
     int bf16, glu;
     size_t ldx;           // elements from row to row
-    int rows, K;          // rows: of the image
-    const int32_t* src;   // optional: image row r is row src[r] / div of x; r is left out where src[r] < 0
-    int div, src_rows;    // ... or src[r] / div >= src_rows
+    int rows, K;          // rows: of x
+    const int32_t* place; // optional, [rows * top]: row r of x goes to the image rows place[r * top ..], -1: none
+    int top, image_rows;
     unsigned char* image;
 };
 cudaError_t launch_image_pack(const PackArgs& a, bool mx, cudaStream_t st);
@@ -75,7 +75,7 @@ struct ImageGemmArgs {
     int bf16;             // y is bf16
     const int32_t* first; // plan (null: one group of M rows): rows go to y[row[image row]]
     const int32_t *count, *row;
-    int experts, pairs;
+    int experts, pairs, rows;  // rows: of the image, at most
     int* err_flag;
     // filled in by launch_image_gemm
     int kblocks, tiles, split, kb_per, wide;

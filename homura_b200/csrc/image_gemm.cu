@@ -31,7 +31,7 @@ constexpr int STAGE_LD = IMG_ROWS * 2 + 16;      // bytes of a staged row of 128
 constexpr int STAGE_HALF = 32 * STAGE_LD;        // ... and 16 rows of 128 f32
 constexpr size_t SMEM = (size_t)SLOTS * SLOT + 4 * STAGE_HALF + 1024;
 constexpr int SF_COLS = 24, SF_BASE = 2 * TN;
-constexpr int MAX_SPLIT = 16;
+constexpr int MAX_SPLIT = 8;
 static_assert(SF_BASE + SLOTS * SF_COLS <= 512, "tensor memory");
 static_assert(TN * IMG_ROWS * 4 <= SLOTS * SLOT, "partial tile");
 
@@ -136,6 +136,12 @@ struct Shared {
 struct Unit {
     int expert, tile, row0, n;  // features tile * 128 ..; image rows row0 .. row0 + n
 };
+// Rows of an expert and the first of them in the image; none where they do not fit (a plan of other pairs).
+__device__ __forceinline__ int group(const ImageGemmArgs& a, int e, int& base) {
+    const int n = __ldg(a.count + e), b = __ldg(a.first + e);
+    base = b * IMG_ROWS;
+    return n > 0 && n <= a.pairs && b >= 0 && b <= (a.rows - n) / IMG_ROWS ? n : 0;
+}
 // Units of an expert: its rows fastest, so that units that run at the same time share weights.
 __device__ __forceinline__ Unit unit_at(const ImageGemmArgs& a, const int* ufirst, int u) {
     Unit r;
@@ -150,8 +156,9 @@ __device__ __forceinline__ Unit unit_at(const ImageGemmArgs& a, const int* ufirs
         }
         r.expert = lo;
         u -= ufirst[lo];
-        rows = __shfl_sync(0xffffffffu, __ldg(a.count + lo), 0);  // the same in all lanes: uniform for the compiler too
-        base = __shfl_sync(0xffffffffu, __ldg(a.first + lo), 0) * IMG_ROWS;
+        rows = group(a, lo, base);
+        rows = __shfl_sync(0xffffffffu, rows, 0);  // the same in all lanes: uniform for the compiler too
+        base = __shfl_sync(0xffffffffu, base, 0);
     }
     const int per = (rows + TN - 1) / TN, t = u % per;
     r.tile = u / per;
@@ -242,7 +249,8 @@ __global__ void __launch_bounds__(THREADS, 1) image_gemm_kernel(const ImageGemmA
         int sum = 0;
         for (int i0 = 0; i0 < a.experts; i0 += 32) {
             const int i = i0 + lane;
-            const int n = i < a.experts ? (__ldg(a.count + i) + TN - 1) / TN * a.tiles : 0;
+            int base;
+            const int n = i < a.experts ? (group(a, i, base) + TN - 1) / TN * a.tiles : 0;
             int inc = n;
 #pragma unroll
             for (int o = 1; o < 32; o <<= 1) {
@@ -326,7 +334,10 @@ __global__ void __launch_bounds__(THREADS, 1) image_gemm_kernel(const ImageGemmA
             const Unit t = unit_at(a, ufirst, u);
             const int n0 = t.tile * IMG_ROWS, *rows = sh.rows[ui & 1] + half * 32;
             // (nobody reads the entries of the unit before the last: its readers have met at the barrier of the last one)
-            if (et < TN) sh.rows[ui & 1][et] = et < t.n ? (a.row ? __ldg(a.row + t.row0 + et) : t.row0 + et) : -1;
+            if (et < TN) {
+                const int row = et < t.n ? (a.row ? __ldg(a.row + t.row0 + et) : t.row0 + et) : -1;
+                sh.rows[ui & 1][et] = a.row && row >= a.pairs ? -1 : row;
+            }
             asm volatile("bar.sync 1, 256;" ::: "memory");
             if (whole) {  // small code: the loops of the other warps stay in the instruction cache
                 const uint32_t buf = ci & 1u;
@@ -407,11 +418,15 @@ __global__ void __launch_bounds__(THREADS, 1) image_gemm_kernel(const ImageGemmA
         const float* part = reinterpret_cast<const float*>(ring);
         // a warp per row of 128 features; the ranks share the rows
         for (int col = rank * (THREADS / 32) + warp; col < t.n; col += a.split * (THREADS / 32)) {
+            const float* at = part + col * IMG_ROWS + lane * 4;
             float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
-            for (int r = 0; r < a.split; ++r) {
-                const float4 p = ld_dsmem_f32x4(dsmem_addr(part + col * IMG_ROWS + lane * 4, r));
-                v = make_float4(v.x + p.x, v.y + p.y, v.z + p.z, v.w + p.w);
-            }
+            float4 p[MAX_SPLIT];  // all are asked for before the first is added
+#pragma unroll
+            for (int r = 0; r < MAX_SPLIT; ++r)
+                if (r < a.split) p[r] = ld_dsmem_f32x4(dsmem_addr(at, r));
+#pragma unroll
+            for (int r = 0; r < MAX_SPLIT; ++r)
+                if (r < a.split) v = make_float4(v.x + p[r].x, v.y + p[r].y, v.z + p[r].z, v.w + p[r].w);
             const int row = a.row ? __ldg(a.row + t.row0 + col) : t.row0 + col, f = t.tile * IMG_ROWS + lane * 4;
             const float o[4] = {v.x, v.y, v.z, v.w};
 #pragma unroll
@@ -438,11 +453,14 @@ cudaError_t launch_image_gemm(ImageGemmArgs a, bool mx, int sm_count, cudaStream
         units = (long long)(a.pairs / TN + std::min(a.pairs, a.experts)) * a.tiles;  // at most
     } else {
         units = (long long)((a.M + TN - 1) / TN) * a.tiles;
-        // Fewer units than half the SMs: their k-blocks are shared out, two at least for a CTA.
-        if (units * 2 <= sm_count) a.split = (int)std::min<long long>(std::min(sm_count / units, (long long)MAX_SPLIT), (a.kblocks + 1) / 2);
+        // Fewer units than half the SMs: their k-blocks are shared out, two at least for a CTA, as far as all clusters run at once (a cluster stays within the 16 or
+        // 18 SMs of a GPC: twelve clusters of twelve took two rounds, 17 us where seven each take one).
+        if (units * 2 <= sm_count) {
+            for (a.split = (int)std::min<long long>(MAX_SPLIT, (a.kblocks + 1) / 2); a.split > 1 && units > 8LL * (16 / a.split); --a.split) {
+            }
+        }
     }
     if (units > 0x7FFFFFFF) return cudaErrorInvalidValue;
-    if (a.split > 8 && (e = ensure_nonportable_clusters(fn)) != cudaSuccess) return e;
     a.kb_per = (a.kblocks + a.split - 1) / a.split;
     a.split = (a.kblocks + a.kb_per - 1) / a.kb_per;
     return launch_after(fn, dim3(a.split > 1 ? (unsigned)units * a.split : (unsigned)std::min<long long>(units, sm_count)), THREADS, SMEM, a.split, st, a);

@@ -86,10 +86,12 @@ __global__ void __launch_bounds__(THREADS, 2) mx4_gemv_kernel(const MxGemvArgs a
         if (lane == 0) {
             const unsigned char* w = a.w + expert * a.w_stride;
             bool ok = true;
+            int s = -1;
+            uint32_t parity = 1;  // of the slot's use before
             for (int t = blockIdx.x / a.split; t < a.tiles && ok; t += step)
                 for (int kb = kb0; kb < kb1; ++kb, ++issued) {
-                    const uint32_t s = issued % a.slots;
-                    if (issued >= (uint32_t)a.slots) ok = mb_wait(&sh.empty[s], ((issued / a.slots) & 1u) ^ 1u, a.err_flag, &sh.abort_flag);
+                    if (++s == a.slots) { s = 0; parity ^= 1u; }
+                    if (issued >= (uint32_t)a.slots) ok = mb_wait(&sh.empty[s], parity, a.err_flag, &sh.abort_flag);
                     if (!ok) break;
                     mb_expect_tx(&sh.full[s], MX_TILE);
                     bulk_copy(ring + (size_t)s * MX_TILE, w + ((size_t)t * a.kblocks + kb) * MX_TILE, MX_TILE, &sh.full[s]);
@@ -102,6 +104,8 @@ __global__ void __launch_bounds__(THREADS, 2) mx4_gemv_kernel(const MxGemvArgs a
         constexpr bool B = TERMS == 1;
         constexpr int NW = B ? 1 : 2;
         const int k0 = kb0 * MX_K, items = a.M * nkb * 32;
+        const uint32_t per = (1u << 22) / nkb + 1;  // (it >> 5) / nkb by multiplication: exact below 2^10, and there are 8 rows of 128 k-blocks at most
+        auto row_of = [&](int it) { return (int)(((uint32_t)it >> 5) * per >> 22); };
         const size_t es = B ? 2 : 4;
         const char* x = static_cast<const char*>(a.x) + (xrow0 * a.ldx + k0) * es;
         const bool aligned = ((uintptr_t)x & 15) == 0 && (a.ldx * es & 15) == 0;
@@ -111,7 +115,7 @@ __global__ void __launch_bounds__(THREADS, 2) mx4_gemv_kernel(const MxGemvArgs a
             for (int u = 0; u < XU; ++u) {
                 const int it = it0 + u * XT;
                 if (it >= items) continue;
-                const int m = (it >> 5) / nkb, k = (it - m * nkb * 32) * 8;
+                const int m = row_of(it), k = (it - m * nkb * 32) * 8;
                 const char* row = x + m * a.ldx * es;
                 if (aligned && k0 + k + 8 <= a.K) {
 #pragma unroll
@@ -135,7 +139,7 @@ __global__ void __launch_bounds__(THREADS, 2) mx4_gemv_kernel(const MxGemvArgs a
                     if (b < 0x7F800000u) top = max(top, b);
                 }
                 top = __reduce_max_sync(0xffffffffu, top);
-                if (lane == 0) atomicMax(&sh.top[(it >> 5) / nkb], top);
+                if (lane == 0) atomicMax(&sh.top[row_of(it)], top);
             }
         }
         asm volatile("bar.sync 1, 256;" ::: "memory");
@@ -145,7 +149,7 @@ __global__ void __launch_bounds__(THREADS, 2) mx4_gemv_kernel(const MxGemvArgs a
             for (int u = 0; u < XU; ++u) {
                 const int it = it0 + u * XT;
                 if (it >= items) continue;
-                const int m = (it >> 5) / nkb, k = (it - m * nkb * 32) * 8;
+                const int m = row_of(it), k = (it - m * nkb * 32) * 8;
                 const float up = __uint_as_float((uint32_t)(row_exponent(sh.top[m]) + 127) << 23);
                 float v[8];
                 widen<8, B>(w[u], v);
@@ -168,7 +172,8 @@ __global__ void __launch_bounds__(THREADS, 2) mx4_gemv_kernel(const MxGemvArgs a
     }
     __syncwarp();
     const int fg = warp & 3, kh = (warp >> 2) & 1, g = lane >> 2, tl = lane & 3;
-    uint32_t used = 0;
+    int s = -1;
+    uint32_t parity = 0;
     for (int t = blockIdx.x / a.split, turn = 0; t < a.tiles; t += step, turn ^= 1) {
         float* part = parts + (size_t)turn * 2 * IMG_ROWS * PART_LD;
         if (warp < MMA_WARPS) {
@@ -179,9 +184,9 @@ __global__ void __launch_bounds__(THREADS, 2) mx4_gemv_kernel(const MxGemvArgs a
                 for (int b = 0; b < NB; ++b)
 #pragma unroll
                     for (int e = 0; e < 4; ++e) sum[i][b][e] = 0.f;
-            for (int kb = 0; kb < nkb; ++kb, ++used) {
-                const uint32_t s = used % a.slots;
-                if (!__all_sync(0xffffffffu, mb_wait(&sh.full[s], (used / a.slots) & 1u, a.err_flag, &sh.abort_flag))) continue;
+            for (int kb = 0; kb < nkb; ++kb) {
+                if (++s == a.slots) { s = 0; parity ^= 1u; }
+                if (!__all_sync(0xffffffffu, mb_wait(&sh.full[s], parity, a.err_flag, &sh.abort_flag))) continue;
                 const unsigned char* tile = ring + (size_t)s * MX_TILE;
                 const uint32_t* sc = reinterpret_cast<const uint32_t*>(tile + kh * 512 + fg * 4);
                 uint32_t scales[4];  // of features g, g + 8, g + 16, g + 24 of the group: a byte per block of this half
@@ -244,22 +249,34 @@ __global__ void __launch_bounds__(THREADS, 2) mx4_gemv_kernel(const MxGemvArgs a
             if (a.split == 1) asm volatile("bar.sync 1, 256;" ::: "memory");
         }
         if (a.split > 1) cluster_sync_all();  // one tile per cluster
-        // thread: a feature and every second row
+        // thread: a feature and every second row (of those that fall to this CTA of a cluster)
         const int f = tid & 127, n = t * IMG_ROWS + f;
         if (warp < MMA_WARPS && n < a.N) {
-            for (int m = tid >> 7; m < a.M; m += 2) {
-                // The CTAs of a cluster scale their own part of a row: each brings its sum back before they are added.
-                float v = 0.f;
-                if (a.split == 1) {
-                    v = (part[f * PART_LD + m] + part[(IMG_ROWS + f) * PART_LD + m]) * row_factor(sh.top[m]);
-                } else if (m % a.split == rank) {
-                    for (int r = 0; r < a.split; ++r)
-                        v += (ld_dsmem_f32(dsmem_addr(part + f * PART_LD + m, r)) + ld_dsmem_f32(dsmem_addr(part + (IMG_ROWS + f) * PART_LD + m, r))) * row_factor(__float_as_uint(ld_dsmem_f32(dsmem_addr(&sh.top[m], r))));
-                } else
-                    continue;
-                const size_t row = a.ids ? blockIdx.y : m;
-                if (a.y_bf16) static_cast<uint16_t*>(a.y)[row * a.ldy + n] = (uint16_t)bf16x2_rne(v, 0.f);
-                else static_cast<float*>(a.y)[row * a.ldy + n] = v;
+            auto store = [&](int m, float v) {
+                const size_t at = (a.ids ? blockIdx.y : m) * a.ldy + n;
+                if (a.y_bf16) static_cast<uint16_t*>(a.y)[at] = (uint16_t)bf16x2_rne(v, 0.f);
+                else static_cast<float*>(a.y)[at] = v;
+            };
+            const float* p = part + f * PART_LD;
+            if (a.split == 1) {
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    const int m = 2 * i + (tid >> 7);
+                    if (m < a.M) store(m, (p[m] + p[IMG_ROWS * PART_LD + m]) * row_factor(sh.top[m]));
+                }
+            } else {
+                for (int m = rank + (tid >> 7) * a.split; m < a.M; m += 2 * a.split) {
+                    // the CTAs scale their own part of a row: each brings its sum back before they are added
+                    float q[MAX_SPLIT];
+#pragma unroll
+                    for (int r = 0; r < MAX_SPLIT; ++r)
+                        if (r < a.split) q[r] = (ld_dsmem_f32(dsmem_addr(p + m, r)) + ld_dsmem_f32(dsmem_addr(p + IMG_ROWS * PART_LD + m, r))) * row_factor(__float_as_uint(ld_dsmem_f32(dsmem_addr(&sh.top[m], r))));
+                    float v = q[0];
+#pragma unroll
+                    for (int r = 1; r < MAX_SPLIT; ++r)
+                        if (r < a.split) v += q[r];
+                    store(m, v);
+                }
             }
         }
         if (a.split > 1) {
