@@ -89,11 +89,36 @@ __device__ __forceinline__ void step_mx(uint32_t d, uint32_t sa, uint32_t a, uin
 __device__ __forceinline__ void mma_commit(uint64_t* bar) {
     asm volatile("{ .reg .pred e;\n elect.sync _|e, 0xffffffff;\n @e tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0]; }" ::"r"(s32(bar)) : "memory");
 }
-__device__ __forceinline__ void expect_tx(uint64_t* b, uint32_t bytes) {
-    asm volatile("{ .reg .pred e;\n .reg .b64 st;\n elect.sync _|e, 0xffffffff;\n @e mbarrier.arrive.expect_tx.shared::cta.b64 st, [%0], %1; }" ::"r"(s32(b)), "r"(bytes) : "memory");
+// Copies of a k-block into a slot: features (`TILE` bytes), the rows' scales and codes of one or two (two) blocks of the rows' image.
+struct Copies {
+    uint64_t w, x0, x1;      // in the images: features; rows, or with scales these; the second block's
+    uint32_t b0, b1, bytes;  // bytes of the rows' parts, and of all copies
+    uint32_t two;
+};
+__device__ __forceinline__ void copy_bf16(const Copies& c, uint32_t bar, uint32_t wa, uint32_t xa) {
+    asm volatile("{ .reg .pred e, q;\n .reg .b64 st;\n .reg .b32 t;\n"
+                 "setp.ne.b32 q, %9, 0;\n add.u32 t, %5, %6;\n"
+                 "elect.sync _|e, 0xffffffff;\n and.pred q, q, e;\n"
+                 "@e mbarrier.arrive.expect_tx.shared::cta.b64 st, [%0], %8;\n"
+                 "@e cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%4], [%1], %10, [%0];\n"
+                 "@e cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%5], [%2], %6, [%0];\n"
+                 "@q cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [t], [%3], %7, [%0]; }" ::"r"(bar), "l"(c.w), "l"(c.x0), "l"(c.x1), "r"(wa), "r"(xa), "r"(c.b0), "r"(c.b1), "r"(c.bytes), "r"(c.two), "n"(IMG_CODES)
+                 : "memory");
 }
-__device__ __forceinline__ void load(void* dst, const void* src, uint32_t bytes, uint64_t* bar) {
-    asm volatile("{ .reg .pred e;\n elect.sync _|e, 0xffffffff;\n @e cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3]; }" ::"r"(s32(dst)), "l"(src), "r"(bytes), "r"(s32(bar)) : "memory");
+// xs: the slot's place for the rows' scales, two times MX_SCALES in front of their codes; off: bytes in front of the first row's codes.
+__device__ __forceinline__ void copy_mx(const Copies& c, uint32_t bar, uint32_t wa, uint32_t xs, uint64_t off) {
+    asm volatile("{ .reg .pred e, q;\n .reg .b64 st, y0, y1;\n .reg .b32 s1, d0, d1;\n"
+                 "setp.ne.b32 q, %8, 0;\n add.u32 s1, %5, %10;\n add.u32 d0, s1, %10;\n add.u32 d1, d0, %6;\n"
+                 "add.u64 y0, %2, %11;\n add.u64 y1, %3, %10;\n"
+                 "elect.sync _|e, 0xffffffff;\n and.pred q, q, e;\n"
+                 "@e mbarrier.arrive.expect_tx.shared::cta.b64 st, [%0], %9;\n"
+                 "@e cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%4], [%1], %12, [%0];\n"
+                 "@e cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%5], [%2], %10, [%0];\n"
+                 "@e cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [d0], [y0], %6, [%0];\n"
+                 "@q cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [s1], [%3], %10, [%0];\n"
+                 "@q cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [d1], [y1], %7, [%0]; }" ::"r"(bar), "l"(c.w), "l"(c.x0), "l"(c.x1), "r"(wa), "r"(xs), "r"(c.b0), "r"(c.b1), "r"(c.two), "r"(c.bytes), "n"(MX_SCALES),
+                 "l"(off), "n"(MX_TILE)
+                 : "memory");
 }
 // 32 features (the warp's lanes of the tensor memory) x 32 rows: a lane has one feature of all rows, or, BF16, the fragments that stmatrix takes: of eight
 // rows and eight features lane 4 f + r has feature f, rows 2 r and 2 r + 1.
@@ -136,14 +161,39 @@ struct Shared {
 struct Unit {
     int expert, tile, row0, n;  // features tile * 128 ..; image rows row0 .. row0 + n
 };
-// Rows of an expert and the first of them in the image; none where they do not fit (a plan of other pairs).
-__device__ __forceinline__ int group(const ImageGemmArgs& a, int e, int& base) {
-    const int n = __ldg(a.count + e), b = __ldg(a.first + e);
-    base = b * IMG_ROWS;
-    return n > 0 && n <= a.pairs && b >= 0 && b <= (a.rows - n) / IMG_ROWS ? n : 0;
+// Groups of rows, in shared memory: an expert's first unit, rows, and first image row.
+struct Groups {
+    int unit[PLAN_EXPERTS], rows[PLAN_EXPERTS], base[PLAN_EXPERTS];
+};
+// A warp reads the plan; returns the number of units.  Groups that do not fit (a plan of other pairs) have no rows.
+__device__ __forceinline__ int read_groups(const ImageGemmArgs& a, Groups& g, int lane) {
+    int sum = 0;
+    for (int i0 = 0; i0 < a.experts; i0 += 32) {
+        const int i = i0 + lane;
+        int rows = 0, base = 0;
+        if (i < a.experts) {
+            const int n = __ldg(a.count + i), b = __ldg(a.first + i);
+            base = b * IMG_ROWS;
+            rows = n > 0 && n <= a.pairs && b >= 0 && b <= (a.rows - n) / IMG_ROWS ? n : 0;
+        }
+        const int units = (rows + TN - 1) / TN * a.tiles;
+        int inc = units;
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) {
+            const int t = __shfl_up_sync(0xffffffffu, inc, o);
+            if (lane >= o) inc += t;
+        }
+        if (i < a.experts) {
+            g.unit[i] = sum + inc - units;
+            g.rows[i] = rows;
+            g.base[i] = base;
+        }
+        sum += __shfl_sync(0xffffffffu, inc, 31);
+    }
+    return sum;
 }
 // Units of an expert: its rows fastest, so that units that run at the same time share weights.
-__device__ __forceinline__ Unit unit_at(const ImageGemmArgs& a, const int* ufirst, int u) {
+__device__ __forceinline__ Unit unit_at(const ImageGemmArgs& a, const Groups& g, int u) {
     Unit r;
     int rows = a.M, base = 0;
     r.expert = 0;
@@ -151,14 +201,13 @@ __device__ __forceinline__ Unit unit_at(const ImageGemmArgs& a, const int* ufirs
         int lo = 0, hi = a.experts;  // the last expert whose first unit is at most u
         while (hi - lo > 1) {
             const int mid = (lo + hi) >> 1;
-            if (ufirst[mid] <= u) lo = mid;
+            if (g.unit[mid] <= u) lo = mid;
             else hi = mid;
         }
-        r.expert = lo;
-        u -= ufirst[lo];
-        rows = group(a, lo, base);
-        rows = __shfl_sync(0xffffffffu, rows, 0);  // the same in all lanes: uniform for the compiler too
-        base = __shfl_sync(0xffffffffu, base, 0);
+        r.expert = __shfl_sync(0xffffffffu, lo, 0);  // the same in all lanes: uniform for the compiler too
+        rows = __shfl_sync(0xffffffffu, g.rows[lo], 0);
+        base = __shfl_sync(0xffffffffu, g.base[lo], 0);
+        u -= __shfl_sync(0xffffffffu, g.unit[lo], 0);
     }
     const int per = (rows + TN - 1) / TN, t = u % per;
     r.tile = u / per;
@@ -167,10 +216,6 @@ __device__ __forceinline__ Unit unit_at(const ImageGemmArgs& a, const int* ufirs
     return r;
 }
 
-__device__ __forceinline__ void store1(const ImageGemmArgs& a, int row, int f, float v) {
-    if (a.bf16) static_cast<uint16_t*>(a.y)[(size_t)row * a.ldy + f] = (uint16_t)bf16x2_rne(v, 0.f);
-    else static_cast<float*>(a.y)[(size_t)row * a.ldy + f] = v;
-}
 // An epilogue warp has 32 features (lane: one) of 32 rows; the four warps of a half bring the rows of 128 features together in shared memory (two buffers in turn,
 // one barrier each) and store them as whole lines, 16 bytes per lane.  Stored from the registers, 4 bytes per lane and a place in y for each, the same tile took
 // three times as long; as bulk copies of one row each, twice.
@@ -224,11 +269,16 @@ __device__ __forceinline__ void emit(const ImageGemmArgs& a, Stage& st, const in
     }
 }
 
+__device__ __forceinline__ void store1(const ImageGemmArgs& a, int row, int f, float v) {
+    if (a.bf16) static_cast<uint16_t*>(a.y)[(size_t)row * a.ldy + f] = (uint16_t)bf16x2_rne(v, 0.f);
+    else static_cast<float*>(a.y)[(size_t)row * a.ldy + f] = v;
+}
+
 template <bool MX, bool BF16>
 __global__ void __launch_bounds__(THREADS, 1) image_gemm_kernel(const ImageGemmArgs a) {
     extern __shared__ __align__(1024) unsigned char dsm[];
     __shared__ Shared sh;
-    __shared__ int ufirst[PLAN_EXPERTS];
+    __shared__ Groups groups;
     unsigned char* ring = dsm + ((1024u - (s32(dsm) & 1023u)) & 1023u);  // swizzle atoms need 1024-byte alignment
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
     pdl_launch_dependents();
@@ -245,22 +295,9 @@ __global__ void __launch_bounds__(THREADS, 1) image_gemm_kernel(const ImageGemmA
         asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
     }
     pdl_wait();
-    if (warp == 2 && a.first) {  // first unit of every expert
-        int sum = 0;
-        for (int i0 = 0; i0 < a.experts; i0 += 32) {
-            const int i = i0 + lane;
-            int base;
-            const int n = i < a.experts ? (group(a, i, base) + TN - 1) / TN * a.tiles : 0;
-            int inc = n;
-#pragma unroll
-            for (int o = 1; o < 32; o <<= 1) {
-                const int t = __shfl_up_sync(0xffffffffu, inc, o);
-                if (lane >= o) inc += t;
-            }
-            if (i < a.experts) ufirst[i] = sum + inc - n;
-            sum += __shfl_sync(0xffffffffu, inc, 31);
-        }
-        if (lane == 0) sh.units = sum;
+    if (warp == 2 && a.first) {
+        const int n = read_groups(a, groups, lane);
+        if (lane == 0) sh.units = n;
     }
     asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
     __syncthreads();
@@ -275,28 +312,24 @@ __global__ void __launch_bounds__(THREADS, 1) image_gemm_kernel(const ImageGemmA
     if (warp == 0) {
         bool ok = true;
         for (int u = u0; u < units && ok; u += step) {
-            const Unit t = unit_at(a, ufirst, u);
+            const Unit t = unit_at(a, groups, u);
             const int off = t.row0 % IMG_ROWS, n0 = min(t.n, IMG_ROWS - off), n1 = t.n - n0;  // rows in the first and in the second block
-            const uint32_t b0 = (uint32_t)(n0 + 7) / 8 * 1024, b1 = (uint32_t)(n1 + 7) / 8 * 1024;
-            const uint32_t bytes = (uint32_t)TILE + b0 + b1 + (MX ? (n1 > 0 ? 2u : 1u) * MX_SCALES : 0u);
-            const unsigned char* w = a.w + t.expert * a.w_stride + ((size_t)t.tile * a.kblocks + kb0) * TILE;
-            const unsigned char* x = a.x + ((size_t)(t.row0 / IMG_ROWS) * a.kblocks + kb0) * TILE;
-            const size_t x_next = (size_t)a.kblocks * TILE;
-            for (int kb = kb0; kb < kb1; ++kb, ++issued, w += TILE, x += TILE) {
-                const uint32_t s = issued % SLOTS;
+            Copies c;
+            c.b0 = (uint32_t)(n0 + 7) / 8 * 1024;
+            c.b1 = (uint32_t)(n1 + 7) / 8 * 1024;
+            c.two = n1 > 0;
+            c.bytes = (uint32_t)TILE + c.b0 + c.b1 + (MX ? (1 + c.two) * MX_SCALES : 0u);
+            c.w = (uint64_t)__cvta_generic_to_global(a.w + t.expert * a.w_stride + ((size_t)t.tile * a.kblocks + kb0) * TILE);
+            c.x0 = (uint64_t)__cvta_generic_to_global(a.x + ((size_t)(t.row0 / IMG_ROWS) * a.kblocks + kb0) * TILE);
+            c.x1 = c.x0 + (size_t)a.kblocks * TILE;
+            if (!MX) c.x0 += off * 128;
+            for (int kb = kb0; kb < kb1; ++kb, ++issued, c.w += TILE, c.x0 += TILE, c.x1 += TILE) {
+                const uint32_t s = issued % SLOTS, sa = ring_at + s * SLOT, sb = sa + A_SLOT;
                 if (issued >= SLOTS) ok = mb_wait(&sh.empty[s], ((issued / SLOTS) & 1u) ^ 1u, a.err_flag, &sh.abort_flag);
                 ok = __all_sync(0xffffffffu, ok);
                 if (!ok) break;
-                unsigned char *sa = ring + (size_t)s * SLOT, *sb = sa + A_SLOT;
-                expect_tx(&sh.full[s], bytes);
-                load(sa + (MX ? 0 : MX_SCALES), w, TILE, &sh.full[s]);
-                if (MX) {
-                    load(sb, x, MX_SCALES, &sh.full[s]);
-                    if (n1 > 0) load(sb + MX_SCALES, x + x_next, MX_SCALES, &sh.full[s]);
-                }
-                const unsigned char* xk = x + (MX ? MX_SCALES : 0);
-                load(sb + 2 * MX_SCALES, xk + off * 128, b0, &sh.full[s]);
-                if (n1 > 0) load(sb + 2 * MX_SCALES + n0 * 128, xk + x_next, b1, &sh.full[s]);
+                if (MX) copy_mx(c, s32(&sh.full[s]), sa, sb, MX_SCALES + off * 128);
+                else copy_bf16(c, s32(&sh.full[s]), sa + MX_SCALES, sb + 2 * MX_SCALES);
             }
         }
     } else if (warp == 1) {
@@ -304,7 +337,7 @@ __global__ void __launch_bounds__(THREADS, 1) image_gemm_kernel(const ImageGemmA
         // results nobody uses.
         uint32_t i = 0, ci = 0;
         for (int u = u0; u < units; u += step) {
-            const Unit t = unit_at(a, ufirst, u);
+            const Unit t = unit_at(a, groups, u);
             const uint32_t off = (uint32_t)t.row0 % IMG_ROWS, n = ((uint32_t)t.n + 15) & ~15u, two = t.n + off > IMG_ROWS;
             // D f32, both operands K-major, M 128, N n; bf16, or e2m1 with e8m0 scales
             const uint32_t idesc = MX ? 1u << 7 | 1u << 10 | (n >> 3) << 17 | 1u << 23 | (128u >> 4) << 24 : 1u << 4 | 1u << 7 | 1u << 10 | (n >> 3) << 17 | (128u >> 4) << 24;
@@ -331,7 +364,7 @@ __global__ void __launch_bounds__(THREADS, 1) image_gemm_kernel(const ImageGemmA
         Stage st{ring + (size_t)SLOTS * SLOT + half * 2 * STAGE_HALF, 0, 2 + half};
         const bool whole = kb1 - kb0 <= CHUNK && a.split == 1;  // one accumulator per unit
         for (int u = u0; u < units; u += step, ++ui) {
-            const Unit t = unit_at(a, ufirst, u);
+            const Unit t = unit_at(a, groups, u);
             const int n0 = t.tile * IMG_ROWS, *rows = sh.rows[ui & 1] + half * 32;
             // (nobody reads the entries of the unit before the last: its readers have met at the barrier of the last one)
             if (et < TN) {
@@ -414,7 +447,7 @@ __global__ void __launch_bounds__(THREADS, 1) image_gemm_kernel(const ImageGemmA
     if (warp == 1) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, 512;" ::"r"(tmem) : "memory");
     if (a.split > 1) {
         cluster_sync_all();
-        const Unit t = unit_at(a, ufirst, u0);
+        const Unit t = unit_at(a, groups, u0);
         const float* part = reinterpret_cast<const float*>(ring);
         // a warp per row of 128 features; the ranks share the rows
         for (int col = rank * (THREADS / 32) + warp; col < t.n; col += a.split * (THREADS / 32)) {

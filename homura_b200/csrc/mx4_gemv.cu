@@ -34,6 +34,12 @@ __device__ __forceinline__ void mma_f16(float (&d)[4], uint32_t a0, uint32_t a1,
         : "=f"(d[0]), "=f"(d[1]), "=f"(d[2]), "=f"(d[3])
         : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1), "f"(c[0]), "f"(c[1]), "f"(c[2]), "f"(c[3]));
 }
+// A load that stays where it is written.
+__device__ __forceinline__ uint4 load_now(const void* p) {
+    uint4 v;
+    asm volatile("ld.global.nc.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "l"(p) : "memory");
+    return v;
+}
 // 2^(byte j of w - 127); 255 counts as infinite here.
 __device__ __forceinline__ float scale_of(uint32_t w, int j) {
     const uint32_t s = (j == 3 ? w >> 1 : w << (23 - 8 * j)) & 0x7F800000u;
@@ -83,6 +89,7 @@ __global__ void __launch_bounds__(THREADS, 2) mx4_gemv_kernel(const MxGemvArgs a
     __syncthreads();
     uint32_t issued = 0;
     if (warp == MMA_WARPS) {
+        asm volatile("bar.sync 2, 288;" ::: "memory");  // x is asked for first: behind the ring's tiles it would arrive after them
         if (lane == 0) {
             const unsigned char* w = a.w + expert * a.w_stride;
             bool ok = true;
@@ -119,13 +126,15 @@ __global__ void __launch_bounds__(THREADS, 2) mx4_gemv_kernel(const MxGemvArgs a
                 const char* row = x + m * a.ldx * es;
                 if (aligned && k0 + k + 8 <= a.K) {
 #pragma unroll
-                    for (int e = 0; e < NW; ++e) w[u][e] = __ldg(reinterpret_cast<const uint4*>(row + k * es) + e);
+                    for (int e = 0; e < NW; ++e) w[u][e] = load_now(row + k * es + 16 * e);
                 } else
                     load_ragged<8, B>(row, k, a.K - k0, w[u]);
             }
         };
+        fetch(tid);
+        asm volatile("bar.arrive 2, 288;" ::: "memory");
         for (int it0 = tid; it0 < items; it0 += XU * XT) {
-            fetch(it0);
+            if (it0 != tid) fetch(it0);
 #pragma unroll
             for (int u = 0; u < XU; ++u) {
                 const int it = it0 + u * XT;
