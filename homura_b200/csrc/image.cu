@@ -197,45 +197,36 @@ __global__ void __launch_bounds__(THREADS) blocks_kernel(const uint8_t* blocks, 
     if (q == 0) tile[mx_scale_at(r, piece)] = (unsigned char)s;
 }
 
-// CTA e: the expert's rows.  A thread looks at PLAN_IDS consecutive ids of a round, so that prefix sums over the threads keep the pairs' order; one round (16384
-// pairs) stays in registers between the two passes.  First the counts of all experts, in copies per lane so that neither a bank nor an address is hit twice by a warp.
-constexpr int PLAN_THREADS = 512, PLAN_IDS = 32;
+// CTA e: the expert's rows.  A warp looks at a run of up to 32 * PLAN_IDS ids of a round, 32 at a time, so that votes and sums in front of a warp keep the pairs'
+// order; one round (16384 pairs) stays in registers between the two passes.  First the counts of all experts, in copies per lane so that neither a bank nor an
+// address is hit twice by a warp.
+constexpr int PLAN_THREADS = 512, PLAN_WARPS = PLAN_THREADS / 32, PLAN_IDS = 32;
 inline int plan_copies(int experts) { return experts <= 256 ? 32 : 8; }
 __global__ void __launch_bounds__(PLAN_THREADS) plan_kernel(const int32_t* __restrict__ ids, const Plan p, int copies) {
     extern __shared__ int hist[];  // [experts][copies], then the sums in the first copy
-    __shared__ int warp_sums[PLAN_THREADS / 32], first_s[2];
+    __shared__ int warp_sums[PLAN_WARPS], first_s[2];
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, e = blockIdx.x;
     pdl_launch_dependents();
     for (int i = tid; i < p.experts * copies; i += PLAN_THREADS) hist[i] = 0;
     __syncthreads();
     pdl_wait();
     int id[PLAN_IDS];
-    const int per = min(PLAN_IDS, max((p.pairs + PLAN_THREADS - 1) / PLAN_THREADS, 1));  // ids of a thread and round
-    const int ids_of = (per + 3) & ~3;  // what a thread holds: whole fours
-    const bool aligned = ((uintptr_t)ids & 15) == 0 && (per & 3) == 0;
-    auto fetch = [&](int c0) {
-        const int i0 = c0 + tid * per;
-#pragma unroll
-        for (int k = 0; k < PLAN_IDS; k += 4) {
-            if (k >= per) break;
-            if (aligned && k < per && i0 + k + 4 <= p.pairs) {
-                const int4 v = __ldg(reinterpret_cast<const int4*>(ids + i0 + k));
-                id[k] = v.x, id[k + 1] = v.y, id[k + 2] = v.z, id[k + 3] = v.w;
-            } else {
-#pragma unroll
-                for (int j = k; j < k + 4; ++j) id[j] = j < per && i0 + j < p.pairs ? __ldg(ids + i0 + j) : -1;
-            }
-        }
-        return i0;
-    };
-    const int round = PLAN_THREADS * per;
-    for (int c0 = 0; c0 < p.pairs; c0 += round) {
-        const int i0 = fetch(c0);
+    const int per = min(PLAN_IDS, max((p.pairs + PLAN_THREADS - 1) / PLAN_THREADS, 1)), round = per * PLAN_THREADS;  // ids of a thread, of all threads
+    auto fetch = [&](int i0) {
 #pragma unroll
         for (int k = 0; k < PLAN_IDS; ++k) {
-            if (k >= ids_of) break;
+            if (k >= per) break;
+            id[k] = i0 + k * 32 < p.pairs ? __ldg(ids + i0 + k * 32) : -1;
+        }
+    };
+    const int at = warp * per * 32 + lane;
+    for (int c0 = 0; c0 < p.pairs; c0 += round) {
+        fetch(c0 + at);
+#pragma unroll
+        for (int k = 0; k < PLAN_IDS; ++k) {
+            if (k >= per) break;
             if (id[k] >= 0 && id[k] < p.experts) atomicAdd(&hist[id[k] * copies + (lane & (copies - 1))], 1);  // counts: the same in any order
-            else if (e == 0 && k < per && i0 + k < p.pairs) p.place[i0 + k] = -1;
+            else if (e == 0 && c0 + at + k * 32 < p.pairs) p.place[c0 + at + k * 32] = -1;
         }
     }
     __syncthreads();
@@ -265,37 +256,34 @@ __global__ void __launch_bounds__(PLAN_THREADS) plan_kernel(const int32_t* __res
     }
     __syncthreads();
     const int row0 = first_s[0] * IMG_ROWS;
-    int base = 0;
-    for (int c0 = 0; c0 < p.pairs && base < n; c0 += round) {
-        if (p.pairs > round) fetch(c0);
-        const int i0 = c0 + tid * per;
+    int base = row0;
+    for (int c0 = 0; c0 < p.pairs && base < row0 + n; c0 += round) {
+        if (p.pairs > round) fetch(c0 + at);
         int mine = 0;
 #pragma unroll
         for (int k = 0; k < PLAN_IDS; ++k) {
-            if (k >= ids_of) break;
+            if (k >= per) break;
             mine += id[k] == e;
         }
-        int inc = mine;
-#pragma unroll
-        for (int o = 1; o < 32; o <<= 1) {
-            const int t = __shfl_up_sync(0xffffffffu, inc, o);
-            if (lane >= o) inc += t;
-        }
-        if (lane == 31) warp_sums[warp] = inc;
+        mine = __reduce_add_sync(0xffffffffu, mine);
+        if (lane == 0) warp_sums[warp] = mine;
         __syncthreads();
-        int r = row0 + base + inc - mine;
+        int r = base;
 #pragma unroll
-        for (int w = 0; w < PLAN_THREADS / 32; ++w) {
+        for (int w = 0; w < PLAN_WARPS; ++w) {
             if (w < warp) r += warp_sums[w];
             base += warp_sums[w];
         }
 #pragma unroll
         for (int k = 0; k < PLAN_IDS; ++k) {
-            if (k >= ids_of) break;
+            if (k >= per) break;
+            const uint32_t votes = __ballot_sync(0xffffffffu, id[k] == e);
             if (id[k] == e) {
-                p.place[i0 + k] = r;
-                p.row[r++] = i0 + k;
+                const int to = r + __popc(votes & ((1u << lane) - 1u));
+                p.place[c0 + at + k * 32] = to;
+                p.row[to] = c0 + at + k * 32;
             }
+            r += __popc(votes);
         }
         __syncthreads();
     }

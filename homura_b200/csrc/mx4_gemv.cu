@@ -59,8 +59,8 @@ __device__ __forceinline__ float row_factor(uint32_t top) { return __uint_as_flo
 __host__ __device__ inline int x_ld(int kb_per) { return kb_per * MX_K + 32; }
 inline size_t smem_bytes(int slots, int kb_per, int cols) { return 1024 + (size_t)slots * MX_TILE + (size_t)cols * x_ld(kb_per) * 2 + 4 * IMG_ROWS * PART_LD * 4; }
 
-// NB: blocks of eight columns; TERMS: f16 terms of x.  Column of row m, term i: m + 8 i where the rows fill a block, else TERMS m + i.
-template <int NB, int TERMS>
+// NB: blocks of eight columns; TERMS: f16 terms of x; XU: items of x in a thread's registers.  Column of row m, term i: m + 8 i where the rows fill a block, else TERMS m + i.
+template <int NB, int TERMS, int XU>
 __global__ void __launch_bounds__(THREADS, 2) mx4_gemv_kernel(const MxGemvArgs a) {
     extern __shared__ __align__(1024) unsigned char dsm[];
     __shared__ Shared sh;
@@ -107,7 +107,7 @@ __global__ void __launch_bounds__(THREADS, 2) mx4_gemv_kernel(const MxGemvArgs a
     } else {
         // x: its largest finite value per row, then f16 terms.  An item is eight values of a row, 32 items of one row to a warp; up to XU items of a thread
         // are loaded once.
-        constexpr int XT = MMA_WARPS * 32, XU = 6;
+        constexpr int XT = MMA_WARPS * 32;
         constexpr bool B = TERMS == 1;
         constexpr int NW = B ? 1 : 2;
         const int k0 = kb0 * MX_K, items = a.M * nkb * 32;
@@ -141,13 +141,15 @@ __global__ void __launch_bounds__(THREADS, 2) mx4_gemv_kernel(const MxGemvArgs a
                 if (it >= items) continue;  // the same for the whole warp
                 float v[8];
                 widen<8, B>(w[u], v);
-                uint32_t top = 0;
+                float most = 0.f;
 #pragma unroll
-                for (int e = 0; e < 8; ++e) {
-                    const uint32_t b = __float_as_uint(v[e]) & 0x7FFFFFFFu;
-                    if (b < 0x7F800000u) top = max(top, b);
+                for (int e = 0; e < 8; ++e) most = fmaxf(most, fabsf(v[e]));  // (leaves NaNs out)
+                if (most == __int_as_float(0x7F800000)) {
+                    most = 0.f;
+#pragma unroll
+                    for (int e = 0; e < 8; ++e) most = fmaxf(most, fabsf(v[e]) < __int_as_float(0x7F800000) ? fabsf(v[e]) : 0.f);
                 }
-                top = __reduce_max_sync(0xffffffffu, top);
+                const uint32_t top = __reduce_max_sync(0xffffffffu, __float_as_uint(most));
                 if (lane == 0) atomicMax(&sh.top[row_of(it)], top);
             }
         }
@@ -315,11 +317,14 @@ cudaError_t launch(MxGemvArgs& a, int sm_count, cudaStream_t st) {
     const size_t limit = smem_bytes(3, a.kb_per, cols) <= HALF ? HALF : MOST;
     while (a.slots > 1 && smem_bytes(a.slots, a.kb_per, cols) > limit) --a.slots;
     const size_t smem = smem_bytes(a.slots, a.kb_per, cols);
-    cudaError_t e = ensure_dyn_smem(mx4_gemv_kernel<NB, TERMS>, smem);
+    // Items of x that a thread loads at once: code that runs once is bound by its instructions' fetch, and loading twice by latency (one f32 row of 896 values
+    // 5.9 us with two, 6.4 with six; seven bf16 rows of 1536 34.1 and 29.9).
+    void (*const fn)(MxGemvArgs) = a.M * a.kb_per * 32 <= 2 * MMA_WARPS * 32 ? mx4_gemv_kernel<NB, TERMS, 2> : mx4_gemv_kernel<NB, TERMS, 6>;
+    cudaError_t e = ensure_dyn_smem(fn, smem);
     if (e != cudaSuccess) return e;
     const int per_sm = smem <= HALF ? 2 : 1;
     const dim3 grid(a.split > 1 || a.ids ? (unsigned)a.tiles * a.split : (unsigned)std::min(a.tiles, per_sm * sm_count), rows);
-    return launch_after(mx4_gemv_kernel<NB, TERMS>, grid, THREADS, smem, a.split, st, a);
+    return launch_after(fn, grid, THREADS, smem, a.split, st, a);
 }
 
 }  // namespace
