@@ -59,7 +59,7 @@ __device__ __forceinline__ float row_factor(uint32_t top) { return __uint_as_flo
 __host__ __device__ inline int x_ld(int kb_per) { return kb_per * MX_K + 32; }
 inline size_t smem_bytes(int slots, int kb_per, int cols) { return 1024 + (size_t)slots * MX_TILE + (size_t)cols * x_ld(kb_per) * 2 + 4 * IMG_ROWS * PART_LD * 4; }
 
-// NB: blocks of eight columns; TERMS: f16 terms of x; XU: items of x in a thread's registers.  Column of row m, term i: m + 8 i where the rows fill a block, else TERMS m + i.
+// NB: blocks of eight columns; TERMS: f16 terms of x; XU: k-blocks of a row of x in a warp's registers.  Column of row m, term i: m + 8 i where the rows fill a block, else TERMS m + i.
 template <int NB, int TERMS, int XU>
 __global__ void __launch_bounds__(THREADS, 2) mx4_gemv_kernel(const MxGemvArgs a) {
     extern __shared__ __align__(1024) unsigned char dsm[];
@@ -85,7 +85,6 @@ __global__ void __launch_bounds__(THREADS, 2) mx4_gemv_kernel(const MxGemvArgs a
         sh.abort_flag = 0;
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
-    if (tid < 8) sh.top[tid] = 0;
     __syncthreads();
     uint32_t issued = 0;
     if (warp == MMA_WARPS) {
@@ -105,25 +104,19 @@ __global__ void __launch_bounds__(THREADS, 2) mx4_gemv_kernel(const MxGemvArgs a
                 }
         }
     } else {
-        // x: its largest finite value per row, then f16 terms.  An item is eight values of a row, 32 items of one row to a warp; up to XU items of a thread
-        // are loaded once.
-        constexpr int XT = MMA_WARPS * 32;
+        // A warp takes a row of x: its largest finite value, then f16 terms.  Up to XU k-blocks (eight values of each per lane) are loaded once.
         constexpr bool B = TERMS == 1;
         constexpr int NW = B ? 1 : 2;
-        const int k0 = kb0 * MX_K, items = a.M * nkb * 32;
-        const uint32_t per = (1u << 22) / nkb + 1;  // (it >> 5) / nkb by multiplication: exact below 2^10, and there are 8 rows of 128 k-blocks at most
-        auto row_of = [&](int it) { return (int)(((uint32_t)it >> 5) * per >> 22); };
+        const int k0 = kb0 * MX_K, m = warp;
         const size_t es = B ? 2 : 4;
-        const char* x = static_cast<const char*>(a.x) + (xrow0 * a.ldx + k0) * es;
-        const bool aligned = ((uintptr_t)x & 15) == 0 && (a.ldx * es & 15) == 0;
+        const char* row = static_cast<const char*>(a.x) + ((size_t)(xrow0 + m) * a.ldx + k0) * es;
+        const bool aligned = ((uintptr_t)row & 15) == 0;
         uint4 w[XU][NW];
-        auto fetch = [&](int it0) {
+        auto fetch = [&](int b0) {
 #pragma unroll
             for (int u = 0; u < XU; ++u) {
-                const int it = it0 + u * XT;
-                if (it >= items) continue;
-                const int m = row_of(it), k = (it - m * nkb * 32) * 8;
-                const char* row = x + m * a.ldx * es;
+                const int k = (b0 + u) * MX_K + lane * 8;
+                if (b0 + u >= nkb) break;
                 if (aligned && k0 + k + 8 <= a.K) {
 #pragma unroll
                     for (int e = 0; e < NW; ++e) w[u][e] = load_now(row + k * es + 16 * e);
@@ -131,52 +124,53 @@ __global__ void __launch_bounds__(THREADS, 2) mx4_gemv_kernel(const MxGemvArgs a
                     load_ragged<8, B>(row, k, a.K - k0, w[u]);
             }
         };
-        fetch(tid);
+        if (m < a.M) fetch(0);
         asm volatile("bar.arrive 2, 288;" ::: "memory");
-        for (int it0 = tid; it0 < items; it0 += XU * XT) {
-            if (it0 != tid) fetch(it0);
+        if (m < a.M) {
+            float most = 0.f;
+            for (int b0 = 0; b0 < nkb; b0 += XU) {
+                if (b0) fetch(b0);
 #pragma unroll
-            for (int u = 0; u < XU; ++u) {
-                const int it = it0 + u * XT;
-                if (it >= items) continue;  // the same for the whole warp
-                float v[8];
-                widen<8, B>(w[u], v);
-                float most = 0.f;
+                for (int u = 0; u < XU; ++u) {
+                    if (b0 + u >= nkb) break;
+                    float v[8];
+                    widen<8, B>(w[u], v);
 #pragma unroll
-                for (int e = 0; e < 8; ++e) most = fmaxf(most, fabsf(v[e]));  // (leaves NaNs out)
-                if (most == __int_as_float(0x7F800000)) {
-                    most = 0.f;
-#pragma unroll
-                    for (int e = 0; e < 8; ++e) most = fmaxf(most, fabsf(v[e]) < __int_as_float(0x7F800000) ? fabsf(v[e]) : 0.f);
+                    for (int e = 0; e < 8; ++e) most = fmaxf(most, fabsf(v[e]));  // (leaves NaNs out)
                 }
-                const uint32_t top = __reduce_max_sync(0xffffffffu, __float_as_uint(most));
-                if (lane == 0) atomicMax(&sh.top[row_of(it)], top);
             }
-        }
-        asm volatile("bar.sync 1, 256;" ::: "memory");
-        for (int it0 = tid; it0 < items; it0 += XU * XT) {
-            if (items > XU * XT) fetch(it0);
-#pragma unroll
-            for (int u = 0; u < XU; ++u) {
-                const int it = it0 + u * XT;
-                if (it >= items) continue;
-                const int m = row_of(it), k = (it - m * nkb * 32) * 8;
-                const float up = __uint_as_float((uint32_t)(row_exponent(sh.top[m]) + 127) << 23);
-                float v[8];
-                widen<8, B>(w[u], v);
-                uint32_t h[4], l[4];
-#pragma unroll
-                for (int e = 0; e < 4; ++e) {
-                    const float p = v[2 * e] * up, q = v[2 * e + 1] * up;
-                    h[e] = f16x2_rn(p, q);
-                    if (TERMS == 2) {  // what the first term leaves; nothing of an infinity
-                        const float rp = p - f16_bits_to_f32((uint16_t)h[e]), rq = q - f16_bits_to_f32((uint16_t)(h[e] >> 16));
-                        l[e] = f16x2_rn(fabsf(p) < __int_as_float(0x7F800000) ? rp : 0.f, fabsf(q) < __int_as_float(0x7F800000) ? rq : 0.f);
-                    }
+            uint32_t top = __reduce_max_sync(0xffffffffu, __float_as_uint(most));
+            if (top == 0x7F800000u) {  // without the infinities
+                top = 0;
+                for (int k = lane; k < min(a.K - k0, nkb * MX_K); k += 32) {
+                    const uint32_t b = (B ? (uint32_t)__ldg(reinterpret_cast<const uint16_t*>(row) + k) << 16 : __ldg(reinterpret_cast<const uint32_t*>(row) + k)) & 0x7FFFFFFFu;
+                    if (b < 0x7F800000u) top = max(top, b);
                 }
-                const int c = NB == 2 ? m : TERMS * m;
-                *reinterpret_cast<uint4*>(xs + (size_t)c * ldx + k) = make_uint4(h[0], h[1], h[2], h[3]);
-                if (TERMS == 2) *reinterpret_cast<uint4*>(xs + (size_t)(NB == 2 ? a.M + m : c + 1) * ldx + k) = make_uint4(l[0], l[1], l[2], l[3]);
+                top = __reduce_max_sync(0xffffffffu, top);
+            }
+            if (lane == 0) sh.top[m] = top;
+            const float up = __uint_as_float((uint32_t)(row_exponent(top) + 127) << 23);
+            uint16_t* to = xs + (size_t)(NB == 2 ? m : TERMS * m) * ldx + lane * 8;
+            for (int b0 = 0; b0 < nkb; b0 += XU) {
+                if (nkb > XU) fetch(b0);
+#pragma unroll
+                for (int u = 0; u < XU; ++u) {
+                    if (b0 + u >= nkb) break;
+                    float v[8];
+                    widen<8, B>(w[u], v);
+                    uint32_t h[4], l[4];
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) {
+                        const float p = v[2 * e] * up, q = v[2 * e + 1] * up;
+                        h[e] = f16x2_rn(p, q);
+                        if (TERMS == 2) {  // what the first term leaves; nothing of an infinity
+                            const float rp = p - f16_bits_to_f32((uint16_t)h[e]), rq = q - f16_bits_to_f32((uint16_t)(h[e] >> 16));
+                            l[e] = f16x2_rn(fabsf(p) < __int_as_float(0x7F800000) ? rp : 0.f, fabsf(q) < __int_as_float(0x7F800000) ? rq : 0.f);
+                        }
+                    }
+                    *reinterpret_cast<uint4*>(to + (b0 + u) * MX_K) = make_uint4(h[0], h[1], h[2], h[3]);
+                    if (TERMS == 2) *reinterpret_cast<uint4*>(to + (b0 + u) * MX_K + (size_t)(NB == 2 ? a.M : 1) * ldx) = make_uint4(l[0], l[1], l[2], l[3]);
+                }
             }
         }
         asm volatile("bar.sync 1, 256;" ::: "memory");
@@ -317,9 +311,7 @@ cudaError_t launch(MxGemvArgs& a, int sm_count, cudaStream_t st) {
     const size_t limit = smem_bytes(3, a.kb_per, cols) <= HALF ? HALF : MOST;
     while (a.slots > 1 && smem_bytes(a.slots, a.kb_per, cols) > limit) --a.slots;
     const size_t smem = smem_bytes(a.slots, a.kb_per, cols);
-    // Items of x that a thread loads at once: code that runs once is bound by its instructions' fetch, and loading twice by latency (one f32 row of 896 values
-    // 5.9 us with two, 6.4 with six; seven bf16 rows of 1536 34.1 and 29.9).
-    void (*const fn)(MxGemvArgs) = a.M * a.kb_per * 32 <= 2 * MMA_WARPS * 32 ? mx4_gemv_kernel<NB, TERMS, 2> : mx4_gemv_kernel<NB, TERMS, 6>;
+    void (*const fn)(MxGemvArgs) = a.kb_per <= 2 ? mx4_gemv_kernel<NB, TERMS, 2> : mx4_gemv_kernel<NB, TERMS, 6>;
     cudaError_t e = ensure_dyn_smem(fn, smem);
     if (e != cudaSuccess) return e;
     const int per_sm = smem <= HALF ? 2 : 1;
