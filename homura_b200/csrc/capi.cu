@@ -213,6 +213,7 @@ bool have_device() {
 
 constexpr size_t MAX_LD = 1 << 30;  // elements from row to row of a product
 constexpr int MAX_K = 1 << 23;      // values of an image's row
+constexpr int MAX_ROWS = INT_MAX - 255;  // rows of an image: sums of tiles stay within an int
 bool misaligned(const void* p, size_t n) { return ((uintptr_t)p & (n - 1)) != 0; }
 bool is_image_dtype(int d) { return d == HM_MXFP4 || d == HM_BF16; }
 bool is_row_dtype(int d) { return d == HM_F32 || d == HM_BF16; }
@@ -1205,11 +1206,11 @@ int hm_post_norm_route(const float* y, const float* identity, float* x, int M, i
     return sg.finish(launch_post_norm(a, sm_count_of_current_device(), st, false));
 }
 
-size_t hm_image_bytes(int dtype, int rows, int K) { return rows < 1 || K < 1 || !is_image_dtype(dtype) ? 0 : img_bytes(dtype == HM_MXFP4, rows, K); }
+size_t hm_image_bytes(int dtype, int rows, int K) { return rows < 1 || rows > MAX_ROWS || K < 1 || K > MAX_K || !is_image_dtype(dtype) ? 0 : img_bytes(dtype == HM_MXFP4, rows, K); }
 
 int hm_image_pack(const void* x, int x_dtype, int rows, int K, size_t ldx, int glu, int dtype, void* image, void* stream) {
     const int width = glu ? 2 : 1;
-    if (!x || !image || rows < 0 || K < 1 || K > MAX_K || ldx < (size_t)K * width) return gfail(HM_ERR_INVALID, "hm_image_pack: bad arguments (ldx >= K, 2 K with glu)");
+    if (!x || !image || rows < 0 || rows > MAX_ROWS || K < 1 || K > MAX_K || ldx < (size_t)K * width) return gfail(HM_ERR_INVALID, "hm_image_pack: bad arguments (ldx >= K, 2 K with glu)");
     if (!is_row_dtype(x_dtype) || !is_image_dtype(dtype)) return gfail(HM_ERR_UNSUPPORTED, "hm_image_pack: rows are HM_F32 or HM_BF16, images HM_MXFP4 or HM_BF16");
     if (misaligned(x, row_bytes(x_dtype)) || misaligned(image, 16)) return gfail(HM_ERR_INVALID, "hm_image_pack: misaligned pointer (images start on 16-byte boundaries)");
     if (rows == 0) return HM_OK;
@@ -1231,7 +1232,7 @@ int hm_image_pack(const void* x, int x_dtype, int rows, int K, size_t ldx, int g
 }
 
 int hm_image_unpack(const void* image, int dtype, int rows, int K, void* out, int out_dtype, size_t ldo, void* stream) {
-    if (!image || !out || rows < 0 || K < 1 || K > MAX_K || ldo < (size_t)K) return gfail(HM_ERR_INVALID, "hm_image_unpack: bad arguments (ldo >= K)");
+    if (!image || !out || rows < 0 || rows > MAX_ROWS || K < 1 || K > MAX_K || ldo < (size_t)K) return gfail(HM_ERR_INVALID, "hm_image_unpack: bad arguments (ldo >= K)");
     if (!is_row_dtype(out_dtype) || !is_image_dtype(dtype)) return gfail(HM_ERR_UNSUPPORTED, "hm_image_unpack: rows are HM_F32 or HM_BF16, images HM_MXFP4 or HM_BF16");
     if (misaligned(out, row_bytes(out_dtype)) || misaligned(image, 16)) return gfail(HM_ERR_INVALID, "hm_image_unpack: misaligned pointer (images start on 16-byte boundaries)");
     if (rows == 0) return HM_OK;
@@ -1247,7 +1248,7 @@ int hm_image_unpack(const void* image, int dtype, int rows, int K, void* out, in
 }
 
 int hm_image_from_blocks(const void* blocks, int rows, int K, void* image, void* stream) {
-    if (!blocks || !image || rows < 0 || K < 32 || K % 32 != 0) return gfail(HM_ERR_INVALID, "hm_image_from_blocks: bad arguments (K a multiple of 32)");
+    if (!blocks || !image || rows < 0 || rows > MAX_ROWS || K > MAX_K || K < 32 || K % 32 != 0) return gfail(HM_ERR_INVALID, "hm_image_from_blocks: bad arguments (K a multiple of 32)");
     if (misaligned(image, 16)) return gfail(HM_ERR_INVALID, "hm_image_from_blocks: images start on 16-byte boundaries");
     if (rows == 0) return HM_OK;
     NEED_DEVICE();
@@ -1270,7 +1271,7 @@ static int finish_product(Staging& sg, cudaError_t launched, const char* timeout
 }
 
 int hm_gemm_image(const void* x_image, const void* w_image, int dtype, int M, int K, int N, void* y, int y_dtype, size_t ldy, void* stream) {
-    if (!x_image || !w_image || !y || M < 0 || K < 1 || K > MAX_K || N < 1 || N > INT_MAX - 128 || ldy < (size_t)N || ldy > MAX_LD) return gfail(HM_ERR_INVALID, "hm_gemm_image: bad arguments (N <= ldy <= 2^30)");
+    if (!x_image || !w_image || !y || M < 0 || M > MAX_ROWS || K < 1 || K > MAX_K || N < 1 || N > MAX_ROWS || ldy < (size_t)N || ldy > MAX_LD) return gfail(HM_ERR_INVALID, "hm_gemm_image: bad arguments (N <= ldy <= 2^30)");
     if (!is_row_dtype(y_dtype) || !is_image_dtype(dtype)) return gfail(HM_ERR_UNSUPPORTED, "hm_gemm_image: y is HM_F32 or HM_BF16, images HM_MXFP4 or HM_BF16");
     if (misaligned(x_image, 16) || misaligned(w_image, 16) || misaligned(y, row_bytes(y_dtype))) return gfail(HM_ERR_INVALID, "hm_gemm_image: misaligned pointer (images start on 16-byte boundaries)");
     if (M == 0) return HM_OK;
@@ -1294,7 +1295,7 @@ int hm_gemm_image(const void* x_image, const void* w_image, int dtype, int M, in
 }
 
 int hm_gemv_mx4(const void* x, int x_dtype, size_t ldx, const void* w_image, int M, int K, int N, void* y, int y_dtype, size_t ldy, void* stream) {
-    if (!x || !w_image || !y || M < 0 || M > 8 || K < 1 || N < 1 || N > INT_MAX - 128 || ldx < (size_t)K || ldy < (size_t)N) return gfail(HM_ERR_INVALID, "hm_gemv_mx4: bad arguments (M <= 8, ldx >= K, ldy >= N)");
+    if (!x || !w_image || !y || M < 0 || M > 8 || K < 1 || N < 1 || N > MAX_ROWS || ldx < (size_t)K || ldy < (size_t)N) return gfail(HM_ERR_INVALID, "hm_gemv_mx4: bad arguments (M <= 8, ldx >= K, ldy >= N)");
     if (!is_row_dtype(x_dtype) || !is_row_dtype(y_dtype) || K > MX_GEMV_K) return gfail(HM_ERR_UNSUPPORTED, "hm_gemv_mx4: x and y are HM_F32 or HM_BF16, K at most 32768");
     if (misaligned(x, row_bytes(x_dtype)) || misaligned(w_image, 16) || misaligned(y, row_bytes(y_dtype))) return gfail(HM_ERR_INVALID, "hm_gemv_mx4: misaligned pointer (images start on 16-byte boundaries)");
     if (M == 0) return HM_OK;
@@ -1364,7 +1365,7 @@ int hm_expert_pack(const void* x, int x_dtype, int K, size_t ldx, int glu, const
 }
 
 int hm_expert_gemm(const void* x_image, const void* w_images, int dtype, const int32_t* plan, int pairs, int experts, int K, int N, void* y, int y_dtype, size_t ldy, void* stream) {
-    if (!x_image || !w_images || !plan || !y || bad_groups(pairs, experts) || K < 1 || K > MAX_K || N < 1 || N > INT_MAX - 128 || ldy < (size_t)N || ldy > MAX_LD) return gfail(HM_ERR_INVALID, "hm_expert_gemm: bad arguments (N <= ldy <= 2^30, experts <= 1024)");
+    if (!x_image || !w_images || !plan || !y || bad_groups(pairs, experts) || K < 1 || K > MAX_K || N < 1 || N > MAX_ROWS || ldy < (size_t)N || ldy > MAX_LD) return gfail(HM_ERR_INVALID, "hm_expert_gemm: bad arguments (N <= ldy <= 2^30, experts <= 1024)");
     if (!is_row_dtype(y_dtype) || !is_image_dtype(dtype)) return gfail(HM_ERR_UNSUPPORTED, "hm_expert_gemm: y is HM_F32 or HM_BF16, images HM_MXFP4 or HM_BF16");
     if (misaligned(x_image, 16) || misaligned(w_images, 16) || misaligned(plan, 4) || misaligned(y, row_bytes(y_dtype))) return gfail(HM_ERR_INVALID, "hm_expert_gemm: misaligned pointer (images start on 16-byte boundaries)");
     if (pairs == 0) return HM_OK;
@@ -1395,7 +1396,7 @@ int hm_expert_gemm(const void* x_image, const void* w_images, int dtype, const i
 }
 
 int hm_expert_gemv(const void* x, int x_dtype, size_t ldx, const void* w_images, const int32_t* ids, int pairs, int top, int experts, int K, int N, void* y, int y_dtype, size_t ldy, void* stream) {
-    if (!x || !w_images || !ids || !y || bad_groups(pairs, experts) || pairs > 65535 || top < 1 || pairs % top != 0 || K < 1 || N < 1 || N > INT_MAX - 128 || ldx < (size_t)K || ldy < (size_t)N)
+    if (!x || !w_images || !ids || !y || bad_groups(pairs, experts) || pairs > 65535 || top < 1 || pairs % top != 0 || K < 1 || N < 1 || N > MAX_ROWS || ldx < (size_t)K || ldy < (size_t)N)
         return gfail(HM_ERR_INVALID, "hm_expert_gemv: bad arguments (pairs <= 65535 and a multiple of top, ldx >= K, ldy >= N, experts <= 1024)");
     if (!is_row_dtype(x_dtype) || !is_row_dtype(y_dtype) || K > MX_GEMV_K) return gfail(HM_ERR_UNSUPPORTED, "hm_expert_gemv: x and y are HM_F32 or HM_BF16, K at most 32768");
     if (misaligned(x, row_bytes(x_dtype)) || misaligned(w_images, 16) || misaligned(ids, 4) || misaligned(y, row_bytes(y_dtype))) return gfail(HM_ERR_INVALID, "hm_expert_gemv: misaligned pointer (images start on 16-byte boundaries)");

@@ -20,7 +20,7 @@ constexpr int MX_TILE = MX_SCALES + IMG_CODES;
 constexpr int MX_K = 256, BF_K = 64;       // values of a k-block
 __host__ __device__ inline int img_kblocks(bool mx, int K) { return mx ? (K + MX_K - 1) / MX_K : (K + BF_K - 1) / BF_K; }
 __host__ __device__ inline size_t img_tile(bool mx) { return mx ? MX_TILE : IMG_CODES; }
-inline size_t img_bytes(bool mx, int rows, int K) { return (size_t)((rows + IMG_ROWS - 1) / IMG_ROWS) * img_kblocks(mx, K) * img_tile(mx); }
+inline size_t img_bytes(bool mx, int rows, int K) { return ((size_t)rows + IMG_ROWS - 1) / IMG_ROWS * img_kblocks(mx, K) * img_tile(mx); }
 // Byte of the scale of row r (of the block), block b (of 32 values of the k-block) in front of its tile.
 __host__ __device__ inline int mx_scale_at(int r, int b) { return (b >> 2) * 512 + (r & 31) * 16 + (r >> 5) * 4 + (b & 3); }
 

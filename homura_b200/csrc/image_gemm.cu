@@ -37,7 +37,7 @@ constexpr int STAGE_HALF = 32 * STAGE_LD;        // ... and 16 rows of 128 f32
 constexpr size_t SMEM = (size_t)SLOTS * SLOT + 4 * STAGE_HALF + 1024;
 constexpr int SF_COLS = 24, SF_BASE = 2 * TN;
 constexpr int MAX_SPLIT = 8;
-static_assert(SF_BASE + SLOTS * SF_COLS <= 512, "tensor memory");
+static_assert(SF_BASE + SLOTS * SF_COLS <= 512 && TN % 64 == 0, "tensor memory");
 static_assert(TN * IMG_ROWS * 4 <= SLOTS * SLOT, "partial tile");
 
 // The warps that copy and multiply stay converged: every lane runs their loops and one, elected in place, issues.  Addresses and
@@ -163,6 +163,8 @@ struct Shared {
     int rows[2][TN];  // places of a unit's rows in y, -1: none; units alternate
 };
 
+// Units begin at rows 0 or 64 of a block: their scales then begin at an even column of the tensor memory (32 rows to a column), as an MMA wants them; an odd one
+// is a misaligned address.
 struct Unit {
     int expert, tile, row0, n;  // features tile * 128 ..; image rows row0 .. row0 + n
 };
@@ -316,8 +318,9 @@ __global__ void __launch_bounds__(THREADS, 1) image_gemm_kernel(const ImageGemmA
     uint32_t issued = 0;
     if (warp == 0) {
         bool ok = true;
+        Unit t = u0 < units ? unit_at(a, groups, u0) : Unit{};
         for (int u = u0; u < units && ok; u += step) {
-            const Unit t = unit_at(a, groups, u);
+            Unit next = t;
             const int off = t.row0 % IMG_ROWS, n0 = min(t.n, IMG_ROWS - off), n1 = t.n - n0;  // rows in the first and in the second block
             Copies c;
             c.b0 = (uint32_t)(n0 + 7) / 8 * 1024;
@@ -335,14 +338,17 @@ __global__ void __launch_bounds__(THREADS, 1) image_gemm_kernel(const ImageGemmA
                 if (!ok) break;
                 if (MX) copy_mx(c, s32(&sh.full[s]), sa, sb, MX_SCALES + off * 128);
                 else copy_bf16(c, s32(&sh.full[s]), sa + MX_SCALES, sb + 2 * MX_SCALES);
+                if (kb == kb0 && u + step < units) next = unit_at(a, groups, u + step);  // looked up while copies and MMAs run
             }
+            t = next;
         }
     } else if (warp == 1) {
         // No wait's result decides anything here: where one has run out, the others return at once and the MMAs read what is there, whose
         // results nobody uses.
         uint32_t i = 0, ci = 0;
+        Unit t = u0 < units ? unit_at(a, groups, u0) : Unit{};
         for (int u = u0; u < units; u += step) {
-            const Unit t = unit_at(a, groups, u);
+            Unit next = t;
             const uint32_t off = (uint32_t)t.row0 % IMG_ROWS, n = ((uint32_t)t.n + 15) & ~15u, two = t.n + off > IMG_ROWS;
             // D f32, both operands K-major, M 128, N n; bf16, or e2m1 with e8m0 scales
             const uint32_t idesc = MX ? 1u << 7 | 1u << 10 | (n >> 3) << 17 | 1u << 23 | (128u >> 4) << 24 : 1u << 4 | 1u << 7 | 1u << 10 | (n >> 3) << 17 | (128u >> 4) << 24;
@@ -357,9 +363,11 @@ __global__ void __launch_bounds__(THREADS, 1) image_gemm_kernel(const ImageGemmA
                     const uint32_t sa = desc_lo(ring_at + s * SLOT), wa = sa + (MX_SCALES >> 4), sb = sa + (A_SLOT >> 4), xa = sb + (2 * MX_SCALES >> 4);
                     if (MX) step_mx(d, sa, wa, sb, xa, idesc, tmem + SF_BASE + s * SF_COLS, off / 32, two, kb > kc, &sh.empty[s]);
                     else step_bf16(d, wa, xa, idesc, kb > kc, &sh.empty[s]);
+                    if (kb == kb0 && u + step < units) next = unit_at(a, groups, u + step);
                 }
                 mma_commit(&sh.afull[buf]);
             }
+            t = next;
         }
     } else {
         const int quarter = warp & 3, half = (warp - 2) >> 2;  // a warp reads its own quarter of the TMEM lanes; chunks of 32 rows alternate
@@ -368,8 +376,10 @@ __global__ void __launch_bounds__(THREADS, 1) image_gemm_kernel(const ImageGemmA
         uint32_t ci = 0, ui = 0;
         Stage st{ring + (size_t)SLOTS * SLOT + half * 2 * STAGE_HALF, 0, 2 + half};
         const bool whole = kb1 - kb0 <= CHUNK && a.split == 1;  // one accumulator per unit
+        Unit t, next = u0 < units ? unit_at(a, groups, u0) : Unit{};
         for (int u = u0; u < units; u += step, ++ui) {
-            const Unit t = unit_at(a, groups, u);
+            t = next;
+            if (u + step < units) next = unit_at(a, groups, u + step);
             const int n0 = t.tile * IMG_ROWS, *rows = sh.rows[ui & 1] + half * 32;
             // (nobody reads the entries of the unit before the last: its readers have met at the barrier of the last one)
             if (et < TN) {

@@ -334,7 +334,7 @@ HM_API int hm_post_norm_route(const float* y, const float* identity, float* x, i
  * An image holds rows the way the tensor cores take them, of dtype
  *   HM_MXFP4  blocks of 32 values along a row: an e8m0 scale 2^e, e = max(floor(log2 max|x|) - 2, -127), and e2m1 codes of x / 2^e (0, 0.5, 1,
  *             1.5, 2, 3, 4, 6) to nearest, ties to the even code, saturated at 6.  A block with an infinity or a NaN is NaN as a whole.  The last
- *             block of a row may be short.  17 / 32 bytes per value.  K <= 2^23.
+ *             block of a row may be short.  17 / 32 bytes per value.  K <= 2^23, here and below.
  *   HM_BF16   bf16, rounded to nearest even: the tiles of hm_pack_bf16_tc, for rows that are rows.
  * Weights are rows too: one per output feature.  Rows of x, y and of weights to be packed are row-major with `ld` elements from row to row.
  * Images start on 16-byte boundaries; device pointers belong to the current device (HM_ERR_INVALID otherwise).  With device pointers only, every call is
@@ -351,7 +351,7 @@ HM_API int hm_image_from_blocks(const void* blocks, int rows, int K, void* image
 /* y [M, N] = x @ W^T from two images of the same dtype; f32 sums; y HM_F32 or HM_BF16 (rounded once). */
 HM_API int hm_gemm_image(const void* x_image, const void* w_image, int dtype, int M, int K, int N, void* y, int y_dtype, size_t ldy, void* stream);
 /* The same for 1 <= M <= 8 rows x that stay as they are (HM_F32 to 2^-22 of a value and 2^-32 of its row's largest, HM_BF16) and an HM_MXFP4
- * image of weights; K <= 32768. */
+ * image of weights whose scales are below 2^100 (a row's own scale is taken back at the end); K <= 32768. */
 HM_API int hm_gemv_mx4(const void* x, int x_dtype, size_t ldx, const void* w_image, int M, int K, int N, void* y, int y_dtype, size_t ldy, void* stream);
 /* Products grouped by expert.  A pair is a (token, choice) with the expert ids[pair]; ids outside [0, experts) (-1 of hm_post_norm_route) have none.
  * The images of the experts' weights stand back to back, hm_image_bytes(dtype, N, K) each.  experts <= 1024.

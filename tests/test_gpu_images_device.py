@@ -103,6 +103,24 @@ def test_more_choices_than_lanes(hm):
                 np.testing.assert_array_equal(held[at], own[p // top])
 
 
+def test_the_same_expert_twice(hm):
+    """A token may choose an expert more than once: each choice is a pair of its own."""
+    rng = np.random.default_rng(6)
+    T, top, E, K, N = 70, 3, 4, 160, 70
+    ids = rng.integers(-1, E, (T, top)).astype(np.int32)
+    x, _ = rows_of(12, T, K, F32)
+    w, _ = rows_of(13, E * N, K, F32)
+    images = np.concatenate([hm.image_pack(bits(w[e * N : (e + 1) * N]), hm.DType.MXFP4) for e in range(E)])
+    plan = hm.expert_plan(ids, E)
+    np.testing.assert_array_equal(plan, np.concatenate(ic.plan(ids, E)))
+    got = hm.expert_gemm(hm.image_pack(bits(x), hm.DType.MXFP4, plan=plan, experts=E, top=top), images, plan, N, hm.DType.MXFP4, T * top, E, K)
+    few = hm.expert_gemv(ic.mx_round(bits(x)).astype(np.float32), images, ids, N, top, E)
+    for p, e in enumerate(ids.reshape(-1)):
+        want = hm.gemm_image(hm.image_pack(bits(x[p // top : p // top + 1]), hm.DType.MXFP4), images.reshape(E, -1)[e], N, hm.DType.MXFP4, K, 1)[0] if e >= 0 else np.zeros(N, np.float32)
+        np.testing.assert_array_equal(got[p], want)  # products of 4-bit values and their sums over 160 of them are exact
+        np.testing.assert_allclose(few[p], want, rtol=0, atol=1e-5 * float(np.abs(want).max() + 1))
+
+
 def feed_forward(hm, s, st):
     """A mixture's feed-forward on the buffers of `s`."""
     pairs, E, top, W, ff, T = s["pairs"], s["E"], s["top"], s["W"], s["ff"], s["T"]

@@ -18,7 +18,8 @@ def test_sizes(hm):
     assert hm.image_bytes(hm.DType.BF16, 129, 65) == 4 * 16384
     for dtype, rows, K in [(0, 1, 1), (3, 1, 1), (10, 0, 1), (10, 1, 0), (10, -1, 5)]:
         assert hm.image_bytes(dtype, rows, K) == 0
-    assert hm.image_bytes(hm.DType.MXFP4, 2**31 - 200, 8192) == (2**31 // 128 - 1) * 32 * 17408  # beyond 32 bits
+    assert hm.image_bytes(hm.DType.MXFP4, 2**31 - 300, 8192) == (2**31 // 128 - 2) * 32 * 17408  # beyond 32 bits
+    assert hm.image_bytes(hm.DType.MXFP4, 2**31 - 1, 32) == 0 and hm.image_bytes(hm.DType.BF16, 1, 2**23 + 1) == 0  # more than a call takes
     for pairs, experts in [(0, 1), (1, 4), (5, 3), (1000, 16), (128 * 9, 8)]:
         first, count, place, row = ic.plan(np.arange(pairs) % experts, experts)
         assert hm.expert_plan_rows(pairs, experts) == row.size and row.size >= first[-1] * 128
@@ -50,6 +51,10 @@ def test_refusals(hm):
     refused(hm, UNS, lib.hm_gemm_image(p, p, F32, 1, 32, 8, p, F32, 8, None))
     refused(hm, UNS, lib.hm_gemm_image(p, p, MX, 1, 32, 8, p, 2, 8, None))
     refused(hm, INV, lib.hm_gemm_image(half, p, MX, 1, 32, 8, p, F32, 8, None))
+    refused(hm, INV, lib.hm_image_pack(p, F32, 2**31 - 1, 32, 32, 0, MX, p, None))
+    refused(hm, INV, lib.hm_image_pack(p, F32, 1, 2**23 + 1, 2**24, 0, MX, p, None))
+    refused(hm, INV, lib.hm_gemm_image(p, p, MX, 2**31 - 1, 32, 8, p, F32, 8, None))
+    refused(hm, INV, lib.hm_gemm_image(p, p, MX, 1, 32, 8, p, F32, 2**30 + 1, None))
     refused(hm, INV, lib.hm_gemv_mx4(p, F32, 32, p, 9, 32, 8, p, F32, 8, None))
     refused(hm, UNS, lib.hm_gemv_mx4(p, F32, 32769, p, 1, 32769, 8, p, F32, 8, None))
     refused(hm, INV, lib.hm_expert_plan(p, 4, 1025, p, None))
