@@ -206,7 +206,6 @@ __global__ void __launch_bounds__(PLAN_THREADS) plan_kernel(const int32_t* __res
     extern __shared__ int hist[];  // [experts][copies], then the sums in the first copy
     __shared__ int warp_sums[PLAN_WARPS], first_s[2];
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, e = blockIdx.x;
-    pdl_launch_dependents();
     for (int i = tid; i < p.experts * copies; i += PLAN_THREADS) hist[i] = 0;
     __syncthreads();
     pdl_wait();
@@ -230,10 +229,9 @@ __global__ void __launch_bounds__(PLAN_THREADS) plan_kernel(const int32_t* __res
         }
     }
     __syncthreads();
-    for (int i = tid; i < p.experts; i += PLAN_THREADS) {
-        int n = 0;
-        for (int c = 0; c < copies; ++c) n += hist[i * copies + ((c + i) & (copies - 1))];
-        hist[i * copies] = n;
+    for (int i = warp; i < p.experts; i += PLAN_WARPS) {
+        const int n = __reduce_add_sync(0xffffffffu, lane < copies ? hist[i * copies + lane] : 0);
+        if (lane == 0) hist[i * copies] = n;
     }
     __syncthreads();
     const int n = hist[e * copies];

@@ -102,7 +102,8 @@ struct MxGemvArgs {
 constexpr int MX_GEMV_K = 32768;  // widest row
 cudaError_t launch_mx4_gemv(MxGemvArgs a, int sm_count, cudaStream_t st);
 
-// Launch that may begin while the kernel in front of it ends (each of these kernels waits for that before it touches memory).
+// Launch that may begin while the kernel in front of it ends (each of these kernels waits for that before it touches memory).  Short kernels let the next one
+// begin at once; the plan and the products do not: what stood by for their end took 1 to 3 us of a chain plan, pack, product.
 template <typename... P, typename... A>
 inline cudaError_t launch_after(void (*k)(P...), dim3 grid, int threads, size_t smem, int cluster, cudaStream_t st, A... args) {
     cudaLaunchConfig_t cfg{};

@@ -14,7 +14,7 @@
 // 1.73 GHz).  A k-block takes 402 clocks of MMAs, 584 with its six scale copies, and 96 KB of shared-memory traffic with the staged results: copies in, operands
 // out and results fill two thirds of that pipe.  64 rows x 8960 -> 1536 in clusters of seven 6.9 us; 32 experts x 16 rows, 58 MB of weights, 11 us.
 // Taken back: pairs of CTAs (cta_group::2, half the rows loaded per CTA; 34.5 us: five slots do not cover the way from CTA to CTA), scales written to the
-// tensor memory by four more warps instead of copied (38 us), waits by one lane of a warp (34 us).
+// tensor memory by four more warps instead of copied (38 us), waits by one lane of a warp (34 us), groups cut into units of equal sizes (within 5 % either way).
 #include "image.h"
 
 #include <algorithm>
@@ -288,7 +288,6 @@ __global__ void __launch_bounds__(THREADS, 1) image_gemm_kernel(const ImageGemmA
     __shared__ Groups groups;
     unsigned char* ring = dsm + ((1024u - (s32(dsm) & 1023u)) & 1023u);  // swizzle atoms need 1024-byte alignment
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
-    pdl_launch_dependents();
     if (tid == 0) {
         for (int s = 0; s < SLOTS; ++s) { mb_init(&sh.full[s], 1); mb_init(&sh.empty[s], 1); }
         for (int s = 0; s < 2; ++s) { mb_init(&sh.afull[s], 1); mb_init(&sh.aempty[s], EPI_WARPS); }
