@@ -5,7 +5,7 @@
 //   unpack_kernel   the way back; f32 rows leave in whole sectors: the same rows 11.8 us (81 MB, 1.05 of it, most of them writes)
 //   blocks_kernel   GGUF blocks into the image
 //   plan_kernel     stable counting sort of the pairs by expert: a CTA per expert reads all ids (they stay in the L2), so that neither order nor
-//                   result depends on atomics' order and nothing is kept between calls.  512 pairs 2.6 us, 16384 pairs 7.5 us: bound by latency
+//                   result depends on atomics' order and nothing is kept between calls.  512 pairs 2.5 us, 16384 pairs 7.3 us: bound by latency
 //   sum_kernel      y = resid + sum of the chosen experts' rows times their weights, in the order of the choice; bound by the rows' bytes
 #include "image.h"
 
