@@ -10,7 +10,7 @@
 //     8 t .. 8 t + 7 of a block, one word of codes.
 //   * tiles that are fewer than the SMs share their k-blocks among the CTAs of a cluster, summed in rank order through distributed shared memory; otherwise
 //     a CTA walks several tiles and converts x once.
-// Measured (graph replays): one f32 row 896 -> 9728 5.7 us (4.6 MB: launch, x and two cluster barriers), seven bf16 rows 1536 -> 151936 29.3 us (128 MB, 0.67 of the
+// Measured (graph replays): one f32 row 896 -> 9728 5.2 us (4.6 MB: launch, x and two cluster barriers), seven bf16 rows 1536 -> 151936 29.3 us (128 MB, 0.67 of the
 // measured copy bandwidth): 6.0 TB/s while tiles flow, at 60 % of the issue slots, behind 5 us of launch and x; 1187 tiles leave three CTAs a fifth one.
 #include <algorithm>
 
@@ -273,16 +273,21 @@ __global__ void __launch_bounds__(THREADS, 2) mx4_gemv_kernel(const MxGemvArgs a
                 }
             } else {
                 for (int m = rank + (tid >> 7) * a.split; m < a.M; m += 2 * a.split) {
-                    // the CTAs scale their own part of a row: each brings its sum back before they are added
+                    // The CTAs scale their own part of a row: each brings its sum back before they are added, in 64 bits, where parts beyond the largest f32 of
+                    // different signs still meet.
                     float q[MAX_SPLIT];
+                    uint32_t top[MAX_SPLIT];
 #pragma unroll
                     for (int r = 0; r < MAX_SPLIT; ++r)
-                        if (r < a.split) q[r] = (ld_dsmem_f32(dsmem_addr(p + m, r)) + ld_dsmem_f32(dsmem_addr(p + IMG_ROWS * PART_LD + m, r))) * row_factor(__float_as_uint(ld_dsmem_f32(dsmem_addr(&sh.top[m], r))));
-                    float v = q[0];
+                        if (r < a.split) {
+                            q[r] = ld_dsmem_f32(dsmem_addr(p + m, r)) + ld_dsmem_f32(dsmem_addr(p + IMG_ROWS * PART_LD + m, r));
+                            top[r] = __float_as_uint(ld_dsmem_f32(dsmem_addr(&sh.top[m], r)));
+                        }
+                    double v = 0.0;
 #pragma unroll
-                    for (int r = 1; r < MAX_SPLIT; ++r)
-                        if (r < a.split) v += q[r];
-                    store(m, v);
+                    for (int r = 0; r < MAX_SPLIT; ++r)
+                        if (r < a.split) v += (double)q[r] * __hiloint2double((1023 - row_exponent(top[r])) << 20, 0);
+                    store(m, (float)v);
                 }
             }
         }

@@ -165,6 +165,44 @@ def test_few_rows_with_infinities(hm):
     np.testing.assert_array_equal(got[1], [64, 62, 63])
 
 
+def test_few_rows_at_the_ends_of_the_scales(hm):
+    """Scales 2^-127 (no normal f32), 2^-126 and 2^100, rows of 2^100 and 2^-90: results from 2^-217 (zero in f32) to beyond its largest."""
+    rng = np.random.default_rng(21)
+    K, N = 320, 12
+    x = rng.standard_normal((4, K)).astype(np.float32)
+    x[1] *= np.float32(2.0**100)
+    x[2] *= np.float32(2.0**-90)
+    x[3] = 0.0
+    codes, scales = rng.integers(0, 16, (N, K), dtype=np.uint8), np.tile(np.array([0, 1, 127, 227], np.uint8)[:, None], (3, K // 32))
+    w = ic.mx_values(codes, scales)
+    got = hm.gemv_mx4(x, ic.mx_image(codes, scales, K), N).astype(np.float64)
+    want, size = x.astype(np.float64) @ w.T, np.abs(x).astype(np.float64) @ np.abs(w).T
+    beyond = np.abs(want) > 3.5e38
+    assert beyond.any() and (got[beyond] == np.sign(want[beyond]) * np.inf).all()
+    # the bound of the head of this file; sums of scaled rows below 2^-126 lose up to 2^-149 per addition, and the row's scale (2^-100 at least) is taken back: 2^-40 of
+    # the largest x times the smallest w covers it; results below 2^-126 are rounded to 2^-149
+    slack = 2.0**-40 * np.abs(x).max(1, keepdims=True).astype(np.float64) * 2.0**-127 * K + 2.0**-149
+    limit = 160 * 2.0**-23 * size + 2.0**-32 * np.abs(x).max(1, keepdims=True) * np.abs(w).sum(1) + slack
+    assert (np.abs(got - want)[~beyond] <= limit[~beyond]).all()
+    assert (got[3] == 0).all()
+
+
+@pytest.mark.parametrize("dtype", ["mxfp4", "bf16"])
+def test_nobody_has_an_expert(hm, dtype):
+    T, top, E, K, N = 9, 2, 4, 64, 40
+    d, ids = hm.DType(TYPES[dtype]), np.full((T, top), -1, np.int32)
+    ids[3, 0] = E  # one beyond the last
+    plan = hm.expert_plan(ids, E)
+    np.testing.assert_array_equal(plan, np.concatenate(ic.plan(np.where(ids < E, ids, -1), E)))
+    x, w = np.ones((T, K), np.float32), np.ones((N, K), np.float32)
+    images = np.concatenate([hm.image_pack(w, d)] * E)
+    y = hm.expert_gemm(hm.image_pack(x, d, plan=plan, experts=E, top=top), images, plan, N, d, T * top, E, K, y=np.full((T * top, N), 5.0, np.float32))
+    assert (y == 5.0).all()
+    if dtype == "mxfp4":
+        assert (hm.expert_gemv(x, images, ids, N, top, E, y=np.full((T * top, N), 5.0, np.float32)) == 5.0).all()
+    np.testing.assert_array_equal(hm.expert_sum(y, ids, np.ones((T, top), np.float32), top, E, resid=np.full((T, N), 2.0, np.float32)), np.full((T, N), 2.0))
+
+
 def routing(rng, tokens, top, experts, none):
     ids = np.stack([rng.permutation(experts + none)[:top] for _ in range(tokens)]) if tokens else np.zeros((0, top), int)
     return np.where(ids < experts, ids, -1).astype(np.int32)
