@@ -739,6 +739,21 @@ def _rows_out(shape, dtype) -> np.ndarray:
     return np.zeros(shape, np.uint16 if dtype == DType.BF16 else np.float32)
 
 
+def _rows_over(y, shape, dtype):
+    """(the caller's rows, what the library writes over): new rows of zeros, or an array of the result's shape and type."""
+    if y is None:
+        y = _rows_out(shape, dtype)
+    elif not isinstance(y, np.ndarray) or y.dtype != (np.uint16 if dtype == DType.BF16 else np.float32) or y.shape != tuple(shape) or not y.flags.writeable:
+        raise HomuraError(HM_ERR_INVALID, f"y is a writable array {list(shape)} of f32 (bf16: uint16)")
+    return y, np.ascontiguousarray(y)
+
+
+def _written(y, over) -> np.ndarray:
+    if over is not y:
+        y[...] = over
+    return y
+
+
 def image_bytes(dtype: DType, rows: int, K: int) -> int:
     """Bytes of an image of `rows` rows of K values (DType.MXFP4 or DType.BF16)."""
     return int(load_library().hm_image_bytes(int(dtype), rows, K))
@@ -879,7 +894,7 @@ def expert_plan(ids, experts: int, plan=None, stream=None):
 
 def expert_gemm(x_image, w_images, plan, N: int, dtype: DType, pairs: int, experts: int, K: int, y=None, y_dtype: DType = DType.F32, ldy: Optional[int] = None, stream=None):
     """y [pairs, N]: each pair's row of the grouped image times its expert's weights (images back to back).  Rows of pairs without an
-    expert stay as they are (host mode: those of y, else zero)."""
+    expert stay as they are.  Host mode writes over y, which has the result's shape and type, and returns it; without y those rows are zero."""
     lib = load_library()
     if not isinstance(x_image, np.ndarray):
         _check(lib.hm_expert_gemm(_ptr(x_image), _ptr(w_images), int(dtype), _ptr(plan), pairs, experts, K, N, _ptr(y), int(y_dtype), ldy or N, _ptr(stream)))
@@ -887,13 +902,14 @@ def expert_gemm(x_image, w_images, plan, N: int, dtype: DType, pairs: int, exper
     xi, wi, p = _image_in(x_image), _image_in(w_images), np.ascontiguousarray(plan, dtype=np.int32)
     _fits(xi, 1, dtype, expert_plan_rows(pairs, experts), K, "x_image")
     _fits(wi, experts, dtype, N, K, "w_images")
-    o = _rows_out((pairs, N), y_dtype) if y is None else np.ascontiguousarray(y)
+    y, o = _rows_over(y, (pairs, N), y_dtype)
     _check(lib.hm_expert_gemm(_ptr(xi), _ptr(wi), int(dtype), _ptr(p), pairs, experts, K, N, _ptr(o), int(y_dtype), N, None))
-    return o
+    return _written(y, o)
 
 
 def expert_gemv(x, w_images, ids, N: int, top: int, experts: int, K: Optional[int] = None, x_dtype=DType.F32, ldx: Optional[int] = None, y=None, y_dtype: DType = DType.F32, ldy: Optional[int] = None, stream=None):
-    """y [pairs, N]: row p // top of x, as it is, times the MXFP4 image of expert ids[p]; for few pairs."""
+    """y [pairs, N]: row p // top of x, as it is, times the MXFP4 image of expert ids[p]; for few pairs.  Rows of pairs
+    without an expert and y in host mode: as in expert_gemm."""
     lib = load_library()
     if isinstance(x, tuple):
         (xa, rows) = x
@@ -905,9 +921,9 @@ def expert_gemv(x, w_images, ids, N: int, top: int, experts: int, K: Optional[in
     _fits(wi, experts, DType.MXFP4, N, K, "w_images")
     if ia.size != rows * top:
         raise HomuraError(HM_ERR_INVALID, "ids are top times the rows")
-    o = _rows_out((rows * top, N), y_dtype) if y is None else np.ascontiguousarray(y)
+    y, o = _rows_over(y, (rows * top, N), y_dtype)
     _check(lib.hm_expert_gemv(_ptr(xa), int(x_dtype), K, _ptr(wi), _ptr(ia), rows * top, top, experts, K, N, _ptr(o), int(y_dtype), N, None))
-    return o
+    return _written(y, o)
 
 
 def expert_sum(rows, ids, weights, top: int, experts: int, width: Optional[int] = None, rows_dtype=DType.F32, resid=None, y=None, y_dtype: DType = DType.F32, stream=None):

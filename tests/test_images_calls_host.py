@@ -1,0 +1,79 @@
+"""Arguments of the host-mode image calls that do not fit are refused before the library (or a device) is asked: without a device a call that
+is let through ends in HM_ERR_CUDA."""
+import numpy as np
+import pytest
+
+MX, BF16, F32 = 10, 1, 0
+T, TOP, E, K, N = 3, 2, 4, 64, 40
+PAIRS = T * TOP
+
+
+def invalid(hm, call):
+    with pytest.raises(hm.HomuraError) as e:
+        call()
+    assert e.value.status == hm.HM_ERR_INVALID, e.value
+
+
+def let_through(hm, call):
+    if hm.device_count():
+        return call()
+    with pytest.raises(hm.HomuraError) as e:
+        call()
+    assert e.value.status == hm.HM_ERR_CUDA, e.value
+
+
+def grouped(hm, **more):
+    plan = np.zeros(hm.expert_plan_ints(PAIRS, E), np.int32)
+    image = np.zeros(hm.image_bytes(MX, hm.expert_plan_rows(PAIRS, E), K), np.uint8)
+    weights = np.zeros(E * hm.image_bytes(MX, N, K), np.uint8)
+    return lambda: hm.expert_gemm(image, weights, more.pop("plan", plan), N, hm.DType.MXFP4, PAIRS, E, K, **more)
+
+
+def pairs(hm, **more):
+    weights = np.zeros(E * hm.image_bytes(MX, N, K), np.uint8)
+    return lambda: hm.expert_gemv(np.zeros((T, K), np.float32), weights, np.full((T, TOP), -1, np.int32), N, TOP, E, **more)
+
+
+@pytest.mark.parametrize("call", [grouped, pairs])
+def test_rows_to_be_written_over_have_the_results_type_and_shape(hm, call):
+    for y in [np.full((PAIRS, N), 7.0), np.zeros((PAIRS, N), np.float16), np.zeros((PAIRS, N), ">f4"), np.zeros((PAIRS, N), np.uint16), np.zeros((PAIRS - 1, N), np.float32), np.zeros((PAIRS, N - 1), np.float32), np.zeros(PAIRS * N, np.float32),
+              np.zeros((T, TOP, N), np.float32), [[0.0] * N] * PAIRS]:
+        invalid(hm, call(hm, y=y))
+    for y in [np.zeros((PAIRS, N), np.float32), np.zeros((PAIRS, N), np.int16), np.zeros((PAIRS, N // 2), np.uint16)]:
+        invalid(hm, call(hm, y=y, y_dtype=hm.DType.BF16))
+    fixed = np.zeros((PAIRS, N), np.float32)
+    fixed.flags.writeable = False
+    invalid(hm, call(hm, y=fixed))
+    let_through(hm, call(hm))
+    let_through(hm, call(hm, y=np.zeros((PAIRS, N), np.float32)))
+    let_through(hm, call(hm, y=np.zeros((PAIRS, N), np.uint16), y_dtype=hm.DType.BF16))
+
+
+@pytest.mark.parametrize("name", ["expert_gemm", "expert_gemv"])
+@pytest.mark.parametrize("y", [np.full((PAIRS, N), 7.0, np.float32), np.full((N, PAIRS), 7.0, np.float32).T, np.full((PAIRS, 2 * N), 7.0, np.float32)[:, ::2]], ids=["rows", "columns", "strided"])
+def test_the_callers_rows_are_what_is_written_and_returned(hm, monkeypatch, name, y):
+    """A stand-in for the library's call writes row 1 of what it is given."""
+    import ctypes as C
+
+    real, before = hm.load_library(), y.copy()
+
+    class Library:
+        def __getattr__(self, at):
+            if at != "hm_" + name:
+                return getattr(real, at)
+
+            def call(*args):
+                rows = np.ctypeslib.as_array(C.cast(args[-4], C.POINTER(C.c_float)), (PAIRS, N))
+                np.testing.assert_array_equal(rows, before)
+                rows[1] = 1.5
+                return 0
+
+            return call
+
+    monkeypatch.setattr(hm, "load_library", Library)
+    got = {"expert_gemm": grouped, "expert_gemv": pairs}[name](hm, y=y)()
+    assert got is y
+    want = before.copy()
+    want[1] = 1.5
+    np.testing.assert_array_equal(y, want)
+    y[...] = 7.0
