@@ -788,6 +788,13 @@ def _image_in(image) -> np.ndarray:
     return image
 
 
+def _plan_in(plan, pairs, experts) -> np.ndarray:
+    plan = np.ascontiguousarray(plan, dtype=np.int32)
+    if plan.size == 0 or plan.size != expert_plan_ints(pairs, experts):
+        raise HomuraError(HM_ERR_INVALID, "the plan does not match the pairs and experts")
+    return plan
+
+
 def _fits(image, count, dtype, rows, K, what):
     if image.size != count * image_bytes(dtype, rows, K) or image.size == 0:
         raise HomuraError(HM_ERR_INVALID, f"{what} does not match its sizes")
@@ -803,9 +810,8 @@ def image_pack(x, dtype: DType, K: Optional[int] = None, x_dtype=DType.F32, ldx:
         rows, ldx = xa.shape
         K = ldx // 2 if glu else ldx
         if plan is not None:
-            plan, pairs = np.ascontiguousarray(plan, dtype=np.int32), rows * top
-            if plan.size != expert_plan_ints(pairs, experts):
-                raise HomuraError(HM_ERR_INVALID, "the plan does not match the pairs and experts")
+            pairs = rows * top
+            plan = _plan_in(plan, pairs, experts)
         image = _image_out(dtype, rows if plan is None else expert_plan_rows(pairs, experts), K)
     else:
         xa, rows = x
@@ -899,7 +905,7 @@ def expert_gemm(x_image, w_images, plan, N: int, dtype: DType, pairs: int, exper
     if not isinstance(x_image, np.ndarray):
         _check(lib.hm_expert_gemm(_ptr(x_image), _ptr(w_images), int(dtype), _ptr(plan), pairs, experts, K, N, _ptr(y), int(y_dtype), ldy or N, _ptr(stream)))
         return None
-    xi, wi, p = _image_in(x_image), _image_in(w_images), np.ascontiguousarray(plan, dtype=np.int32)
+    xi, wi, p = _image_in(x_image), _image_in(w_images), _plan_in(plan, pairs, experts)
     _fits(xi, 1, dtype, expert_plan_rows(pairs, experts), K, "x_image")
     _fits(wi, experts, dtype, N, K, "w_images")
     y, o = _rows_over(y, (pairs, N), y_dtype)

@@ -77,3 +77,9 @@ def test_the_callers_rows_are_what_is_written_and_returned(hm, monkeypatch, name
     want[1] = 1.5
     np.testing.assert_array_equal(y, want)
     y[...] = 7.0
+
+
+def test_a_plan_of_other_pairs_or_experts(hm):
+    for words in [0, 3, hm.expert_plan_ints(PAIRS, E) - 1, hm.expert_plan_ints(PAIRS, E) + 1, hm.expert_plan_ints(PAIRS + 1, E), hm.expert_plan_ints(PAIRS, E + 1)]:
+        invalid(hm, grouped(hm, plan=np.zeros(words, np.int32)))
+    let_through(hm, grouped(hm))
