@@ -735,6 +735,13 @@ def _rows_in(x):
     return np.ascontiguousarray(x, dtype=np.uint16 if bits else np.float32), DType.BF16 if bits else DType.F32
 
 
+def _width(K, given) -> int:
+    """The width of host rows; a K beside them says the same."""
+    if given not in (None, K):
+        raise HomuraError(HM_ERR_INVALID, f"K = {given} beside rows of {K} values")
+    return K
+
+
 def _rows_out(shape, dtype) -> np.ndarray:
     return np.zeros(shape, np.uint16 if dtype == DType.BF16 else np.float32)
 
@@ -808,7 +815,9 @@ def image_pack(x, dtype: DType, K: Optional[int] = None, x_dtype=DType.F32, ldx:
     if host:
         xa, x_dtype = _rows_in(x)
         rows, ldx = xa.shape
-        K = ldx // 2 if glu else ldx
+        if glu and ldx % 2:
+            raise HomuraError(HM_ERR_INVALID, "gated rows have 2 K values")
+        K = _width(ldx // 2 if glu else ldx, K)
         if plan is not None:
             pairs = rows * top
             plan = _plan_in(plan, pairs, experts)
@@ -847,7 +856,10 @@ def image_from_blocks(blocks, K: int, image=None, stream=None):
         _check(lib.hm_image_from_blocks(_ptr(ba), rows, K, _ptr(image), _ptr(stream)))
         return None
     b = np.ascontiguousarray(blocks, dtype=np.uint8)
-    rows = b.size // (17 * max(K // 32, 1))
+    per = K // 32 * 17
+    if K % 32 or per <= 0 or b.size == 0 or b.size % per or (b.ndim > 1 and b[0].size != per):
+        raise HomuraError(HM_ERR_INVALID, "blocks are rows of K / 32 times 17 bytes")
+    rows = b.size // per
     im = _image_out(DType.MXFP4, rows, K)
     _check(lib.hm_image_from_blocks(_ptr(b), rows, K, _ptr(im), None))
     return im
@@ -876,7 +888,8 @@ def gemv_mx4(x, w_image, N: int, K: Optional[int] = None, x_dtype=DType.F32, ldx
         _check(lib.hm_gemv_mx4(_ptr(xa), int(x_dtype), ldx or K, _ptr(w_image), M, K, N, _ptr(y), int(y_dtype), ldy or N, _ptr(stream)))
         return None
     xa, x_dtype = _rows_in(x)
-    M, K = xa.shape
+    M, width = xa.shape
+    K = _width(width, K)
     wi = _image_in(w_image)
     _fits(wi, 1, DType.MXFP4, N, K, "w_image")
     o = _rows_out((M, N), y_dtype)
@@ -922,7 +935,8 @@ def expert_gemv(x, w_images, ids, N: int, top: int, experts: int, K: Optional[in
         _check(lib.hm_expert_gemv(_ptr(xa), int(x_dtype), ldx or K, _ptr(w_images), _ptr(ids), rows * top, top, experts, K, N, _ptr(y), int(y_dtype), ldy or N, _ptr(stream)))
         return None
     xa, x_dtype = _rows_in(x)
-    rows, K = xa.shape
+    rows, width = xa.shape
+    K = _width(width, K)
     wi, ia = _image_in(w_images), np.ascontiguousarray(ids, dtype=np.int32)
     _fits(wi, experts, DType.MXFP4, N, K, "w_images")
     if ia.size != rows * top:

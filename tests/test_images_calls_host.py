@@ -83,3 +83,25 @@ def test_a_plan_of_other_pairs_or_experts(hm):
     for words in [0, 3, hm.expert_plan_ints(PAIRS, E) - 1, hm.expert_plan_ints(PAIRS, E) + 1, hm.expert_plan_ints(PAIRS + 1, E), hm.expert_plan_ints(PAIRS, E + 1)]:
         invalid(hm, grouped(hm, plan=np.zeros(words, np.int32)))
     let_through(hm, grouped(hm))
+
+
+def test_rows_that_do_not_come_out_even(hm):
+    invalid(hm, lambda: hm.image_pack(np.zeros((3, 65), np.float32), hm.DType.MXFP4, glu=True))  # gate and up: half of 65
+    let_through(hm, lambda: hm.image_pack(np.zeros((3, 64), np.float32), hm.DType.MXFP4, glu=True))
+    for blocks, width in [(np.zeros((3, 1, 17), np.uint8), 64), (np.zeros(3 * 17 + 1, np.uint8), 32), (np.zeros((2, 4, 17), np.uint8), 64), (np.zeros((2, 34), np.uint8), 32), (np.zeros((2, 34), np.uint8), 48), (np.zeros(0, np.uint8), 32)]:
+        invalid(hm, lambda: hm.image_from_blocks(blocks, width))
+    for blocks, width in [(np.zeros((3, 2, 17), np.uint8), 64), (np.zeros((2, 34), np.uint8), 64), (np.zeros(3 * 17, np.uint8), 32)]:
+        let_through(hm, lambda: hm.image_from_blocks(blocks, width))
+
+
+def test_a_width_that_is_not_the_rows(hm):
+    """Host rows say their width themselves; a K beside them has to be the same."""
+    w = np.zeros(E * hm.image_bytes(MX, N, 32), np.uint8)
+    x, ids = np.zeros((T, K), np.float32), np.zeros((T, TOP), np.int32)
+    invalid(hm, lambda: hm.image_pack(x, hm.DType.MXFP4, K=32))
+    invalid(hm, lambda: hm.image_pack(x, hm.DType.MXFP4, K=64, glu=True))
+    invalid(hm, lambda: hm.gemv_mx4(x, w[: hm.image_bytes(MX, N, 32)], N, K=32))
+    invalid(hm, lambda: hm.expert_gemv(x, w, ids, N, TOP, E, K=32))
+    let_through(hm, lambda: hm.image_pack(x, hm.DType.MXFP4, K=64))
+    let_through(hm, lambda: hm.image_pack(x, hm.DType.MXFP4, K=32, glu=True))
+    let_through(hm, lambda: hm.gemv_mx4(x, w[: hm.image_bytes(MX, N, 32)], N, K=64))
