@@ -742,6 +742,16 @@ def _width(K, given) -> int:
     return K
 
 
+def _ids_in(ids) -> np.ndarray:
+    """Experts' ids as int32; those beyond 32 bits are no expert's: -1, not what is left of their bits."""
+    ids = np.asarray(ids)
+    if ids.dtype != np.int32:
+        within = (ids >= -(2**31)) & (ids <= 2**31 - 1)
+        ids = np.where(within, ids, 0).astype(np.int32)
+        ids[~within] = -1
+    return np.ascontiguousarray(ids)
+
+
 def _rows_out(shape, dtype) -> np.ndarray:
     return np.zeros(shape, np.uint16 if dtype == DType.BF16 else np.float32)
 
@@ -905,7 +915,7 @@ def expert_plan(ids, experts: int, plan=None, stream=None):
         (ia, pairs) = ids
         _check(lib.hm_expert_plan(_ptr(ia), pairs, experts, _ptr(plan), _ptr(stream)))
         return None
-    ia = np.ascontiguousarray(ids, dtype=np.int32)
+    ia = _ids_in(ids)
     out = np.empty(max(expert_plan_ints(ia.size, experts), 1), np.int32)
     _check(lib.hm_expert_plan(_ptr(ia), ia.size, experts, _ptr(out), None))
     return out
@@ -937,7 +947,7 @@ def expert_gemv(x, w_images, ids, N: int, top: int, experts: int, K: Optional[in
     xa, x_dtype = _rows_in(x)
     rows, width = xa.shape
     K = _width(width, K)
-    wi, ia = _image_in(w_images), np.ascontiguousarray(ids, dtype=np.int32)
+    wi, ia = _image_in(w_images), _ids_in(ids)
     _fits(wi, experts, DType.MXFP4, N, K, "w_images")
     if ia.size != rows * top:
         raise HomuraError(HM_ERR_INVALID, "ids are top times the rows")
@@ -955,7 +965,7 @@ def expert_sum(rows, ids, weights, top: int, experts: int, width: Optional[int] 
         return None
     ra, rows_dtype = _rows_in(rows)
     tokens, width = ra.shape[0] // top, ra.shape[1]
-    ia, w = np.ascontiguousarray(ids, dtype=np.int32), np.ascontiguousarray(weights, dtype=np.float32)
+    ia, w = _ids_in(ids), np.ascontiguousarray(weights, dtype=np.float32)
     r = None if resid is None else np.ascontiguousarray(resid, dtype=np.float32)
     if ia.size != ra.shape[0] or w.size != ia.size or ia.size != tokens * top or (r is not None and r.shape != (tokens, width)):
         raise HomuraError(HM_ERR_INVALID, "ids, weights and resid do not match the rows")

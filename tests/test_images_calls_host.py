@@ -105,3 +105,31 @@ def test_a_width_that_is_not_the_rows(hm):
     let_through(hm, lambda: hm.image_pack(x, hm.DType.MXFP4, K=64))
     let_through(hm, lambda: hm.image_pack(x, hm.DType.MXFP4, K=32, glu=True))
     let_through(hm, lambda: hm.gemv_mx4(x, w[: hm.image_bytes(MX, N, 32)], N, K=64))
+
+
+def test_ids_beyond_32_bits_are_nobodys(hm, monkeypatch):
+    """An id that is no expert's stays one: 2^32 + 1 is not expert 1.  A stand-in for the library keeps the ids it is given."""
+    import ctypes as C
+
+    real, seen = hm.load_library(), {}
+
+    class Library:
+        def __getattr__(self, at):
+            if not at.startswith("hm_expert_") or at.startswith("hm_expert_plan_"):
+                return getattr(real, at)
+
+            def call(*args):
+                where = {"hm_expert_plan": 0, "hm_expert_gemv": 4, "hm_expert_sum": 2}[at]
+                seen[at] = np.ctypeslib.as_array(C.cast(args[where], C.POINTER(C.c_int32)), (PAIRS,)).tolist()
+                return 0
+
+            return call
+
+    monkeypatch.setattr(hm, "load_library", Library)
+    weights = np.zeros(E * hm.image_bytes(MX, N, K), np.uint8)
+    for ids, want in [(np.array([0, 2**32 + 1, -(2**32), 3, 2**31, 7]), [0, -1, -1, 3, -1, 7]), (np.array([1, 2**63, 2**32, 0, 2, 3], np.uint64), [1, -1, -1, 0, 2, 3]), ([[0, 1], [2, 3], [-1, 2**40]], [0, 1, 2, 3, -1, -1]),
+                      (np.array([0, 1, -1, -(2**31), 2**31 - 1, 2], np.int32), [0, 1, -1, -(2**31), 2**31 - 1, 2])]:
+        hm.expert_plan(ids, E)
+        hm.expert_gemv(np.zeros((T, K), np.float32), weights, ids, N, TOP, E)
+        hm.expert_sum(np.zeros((PAIRS, N), np.float32), ids, np.zeros((T, TOP), np.float32), TOP, E)
+        assert seen == {"hm_expert_plan": want, "hm_expert_gemv": want, "hm_expert_sum": want}
