@@ -1430,6 +1430,9 @@ int hm_expert_sum(const void* rows, int rows_dtype, const int32_t* ids, const fl
     if (!rows || !ids || !weights || !y || tokens < 0 || top < 1 || W < 1 || (long long)tokens * top > (1 << 28) || experts < 1) return gfail(HM_ERR_INVALID, "hm_expert_sum: bad arguments");
     if (!is_row_dtype(rows_dtype) || !is_row_dtype(y_dtype)) return gfail(HM_ERR_UNSUPPORTED, "hm_expert_sum: rows and y are HM_F32 or HM_BF16");
     if (misaligned(rows, row_bytes(rows_dtype)) || misaligned(ids, 4) || misaligned(weights, 4) || misaligned(resid, 4) || misaligned(y, row_bytes(y_dtype))) return gfail(HM_ERR_INVALID, "hm_expert_sum: misaligned pointer");
+    // bf16 rows over f32 ones: results of a token would land in residuals that other tokens still read
+    const uintptr_t r0 = (uintptr_t)resid, y0 = (uintptr_t)y, values = (uintptr_t)tokens * W;
+    if (resid && y_dtype == HM_BF16 && y0 < r0 + values * 4 && r0 < y0 + values * 2) return gfail(HM_ERR_INVALID, "hm_expert_sum: a bf16 y overlaps the f32 resid");
     if (tokens == 0) return HM_OK;
     NEED_DEVICE();
     cudaStream_t st = (cudaStream_t)stream;

@@ -1,0 +1,33 @@
+"""Calls of the image entry points that cannot be answered, refused on the host before a device is asked."""
+import ctypes as C
+
+import numpy as np
+import pytest
+
+F32, BF16, MX = 0, 1, 10
+
+
+@pytest.fixture
+def memory():
+    raw = np.zeros((1 << 16) + 16, np.uint8)
+    return raw[-raw.ctypes.data % 16 :]
+
+
+def at(memory, offset=0):
+    return C.c_void_p(memory.ctypes.data + offset)
+
+
+def test_bf16_sums_over_the_residual(hm, memory):
+    """A bf16 row takes half the room of its f32 residual: written over it, a token's results would land in residuals that other tokens still read."""
+    lib = hm.load_library()
+    T, W, p = 4, 8, at(memory)
+    rows, ids, weights = at(memory, 4096), at(memory, 8192), at(memory, 12288)
+    call = lambda resid, y, dtype: lib.hm_expert_sum(rows, F32, ids, weights, T, 1, 4, W, resid, y, dtype, None)
+    for y in [p, at(memory, 4 * W * T - 2), at(memory, 64)]:
+        assert call(p, y, BF16) == hm.HM_ERR_INVALID
+    assert call(at(memory, 2 * W * T - 4), p, BF16) == hm.HM_ERR_INVALID
+    if not hm.device_count():
+        assert call(p, p, F32) == hm.HM_ERR_CUDA  # y may be resid
+        assert call(p, at(memory, 4 * W * T), BF16) == hm.HM_ERR_CUDA
+        assert call(at(memory, 2 * W * T), p, BF16) == hm.HM_ERR_CUDA
+        assert call(None, p, BF16) == hm.HM_ERR_CUDA
