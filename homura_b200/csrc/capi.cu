@@ -218,6 +218,8 @@ bool misaligned(const void* p, size_t n) { return ((uintptr_t)p & (n - 1)) != 0;
 bool is_image_dtype(int d) { return d == HM_MXFP4 || d == HM_BF16; }
 bool is_row_dtype(int d) { return d == HM_F32 || d == HM_BF16; }
 size_t row_bytes(int dtype) { return dtype == HM_BF16 ? 2 : 4; }
+// Rows of `width` elements, ld apart, cannot be: they overlap, or their bytes do not fit 64 bits.
+bool bad_rows(int rows, size_t width, size_t ld) { return ld < width || ld > ((size_t)1 << 60) / std::max(rows, 1); }
 // Bytes of rows of `width` elements, ld apart.
 size_t span_bytes(int rows, int width, size_t ld, int dtype) { return rows < 1 ? 0 : ((size_t)(rows - 1) * ld + width) * row_bytes(dtype); }
 
@@ -1210,7 +1212,7 @@ size_t hm_image_bytes(int dtype, int rows, int K) { return rows < 1 || rows > MA
 
 int hm_image_pack(const void* x, int x_dtype, int rows, int K, size_t ldx, int glu, int dtype, void* image, void* stream) {
     const int width = glu ? 2 : 1;
-    if (!x || !image || rows < 0 || rows > MAX_ROWS || K < 1 || K > MAX_K || ldx < (size_t)K * width) return gfail(HM_ERR_INVALID, "hm_image_pack: bad arguments (ldx >= K, 2 K with glu)");
+    if (!x || !image || rows < 0 || rows > MAX_ROWS || K < 1 || K > MAX_K || bad_rows(rows, (size_t)K * width, ldx)) return gfail(HM_ERR_INVALID, "hm_image_pack: bad arguments (ldx >= K, 2 K with glu)");
     if (!is_row_dtype(x_dtype) || !is_image_dtype(dtype)) return gfail(HM_ERR_UNSUPPORTED, "hm_image_pack: rows are HM_F32 or HM_BF16, images HM_MXFP4 or HM_BF16");
     if (misaligned(x, row_bytes(x_dtype)) || misaligned(image, 16)) return gfail(HM_ERR_INVALID, "hm_image_pack: misaligned pointer (images start on 16-byte boundaries)");
     if (rows == 0) return HM_OK;
@@ -1232,7 +1234,7 @@ int hm_image_pack(const void* x, int x_dtype, int rows, int K, size_t ldx, int g
 }
 
 int hm_image_unpack(const void* image, int dtype, int rows, int K, void* out, int out_dtype, size_t ldo, void* stream) {
-    if (!image || !out || rows < 0 || rows > MAX_ROWS || K < 1 || K > MAX_K || ldo < (size_t)K) return gfail(HM_ERR_INVALID, "hm_image_unpack: bad arguments (ldo >= K)");
+    if (!image || !out || rows < 0 || rows > MAX_ROWS || K < 1 || K > MAX_K || bad_rows(rows, K, ldo)) return gfail(HM_ERR_INVALID, "hm_image_unpack: bad arguments (ldo >= K)");
     if (!is_row_dtype(out_dtype) || !is_image_dtype(dtype)) return gfail(HM_ERR_UNSUPPORTED, "hm_image_unpack: rows are HM_F32 or HM_BF16, images HM_MXFP4 or HM_BF16");
     if (misaligned(out, row_bytes(out_dtype)) || misaligned(image, 16)) return gfail(HM_ERR_INVALID, "hm_image_unpack: misaligned pointer (images start on 16-byte boundaries)");
     if (rows == 0) return HM_OK;
@@ -1295,7 +1297,7 @@ int hm_gemm_image(const void* x_image, const void* w_image, int dtype, int M, in
 }
 
 int hm_gemv_mx4(const void* x, int x_dtype, size_t ldx, const void* w_image, int M, int K, int N, void* y, int y_dtype, size_t ldy, void* stream) {
-    if (!x || !w_image || !y || M < 0 || M > 8 || K < 1 || N < 1 || N > MAX_ROWS || ldx < (size_t)K || ldy < (size_t)N) return gfail(HM_ERR_INVALID, "hm_gemv_mx4: bad arguments (M <= 8, ldx >= K, ldy >= N)");
+    if (!x || !w_image || !y || M < 0 || M > 8 || K < 1 || N < 1 || N > MAX_ROWS || bad_rows(M, K, ldx) || bad_rows(M, N, ldy)) return gfail(HM_ERR_INVALID, "hm_gemv_mx4: bad arguments (M <= 8, ldx >= K, ldy >= N)");
     if (!is_row_dtype(x_dtype) || !is_row_dtype(y_dtype) || K > MX_GEMV_K) return gfail(HM_ERR_UNSUPPORTED, "hm_gemv_mx4: x and y are HM_F32 or HM_BF16, K at most 32768");
     if (misaligned(x, row_bytes(x_dtype)) || misaligned(w_image, 16) || misaligned(y, row_bytes(y_dtype))) return gfail(HM_ERR_INVALID, "hm_gemv_mx4: misaligned pointer (images start on 16-byte boundaries)");
     if (M == 0) return HM_OK;
@@ -1338,7 +1340,7 @@ int hm_expert_plan(const int32_t* ids, int pairs, int experts, int32_t* plan, vo
 
 int hm_expert_pack(const void* x, int x_dtype, int K, size_t ldx, int glu, const int32_t* plan, int pairs, int experts, int top, int dtype, void* image, void* stream) {
     const int width = glu ? 2 : 1;
-    if (!x || !plan || !image || K < 1 || K > MAX_K || ldx < (size_t)K * width || bad_groups(pairs, experts) || top < 1 || pairs % top != 0)
+    if (!x || !plan || !image || K < 1 || K > MAX_K || bad_groups(pairs, experts) || top < 1 || pairs % top != 0 || bad_rows(pairs / top, (size_t)K * width, ldx))
         return gfail(HM_ERR_INVALID, "hm_expert_pack: bad arguments (ldx >= K, 2 K with glu; pairs a multiple of top; experts <= 1024)");
     if (!is_row_dtype(x_dtype) || !is_image_dtype(dtype)) return gfail(HM_ERR_UNSUPPORTED, "hm_expert_pack: rows are HM_F32 or HM_BF16, images HM_MXFP4 or HM_BF16");
     if (misaligned(x, row_bytes(x_dtype)) || misaligned(plan, 4) || misaligned(image, 16)) return gfail(HM_ERR_INVALID, "hm_expert_pack: misaligned pointer (images start on 16-byte boundaries)");
@@ -1396,7 +1398,7 @@ int hm_expert_gemm(const void* x_image, const void* w_images, int dtype, const i
 }
 
 int hm_expert_gemv(const void* x, int x_dtype, size_t ldx, const void* w_images, const int32_t* ids, int pairs, int top, int experts, int K, int N, void* y, int y_dtype, size_t ldy, void* stream) {
-    if (!x || !w_images || !ids || !y || bad_groups(pairs, experts) || pairs > 65535 || top < 1 || pairs % top != 0 || K < 1 || N < 1 || N > MAX_ROWS || ldx < (size_t)K || ldy < (size_t)N)
+    if (!x || !w_images || !ids || !y || bad_groups(pairs, experts) || pairs > 65535 || top < 1 || pairs % top != 0 || K < 1 || N < 1 || N > MAX_ROWS || bad_rows(pairs / top, K, ldx) || bad_rows(pairs, N, ldy))
         return gfail(HM_ERR_INVALID, "hm_expert_gemv: bad arguments (pairs <= 65535 and a multiple of top, ldx >= K, ldy >= N, experts <= 1024)");
     if (!is_row_dtype(x_dtype) || !is_row_dtype(y_dtype) || K > MX_GEMV_K) return gfail(HM_ERR_UNSUPPORTED, "hm_expert_gemv: x and y are HM_F32 or HM_BF16, K at most 32768");
     if (misaligned(x, row_bytes(x_dtype)) || misaligned(w_images, 16) || misaligned(ids, 4) || misaligned(y, row_bytes(y_dtype))) return gfail(HM_ERR_INVALID, "hm_expert_gemv: misaligned pointer (images start on 16-byte boundaries)");

@@ -31,3 +31,18 @@ def test_bf16_sums_over_the_residual(hm, memory):
         assert call(p, at(memory, 4 * W * T), BF16) == hm.HM_ERR_CUDA
         assert call(at(memory, 2 * W * T), p, BF16) == hm.HM_ERR_CUDA
         assert call(None, p, BF16) == hm.HM_ERR_CUDA
+
+
+def test_rows_too_far_apart_to_count(hm, memory):
+    """Rows so far apart that their bytes do not fit 64 bits: the room of host rows was the remainder."""
+    lib, INV, p = hm.load_library(), hm.HM_ERR_INVALID, at(memory)
+    for ld in [2**64 - 64, 2**62, 2**60]:
+        assert lib.hm_image_pack(p, F32, 5, 32, ld, 0, MX, p, None) == INV
+        assert lib.hm_image_unpack(p, MX, 5, 32, p, F32, ld, None) == INV
+        assert lib.hm_gemv_mx4(p, F32, ld, p, 5, 32, 8, p, F32, 8, None) == INV
+        assert lib.hm_gemv_mx4(p, F32, 32, p, 5, 32, 8, p, F32, ld, None) == INV
+        assert lib.hm_expert_pack(p, F32, 32, ld, 0, p, 4, 4, 2, MX, p, None) == INV
+        assert lib.hm_expert_gemv(p, F32, ld, p, p, 4, 1, 4, 32, 8, p, F32, 8, None) == INV
+        assert lib.hm_expert_gemv(p, F32, 32, p, p, 4, 1, 4, 32, 8, p, F32, ld, None) == INV
+    if not hm.device_count():
+        assert lib.hm_image_pack(p, F32, 1, 32, 2**40, 0, MX, p, None) == hm.HM_ERR_CUDA
