@@ -1429,7 +1429,7 @@ int hm_expert_gemv(const void* x, int x_dtype, size_t ldx, const void* w_images,
 }
 
 int hm_expert_sum(const void* rows, int rows_dtype, const int32_t* ids, const float* weights, int tokens, int top, int experts, int W, const float* resid, void* y, int y_dtype, void* stream) {
-    if (!rows || !ids || !weights || !y || tokens < 0 || top < 1 || W < 1 || (long long)tokens * top > (1 << 28) || experts < 1) return gfail(HM_ERR_INVALID, "hm_expert_sum: bad arguments");
+    if (!rows || !ids || !weights || !y || tokens < 0 || top < 1 || W < 1 || W > MAX_ROWS || (long long)tokens * top > (1 << 28) || experts < 1) return gfail(HM_ERR_INVALID, "hm_expert_sum: bad arguments");
     if (!is_row_dtype(rows_dtype) || !is_row_dtype(y_dtype)) return gfail(HM_ERR_UNSUPPORTED, "hm_expert_sum: rows and y are HM_F32 or HM_BF16");
     if (misaligned(rows, row_bytes(rows_dtype)) || misaligned(ids, 4) || misaligned(weights, 4) || misaligned(resid, 4) || misaligned(y, row_bytes(y_dtype))) return gfail(HM_ERR_INVALID, "hm_expert_sum: misaligned pointer");
     // bf16 rows over f32 ones: results of a token would land in residuals that other tokens still read

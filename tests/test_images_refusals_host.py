@@ -46,3 +46,12 @@ def test_rows_too_far_apart_to_count(hm, memory):
         assert lib.hm_expert_gemv(p, F32, 32, p, p, 4, 1, 4, 32, 8, p, F32, ld, None) == INV
     if not hm.device_count():
         assert lib.hm_image_pack(p, F32, 1, 32, 2**40, 0, MX, p, None) == hm.HM_ERR_CUDA
+
+
+def test_sums_of_rows_as_wide_as_int_goes(hm, memory):
+    """The number of blocks over a row of nearly 2^31 values was counted in an int that does not hold it."""
+    lib, p = hm.load_library(), at(memory)
+    for W in [2**31 - 1, 2**31 - 255]:
+        assert lib.hm_expert_sum(p, F32, p, p, 1, 1, 4, W, None, p, F32, None) == hm.HM_ERR_INVALID
+    if not hm.device_count():
+        assert lib.hm_expert_sum(p, F32, p, p, 1, 1, 4, 2**31 - 256, None, p, F32, None) == hm.HM_ERR_CUDA
