@@ -88,12 +88,12 @@ __global__ void __launch_bounds__(THREADS, 2) mx4_gemv_kernel(const MxGemvArgs a
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
     __syncthreads();
-    uint32_t issued = 0;
     if (warp == MMA_WARPS) {
         asm volatile("bar.sync 2, 288;" ::: "memory");  // x is asked for first: behind the ring's tiles it would arrive after them
         if (lane == 0) {
             const unsigned char* w = a.w + expert * a.w_stride;
             bool ok = true;
+            uint32_t issued = 0;
             int s = -1;
             uint32_t parity = 1;  // of the slot's use before
             for (int t = blockIdx.x / a.split; t < a.tiles && ok; t += step)
@@ -104,6 +104,7 @@ __global__ void __launch_bounds__(THREADS, 2) mx4_gemv_kernel(const MxGemvArgs a
                     mb_expect_tx(&sh.full[s], MX_TILE);
                     bulk_copy(ring + (size_t)s * MX_TILE, w + ((size_t)t * a.kblocks + kb) * MX_TILE, MX_TILE, &sh.full[s]);
                 }
+            mb_land_ring(sh.full, issued, (uint32_t)a.slots);  // always: a wait of the others may run out after this thread's last look at the flag
         }
     } else {
         // A warp takes a row of x: its largest finite value, then f16 terms.  Up to XU k-blocks (eight values of each per lane) are loaded once.
@@ -296,7 +297,6 @@ __global__ void __launch_bounds__(THREADS, 2) mx4_gemv_kernel(const MxGemvArgs a
             break;
         }
     }
-    if (warp == MMA_WARPS && lane == 0 && sh.abort_flag) mb_land_ring(sh.full, issued, (uint32_t)a.slots);
 }
 
 template <int NB, int TERMS>
