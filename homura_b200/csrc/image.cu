@@ -19,7 +19,12 @@ constexpr int THREADS = 256, WARPS = THREADS / 32;
 
 __device__ __forceinline__ float load1(const void* x, int bf16, size_t i) { return bf16 ? bf16_bits_to_f32(__ldg(static_cast<const uint16_t*>(x) + i)) : __ldg(static_cast<const float*>(x) + i); }
 
-__device__ __forceinline__ float gated(float g, float u) { return __fdividef(g, 1.0f + expf(-g)) * u; }  // the quotient to 2 ulp
+// silu(g) u from e^-|g|: gates below -87 keep what a large u makes of them, and the divisor is from 1 to 2, where the fast quotient is good to 2 ulp (the full one:
+// 11.7 us for 4136 x 1120 f32 pairs, 4-bit).
+__device__ __forceinline__ float gated(float g, float u) {
+    const float t = expf(-fabsf(g));
+    return __fdividef(g < 0.f ? g * t : g, 1.0f + t) * u;
+}
 
 // Eight codes of a lane, and the scales of its four blocks (the same in sixteen lanes).  Block of 32 values over four lanes (eight each): e = floor(log2 max) - 2, at least -127, as byte e + 127; codes x 2^-e to nearest even, saturated at 6.
 // The largest exponent field is 255 where a value is infinite or no number: the whole block is then no number.
