@@ -2,16 +2,18 @@
 //
 // Bound by the weights' 17/32 bytes each, if a weight costs few enough instructions: the codes go to f16 by conversion (exactly) and are multiplied
 // on mma.sync m16n8k16, whose eight columns are the rows of x; a block of 32 values is two MMAs into accumulators of their own, which the block's
-// scale then joins to the sum in f32.  x enters as f16: 2^s x with its largest value in [2^7, 2^8), as one term (bf16) or as a sum of two (f32: 2^-22 of a value
-// and 2^-32 of the row's largest), so that a launch of up to eight bf16 or four f32 rows has one MMA column block, eight f32 rows have two.
+// scale then joins to the sum in f32.  x enters as f16: 2^e x with the row's largest value in [2^14, 2^15), so that a channel that stands out leaves the others their
+// bits.  bf16 is one term: exact down to 2^-31 of the row's largest, then to 2^-39 of it (half a subnormal step).  f32 is two, the second 2^12 times what the first
+// leaves: 2^-22 of a value, 2^-51 of the row's largest.  So a launch of up to eight bf16 or four f32 rows has one MMA column block, eight f32 rows have two.
 //
 //   * a CTA = 128 features (a tile of the image) x its k-blocks; a producer warp copies tiles of 17 KB into a ring, eight warps multiply: four groups of 32
 //     features, two halves of a k-block.  The k order of an MMA is free as long as both operands agree: lane t of a group of four takes values
 //     8 t .. 8 t + 7 of a block, one word of codes.
 //   * tiles that are fewer than the SMs share their k-blocks among the CTAs of a cluster, summed in rank order through distributed shared memory; otherwise
 //     a CTA walks several tiles and converts x once.
-// Measured (graph replays): one f32 row 896 -> 9728 5.2 us (4.6 MB: launch, x and two cluster barriers), seven bf16 rows 1536 -> 151936 29.3 us (128 MB, 0.67 of the
-// measured copy bandwidth): 6.0 TB/s while tiles flow, at 60 % of the issue slots, behind 5 us of launch and x; 1187 tiles leave three CTAs a fifth one.
+// Measured (graph replays): one f32 row 896 -> 9728 5.4 us (4.6 MB: launch, x and two cluster barriers), seven bf16 rows 1536 -> 151936 29.4 us (128 MB, 0.66 of the
+// measured copy bandwidth): 6.0 TB/s while tiles flow, at 60 % of the issue slots, behind 5 us of launch and x; 1187 tiles leave three CTAs a fifth one.  Eight f32 rows
+// of the same size 46.2 us: twice the MMAs, one CTA per SM.
 #include <algorithm>
 
 #include "image.h"
@@ -42,10 +44,14 @@ __device__ __forceinline__ uint4 load_now(const void* p) {
     asm volatile("ld.global.nc.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "l"(p) : "memory");
     return v;
 }
-// 2^(byte j of w - 127); 255 counts as infinite here.
+constexpr int X_TOP = 14;          // a row's largest value is brought into [2^X_TOP, 2^(X_TOP + 1))
+constexpr int SUM_DOWN = 7;        // block sums join the f32 sum 2^-SUM_DOWN times: scales up to 2^100 then stay below its largest value
+constexpr float LOW_UP = 4096.f;   // what the first term of an f32 leaves enters that many times
+
+// 2^(byte j of w - 127 - SUM_DOWN); 255 counts as infinite here.
 __device__ __forceinline__ float scale_of(uint32_t w, int j) {
     const uint32_t s = (j == 3 ? w >> 1 : w << (23 - 8 * j)) & 0x7F800000u;
-    return __uint_as_float(max(s, 0x00400000u));
+    return __uint_as_float(max(s, 0x00400000u)) * (1.f / (1 << SUM_DOWN));
 }
 __device__ __forceinline__ uint32_t f16x2_rn(float lo, float hi) {
     uint32_t r;
@@ -53,9 +59,10 @@ __device__ __forceinline__ uint32_t f16x2_rn(float lo, float hi) {
     return r;
 }
 
-// 2^e brings a row's largest value into [2^7, 2^8).
-__device__ __forceinline__ int row_exponent(uint32_t top) { return min(max(134 - (int)(top >> 23), -126), 126); }
-__device__ __forceinline__ float row_factor(uint32_t top) { return __uint_as_float((uint32_t)(127 - row_exponent(top)) << 23); }
+// 2^e brings a row's largest value to its place (rows below 2^-112: as far as a factor of 2^126 goes); the sums are 2^back times the row's.
+__device__ __forceinline__ int row_exponent(uint32_t top) { return min(127 + X_TOP - (int)(top >> 23), 126); }
+__device__ __forceinline__ int row_back(uint32_t top) { return SUM_DOWN - row_exponent(top); }
+__device__ __forceinline__ float row_factor(uint32_t top) { return __uint_as_float((uint32_t)(127 + row_back(top)) << 23); }
 
 // Elements of a column of x in shared memory: the k-blocks of a CTA and half a line, so that neighbouring columns lie in different banks.
 __host__ __device__ inline int x_ld(int kb_per) { return kb_per * MX_K + 32; }
@@ -168,7 +175,7 @@ __global__ void __launch_bounds__(THREADS, 2) mx4_gemv_kernel(const MxGemvArgs a
                         h[e] = f16x2_rn(p, q);
                         if (TERMS == 2) {  // what the first term leaves; nothing of an infinity
                             const float rp = p - f16_bits_to_f32((uint16_t)h[e]), rq = q - f16_bits_to_f32((uint16_t)(h[e] >> 16));
-                            l[e] = f16x2_rn(fabsf(p) < __int_as_float(0x7F800000) ? rp : 0.f, fabsf(q) < __int_as_float(0x7F800000) ? rq : 0.f);
+                            l[e] = f16x2_rn(fabsf(p) < __int_as_float(0x7F800000) ? rp * LOW_UP : 0.f, fabsf(q) < __int_as_float(0x7F800000) ? rq * LOW_UP : 0.f);
                         }
                     }
                     *reinterpret_cast<uint4*>(to + (b0 + u) * MX_K) = make_uint4(h[0], h[1], h[2], h[3]);
@@ -245,10 +252,10 @@ __global__ void __launch_bounds__(THREADS, 2) mx4_gemv_kernel(const MxGemvArgs a
                 for (int h = 0; h < 2; ++h) {
                     float* q = p + (fg * 32 + i * 16 + h * 8 + g) * PART_LD;
                     if (NB == 2) {
-                        q[2 * tl] = sum[i][0][2 * h] + sum[i][NB - 1][2 * h];
-                        q[2 * tl + 1] = sum[i][0][2 * h + 1] + sum[i][NB - 1][2 * h + 1];
+                        q[2 * tl] = fmaf(sum[i][NB - 1][2 * h], 1.f / LOW_UP, sum[i][0][2 * h]);
+                        q[2 * tl + 1] = fmaf(sum[i][NB - 1][2 * h + 1], 1.f / LOW_UP, sum[i][0][2 * h + 1]);
                     } else if (TERMS == 2) {
-                        q[tl] = sum[i][0][2 * h] + sum[i][0][2 * h + 1];
+                        q[tl] = fmaf(sum[i][0][2 * h + 1], 1.f / LOW_UP, sum[i][0][2 * h]);
                     } else {
                         q[2 * tl] = sum[i][0][2 * h];
                         q[2 * tl + 1] = sum[i][0][2 * h + 1];
@@ -287,7 +294,7 @@ __global__ void __launch_bounds__(THREADS, 2) mx4_gemv_kernel(const MxGemvArgs a
                     double v = 0.0;
 #pragma unroll
                     for (int r = 0; r < MAX_SPLIT; ++r)
-                        if (r < a.split) v += (double)q[r] * __hiloint2double((1023 - row_exponent(top[r])) << 20, 0);
+                        if (r < a.split) v += (double)q[r] * __hiloint2double((1023 + row_back(top[r])) << 20, 0);
                     store(m, (float)v);
                 }
             }

@@ -350,8 +350,10 @@ HM_API int hm_image_unpack(const void* image, int dtype, int rows, int K, void* 
 HM_API int hm_image_from_blocks(const void* blocks, int rows, int K, void* image, void* stream);
 /* y [M, N] = x @ W^T from two images of the same dtype; f32 sums; y HM_F32 or HM_BF16 (rounded once). */
 HM_API int hm_gemm_image(const void* x_image, const void* w_image, int dtype, int M, int K, int N, void* y, int y_dtype, size_t ldy, void* stream);
-/* The same for 1 <= M <= 8 rows x that stay as they are (HM_F32 to 2^-22 of a value and 2^-32 of its row's largest, HM_BF16) and an HM_MXFP4
- * image of weights whose scales are below 2^100 (a row's own scale is taken back at the end); K <= 32768. */
+/* The same for 1 <= M <= 8 rows x that are not rounded to 4 bits, and an HM_MXFP4 image of weights.  A value of x enters to
+ *   HM_F32   2^-22 of itself and 2^-51 of its row's largest value
+ *   HM_BF16  exactly where it is at least 2^-31 of its row's largest value, else to 2^-39 of that
+ * (rows whose largest value is below 2^-112: to 2^-163 and 2^-151).  The weights' scales are below 2^100 (a row's own scale is taken back at the end); K <= 32768. */
 HM_API int hm_gemv_mx4(const void* x, int x_dtype, size_t ldx, const void* w_image, int M, int K, int N, void* y, int y_dtype, size_t ldy, void* stream);
 /* Products grouped by expert.  A pair is a (token, choice) with the expert ids[pair]; ids outside [0, experts) (-1 of hm_post_norm_route) have none.
  * The images of the experts' weights stand back to back, hm_image_bytes(dtype, N, K) each.  experts <= 1024.
