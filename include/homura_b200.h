@@ -370,7 +370,7 @@ HM_API int hm_expert_gemm(const void* x_image, const void* w_images, int dtype, 
 /* The same without a plan for few pairs: x [pairs / top, K] as it is (see hm_gemv_mx4), HM_MXFP4 images; pairs <= 65535. */
 HM_API int hm_expert_gemv(const void* x, int x_dtype, size_t ldx, const void* w_images, const int32_t* ids, int pairs, int top, int experts, int K, int N, void* y, int y_dtype, size_t ldy, void* stream);
 /* y [tokens, W] = resid (f32, or NULL) + sum over the choices j with an expert of weights[t, j] * rows[t * top + j] (HM_F32 or HM_BF16), in their order; an f32 y may be
- * resid, a bf16 y and resid do not overlap. */
+ * resid, a bf16 y and resid do not overlap.  Identity experts (ids -1) have no part here: theirs is id_weight of hm_post_norm_route, which its next call takes. */
 HM_API int hm_expert_sum(const void* rows, int rows_dtype, const int32_t* ids, const float* weights, int tokens, int top, int experts, int W, const float* resid, void* y, int y_dtype, void* stream);
 
 /* argmax with ties to the highest index (src/generate.rs:457-468): logits [rows, n]. */

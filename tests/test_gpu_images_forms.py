@@ -1,5 +1,5 @@
 """Forms of the image calls at sizes where a CTA or a warp has several pieces of work: products of many units, packs of three k-blocks per warp, gated rows of either type,
-pairs with bf16 rows and results, and sums of more tokens than a grid's second dimension.
+pairs with bf16 rows and results, sums of more tokens than a grid's second dimension, and a mixture with identity experts.
 
 Images are compared bit for bit with the format restated over all rows at once; products with 64-bit results, to the tolerances derived in test_gpu_images.py."""
 import numpy as np
@@ -259,3 +259,40 @@ def test_sums_of_more_tokens_than_a_grid_has_rows(hm, W, rows_t, out):
     want, size = terms.sum(1) + x.double(), terms.abs().sum(1) + x.double().abs()
     # two products and three sums, 2^-24 each
     close(y.cpu().numpy() if out == F32 else y.view(torch.int16).cpu().numpy().view(np.uint16), want.cpu().numpy(), size.cpu().numpy(), 3, "weighted sum of many tokens")
+
+
+@pytest.mark.parametrize("dtype", [MX, BF16])
+@pytest.mark.parametrize("tokens", [3, 150])
+def test_a_mixture_with_identity_experts(hm, dtype, tokens):
+    """Two layers' ends: the sum of the chosen experts without a residual, the identity experts' share and the norm from hm_post_norm_route.
+
+    x + mult * n(z) * w with z = y + share * x, n(z) = z / sqrt(mean(z^2) + eps), from the rows as they came out.  In f32, with u = 2^-24: z is off by at most
+    e = 6 u (sum of magnitudes); the mean of W squares by W u of itself, what z's error makes of it aside, the root by half of that; a few more roundings of the
+    factor and the products: |error| <= |mult w| (e / r + |z| / r (W u / 2 + |e| / |z| over the row + 8 u)) + 2 u |result|."""
+    rng = np.random.default_rng(tokens + dtype)
+    W, ff, experts, identities, top = 320, 96, 6, 3, 3
+    d, name = hm.DType(dtype), NAMES[dtype]
+    f = lambda *n: rng.standard_normal(n).astype(np.float32)
+    router = ic.bf16_bits(f(experts + identities, W) * 0.1)
+    x, ids, wts, share = hm.post_norm_route(f(tokens, W), f(tokens, W), np.ones(W, np.float32), 0.25, 1e-6, router=router, correction=np.zeros(experts + identities, np.float32), experts=experts, top=top)
+    assert (ids < 0).any() and (share > 0).any() and (ids >= 0).any()
+    pairs = tokens * top
+    image = lambda w: np.concatenate([hm.image_pack(w[e], d) for e in range(experts)])
+    plan = hm.expert_plan(ids, experts)
+    h = hm.expert_gemm(hm.image_pack(x, d, plan=plan, experts=experts, top=top), image(f(experts, 2 * ff, W) * 0.05), plan, 2 * ff, d, pairs, experts, W)
+    rows = hm.expert_gemm(hm.image_pack(h, d, plan=plan, experts=experts, glu=True), image(f(experts, W, ff) * 0.05), plan, W, d, pairs, experts, ff)
+    y = hm.expert_sum(rows, ids, wts, top, experts)
+    nw, mult, eps = (1 + 0.1 * f(W)).astype(np.float32), 0.5, 1e-6
+    got = hm.post_norm_route(y, x, nw, mult, eps, identity=share).astype(np.float64)
+    terms = np.where(ids[..., None] >= 0, wts[..., None].astype(np.float64) * rows.reshape(tokens, top, W), 0.0)
+    own = share[:, None].astype(np.float64) * x
+    z, u = terms.sum(1) + own, 2.0**-24
+    r = np.sqrt((z**2).mean(1, keepdims=True) + eps)
+    want = x + mult * z / r * nw
+    e = 6 * u * (np.abs(terms).sum(1) + np.abs(own))
+    norm = lambda a: np.sqrt((a**2).sum(1, keepdims=True))
+    limit = np.abs(mult * nw) * (e / r + np.abs(z) / r * (W * u / 2 + norm(e) / norm(z) + 8 * u)) + 2 * u * np.abs(want)
+    assert (np.abs(got - want) <= limit).all(), float((np.abs(got - want) / limit).max())
+    # the share of the identity experts is no rounding: without it the result is another
+    without = x + mult * terms.sum(1) / np.sqrt((terms.sum(1) ** 2).mean(1, keepdims=True) + eps) * nw
+    assert (np.abs(without - want) > limit).any(1).sum() >= (share > 0).sum() * 0.9
