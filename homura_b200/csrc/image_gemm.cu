@@ -12,7 +12,8 @@
 //     ranks through distributed shared memory: no scratch outlives the launch.
 // Measured (graph replays): 1999 x 17920 x 1536 4-bit to bf16 32 us = 3.4 PFLOP/s, 2.1 times the measured bf16 rate; the GPU is at its power limit then (990 W,
 // 1.73 GHz).  A k-block takes 402 clocks of MMAs, 584 with its six scale copies, and 96 KB of shared-memory traffic with the staged results: copies in, operands
-// out and results fill two thirds of that pipe.  64 rows x 8960 -> 1536 in clusters of seven 6.9 us; 32 experts x 16 rows, 58 MB of weights, 11 us.
+// out and results fill two thirds of that pipe.  64 rows x 8960 -> 1536 in clusters of seven 6.9 us; 32 experts x 16 rows, 60 MB of weights, 11.8 us from the L2, 15.7 from
+// memory.
 // Taken back: pairs of CTAs (cta_group::2, half the rows loaded per CTA; 34.5 us: five slots do not cover the way from CTA to CTA, six leave too little
 // shared memory for the results, 40 us), scales written to the
 // tensor memory by four more warps instead of copied (38 us), waits by one lane of a warp (34 us), groups cut into units of equal sizes (within 5 % either way).
