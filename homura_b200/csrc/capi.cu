@@ -162,6 +162,25 @@ cudaError_t get_scratch(size_t partial_floats, size_t ntickets, float** partial,
     return cudaSuccess;
 }
 
+// A zeroed word of device memory, also while a stream of this or another thread is being captured: the calls are allowed in relaxed mode, and the word is
+// zeroed on a stream of its own, since the default stream would join the capture.
+cudaError_t alloc_word(int** out) {
+    cudaStreamCaptureMode mode = cudaStreamCaptureModeRelaxed;
+    cudaError_t e = cudaThreadExchangeStreamCaptureMode(&mode);
+    if (e != cudaSuccess) return e;
+    int* word = nullptr;
+    cudaStream_t own = nullptr;
+    e = cudaMalloc(&word, sizeof(int));
+    if (e == cudaSuccess) e = cudaStreamCreateWithFlags(&own, cudaStreamNonBlocking);
+    if (e == cudaSuccess) e = cudaMemsetAsync(word, 0, sizeof(int), own);
+    if (e == cudaSuccess) e = cudaStreamSynchronize(own);
+    if (own) cudaStreamDestroy(own);
+    if (e != cudaSuccess && word) cudaFree(word);
+    cudaThreadExchangeStreamCaptureMode(&mode);
+    if (e == cudaSuccess) *out = word;
+    return e;
+}
+
 // Device word that kernels with bounded waits raise; allocated once per device.
 cudaError_t get_wait_err(int** out) {
     int dev = 0;
@@ -169,12 +188,7 @@ cudaError_t get_wait_err(int** out) {
     if (e != cudaSuccess) return e;
     std::lock_guard<std::mutex> lk(g_scratch_mu);
     DeviceScratch& s = g_scratch[dev];
-    if (!s.wait_err) {
-        e = cudaMalloc(&s.wait_err, sizeof(int));
-        if (e != cudaSuccess) return e;
-        e = cudaMemset(s.wait_err, 0, sizeof(int));
-        if (e != cudaSuccess) return e;
-    }
+    if (!s.wait_err && (e = alloc_word(&s.wait_err)) != cudaSuccess) return e;
     *out = s.wait_err;
     return cudaSuccess;
 }
