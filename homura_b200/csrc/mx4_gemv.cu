@@ -4,7 +4,7 @@
 // on mma.sync m16n8k16, whose eight columns are the rows of x; a block of 32 values is two MMAs into accumulators of their own, which the block's
 // scale then joins to the sum in f32.  x enters as f16: 2^e x with the row's largest value in [2^14, 2^15), so that a channel that stands out leaves the others their
 // bits.  bf16 is one term: exact down to 2^-31 of the row's largest, then to 2^-39 of it (half a subnormal step).  f32 is two, the second 2^12 times what the first
-// leaves: 2^-22 of a value, 2^-51 of the row's largest.  So a launch of up to eight bf16 or four f32 rows has one MMA column block, eight f32 rows have two.
+// leaves: 2^-22 of a value, 2^-51 of the row's largest (a third would bring two more bits, which a row's sum in f32 does not keep).  So a launch of up to eight bf16 or four f32 rows has one MMA column block, eight f32 rows have two.
 //
 //   * a CTA = 128 features (a tile of the image) x its k-blocks; a producer warp copies tiles of 17 KB into a ring, eight warps multiply: four groups of 32
 //     features, two halves of a k-block.  The k order of an MMA is free as long as both operands agree: lane t of a group of four takes values
