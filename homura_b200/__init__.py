@@ -100,6 +100,12 @@ class _StepEntry(C.Structure):
 
 _vp, _i32, _u32p, _i32p, _f32p, _i64p = C.c_void_p, C.c_int, C.POINTER(C.c_uint32), C.POINTER(C.c_int32), C.POINTER(C.c_float), C.POINTER(C.c_int64)
 
+class HmKv8(C.Structure):
+    """hm_kv8."""
+
+    _fields_ = [("pages", C.c_void_p), ("page_table", C.c_void_p)] + [(n, C.c_int32) for n in ("n_pages", "n_seq", "max_pages", "kv_heads", "dim", "vdim")]
+
+
 # name -> (restype, argtypes); every symbol include/homura_b200.h declares
 SIGNATURES = {
     "hm_version": (C.c_char_p, []),
@@ -171,6 +177,13 @@ SIGNATURES = {
     "hm_expert_gemm": (_i32, [_vp, _vp, _i32, _vp, _i32, _i32, _i32, _i32, _vp, _i32, C.c_size_t, _vp]),
     "hm_expert_gemv": (_i32, [_vp, _i32, C.c_size_t, _vp, _vp, _i32, _i32, _i32, _i32, _i32, _vp, _i32, C.c_size_t, _vp]),
     "hm_expert_sum": (_i32, [_vp, _i32, _vp, _vp, _i32, _i32, _i32, _i32, _vp, _vp, _i32, _vp]),
+    "hm_rope_turns": (_i32, [C.c_double, _i32, _i32, C.c_double, C.c_double, C.c_double, C.c_double, _vp, C.POINTER(C.c_float)]),
+    "hm_rope": (_i32, [_vp, _i32, C.c_size_t, _i32, _i32, _i32, _i32, _i32, _vp, _vp, C.c_float, _vp, C.c_size_t, _vp]),
+    "hm_kv8_pool_bytes": (C.c_size_t, [_i32, _i32, _i32, _i32]),
+    "hm_kv8_write": (_i32, [C.POINTER(HmKv8), _vp, _vp, _i32, C.c_size_t, C.c_size_t, _vp, _vp, _i32, _vp]),
+    "hm_kv8_read": (_i32, [C.POINTER(HmKv8), _vp, _vp, _i32, _vp, _vp, _i32, C.c_size_t, C.c_size_t, _vp]),
+    "hm_kv8_attn_bytes": (C.c_size_t, [C.POINTER(HmKv8), _i32, _i32, _i32]),
+    "hm_kv8_attn": (_i32, [C.POINTER(HmKv8), _vp, _i32, C.c_size_t, _vp, _vp, _i32, _i32, C.c_float, _vp, _i32, _vp, C.c_size_t, _vp, _vp]),
     "hm_argmax": (_i32, [_vp, _i32, _i32, _vp, _vp]),
     "hm_dev_alloc": (_i32, [C.c_size_t, C.POINTER(_vp)]),
     "hm_dev_free": (_i32, [_vp]),
@@ -1011,6 +1024,117 @@ class DeviceBuffer:
             self.free()
         except Exception:
             pass
+
+
+# ---- rotary positions, and attention over a cache in 8 bits ---------------------------------------------
+#
+# Host mode: numpy arrays in, numpy arrays out; bf16 rows are uint16 bit patterns.  Device mode (asynchronous): the first rows as (addr, rows), the other
+# arguments integer device addresses, sizes and types given; rows may be `ld` elements apart.
+
+ROPE_KINDS = {"plain": 0, "linear": 1, "bands": 2, "yarn": 3}
+
+
+def rope_turns(theta: float, rot: int, kind: str = "plain", factor: float = 1.0, low: float = 1.0, high: float = 4.0, fast: float = 32.0, slow: float = 1.0, original: float = 0.0):
+    """(turns per position of the rot / 2 pairs as f64, magnitude) for rope(); `low` and `high` belong to "bands", `slow` and `fast` to "yarn"."""
+    if kind not in ROPE_KINDS:
+        raise HomuraError(HM_ERR_UNSUPPORTED, f"rope scaling {kind!r}: one of {sorted(ROPE_KINDS)}")
+    turns, magnitude = np.empty(max(rot // 2, 1), np.float64), C.c_float()
+    a, b = (slow, fast) if kind == "yarn" else (low, high)
+    _check(load_library().hm_rope_turns(theta, rot, ROPE_KINDS[kind], factor, a, b, original, _ptr(turns), C.byref(magnitude)))
+    return turns[: rot // 2], magnitude.value
+
+
+def rope(x, heads: int, dim: int, turns, pos, rot: Optional[int] = None, neighbours: bool = False, magnitude: float = 1.0, dtype: DType = DType.F32, ldx: Optional[int] = None, y=None, ldy: Optional[int] = None, stream=None):
+    """Rows of heads [M, heads * dim], the first `rot` elements (default: all) of every head turned by the rows' positions.  Device mode: x=(addr, M); y may be x."""
+    lib = load_library()
+    rot = dim if rot is None else rot
+    if isinstance(x, tuple):
+        (xa, M) = x
+        _check(lib.hm_rope(_ptr(xa), int(dtype), ldx or heads * dim, M, heads, dim, rot, int(neighbours), _ptr(pos), _ptr(turns), magnitude, _ptr(y), ldy or heads * dim, _ptr(stream)))
+        return None
+    xa, dtype = _rows_in(np.asarray(x).reshape(len(x), -1))
+    M = xa.shape[0]
+    turns, pos = np.ascontiguousarray(turns, dtype=np.float64), np.ascontiguousarray(pos, dtype=np.int32)
+    if xa.shape[1] != heads * dim or turns.size != rot // 2 or pos.size != M:
+        raise HomuraError(HM_ERR_INVALID, "rows are heads * dim elements, turns rot / 2, positions one per row")
+    o = _rows_out(xa.shape, dtype)
+    _check(lib.hm_rope(_ptr(xa), int(dtype), heads * dim, M, heads, dim, rot, int(neighbours), _ptr(pos), _ptr(turns), magnitude, _ptr(o), heads * dim, None))
+    return o
+
+
+def kv8_pool_bytes(kv_heads: int, dim: int, vdim: int, n_pages: int) -> int:
+    """Bytes of a pool of n_pages pages of 64 tokens."""
+    return int(load_library().hm_kv8_pool_bytes(kv_heads, dim, vdim, n_pages))
+
+
+class KV8Cache:
+    """A paged cache of 8 bits (hm_kv8).  `pages` is the device address of kv8_pool_bytes bytes, or None: memory of its own.  `page_table` is (device address, n_seq,
+    max_pages), or an array [n_seq, max_pages] that is kept on the host and copied by every call.  Rows' sequences and positions are int32 arrays, or device addresses
+    where the rows are (addr, rows)."""
+
+    def __init__(self, kv_heads: int, dim: int, vdim: int, pages, n_pages: int, page_table):
+        size = kv8_pool_bytes(kv_heads, dim, vdim, n_pages)
+        if size == 0:
+            raise HomuraError(HM_ERR_INVALID, "a cache has 1 to 1024 heads, keys and values of 1 to 256 elements, and pages")
+        self._own = DeviceBuffer(size) if pages is None else None
+        if not isinstance(page_table, tuple):
+            table = np.array(page_table, dtype=np.int32, ndmin=2)  # a copy of its own
+            page_table = (table.ctypes.data, *table.shape)
+            self._table = table
+        at, n_seq, max_pages = page_table
+        self.c = HmKv8(self._own.ptr if pages is None else int(pages), int(at), n_pages, n_seq, max_pages, kv_heads, dim, vdim)
+
+    def _rows(self, row_seq, row_pos, M):
+        seq, pos = (np.ascontiguousarray(r, dtype=np.int32) for r in (row_seq, row_pos))
+        if seq.size != M or pos.size != M:
+            raise HomuraError(HM_ERR_INVALID, "a sequence and a position per row")
+        return seq, pos
+
+    def write(self, k, v, row_seq, row_pos, dtype: DType = DType.F32, ldk: Optional[int] = None, ldv: Optional[int] = None, stream=None):
+        """Quantises keys [M, kv_heads * dim] and values [M, kv_heads * vdim] into their places.  Device mode: k=(addr, M)."""
+        lib, c, wk, wv = load_library(), self.c, self.c.kv_heads * self.c.dim, self.c.kv_heads * self.c.vdim
+        if isinstance(k, tuple):
+            (ka, M) = k
+            _check(lib.hm_kv8_write(C.byref(c), _ptr(ka), _ptr(v), int(dtype), ldk or wk, ldv or wv, _ptr(row_seq), _ptr(row_pos), M, _ptr(stream)))
+            return
+        (ka, dtype), (va, other) = _rows_in(np.asarray(k).reshape(len(k), -1)), _rows_in(np.asarray(v).reshape(len(v), -1))
+        seq, pos = self._rows(row_seq, row_pos, len(ka))
+        if dtype != other or len(ka) != len(va) or ka.shape[1] != wk or va.shape[1] != wv:
+            raise HomuraError(HM_ERR_INVALID, "keys and values are rows [M, kv_heads * dim] and [M, kv_heads * vdim] of one type")
+        _check(lib.hm_kv8_write(C.byref(c), _ptr(ka), _ptr(va), int(dtype), wk, wv, _ptr(seq), _ptr(pos), len(ka), None))
+
+    def read(self, row_seq, row_pos, k=None, v=None, dtype: DType = DType.F32, ldk: Optional[int] = None, ldv: Optional[int] = None, stream=None):
+        """The values held at the rows' places: (keys, values), zeros where there is no place.  Device mode: row_seq=(addr, M), into k and v (left as they are where there is no place)."""
+        lib, c, wk, wv = load_library(), self.c, self.c.kv_heads * self.c.dim, self.c.kv_heads * self.c.vdim
+        if isinstance(row_seq, tuple):
+            (sa, M) = row_seq
+            _check(lib.hm_kv8_read(C.byref(c), _ptr(sa), _ptr(row_pos), M, _ptr(k), _ptr(v), int(dtype), ldk or wk, ldv or wv, _ptr(stream)))
+            return None
+        seq, pos = self._rows(row_seq, row_pos, np.asarray(row_seq).size)
+        ko, vo = _rows_out((seq.size, wk), dtype), _rows_out((seq.size, wv), dtype)
+        _check(lib.hm_kv8_read(C.byref(c), _ptr(seq), _ptr(pos), seq.size, _ptr(ko), _ptr(vo), int(dtype), wk, wv, None))
+        return ko, vo
+
+    def attend_bytes(self, M: int, heads: int, n_shared: int = 0) -> int:
+        """Bytes of work memory that attend() takes on the current device."""
+        return int(load_library().hm_kv8_attn_bytes(C.byref(self.c), M, heads, n_shared))
+
+    def attend(self, q, row_seq, row_pos, heads: int, scale: float, shared=None, dtype: DType = DType.F32, ldq: Optional[int] = None, out=None, ldo: Optional[int] = None, work=None, stream=None):
+        """softmax(scale q . k) v over the positions up to each row's own.  `shared`: the first pages of every row's sequence, read once for all rows.  Device mode: q=(addr, M),
+        shared=(addr, pages)."""
+        lib, c, wq, wo = load_library(), self.c, heads * self.c.dim, heads * self.c.vdim
+        if isinstance(q, tuple):
+            (qa, M), (sa, n) = q, shared or (None, 0)
+            _check(lib.hm_kv8_attn(C.byref(c), _ptr(qa), int(dtype), ldq or wq, _ptr(row_seq), _ptr(row_pos), M, heads, scale, _ptr(sa), n, _ptr(out), ldo or wo, _ptr(work), _ptr(stream)))
+            return None
+        qa, dtype = _rows_in(np.asarray(q).reshape(len(q), -1))
+        seq, pos = self._rows(row_seq, row_pos, len(qa))
+        if qa.shape[1] != wq:
+            raise HomuraError(HM_ERR_INVALID, "queries are rows [M, heads * dim]")
+        sa = np.ascontiguousarray([] if shared is None else shared, dtype=np.int32)
+        o = _rows_out((len(qa), wo), dtype)
+        _check(lib.hm_kv8_attn(C.byref(c), _ptr(qa), int(dtype), wq, _ptr(seq), _ptr(pos), len(qa), heads, scale, _ptr(sa) if sa.size else None, sa.size, _ptr(o), wo, None, None))
+        return o
 
 
 def attn_decode_paged(q, k_pages: DeviceBuffer, v_pages: DeviceBuffer, kv_dtype: DType, page_table, kv_len, heads: int, kv_heads: int, hd: int, max_pages: int, page_tokens: int = 16) -> np.ndarray:

@@ -17,7 +17,9 @@
 #include "image.h"
 #include "moe.h"
 #include "kquant.h"
+#include "kv8.h"
 #include "latent_attn.h"
+#include "rope.h"
 #include "sampler.h"
 #include "loaders.h"
 
@@ -236,6 +238,16 @@ size_t row_bytes(int dtype) { return dtype == HM_BF16 ? 2 : 4; }
 bool bad_rows(int rows, size_t width, size_t ld) { return ld < width || ld > ((size_t)1 << 60) / std::max(rows, 1); }
 // Bytes of rows of `width` elements, ld apart.
 size_t span_bytes(int rows, int width, size_t ld, int dtype) { return rows < 1 ? 0 : ((size_t)(rows - 1) * ld + width) * row_bytes(dtype); }
+
+// Whether rows of `wa` elements, `lda` apart, and rows of `wb`, `ldb` apart, of one type have a byte in common (or cannot be told apart).
+bool rows_meet(const void* a, size_t wa, size_t lda, const void* b, size_t wb, size_t ldb, int rows, int dtype) {
+    const uintptr_t pa = (uintptr_t)a, pb = (uintptr_t)b;
+    const size_t size = row_bytes(dtype);
+    if (rows < 1 || pa + span_bytes(rows, (int)wa, lda, dtype) <= pb || pb + span_bytes(rows, (int)wb, ldb, dtype) <= pa) return false;
+    if (rows == 1 || lda != ldb) return true;
+    const size_t step = lda * size, at = pb >= pa ? (pb - pa) % step : (step - (pa - pb) % step) % step;  // where b's rows begin within a's steps
+    return at < wa * size || at + wb * size > step;
+}
 
 #define NEED_DEVICE()                                                                             \
     do {                                                                                          \
@@ -1468,6 +1480,159 @@ int hm_expert_sum(const void* rows, int rows_dtype, const int32_t* ids, const fl
     if (!a.rows || !a.ids || !a.weights || (resid && !a.resid) || !a.y) return sg.finish(cudaErrorMemoryAllocation);
     if (sg.elsewhere()) return gfail(HM_ERR_INVALID, "hm_expert_sum: memory of another device than the current one");
     return sg.finish(launch_expert_sum(a, st));
+}
+
+int hm_rope_turns(double theta, int rot, int kind, double factor, double low, double high, double original, double* turns, float* magnitude) {
+    if (!turns || rot < 0 || rot > ROPE_MAX_DIM || (rot & 1) || !(theta > 0.0) || !std::isfinite(theta)) return gfail(HM_ERR_INVALID, "hm_rope_turns: bad arguments (rot even and at most 1024, theta > 0)");
+    if (kind < HM_ROPE_PLAIN || kind > HM_ROPE_YARN) return gfail(HM_ERR_UNSUPPORTED, "hm_rope_turns: unknown kind");
+    const bool bands = kind == HM_ROPE_BANDS, yarn = kind == HM_ROPE_YARN;
+    if (kind != HM_ROPE_PLAIN && !(factor > 0.0 && std::isfinite(factor))) return gfail(HM_ERR_INVALID, "hm_rope_turns: factor must be positive");
+    if ((bands || yarn) && !(original > 0.0 && std::isfinite(original) && low > 0.0 && high > low && std::isfinite(high))) return gfail(HM_ERR_INVALID, "hm_rope_turns: 0 < low < high, original > 0");
+    if (yarn && theta == 1.0) return gfail(HM_ERR_INVALID, "hm_rope_turns: theta 1 has no index that turns a given number of times");
+    const double pi = 3.14159265358979323846;
+    double from = 0.0, to = 0.0;
+    if (yarn) {
+        auto index = [&](double times) { return rot * std::log(original / (2.0 * pi * times)) / (2.0 * std::log(theta)); };
+        from = std::max(std::floor(index(high)), 0.0);
+        to = std::min(std::ceil(index(low)), (double)rot - 1.0);
+    }
+    for (int i = 0; i < rot / 2; ++i) {
+        const double f = std::pow(theta, -2.0 * i / rot);
+        double keep = 1.0;  // the share that is not divided
+        if (kind == HM_ROPE_LINEAR) keep = 0.0;
+        else if (bands) keep = std::min(std::max((original * f / (2.0 * pi) - low) / (high - low), 0.0), 1.0);
+        else if (yarn) keep = 1.0 - std::min(std::max((i - from) / std::max(to - from, 0.001), 0.0), 1.0);
+        turns[i] = (kind == HM_ROPE_PLAIN ? f : f * ((1.0 - keep) / factor + keep)) / (2.0 * pi);
+    }
+    if (magnitude) *magnitude = yarn && factor > 1.0 ? (float)(0.1 * std::log(factor) + 1.0) : 1.0f;
+    return HM_OK;
+}
+
+int hm_rope(const void* x, int dtype, size_t ldx, int M, int heads, int dim, int rot, int neighbours, const int32_t* pos, const double* turns, float magnitude, void* y, size_t ldy, void* stream) {
+    if (!x || !y || !pos || (!turns && rot > 0) || M < 0 || heads < 1 || heads > 65536 || dim < 1 || dim > ROPE_MAX_DIM || rot < 0 || rot > dim || (rot & 1) || bad_rows(M, (size_t)heads * dim, ldx) || bad_rows(M, (size_t)heads * dim, ldy))
+        return gfail(HM_ERR_INVALID, "hm_rope: bad arguments (rot even and at most dim, dim <= 1024, ldx and ldy >= heads * dim)");
+    if (!is_row_dtype(dtype)) return gfail(HM_ERR_UNSUPPORTED, "hm_rope: rows are HM_F32 or HM_BF16");
+    if (misaligned(x, row_bytes(dtype)) || misaligned(y, row_bytes(dtype)) || misaligned(pos, 4) || misaligned(turns, 8)) return gfail(HM_ERR_INVALID, "hm_rope: misaligned pointer");
+    const size_t width = (size_t)heads * dim;
+    if (x == y ? ldx != ldy : rows_meet(x, width, ldx, y, width, ldy, M, dtype)) return gfail(HM_ERR_INVALID, "hm_rope: y is x, or does not overlap it");
+    if (M == 0) return HM_OK;
+    NEED_DEVICE();
+    cudaStream_t st = (cudaStream_t)stream;
+    Staging sg(st);
+    RopeArgs a{};
+    uint8_t* out = sg.out((uint8_t*)y, span_bytes(M, (int)width, ldy, dtype), true);
+    a.y = out;
+    a.x = x == y ? out : sg.in((const uint8_t*)x, span_bytes(M, (int)width, ldx, dtype));
+    a.ldx = ldx;
+    a.ldy = ldy;
+    a.bf16 = dtype == HM_BF16;
+    a.M = M;
+    a.heads = heads;
+    a.dim = dim;
+    a.rot = rot;
+    a.neighbours = neighbours != 0;
+    a.pos = sg.in(pos, (size_t)M);
+    a.turns = sg.in(turns, (size_t)rot / 2);
+    a.magnitude = magnitude;
+    if (!a.x || !a.y || !a.pos || (rot > 0 && !a.turns)) return sg.finish(cudaErrorMemoryAllocation);
+    if (sg.elsewhere()) return gfail(HM_ERR_INVALID, "hm_rope: memory of another device than the current one");
+    return sg.finish(launch_rope(a, st));
+}
+
+// Sizes that a cache of 8 bits cannot have.
+static bool bad_kv8(int kv_heads, int dim, int vdim, int n_pages) { return kv_heads < 1 || kv_heads > 1024 || dim < 1 || dim > KV8_MAX_DIM || vdim < 1 || vdim > KV8_MAX_DIM || n_pages < 1; }
+static bool bad_cache(const hm_kv8* c) { return !c || !c->pages || !c->page_table || bad_kv8(c->kv_heads, c->dim, c->vdim, c->n_pages) || c->n_seq < 1 || c->max_pages < 1 || c->max_pages > 1 << 24; }
+static Kv8Pool kv8_pool(const hm_kv8* c, Staging& sg) {
+    return Kv8Pool{(unsigned char*)c->pages, sg.in(c->page_table, (size_t)c->n_seq * c->max_pages), c->n_pages, c->n_seq, c->max_pages, c->kv_heads, c->dim, c->vdim};
+}
+
+size_t hm_kv8_pool_bytes(int kv_heads, int dim, int vdim, int n_pages) { return bad_kv8(kv_heads, dim, vdim, n_pages) ? 0 : (size_t)n_pages * kv_heads * kv8_block_bytes(dim, vdim); }
+
+// hm_kv8_write and hm_kv8_read: what they have in common.
+static int kv8_rows(const char* name, const hm_kv8* cache, void* k, void* v, int dtype, size_t ldk, size_t ldv, const int32_t* row_seq, const int32_t* row_pos, int M, bool write, void* stream) {
+    auto refuse = [&](int code, const char* why) { return gfail(code, std::string(name) + ": " + why); };
+    if (bad_cache(cache) || !k || !v || !row_seq || !row_pos || M < 0 || (size_t)M * cache->kv_heads > (size_t)1 << 30 || bad_rows(M, (size_t)cache->kv_heads * cache->dim, ldk) || bad_rows(M, (size_t)cache->kv_heads * cache->vdim, ldv))
+        return refuse(HM_ERR_INVALID, "bad arguments (dim and vdim <= 256, kv_heads <= 1024, M * kv_heads <= 2^30, ldk >= kv_heads * dim, ldv >= kv_heads * vdim)");
+    if (!is_row_dtype(dtype)) return refuse(HM_ERR_UNSUPPORTED, "rows are HM_F32 or HM_BF16");
+    if (misaligned(cache->pages, 16) || misaligned(cache->page_table, 4) || misaligned(k, row_bytes(dtype)) || misaligned(v, row_bytes(dtype)) || misaligned(row_seq, 4) || misaligned(row_pos, 4))
+        return refuse(HM_ERR_INVALID, "misaligned pointer (pages start on 16-byte boundaries)");
+    if (M == 0) return HM_OK;
+    NEED_DEVICE();
+    if (!is_device_ptr(cache->pages)) return refuse(HM_ERR_INVALID, "the pages must live in device memory");
+    cudaStream_t st = (cudaStream_t)stream;
+    Staging sg(st);
+    Kv8RowsArgs a{};
+    a.pool = kv8_pool(cache, sg);
+    sg.in((const uint8_t*)cache->pages, 0);  // device memory: only looked at
+    const size_t nk = span_bytes(M, cache->kv_heads * cache->dim, ldk, dtype), nv = span_bytes(M, cache->kv_heads * cache->vdim, ldv, dtype);
+    a.k = write ? (void*)sg.in((const uint8_t*)k, nk) : sg.out((uint8_t*)k, nk, true);
+    a.v = write ? (void*)sg.in((const uint8_t*)v, nv) : sg.out((uint8_t*)v, nv, true);
+    a.ldk = ldk;
+    a.ldv = ldv;
+    a.bf16 = dtype == HM_BF16;
+    a.M = M;
+    a.row_seq = sg.in(row_seq, (size_t)M);
+    a.row_pos = sg.in(row_pos, (size_t)M);
+    if (!a.pool.page_table || !a.k || !a.v || !a.row_seq || !a.row_pos) return sg.finish(cudaErrorMemoryAllocation);
+    if (sg.elsewhere()) return refuse(HM_ERR_INVALID, "memory of another device than the current one");
+    return sg.finish(write ? launch_kv8_write(a, st) : launch_kv8_read(a, st));
+}
+
+int hm_kv8_write(const hm_kv8* cache, const void* k, const void* v, int dtype, size_t ldk, size_t ldv, const int32_t* row_seq, const int32_t* row_pos, int M, void* stream) {
+    return kv8_rows("hm_kv8_write", cache, const_cast<void*>(k), const_cast<void*>(v), dtype, ldk, ldv, row_seq, row_pos, M, true, stream);
+}
+
+int hm_kv8_read(const hm_kv8* cache, const int32_t* row_seq, const int32_t* row_pos, int M, void* k, void* v, int dtype, size_t ldk, size_t ldv, void* stream) {
+    return kv8_rows("hm_kv8_read", cache, k, v, dtype, ldk, ldv, row_seq, row_pos, M, false, stream);
+}
+
+static bool bad_kv8_attn(const hm_kv8* c, int M, int heads, int n_shared) {
+    return M < 0 || M > KV8_MAX_ROWS || heads < 1 || heads > 4096 || heads % c->kv_heads != 0 || n_shared < 0 || n_shared > c->max_pages;
+}
+
+size_t hm_kv8_attn_bytes(const hm_kv8* cache, int M, int heads, int n_shared) {
+    if (!cache || bad_kv8(cache->kv_heads, cache->dim, cache->vdim, 1) || bad_kv8_attn(cache, M, heads, n_shared)) return 0;
+    return kv8_attn_bytes(cache->kv_heads, cache->vdim, M, heads, n_shared, sm_count_of_current_device());
+}
+
+int hm_kv8_attn(const hm_kv8* cache, const void* q, int dtype, size_t ldq, const int32_t* row_seq, const int32_t* row_pos, int M, int heads, float scale, const int32_t* shared_pages, int n_shared, void* out, size_t ldo, void* work,
+                void* stream) {
+    if (bad_cache(cache) || bad_kv8_attn(cache, M, heads, n_shared) || !q || !out || !row_seq || !row_pos || (n_shared > 0 && !shared_pages) || !std::isfinite(scale) || bad_rows(M, (size_t)heads * cache->dim, ldq) ||
+        bad_rows(M, (size_t)heads * cache->vdim, ldo))
+        return gfail(HM_ERR_INVALID, "hm_kv8_attn: bad arguments (M <= 8192, heads <= 4096 and a multiple of kv_heads, dim and vdim <= 256, n_shared <= max_pages, ldq >= heads * dim, ldo >= heads * vdim)");
+    if (!is_row_dtype(dtype)) return gfail(HM_ERR_UNSUPPORTED, "hm_kv8_attn: rows are HM_F32 or HM_BF16");
+    if (misaligned(cache->pages, 16) || misaligned(cache->page_table, 4) || misaligned(q, row_bytes(dtype)) || misaligned(out, row_bytes(dtype)) || misaligned(row_seq, 4) || misaligned(row_pos, 4) || misaligned(shared_pages, 4) ||
+        misaligned(work, 16))
+        return gfail(HM_ERR_INVALID, "hm_kv8_attn: misaligned pointer (pages and work start on 16-byte boundaries)");
+    const int wq = heads * cache->dim, wo = heads * cache->vdim;
+    if (rows_meet(q, wq, ldq, out, wo, ldo, M, dtype)) return gfail(HM_ERR_INVALID, "hm_kv8_attn: q and out overlap");
+    if (M == 0) return HM_OK;
+    NEED_DEVICE();
+    if (!is_device_ptr(cache->pages) || (work && !is_device_ptr(work))) return gfail(HM_ERR_INVALID, "hm_kv8_attn: the pages and the work memory must live in device memory");
+    cudaStream_t st = (cudaStream_t)stream;
+    Staging sg(st);
+    const int sms = sm_count_of_current_device();
+    Kv8AttnArgs a{};
+    a.pool = kv8_pool(cache, sg);
+    sg.in((const uint8_t*)cache->pages, 0);  // device memory: only looked at
+    sg.in((const uint8_t*)work, 0);
+    a.q = sg.in((const uint8_t*)q, span_bytes(M, wq, ldq, dtype));
+    a.out = sg.out((uint8_t*)out, span_bytes(M, wo, ldo, dtype), true);
+    a.ldq = ldq;
+    a.ldo = ldo;
+    a.bf16 = dtype == HM_BF16;
+    a.M = M;
+    a.heads = heads;
+    a.row_seq = sg.in(row_seq, (size_t)M);
+    a.row_pos = sg.in(row_pos, (size_t)M);
+    a.scale = scale;
+    a.shared = sg.in(shared_pages, (size_t)n_shared);
+    a.n_shared = n_shared;
+    a.work = work ? work : sg.scratch(kv8_attn_bytes(cache->kv_heads, cache->vdim, M, heads, n_shared, sms), false);
+    if (!a.pool.page_table || !a.q || !a.out || !a.row_seq || !a.row_pos || (n_shared > 0 && !a.shared) || !a.work) return sg.finish(cudaErrorMemoryAllocation);
+    if (sg.elsewhere()) return gfail(HM_ERR_INVALID, "hm_kv8_attn: memory of another device than the current one");
+    if (!sg.ok(get_wait_err(&a.err_flag))) return sg.finish(cudaSuccess);
+    return finish_product(sg, launch_kv8_attn(a, sms, st), "hm_kv8_attn: a bounded device-side wait ran out");
 }
 
 int hm_argmax(const float* logits, int rows, int n, uint32_t* out, void* stream) {

@@ -373,6 +373,50 @@ HM_API int hm_expert_gemv(const void* x, int x_dtype, size_t ldx, const void* w_
  * resid, a bf16 y and resid do not overlap.  Identity experts (ids -1) have no part here: theirs is id_weight of hm_post_norm_route, which its next call takes. */
 HM_API int hm_expert_sum(const void* rows, int rows_dtype, const int32_t* ids, const float* weights, int tokens, int top, int experts, int W, const float* resid, void* y, int y_dtype, void* stream);
 
+/* ---- rotary positions, and attention over a cache in 8 bits ------------------------------------------------------
+ * Rows are HM_F32 or HM_BF16, `ld` elements from row to row; positions, sequences and pages are int32.  Device pointers belong to the current device
+ * (HM_ERR_INVALID otherwise).  With device pointers only, every call is asynchronous on `stream`, keeps nothing between calls and may run beside others
+ * and be captured; make one call on each device before the first capture.  No counterpart in the reference. */
+/* Turns per position of the rot / 2 pairs of a head, theta^(-2 i / rot) / (2 pi), scaled for long contexts; computed on the host in 64 bits.
+ *   HM_ROPE_LINEAR  divided by factor
+ *   HM_ROPE_BANDS   pairs that turn less than `low` times within `original` positions divided by factor, those that turn more than `high` times as they are, a
+ *                   linear mixture of both between
+ *   HM_ROPE_YARN    pairs mixed by their index instead: as they are up to the (rounded down) index that turns `high` times within `original`, divided by factor from
+ *                   the (rounded up) one that turns `low` times; magnitude 0.1 ln(factor) + 1 (factor > 1)
+ * turns [rot / 2] and magnitude (1 but for HM_ROPE_YARN) are host memory; magnitude may be NULL. */
+enum hm_rope_kind { HM_ROPE_PLAIN = 0, HM_ROPE_LINEAR = 1, HM_ROPE_BANDS = 2, HM_ROPE_YARN = 3 };
+HM_API int hm_rope_turns(double theta, int rot, int kind, double factor, double low, double high, double original, double* turns, float* magnitude);
+/* y = the heads [M, heads, dim] of x with their first `rot` elements turned: pair (a, b) -> magnitude * (a cos - b sin, a sin + b cos) of turns[i] * pos[row] full turns.
+ * Pairs are (i, i + rot / 2), or (2 i, 2 i + 1) with neighbours != 0.  Elements from `rot` on are copied.  y may be x (ldy = ldx); other overlaps of their rows are refused.
+ * dim <= 1024; rot even.  The heads of queries and keys that stand side by side in a projection's rows are one call. */
+HM_API int hm_rope(const void* x, int dtype, size_t ldx, int M, int heads, int dim, int rot, int neighbours, const int32_t* pos, const double* turns, float magnitude, void* y, size_t ldy, void* stream);
+/* A paged cache of 8 bits: 64 tokens per page; per token and head one f32 scale for the key and one for the value.  With m the largest magnitude of a key (of a value):
+ * codes rint(x * (127 / m)), scale m / 127, each step rounded to f32 (so a value is off by at most half a scale); m < 2^-100: zeros; an infinity or a NaN: the whole
+ * vector is NaN.  `pages` is device memory of hm_kv8_pool_bytes, 16-byte aligned, that needs no clearing; one pool holds keys and values of a layer.
+ * A position whose entry of page_table [n_seq, max_pages] lies outside [0, n_pages) has no place (-1: not there, or given up again).
+ * dim, vdim <= 256; kv_heads <= 1024; max_pages <= 2^24. */
+typedef struct hm_kv8 {
+    void* pages;
+    const int32_t* page_table;
+    int32_t n_pages, n_seq, max_pages;
+    int32_t kv_heads, dim, vdim;
+} hm_kv8;
+HM_API size_t hm_kv8_pool_bytes(int kv_heads, int dim, int vdim, int n_pages);
+/* Quantises row m's keys k [M, kv_heads, dim] and values v [M, kv_heads, vdim] into position row_pos[m] of sequence row_seq[m].  Rows without a place are not written;
+ * of two rows with one place either may stay, or parts of both. */
+HM_API int hm_kv8_write(const hm_kv8* cache, const void* k, const void* v, int dtype, size_t ldk, size_t ldv, const int32_t* row_seq, const int32_t* row_pos, int M, void* stream);
+/* The values that the cache holds at those places (code * scale, HM_BF16 rounded once).  Rows without a place are left as they are. */
+HM_API int hm_kv8_read(const hm_kv8* cache, const int32_t* row_seq, const int32_t* row_pos, int M, void* k, void* v, int dtype, size_t ldk, size_t ldv, void* stream);
+/* out [M, heads, vdim] = softmax(scale q . k) v of q [M, heads, dim] over the positions 0 .. row_pos[m] of sequence row_seq[m] that have a place; zeros where there are none
+ * (row_pos -1).  Rows whose sequence lies outside [0, n_seq) are left as they are; a row_pos beyond the table means its last position.
+ * shared_pages [n_shared] (NULL with 0): pages that stand for the first n_shared pages of every row's sequence, whatever page_table says there; the keys and values
+ * of a common prefix are then read once for all rows.  Rows of one sequence that follow one another (a portion of a prompt) share its whole table.
+ * q and out have one type; their rows do not overlap.  M <= 8192, heads <= 4096.  work: device memory of hm_kv8_attn_bytes, 16-byte aligned, for this call alone until it has
+ * ended; needs no clearing.  NULL: the call takes its own and waits. */
+HM_API size_t hm_kv8_attn_bytes(const hm_kv8* cache, int M, int heads, int n_shared);
+HM_API int hm_kv8_attn(const hm_kv8* cache, const void* q, int dtype, size_t ldq, const int32_t* row_seq, const int32_t* row_pos, int M, int heads, float scale, const int32_t* shared_pages, int n_shared, void* out, size_t ldo, void* work,
+                       void* stream);
+
 /* argmax with ties to the highest index (src/generate.rs:457-468): logits [rows, n]. */
 HM_API int hm_argmax(const float* logits, int rows, int n, uint32_t* out, void* stream);
 
