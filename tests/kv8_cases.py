@@ -31,14 +31,14 @@ def held(x):
 
 
 def attention(q, ks, vs, scale):
-    """q [heads, dim], ks [tokens, kv_heads, dim], vs [tokens, kv_heads, vdim] (f64) -> out [heads, vdim], the sum of weighted magnitudes [heads, vdim], the largest sum of
-    magnitudes of a score's terms [heads]."""
+    """q [heads, dim], ks [tokens, kv_heads, dim], vs [tokens, kv_heads, vdim] (f64) -> out [heads, vdim], and what the bound is made of: the sum of weighted magnitudes
+    [heads, vdim], the largest sum of magnitudes of a score's terms [heads], the granules of queries (in scores) and of weights (in results) [heads]."""
     H, G = q.shape[0], ks.shape[1]
     if ks.shape[0] == 0:
         z = np.zeros((H, vs.shape[2]))
-        return z, z, np.zeros(H)
+        return z, (z, np.zeros(H), np.zeros(H), np.zeros(H))
     group = H // G
-    out, mag, terms = [], [], []
+    out, mag, terms, fine_q, fine_w = [], [], [], [], []
     for h in range(H):
         k, v = ks[:, h // group], vs[:, h // group]
         s = scale * (k @ q[h])
@@ -47,15 +47,20 @@ def attention(q, ks, vs, scale):
         out.append(p @ v)
         mag.append(p @ np.abs(v))
         terms.append(abs(scale) * (np.abs(k) @ np.abs(q[h])).max())
-    return np.array(out), np.array(mag), np.array(terms)
+        fine_q.append(abs(scale) * np.abs(q[h]).max() * np.abs(k).sum(-1).max())
+        fine_w.append(len(p) * (p * np.abs(v).max(-1)).max())
+    return np.array(out), (np.array(mag), np.array(terms), np.array(fine_q), np.array(fine_w))
 
 
-def bound(out, mag, terms, bf16):
+def bound(out, parts, bf16):
     """Scores: products of a value's f16 terms (2^-22 of it) and codes are exact, a chain of at most 16 truncating sums of 2^-23 and a few roundings: 2^-18.9 of the terms'
     magnitudes; a weight is off by that much twice (itself and the sum it is divided by).  Weights: f16 terms 2^-22, sums of at most 64 tokens by truncation, partial results
-    by roundings: 2^-18.  bf16 rows: weights may be one f16 term (2^-11), the result is rounded (2^-8)."""
-    e = 2 * terms[..., None] * 2.0**-18.9 + 2.0**-18
-    tol = mag * e + 1e-37
+    by roundings: 2^-18.  f16 has no step below 2^-24: the second term of a query whose row's largest is at least 2^14 ends at 2^-39 of that, and the second term of a weight
+    whose pair's largest (times its value scale, 127 of which are the token's largest value) is at least 2^13 at 2^-38 of that, for each token.  bf16 rows: weights may be one
+    f16 term (2^-11), the result is rounded (2^-8)."""
+    mag, terms, fine_q, fine_w = parts
+    e = 2 * (terms * 2.0**-18.9 + fine_q * 2.0**-39)[..., None] + 2.0**-18
+    tol = mag * e + fine_w[..., None] * 2.0**-38 + 1e-37
     return tol + mag * 2.0**-11 + np.abs(out) * 2.0**-8 if bf16 else tol
 
 
@@ -123,8 +128,8 @@ class Model:
             if seen is not None:
                 at = at[seen(i)[: len(at)]]
             k, v = held(self.k[i])[at].astype(np.float64), held(self.v[i])[at].astype(np.float64)
-            want, mag, terms = attention(x[m].astype(np.float64).reshape(heads, self.dim), k, v, scale)
-            err, tol = np.abs(o[m].reshape(heads, self.vdim) - want), bound(want, mag, terms, bf16)
+            want, parts = attention(x[m].astype(np.float64).reshape(heads, self.dim), k, v, scale)
+            err, tol = np.abs(o[m].reshape(heads, self.vdim) - want), bound(want, parts, bf16)
             assert (err <= tol).all(), (m, i, p, float((err / tol).max()), float(err.max()))
             worst = max(worst, float((err / tol).max()))
         return worst
