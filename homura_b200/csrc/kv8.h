@@ -10,9 +10,10 @@ constexpr int KV8_PAGE = 64;        // tokens per page
 constexpr int KV8_MAX_DIM = 256;    // elements of a key or a value
 constexpr int KV8_MAX_ROWS = 8192;  // rows of one attention call
 
-// A page holds one block per key/value head: 64 scales of keys, 64 of values (f32), then the codes of keys and of values (value + 128, one byte), in slabs
-// of 32 elements, [pad / 32][64 rows][32].  Row r of a slab is token r of the values; of the keys it is token key_token(r): within every eight tokens
-// 0 4 1 5 2 6 3 7, the order in which the lanes of a warp-level MMA want them.
+// A page holds one block per key/value head, in two halves of 32 tokens: the 32 scales of its keys (f32) and their codes, one signed byte each, then the same of its values.
+// Codes stand in the order in which the lanes of warp-level MMAs want them:
+//   keys    slabs of 32 elements, [pad / 32][32 rows][32]; row r holds the token t with kv8_key_row(t) = r
+//   values  [pad][32 tokens]
 struct Kv8Pool {
     unsigned char* pages;
     const int32_t* page_table;  // [n_seq][max_pages]
@@ -20,8 +21,15 @@ struct Kv8Pool {
     int kv_heads, dim, vdim;
 };
 __host__ __device__ __forceinline__ int kv8_pad(int d) { return (d + 31) & ~31; }
-__host__ __device__ __forceinline__ size_t kv8_block_bytes(int dim, int vdim) { return (size_t)KV8_PAGE * (8 + kv8_pad(dim) + kv8_pad(vdim)); }
-__host__ __device__ __forceinline__ int kv8_key_row(int t) { return (t & ~7) | ((t & 3) << 1) | ((t >> 2) & 1); }
+constexpr int KV8_HALF = 32;  // tokens of a half
+__host__ __device__ __forceinline__ int kv8_part_bytes(int d) { return KV8_HALF * (4 + kv8_pad(d)); }  // keys or values of a half
+__host__ __device__ __forceinline__ size_t kv8_half_bytes(int dim, int vdim) { return (size_t)kv8_part_bytes(dim) + kv8_part_bytes(vdim); }
+__host__ __device__ __forceinline__ size_t kv8_block_bytes(int dim, int vdim) { return 2 * kv8_half_bytes(dim, vdim); }
+// Token 8 i + 2 j + e of a half (i, j < 4) is column 2 i + e of the scores' tile j: the lane with columns 2 i and 2 i + 1 of all tiles has eight tokens that follow one another.
+__host__ __device__ __forceinline__ int kv8_key_row(int t) { return (((t >> 1) & 3) << 3) | ((t >> 3) << 1) | (t & 1); }
+// Places in their part of a half of token t's codes of element d.
+__host__ __device__ __forceinline__ int kv8_key_at(int t, int d) { return KV8_HALF * 4 + ((d >> 5) * KV8_HALF + kv8_key_row(t)) * 32 + (d & 31); }
+__host__ __device__ __forceinline__ int kv8_value_at(int t, int d) { return KV8_HALF * 4 + d * KV8_HALF + t; }
 
 // Page of a position, or -1 where there is none (a sequence, a position or a page that is out of range).
 __device__ __forceinline__ int kv8_page(const Kv8Pool& p, int seq, int pos) {
@@ -38,8 +46,8 @@ struct Kv8RowsArgs {
     int M;
     const int32_t *row_seq, *row_pos;
 };
-cudaError_t launch_kv8_write(const Kv8RowsArgs& a, cudaStream_t st);
-cudaError_t launch_kv8_read(const Kv8RowsArgs& a, cudaStream_t st);
+cudaError_t launch_kv8_write(const Kv8RowsArgs& a, int sm_count, cudaStream_t st);
+cudaError_t launch_kv8_read(const Kv8RowsArgs& a, int sm_count, cudaStream_t st);
 
 struct Kv8AttnArgs {
     Kv8Pool pool;

@@ -5,21 +5,26 @@
 // kv8_stream_kernel   rows' contexts, eight (row, head) pairs of one key/value head at a time; bound by the bytes of the cache
 // kv8_join_kernel     joins the parts of contexts that several CTAs share
 //
-// Arithmetic of the first.  A warp takes 32 tokens of a page for eight pairs on m16n8k16 MMAs of f16 with f32 sums:
-//   scores [16 x 8 tokens] = Q [16 x dim] . K^T,   out [16 x 8 elements] = W [16 x 16 tokens] . V
-// Codes are whole numbers below 128 and so exact in f16: a byte becomes the last bits of 1024 + byte (one permutation for two of them), from which 1152 is
-// subtracted.  Rows 0 .. 7 of Q are the pairs' queries times a power of two and rounded, rows 8 .. 15 what that leaves (together 2^-22 of a value): the tile's
-// two halves are added up after the product.  A token's key scale joins behind the product, its value scale goes into the weight, W = 2^(s - max) * scale, which
-// enters the same way in two terms, times a power of two that follows the pair's largest W (granules of 2^-38 of it).  So the cache's values are used as they are,
-// and results are f32 products but for 2^-22.  A step's 32 tokens have accumulators of their own, added up in f32 outside: tensor core sums are truncated.
+// Arithmetic of the first.  A warp takes a piece, 32 tokens (half of a page), for eight pairs, on m16n8k32 MMAs of 8-bit whole numbers with 32-bit sums, whose B operands are the
+// codes as they are cached:
+//   scores [16 x 8 tokens] = Q [16 x dim] . K^T,   out [16 x 8 elements] = W [16 x 32 tokens] . V
+// Queries and weights enter as digits of base 256: rows 0 .. 7 are the pairs' upper digits, rows 8 .. 15 the lower ones, so that a tile's two halves are added up
+// after the product (the first times 256).  bf16 rows take two digits: a query is whole numbers up to 32639 for its largest element (2^-16 of that), a weight up to
+// 65535 for the largest of its piece (2^-16 of that).  f32 rows take four, in two products: 2^-31 of the largest, or a value's own 24 bits.  Sums of digits times
+// codes are exact; what f32 rounds is what one would round without digits.  A token's key scale joins behind the product, its value scale goes into the weight,
+// W = 2^(s - max) * scale, so that the largest of a piece is found with it.
+// Against f16 operands (codes become f16 by two instructions for two codes, queries and weights by two terms): 981 instructions for 32 tokens x 256 elements, of which
+// a third made f16 of codes, 105 us for 64 sequences of up to 8000 tokens (366 MB).
 //
-// Work.  The pages of all rows, heads and tiles of eight pairs stand in one line, which the CTAs cut into equal lengths: contexts of any lengths keep all SMs
-// busy to the end, and no length needs to be known on the host.  A CTA writes what it has as a whole and leaves the rest (its first and its last item) in `work`.
+// Work.  The pieces of all rows, heads and tiles of eight pairs stand in one line, which the CTAs cut into equal lengths: contexts of any lengths keep all SMs busy to the
+// end, and no length needs to be known on the host.  A CTA's warps take its pieces in turn, each with a ring of copies of its own; what they have of an item is added up in shared
+// memory.  The CTA writes the items that it has as a whole and leaves the rest (its first and its last) in `work`, for kv8_join_kernel.
+// Slower where tried, at 64 sequences of up to 8000 tokens (93 us with each of them): a range of pieces for every warp, which then has more partial items than are worth joining; whole
+// pages for a warp, of which 12 do not fit twice; 16 warps with one piece each.
 #include "kv8.h"
 
-#include <cuda_fp16.h>
-
 #include <algorithm>
+#include <type_traits>
 
 #include "launch_attrs.h"
 #include "mbarrier.cuh"
@@ -28,34 +33,34 @@
 namespace hm {
 namespace {
 
-constexpr int WARPS = 8, THREADS = WARPS * 32 + 32;
-constexpr int PAIRS = 8;       // of an item
-constexpr int TURN = WARPS / 2;    // pages that the warps take at once, two warps a page.  The stages are a multiple of it: a stage is always the same two warps', so
-constexpr int MAX_STAGES = 12;     // that nobody waits for a stage's next page while the one in front of it is still on its way
-constexpr size_t ROOM = 224 * 1024;  // shared memory of an SM for CTAs of this kernel, what they hold outside the dynamic part taken off
-constexpr int LEAST_PAGES = TURN;  // of a CTA: fewer would only leave more to be joined
+constexpr int PAIRS = 8;           // of an item
+constexpr int LEAST_PIECES = 12;   // of a CTA, one for each of its warps: fewer would only leave more to be joined
+constexpr int MAX_DEPTH = 4;
+constexpr int MERGE_ROWS = 32;      // pairs' results of several warps that stand in shared memory when those of all are added up
+constexpr size_t ROOM = 225 * 1024;  // shared memory of a CTA
 constexpr float LOG2E = 1.4426950408889634f;
 
-// ---- the line of pages ------------------------------------------------------------------------------
+// ---- the line of pieces ------------------------------------------------------------------------------
 struct Line {
-    long long total, chunk;  // pages of all items; of a CTA
+    long long total, chunk;  // pieces of all items; of a CTA
 };
 
 __device__ __forceinline__ int row_len(const Kv8AttnArgs& a, int m) {
     const int seq = __ldg(a.row_seq + m);
     return (unsigned)seq < (unsigned)a.pool.n_seq ? min(__ldg(a.row_pos + m), a.pool.max_pages * KV8_PAGE - 1) + 1 : 0;
 }
-__device__ __forceinline__ int row_pages(const Kv8AttnArgs& a, int m) { return max(0, (row_len(a, m) + KV8_PAGE - 1) / KV8_PAGE); }
+__device__ __forceinline__ int row_pieces(const Kv8AttnArgs& a, int m) { return max(0, (row_len(a, m) + KV8_HALF - 1) / KV8_HALF); }
 
-// first[m]: pages of the rows in front of row m, first[M]: of all.  Every thread of the CTA takes part; ends with a barrier.
+// Every thread of the CTA adds up the pieces of some rows that follow one another, ceil(M / THREADS) of them; first[t]: pieces in front of thread t's rows,
+// first[THREADS]: of all.  Ends with a barrier.
+template <int THREADS>
 __device__ __forceinline__ Line make_line(const Kv8AttnArgs& a, int items, int ctas, int* first) {
     __shared__ int s_sum[THREADS / 32], s_most;
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, per = (a.M + THREADS - 1) / THREADS, m0 = min(a.M, tid * per), m1 = min(a.M, m0 + per);
     if (tid == 0) s_most = 0;
     int sum = 0, most = 0;
     for (int m = m0; m < m1; ++m) {
-        const int n = row_pages(a, m);
-        first[m] = sum;
+        const int n = row_pieces(a, m);
         sum += n;
         most = max(most, n);
     }
@@ -75,363 +80,468 @@ __device__ __forceinline__ Line make_line(const Kv8AttnArgs& a, int items, int c
         if (w < warp) before += s_sum[w];
         all += s_sum[w];
     }
-    for (int m = m0; m < m1; ++m) first[m] += before;
-    if (tid == 0) first[a.M] = all;
+    first[tid] = before;
+    if (tid == 0) first[THREADS] = all;
     __syncthreads();
     Line l;
     l.total = (long long)all * items;
-    l.chunk = max((l.total + ctas - 1) / ctas, (long long)min(LEAST_PAGES, s_most));
+    l.chunk = max((l.total + ctas - 1) / ctas, (long long)min(LEAST_PIECES, s_most));
     return l;
 }
 
-// A CTA's pages of one item.
+// Pieces of one item that follow one another.
 struct Segment {
-    int m, item, page, n, of;  // row, its item, first page, pages, pages of the whole item
+    int m, item, at, n, of;  // row, its item, first piece, pieces, pieces of the whole item
 };
+template <int THREADS>
 __device__ __forceinline__ Segment segment_at(const Kv8AttnArgs& a, const int* first, int items, long long u, long long end) {
-    int lo = 0, hi = a.M;  // the last row that begins at or in front of u; rows without pages are passed over
+    const bool small = (unsigned long long)u >> 32 == 0;
+    const int rank = small ? (int)((uint32_t)u / (uint32_t)items) : (int)(u / items);  // that many pieces of an item of every row are in front
+    int lo = 0, hi = THREADS;           // the last thread whose rows begin there or in front; those without pieces are passed over
     while (hi - lo > 1) {
         const int mid = (lo + hi) / 2;
-        if ((long long)first[mid] * items <= u) lo = mid;
+        if (first[mid] <= rank) lo = mid;
         else hi = mid;
     }
     Segment s;
-    s.m = lo;
-    s.of = first[lo + 1] - first[lo];
-    const long long off = u - (long long)first[lo] * items;
-    s.item = (int)(off / s.of);
-    s.page = (int)(off - (long long)s.item * s.of);
-    s.n = (int)min((long long)(s.of - s.page), end - u);
+    int at = first[lo];
+    s.m = lo * ((a.M + THREADS - 1) / THREADS);
+    for (s.of = row_pieces(a, s.m); rank >= at + s.of; s.of = row_pieces(a, ++s.m)) at += s.of;
+    const long long off = u - (long long)at * items;  // below of * items
+    s.item = small ? (int)((uint32_t)off / (uint32_t)s.of) : (int)(off / s.of);
+    s.at = (int)(off - (long long)s.item * s.of);
+    s.n = (int)min((long long)(s.of - s.at), end - u);
     return s;
 }
 
+// The segment behind s, `left` pieces from the end (not 0).
+__device__ __forceinline__ void next_segment(const Kv8AttnArgs& a, int items, Segment& s, int left) {
+    s.at = 0;
+    if (++s.item == items) {
+        s.item = 0;
+        do s.of = row_pieces(a, ++s.m);
+        while (s.of == 0);
+    }
+    s.n = min(s.of, left);
+}
+
 // ---- pieces of the arithmetic --------------------------------------------------------------------------
-__device__ __forceinline__ void mma_f16(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
-    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
-                 : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
-                 : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+// c (+)= a . b; the first product of a sum begins with zeros.
+template <bool UNSIGNED_A, bool FIRST>
+__device__ __forceinline__ void mma_s8(int (&c)[4], const uint4& a, const uint2& b) {
+    const int c0 = FIRST ? 0 : c[0], c1 = FIRST ? 0 : c[1], c2 = FIRST ? 0 : c[2], c3 = FIRST ? 0 : c[3];
+    if constexpr (UNSIGNED_A)
+        asm("mma.sync.aligned.m16n8k32.row.col.s32.u8.s8.s32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%10,%11,%12,%13};"
+            : "=r"(c[0]), "=r"(c[1]), "=r"(c[2]), "=r"(c[3])
+            : "r"(a.x), "r"(a.y), "r"(a.z), "r"(a.w), "r"(b.x), "r"(b.y), "r"(c0), "r"(c1), "r"(c2), "r"(c3));
+    else
+        asm("mma.sync.aligned.m16n8k32.row.col.s32.s8.s8.s32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%10,%11,%12,%13};"
+            : "=r"(c[0]), "=r"(c[1]), "=r"(c[2]), "=r"(c[3])
+            : "r"(a.x), "r"(a.y), "r"(a.z), "r"(a.w), "r"(b.x), "r"(b.y), "r"(c0), "r"(c1), "r"(c2), "r"(c3));
 }
-__device__ __forceinline__ uint32_t h2_bits(__half2 h) { return *reinterpret_cast<uint32_t*>(&h); }
-// Two codes (bytes of w, chosen by `sel`: 0x4140 the first two, 0x4342 the others) as f16.
-template <uint32_t SEL>
-__device__ __forceinline__ uint32_t codes_f16(uint32_t w) {
-    const uint32_t u = __byte_perm(w, 0x64646464u, SEL);
-    return h2_bits(__hsub2(*reinterpret_cast<const __half2*>(&u), __half2half2(__ushort_as_half(0x6480))));
-}
-// x, y as f16, and what that leaves.
-__device__ __forceinline__ void split_f16(float x, float y, uint32_t& hi, uint32_t& lo) {
-    const __half2 h = __floats2half2_rn(x, y);
-    const float2 f = __half22float2(h);
-    hi = h2_bits(h);
-    lo = h2_bits(__floats2half2_rn(x - f.x, y - f.y));
+// 2^x; results below the normal range are zero.
+__device__ __forceinline__ float exp2_ftz(float x) {
+    float y;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
 }
 __device__ __forceinline__ float pow2_bits(int biased) { return __uint_as_float((uint32_t)biased << 23); }  // 2^(biased - 127), 1 <= biased <= 254
-constexpr int UP = 14;         // queries and weights enter with their largest between 2^UP and 2^(UP + 1)
-constexpr int LEAST_EXP = 14;  // smallest exponent field that a factor of 2^UP can be brought to
+
+// Digits of four values x[i], one word per digit, the lowest first (DIGITS 2: of 16 bits, else of 32).
+template <int DIGITS>
+__device__ __forceinline__ void digits_of(const uint32_t (&x)[4], uint32_t (&d)[DIGITS]) {
+    const uint32_t a01 = __byte_perm(x[0], x[1], 0x5140), a23 = __byte_perm(x[2], x[3], 0x5140);  // digit 0 of both, digit 1 of both
+    d[0] = __byte_perm(a01, a23, 0x5410);
+    d[1] = __byte_perm(a01, a23, 0x7632);
+    if constexpr (DIGITS == 4) {
+        const uint32_t b01 = __byte_perm(x[0], x[1], 0x7362), b23 = __byte_perm(x[2], x[3], 0x7362);
+        d[2] = __byte_perm(b01, b23, 0x5410);
+        d[3] = __byte_perm(b01, b23, 0x7632);
+    }
+}
+// What the upper and lower digits' sums of one or two products stand for.
+template <int PASSES>
+__device__ __forceinline__ float from_digits(const int (&c)[PASSES][4], int e) {
+    const float low = (float)(c[PASSES - 1][e] * 256 + c[PASSES - 1][2 + e]);
+    return PASSES == 1 ? low : fmaf((float)(c[0][e] * 256 + c[0][2 + e]), 65536.f, low);
+}
+constexpr float Q_MOST = 32639.f;   // two signed digits: 127 * 256 + 127
+constexpr float W_PART = 65535.f / 65536.f;
+constexpr float Q_TINY = 1.262177448353619e-29f;  // 2^-96: queries whose largest element is below count as zeros
+constexpr int W_LEAST = 32;         // smallest exponent field that weights are brought up from
 
 struct StreamShape {
-    int dp, vp, ldo, block, stages;
-    size_t q_at, merge_at, first_at, bytes;
+    int dp, vp, ldo, kpart, vpart, queries;  // padded sizes, row of the warps' results, bytes of a piece's keys and values, words of 16 bytes of an item's queries
+    size_t q_at, merge_at, bytes;
 };
-__host__ __device__ inline StreamShape stream_shape(int dim, int vdim, int M, int stages) {
+__host__ __device__ inline StreamShape stream_shape(int dim, int vdim, int passes, int warps, int depth) {
     StreamShape s;
     s.dp = kv8_pad(dim);
     s.vp = kv8_pad(vdim);
-    s.ldo = s.vp + 4;
-    s.block = (int)kv8_block_bytes(dim, vdim);
-    s.stages = stages;
-    s.q_at = (size_t)stages * s.block;
-    s.merge_at = s.q_at + (size_t)s.dp / 16 * 32 * 16;
-    s.first_at = s.merge_at + sizeof(float) * (WARPS / 2 * PAIRS * s.ldo);
-    s.bytes = s.first_at + sizeof(int) * (M + 1);
+    s.ldo = s.vp + 8;
+    s.kpart = kv8_part_bytes(dim);
+    s.vpart = kv8_part_bytes(vdim);
+    s.q_at = (size_t)warps * depth * (s.kpart + s.vpart);
+    s.queries = s.dp / 32 * passes * 32;
+    s.merge_at = s.q_at + 2 * sizeof(uint4) * s.queries;
+    s.bytes = s.merge_at + sizeof(float) * MERGE_ROWS * s.ldo;
     return s;
 }
 
 // What is left of an item in `work`: maximum and sum of every pair, then its elements (relative to the maximum, not divided).
 __host__ __device__ inline size_t part_floats(int vp) { return PAIRS * (size_t)(vp + 4); }
 
-__device__ __forceinline__ void consumers_sync() { asm volatile("bar.sync 1, 256;" ::: "memory"); }
-
+// Two results of a row: elements d and d + 1 of a head.
 template <bool BF16>
-__device__ __forceinline__ void store4(const Kv8AttnArgs& a, int m, int head, int d, const float (&v)[4], bool wide) {
+__device__ __forceinline__ void store2(const Kv8AttnArgs& a, int m, int head, int d, float x, float y, bool wide) {
     const size_t at = (size_t)m * a.ldo + (size_t)head * a.pool.vdim + d;
-    if (wide) {
-        store_row<BF16, 4>(a.out, at, v);
+    if (wide) {  // an even number of elements, pairs aligned
+        if (d >= a.pool.vdim) return;
+        if (BF16) *reinterpret_cast<uint32_t*>(static_cast<uint16_t*>(a.out) + at) = bf16x2_rne(x, y);
+        else *reinterpret_cast<float2*>(static_cast<float*>(a.out) + at) = make_float2(x, y);
         return;
     }
-#pragma unroll
-    for (int e = 0; e < 4; ++e) {
-        const float one[1] = {v[e]};
-        if (d + e < a.pool.vdim) store_row<BF16, 1>(a.out, at + e, one);
-    }
+    const float v[2][1] = {{x}, {y}};
+    if (d < a.pool.vdim) store_row<BF16, 1>(a.out, at, v[0]);
+    if (d + 1 < a.pool.vdim) store_row<BF16, 1>(a.out, at + 1, v[1]);
 }
 
-// VS: slabs of 32 value elements (at most).
-template <bool BF16, int VS>
-__global__ void __launch_bounds__(THREADS, VS <= 4 ? 2 : 1) kv8_stream_kernel(const Kv8AttnArgs a, int stages, int tiles, int wide) {
+// Parts in `work`: of CTA c its first item (0) and its last (1).
+__device__ __forceinline__ float* cta_part(const Kv8AttnArgs& a, int vp, int cta, int which) { return static_cast<float*>(a.work) + (size_t)(2 * cta + which) * part_floats(vp); }
+
+// VS: slabs of 32 value elements (at most).  A warp's ring holds `depth` pieces; the keys of a piece make room for those of a later one as soon as the scores are
+// there, the values when the piece is done.
+template <bool BF16, int VS, int WARPS>
+__global__ void __launch_bounds__(WARPS * 32, 1) kv8_stream_kernel(const Kv8AttnArgs a, int depth, int tiles, int wide) {
+    constexpr int PASSES = BF16 ? 1 : 2, THREADS = WARPS * 32;
     extern __shared__ __align__(128) unsigned char dyn[];
-    __shared__ uint64_t full[MAX_STAGES], empty[MAX_STAGES];
+    __shared__ uint64_t bars[WARPS][2][MAX_DEPTH];
     __shared__ volatile int s_abort;
-    __shared__ int s_there[MAX_STAGES];
-    __shared__ float s_c[PAIRS];                                   // what scores are multiplied with
-    __shared__ float s_m[WARPS / 2][PAIRS], s_l[WARPS / 2][PAIRS];
-    const StreamShape sh = stream_shape(a.pool.dim, a.pool.vdim, a.M, stages);
+    __shared__ int first[THREADS + 1];
+    __shared__ uint64_t s_added;         // the sums of the segment in front have been read
+    __shared__ float s_c[2][PAIRS];      // what scores are multiplied with
+    __shared__ float s_m[MERGE_ROWS], s_l[MERGE_ROWS];
+    const StreamShape sh = stream_shape(a.pool.dim, a.pool.vdim, PASSES, WARPS, depth);
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, group = a.heads / a.pool.kv_heads, items = a.pool.kv_heads * tiles, ctas = gridDim.x;
-    uint4* qf = reinterpret_cast<uint4*>(dyn + sh.q_at);
+    unsigned char* kbuf = dyn + (size_t)warp * depth * (sh.kpart + sh.vpart);
+    unsigned char* vbuf = kbuf + (size_t)depth * sh.kpart;
+    uint4* queries = reinterpret_cast<uint4*>(dyn + sh.q_at);  // of this segment and the one behind it
     float* merge = reinterpret_cast<float*>(dyn + sh.merge_at);
-    int* first = reinterpret_cast<int*>(dyn + sh.first_at);
-    if (tid == 0) {
-        for (int s = 0; s < stages; ++s) {
-            mb_init(&full[s], 1);
-            mb_init(&empty[s], 2);
+    uint64_t *kfull = bars[warp][0], *vfull = bars[warp][1];
+    if (tid == 0) mb_init(&s_added, WARPS);
+    if (lane == 0) {
+        for (int s = 0; s < depth; ++s) {
+            mb_init(&kfull[s], 1);
+            mb_init(&vfull[s], 1);
         }
         s_abort = 0;
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
-    const Line line = make_line(a, items, ctas, first);
+    const Line line = make_line<THREADS>(a, items, ctas, first);
     const long long u0 = min(line.total, blockIdx.x * line.chunk), u1 = min(line.total, u0 + line.chunk);
+    const int count = (int)(u1 - u0);  // pieces of this CTA
     pdl_launch_dependents();
-    if (warp == WARPS) {
-        // ---- copies ----
-        uint32_t i = 0;
-        bool go = true;
-        for (long long u = u0; u < u1 && go;) {
-            const Segment sg = segment_at(a, first, items, u, u1);
-            const int kvh = sg.item / tiles;
-            const int32_t* table = a.pool.page_table + (size_t)__ldg(a.row_seq + sg.m) * a.pool.max_pages;
-            for (int p0 = 0; p0 < sg.n && go; p0 += 32) {
-                const int p = sg.page + p0 + lane;
-                const int id = p0 + lane < sg.n ? p < a.n_shared ? __ldg(a.shared + p) : __ldg(table + p) : 0;
-                for (int j = 0; j < min(32, sg.n - p0); ++j, ++i) {
-                    const int page = __shfl_sync(0xffffffffu, id, j), s = (int)(i % stages);
-                    if (i >= (uint32_t)stages && !__all_sync(0xffffffffu, mb_wait(&empty[s], ((i / stages) & 1u) ^ 1u, a.err_flag, &s_abort))) {
-                        go = false;
-                        break;
-                    }
-                    if (lane == 0) {
-                        const bool there = (unsigned)page < (unsigned)a.pool.n_pages;
-                        s_there[s] = there;
-                        if (there) {
-                            mb_expect_tx(&full[s], (uint32_t)sh.block);
-                            bulk_copy(dyn + (size_t)s * sh.block, a.pool.pages + ((size_t)page * a.pool.kv_heads + kvh) * sh.block, (uint32_t)sh.block, &full[s]);
-                        } else {
-                            mb_arrive(&full[s]);
-                        }
-                    }
-                    __syncwarp();
-                }
-            }
-            u += sg.n;
-        }
-        if (lane == 0) mb_land_ring(full, i, (uint32_t)stages);
-        return;
-    }
 
     // ---- rows without a context ----
     for (int m = blockIdx.x; m < a.M; m += ctas) {
-        if (first[m + 1] != first[m] || (unsigned)__ldg(a.row_seq + m) >= (unsigned)a.pool.n_seq) continue;
+        if (row_pieces(a, m) > 0 || (unsigned)__ldg(a.row_seq + m) >= (unsigned)a.pool.n_seq) continue;
         const float zero[1] = {0.f};
-        for (int i = tid; i < a.heads * a.pool.vdim; i += WARPS * 32) store_row<BF16, 1>(a.out, (size_t)m * a.ldo + i, zero);
+        for (int i = tid; i < a.heads * a.pool.vdim; i += THREADS) store_row<BF16, 1>(a.out, (size_t)m * a.ldo + i, zero);
+    }
+    if (count == 0) return;
+
+    // ---- copies: `ahead` runs `depth` pieces of this warp ahead of the arithmetic ----
+    Segment sg = segment_at<THREADS>(a, first, items, u0, u1), ahead = sg;
+    int ahead_at = warp, ahead_begin = 0, ahead_page = -1;  // its piece, counted over the CTA; the first of its segment; its page in the pool
+    const int32_t* ahead_table = nullptr;                   // of its segment's sequence
+    const unsigned char* ahead_head = nullptr;              // its head's block of page 0
+    const uint32_t half = (uint32_t)(sh.kpart + sh.vpart), page_bytes = 2 * half * (uint32_t)a.pool.kv_heads;
+    auto enter = [&]() {
+        ahead_table = a.pool.page_table + (size_t)__ldg(a.row_seq + ahead.m) * a.pool.max_pages;
+        ahead_head = a.pool.pages + (size_t)(ahead.item / tiles) * (2 * half);
+    };
+    auto settle = [&]() {
+        if (ahead_at >= count) return;
+        if (ahead_at >= ahead_begin + ahead.n) {
+            do {
+                ahead_begin += ahead.n;
+                next_segment(a, items, ahead, count - ahead_begin);
+            } while (ahead_at >= ahead_begin + ahead.n);
+            enter();
+        }
+        const int p = (ahead.at + ahead_at - ahead_begin) >> 1;
+        ahead_page = __ldg(p < a.n_shared ? a.shared + p : ahead_table + p);
+    };
+    // the piece that it stands at, null where there is none; on to the next
+    auto take = [&]() -> const unsigned char* {
+        const unsigned char* src = nullptr;
+        if (ahead_at < count && (unsigned)ahead_page < (unsigned)a.pool.n_pages) src = ahead_head + (unsigned long long)(uint32_t)ahead_page * page_bytes + (((ahead.at + ahead_at - ahead_begin) & 1) ? half : 0u);
+        ahead_at += WARPS;
+        settle();
+        return src;
+    };
+    auto copy = [&](unsigned char* dst, const unsigned char* src, int bytes, uint64_t* bar) {
+        if (lane == 0) {
+            mb_expect_tx(bar, (uint32_t)bytes);
+            bulk_copy(dst, src, (uint32_t)bytes, bar);
+        }
+    };
+    uint32_t there = 0, phase = 0;  // bit s: slot s holds a piece; the parity of its next wait
+    enter();
+    settle();
+    for (int s = 0; s < depth; ++s) {
+        const unsigned char* src = take();
+        if (!src) continue;
+        copy(kbuf + (size_t)s * sh.kpart, src, sh.kpart, &kfull[s]);
+        copy(vbuf + (size_t)s * sh.vpart, src + sh.kpart, sh.vpart, &vfull[s]);
+        there |= 1u << s;
     }
 
-    const int gid = lane >> 2, tig = lane & 3, slabs = sh.dp / 32, vslabs = sh.vp / 32;
-    uint32_t i = 0;  // pages of this CTA so far
-    for (long long u = u0; u < u1;) {
-        const Segment sg = segment_at(a, first, items, u, u1);
-        const int kvh = sg.item / tiles, tile = sg.item - kvh * tiles, pairs = min(PAIRS, group - tile * PAIRS), head0 = kvh * group + tile * PAIRS;
-        const int len = row_len(a, sg.m);
-        consumers_sync();  // the segment in front has read its queries
-        {                  // warp w: the queries of pair w, eight elements a lane
-            const int d0 = lane * 8;
-            float x[8];
-            uint32_t top = 0;
+    // ---- queries: warp w has pair w, eight elements a lane; they are fetched a segment ahead ----
+    static_assert(WARPS >= PAIRS, "a warp for every pair");
+    auto fetch_query = [&](const Segment& of, float (&x)[8]) {
+        const int kvh = of.item / tiles, tile = of.item - kvh * tiles, d0 = lane * 8;
+#pragma unroll
+        for (int e = 0; e < 8; ++e) x[e] = 0.f;
+        if (warp >= min(PAIRS, group - tile * PAIRS) || d0 >= a.pool.dim) return;
+        const size_t at = (size_t)of.m * a.ldq + (size_t)(kvh * group + tile * PAIRS + warp) * a.pool.dim + d0;
+        if (wide & 2) {
+            float y[4], z[4];
+            load_row<BF16, 4>(a.q, at, y);
+            load_row<BF16, 4>(a.q, at + 4, z);
+#pragma unroll
+            for (int e = 0; e < 8; ++e) x[e] = e < 4 ? y[e & 3] : z[e & 3];
+        } else {
 #pragma unroll
             for (int e = 0; e < 8; ++e) {
                 float one[1] = {0.f};
-                if (warp < pairs && d0 + e < a.pool.dim) load_row<BF16, 1>(a.q, (size_t)sg.m * a.ldq + (size_t)(head0 + warp) * a.pool.dim + d0 + e, one);
+                if (d0 + e < a.pool.dim) load_row<BF16, 1>(a.q, at + e, one);
                 x[e] = one[0];
-                top = max(top, __float_as_uint(one[0]) & 0x7FFFFFFFu);
             }
-            top = __reduce_max_sync(0xffffffffu, top);
-            const int ex = top >= 0x7F800000u ? 127 + UP : max((int)(top >> 23), LEAST_EXP);
-            const float up = pow2_bits(254 + UP - ex);
-            if (d0 < sh.dp) {
-#pragma unroll
-                for (int h = 0; h < 2; ++h) {
-                    uint4 f;
-                    split_f16(x[4 * h] * up, x[4 * h + 1] * up, f.x, f.y);
-                    split_f16(x[4 * h + 2] * up, x[4 * h + 3] * up, f.z, f.w);
-                    qf[(2 * (lane >> 2) + h) * 32 + warp * 4 + (lane & 3)] = f;
-                }
-            }
-            if (lane == 0) s_c[warp] = a.scale * LOG2E * exp2f((float)(ex - 127 - UP));
         }
-        consumers_sync();
-        const float c = s_c[gid];
-        float mx = -INFINITY, l = 0.f, o[VS][4][2];
-        float ve = LEAST_EXP, largest = LEAST_EXP;  // exponent field of the unit of o, which follows the largest W so far (the exponent of that, as it was rounded down)
+    };
+    auto put_query = [&](const float (&x)[8], int buffer) {  // as digits, in the order of the MMAs' operands
+        if (warp >= PAIRS) return;
+        uint32_t top = 0;
 #pragma unroll
-        for (int s = 0; s < VS; ++s)
+        for (int e = 0; e < 8; ++e) top = max(top, __float_as_uint(x[e]) & 0x7FFFFFFFu);
+        top = __reduce_max_sync(0xffffffffu, top);
+        const float most = __uint_as_float(top);
+        const bool some = top < 0x7F800000u && most >= Q_TINY;
+        const int ex = (int)(top >> 23);  // f32: a power of two brings the largest to 2^29 .. 2^30
+        const float up = !some ? 0.f : BF16 ? Q_MOST / most : pow2_bits(127 + 29 - (ex - 127)), down = !some ? 0.f : BF16 ? most / Q_MOST : exp2f((float)(ex - 127 - 29));
+        if (lane * 8 < sh.dp) {
+            uint32_t y[2][4], d[2][2 * PASSES];
 #pragma unroll
-            for (int e = 0; e < 4; ++e) o[s][e][0] = o[s][e][1] = 0.f;
-        const int half = warp & 1;
-        for (int p = (int)(((uint32_t)(warp >> 1) - i) % TURN); p < sg.n; p += TURN) {
-            const int st = (int)((i + p) % stages);
-            if (!__all_sync(0xffffffffu, mb_wait(&full[st], ((i + p) / stages) & 1u, a.err_flag, &s_abort))) break;
-            const int nt = len - ((sg.page + p) * KV8_PAGE + half * 32);  // tokens that are seen
-            if (nt > 0 && s_there[st]) {
-                const unsigned char* block = dyn + (size_t)st * sh.block;
-                const float *ks = reinterpret_cast<const float*>(block) + half * 32, *vs = ks + KV8_PAGE;
-                const unsigned char* kc = block + 8 * KV8_PAGE + (half * 32 + gid) * 32 + tig * 8;
-                const unsigned char* vc = block + 8 * KV8_PAGE + KV8_PAGE * sh.dp + (half * 32 + tig) * 32 + gid * 4;
-                float sc[4][4];
+            for (int e = 0; e < 8; ++e) {
+                const int whole = some ? __float2int_rn(x[e] * up) : 0;
+                y[e >> 2][e & 3] = BF16 ? (uint32_t)(whole + 0x80) ^ 0x80u : (uint32_t)(whole + 0x808080) ^ 0x808080u;  // signed digits
+            }
+            digits_of<2 * PASSES>(y[0], d[0]);
+            digits_of<2 * PASSES>(y[1], d[1]);
 #pragma unroll
-                for (int j = 0; j < 4; ++j) sc[j][0] = sc[j][1] = sc[j][2] = sc[j][3] = 0.f;
-#pragma unroll 2
-                for (int s = 0; s < slabs; ++s) {
-                    const uint4 q0 = qf[2 * s * 32 + lane], q1 = qf[(2 * s + 1) * 32 + lane];
-                    const uint32_t a0[4] = {q0.x, q0.y, q0.z, q0.w}, a1[4] = {q1.x, q1.y, q1.z, q1.w};
+            for (int h = 0; h < PASSES; ++h) {  // the upper two digits first
+                const int k = 2 * (PASSES - 1 - h);
+                queries[buffer * sh.queries + ((lane >> 2) * PASSES + h) * 32 + warp * 4 + (lane & 3)] = make_uint4(d[0][k + 1], d[0][k], d[1][k + 1], d[1][k]);
+            }
+        }
+        if (lane == 0) s_c[buffer][warp] = top < 0x7F800000u ? a.scale * LOG2E * down : __uint_as_float(0x7FC00000u);
+    };
+
+    const int gid = lane >> 2, tig = lane & 3, slabs = sh.dp / 32, vslabs = sh.vp / 32;
+    int i = warp, slot = 0, len = row_len(a, sg.m);  // this warp's next piece, counted over the CTA, and its slot; tokens of the segment's row
+    bool good = true;                                // no wait has run out
+    float next_q[8];
+    fetch_query(sg, next_q);
+    put_query(next_q, 0);
+    __syncthreads();
+    for (int begin = 0, turn = 0; begin < count; turn ^= 1) {
+        const int kvh = sg.item / tiles, tile = sg.item - kvh * tiles, pairs = min(PAIRS, group - tile * PAIRS), head0 = kvh * group + tile * PAIRS;
+        const uint4* qf = queries + turn * sh.queries;
+        const float c = s_c[turn][gid];
+        Segment behind = sg;
+        int len_behind = 0;
+        const bool last = begin + sg.n >= count;
+        if (!last) {
+            next_segment(a, items, behind, count - begin - sg.n);
+            len_behind = row_len(a, behind.m);
+            fetch_query(behind, next_q);
+        }
+        float mx = -INFINITY, l = 0.f, o[VS * 4][2];  // elements 8 i + 2 tig + 0, 1 of pair gid
 #pragma unroll
-                    for (int j = 0; j < 4; ++j) {
-                        const uint2 w = *reinterpret_cast<const uint2*>(kc + s * (KV8_PAGE * 32) + j * 256);
-                        mma_f16(sc[j], a0, codes_f16<0x4140>(w.x), codes_f16<0x4342>(w.x));
-                        mma_f16(sc[j], a1, codes_f16<0x4140>(w.y), codes_f16<0x4342>(w.y));
+        for (int s = 0; s < VS * 4; ++s) o[s][0] = o[s][1] = 0.f;
+        for (; good && i < begin + sg.n; i += WARPS) {
+            const int nt = len - ((sg.at + i - begin) * KV8_HALF + 8 * tig);  // this lane's tokens are 8 tig .. 8 tig + 7: how many of them are seen
+            const bool partial = nt + 8 * tig < KV8_HALF;
+            const unsigned char* next = take();  // the piece that comes into this slot next
+            unsigned char *keys = kbuf + (size_t)slot * sh.kpart, *values = vbuf + (size_t)slot * sh.vpart;
+            if ((there >> slot) & 1u) {
+                const uint32_t parity = (phase >> slot) & 1u;
+                const unsigned char *kc = keys + KV8_HALF * 4 + gid * 32 + tig * 8, *vc = values + KV8_HALF * 4 + gid * 32 + tig * 8;
+                if (!(good = __all_sync(0xffffffffu, mb_wait(&kfull[slot], parity, a.err_flag, &s_abort)))) break;
+                int sc[4][PASSES][4];
+                auto product = [&](int s, auto head) {
+                    uint2 k[4];
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) k[j] = *reinterpret_cast<const uint2*>(kc + s * (KV8_HALF * 32) + j * 256);
+#pragma unroll
+                    for (int h = 0; h < PASSES; ++h) {
+                        const uint4 q = qf[(s * PASSES + h) * 32 + lane];
+#pragma unroll
+                        for (int j = 0; j < 4; ++j) mma_s8<false, decltype(head)::value>(sc[j][h], q, k[j]);
                     }
+                };
+                product(0, std::true_type{});
+#pragma unroll VS <= 4 ? VS : 4
+                for (int s = 1; s < slabs; ++s) product(s, std::false_type{});
+                // column 2 tig + e of tile j is token 8 tig + 2 j + e
+                float w[8], most = -INFINITY;
+#pragma unroll
+                for (int t = 0; t < 8; t += 4) {
+                    const float4 x = *reinterpret_cast<const float4*>(keys + (8 * tig + t) * 4);
+                    w[t] = from_digits<PASSES>(sc[t >> 1], 0) * (x.x * c);
+                    w[t + 1] = from_digits<PASSES>(sc[t >> 1], 1) * (x.y * c);
+                    w[t + 2] = from_digits<PASSES>(sc[(t >> 1) + 1], 0) * (x.z * c);
+                    w[t + 3] = from_digits<PASSES>(sc[(t >> 1) + 1], 1) * (x.w * c);
                 }
-                // column 2 tig + e of tile j is token 8 j + 4 e + tig
-                float w[4][2], most = -INFINITY;
+                __syncwarp();  // the keys have been read: the next ones may come
+                if (next) copy(keys, next, sh.kpart, &kfull[slot]);
+                if (partial)
 #pragma unroll
-                for (int j = 0; j < 4; ++j)
+                    for (int t = 0; t < 8; ++t) w[t] = t < nt ? w[t] : -INFINITY;
 #pragma unroll
-                    for (int e = 0; e < 2; ++e) {
-                        const int t = 8 * j + 4 * e + tig;
-                        const float s = (sc[j][e] + sc[j][2 + e]) * (ks[t] * c);
-                        w[j][e] = t < nt ? s : -INFINITY;
-                        most = fmaxf(most, w[j][e]);
-                    }
+                for (int t = 0; t < 8; ++t) most = fmaxf(most, w[t]);
                 most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, 1));
                 most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, 2));
-                const float now = fmaxf(mx, most), ref = now == -INFINITY ? 0.f : now, corr = exp2f(mx - ref);
-                float top = 0.f;
-                l *= corr;
-#pragma unroll
-                for (int j = 0; j < 4; ++j)
-#pragma unroll
-                    for (int e = 0; e < 2; ++e) {
-                        const int t = 8 * j + 4 * e + tig;
-                        const float pr = exp2f(w[j][e] - ref);
-                        l += pr;
-                        w[j][e] = t < nt ? pr * vs[t] : 0.f;
-                        top = fmaxf(top, w[j][e]);
-                    }
-                top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
-                top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
-                // the unit follows the maximum down and the weights up
-                largest = fmaxf(fmaxf(largest + (mx - ref), (float)(__float_as_uint(top) >> 23)), (float)LEAST_EXP);
-                const float ve_now = ceilf(largest);
-                const float f = corr * exp2f(ve - ve_now), up = pow2_bits(254 + UP - (int)ve_now);
+                const float now = fmaxf(mx, most), ref = now == -INFINITY ? 0.f : now, corr = exp2_ftz(mx - ref);
                 mx = now;
-                ve = ve_now;
-                uint32_t wa[2][4];
+                l *= corr;
+                if (!(good = __all_sync(0xffffffffu, mb_wait(&vfull[slot], parity, a.err_flag, &s_abort)))) {
+                    if (next) mb_land(&kfull[slot], parity ^ 1u);
+                    break;
+                }
+                uint32_t top = 0;  // bits of the largest weight: of NaN where a scale is
+                float sum = 0.f;
 #pragma unroll
-                for (int j = 0; j < 4; ++j) split_f16(w[j][0] * up, w[j][1] * up, wa[j >> 1][(j & 1) * 2], wa[j >> 1][(j & 1) * 2 + 1]);
+                for (int t = 0; t < 8; t += 4) {
+                    const float4 y = *reinterpret_cast<const float4*>(values + (8 * tig + t) * 4);
+                    float v[4] = {y.x, y.y, y.z, y.w};
+                    if (partial)
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) v[e] = t + e < nt ? v[e] : 0.f;
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) {
+                        const float pr = exp2_ftz(w[t + e] - ref);
+                        sum += pr;
+                        w[t + e] = pr * v[e];
+                        top = max(top, __float_as_uint(w[t + e]));
+                    }
+                }
+                l += sum;
+                top = max(top, __shfl_xor_sync(0xffffffffu, top, 1));
+                top = max(top, __shfl_xor_sync(0xffffffffu, top, 2));
+                if (top >= 0x7F800000u) l = __uint_as_float(0x7FC00000u);
+                const int ex = min(max((int)(top >> 23), W_LEAST), 254);
+                // bf16: whole numbers up to 65535, f32: below 2^31, for the largest
+                const float up = BF16 ? pow2_bits(127 + 15 - (ex - 127)) * W_PART : pow2_bits(127 + 30 - (ex - 127)), unit = exp2_ftz((float)(ex - 127 - (BF16 ? 15 : 30))) * (BF16 ? 1.f / W_PART : 1.f);
+                uint4 wa[PASSES];
+                {
+                    uint32_t x[2][4], d[2][2 * PASSES];
+#pragma unroll
+                    for (int t = 0; t < 8; ++t) x[t >> 2][t & 3] = BF16 ? __float_as_uint(fmaf(w[t], up, 8388608.f)) : __float2uint_rn(w[t] * up);
+                    digits_of<2 * PASSES>(x[0], d[0]);
+                    digits_of<2 * PASSES>(x[1], d[1]);
+#pragma unroll
+                    for (int h = 0; h < PASSES; ++h) wa[h] = make_uint4(d[0][2 * (PASSES - 1 - h) + 1], d[0][2 * (PASSES - 1 - h)], d[1][2 * (PASSES - 1 - h) + 1], d[1][2 * (PASSES - 1 - h)]);
+                }
+                if (__any_sync(0xffffffffu, corr != 1.f)) {
+#pragma unroll
+                    for (int s = 0; s < VS * 4; ++s) {
+                        o[s][0] *= corr;
+                        o[s][1] *= corr;
+                    }
+                }
 #pragma unroll
                 for (int s = 0; s < VS; ++s) {
                     if (s >= vslabs) break;
-                    float acc[4][4];
-#pragma unroll
-                    for (int e = 0; e < 4; ++e) acc[e][0] = acc[e][1] = acc[e][2] = acc[e][3] = 0.f;
-#pragma unroll
-                    for (int h = 0; h < 2; ++h) {
-                        uint32_t x[4];
-#pragma unroll
-                        for (int r = 0; r < 4; ++r) x[r] = *reinterpret_cast<const uint32_t*>(vc + s * (KV8_PAGE * 32) + (h * 16 + r * 4) * 32);
-                        const uint32_t p01 = __byte_perm(x[0], x[1], 0x5140), p23 = __byte_perm(x[0], x[1], 0x7362), r01 = __byte_perm(x[2], x[3], 0x5140), r23 = __byte_perm(x[2], x[3], 0x7362);
-                        mma_f16(acc[0], wa[h], codes_f16<0x4140>(p01), codes_f16<0x4140>(r01));
-                        mma_f16(acc[1], wa[h], codes_f16<0x4342>(p01), codes_f16<0x4342>(r01));
-                        mma_f16(acc[2], wa[h], codes_f16<0x4140>(p23), codes_f16<0x4140>(r23));
-                        mma_f16(acc[3], wa[h], codes_f16<0x4342>(p23), codes_f16<0x4342>(r23));
-                    }
 #pragma unroll
                     for (int e = 0; e < 4; ++e) {
-                        o[s][e][0] = fmaf(o[s][e][0], f, acc[e][0] + acc[e][2]);
-                        o[s][e][1] = fmaf(o[s][e][1], f, acc[e][1] + acc[e][3]);
+                        const uint2 v = *reinterpret_cast<const uint2*>(vc + (s * 4 + e) * (8 * KV8_HALF));
+                        int acc[PASSES][4];
+#pragma unroll
+                        for (int h = 0; h < PASSES; ++h) mma_s8<true, true>(acc[h], wa[h], v);
+                        o[s * 4 + e][0] = fmaf(from_digits<PASSES>(acc, 0), unit, o[s * 4 + e][0]);
+                        o[s * 4 + e][1] = fmaf(from_digits<PASSES>(acc, 1), unit, o[s * 4 + e][1]);
                     }
                 }
+                __syncwarp();
+                phase ^= 1u << slot;
+            } else if (next) {
+                copy(keys, next, sh.kpart, &kfull[slot]);
             }
-            __syncwarp();
-            if (lane == 0) mb_arrive(&empty[st]);
+            if (next) copy(values, next + sh.kpart, sh.vpart, &vfull[slot]);
+            there = (there & ~(1u << slot)) | (next ? 1u << slot : 0u);
+            slot = slot + 1 == depth ? 0 : slot + 1;
         }
-        i += sg.n;
-        u += sg.n;
 
-        // ---- the warps' results added up: first those of warps 4 .. 7 to those of 0 .. 3, then these four ----
+        // ---- the warps' results added up: `slots` warps at a time to those of the first `slots` warps, then these ----
         l += __shfl_xor_sync(0xffffffffu, l, 1);
         l += __shfl_xor_sync(0xffffffffu, l, 2);
-        const float down = exp2f(ve - (127 + UP));
-#pragma unroll
-        for (int s = 0; s < VS; ++s)
-#pragma unroll
-            for (int e = 0; e < 4; ++e) {
-                o[s][e][0] *= down;
-                o[s][e][1] *= down;
-            }
-        const int slot = warp & (WARPS / 2 - 1);
-        float* mine = merge + ((size_t)slot * PAIRS + gid) * sh.ldo + tig * 8;  // elements 8 tig + 4 e + 0 .. 3 of a slab
+        const int room = pairs <= 2 ? 2 : pairs <= 4 ? 4 : PAIRS, slots = min(WARPS, MERGE_ROWS / room);
+        const int row = warp % slots * room + gid;
+        float* mine = merge + (size_t)row * sh.ldo + tig * 2;
         auto put = [&]() {
+            if (gid >= pairs) return;
             if (tig == 0) {
-                s_m[slot][gid] = mx;
-                s_l[slot][gid] = l;
+                s_m[row] = mx;
+                s_l[row] = l;
             }
 #pragma unroll
-            for (int s = 0; s < VS; ++s) {
-                if (s >= vslabs) break;
-#pragma unroll
-                for (int e = 0; e < 2; ++e) *reinterpret_cast<float4*>(mine + s * 32 + 4 * e) = make_float4(o[s][0][e], o[s][1][e], o[s][2][e], o[s][3][e]);
+            for (int s = 0; s < VS * 4; ++s) {
+                if (s >= vslabs * 4) break;
+                *reinterpret_cast<float2*>(mine + s * 8) = make_float2(o[s][0], o[s][1]);
             }
         };
-        if (warp >= WARPS / 2) put();
-        consumers_sync();
-        if (warp < WARPS / 2) {
-            const float om = s_m[slot][gid], now = fmaxf(mx, om), ref = now == -INFINITY ? 0.f : now, f0 = exp2f(mx - ref), f1 = exp2f(om - ref);
-            l = fmaf(l, f0, s_l[slot][gid] * f1);
-            mx = now;
+        if (begin > 0)  // the sums of the segment in front have been read by all
+            good = __all_sync(0xffffffffu, mb_wait(&s_added, turn ^ 1, a.err_flag, &s_abort)) && good;
+        for (int w0 = slots; w0 < WARPS; w0 += slots) {
+            if (warp >= w0 && warp < w0 + slots) put();
+            __syncthreads();
+            if (warp < slots && warp + w0 < WARPS && gid < pairs) {
+                const float om = s_m[row], now = fmaxf(mx, om), ref = now == -INFINITY ? 0.f : now, f0 = exp2f(mx - ref), f1 = exp2f(om - ref);
+                l = fmaf(l, f0, s_l[row] * f1);
+                mx = now;
 #pragma unroll
-            for (int s = 0; s < VS; ++s) {
-                if (s >= vslabs) break;
-#pragma unroll
-                for (int e = 0; e < 2; ++e) {
-                    const float4 x = *reinterpret_cast<const float4*>(mine + s * 32 + 4 * e);
-                    o[s][0][e] = fmaf(o[s][0][e], f0, x.x * f1);
-                    o[s][1][e] = fmaf(o[s][1][e], f0, x.y * f1);
-                    o[s][2][e] = fmaf(o[s][2][e], f0, x.z * f1);
-                    o[s][3][e] = fmaf(o[s][3][e], f0, x.w * f1);
+                for (int s = 0; s < VS * 4; ++s) {
+                    if (s >= vslabs * 4) break;
+                    const float2 x = *reinterpret_cast<const float2*>(mine + s * 8);
+                    o[s][0] = fmaf(o[s][0], f0, x.x * f1);
+                    o[s][1] = fmaf(o[s][1], f0, x.y * f1);
                 }
             }
-            __syncwarp();
-            put();
+            __syncthreads();
         }
-        consumers_sync();
+        if (warp < slots) put();
+        if (!last) put_query(next_q, turn ^ 1);
+        __syncthreads();
         const bool whole = sg.n == sg.of;
-        float* part = static_cast<float*>(a.work) + (size_t)(2 * blockIdx.x + (sg.page == 0)) * part_floats(sh.vp);
-        for (int k = tid; k < pairs * (sh.vp / 4); k += WARPS * 32) {
+        float* part = cta_part(a, sh.vp, blockIdx.x, sg.at == 0);
+        for (int k = tid; k < pairs * (sh.vp / 4); k += THREADS) {
             const int pr = k / (sh.vp / 4), d = (k - pr * (sh.vp / 4)) * 4;
-            float f[WARPS / 2], top = -INFINITY, sum = 0.f, v[4] = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-            for (int w = 0; w < WARPS / 2; ++w) top = fmaxf(top, s_m[w][pr]);
+            float top = -INFINITY, sum = 0.f, v[4] = {0.f, 0.f, 0.f, 0.f};
+            for (int w = 0; w < slots; ++w) top = fmaxf(top, s_m[w * room + pr]);
             const float ref = top == -INFINITY ? 0.f : top;
-#pragma unroll
-            for (int w = 0; w < WARPS / 2; ++w) {
-                f[w] = exp2f(s_m[w][pr] - ref);
-                const float4 x = *reinterpret_cast<const float4*>(merge + ((size_t)w * PAIRS + pr) * sh.ldo + d);
-                v[0] = fmaf(f[w], x.x, v[0]); v[1] = fmaf(f[w], x.y, v[1]); v[2] = fmaf(f[w], x.z, v[2]); v[3] = fmaf(f[w], x.w, v[3]);
-                sum = fmaf(f[w], s_l[w][pr], sum);
+#pragma unroll 4
+            for (int w = 0; w < slots; ++w) {
+                const float f = exp2f(s_m[w * room + pr] - ref);
+                const float4 x = *reinterpret_cast<const float4*>(merge + (size_t)(w * room + pr) * sh.ldo + d);
+                v[0] = fmaf(f, x.x, v[0]); v[1] = fmaf(f, x.y, v[1]); v[2] = fmaf(f, x.z, v[2]); v[3] = fmaf(f, x.w, v[3]);
+                sum = fmaf(f, s_l[w * room + pr], sum);
             }
             if (whole) {
                 const float inv = sum == 0.f ? 0.f : 1.0f / sum;
-#pragma unroll
-                for (int e = 0; e < 4; ++e) v[e] *= inv;
-                if (d < a.pool.vdim) store4<BF16>(a, sg.m, head0 + pr, d, v, wide);
+                store2<BF16>(a, sg.m, head0 + pr, d, v[0] * inv, v[1] * inv, wide & 1);
+                store2<BF16>(a, sg.m, head0 + pr, d + 2, v[2] * inv, v[3] * inv, wide & 1);
             } else {
                 float* at = part + (size_t)pr * (sh.vp + 4);
                 *reinterpret_cast<float4*>(at + 4 + d) = make_float4(v[0], v[1], v[2], v[3]);
@@ -441,43 +551,93 @@ __global__ void __launch_bounds__(THREADS, VS <= 4 ? 2 : 1) kv8_stream_kernel(co
                 }
             }
         }
+        __syncwarp();
+        if (lane == 0) mb_arrive(&s_added);
+        begin += sg.n;
+        sg = behind;
+        len = len_behind;
     }
+    // every copy has been waited for, unless a wait ran out: then what is still on its way has to land before this CTA's shared memory is another's
+    if (!good)
+        for (int s = 0; s < depth; ++s) {
+            if (!((there >> s) & 1u)) continue;
+            mb_land(&kfull[s], (phase >> s) & 1u);
+            mb_land(&vfull[s], (phase >> s) & 1u);
+        }
 }
 
-// One CTA per cut of the line: the item that a cut falls into, if the CTA in front of the cut holds its beginning.
-template <bool BF16>
-__global__ void __launch_bounds__(THREADS) kv8_join_kernel(const Kv8AttnArgs a, int tiles, int wide) {
-    extern __shared__ int first[];
-    const int tid = threadIdx.x, items = a.pool.kv_heads * tiles, group = a.heads / a.pool.kv_heads, ctas = gridDim.x + 1, cut = blockIdx.x + 1, vp = kv8_pad(a.pool.vdim);
-    const Line line = make_line(a, items, ctas, first);
+// One CTA per cut of the line: the item that a cut falls into, if the CTA in front of the cut holds its beginning.  A long context has a hundred parts and
+// more: the warps share them, every lane with its elements of all pairs of a part in flight at once.
+constexpr int JOIN_THREADS = 288;
+template <bool BF16, int VS>
+__global__ void __launch_bounds__(JOIN_THREADS) kv8_join_kernel(const Kv8AttnArgs a, int tiles, int wide) {
+    constexpr int THREADS = JOIN_THREADS, JW = THREADS / 32, NI = PAIRS * VS * 8 / 32;  // warps; groups of four elements a lane
+    extern __shared__ __align__(128) unsigned char dyn[];       // factors [parts][PAIRS], then the warps' sums
+    __shared__ float s_inv[PAIRS];
+    __shared__ int first[THREADS + 1];
+    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, items = a.pool.kv_heads * tiles, group = a.heads / a.pool.kv_heads, ctas = gridDim.x + 1, cut = blockIdx.x + 1, vp = kv8_pad(a.pool.vdim), quads = vp / 4;
+    const Line line = make_line<THREADS>(a, items, ctas, first);
     pdl_wait();
     const long long u = cut * line.chunk;
     if (u >= line.total) return;
-    const Segment sg = segment_at(a, first, items, u, line.total);
-    if (sg.page == 0) return;
-    const long long begin = u - sg.page, end = begin + sg.of;
-    if (begin / line.chunk != cut - 1) return;
-    const int last = (int)((end - 1) / line.chunk), kvh = sg.item / tiles, tile = sg.item - kvh * tiles, pairs = min(PAIRS, group - tile * PAIRS), head0 = kvh * group + tile * PAIRS;
-    const float* work = static_cast<const float*>(a.work);
-    for (int k = tid; k < pairs * (vp / 4); k += THREADS) {
-        const int pr = k / (vp / 4), d = (k - pr * (vp / 4)) * 4;
-        // the beginning is the second part of its CTA, what follows the first of theirs
-        auto part = [&](int c) { return work + (size_t)(2 * c + (c == cut - 1)) * part_floats(vp) + (size_t)pr * (vp + 4); };
-        float top = -INFINITY, sum = 0.f, v[4] = {0.f, 0.f, 0.f, 0.f};
-        for (int c = cut - 1; c <= last; ++c) top = fmaxf(top, __ldcg(part(c)));
+    const Segment sg = segment_at<THREADS>(a, first, items, u, line.total);
+    const long long begin = u - sg.at, end = begin + sg.of;
+    if (sg.at == 0 || begin / line.chunk != cut - 1) return;
+    const int parts = (int)((end - 1) / line.chunk) - (cut - 1) + 1, kvh = sg.item / tiles, tile = sg.item - kvh * tiles, pairs = min(PAIRS, group - tile * PAIRS), head0 = kvh * group + tile * PAIRS;
+    // the beginning is the second part of its CTA, what follows the first of theirs
+    auto part = [&](int i) -> const float* { return cta_part(a, vp, cut - 1 + i, i == 0); };
+    float* factor = reinterpret_cast<float*>(dyn);
+    float4* sums = reinterpret_cast<float4*>(dyn + (sizeof(float) * PAIRS * parts + 15) / 16 * 16);  // [JW][NI * 32]
+    for (int k = tid; k < parts * PAIRS; k += THREADS) factor[k] = k % PAIRS < pairs ? __ldcg(part(k / PAIRS) + (size_t)(k % PAIRS) * (vp + 4)) : -INFINITY;
+    __syncthreads();
+    if (warp < PAIRS) {  // warp w: pair w
+        float top = -INFINITY, sum = 0.f;
+        for (int i = lane; i < parts; i += 32) top = fmaxf(top, factor[i * PAIRS + warp]);
+        top = warp_max(top);
         const float ref = top == -INFINITY ? 0.f : top;
-#pragma unroll 4
-        for (int c = cut - 1; c <= last; ++c) {
-            const float* at = part(c);
-            const float f = exp2f(__ldcg(at) - ref);
-            const float4 x = __ldcg(reinterpret_cast<const float4*>(at + 4 + d));
-            sum = fmaf(f, __ldcg(at + 1), sum);
-            v[0] = fmaf(f, x.x, v[0]); v[1] = fmaf(f, x.y, v[1]); v[2] = fmaf(f, x.z, v[2]); v[3] = fmaf(f, x.w, v[3]);
+        for (int i = lane; i < parts; i += 32) {
+            const float f = exp2f(factor[i * PAIRS + warp] - ref);
+            factor[i * PAIRS + warp] = f;
+            if (warp < pairs) sum = fmaf(f, __ldcg(part(i) + (size_t)warp * (vp + 4) + 1), sum);
         }
-        const float inv = sum == 0.f ? 0.f : 1.0f / sum;
+        sum = warp_sum(sum);
+        if (lane == 0) s_inv[warp] = sum == 0.f ? 0.f : 1.0f / sum;
+    }
+    __syncthreads();
+    float4 acc[NI];
+    int off[NI];  // where a lane's groups stand in a part
 #pragma unroll
-        for (int e = 0; e < 4; ++e) v[e] *= inv;
-        if (d < a.pool.vdim) store4<BF16>(a, sg.m, head0 + pr, d, v, wide);
+    for (int n = 0; n < NI; ++n) {
+        const int k = lane + 32 * n, pr = k / quads;
+        acc[n] = make_float4(0.f, 0.f, 0.f, 0.f);
+        off[n] = pr < pairs ? pr * (vp + 4) + 4 + (k - pr * quads) * 4 : -1;
+    }
+    for (int i = warp; i < parts; i += JW) {
+        const float* at = part(i);
+        float4 x[NI];
+#pragma unroll
+        for (int n = 0; n < NI; ++n) x[n] = off[n] >= 0 ? __ldcg(reinterpret_cast<const float4*>(at + off[n])) : make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+        for (int n = 0; n < NI; ++n) {
+            const float f = factor[i * PAIRS + (lane + 32 * n) / quads % PAIRS];
+            acc[n].x = fmaf(f, x[n].x, acc[n].x); acc[n].y = fmaf(f, x[n].y, acc[n].y); acc[n].z = fmaf(f, x[n].z, acc[n].z); acc[n].w = fmaf(f, x[n].w, acc[n].w);
+        }
+    }
+#pragma unroll
+    for (int n = 0; n < NI; ++n) sums[(warp * NI + n) * 32 + lane] = acc[n];
+    __syncthreads();
+    for (int k = tid; k < pairs * quads; k += THREADS) {
+        const int pr = k / quads, d = (k - pr * quads) * 4;
+        float v[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int w = 0; w < JW; ++w) {
+            const float4 x = sums[w * NI * 32 + k];
+            v[0] += x.x; v[1] += x.y; v[2] += x.z; v[3] += x.w;
+        }
+#pragma unroll
+        for (int e = 0; e < 4; ++e) v[e] *= s_inv[pr];
+        store2<BF16>(a, sg.m, head0 + pr, d, v[0], v[1], wide & 1);
+        store2<BF16>(a, sg.m, head0 + pr, d + 2, v[2], v[3], wide & 1);
     }
 }
 
@@ -496,34 +656,42 @@ cudaError_t launch_behind(void (*kern)(KArgs...), int grid, int threads, size_t 
     return cudaLaunchKernelEx(&cfg, kern, KArgs(args)...);
 }
 
-template <bool BF16, int VS>
+template <bool BF16, int VS, int WARPS>
 cudaError_t launch_stream(const Kv8AttnArgs& a, int sm_count, cudaStream_t st) {
-    const int group = a.heads / a.pool.kv_heads, tiles = (group + PAIRS - 1) / PAIRS, size = BF16 ? 2 : 4;
-    const int wide = a.pool.vdim % 4 == 0 && (((uintptr_t)a.out | a.ldo * size) & (4 * size - 1)) == 0;
-    auto bytes = [&](int stages) { return stream_shape(a.pool.dim, a.pool.vdim, a.M, stages).bytes; };
-    // two CTAs per SM where registers (VS) and shared memory let them
-    const int per_sm = VS <= 4 && bytes(TURN) <= ROOM / 2 ? 2 : 1, ctas = per_sm * sm_count;
-    int stages = MAX_STAGES;
-    while (stages > TURN && bytes(stages) > ROOM / per_sm) stages -= TURN;
-    const size_t smem = bytes(stages);
-    cudaError_t e = ensure_dyn_smem(kv8_stream_kernel<BF16, VS>, smem);
-    if (e == cudaSuccess) e = ensure_dyn_smem(kv8_join_kernel<BF16>, sizeof(int) * (a.M + 1));
+    const int group = a.heads / a.pool.kv_heads, tiles = (group + PAIRS - 1) / PAIRS, size = BF16 ? 2 : 4, ctas = sm_count;
+    // bit 0: results in pairs, bit 1: queries in groups of four
+    const int wide = (a.pool.vdim % 2 == 0 && (((uintptr_t)a.out | a.ldo * size) & (2 * size - 1)) == 0 ? 1 : 0) | (a.pool.dim % 8 == 0 && (((uintptr_t)a.q | a.ldq * size) & (4 * size - 1)) == 0 ? 2 : 0);
+    auto bytes = [&](int depth) { return stream_shape(a.pool.dim, a.pool.vdim, BF16 ? 1 : 2, WARPS, depth).bytes; };
+    int depth = MAX_DEPTH;
+    while (depth > 1 && bytes(depth) > ROOM) --depth;
+    const size_t smem = bytes(depth), join_smem = sizeof(float) * PAIRS * ctas + 16 + sizeof(float) * JOIN_THREADS * PAIRS * VS;
+    cudaError_t e = ensure_dyn_smem(kv8_stream_kernel<BF16, VS, WARPS>, smem);
+    if (e == cudaSuccess) e = ensure_dyn_smem(kv8_join_kernel<BF16, VS>, join_smem);
     if (e != cudaSuccess) return e;
-    kv8_stream_kernel<BF16, VS><<<(unsigned)ctas, THREADS, smem, st>>>(a, stages, tiles, wide);
+    kv8_stream_kernel<BF16, VS, WARPS><<<(unsigned)ctas, WARPS * 32, smem, st>>>(a, depth, tiles, wide);
     if ((e = cudaGetLastError()) != cudaSuccess) return e;
-    return launch_behind(kv8_join_kernel<BF16>, ctas - 1, THREADS, sizeof(int) * (a.M + 1), st, a, tiles, wide);
+    return launch_behind(kv8_join_kernel<BF16, VS>, ctas - 1, JOIN_THREADS, join_smem, st, a, tiles, wide);
+}
+
+// 12 warps (168 registers a thread) where their pieces fit, else eight.
+template <bool BF16, int VS>
+cudaError_t launch_warps(const Kv8AttnArgs& a, int sm_count, cudaStream_t st) {
+    auto fits = [&](int warps) { return stream_shape(a.pool.dim, a.pool.vdim, BF16 ? 1 : 2, warps, 1).bytes <= ROOM; };
+    if constexpr (VS <= 4)
+        if (fits(12)) return launch_stream<BF16, VS, 12>(a, sm_count, st);
+    return launch_stream<BF16, VS, 8>(a, sm_count, st);
 }
 
 template <bool BF16>
 cudaError_t launch_typed(const Kv8AttnArgs& a, int sm_count, cudaStream_t st) {
-    if (a.pool.vdim <= 64) return launch_stream<BF16, 2>(a, sm_count, st);
-    if (a.pool.vdim <= 128) return launch_stream<BF16, 4>(a, sm_count, st);
-    return launch_stream<BF16, 8>(a, sm_count, st);
+    if (a.pool.vdim <= 64) return launch_warps<BF16, 2>(a, sm_count, st);
+    if (a.pool.vdim <= 128) return launch_warps<BF16, 4>(a, sm_count, st);
+    return launch_warps<BF16, 8>(a, sm_count, st);
 }
 
 }  // namespace
 
-size_t kv8_attn_bytes(int, int vdim, int, int, int, int sm_count) { return sizeof(float) * 2 * 2 * (size_t)sm_count * part_floats(kv8_pad(vdim)); }
+size_t kv8_attn_bytes(int, int vdim, int, int, int, int sm_count) { return sizeof(float) * 2 * (size_t)sm_count * part_floats(kv8_pad(vdim)); }
 
 cudaError_t launch_kv8_attn(const Kv8AttnArgs& a, int sm_count, cudaStream_t st) { return a.bf16 ? launch_typed<true>(a, sm_count, st) : launch_typed<false>(a, sm_count, st); }
 

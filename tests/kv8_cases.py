@@ -32,13 +32,14 @@ def held(x):
 
 def attention(q, ks, vs, scale):
     """q [heads, dim], ks [tokens, kv_heads, dim], vs [tokens, kv_heads, vdim] (f64) -> out [heads, vdim], and what the bound is made of: the sum of weighted magnitudes
-    [heads, vdim], the largest sum of magnitudes of a score's terms [heads], the granules of queries (in scores) and of weights (in results) [heads]."""
+    [heads, vdim], the largest sum of magnitudes of a score's terms [heads], the largest sum of a score's terms with the queries' largest
+    element in every place [heads], the weighted largest magnitudes of the values [heads]."""
     H, G = q.shape[0], ks.shape[1]
     if ks.shape[0] == 0:
         z = np.zeros((H, vs.shape[2]))
         return z, (z, np.zeros(H), np.zeros(H), np.zeros(H))
     group = H // G
-    out, mag, terms, fine_q, fine_w = [], [], [], [], []
+    out, mag, terms, full, wide = [], [], [], [], []
     for h in range(H):
         k, v = ks[:, h // group], vs[:, h // group]
         s = scale * (k @ q[h])
@@ -47,21 +48,20 @@ def attention(q, ks, vs, scale):
         out.append(p @ v)
         mag.append(p @ np.abs(v))
         terms.append(abs(scale) * (np.abs(k) @ np.abs(q[h])).max())
-        fine_q.append(abs(scale) * np.abs(q[h]).max() * np.abs(k).sum(-1).max())
-        fine_w.append(len(p) * (p * np.abs(v).max(-1)).max())
-    return np.array(out), (np.array(mag), np.array(terms), np.array(fine_q), np.array(fine_w))
+        full.append(abs(scale) * np.abs(q[h]).max() * np.abs(k).sum(-1).max())
+        wide.append((p * np.abs(v).max(-1)).sum())
+    return np.array(out), (np.array(mag), np.array(terms), np.array(full), np.array(wide))
 
 
 def bound(out, parts, bf16):
-    """Scores: products of a value's f16 terms (2^-22 of it) and codes are exact, a chain of at most 16 truncating sums of 2^-23 and a few roundings: 2^-18.9 of the terms'
-    magnitudes; a weight is off by that much twice (itself and the sum it is divided by).  Weights: f16 terms 2^-22, sums of at most 64 tokens by truncation, partial results
-    by roundings: 2^-18.  f16 has no step below 2^-24: the second term of a query whose row's largest is at least 2^14 ends at 2^-39 of that, and the second term of a weight
-    whose pair's largest (times its value scale, 127 of which are the token's largest value) is at least 2^13 at 2^-38 of that, for each token.  bf16 rows: weights may be one
-    f16 term (2^-11), the result is rounded (2^-8)."""
-    mag, terms, fine_q, fine_w = parts
-    e = 2 * (terms * 2.0**-18.9 + fine_q * 2.0**-39)[..., None] + 2.0**-18
-    tol = mag * e + fine_w[..., None] * 2.0**-38 + 1e-37
-    return tol + mag * 2.0**-11 + np.abs(out) * 2.0**-8 if bf16 else tol
+    """Scores: sums of digits times codes are exact; a query's element is off by half of the last digit's step, 2^-30 (bf16 rows: 1 / 32639 / 2) of its largest one, the
+    digits' sums and the factors are f32: together 2^-21 of the terms' magnitudes.  A weight is off by twice what its score is (itself and the sum it is divided by), and by half a
+    step of its digits: 2^-31 (bf16 rows: 2^-16) of the largest weight times value among 32 tokens, so that these 32 are off by at most 2^-26 (2^-11) of the sum of their
+    weights times their largest values.  The exponential and f32 sums over at most a few hundred parts: 2^-18.  bf16 results are rounded (2^-8)."""
+    mag, terms, full, wide = parts
+    e = 2 * (terms * 2.0**-21 + full * (2.0**-15.9 if bf16 else 2.0**-30))[..., None] + 2.0**-18
+    tol = mag * e + wide[..., None] * (2.0**-11 if bf16 else 2.0**-26) + 1e-37
+    return tol + np.abs(out) * 2.0**-8 if bf16 else tol
 
 
 class Model:
