@@ -1593,7 +1593,7 @@ static bool bad_kv8_attn(const hm_kv8* c, int M, int heads, int n_shared) {
 
 size_t hm_kv8_attn_bytes(const hm_kv8* cache, int M, int heads, int n_shared) {
     if (!cache || bad_kv8(cache->kv_heads, cache->dim, cache->vdim, 1) || bad_kv8_attn(cache, M, heads, n_shared)) return 0;
-    return kv8_attn_bytes(cache->kv_heads, cache->vdim, M, heads, n_shared, sm_count_of_current_device());
+    return kv8_attn_bytes(cache->kv_heads, cache->dim, cache->vdim, M, heads, n_shared, sm_count_of_current_device());
 }
 
 int hm_kv8_attn(const hm_kv8* cache, const void* q, int dtype, size_t ldq, const int32_t* row_seq, const int32_t* row_pos, int M, int heads, float scale, const int32_t* shared_pages, int n_shared, void* out, size_t ldo, void* work,
@@ -1629,7 +1629,7 @@ int hm_kv8_attn(const hm_kv8* cache, const void* q, int dtype, size_t ldq, const
     a.scale = scale;
     a.shared = sg.in(shared_pages, (size_t)n_shared);
     a.n_shared = n_shared;
-    a.work = work ? work : sg.scratch(kv8_attn_bytes(cache->kv_heads, cache->vdim, M, heads, n_shared, sms), false);
+    a.work = work ? work : sg.scratch(kv8_attn_bytes(cache->kv_heads, cache->dim, cache->vdim, M, heads, n_shared, sms), false);
     if (!a.pool.page_table || !a.q || !a.out || !a.row_seq || !a.row_pos || (n_shared > 0 && !a.shared) || !a.work) return sg.finish(cudaErrorMemoryAllocation);
     if (sg.elsewhere()) return gfail(HM_ERR_INVALID, "hm_kv8_attn: memory of another device than the current one");
     if (!sg.ok(get_wait_err(&a.err_flag))) return sg.finish(cudaSuccess);

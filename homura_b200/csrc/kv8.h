@@ -1,4 +1,4 @@
-// A paged cache of keys and values in 8 bits (kv8.cu) and attention over it (kv8_attn.cu).
+// A paged cache of keys and values in 8 bits (kv8.cu) and attention over it (kv8_attn.cu, kv8_prefix.cu).
 #pragma once
 #include <cuda_runtime.h>
 #include <stddef.h>
@@ -62,8 +62,21 @@ struct Kv8AttnArgs {
     int n_shared;
     void* work;
     int* err_flag;
+    // filled in by the launcher
+    int solo;                // items of at most so many pieces are a warp's own
+    int own_from;            // the rows' own pieces (halves of pages) begin here: what stands in front is in `prefix`
+    const float* prefix;     // [prefix_n parts][kv_heads][M * heads / kv_heads][padded vdim + 4]: reference and sum of a pair, then from the fifth on its elements
+    int prefix_n;
 };
+// How the shared pages are taken on their own (kv8_prefix.cu): tiles of 128 (row, head) pairs, or of 256, times splits of the pages.
+struct Kv8Prefix {
+    int paired, groups, splits, cluster;
+    int parts;               // splits / cluster; 0: they are taken with the rows' own
+};
+Kv8Prefix kv8_prefix_plan(int kv_heads, int dim, int vdim, int bf16, int M, int heads, int n_shared, int sm_count);
+int kv8_prefix_most_parts(int kv_heads, int M, int heads, int n_shared, int sm_count);  // of any plan
+cudaError_t launch_kv8_prefix(const Kv8AttnArgs& a, const Kv8Prefix& p, float* parts, cudaStream_t st);
 cudaError_t launch_kv8_attn(const Kv8AttnArgs& a, int sm_count, cudaStream_t st);
-size_t kv8_attn_bytes(int kv_heads, int vdim, int M, int heads, int n_shared, int sm_count);
+size_t kv8_attn_bytes(int kv_heads, int dim, int vdim, int M, int heads, int n_shared, int sm_count);
 
 }  // namespace hm

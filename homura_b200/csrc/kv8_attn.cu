@@ -1,6 +1,7 @@
 // Softmax attention over the 8-bit paged cache:
 //   out[row, head] = sum over the positions t <= row_pos whose page exists of softmax_t(scale q . k_t) v_t,   zeros where there is no such position.
-// Page i of a row is shared[i] for i < n_shared and its sequence's page table entry behind them.
+// Page i of a row is shared[i] for i < n_shared and its sequence's page table entry behind them.  Where there is more than one item of rows, the shared pages are taken on their own
+// (kv8_prefix.cu), and what follows here begins behind them and joins both.
 //
 // kv8_stream_kernel   rows' contexts, eight (row, head) pairs of one key/value head at a time; bound by the bytes of the cache
 // kv8_join_kernel     joins the parts of contexts that several CTAs share
@@ -18,7 +19,8 @@
 //
 // Work.  The pieces of all rows, heads and tiles of eight pairs stand in one line, which the CTAs cut into equal lengths: contexts of any lengths keep all SMs busy to the
 // end, and no length needs to be known on the host.  A CTA's warps take its pieces in turn, each with a ring of copies of its own; what they have of an item is added up in shared
-// memory.  The CTA writes the items that it has as a whole and leaves the rest (its first and its last) in `work`, for kv8_join_kernel.
+// memory.  The CTA writes the items that it has as a whole and leaves the rest (its first and its last) in `work`, for kv8_join_kernel.  Items of a few pieces are not worth a CTA's
+// attention (adding up and two barriers take some 5 us): they are no part of the line, and every warp takes some of them alone before it joins in.
 // Slower where tried, at 64 sequences of up to 8000 tokens (93 us with each of them): a range of pieces for every warp, which then has more partial items than are worth joining; whole
 // pages for a warp, of which 12 do not fit twice; 16 warps with one piece each.
 #include "kv8.h"
@@ -43,13 +45,20 @@ constexpr float LOG2E = 1.4426950408889634f;
 // ---- the line of pieces ------------------------------------------------------------------------------
 struct Line {
     long long total, chunk;  // pieces of all items; of a CTA
+    bool solo;               // there are items of a few pieces
 };
 
 __device__ __forceinline__ int row_len(const Kv8AttnArgs& a, int m) {
     const int seq = __ldg(a.row_seq + m);
     return (unsigned)seq < (unsigned)a.pool.n_seq ? min(__ldg(a.row_pos + m), a.pool.max_pages * KV8_PAGE - 1) + 1 : 0;
 }
-__device__ __forceinline__ int row_pieces(const Kv8AttnArgs& a, int m) { return max(0, (row_len(a, m) + KV8_HALF - 1) / KV8_HALF); }
+__device__ __forceinline__ int row_pieces(const Kv8AttnArgs& a, int m) { return max(0, (row_len(a, m) + KV8_HALF - 1) / KV8_HALF - a.own_from); }
+
+// Pieces of a row's items that stand in the line.
+__device__ __forceinline__ int line_pieces(const Kv8AttnArgs& a, int m) {
+    const int n = row_pieces(a, m);
+    return n > a.solo ? n : 0;
+}
 
 // Every thread of the CTA adds up the pieces of some rows that follow one another, ceil(M / THREADS) of them; first[t]: pieces in front of thread t's rows,
 // first[THREADS]: of all.  Ends with a barrier.
@@ -59,9 +68,11 @@ __device__ __forceinline__ Line make_line(const Kv8AttnArgs& a, int items, int c
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, per = (a.M + THREADS - 1) / THREADS, m0 = min(a.M, tid * per), m1 = min(a.M, m0 + per);
     if (tid == 0) s_most = 0;
     int sum = 0, most = 0;
+    bool solo = false;
     for (int m = m0; m < m1; ++m) {
         const int n = row_pieces(a, m);
-        sum += n;
+        if (n > a.solo) sum += n;
+        else solo |= n > 0;
         most = max(most, n);
     }
     int incl = sum;
@@ -82,8 +93,8 @@ __device__ __forceinline__ Line make_line(const Kv8AttnArgs& a, int items, int c
     }
     first[tid] = before;
     if (tid == 0) first[THREADS] = all;
-    __syncthreads();
     Line l;
+    l.solo = __syncthreads_or(solo);
     l.total = (long long)all * items;
     l.chunk = max((l.total + ctas - 1) / ctas, (long long)min(LEAST_PIECES, s_most));
     return l;
@@ -91,7 +102,7 @@ __device__ __forceinline__ Line make_line(const Kv8AttnArgs& a, int items, int c
 
 // Pieces of one item that follow one another.
 struct Segment {
-    int m, item, at, n, of;  // row, its item, first piece, pieces, pieces of the whole item
+    int m, item, at, n, of;  // row, its item, first piece (counted from own_from), pieces, pieces of the whole item
 };
 template <int THREADS>
 __device__ __forceinline__ Segment segment_at(const Kv8AttnArgs& a, const int* first, int items, long long u, long long end) {
@@ -106,7 +117,7 @@ __device__ __forceinline__ Segment segment_at(const Kv8AttnArgs& a, const int* f
     Segment s;
     int at = first[lo];
     s.m = lo * ((a.M + THREADS - 1) / THREADS);
-    for (s.of = row_pieces(a, s.m); rank >= at + s.of; s.of = row_pieces(a, ++s.m)) at += s.of;
+    for (s.of = line_pieces(a, s.m); rank >= at + s.of; s.of = line_pieces(a, ++s.m)) at += s.of;
     const long long off = u - (long long)at * items;  // below of * items
     s.item = small ? (int)((uint32_t)off / (uint32_t)s.of) : (int)(off / s.of);
     s.at = (int)(off - (long long)s.item * s.of);
@@ -119,7 +130,7 @@ __device__ __forceinline__ void next_segment(const Kv8AttnArgs& a, int items, Se
     s.at = 0;
     if (++s.item == items) {
         s.item = 0;
-        do s.of = row_pieces(a, ++s.m);
+        do s.of = line_pieces(a, ++s.m);
         while (s.of == 0);
     }
     s.n = min(s.of, left);
@@ -209,6 +220,60 @@ __device__ __forceinline__ void store2(const Kv8AttnArgs& a, int m, int head, in
 // Parts in `work`: of CTA c its first item (0) and its last (1).
 __device__ __forceinline__ float* cta_part(const Kv8AttnArgs& a, int vp, int cta, int which) { return static_cast<float*>(a.work) + (size_t)(2 * cta + which) * part_floats(vp); }
 
+// Joins four elements of a pair (relative to 2^top, with their sum) with the parts of the prefix.
+__device__ __forceinline__ void add_prefix(const Kv8AttnArgs& a, int vp, int kvh, int pair, int d, float& top, float& sum, float (&v)[4]) {
+    const size_t pairs = (size_t)a.M * (a.heads / a.pool.kv_heads), step = (size_t)a.pool.kv_heads * pairs * (vp + 4);
+    const float* at = a.prefix + ((size_t)kvh * pairs + pair) * (vp + 4);
+    float most = top;
+#pragma unroll 4
+    for (int i = 0; i < a.prefix_n; ++i) most = fmaxf(most, __ldcg(at + i * step));
+    const float ref = most == -INFINITY ? 0.f : most, own = exp2f(top - ref);
+    sum *= own;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) v[e] *= own;
+#pragma unroll 4
+    for (int i = 0; i < a.prefix_n; ++i) {
+        const float2 ml = __ldcg(reinterpret_cast<const float2*>(at + i * step));
+        if (ml.x == -INFINITY) continue;  // nothing seen
+        const float f = exp2f(ml.x - ref);
+        const float4 x = __ldcg(reinterpret_cast<const float4*>(at + i * step + 4 + d));
+        sum = fmaf(f, ml.y, sum);
+        v[0] = fmaf(f, x.x, v[0]); v[1] = fmaf(f, x.y, v[1]); v[2] = fmaf(f, x.z, v[2]); v[3] = fmaf(f, x.w, v[3]);
+    }
+    top = most;
+}
+
+// The same for what a lane of a warp's own item has: elements 8 i + 2 tig + 0, 1 of a pair.
+template <int VS>
+__device__ __forceinline__ void add_prefix_to(const Kv8AttnArgs& a, int vp, int kvh, int pair, int tig, float& top, float& sum, float (&o)[VS * 4][2]) {
+    const size_t pairs = (size_t)a.M * (a.heads / a.pool.kv_heads), step = (size_t)a.pool.kv_heads * pairs * (vp + 4);
+    const float* at = a.prefix + ((size_t)kvh * pairs + pair) * (vp + 4);
+    float most = top;
+#pragma unroll 4
+    for (int i = 0; i < a.prefix_n; ++i) most = fmaxf(most, __ldcg(at + i * step));
+    const float ref = most == -INFINITY ? 0.f : most, own = exp2f(top - ref);
+    sum *= own;
+#pragma unroll
+    for (int s = 0; s < VS * 4; ++s) {
+        o[s][0] *= own;
+        o[s][1] *= own;
+    }
+#pragma unroll 1
+    for (int i = 0; i < a.prefix_n; ++i) {
+        const float2 ml = __ldcg(reinterpret_cast<const float2*>(at + i * step));
+        const float f = ml.x == -INFINITY ? 0.f : exp2f(ml.x - ref);
+        if (ml.x != -INFINITY) sum = fmaf(f, ml.y, sum);
+#pragma unroll
+        for (int s = 0; s < VS * 4; ++s) {
+            if (8 * s >= vp) break;
+            const float2 x = __ldcg(reinterpret_cast<const float2*>(at + i * step + 4 + 8 * s + 2 * tig));
+            o[s][0] = fmaf(f, x.x, o[s][0]);
+            o[s][1] = fmaf(f, x.y, o[s][1]);
+        }
+    }
+    top = most;
+}
+
 // VS: slabs of 32 value elements (at most).  A warp's ring holds `depth` pieces; the keys of a piece make room for those of a later one as soon as the scores are
 // there, the values when the piece is done.
 template <bool BF16, int VS, int WARPS>
@@ -242,41 +307,41 @@ __global__ void __launch_bounds__(WARPS * 32, 1) kv8_stream_kernel(const Kv8Attn
     const int count = (int)(u1 - u0);  // pieces of this CTA
     pdl_launch_dependents();
 
-    // ---- rows without a context ----
-    for (int m = blockIdx.x; m < a.M; m += ctas) {
+    // ---- rows without a context (where there is a prefix, kv8_join_kernel writes them) ----
+    for (int m = blockIdx.x; m < a.M && a.prefix_n == 0; m += ctas) {
         if (row_pieces(a, m) > 0 || (unsigned)__ldg(a.row_seq + m) >= (unsigned)a.pool.n_seq) continue;
         const float zero[1] = {0.f};
         for (int i = tid; i < a.heads * a.pool.vdim; i += THREADS) store_row<BF16, 1>(a.out, (size_t)m * a.ldo + i, zero);
     }
-    if (count == 0) return;
 
-    // ---- copies: `ahead` runs `depth` pieces of this warp ahead of the arithmetic ----
-    Segment sg = segment_at<THREADS>(a, first, items, u0, u1), ahead = sg;
-    int ahead_at = warp, ahead_begin = 0, ahead_page = -1;  // its piece, counted over the CTA; the first of its segment; its page in the pool
-    const int32_t* ahead_table = nullptr;                   // of its segment's sequence
-    const unsigned char* ahead_head = nullptr;              // its head's block of page 0
+    // ---- copies: `ahead` runs some pieces of this warp ahead of the arithmetic ----
+    Segment sg{}, ahead{};
+    int ahead_at = 0, ahead_begin = 0, ahead_page = -1;  // its piece, counted over the CTA (or the item that is this warp's own); the first of its segment; its page in the pool
+    int end = 0, step = 1;                               // pieces of the CTA (of the item); this warp has every step-th
+    const int32_t* ahead_table = nullptr;                // of its segment's sequence
+    const unsigned char* ahead_head = nullptr;           // its head's block of page 0
     const uint32_t half = (uint32_t)(sh.kpart + sh.vpart), page_bytes = 2 * half * (uint32_t)a.pool.kv_heads;
     auto enter = [&]() {
         ahead_table = a.pool.page_table + (size_t)__ldg(a.row_seq + ahead.m) * a.pool.max_pages;
         ahead_head = a.pool.pages + (size_t)(ahead.item / tiles) * (2 * half);
     };
     auto settle = [&]() {
-        if (ahead_at >= count) return;
+        if (ahead_at >= end) return;
         if (ahead_at >= ahead_begin + ahead.n) {
             do {
                 ahead_begin += ahead.n;
-                next_segment(a, items, ahead, count - ahead_begin);
+                next_segment(a, items, ahead, end - ahead_begin);
             } while (ahead_at >= ahead_begin + ahead.n);
             enter();
         }
-        const int p = (ahead.at + ahead_at - ahead_begin) >> 1;
+        const int p = (a.own_from + ahead.at + ahead_at - ahead_begin) >> 1;
         ahead_page = __ldg(p < a.n_shared ? a.shared + p : ahead_table + p);
     };
     // the piece that it stands at, null where there is none; on to the next
     auto take = [&]() -> const unsigned char* {
         const unsigned char* src = nullptr;
-        if (ahead_at < count && (unsigned)ahead_page < (unsigned)a.pool.n_pages) src = ahead_head + (unsigned long long)(uint32_t)ahead_page * page_bytes + (((ahead.at + ahead_at - ahead_begin) & 1) ? half : 0u);
-        ahead_at += WARPS;
+        if (ahead_at < end && (unsigned)ahead_page < (unsigned)a.pool.n_pages) src = ahead_head + (unsigned long long)(uint32_t)ahead_page * page_bytes + (((ahead.at + ahead_at - ahead_begin) & 1) ? half : 0u);
+        ahead_at += step;
         settle();
         return src;
     };
@@ -287,24 +352,31 @@ __global__ void __launch_bounds__(WARPS * 32, 1) kv8_stream_kernel(const Kv8Attn
         }
     };
     uint32_t there = 0, phase = 0;  // bit s: slot s holds a piece; the parity of its next wait
-    enter();
-    settle();
-    for (int s = 0; s < depth; ++s) {
-        const unsigned char* src = take();
-        if (!src) continue;
-        copy(kbuf + (size_t)s * sh.kpart, src, sh.kpart, &kfull[s]);
-        copy(vbuf + (size_t)s * sh.vpart, src + sh.kpart, sh.vpart, &vfull[s]);
-        there |= 1u << s;
-    }
+    auto start = [&](const Segment& at, int from, int pieces, int stride, int slots) {
+        ahead = at;
+        ahead_at = from;
+        ahead_begin = 0;
+        end = pieces;
+        step = stride;
+        enter();
+        settle();
+        for (int s = 0; s < slots; ++s) {
+            const unsigned char* src = take();
+            there = (there & ~(1u << s)) | (src ? 1u << s : 0u);
+            if (!src) continue;
+            copy(kbuf + (size_t)s * sh.kpart, src, sh.kpart, &kfull[s]);
+            copy(vbuf + (size_t)s * sh.vpart, src + sh.kpart, sh.vpart, &vfull[s]);
+        }
+    };
 
-    // ---- queries: warp w has pair w, eight elements a lane; they are fetched a segment ahead ----
+    // ---- queries: eight elements a lane ----
     static_assert(WARPS >= PAIRS, "a warp for every pair");
-    auto fetch_query = [&](const Segment& of, float (&x)[8]) {
+    auto fetch_query = [&](const Segment& of, int pr, float (&x)[8]) {
         const int kvh = of.item / tiles, tile = of.item - kvh * tiles, d0 = lane * 8;
 #pragma unroll
         for (int e = 0; e < 8; ++e) x[e] = 0.f;
-        if (warp >= min(PAIRS, group - tile * PAIRS) || d0 >= a.pool.dim) return;
-        const size_t at = (size_t)of.m * a.ldq + (size_t)(kvh * group + tile * PAIRS + warp) * a.pool.dim + d0;
+        if (pr >= min(PAIRS, group - tile * PAIRS) || d0 >= a.pool.dim) return;
+        const size_t at = (size_t)of.m * a.ldq + (size_t)(kvh * group + tile * PAIRS + pr) * a.pool.dim + d0;
         if (wide & 2) {
             float y[4], z[4];
             load_row<BF16, 4>(a.q, at, y);
@@ -320,8 +392,8 @@ __global__ void __launch_bounds__(WARPS * 32, 1) kv8_stream_kernel(const Kv8Attn
             }
         }
     };
-    auto put_query = [&](const float (&x)[8], int buffer) {  // as digits, in the order of the MMAs' operands
-        if (warp >= PAIRS) return;
+    // as digits, in the order of the MMAs' operands; returns what the pair's scores are multiplied with
+    auto put_query = [&](const float (&x)[8], int pr, uint4* to) -> float {
         uint32_t top = 0;
 #pragma unroll
         for (int e = 0; e < 8; ++e) top = max(top, __float_as_uint(x[e]) & 0x7FFFFFFFu);
@@ -342,36 +414,89 @@ __global__ void __launch_bounds__(WARPS * 32, 1) kv8_stream_kernel(const Kv8Attn
 #pragma unroll
             for (int h = 0; h < PASSES; ++h) {  // the upper two digits first
                 const int k = 2 * (PASSES - 1 - h);
-                queries[buffer * sh.queries + ((lane >> 2) * PASSES + h) * 32 + warp * 4 + (lane & 3)] = make_uint4(d[0][k + 1], d[0][k], d[1][k + 1], d[1][k]);
+                to[((lane >> 2) * PASSES + h) * 32 + pr * 4 + (lane & 3)] = make_uint4(d[0][k + 1], d[0][k], d[1][k + 1], d[1][k]);
             }
         }
-        if (lane == 0) s_c[buffer][warp] = top < 0x7F800000u ? a.scale * LOG2E * down : __uint_as_float(0x7FC00000u);
+        return top < 0x7F800000u ? a.scale * LOG2E * down : __uint_as_float(0x7FC00000u);
     };
 
     const int gid = lane >> 2, tig = lane & 3, slabs = sh.dp / 32, vslabs = sh.vp / 32;
-    int i = warp, slot = 0, len = row_len(a, sg.m);  // this warp's next piece, counted over the CTA, and its slot; tokens of the segment's row
-    bool good = true;                                // no wait has run out
+    int i = 0, slot = 0, rings = 1, len = 0;  // this warp's next piece, counted over the CTA (or its own item), and its slot; slots in use; tokens of the segment's row
+    bool good = true;                         // no wait has run out
+    bool alone = line.solo;                   // with items of this warp's own; then with the line
+    int own = warp * ctas + (int)blockIdx.x;  // those are every WARPS * ctas-th of all
+    uint4* own_queries = reinterpret_cast<uint4*>(kbuf + sh.kpart);  // where the second slot's keys will stand
     float next_q[8];
-    fetch_query(sg, next_q);
-    put_query(next_q, 0);
-    __syncthreads();
-    for (int begin = 0, turn = 0; begin < count; turn ^= 1) {
-        const int kvh = sg.item / tiles, tile = sg.item - kvh * tiles, pairs = min(PAIRS, group - tile * PAIRS), head0 = kvh * group + tile * PAIRS;
-        const uint4* qf = queries + turn * sh.queries;
-        const float c = s_c[turn][gid];
-        Segment behind = sg;
+    int begin = 0, turn = 0;
+    bool joined = false, waited = false;  // at the line; for the prefix
+    for (;;) {
+        Segment behind{};
         int len_behind = 0;
-        const bool last = begin + sg.n >= count;
-        if (!last) {
-            next_segment(a, items, behind, count - begin - sg.n);
-            len_behind = row_len(a, behind.m);
-            fetch_query(behind, next_q);
+        bool last = true;
+        float c = 0.f;
+        const uint4* qf;
+        if (alone) {
+            int m = 0, n = 0;
+            for (; own < a.M * items; own += WARPS * ctas) {
+                m = own / items;
+                n = row_pieces(a, m);
+                if (n > 0 && n <= a.solo) break;
+            }
+            if (own >= a.M * items || !good) {
+                alone = false;
+                continue;
+            }
+            sg = Segment{m, own - m * items, 0, n, n};
+            own += WARPS * ctas;
+            __syncwarp();
+            start(sg, 0, n, 1, 1);
+            len = row_len(a, m);
+            i = begin = slot = 0;
+            const int pairs = min(PAIRS, group - (sg.item % tiles) * PAIRS);
+#pragma unroll 2
+            for (int pr = 0; pr < pairs; ++pr) {
+                fetch_query(sg, pr, next_q);
+                const float f = put_query(next_q, pr, own_queries);
+                if (gid == pr) c = f;
+            }
+            __syncwarp();
+            qf = own_queries;
+        } else {
+            if (!joined) {
+                joined = true;
+                if (count == 0) break;
+                asm volatile("fence.proxy.async.shared::cta;" ::: "memory");  // queries stood where pieces are copied to
+                __syncwarp();
+                sg = segment_at<THREADS>(a, first, items, u0, u1);
+                rings = depth;
+                start(sg, warp, count, WARPS, depth);
+                len = row_len(a, sg.m);
+                i = warp;
+                begin = slot = 0;
+                if (warp < PAIRS) {
+                    fetch_query(sg, warp, next_q);
+                    const float f = put_query(next_q, warp, queries);
+                    if (lane == 0) s_c[0][warp] = f;
+                }
+                __syncthreads();
+            }
+            if (begin >= count) break;
+            qf = queries + turn * sh.queries;
+            c = s_c[turn][gid];
+            last = begin + sg.n >= count;
+            behind = sg;
+            if (!last) {  // the next segment's queries are fetched now
+                next_segment(a, items, behind, count - begin - sg.n);
+                len_behind = row_len(a, behind.m);
+                if (warp < PAIRS) fetch_query(behind, warp, next_q);
+            }
         }
+        const int kvh = sg.item / tiles, tile = sg.item - kvh * tiles, pairs = min(PAIRS, group - tile * PAIRS), head0 = kvh * group + tile * PAIRS;
         float mx = -INFINITY, l = 0.f, o[VS * 4][2];  // elements 8 i + 2 tig + 0, 1 of pair gid
 #pragma unroll
         for (int s = 0; s < VS * 4; ++s) o[s][0] = o[s][1] = 0.f;
-        for (; good && i < begin + sg.n; i += WARPS) {
-            const int nt = len - ((sg.at + i - begin) * KV8_HALF + 8 * tig);  // this lane's tokens are 8 tig .. 8 tig + 7: how many of them are seen
+        for (; good && i < begin + sg.n; i += step) {
+            const int nt = len - ((a.own_from + sg.at + i - begin) * KV8_HALF + 8 * tig);  // this lane's tokens are 8 tig .. 8 tig + 7: how many of them are seen
             const bool partial = nt + 8 * tig < KV8_HALF;
             const unsigned char* next = take();  // the piece that comes into this slot next
             unsigned char *keys = kbuf + (size_t)slot * sh.kpart, *values = vbuf + (size_t)slot * sh.vpart;
@@ -481,12 +606,22 @@ __global__ void __launch_bounds__(WARPS * 32, 1) kv8_stream_kernel(const Kv8Attn
             }
             if (next) copy(values, next + sh.kpart, sh.vpart, &vfull[slot]);
             there = (there & ~(1u << slot)) | (next ? 1u << slot : 0u);
-            slot = slot + 1 == depth ? 0 : slot + 1;
+            slot = slot + 1 == rings ? 0 : slot + 1;
         }
 
-        // ---- the warps' results added up: `slots` warps at a time to those of the first `slots` warps, then these ----
         l += __shfl_xor_sync(0xffffffffu, l, 1);
         l += __shfl_xor_sync(0xffffffffu, l, 2);
+        if (alone) {
+            if (!waited) pdl_wait();  // the parts of the prefix are there
+            waited = true;
+            if (a.prefix_n) add_prefix_to<VS>(a, sh.vp, kvh, sg.m * group + tile * PAIRS + min(gid, pairs - 1), tig, mx, l, o);
+            const float inv = l == 0.f ? 0.f : 1.0f / l;
+#pragma unroll
+            for (int s = 0; s < VS * 4; ++s)
+                if (s < vslabs * 4 && gid < pairs) store2<BF16>(a, sg.m, head0 + gid, 8 * s + 2 * tig, o[s][0] * inv, o[s][1] * inv, wide & 1);
+            continue;
+        }
+        // ---- the warps' results added up: `slots` warps at a time to those of the first `slots` warps, then these ----
         const int room = pairs <= 2 ? 2 : pairs <= 4 ? 4 : PAIRS, slots = min(WARPS, MERGE_ROWS / room);
         const int row = warp % slots * room + gid;
         float* mine = merge + (size_t)row * sh.ldo + tig * 2;
@@ -522,10 +657,15 @@ __global__ void __launch_bounds__(WARPS * 32, 1) kv8_stream_kernel(const Kv8Attn
             __syncthreads();
         }
         if (warp < slots) put();
-        if (!last) put_query(next_q, turn ^ 1);
+        if (!last && warp < PAIRS) {
+            const float f = put_query(next_q, warp, queries + (turn ^ 1) * sh.queries);
+            if (lane == 0) s_c[turn ^ 1][warp] = f;
+        }
         __syncthreads();
         const bool whole = sg.n == sg.of;
         float* part = cta_part(a, sh.vp, blockIdx.x, sg.at == 0);
+        if (!waited) pdl_wait();  // the parts of the prefix are there
+        waited = true;
         for (int k = tid; k < pairs * (sh.vp / 4); k += THREADS) {
             const int pr = k / (sh.vp / 4), d = (k - pr * (sh.vp / 4)) * 4;
             float top = -INFINITY, sum = 0.f, v[4] = {0.f, 0.f, 0.f, 0.f};
@@ -539,6 +679,10 @@ __global__ void __launch_bounds__(WARPS * 32, 1) kv8_stream_kernel(const Kv8Attn
                 sum = fmaf(f, s_l[w * room + pr], sum);
             }
             if (whole) {
+                if (a.prefix_n) {
+                    top = ref;  // v is relative to it
+                    add_prefix(a, sh.vp, kvh, sg.m * group + tile * PAIRS + pr, d, top, sum, v);
+                }
                 const float inv = sum == 0.f ? 0.f : 1.0f / sum;
                 store2<BF16>(a, sg.m, head0 + pr, d, v[0] * inv, v[1] * inv, wide & 1);
                 store2<BF16>(a, sg.m, head0 + pr, d + 2, v[2] * inv, v[3] * inv, wide & 1);
@@ -554,12 +698,14 @@ __global__ void __launch_bounds__(WARPS * 32, 1) kv8_stream_kernel(const Kv8Attn
         __syncwarp();
         if (lane == 0) mb_arrive(&s_added);
         begin += sg.n;
+        turn ^= 1;
         sg = behind;
         len = len_behind;
     }
+    if (!waited) pdl_wait();  // kv8_join_kernel waits for this launch alone
     // every copy has been waited for, unless a wait ran out: then what is still on its way has to land before this CTA's shared memory is another's
     if (!good)
-        for (int s = 0; s < depth; ++s) {
+        for (int s = 0; s < rings; ++s) {
             if (!((there >> s) & 1u)) continue;
             mb_land(&kfull[s], (phase >> s) & 1u);
             mb_land(&vfull[s], (phase >> s) & 1u);
@@ -570,12 +716,26 @@ __global__ void __launch_bounds__(WARPS * 32, 1) kv8_stream_kernel(const Kv8Attn
 // more: the warps share them, every lane with its elements of all pairs of a part in flight at once.
 constexpr int JOIN_THREADS = 288;
 template <bool BF16, int VS>
-__global__ void __launch_bounds__(JOIN_THREADS) kv8_join_kernel(const Kv8AttnArgs a, int tiles, int wide) {
+__global__ void __launch_bounds__(JOIN_THREADS) kv8_join_kernel(const Kv8AttnArgs a, int ctas, int tiles, int wide) {
     constexpr int THREADS = JOIN_THREADS, JW = THREADS / 32, NI = PAIRS * VS * 8 / 32;  // warps; groups of four elements a lane
     extern __shared__ __align__(128) unsigned char dyn[];       // factors [parts][PAIRS], then the warps' sums
-    __shared__ float s_inv[PAIRS];
+    __shared__ float s_top[PAIRS], s_sum[PAIRS];
     __shared__ int first[THREADS + 1];
-    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, items = a.pool.kv_heads * tiles, group = a.heads / a.pool.kv_heads, ctas = gridDim.x + 1, cut = blockIdx.x + 1, vp = kv8_pad(a.pool.vdim), quads = vp / 4;
+    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, items = a.pool.kv_heads * tiles, group = a.heads / a.pool.kv_heads, cut = blockIdx.x + 1, vp = kv8_pad(a.pool.vdim), quads = vp / 4;
+    if (cut >= ctas) {  // rows that have nothing but the prefix
+        pdl_wait();
+        const long all = (long)a.M * a.heads * quads, step = (long)(gridDim.x - (ctas - 1)) * THREADS;
+        for (long k = (long)(cut - ctas) * THREADS + tid; k < all; k += step) {
+            const int m = (int)(k / ((long)a.heads * quads)), r = (int)(k - (long)m * a.heads * quads), head = r / quads, d = (r - head * quads) * 4;
+            if (row_pieces(a, m) > 0 || (unsigned)__ldg(a.row_seq + m) >= (unsigned)a.pool.n_seq) continue;
+            float top = -INFINITY, sum = 0.f, v[4] = {0.f, 0.f, 0.f, 0.f};
+            add_prefix(a, vp, head / group, m * group + head % group, d, top, sum, v);
+            const float inv = sum == 0.f ? 0.f : 1.0f / sum;
+            store2<BF16>(a, m, head, d, v[0] * inv, v[1] * inv, wide & 1);
+            store2<BF16>(a, m, head, d + 2, v[2] * inv, v[3] * inv, wide & 1);
+        }
+        return;
+    }
     const Line line = make_line<THREADS>(a, items, ctas, first);
     pdl_wait();
     const long long u = cut * line.chunk;
@@ -601,7 +761,10 @@ __global__ void __launch_bounds__(JOIN_THREADS) kv8_join_kernel(const Kv8AttnArg
             if (warp < pairs) sum = fmaf(f, __ldcg(part(i) + (size_t)warp * (vp + 4) + 1), sum);
         }
         sum = warp_sum(sum);
-        if (lane == 0) s_inv[warp] = sum == 0.f ? 0.f : 1.0f / sum;
+        if (lane == 0) {
+            s_top[warp] = ref;
+            s_sum[warp] = sum;
+        }
     }
     __syncthreads();
     float4 acc[NI];
@@ -634,10 +797,11 @@ __global__ void __launch_bounds__(JOIN_THREADS) kv8_join_kernel(const Kv8AttnArg
             const float4 x = sums[w * NI * 32 + k];
             v[0] += x.x; v[1] += x.y; v[2] += x.z; v[3] += x.w;
         }
-#pragma unroll
-        for (int e = 0; e < 4; ++e) v[e] *= s_inv[pr];
-        store2<BF16>(a, sg.m, head0 + pr, d, v[0], v[1], wide & 1);
-        store2<BF16>(a, sg.m, head0 + pr, d + 2, v[2], v[3], wide & 1);
+        float top = s_top[pr], sum = s_sum[pr];
+        if (a.prefix_n) add_prefix(a, vp, kvh, sg.m * group + tile * PAIRS + pr, d, top, sum, v);
+        const float inv = sum == 0.f ? 0.f : 1.0f / sum;
+        store2<BF16>(a, sg.m, head0 + pr, d, v[0] * inv, v[1] * inv, wide & 1);
+        store2<BF16>(a, sg.m, head0 + pr, d + 2, v[2] * inv, v[3] * inv, wide & 1);
     }
 }
 
@@ -657,20 +821,29 @@ cudaError_t launch_behind(void (*kern)(KArgs...), int grid, int threads, size_t 
 }
 
 template <bool BF16, int VS, int WARPS>
-cudaError_t launch_stream(const Kv8AttnArgs& a, int sm_count, cudaStream_t st) {
+cudaError_t launch_stream(const Kv8AttnArgs& a_in, int sm_count, cudaStream_t st) {
+    Kv8AttnArgs a = a_in;
     const int group = a.heads / a.pool.kv_heads, tiles = (group + PAIRS - 1) / PAIRS, size = BF16 ? 2 : 4, ctas = sm_count;
     // bit 0: results in pairs, bit 1: queries in groups of four
     const int wide = (a.pool.vdim % 2 == 0 && (((uintptr_t)a.out | a.ldo * size) & (2 * size - 1)) == 0 ? 1 : 0) | (a.pool.dim % 8 == 0 && (((uintptr_t)a.q | a.ldq * size) & (4 * size - 1)) == 0 ? 2 : 0);
     auto bytes = [&](int depth) { return stream_shape(a.pool.dim, a.pool.vdim, BF16 ? 1 : 2, WARPS, depth).bytes; };
     int depth = MAX_DEPTH;
     while (depth > 1 && bytes(depth) > ROOM) --depth;
+    // a warp's own items need a second slot for their queries.  Where there are more items than CTAs, a CTA would take them one by one
+    a.solo = depth < 2 ? 0 : (long)a.M * a.pool.kv_heads * tiles >= 2 * sm_count ? 12 : 4;
     const size_t smem = bytes(depth), join_smem = sizeof(float) * PAIRS * ctas + 16 + sizeof(float) * JOIN_THREADS * PAIRS * VS;
     cudaError_t e = ensure_dyn_smem(kv8_stream_kernel<BF16, VS, WARPS>, smem);
     if (e == cudaSuccess) e = ensure_dyn_smem(kv8_join_kernel<BF16, VS>, join_smem);
     if (e != cudaSuccess) return e;
-    kv8_stream_kernel<BF16, VS, WARPS><<<(unsigned)ctas, WARPS * 32, smem, st>>>(a, depth, tiles, wide);
-    if ((e = cudaGetLastError()) != cudaSuccess) return e;
-    return launch_behind(kv8_join_kernel<BF16, VS>, ctas - 1, JOIN_THREADS, join_smem, st, a, tiles, wide);
+    if (a.prefix_n) {
+        e = launch_behind(kv8_stream_kernel<BF16, VS, WARPS>, ctas, WARPS * 32, smem, st, a, depth, tiles, wide);
+    } else {
+        kv8_stream_kernel<BF16, VS, WARPS><<<(unsigned)ctas, WARPS * 32, smem, st>>>(a, depth, tiles, wide);
+        e = cudaGetLastError();
+    }
+    if (e != cudaSuccess) return e;
+    const long rest = a.prefix_n ? std::min(((long)a.M * a.heads * kv8_pad(a.pool.vdim) / 4 + JOIN_THREADS - 1) / JOIN_THREADS, 4096l) : 0;
+    return launch_behind(kv8_join_kernel<BF16, VS>, ctas - 1 + (int)rest, JOIN_THREADS, join_smem, st, a, ctas, tiles, wide);
 }
 
 // 12 warps (168 registers a thread) where their pieces fit, else eight.
@@ -691,8 +864,28 @@ cudaError_t launch_typed(const Kv8AttnArgs& a, int sm_count, cudaStream_t st) {
 
 }  // namespace
 
-size_t kv8_attn_bytes(int, int vdim, int, int, int, int sm_count) { return sizeof(float) * 2 * (size_t)sm_count * part_floats(kv8_pad(vdim)); }
+// `work`: parts of the line's cuts, then those of the prefix.
+static size_t line_floats(int vdim, int sm_count) { return 2 * (size_t)sm_count * part_floats(kv8_pad(vdim)); }
 
-cudaError_t launch_kv8_attn(const Kv8AttnArgs& a, int sm_count, cudaStream_t st) { return a.bf16 ? launch_typed<true>(a, sm_count, st) : launch_typed<false>(a, sm_count, st); }
+size_t kv8_attn_bytes(int kv_heads, int dim, int vdim, int M, int heads, int n_shared, int sm_count) {
+    const bool own = kv8_prefix_plan(kv_heads, dim, vdim, 0, M, heads, n_shared, sm_count).parts == 0;
+    const int parts = own ? 0 : kv8_prefix_most_parts(kv_heads, M, heads, n_shared, sm_count);
+    return sizeof(float) * (line_floats(vdim, sm_count) + (size_t)parts * M * heads * (kv8_pad(vdim) + 4));
+}
+
+cudaError_t launch_kv8_attn(const Kv8AttnArgs& a_in, int sm_count, cudaStream_t st) {
+    Kv8AttnArgs a = a_in;
+    const Kv8Prefix p = kv8_prefix_plan(a.pool.kv_heads, a.pool.dim, a.pool.vdim, a.bf16, a.M, a.heads, a.n_shared, sm_count);
+    a.own_from = 0;
+    a.prefix_n = p.parts;
+    if (p.parts) {
+        float* parts = static_cast<float*>(a.work) + line_floats(a.pool.vdim, sm_count);
+        const cudaError_t e = launch_kv8_prefix(a, p, parts, st);
+        if (e != cudaSuccess) return e;
+        a.prefix = parts;
+        a.own_from = a.n_shared * (KV8_PAGE / KV8_HALF);
+    }
+    return a.bf16 ? launch_typed<true>(a, sm_count, st) : launch_typed<false>(a, sm_count, st);
+}
 
 }  // namespace hm

@@ -1,0 +1,718 @@
+// The shared pages of kv8_attn on the 5th-generation tensor cores: scores and sums of all rows over a prefix that is read once for 128 or 256 (row, head) pairs.
+//
+// Per block of 128 tokens (two pages), for 128 pairs of one key/value head, with f32 sums in tensor memory:
+//   S [128 pairs x 128 tokens] = Q [128 x dim] . K^T         Q, K in shared memory
+//   O [128 pairs x vdim]      += P [128 x 128 tokens] . V    P in tensor memory, where S was; V in shared memory, element by token
+// Codes are whole numbers below 128, exact in f16.  A query row enters times a power of two (largest element 2^14 .. 2^15): a bf16 row is exact in one f16 term down to 2^-30 of
+// its largest element, an f32 row takes two terms (2^-22 of a value).  A token's key scale joins the scores, its value scale the weights: P = 2^(s - ref) * scale enters as f16 in one
+// term (2^-12 of itself) for bf16 rows, in two for f32 rows.  `ref` is a pair's reference in the units of the weights: it follows its largest score and the largest value
+// scale of the blocks so far, each with some room (2^8 and 2^2), so that O in tensor memory is hardly ever multiplied; P stays below 2^15, and a weight of 2^-30
+// of the largest still has a step.
+//
+// 24 warps: 0 .. 7 and 8 .. 15 turn scores into weights, two threads for every pair, a page each; 16 .. 18 make f16 of keys' codes, 19 .. 21 of values'; 22 copies pages; 23 issues the MMAs.  Two streams of
+// blocks take turns on the tensor cores, so that one's MMAs run beside the other's exponentials: the two halves of 256 pairs over the same blocks (a block's codes are then converted once
+// for both), or, for fewer pairs and f32 rows, whose two terms leave room for one tile of queries, the even and the odd blocks of 128 pairs.  The token axis is split where there are too few pairs for all SMs; splits form
+// clusters that join what they have over their shared memory, and what is left goes to `work`, relative to its references, to be joined with the rows' own pages.
+#include <algorithm>
+#include <map>
+#include <mutex>
+#include <type_traits>
+#include <utility>
+
+#include "kv8.h"
+#include "launch_attrs.h"
+#include "mbarrier.cuh"
+#include "rows.cuh"
+
+namespace hm {
+namespace {
+
+constexpr int TILE = 128, BLOCK = 128;  // pairs of a tile, tokens of a block
+constexpr int SOFT_WARPS = 16, CONV_WARPS = 3, THREADS = 768;  // those of keys, as many of values
+constexpr int COPY_WARP = SOFT_WARPS + 2 * CONV_WARPS, MMA_WARP = COPY_WARP + 1;
+constexpr int STREAM_WARPS = SOFT_WARPS / 2;
+constexpr int MAX_RAW = 8;              // pages in flight or being converted
+constexpr int RING = 4;                 // blocks whose scales are kept
+constexpr int MOST_PARTS = 8;           // that are left to be joined with the rows' own pages
+constexpr size_t ROOM = 226 * 1024;
+constexpr float LOG2E = 1.4426950408889634f;
+constexpr float SLACK = 8.f;            // how far a score may exceed its reference, as an exponent
+constexpr float VALUE_ROOM = 2.f;       // how far the reference value scale is set above the largest so far, where it moves
+constexpr float DROP = 5.f;             // weights enter as 2^(DROP - exponent of the value scale) times themselves: 2^(SLACK + DROP + 1) < 2^15
+
+struct Shape {
+    int dp, vp, katoms, kpart, half;  // padded sizes, pieces of 64 elements of keys, bytes of a half's keys, of a half
+    int raw, kst, vst;                // pages of the ring, blocks of keys and of values as f16
+    uint32_t q_tile, k_tile, v_tile, q_at, k_at, v_at, raw_at, bytes;
+};
+__host__ __device__ inline Shape shape_of(int dim, int vdim, int terms, int q_tiles) {
+    Shape s;
+    s.dp = kv8_pad(dim);
+    s.vp = kv8_pad(vdim);
+    s.katoms = (s.dp + 63) / 64;
+    s.kpart = kv8_part_bytes(dim);
+    s.half = (int)kv8_half_bytes(dim, vdim);
+    s.q_tile = (uint32_t)terms * s.katoms * TILE * 128;
+    s.k_tile = (uint32_t)s.katoms * BLOCK * 128;
+    s.v_tile = 2u * s.vp * 128;
+    // two blocks of values, then of keys, where they leave the ring four pages (two blocks); then as many pages as fit
+    const uint32_t page = 2u * s.half, room = (uint32_t)ROOM - 8192 - 1024 - q_tiles * s.q_tile;
+    s.vst = s.k_tile + 2 * s.v_tile + 4 * page <= room ? 2 : 1;
+    s.kst = 2 * s.k_tile + s.vst * s.v_tile + 4 * page <= room ? 2 : 1;
+    s.raw = (int)((room - s.kst * s.k_tile - s.vst * s.v_tile) / page);
+    if (s.raw > MAX_RAW) s.raw = MAX_RAW;
+    s.q_at = 0;
+    s.k_at = s.q_at + q_tiles * s.q_tile;
+    s.v_at = s.k_at + s.kst * s.k_tile;
+    s.raw_at = s.v_at + s.vst * s.v_tile;
+    s.bytes = 1024 + s.raw_at + (uint32_t)s.raw * page;
+    const uint32_t results = 1024 + 2u * TILE * (s.vp + 4) * 4u;  // the streams' results stand there at the end
+    if (s.bytes < results) s.bytes = results;
+    return s;
+}
+
+struct Shared {
+    uint64_t raw_full[MAX_RAW], raw_empty[MAX_RAW], k_full[2], k_empty[2], v_full[2], v_empty[2], s_full[2], p_full[2], pv_done[2], sc_full[RING], q_full, done;
+    uint32_t tmem;
+    volatile int abort_flag;
+    int longest;
+    alignas(16) float ks[RING][BLOCK];
+    alignas(16) float vs[RING][BLOCK];
+    int ve[RING];      // exponent field of the largest value scale of a block's tokens that a row sees
+    int there[RING];   // bit i: page i of the block exists
+    int raw_there[MAX_RAW];
+    float half[2][2][2][TILE];  // [stream][turn][page of the block][pair]: what the two threads of a pair tell one another
+};
+
+__device__ __forceinline__ uint32_t desc_lo(uint32_t addr) { return ((addr >> 4) & 0x3FFF) | (1u << 16); }
+constexpr uint32_t DESC_HI = (1024u >> 4) | (1u << 14) | (2u << 29);  // rows of 128 bytes in groups of eight, 128-byte swizzle
+__device__ __forceinline__ uint32_t idesc_f16(int n) { return (1u << 4) | ((uint32_t)(n >> 3) << 17) | ((uint32_t)(TILE >> 4) << 24); }  // f32 sums of f16, M 128, both K-major
+__device__ __forceinline__ void mma_ss(uint32_t d, uint32_t a_lo, uint32_t b_lo, uint32_t idesc, bool accumulate) {
+    asm volatile("{ .reg .pred p; .reg .b64 da, db; setp.ne.b32 p, %5, 0; mov.b64 da, {%1, %4}; mov.b64 db, {%2, %4};\n"
+                 "tcgen05.mma.cta_group::1.kind::f16 [%0], da, db, %3, p; }" ::"r"(d), "r"(a_lo), "r"(b_lo), "r"(idesc), "n"(DESC_HI), "r"((uint32_t)accumulate) : "memory");
+}
+__device__ __forceinline__ void mma_ts(uint32_t d, uint32_t a_tmem, uint32_t b_lo, uint32_t idesc, bool accumulate) {
+    asm volatile("{ .reg .pred p; .reg .b64 db; setp.ne.b32 p, %5, 0; mov.b64 db, {%2, %4};\n"
+                 "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], db, %3, p; }" ::"r"(d), "r"(a_tmem), "r"(b_lo), "r"(idesc), "n"(DESC_HI), "r"((uint32_t)accumulate) : "memory");
+}
+__device__ __forceinline__ void mma_commit(uint64_t* bar) { asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(s32(bar)) : "memory"); }
+__device__ __forceinline__ void tmem_ld32(uint32_t (&r)[32], uint32_t addr) {
+    asm volatile("tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31}, [%32];"
+                 : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15]),
+                   "=r"(r[16]), "=r"(r[17]), "=r"(r[18]), "=r"(r[19]), "=r"(r[20]), "=r"(r[21]), "=r"(r[22]), "=r"(r[23]), "=r"(r[24]), "=r"(r[25]), "=r"(r[26]), "=r"(r[27]), "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31])
+                 : "r"(addr));
+}
+// Names the registers, so that no use of them moves in front of the wait.
+__device__ __forceinline__ void tmem_wait(uint32_t (&r)[32]) {
+    asm volatile("tcgen05.wait::ld.sync.aligned;"
+                 : "+r"(r[0]), "+r"(r[1]), "+r"(r[2]), "+r"(r[3]), "+r"(r[4]), "+r"(r[5]), "+r"(r[6]), "+r"(r[7]), "+r"(r[8]), "+r"(r[9]), "+r"(r[10]), "+r"(r[11]), "+r"(r[12]), "+r"(r[13]), "+r"(r[14]), "+r"(r[15]),
+                   "+r"(r[16]), "+r"(r[17]), "+r"(r[18]), "+r"(r[19]), "+r"(r[20]), "+r"(r[21]), "+r"(r[22]), "+r"(r[23]), "+r"(r[24]), "+r"(r[25]), "+r"(r[26]), "+r"(r[27]), "+r"(r[28]), "+r"(r[29]), "+r"(r[30]), "+r"(r[31])
+                 :: "memory");
+}
+__device__ __forceinline__ void tmem_ld16(uint32_t (&r)[16], uint32_t addr) {
+    asm volatile("tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%16];"
+                 : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
+                 : "r"(addr));
+}
+__device__ __forceinline__ void tmem_wait16(uint32_t (&r)[16]) {
+    asm volatile("tcgen05.wait::ld.sync.aligned;"
+                 : "+r"(r[0]), "+r"(r[1]), "+r"(r[2]), "+r"(r[3]), "+r"(r[4]), "+r"(r[5]), "+r"(r[6]), "+r"(r[7]), "+r"(r[8]), "+r"(r[9]), "+r"(r[10]), "+r"(r[11]), "+r"(r[12]), "+r"(r[13]), "+r"(r[14]), "+r"(r[15])
+                 :: "memory");
+}
+__device__ __forceinline__ void tmem_st16(uint32_t addr, const uint32_t (&r)[16]) {
+    asm volatile("tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16};" ::"r"(addr), "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]),
+                 "r"(r[9]), "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15])
+                 : "memory");
+}
+__device__ __forceinline__ void tmem_st_wait() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
+__device__ __forceinline__ void tc_fence_before() { asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory"); }
+__device__ __forceinline__ void tc_fence_after() { asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory"); }
+__device__ __forceinline__ void fence_async_smem() { asm volatile("fence.proxy.async.shared::cta;" ::: "memory"); }
+__device__ __forceinline__ uint32_t elect_lane() {
+    uint32_t p;
+    asm volatile("{ .reg .pred P; .reg .b32 r; elect.sync r|P, 0xffffffff; selp.u32 %0, 1, 0, P; }" : "=r"(p));
+    return p;
+}
+__device__ __forceinline__ float exp2_ftz(float x) {
+    float y;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
+// Two f32 side by side: half the instructions of one by one.
+__device__ __forceinline__ uint64_t pair_of(uint32_t lo, uint32_t hi) {
+    uint64_t r;
+    asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "r"(lo), "r"(hi));
+    return r;
+}
+__device__ __forceinline__ uint64_t pair_of(float lo, float hi) { return pair_of(__float_as_uint(lo), __float_as_uint(hi)); }
+__device__ __forceinline__ float2 of_pair(uint64_t v) {
+    uint32_t lo, hi;
+    asm("mov.b64 {%0, %1}, %2;" : "=r"(lo), "=r"(hi) : "l"(v));
+    return make_float2(__uint_as_float(lo), __uint_as_float(hi));
+}
+__device__ __forceinline__ uint64_t mul2(uint64_t a, uint64_t b) {
+    uint64_t r;
+    asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+    return r;
+}
+__device__ __forceinline__ uint64_t add2(uint64_t a, uint64_t b) {
+    uint64_t r;
+    asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+    return r;
+}
+__device__ __forceinline__ uint64_t fma2(uint64_t a, uint64_t b, uint64_t c) {
+    uint64_t r;
+    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+    return r;
+}
+__device__ __forceinline__ uint32_t f16x2(float lo, float hi) {
+    uint32_t r;
+    asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
+    return r;
+}
+__device__ __forceinline__ float f16_lo(uint32_t w) {
+    float f;
+    asm("{ .reg .b16 l, h; mov.b32 {l, h}, %1; cvt.f32.f16 %0, l; }" : "=f"(f) : "r"(w));
+    return f;
+}
+__device__ __forceinline__ float f16_hi(uint32_t w) {
+    float f;
+    asm("{ .reg .b16 l, h; mov.b32 {l, h}, %1; cvt.f32.f16 %0, h; }" : "=f"(f) : "r"(w));
+    return f;
+}
+// Four codes as f16: a byte with its sign bit turned becomes the last bits of 1024 + 128 + code, from which 1152 is subtracted.
+__device__ __forceinline__ void codes_f16(uint32_t w, uint32_t& a, uint32_t& b) {
+    w ^= 0x80808080u;
+    const uint32_t x = __byte_perm(w, 0x64646464u, 0x4140), y = __byte_perm(w, 0x64646464u, 0x4342);
+    asm("sub.rn.f16x2 %0, %1, %2;" : "=r"(a) : "r"(x), "r"(0x64806480u));
+    asm("sub.rn.f16x2 %0, %1, %2;" : "=r"(b) : "r"(y), "r"(0x64806480u));
+}
+
+// Barrier of the two warps that share 32 pairs, with an OR over their predicates.
+__device__ __forceinline__ bool both_any(int id, bool v) {
+    uint32_t r;
+    asm volatile("{ .reg .pred p, q; setp.ne.u32 p, %1, 0; barrier.cta.red.or.aligned.pred q, %2, 64, p; selp.u32 %0, 1, 0, q; }" : "=r"(r) : "r"((uint32_t)v), "r"(1 + id) : "memory");
+    return r != 0;
+}
+
+// TERMS: f16 terms of queries and weights; PAIRED: the streams are two tiles of pairs over the same blocks.
+template <bool BF16, int TERMS, bool PAIRED>
+__global__ void __launch_bounds__(THREADS, 1) kv8_prefix_kernel(const Kv8AttnArgs a, int splits, int cluster, float* parts, int wide) {
+    extern __shared__ __align__(128) unsigned char dsm[];
+    __shared__ Shared sh;
+    const Shape g = shape_of(a.pool.dim, a.pool.vdim, TERMS, PAIRED ? 2 : 1);
+    unsigned char* base = dsm + ((1024u - (s32(dsm) & 1023u)) & 1023u);  // swizzled tiles need 1024-byte alignment
+    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, kvh = blockIdx.y, split = blockIdx.x % splits, tiles0 = blockIdx.x / splits * (PAIRED ? 2 : 1);
+    const int group = a.heads / a.pool.kv_heads, pairs = a.M * group, ldo = g.vp + 4;
+    pdl_launch_dependents();
+    if (tid == 0) {
+        for (int s = 0; s < g.raw; ++s) {
+            mb_init(&sh.raw_full[s], 1);
+            mb_init(&sh.raw_empty[s], 2 * CONV_WARPS);
+        }
+        for (int s = 0; s < 2; ++s) {
+            mb_init(&sh.k_full[s], CONV_WARPS);
+            mb_init(&sh.k_empty[s], 1);
+            mb_init(&sh.v_full[s], CONV_WARPS);
+            mb_init(&sh.v_empty[s], 1);
+            mb_init(&sh.s_full[s], 1);
+            mb_init(&sh.p_full[s], STREAM_WARPS);
+            mb_init(&sh.pv_done[s], 1);
+        }
+        for (int s = 0; s < RING; ++s) mb_init(&sh.sc_full[s], CONV_WARPS);
+        mb_init(&sh.q_full, (PAIRED ? 2 : 1) * STREAM_WARPS);
+        mb_init(&sh.done, 1);
+        sh.abort_flag = 0;
+        sh.longest = 0;
+        asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    }
+    __syncthreads();
+    // ---- the pair of a thread of the first warps, and how far it sees; its page of the blocks ----
+    const int stream = (warp >> 3) & 1, side = (warp >> 2) & 1, tile = tiles0 + (PAIRED ? stream : 0), pair = tile * TILE + (tid & (TILE - 1));
+    const bool mine = warp < SOFT_WARPS && pair < pairs;
+    const int row = mine ? pair / group : 0, head = kvh * group + (mine ? pair - row * group : 0);
+    int len = 0;
+    if (mine) {
+        const int seq = __ldg(a.row_seq + row);
+        if ((unsigned)seq < (unsigned)a.pool.n_seq) len = max(0, min(__ldg(a.row_pos + row), a.n_shared * KV8_PAGE - 1) + 1);
+    }
+    {
+        const int most = __reduce_max_sync(0xffffffffu, len);
+        if (lane == 0 && warp < SOFT_WARPS) atomicMax(&sh.longest, most);
+    }
+    if (warp == MMA_WARP) {
+        asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], 512;" ::"r"(s32(&sh.tmem)) : "memory");
+        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+    }
+    tc_fence_before();
+    __syncthreads();
+    tc_fence_after();
+    const uint32_t tmem = sh.tmem;
+    const int longest = sh.longest, nb = (longest + BLOCK - 1) / BLOCK, per = (nb + splits - 1) / splits, b0 = min(nb, split * per), n = min(nb, b0 + per) - b0;  // this CTA's blocks
+    const int tasks = PAIRED ? 2 * n : n;  // task j belongs to stream j & 1
+    auto block_of = [&](int j) { return PAIRED ? j >> 1 : j; };  // counted from b0
+
+    if (warp == COPY_WARP) {
+        const int pages = min(a.n_shared - 2 * b0, 2 * n);
+        bool ok = true;
+        uint32_t i = 0;
+        for (int p0 = 0; p0 < 2 * n && ok; p0 += 32) {
+            const int id = p0 + lane < pages ? __ldg(a.shared + 2 * b0 + p0 + lane) : -1;
+            for (int j = 0; j < min(32, 2 * n - p0); ++j, ++i) {
+                const int page = __shfl_sync(0xffffffffu, id, j), s = (int)(i % g.raw);
+                if (i >= (uint32_t)g.raw && !__all_sync(0xffffffffu, mb_wait(&sh.raw_empty[s], ((i / g.raw) & 1u) ^ 1u, a.err_flag, &sh.abort_flag))) {
+                    ok = false;
+                    break;
+                }
+                if (lane == 0) {
+                    const bool there = (unsigned)page < (unsigned)a.pool.n_pages;
+                    sh.raw_there[s] = there;
+                    if (there) {
+                        mb_expect_tx(&sh.raw_full[s], 2u * g.half);
+                        bulk_copy(base + g.raw_at + (size_t)s * 2 * g.half, a.pool.pages + ((size_t)page * a.pool.kv_heads + kvh) * (size_t)(2 * g.half), 2u * g.half, &sh.raw_full[s]);
+                    } else {
+                        mb_arrive(&sh.raw_full[s]);  // what the slot holds is converted again, and not seen
+                    }
+                }
+                __syncwarp();
+            }
+        }
+        if (lane == 0) mb_land_ring(sh.raw_full, i, (uint32_t)g.raw);
+    } else if (warp == MMA_WARP) {
+        const uint32_t lead = elect_lane();
+        const uint32_t id_s = idesc_f16(BLOCK), id_o = idesc_f16(g.vp);
+        const uint32_t q_lo = desc_lo(s32(base + g.q_at)), k_lo = desc_lo(s32(base + g.k_at)), v_lo = desc_lo(s32(base + g.v_at));
+        auto wait = [&](uint64_t* bar, uint32_t parity) { return __all_sync(0xffffffffu, mb_wait(bar, parity, a.err_flag, &sh.abort_flag)); };
+        bool ok = tasks == 0 || wait(&sh.q_full, 0);
+        for (int j = 0; j < tasks + 2 && ok; ++j) {
+            const int s = j & 1;
+            const uint32_t d_s = tmem + (uint32_t)s * BLOCK, d_o = tmem + 2 * BLOCK + (uint32_t)s * 128;
+            if (j >= 2) {  // the product of task j - 2
+                const int t = j - 2, b = block_of(t);
+                const int vs = b % g.vst;
+                if ((!PAIRED || s == 0) && !(ok = wait(&sh.v_full[vs], (b / g.vst) & 1))) break;
+                if (!(ok = wait(&sh.p_full[s], (t >> 1) & 1))) break;
+                tc_fence_after();
+                const uint32_t v = v_lo + (uint32_t)vs * (g.v_tile / 16);
+                if (lead) {
+#pragma unroll
+                    for (int h = 0; h < TERMS; ++h)
+#pragma unroll
+                        for (int k = 0; k < BLOCK / 16; ++k)
+                            mma_ts(d_o, d_s + (k >> 1) * 32 + h * 16 + (k & 1) * 8, v + (uint32_t)(k >> 2) * (g.v_tile / 32) + (k & 3) * 2, id_o, t > 1 || h > 0 || k > 0);
+                    mma_commit(&sh.pv_done[s]);
+                    if (!PAIRED || s == 1) mma_commit(&sh.v_empty[vs]);
+                }
+                __syncwarp();
+            }
+            if (j < tasks) {
+                const int b = block_of(j);
+                const int ks = b % g.kst;
+                if ((!PAIRED || s == 0) && !(ok = wait(&sh.k_full[ks], (b / g.kst) & 1))) break;
+                if (j >= 2 && !(ok = wait(&sh.pv_done[s], ((j - 2) >> 1) & 1))) break;  // the weights stand where the scores go
+                tc_fence_after();
+                if (lead) {
+                    const uint32_t q = q_lo + (PAIRED ? (uint32_t)s * (g.q_tile / 16) : 0u), key = k_lo + (uint32_t)ks * (g.k_tile / 16);
+                    bool more = false;
+#pragma unroll
+                    for (int h = 0; h < TERMS; ++h)
+                        for (int k = 0; k < g.dp / 16; ++k) {
+                            const uint32_t at = (uint32_t)(k >> 2) * (TILE * 128 / 16) + (k & 3) * 2;
+                            mma_ss(d_s, q + (uint32_t)h * (g.q_tile / TERMS / 16) + at, key + at, id_s, more);
+                            more = true;
+                        }
+                    mma_commit(&sh.s_full[s]);
+                    if (!PAIRED || s == 1) mma_commit(&sh.k_empty[ks]);
+                }
+                __syncwarp();
+            }
+        }
+        // what was issued has to end before the tensor memory is given back
+        if (lead) mma_commit(&sh.done);
+        __syncwarp();
+        mb_land(&sh.done, 0);
+    } else if (warp >= SOFT_WARPS) {
+        // ---- codes to f16: keys (and the scales), values ----
+        const bool values = warp >= SOFT_WARPS + CONV_WARPS;
+        const int cw = (warp - SOFT_WARPS) % CONV_WARPS, units = values ? g.vp / 32 : g.dp / 32;
+        auto wait = [&](uint64_t* bar, uint32_t parity) { return __all_sync(0xffffffffu, mb_wait(bar, parity, a.err_flag, &sh.abort_flag)); };
+        bool ok = true;
+        for (int b = 0; b < n; ++b) {
+            const int stages = values ? g.vst : g.kst, st = b % stages, slot[2] = {2 * b % g.raw, (2 * b + 1) % g.raw};
+            for (int pg = 0; pg < 2 && ok; ++pg) ok = wait(&sh.raw_full[slot[pg]], ((2 * b + pg) / g.raw) & 1);
+            if (ok && b >= stages) ok = wait(values ? &sh.v_empty[st] : &sh.k_empty[st], (b / stages - 1) & 1);
+            if (!ok) break;
+            if (!values) {
+                // scales, and what there is of the block.  What stood in their ring is four blocks old: the scores of the block two in front are done, whose place the keys take, or of
+                // the one in front, and its stream's products were done before those were begun
+                const int ring = b % RING, left = longest - (b0 + b) * BLOCK;
+                uint32_t top = 0;
+                int there = 0;
+                for (int ph = cw; ph < 4; ph += CONV_WARPS) {
+                    const unsigned char* from = base + g.raw_at + (size_t)slot[ph >> 1] * 2 * g.half + (size_t)(ph & 1) * g.half;
+                    sh.ks[ring][ph * 32 + lane] = reinterpret_cast<const float*>(from)[lane];
+                    sh.vs[ring][ph * 32 + lane] = reinterpret_cast<const float*>(from + g.kpart)[lane];
+                }
+                if (cw == 0) {
+                    for (int ph = 0; ph < 4; ++ph) {
+                        if (!sh.raw_there[slot[ph >> 1]]) continue;
+                        there |= 1 << (ph >> 1);
+                        const uint32_t v = __float_as_uint(reinterpret_cast<const float*>(base + g.raw_at + (size_t)slot[ph >> 1] * 2 * g.half + (size_t)(ph & 1) * g.half + g.kpart)[lane]);
+                        if (ph * 32 + lane < left && v < 0x7F800000u) top = max(top, v);
+                    }
+                    top = __reduce_max_sync(0xffffffffu, top);
+                    if (lane == 0) {
+                        sh.ve[ring] = (int)(top >> 23);
+                        sh.there[ring] = there;
+                    }
+                }
+                __syncwarp();
+                if (lane == 0) mb_arrive(&sh.sc_full[ring]);
+            }
+            // a warp takes 32 elements of a half at a time: a lane 16 elements of two tokens, 16 tokens of two elements
+            const int per_half = units;
+            for (int u = cw; u < 4 * per_half; u += CONV_WARPS) {
+                const int ph = u / per_half, q = u - ph * per_half;
+                const unsigned char* from = base + g.raw_at + (size_t)slot[ph >> 1] * 2 * g.half + (size_t)(ph & 1) * g.half + (values ? g.kpart : 0) + KV8_HALF * 4 + q * 1024;
+                unsigned char* tile = base + (values ? g.v_at + (size_t)st * g.v_tile + (size_t)(ph >> 1) * (g.v_tile / 2) + q * 32 * 128 : g.k_at + (size_t)st * g.k_tile + (size_t)(q >> 1) * (BLOCK * 128) + ph * KV8_HALF * 128);
+                const int c = lane & 1, chunk = ((values ? ph : q) & 1) * 4 + c * 2;
+                uint4 w[2];
+#pragma unroll
+                for (int i = 0; i < 2; ++i) w[i] = *reinterpret_cast<const uint4*>(from + ((lane >> 1) + 16 * i) * 32 + c * 16);
+#pragma unroll
+                for (int i = 0; i < 2; ++i) {
+                    const int r = (lane >> 1) + 16 * i, t = values ? r : ((r >> 1) & 3) * 8 + (r >> 3) * 2 + (r & 1);  // of keys: kv8_key_row(t) = r
+                    uint4 x, y;
+                    codes_f16(w[i].x, x.x, x.y);
+                    codes_f16(w[i].y, x.z, x.w);
+                    codes_f16(w[i].z, y.x, y.y);
+                    codes_f16(w[i].w, y.z, y.w);
+                    *reinterpret_cast<uint4*>(tile + t * 128 + ((chunk ^ (t & 7)) << 4)) = x;
+                    *reinterpret_cast<uint4*>(tile + t * 128 + (((chunk + 1) ^ (t & 7)) << 4)) = y;
+                }
+            }
+            fence_async_smem();
+            __syncwarp();
+            if (lane == 0) {
+                mb_arrive(values ? &sh.v_full[st] : &sh.k_full[st]);
+                mb_arrive(&sh.raw_empty[slot[0]]);
+                mb_arrive(&sh.raw_empty[slot[1]]);
+            }
+        }
+    } else {
+        // ---- scores to weights ----
+        const uint32_t lanes = (uint32_t)(warp & 3) * 32 << 16, s_at = tmem + lanes + (uint32_t)stream * BLOCK, o_at = tmem + lanes + 2 * BLOCK + (uint32_t)stream * 128;
+        float c = 0.f;  // what scores are multiplied with
+        if (n > 0) {
+            const size_t q_at = (size_t)row * a.ldq + (size_t)head * a.pool.dim;
+            auto load8 = [&](int d, float (&x)[8]) {
+#pragma unroll
+                for (int e = 0; e < 8; ++e) x[e] = 0.f;
+                if (!mine || d >= a.pool.dim) return;
+                if (wide & 2) {
+                    float y[4], z[4];
+                    load_row<BF16, 4>(a.q, q_at + d, y);
+                    load_row<BF16, 4>(a.q, q_at + d + 4, z);
+#pragma unroll
+                    for (int e = 0; e < 8; ++e) x[e] = e < 4 ? y[e & 3] : z[e & 3];
+                } else {
+#pragma unroll
+                    for (int e = 0; e < 8; ++e) {
+                        float one[1] = {0.f};
+                        if (d + e < a.pool.dim) load_row<BF16, 1>(a.q, q_at + d + e, one);
+                        x[e] = one[0];
+                    }
+                }
+            };
+            uint32_t top = 0;
+#pragma unroll 2
+            for (int d = 0; d < g.dp; d += 8) {
+                float x[8];
+                load8(d, x);
+#pragma unroll
+                for (int e = 0; e < 8; ++e) top = max(top, __float_as_uint(x[e]) & 0x7FFFFFFFu);
+            }
+            const bool finite = top < 0x7F800000u;
+            const int ex = min(max((int)(top >> 23), 15), 254);
+            const float up = finite ? __uint_as_float((uint32_t)(254 + 14 - ex) << 23) * (a.scale < 0.f ? -1.f : 1.f) : 0.f;
+            c = finite ? fabsf(a.scale) * LOG2E * exp2f((float)(ex - 127 - 14)) : __uint_as_float(0x7FC00000u);
+            if (PAIRED || stream == 0) {
+                unsigned char* to = base + g.q_at + (PAIRED ? stream * g.q_tile : 0u) + (tid & (TILE - 1)) * 128;
+#pragma unroll 1
+                for (int d = side * 32; d < g.katoms * 64; d += (d & 31) == 24 ? 40 : 8) {  // every other 32 elements
+                    float x[8];
+                    load8(d, x);
+                    uint32_t hi[4], lo[4];
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) {
+                        const float u = x[2 * e] * up, v = x[2 * e + 1] * up;
+                        hi[e] = f16x2(u, v);
+                        lo[e] = f16x2(u - f16_lo(hi[e]), v - f16_hi(hi[e]));
+                    }
+                    const size_t at = (size_t)(d >> 6) * (TILE * 128) + ((((d >> 3) & 7) ^ (tid & 7)) << 4);
+                    *reinterpret_cast<uint4*>(to + at) = make_uint4(hi[0], hi[1], hi[2], hi[3]);
+                    if (TERMS == 2) *reinterpret_cast<uint4*>(to + g.q_tile / 2 + at) = make_uint4(lo[0], lo[1], lo[2], lo[3]);
+                }
+                fence_async_smem();
+                __syncwarp();
+                if (lane == 0) mb_arrive(&sh.q_full);
+            }
+        }
+        bool ok = true;
+        float ref = -INFINITY, over = -INFINITY, l = 0.f;  // the pair's largest score at the last move; the exponent that value scales are brought down from; sum of the weights of this side
+        float unit = -INFINITY;                            // reference of the weights: ref + over - DROP
+        const int mine_n = PAIRED ? n : (n + 1 - stream) / 2, t0 = 64 * side;
+        for (int i = 0; i < mine_n; ++i) {
+            const int b = PAIRED ? i : 2 * i + stream, ring = b % RING;
+            ok = __all_sync(0xffffffffu, mb_wait(&sh.sc_full[ring], (b / RING) & 1, a.err_flag, &sh.abort_flag) && mb_wait(&sh.s_full[stream], i & 1, a.err_flag, &sh.abort_flag));
+            tc_fence_after();
+            const int seen = (sh.there[ring] >> side) & 1 ? len - (b0 + b) * BLOCK - t0 : 0;  // tokens of this side in front of the row's end
+            const bool masked = __any_sync(0xffffffffu, seen < 64);
+            // tokens c0 .. c0 + 31 of this side that are seen, a bit for each
+            auto visible = [&](int c0) -> uint32_t {
+                const int k = seen - c0;
+                return k <= 0 ? 0u : k >= 32 ? 0xffffffffu : (1u << k) - 1u;
+            };
+            const ulonglong2 *ks2 = reinterpret_cast<const ulonglong2*>(&sh.ks[ring][t0]), *vs2 = reinterpret_cast<const ulonglong2*>(&sh.vs[ring][t0]);  // two pairs of scales
+            // ---- the largest score of both sides ----
+            float top = -INFINITY;
+            auto find = [&](auto mask) {
+#pragma unroll 1
+                for (int c0 = 0; c0 < 64; c0 += 32) {
+                    uint32_t x[32];
+                    tmem_ld32(x, s_at + t0 + c0);
+                    const uint32_t vis = decltype(mask)::value ? visible(c0) : 0u;
+                    tmem_wait(x);
+#pragma unroll
+                    for (int e = 0; e < 32; e += 4) {
+                        const ulonglong2 k = ks2[(c0 + e) >> 2];
+                        const float2 y = of_pair(mul2(pair_of(x[e], x[e + 1]), k.x)), z = of_pair(mul2(pair_of(x[e + 2], x[e + 3]), k.y));
+                        if (decltype(mask)::value) {
+                            if ((vis >> e) & 1) top = fmaxf(top, y.x);
+                            if ((vis >> (e + 1)) & 1) top = fmaxf(top, y.y);
+                            if ((vis >> (e + 2)) & 1) top = fmaxf(top, z.x);
+                            if ((vis >> (e + 3)) & 1) top = fmaxf(top, z.y);
+                        } else {
+                            top = fmaxf(fmaxf(top, y.x), y.y);
+                            top = fmaxf(fmaxf(top, z.x), z.y);
+                        }
+                    }
+                }
+            };
+            if (masked) find(std::true_type{});
+            else find(std::false_type{});
+            sh.half[stream][i & 1][side][tid & (TILE - 1)] = top;  // two places in turn: the other side may be a block behind
+            if (both_any(stream * 4 + (warp & 3), !ok)) {
+                ok = false;
+                break;
+            }
+            top = fmaxf(top, sh.half[stream][i & 1][side ^ 1][tid & (TILE - 1)]);
+            // ---- the references, which move only where they have to ----
+            if (top > -INFINITY) {
+                top *= c;
+                if (!(top <= ref + SLACK)) ref = top;
+            }
+            const float ve = (float)(max(sh.ve[ring], 27) - 127);
+            if (ve > over) over = ve + VALUE_ROOM;
+            const float now = ref + over - DROP;  // -inf while the pair has seen nothing
+            if (i > 0 && __any_sync(0xffffffffu, now != unit)) {  // O is the product of the blocks so far: complete, since its stream's scores came behind it
+                const float corr = unit == -INFINITY || now == unit ? 1.f : exp2_ftz(unit - now);
+                l *= corr;
+#pragma unroll 1
+                for (int c0 = 16 * side; c0 < g.vp; c0 += 32) {
+                    uint32_t x[16];
+                    tmem_ld16(x, o_at + c0);
+                    tmem_wait16(x);
+#pragma unroll
+                    for (int e = 0; e < 16; ++e) x[e] = __float_as_uint(__uint_as_float(x[e]) * corr);
+                    tmem_st16(o_at + c0, x);
+                }
+            }
+            unit = now;
+            // ---- scores to weights ----
+            const float shift = now == -INFINITY ? 0.f : now;
+            const uint64_t c2 = pair_of(c, c), shift2 = pair_of(-shift, -shift);
+            uint64_t sum[2] = {0, 0};
+            auto weigh = [&](auto mask) {
+#pragma unroll 1
+                for (int c0 = 0; c0 < 64; c0 += 32) {
+                    uint32_t x[32], p[TERMS][16];
+                    tmem_ld32(x, s_at + t0 + c0);
+                    const uint32_t vis = decltype(mask)::value ? visible(c0) : 0u;
+                    tmem_wait(x);
+#pragma unroll
+                    for (int e = 0; e < 32; e += 4) {
+                        const ulonglong2 k = ks2[(c0 + e) >> 2], v = vs2[(c0 + e) >> 2];
+#pragma unroll
+                        for (int f = 0; f < 2; ++f) {
+                            float2 t = of_pair(fma2(mul2(pair_of(x[e + 2 * f], x[e + 2 * f + 1]), f ? k.y : k.x), c2, shift2));
+                            if (decltype(mask)::value) {
+                                if (!((vis >> (e + 2 * f)) & 1)) t.x = -INFINITY;
+                                if (!((vis >> (e + 2 * f + 1)) & 1)) t.y = -INFINITY;
+                            }
+                            const uint64_t pp = pair_of(exp2_ftz(t.x), exp2_ftz(t.y));
+                            sum[f] = add2(sum[f], pp);
+                            float2 w = of_pair(mul2(pp, f ? v.y : v.x));
+                            if (decltype(mask)::value) {  // scales of tokens that are not there may be anything
+                                if (!((vis >> (e + 2 * f)) & 1)) w.x = 0.f;
+                                if (!((vis >> (e + 2 * f + 1)) & 1)) w.y = 0.f;
+                            }
+                            uint32_t& hi = p[0][e / 2 + f];
+                            hi = f16x2(w.x, w.y);
+                            if (TERMS == 2) p[TERMS - 1][e / 2 + f] = f16x2(w.x - f16_lo(hi), w.y - f16_hi(hi));
+                        }
+                    }
+#pragma unroll
+                    for (int h = 0; h < TERMS; ++h) tmem_st16(s_at + t0 + c0 + 16 * h, p[h]);
+                }
+            };
+            if (masked) weigh(std::true_type{});
+            else weigh(std::false_type{});
+            const float2 sums = of_pair(add2(sum[0], sum[1]));
+            l += sums.x + sums.y;
+            tmem_st_wait();
+            tc_fence_before();
+            __syncwarp();
+            if (lane == 0) mb_arrive(&sh.p_full[stream]);
+        }
+        // all products are done: of this stream, and those that read what stands where the results go
+        ok = __all_sync(0xffffffffu, mb_wait(&sh.done, 0, a.err_flag, &sh.abort_flag)) && ok;
+        tc_fence_after();
+        // ---- what this stream has: into shared memory, where queries, keys and values stood ----
+        sh.half[stream][mine_n & 1][side][tid & (TILE - 1)] = l;
+        both_any(stream * 4 + (warp & 3), false);
+        l += sh.half[stream][mine_n & 1][side ^ 1][tid & (TILE - 1)];
+        float* to = reinterpret_cast<float*>(base) + (size_t)(stream * TILE + (tid & (TILE - 1))) * ldo;
+        if (side == 0) *reinterpret_cast<float2*>(to) = make_float2(unit == -INFINITY && l != 0.f ? 0.f : unit, l);  // a sum that is NaN is not passed over
+#pragma unroll 1
+        for (int c0 = 16 * side; c0 < g.vp; c0 += 32) {
+            uint32_t x[16];
+            tmem_ld16(x, o_at + c0);
+            tmem_wait16(x);
+            const bool some = ok && mine_n > 0;
+#pragma unroll
+            for (int e = 0; e < 16; e += 4) *reinterpret_cast<uint4*>(to + 4 + c0 + e) = some ? make_uint4(x[e], x[e + 1], x[e + 2], x[e + 3]) : make_uint4(0u, 0u, 0u, 0u);
+        }
+    }
+    __syncwarp();
+    tc_fence_before();
+    if (cluster > 1) cluster_sync_all();
+    else __syncthreads();
+    if (warp == MMA_WARP) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, 512;" ::"r"(tmem) : "memory");
+    // ---- the splits of a cluster (and the two streams of a tile) joined: a warp to a pair, the CTAs take turns ----
+    const int rank = cluster > 1 ? (int)cluster_ctarank() : 0, rows = PAIRED ? 2 * TILE : TILE, sources = PAIRED ? cluster : 2 * cluster;
+    for (int r = rank * (THREADS / 32) + warp; r < rows; r += cluster * (THREADS / 32)) {
+        const int p = tiles0 * TILE + r;
+        if (p >= pairs) break;
+        // source s: CTA s, or CTA s / 2 and stream s % 2
+        auto source = [&](int s) { return dsmem_addr(reinterpret_cast<const float*>(base) + (size_t)(PAIRED ? r : r + (s & 1) * TILE) * ldo, (uint32_t)(PAIRED ? s : s >> 1)); };
+        float m = -INFINITY, l = 0.f;
+        if (lane < sources) {
+            const uint32_t at = source(lane);
+            m = ld_dsmem_f32(at);
+            l = ld_dsmem_f32(at + 4);
+        }
+        const float top = warp_max(m), ref = top == -INFINITY ? 0.f : top, f = exp2f(m - ref);
+        l = warp_sum(f * l);
+        float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
+        for (int s = 0; s < sources; ++s) {
+            const float fs = __shfl_sync(0xffffffffu, f, s);
+            if (4 * lane >= g.vp) continue;
+            const float4 x = ld_dsmem_f32x4(source(s) + 16 + 16 * lane);
+            v.x = fmaf(fs, x.x, v.x); v.y = fmaf(fs, x.y, v.y); v.z = fmaf(fs, x.z, v.z); v.w = fmaf(fs, x.w, v.w);
+        }
+        float* to = parts + (((size_t)(split / cluster) * a.pool.kv_heads + kvh) * pairs + p) * (g.vp + 4);
+        if (lane == 0) *reinterpret_cast<float2*>(to) = make_float2(top, l);
+        if (4 * lane < g.vp) *reinterpret_cast<float4*>(to + 4 + 4 * lane) = v;
+    }
+    if (cluster > 1) cluster_sync_all();  // nobody leaves while a peer reads its shared memory
+}
+
+template <bool BF16, int TERMS, bool PAIRED>
+cudaError_t launch(const Kv8AttnArgs& a, const Kv8Prefix& p, float* parts, cudaStream_t st) {
+    const Shape g = shape_of(a.pool.dim, a.pool.vdim, TERMS, PAIRED ? 2 : 1);
+    const int size = BF16 ? 2 : 4, wide = a.pool.dim % 8 == 0 && (((uintptr_t)a.q | a.ldq * size) & (4 * size - 1)) == 0 ? 2 : 0;
+    const cudaError_t e = ensure_dyn_smem(kv8_prefix_kernel<BF16, TERMS, PAIRED>, g.bytes);
+    if (e != cudaSuccess) return e;
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3((unsigned)(p.groups * p.splits), (unsigned)a.pool.kv_heads);
+    cfg.blockDim = dim3(THREADS);
+    cfg.dynamicSmemBytes = g.bytes;
+    cfg.stream = st;
+    cudaLaunchAttribute at[1];
+    at[0].id = cudaLaunchAttributeClusterDimension;
+    at[0].val.clusterDim.x = (unsigned)p.cluster;
+    at[0].val.clusterDim.y = at[0].val.clusterDim.z = 1;
+    cfg.attrs = at;
+    cfg.numAttrs = p.cluster > 1 ? 1 : 0;
+    return cudaLaunchKernelEx(&cfg, kv8_prefix_kernel<BF16, TERMS, PAIRED>, a, p.splits, p.cluster, parts, wide);
+}
+
+// Clusters of CTAs that have an SM each which the current device holds at the same time; asked once per size.
+int clusters_at_once(int cluster, int sm_count) {
+    static std::mutex mu;
+    static std::map<std::pair<int, int>, int> known;
+    int dev = 0;
+    if (cudaGetDevice(&dev) != cudaSuccess) return sm_count / cluster;
+    std::lock_guard<std::mutex> lk(mu);
+    const auto key = std::make_pair(dev, cluster);
+    const auto it = known.find(key);
+    if (it != known.end()) return it->second;
+    int n = 0;
+    const size_t smem = shape_of(128, 128, 1, 2).bytes;
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3((unsigned)cluster);
+    cfg.blockDim = dim3(THREADS);
+    cfg.dynamicSmemBytes = smem;
+    cudaLaunchAttribute at[1];
+    at[0].id = cudaLaunchAttributeClusterDimension;
+    at[0].val.clusterDim.x = (unsigned)cluster;
+    at[0].val.clusterDim.y = at[0].val.clusterDim.z = 1;
+    cfg.attrs = at;
+    cfg.numAttrs = 1;
+    if (ensure_dyn_smem(kv8_prefix_kernel<true, 1, true>, smem) != cudaSuccess || cudaOccupancyMaxActiveClusters(&n, kv8_prefix_kernel<true, 1, true>, &cfg) != cudaSuccess) {
+        cudaGetLastError();
+        n = sm_count / cluster;
+    }
+    return known[key] = n;
+}
+
+}  // namespace
+
+Kv8Prefix kv8_prefix_plan(int kv_heads, int dim, int vdim, int bf16, int M, int heads, int n_shared, int sm_count) {
+    Kv8Prefix p{};
+    const long pairs = (long)M * (heads / kv_heads);
+    // wider heads do not fit tensor memory (two streams of scores and results) or shared memory; few pairs are one item of the streaming kernel anyway
+    if (n_shared < 1 || dim > 128 || vdim > 128 || pairs <= 8) return p;
+    const long tiles = (pairs + TILE - 1) / TILE;
+    p.paired = bf16 && tiles > 1;
+    const long groups = p.paired ? (tiles + 1) / 2 : tiles, items = groups * kv_heads, blocks = (n_shared + 1) / 2;
+    // A CTA per SM: splits and clusters with the least time, in blocks; four for a CTA's beginning and end, one for every part that is left to be joined.
+    const long most = std::min<long>({blocks, 64, std::max<long>(1, (2l * sm_count + items - 1) / items)});
+    double best = 0.0;
+    for (int cluster : {8, 4, 2, 1})
+        for (int s = cluster; s <= most && s <= cluster * MOST_PARTS; s += cluster) {
+            const long at_once = std::max(1, cluster > 1 ? clusters_at_once(cluster, sm_count) : sm_count);
+            const double cost = (double)((items * s / cluster + at_once - 1) / at_once) * ((double)((blocks + s - 1) / s) * (p.paired ? 2.0 : 1.0) + 4.0) + s / cluster;
+            if (p.splits == 0 || cost < best) {
+                best = cost;
+                p.splits = s;
+                p.cluster = cluster;
+            }
+        }
+    p.groups = (int)groups;
+    p.parts = p.splits / p.cluster;
+    return p;
+}
+
+int kv8_prefix_most_parts(int kv_heads, int M, int heads, int n_shared, int sm_count) {
+    const long tiles = ((long)M * (heads / kv_heads) + TILE - 1) / TILE, items = (tiles + 1) / 2 * kv_heads;
+    return (int)std::min<long>({(n_shared + 1) / 2, MOST_PARTS, std::max<long>(1, (2l * sm_count + items - 1) / items)});
+}
+
+cudaError_t launch_kv8_prefix(const Kv8AttnArgs& a, const Kv8Prefix& p, float* parts, cudaStream_t st) {
+    if (!a.bf16) return launch<false, 2, false>(a, p, parts, st);
+    return p.paired ? launch<true, 1, true>(a, p, parts, st) : launch<true, 1, false>(a, p, parts, st);
+}
+
+}  // namespace hm

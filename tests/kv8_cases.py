@@ -53,7 +53,7 @@ def attention(q, ks, vs, scale):
     return np.array(out), (np.array(mag), np.array(terms), np.array(full), np.array(wide))
 
 
-def bound(out, parts, bf16):
+def bound(out, parts, bf16, prefix=None):
     """Scores: sums of digits times codes are exact; a query's element is off by half of the last digit's step, 2^-30 (bf16 rows: 1 / 32639 / 2) of its largest one, the
     digits' sums and the factors are f32: together 2^-21 of the terms' magnitudes.  A weight is off by twice what its score is (itself and the sum it is divided by), and by half a
     step of its digits: 2^-31 (bf16 rows: 2^-16) of the largest weight times value among 32 tokens, so that these 32 are off by at most 2^-26 (2^-11) of the sum of their
@@ -61,6 +61,13 @@ def bound(out, parts, bf16):
     mag, terms, full, wide = parts
     e = 2 * (terms * 2.0**-21 + full * (2.0**-15.9 if bf16 else 2.0**-30))[..., None] + 2.0**-18
     tol = mag * e + wide[..., None] * (2.0**-11 if bf16 else 2.0**-26) + 1e-37
+    if prefix:
+        # Shared pages on their own: (tokens, largest value that any row sees).  Scores: products exact but for the f16 terms of a query (2^-22 of a value, bf16 rows exactly; no step
+        # below 2^-38 of the row's largest), a chain of at most 16 truncating sums of 2^-23: 2^-18.9.  A weight has one f16 term in bf16 rows (2^-11) or two (2^-22), and no step
+        # below 2^-24: half of it is 2^-28 of the weight 1 of the reference times the largest value, to each token's share.
+        n, largest = prefix
+        e = 2 * (terms * 2.0**-18.9 + full * 2.0**-38)[..., None] + 2.0**-18
+        tol = tol + mag * e + n * 2.0**-28 * largest + (mag * 2.0**-11 if bf16 else 0)
     return tol + np.abs(out) * 2.0**-8 if bf16 else tol
 
 
@@ -116,11 +123,13 @@ class Model:
         q = (self.rng.standard_normal((M, heads * self.dim)) * np.exp(0.5 * self.rng.standard_normal((M, 1)))).astype(np.float32)
         return bf16_bits(q) if bf16 else q
 
-    def check(self, out, q, row_seq, row_pos, heads, scale, seen=None):
+    def check(self, out, q, row_seq, row_pos, heads, scale, seen=None, shared=False):
         """Every row of out against the formula; rows of other sequences are not looked at.  seen(i): positions of sequence i that have a place."""
         bf16 = out.dtype == np.uint16
         o, x = (bf16_value(out), bf16_value(q)) if bf16 else (out, q)
         worst = 0.0
+        finite = lambda x: np.where(np.isfinite(x), x, 0)
+        prefix = (self.n_shared * PAGE, max([float(np.abs(finite(held(x))).max()) for x in [*self.v, self.common[1]] if x.size] + [0.0])) if shared else None
         for m, (i, p) in enumerate(zip(row_seq, row_pos)):
             if not 0 <= i < len(self.lens):
                 continue
@@ -129,7 +138,7 @@ class Model:
                 at = at[seen(i)[: len(at)]]
             k, v = held(self.k[i])[at].astype(np.float64), held(self.v[i])[at].astype(np.float64)
             want, parts = attention(x[m].astype(np.float64).reshape(heads, self.dim), k, v, scale)
-            err, tol = np.abs(o[m].reshape(heads, self.vdim) - want), bound(want, parts, bf16)
+            err, tol = np.abs(o[m].reshape(heads, self.vdim) - want), bound(want, parts, bf16, prefix)
             assert (err <= tol).all(), (m, i, p, float((err / tol).max()), float(err.max()))
             worst = max(worst, float((err / tol).max()))
         return worst

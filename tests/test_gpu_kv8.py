@@ -81,7 +81,7 @@ def attend(m, row_seq, row_pos, heads, bf16, scale=None, shared=False, seen=None
     scale = m.dim**-0.5 if scale is None else scale
     q = m.queries(M, heads, bf16)
     out = m.cache.attend(q, row_seq, row_pos, heads, scale, shared=m.shared if shared else None)
-    worst = m.check(out, q, row_seq, row_pos, heads, scale, seen)
+    worst = m.check(out, q, row_seq, row_pos, heads, scale, seen, shared)
     record_error(f"{what} {'bf16' if bf16 else 'f32'}, of the bound", worst, 1.0)
     return q, out
 
@@ -244,8 +244,8 @@ def test_shared_rows_of_no_sequence_and_nan_behind_a_row(hm):
     m.cache.write(m.k[0][150], bad, [0], [150])
     out = m.cache.attend(q, np.zeros(200, int), np.arange(200), 4, 0.125, shared=m.shared)
     assert np.isnan(out[150:]).all() and np.isfinite(out[:150]).all()
-    m.check(out[:150], q[:150], np.zeros(150, int), np.arange(150), 4, 0.125)
+    m.check(out[:150], q[:150], np.zeros(150, int), np.arange(150), 4, 0.125, shared=True)
     seq = np.where(np.arange(200) % 3 == 0, -1, 0)
     out = m.cache.attend(q[:150], seq[:150], np.arange(150), 4, 0.125, shared=m.shared)
     assert (out[0::3] == 0).all()
-    m.check(out, q[:150], seq[:150], np.arange(150), 4, 0.125)
+    m.check(out, q[:150], seq[:150], np.arange(150), 4, 0.125, shared=True)
