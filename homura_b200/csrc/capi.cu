@@ -1588,7 +1588,7 @@ int hm_kv8_read(const hm_kv8* cache, const int32_t* row_seq, const int32_t* row_
 }
 
 static bool bad_kv8_attn(const hm_kv8* c, int M, int heads, int n_shared) {
-    return M < 0 || M > KV8_MAX_ROWS || heads < 1 || heads > 4096 || heads % c->kv_heads != 0 || n_shared < 0 || n_shared > c->max_pages || (long long)M * c->max_pages > 1ll << 29;
+    return M < 0 || M > KV8_MAX_ROWS || heads < 1 || heads > 4096 || heads % c->kv_heads != 0 || n_shared < 0 || n_shared > c->max_pages || (long long)M * c->max_pages > std::min(1ll << 29, (1ll << 36) / heads);
 }
 
 size_t hm_kv8_attn_bytes(const hm_kv8* cache, int M, int heads, int n_shared) {
@@ -1600,7 +1600,7 @@ int hm_kv8_attn(const hm_kv8* cache, const void* q, int dtype, size_t ldq, const
                 void* stream) {
     if (bad_cache(cache) || bad_kv8_attn(cache, M, heads, n_shared) || !q || !out || !row_seq || !row_pos || (n_shared > 0 && !shared_pages) || !std::isfinite(scale) || bad_rows(M, (size_t)heads * cache->dim, ldq) ||
         bad_rows(M, (size_t)heads * cache->vdim, ldo))
-        return gfail(HM_ERR_INVALID, "hm_kv8_attn: bad arguments (M <= 8192, M * max_pages <= 2^29, heads <= 4096 and a multiple of kv_heads, dim and vdim <= 256, n_shared <= max_pages, ldq >= heads * dim, ldo >= heads * vdim)");
+        return gfail(HM_ERR_INVALID, "hm_kv8_attn: bad arguments (M <= 8192, M * max_pages <= 2^29 and 2^36 / heads, heads <= 4096 and a multiple of kv_heads, dim and vdim <= 256, n_shared <= max_pages, ldq >= heads * dim, ldo >= heads * vdim)");
     if (!is_row_dtype(dtype)) return gfail(HM_ERR_UNSUPPORTED, "hm_kv8_attn: rows are HM_F32 or HM_BF16");
     if (misaligned(cache->pages, 16) || misaligned(cache->page_table, 4) || misaligned(q, row_bytes(dtype)) || misaligned(out, row_bytes(dtype)) || misaligned(row_seq, 4) || misaligned(row_pos, 4) || misaligned(shared_pages, 4) ||
         misaligned(work, 16))

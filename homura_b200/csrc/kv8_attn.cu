@@ -37,14 +37,16 @@ namespace {
 
 constexpr int PAIRS = 8;           // of an item
 constexpr int LEAST_PIECES = 12;   // of a CTA, one for each of its warps: fewer would only leave more to be joined
+constexpr int BEGIN = 12;           // pieces that take a CTA as long as the beginning and end of an item
 constexpr int MAX_DEPTH = 4;
 constexpr int MERGE_ROWS = 32;      // pairs' results of several warps that stand in shared memory when those of all are added up
-constexpr size_t ROOM = 225 * 1024;  // shared memory of a CTA
+constexpr size_t ROOM = 222 * 1024;  // shared memory of a CTA, beside the static
 constexpr float LOG2E = 1.4426950408889634f;
 
-// ---- the line of pieces ------------------------------------------------------------------------------
+// ---- the line of pieces -----------------------------------------------------------------------------
+// An item is BEGIN units and one for every piece: what its queries, sums and barriers cost a CTA, so that those who have many short items have fewer pieces.
 struct Line {
-    long long total, chunk;  // pieces of all items; of a CTA
+    long long total, chunk;  // units of all items; of a CTA
     bool solo;               // there are items of a few pieces
 };
 
@@ -60,32 +62,38 @@ __device__ __forceinline__ int line_pieces(const Kv8AttnArgs& a, int m) {
     return n > a.solo ? n : 0;
 }
 
-// Every thread of the CTA adds up the pieces of some rows that follow one another, ceil(M / THREADS) of them; first[t]: pieces in front of thread t's rows,
-// first[THREADS]: of all.  Ends with a barrier.
+// Units in the lower half, rows that have pieces in the line in the upper.
+__device__ __forceinline__ int units_of(long long x) { return (int)(uint32_t)x; }
+__device__ __forceinline__ int rows_of(long long x) { return (int)(x >> 32); }
+
+// Every thread of the CTA adds up the units of some rows that follow one another, ceil(M / THREADS) of them; first[t]: units (of one item of each row) and rows in front of thread t's
+// rows, first[THREADS]: of all.  Ends with a barrier.
 template <int THREADS>
-__device__ __forceinline__ Line make_line(const Kv8AttnArgs& a, int items, int ctas, int* first) {
-    __shared__ int s_sum[THREADS / 32], s_most;
+__device__ __forceinline__ Line make_line(const Kv8AttnArgs& a, int items, int ctas, long long* first) {
+    __shared__ long long s_sum[THREADS / 32];
+    __shared__ int s_most;
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, per = (a.M + THREADS - 1) / THREADS, m0 = min(a.M, tid * per), m1 = min(a.M, m0 + per);
     if (tid == 0) s_most = 0;
-    int sum = 0, most = 0;
+    long long sum = 0;
+    int most = 0;
     bool solo = false;
     for (int m = m0; m < m1; ++m) {
         const int n = row_pieces(a, m);
-        if (n > a.solo) sum += n;
+        if (n > a.solo) sum += (1ll << 32) + n + BEGIN;
         else solo |= n > 0;
         most = max(most, n);
     }
-    int incl = sum;
+    long long incl = sum;
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
-        const int up = __shfl_up_sync(0xffffffffu, incl, o);
+        const long long up = __shfl_up_sync(0xffffffffu, incl, o);
         if (lane >= o) incl += up;
     }
     if (lane == 31) s_sum[warp] = incl;
     __syncthreads();
     most = __reduce_max_sync(0xffffffffu, most);
     if (lane == 0) atomicMax(&s_most, most);
-    int before = incl - sum, all = 0;
+    long long before = incl - sum, all = 0;
 #pragma unroll
     for (int w = 0; w < THREADS / 32; ++w) {
         if (w < warp) before += s_sum[w];
@@ -95,8 +103,8 @@ __device__ __forceinline__ Line make_line(const Kv8AttnArgs& a, int items, int c
     if (tid == 0) first[THREADS] = all;
     Line l;
     l.solo = __syncthreads_or(solo);
-    l.total = (long long)all * items;
-    l.chunk = max((l.total + ctas - 1) / ctas, (long long)min(LEAST_PIECES, s_most));
+    l.total = (long long)units_of(all) * items;
+    l.chunk = max((l.total + ctas - 1) / ctas, (long long)min(LEAST_PIECES, s_most) + BEGIN);
     return l;
 }
 
@@ -104,27 +112,36 @@ __device__ __forceinline__ Line make_line(const Kv8AttnArgs& a, int items, int c
 struct Segment {
     int m, item, at, n, of;  // row, its item, first piece (counted from own_from), pieces, pieces of the whole item
 };
+// The piece that unit u (of the line) stands for, or the item's first where it stands for the item's beginning (n is not set); `begin`: the item's first unit, `before`: pieces of
+// the line in front of this one.
 template <int THREADS>
-__device__ __forceinline__ Segment segment_at(const Kv8AttnArgs& a, const int* first, int items, long long u, long long end) {
+__device__ __forceinline__ Segment unit_at(const Kv8AttnArgs& a, const long long* first, int items, long long u, long long& begin, long long& before) {
     const bool small = (unsigned long long)u >> 32 == 0;
-    const int rank = small ? (int)((uint32_t)u / (uint32_t)items) : (int)(u / items);  // that many pieces of an item of every row are in front
-    int lo = 0, hi = THREADS;           // the last thread whose rows begin there or in front; those without pieces are passed over
+    const int rank = small ? (int)((uint32_t)u / (uint32_t)items) : (int)(u / items);  // that many units of an item of every row are in front
+    const int per = (a.M + THREADS - 1) / THREADS;
+    int lo = 0, hi = (a.M + per - 1) / per;  // the last thread whose rows begin there or in front; those without pieces are passed over
     while (hi - lo > 1) {
         const int mid = (lo + hi) / 2;
-        if (first[mid] <= rank) lo = mid;
+        if (units_of(first[mid]) <= rank) lo = mid;
         else hi = mid;
     }
     Segment s;
-    int at = first[lo];
-    s.m = lo * ((a.M + THREADS - 1) / THREADS);
-    for (s.of = line_pieces(a, s.m); rank >= at + s.of; s.of = line_pieces(a, ++s.m)) at += s.of;
-    const long long off = u - (long long)at * items;  // below of * items
-    s.item = small ? (int)((uint32_t)off / (uint32_t)s.of) : (int)(off / s.of);
-    s.at = (int)(off - (long long)s.item * s.of);
-    s.n = (int)min((long long)(s.of - s.at), end - u);
+    int at = units_of(first[lo]), rows = rows_of(first[lo]);
+    s.m = lo * per;
+    for (s.of = line_pieces(a, s.m); s.of == 0 || rank >= at + s.of + BEGIN; s.of = line_pieces(a, ++s.m)) {
+        at += s.of ? s.of + BEGIN : 0;
+        rows += s.of > 0;
+    }
+    const long long off = u - (long long)at * items;  // below (of + BEGIN) * items
+    const int units = s.of + BEGIN;
+    s.item = small ? (int)((uint32_t)off / (uint32_t)units) : (int)(off / units);
+    const int in = (int)(off - (long long)s.item * units);
+    begin = u - in;
+    s.at = max(0, in - BEGIN);
+    s.n = 0;
+    before = (long long)items * (at - rows * BEGIN) + (long long)s.item * s.of + s.at;
     return s;
 }
-
 // The segment behind s, `left` pieces from the end (not 0).
 __device__ __forceinline__ void next_segment(const Kv8AttnArgs& a, int items, Segment& s, int left) {
     s.at = 0;
@@ -197,6 +214,36 @@ __host__ __device__ inline StreamShape stream_shape(int dim, int vdim, int passe
     s.merge_at = s.q_at + 2 * sizeof(uint4) * s.queries;
     s.bytes = s.merge_at + sizeof(float) * MERGE_ROWS * s.ldo;
     return s;
+}
+
+// A query with the largest magnitude `top` (as bits): what its elements are multiplied with to be whole numbers (f32: a power of two that brings the largest to 2^29 .. 2^30; 0: the
+// query counts as zeros), and what its scores are multiplied with.
+template <bool BF16>
+__device__ __forceinline__ float query_factors(float scale, uint32_t top, float& up) {
+    const float most = __uint_as_float(top);
+    const bool some = top < 0x7F800000u && most >= Q_TINY;
+    const int ex = (int)(top >> 23);
+    up = !some ? 0.f : BF16 ? Q_MOST / most : pow2_bits(127 + 29 - (ex - 127));
+    const float down = !some ? 0.f : BF16 ? most / Q_MOST : exp2f((float)(ex - 127 - 29));
+    return top < 0x7F800000u ? scale * LOG2E * down : __uint_as_float(0x7FC00000u);
+}
+// Eight elements of a query as signed digits, the upper two first, a product 32 words of 16 bytes behind the other.
+template <bool BF16>
+__device__ __forceinline__ void put_digits(const float (&x)[8], float up, uint4* to) {
+    constexpr int PASSES = BF16 ? 1 : 2;
+    uint32_t y[2][4], d[2][2 * PASSES];
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+        const int whole = up != 0.f ? __float2int_rn(x[e] * up) : 0;
+        y[e >> 2][e & 3] = BF16 ? (uint32_t)(whole + 0x80) ^ 0x80u : (uint32_t)(whole + 0x808080) ^ 0x808080u;
+    }
+    digits_of<2 * PASSES>(y[0], d[0]);
+    digits_of<2 * PASSES>(y[1], d[1]);
+#pragma unroll
+    for (int h = 0; h < PASSES; ++h) {
+        const int k = 2 * (PASSES - 1 - h);
+        to[h * 32] = make_uint4(d[0][k + 1], d[0][k], d[1][k + 1], d[1][k]);
+    }
 }
 
 // What is left of an item in `work`: maximum and sum of every pair, then its elements (relative to the maximum, not divided).
@@ -282,7 +329,7 @@ __global__ void __launch_bounds__(WARPS * 32, 1) kv8_stream_kernel(const Kv8Attn
     extern __shared__ __align__(128) unsigned char dyn[];
     __shared__ uint64_t bars[WARPS][2][MAX_DEPTH];
     __shared__ volatile int s_abort;
-    __shared__ int first[THREADS + 1];
+    __shared__ long long first[THREADS + 1];
     __shared__ uint64_t s_added;         // the sums of the segment in front have been read
     __shared__ float s_c[2][PAIRS];      // what scores are multiplied with
     __shared__ float s_m[MERGE_ROWS], s_l[MERGE_ROWS];
@@ -304,7 +351,15 @@ __global__ void __launch_bounds__(WARPS * 32, 1) kv8_stream_kernel(const Kv8Attn
     }
     const Line line = make_line<THREADS>(a, items, ctas, first);
     const long long u0 = min(line.total, blockIdx.x * line.chunk), u1 = min(line.total, u0 + line.chunk);
-    const int count = (int)(u1 - u0);  // pieces of this CTA
+    Segment line_begin{};
+    int count = 0;  // pieces of this CTA
+    if (u0 < u1) {
+        long long begin, before, behind = (long long)items * (units_of(first[THREADS]) - rows_of(first[THREADS]) * BEGIN);
+        if (u1 < line.total) unit_at<THREADS>(a, first, items, u1, begin, behind);
+        line_begin = unit_at<THREADS>(a, first, items, u0, begin, before);
+        count = (int)(behind - before);
+        line_begin.n = min(line_begin.of - line_begin.at, count);
+    }
     pdl_launch_dependents();
 
     // ---- rows without a context (where there is a prefix, kv8_join_kernel writes them) ----
@@ -397,27 +452,10 @@ __global__ void __launch_bounds__(WARPS * 32, 1) kv8_stream_kernel(const Kv8Attn
         uint32_t top = 0;
 #pragma unroll
         for (int e = 0; e < 8; ++e) top = max(top, __float_as_uint(x[e]) & 0x7FFFFFFFu);
-        top = __reduce_max_sync(0xffffffffu, top);
-        const float most = __uint_as_float(top);
-        const bool some = top < 0x7F800000u && most >= Q_TINY;
-        const int ex = (int)(top >> 23);  // f32: a power of two brings the largest to 2^29 .. 2^30
-        const float up = !some ? 0.f : BF16 ? Q_MOST / most : pow2_bits(127 + 29 - (ex - 127)), down = !some ? 0.f : BF16 ? most / Q_MOST : exp2f((float)(ex - 127 - 29));
-        if (lane * 8 < sh.dp) {
-            uint32_t y[2][4], d[2][2 * PASSES];
-#pragma unroll
-            for (int e = 0; e < 8; ++e) {
-                const int whole = some ? __float2int_rn(x[e] * up) : 0;
-                y[e >> 2][e & 3] = BF16 ? (uint32_t)(whole + 0x80) ^ 0x80u : (uint32_t)(whole + 0x808080) ^ 0x808080u;  // signed digits
-            }
-            digits_of<2 * PASSES>(y[0], d[0]);
-            digits_of<2 * PASSES>(y[1], d[1]);
-#pragma unroll
-            for (int h = 0; h < PASSES; ++h) {  // the upper two digits first
-                const int k = 2 * (PASSES - 1 - h);
-                to[((lane >> 2) * PASSES + h) * 32 + pr * 4 + (lane & 3)] = make_uint4(d[0][k + 1], d[0][k], d[1][k + 1], d[1][k]);
-            }
-        }
-        return top < 0x7F800000u ? a.scale * LOG2E * down : __uint_as_float(0x7FC00000u);
+        float up;
+        const float f = query_factors<BF16>(a.scale, __reduce_max_sync(0xffffffffu, top), up);
+        if (lane * 8 < sh.dp) put_digits<BF16>(x, up, to + (lane >> 2) * PASSES * 32 + pr * 4 + (lane & 3));
+        return f;
     };
 
     const int gid = lane >> 2, tig = lane & 3, slabs = sh.dp / 32, vslabs = sh.vp / 32;
@@ -425,7 +463,7 @@ __global__ void __launch_bounds__(WARPS * 32, 1) kv8_stream_kernel(const Kv8Attn
     bool good = true;                         // no wait has run out
     bool alone = line.solo;                   // with items of this warp's own; then with the line
     int own = warp * ctas + (int)blockIdx.x;  // those are every WARPS * ctas-th of all
-    uint4* own_queries = reinterpret_cast<uint4*>(kbuf + sh.kpart);  // where the second slot's keys will stand
+    uint4* own_queries = reinterpret_cast<uint4*>(kbuf + (size_t)(depth - 1) * sh.kpart);  // where the last slot's keys will stand
     float next_q[8];
     int begin = 0, turn = 0;
     bool joined = false, waited = false;  // at the line; for the prefix
@@ -449,15 +487,48 @@ __global__ void __launch_bounds__(WARPS * 32, 1) kv8_stream_kernel(const Kv8Attn
             sg = Segment{m, own - m * items, 0, n, n};
             own += WARPS * ctas;
             __syncwarp();
-            start(sg, 0, n, 1, 1);
+            rings = depth - 1;
+            start(sg, 0, n, 1, rings);
             len = row_len(a, m);
             i = begin = slot = 0;
-            const int pairs = min(PAIRS, group - (sg.item % tiles) * PAIRS);
+            // lane (gid, tig): elements 8 tig .. 8 tig + 7 of every slab of pair gid
+            const int kvh = sg.item / tiles, tile = sg.item - kvh * tiles;
+            const bool is = gid < min(PAIRS, group - tile * PAIRS);
+            const size_t q_at = (size_t)m * a.ldq + (size_t)(kvh * group + tile * PAIRS + (is ? gid : 0)) * a.pool.dim + 8 * tig;
+            auto elements = [&](int s, float (&x)[8]) {
+                const int left = is ? a.pool.dim - (32 * s + 8 * tig) : 0;
+                if (wide & 2) {
+                    float y[2][4] = {};
+                    if (left > 0) {
+                        load_row<BF16, 4>(a.q, q_at + 32 * s, y[0]);
+                        load_row<BF16, 4>(a.q, q_at + 32 * s + 4, y[1]);
+                    }
+#pragma unroll
+                    for (int e = 0; e < 8; ++e) x[e] = y[e >> 2][e & 3];
+                } else {
+#pragma unroll
+                    for (int e = 0; e < 8; ++e) {
+                        float one[1] = {0.f};
+                        if (e < left) load_row<BF16, 1>(a.q, q_at + 32 * s + e, one);
+                        x[e] = one[0];
+                    }
+                }
+            };
+            uint32_t top = 0;
+#pragma unroll 4
+            for (int s = 0; s < slabs; ++s) {
+                elements(s, next_q);
+#pragma unroll
+                for (int e = 0; e < 8; ++e) top = max(top, __float_as_uint(next_q[e]) & 0x7FFFFFFFu);
+            }
+            top = max(top, __shfl_xor_sync(0xffffffffu, top, 1));
+            top = max(top, __shfl_xor_sync(0xffffffffu, top, 2));
+            float up;
+            c = query_factors<BF16>(a.scale, top, up);
 #pragma unroll 2
-            for (int pr = 0; pr < pairs; ++pr) {
-                fetch_query(sg, pr, next_q);
-                const float f = put_query(next_q, pr, own_queries);
-                if (gid == pr) c = f;
+            for (int s = 0; s < slabs; ++s) {
+                elements(s, next_q);
+                put_digits<BF16>(next_q, up, own_queries + s * PASSES * 32 + lane);
             }
             __syncwarp();
             qf = own_queries;
@@ -467,14 +538,14 @@ __global__ void __launch_bounds__(WARPS * 32, 1) kv8_stream_kernel(const Kv8Attn
                 if (count == 0) break;
                 asm volatile("fence.proxy.async.shared::cta;" ::: "memory");  // queries stood where pieces are copied to
                 __syncwarp();
-                sg = segment_at<THREADS>(a, first, items, u0, u1);
+                sg = line_begin;
                 rings = depth;
-                start(sg, warp, count, WARPS, depth);
+                if (warp < PAIRS) fetch_query(sg, warp, next_q);  // in front of the copies, behind which they would wait
+                start(sg, warp, count, WARPS, good ? depth : 0);  // nothing into slots whose copies were given up
                 len = row_len(a, sg.m);
                 i = warp;
                 begin = slot = 0;
                 if (warp < PAIRS) {
-                    fetch_query(sg, warp, next_q);
                     const float f = put_query(next_q, warp, queries);
                     if (lane == 0) s_c[0][warp] = f;
                 }
@@ -712,20 +783,20 @@ __global__ void __launch_bounds__(WARPS * 32, 1) kv8_stream_kernel(const Kv8Attn
         }
 }
 
-// One CTA per cut of the line: the item that a cut falls into, if the CTA in front of the cut holds its beginning.  A long context has a hundred parts and
-// more: the warps share them, every lane with its elements of all pairs of a part in flight at once.
-constexpr int JOIN_THREADS = 288;
+// One column of CTAs per cut of the line: the item that a cut falls into, if the CTA in front of the cut holds its beginning; a CTA has JOIN_PAIRS of its pairs.  A long context has a
+// hundred parts and more: the warps share them, every lane with its elements of several parts in flight at once.  The CTAs behind those have rows that have nothing but the prefix.
+constexpr int JOIN_THREADS = 256, JOIN_PAIRS = 2;
 template <bool BF16, int VS>
 __global__ void __launch_bounds__(JOIN_THREADS) kv8_join_kernel(const Kv8AttnArgs a, int ctas, int tiles, int wide) {
-    constexpr int THREADS = JOIN_THREADS, JW = THREADS / 32, NI = PAIRS * VS * 8 / 32;  // warps; groups of four elements a lane
-    extern __shared__ __align__(128) unsigned char dyn[];       // factors [parts][PAIRS], then the warps' sums
-    __shared__ float s_top[PAIRS], s_sum[PAIRS];
-    __shared__ int first[THREADS + 1];
+    constexpr int THREADS = JOIN_THREADS, JW = THREADS / 32, NI = JOIN_PAIRS * VS * 8 / 32, AHEAD = 4;  // warps; groups of four elements a lane; parts in flight
+    extern __shared__ __align__(128) unsigned char dyn[];                                               // factors [parts][JOIN_PAIRS], then the warps' sums
+    __shared__ float s_top[JOIN_PAIRS], s_sum[JOIN_PAIRS];
+    __shared__ long long first[THREADS + 1];
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, items = a.pool.kv_heads * tiles, group = a.heads / a.pool.kv_heads, cut = blockIdx.x + 1, vp = kv8_pad(a.pool.vdim), quads = vp / 4;
-    if (cut >= ctas) {  // rows that have nothing but the prefix
+    if (cut >= ctas) {
         pdl_wait();
-        const long all = (long)a.M * a.heads * quads, step = (long)(gridDim.x - (ctas - 1)) * THREADS;
-        for (long k = (long)(cut - ctas) * THREADS + tid; k < all; k += step) {
+        const long all = (long)a.M * a.heads * quads, step = (long)(gridDim.x - (ctas - 1)) * gridDim.y * THREADS;
+        for (long k = ((long)(cut - ctas) * gridDim.y + blockIdx.y) * THREADS + tid; k < all; k += step) {
             const int m = (int)(k / ((long)a.heads * quads)), r = (int)(k - (long)m * a.heads * quads), head = r / quads, d = (r - head * quads) * 4;
             if (row_pieces(a, m) > 0 || (unsigned)__ldg(a.row_seq + m) >= (unsigned)a.pool.n_seq) continue;
             float top = -INFINITY, sum = 0.f, v[4] = {0.f, 0.f, 0.f, 0.f};
@@ -737,28 +808,49 @@ __global__ void __launch_bounds__(JOIN_THREADS) kv8_join_kernel(const Kv8AttnArg
         return;
     }
     const Line line = make_line<THREADS>(a, items, ctas, first);
-    pdl_wait();
     const long long u = cut * line.chunk;
-    if (u >= line.total) return;
-    const Segment sg = segment_at<THREADS>(a, first, items, u, line.total);
-    const long long begin = u - sg.at, end = begin + sg.of;
-    if (sg.at == 0 || begin / line.chunk != cut - 1) return;
-    const int parts = (int)((end - 1) / line.chunk) - (cut - 1) + 1, kvh = sg.item / tiles, tile = sg.item - kvh * tiles, pairs = min(PAIRS, group - tile * PAIRS), head0 = kvh * group + tile * PAIRS;
+    bool mine = u < line.total;
+    long long begin = 0, before;
+    Segment sg{};
+    if (mine) {
+        sg = unit_at<THREADS>(a, first, items, u, begin, before);
+        mine = sg.at > 0 && (begin + BEGIN) / line.chunk == cut - 1;
+    }
+    const int kvh = sg.item / tiles, tile = sg.item - kvh * tiles, pr0 = (int)blockIdx.y * JOIN_PAIRS, pairs = min(JOIN_PAIRS, min(PAIRS, group - tile * PAIRS) - pr0), head0 = kvh * group + tile * PAIRS + pr0;
+    const int parts = mine ? (int)((begin + BEGIN + sg.of - 1) / line.chunk) - (cut - 1) + 1 : 0;
+    pdl_wait();
+    if (!mine || pairs <= 0) return;
     // the beginning is the second part of its CTA, what follows the first of theirs
-    auto part = [&](int i) -> const float* { return cta_part(a, vp, cut - 1 + i, i == 0); };
-    float* factor = reinterpret_cast<float*>(dyn);
-    float4* sums = reinterpret_cast<float4*>(dyn + (sizeof(float) * PAIRS * parts + 15) / 16 * 16);  // [JW][NI * 32]
-    for (int k = tid; k < parts * PAIRS; k += THREADS) factor[k] = k % PAIRS < pairs ? __ldcg(part(k / PAIRS) + (size_t)(k % PAIRS) * (vp + 4)) : -INFINITY;
+    auto part = [&](int i) -> const float* { return cta_part(a, vp, cut - 1 + i, i == 0) + (size_t)pr0 * (vp + 4); };
+    float2* ml = reinterpret_cast<float2*>(dyn);  // reference and sum, then factor and sum
+    float4* sums = reinterpret_cast<float4*>(dyn + (sizeof(float2) * JOIN_PAIRS * parts + 15) / 16 * 16);  // [JW][NI * 32]
+    for (int k = tid; k < parts * JOIN_PAIRS; k += THREADS) ml[k] = k % JOIN_PAIRS < pairs ? __ldcg(reinterpret_cast<const float2*>(part(k / JOIN_PAIRS) + (size_t)(k % JOIN_PAIRS) * (vp + 4))) : make_float2(-INFINITY, 0.f);
+    float4 acc[NI], x[AHEAD][NI];
+    int off[NI];  // where a lane's groups stand in a part
+#pragma unroll
+    for (int n = 0; n < NI; ++n) {
+        const int k = lane + 32 * n, pr = k / quads;
+        acc[n] = make_float4(0.f, 0.f, 0.f, 0.f);
+        off[n] = pr < pairs ? pr * (vp + 4) + 4 + (k - pr * quads) * 4 : -1;
+    }
+    auto fetch = [&](int i0) {
+#pragma unroll
+        for (int j = 0; j < AHEAD; ++j)
+#pragma unroll
+            for (int n = 0; n < NI; ++n) x[j][n] = i0 + j * JW < parts && off[n] >= 0 ? __ldcg(reinterpret_cast<const float4*>(part(i0 + j * JW) + off[n])) : make_float4(0.f, 0.f, 0.f, 0.f);
+    };
+    fetch(warp);  // on their way while the references are compared
     __syncthreads();
-    if (warp < PAIRS) {  // warp w: pair w
+    if (warp < JOIN_PAIRS) {  // warp w: pair w
         float top = -INFINITY, sum = 0.f;
-        for (int i = lane; i < parts; i += 32) top = fmaxf(top, factor[i * PAIRS + warp]);
+        for (int i = lane; i < parts; i += 32) top = fmaxf(top, ml[i * JOIN_PAIRS + warp].x);
         top = warp_max(top);
         const float ref = top == -INFINITY ? 0.f : top;
         for (int i = lane; i < parts; i += 32) {
-            const float f = exp2f(factor[i * PAIRS + warp] - ref);
-            factor[i * PAIRS + warp] = f;
-            if (warp < pairs) sum = fmaf(f, __ldcg(part(i) + (size_t)warp * (vp + 4) + 1), sum);
+            const float2 y = ml[i * JOIN_PAIRS + warp];
+            const float f = exp2f(y.x - ref);
+            ml[i * JOIN_PAIRS + warp].x = f;
+            sum = fmaf(f, y.y, sum);
         }
         sum = warp_sum(sum);
         if (lane == 0) {
@@ -767,23 +859,16 @@ __global__ void __launch_bounds__(JOIN_THREADS) kv8_join_kernel(const Kv8AttnArg
         }
     }
     __syncthreads();
-    float4 acc[NI];
-    int off[NI];  // where a lane's groups stand in a part
+    for (int i0 = warp; i0 < parts; i0 += AHEAD * JW) {
+        if (i0 > warp) fetch(i0);
 #pragma unroll
-    for (int n = 0; n < NI; ++n) {
-        const int k = lane + 32 * n, pr = k / quads;
-        acc[n] = make_float4(0.f, 0.f, 0.f, 0.f);
-        off[n] = pr < pairs ? pr * (vp + 4) + 4 + (k - pr * quads) * 4 : -1;
-    }
-    for (int i = warp; i < parts; i += JW) {
-        const float* at = part(i);
-        float4 x[NI];
+        for (int j = 0; j < AHEAD; ++j) {
+            if (i0 + j * JW >= parts) break;
 #pragma unroll
-        for (int n = 0; n < NI; ++n) x[n] = off[n] >= 0 ? __ldcg(reinterpret_cast<const float4*>(at + off[n])) : make_float4(0.f, 0.f, 0.f, 0.f);
-#pragma unroll
-        for (int n = 0; n < NI; ++n) {
-            const float f = factor[i * PAIRS + (lane + 32 * n) / quads % PAIRS];
-            acc[n].x = fmaf(f, x[n].x, acc[n].x); acc[n].y = fmaf(f, x[n].y, acc[n].y); acc[n].z = fmaf(f, x[n].z, acc[n].z); acc[n].w = fmaf(f, x[n].w, acc[n].w);
+            for (int n = 0; n < NI; ++n) {
+                const float f = ml[(i0 + j * JW) * JOIN_PAIRS + min((lane + 32 * n) / quads, JOIN_PAIRS - 1)].x;
+                acc[n].x = fmaf(f, x[j][n].x, acc[n].x); acc[n].y = fmaf(f, x[j][n].y, acc[n].y); acc[n].z = fmaf(f, x[j][n].z, acc[n].z); acc[n].w = fmaf(f, x[j][n].w, acc[n].w);
+            }
         }
     }
 #pragma unroll
@@ -794,11 +879,11 @@ __global__ void __launch_bounds__(JOIN_THREADS) kv8_join_kernel(const Kv8AttnArg
         float v[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
         for (int w = 0; w < JW; ++w) {
-            const float4 x = sums[w * NI * 32 + k];
-            v[0] += x.x; v[1] += x.y; v[2] += x.z; v[3] += x.w;
+            const float4 y = sums[w * NI * 32 + k];
+            v[0] += y.x; v[1] += y.y; v[2] += y.z; v[3] += y.w;
         }
         float top = s_top[pr], sum = s_sum[pr];
-        if (a.prefix_n) add_prefix(a, vp, kvh, sg.m * group + tile * PAIRS + pr, d, top, sum, v);
+        if (a.prefix_n) add_prefix(a, vp, kvh, sg.m * group + tile * PAIRS + pr0 + pr, d, top, sum, v);
         const float inv = sum == 0.f ? 0.f : 1.0f / sum;
         store2<BF16>(a, sg.m, head0 + pr, d, v[0] * inv, v[1] * inv, wide & 1);
         store2<BF16>(a, sg.m, head0 + pr, d + 2, v[2] * inv, v[3] * inv, wide & 1);
@@ -806,9 +891,9 @@ __global__ void __launch_bounds__(JOIN_THREADS) kv8_join_kernel(const Kv8AttnArg
 }
 
 template <typename... KArgs, typename... Args>
-cudaError_t launch_behind(void (*kern)(KArgs...), int grid, int threads, size_t smem, cudaStream_t st, Args... args) {
+cudaError_t launch_behind(void (*kern)(KArgs...), dim3 grid, int threads, size_t smem, cudaStream_t st, Args... args) {
     cudaLaunchConfig_t cfg = {};
-    cfg.gridDim = dim3((unsigned)grid);
+    cfg.gridDim = grid;
     cfg.blockDim = dim3((unsigned)threads);
     cfg.dynamicSmemBytes = smem;
     cfg.stream = st;
@@ -830,20 +915,21 @@ cudaError_t launch_stream(const Kv8AttnArgs& a_in, int sm_count, cudaStream_t st
     int depth = MAX_DEPTH;
     while (depth > 1 && bytes(depth) > ROOM) --depth;
     // a warp's own items need a second slot for their queries.  Where there are more items than CTAs, a CTA would take them one by one
-    a.solo = depth < 2 ? 0 : (long)a.M * a.pool.kv_heads * tiles >= 2 * sm_count ? 12 : 4;
-    const size_t smem = bytes(depth), join_smem = sizeof(float) * PAIRS * ctas + 16 + sizeof(float) * JOIN_THREADS * PAIRS * VS;
+    a.solo = depth >= 2 && (long)a.M * a.pool.kv_heads * tiles >= 2 * sm_count ? 12 : 0;
+    const size_t smem = bytes(depth), join_smem = sizeof(float2) * JOIN_PAIRS * ctas + 16 + sizeof(float) * JOIN_THREADS * JOIN_PAIRS * VS;
     cudaError_t e = ensure_dyn_smem(kv8_stream_kernel<BF16, VS, WARPS>, smem);
     if (e == cudaSuccess) e = ensure_dyn_smem(kv8_join_kernel<BF16, VS>, join_smem);
     if (e != cudaSuccess) return e;
     if (a.prefix_n) {
-        e = launch_behind(kv8_stream_kernel<BF16, VS, WARPS>, ctas, WARPS * 32, smem, st, a, depth, tiles, wide);
+        e = launch_behind(kv8_stream_kernel<BF16, VS, WARPS>, dim3((unsigned)ctas), WARPS * 32, smem, st, a, depth, tiles, wide);
     } else {
         kv8_stream_kernel<BF16, VS, WARPS><<<(unsigned)ctas, WARPS * 32, smem, st>>>(a, depth, tiles, wide);
         e = cudaGetLastError();
     }
     if (e != cudaSuccess) return e;
-    const long rest = a.prefix_n ? std::min(((long)a.M * a.heads * kv8_pad(a.pool.vdim) / 4 + JOIN_THREADS - 1) / JOIN_THREADS, 4096l) : 0;
-    return launch_behind(kv8_join_kernel<BF16, VS>, ctas - 1 + (int)rest, JOIN_THREADS, join_smem, st, a, ctas, tiles, wide);
+    const int columns = (std::min(group, PAIRS) + JOIN_PAIRS - 1) / JOIN_PAIRS;
+    const long rest = a.prefix_n ? std::min(((long)a.M * a.heads * kv8_pad(a.pool.vdim) / 4 + JOIN_THREADS * columns - 1) / (JOIN_THREADS * columns), 4096l) : 0;
+    return launch_behind(kv8_join_kernel<BF16, VS>, dim3((unsigned)(ctas - 1 + rest), (unsigned)columns), JOIN_THREADS, join_smem, st, a, ctas, tiles, wide);
 }
 
 // 12 warps (168 registers a thread) where their pieces fit, else eight.

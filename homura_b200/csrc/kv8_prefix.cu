@@ -336,6 +336,13 @@ __global__ void __launch_bounds__(THREADS, 1) kv8_prefix_kernel(const Kv8AttnArg
         const bool values = warp >= SOFT_WARPS + CONV_WARPS;
         const int cw = (warp - SOFT_WARPS) % CONV_WARPS, units = values ? g.vp / 32 : g.dp / 32;
         auto wait = [&](uint64_t* bar, uint32_t parity) { return __all_sync(0xffffffffu, mb_wait(bar, parity, a.err_flag, &sh.abort_flag)); };
+        // a lane's place in 32 rows of 32 bytes, and where its rows go: a 16-byte piece of a row of 128 bytes has its number turned by the row's
+        const int r0 = lane >> 1, c = lane & 1, part = (values ? g.kpart : 0) + KV8_HALF * 4 + r0 * 32 + c * 16;
+        auto place = [&](int r) {
+            const int t = values ? r : ((r >> 1) & 3) * 8 + (r >> 3) * 2 + (r & 1);  // of keys: kv8_key_row(t) = r
+            return t * 128 + (((2 * c) ^ (t & 7)) << 4);
+        };
+        const int off0 = place(r0), off1 = place(r0 + 16);
         bool ok = true;
         for (int b = 0; b < n; ++b) {
             const int stages = values ? g.vst : g.kst, st = b % stages, slot[2] = {2 * b % g.raw, (2 * b + 1) % g.raw};
@@ -369,26 +376,36 @@ __global__ void __launch_bounds__(THREADS, 1) kv8_prefix_kernel(const Kv8AttnArg
                 __syncwarp();
                 if (lane == 0) mb_arrive(&sh.sc_full[ring]);
             }
-            // a warp takes 32 elements of a half at a time: a lane 16 elements of two tokens, 16 tokens of two elements
-            const int per_half = units;
-            for (int u = cw; u < 4 * per_half; u += CONV_WARPS) {
-                const int ph = u / per_half, q = u - ph * per_half;
-                const unsigned char* from = base + g.raw_at + (size_t)slot[ph >> 1] * 2 * g.half + (size_t)(ph & 1) * g.half + (values ? g.kpart : 0) + KV8_HALF * 4 + q * 1024;
-                unsigned char* tile = base + (values ? g.v_at + (size_t)st * g.v_tile + (size_t)(ph >> 1) * (g.v_tile / 2) + q * 32 * 128 : g.k_at + (size_t)st * g.k_tile + (size_t)(q >> 1) * (BLOCK * 128) + ph * KV8_HALF * 128);
-                const int c = lane & 1, chunk = ((values ? ph : q) & 1) * 4 + c * 2;
-                uint4 w[2];
-#pragma unroll
-                for (int i = 0; i < 2; ++i) w[i] = *reinterpret_cast<const uint4*>(from + ((lane >> 1) + 16 * i) * 32 + c * 16);
-#pragma unroll
-                for (int i = 0; i < 2; ++i) {
-                    const int r = (lane >> 1) + 16 * i, t = values ? r : ((r >> 1) & 3) * 8 + (r >> 3) * 2 + (r & 1);  // of keys: kv8_key_row(t) = r
-                    uint4 x, y;
-                    codes_f16(w[i].x, x.x, x.y);
-                    codes_f16(w[i].y, x.z, x.w);
-                    codes_f16(w[i].z, y.x, y.y);
-                    codes_f16(w[i].w, y.z, y.w);
-                    *reinterpret_cast<uint4*>(tile + t * 128 + ((chunk ^ (t & 7)) << 4)) = x;
-                    *reinterpret_cast<uint4*>(tile + t * 128 + (((chunk + 1) ^ (t & 7)) << 4)) = y;
+            // a warp takes 32 elements of a half at a time: a lane 16 elements of two tokens, or 16 tokens of two elements
+            const unsigned char* raw[2] = {base + g.raw_at + (size_t)slot[0] * 2 * g.half + part, base + g.raw_at + (size_t)slot[1] * 2 * g.half + part};
+            unsigned char* tile = base + (values ? g.v_at + (uint32_t)st * g.v_tile : g.k_at + (uint32_t)st * g.k_tile);
+            int ph = 0, q = cw;
+            while (q >= units) {
+                q -= units;
+                ++ph;
+            }
+            while (ph < 4) {
+                const unsigned char* from = raw[ph >> 1] + (ph & 1) * g.half + q * 1024;
+                const uint4 w0 = *reinterpret_cast<const uint4*>(from), w1 = *reinterpret_cast<const uint4*>(from + 512);
+                unsigned char* to = tile + (values ? (uint32_t)(ph >> 1) * (g.v_tile / 2) + q * 4096 : (uint32_t)(q >> 1) * (BLOCK * 128) + ph * 4096);
+                const int flip = ((values ? ph : q) & 1) << 6;
+                uint4 x, y;
+                codes_f16(w0.x, x.x, x.y);
+                codes_f16(w0.y, x.z, x.w);
+                codes_f16(w0.z, y.x, y.y);
+                codes_f16(w0.w, y.z, y.w);
+                *reinterpret_cast<uint4*>(to + (off0 ^ flip)) = x;
+                *reinterpret_cast<uint4*>(to + (off0 ^ flip ^ 16)) = y;
+                codes_f16(w1.x, x.x, x.y);
+                codes_f16(w1.y, x.z, x.w);
+                codes_f16(w1.z, y.x, y.y);
+                codes_f16(w1.w, y.z, y.w);
+                *reinterpret_cast<uint4*>(to + (off1 ^ flip)) = x;
+                *reinterpret_cast<uint4*>(to + (off1 ^ flip ^ 16)) = y;
+                q += CONV_WARPS;
+                while (q >= units) {
+                    q -= units;
+                    ++ph;
                 }
             }
             fence_async_smem();
@@ -690,7 +707,7 @@ Kv8Prefix kv8_prefix_plan(int kv_heads, int dim, int vdim, int bf16, int M, int 
     // A CTA per SM: splits and clusters with the least time, in blocks; four for a CTA's beginning and end, one for every part that is left to be joined.
     const long most = std::min<long>({blocks, 64, std::max<long>(1, (2l * sm_count + items - 1) / items)});
     double best = 0.0;
-    for (int cluster : {8, 4, 2, 1})
+    for (int cluster = 8; cluster > 0; --cluster)
         for (int s = cluster; s <= most && s <= cluster * MOST_PARTS; s += cluster) {
             const long at_once = std::max(1, cluster > 1 ? clusters_at_once(cluster, sm_count) : sm_count);
             const double cost = (double)((items * s / cluster + at_once - 1) / at_once) * ((double)((blocks + s - 1) / s) * (p.paired ? 2.0 : 1.0) + 4.0) + s / cluster;
