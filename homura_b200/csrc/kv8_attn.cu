@@ -37,7 +37,7 @@ namespace {
 
 constexpr int PAIRS = 8;           // of an item
 constexpr int LEAST_PIECES = 12;   // of a CTA, one for each of its warps: fewer would only leave more to be joined
-constexpr int BEGIN = 12;           // pieces that take a CTA as long as the beginning and end of an item
+constexpr int BEGIN = 20;           // pieces that take a CTA as long as the beginning and end of an item
 constexpr int MAX_DEPTH = 4;
 constexpr int MERGE_ROWS = 32;      // pairs' results of several warps that stand in shared memory when those of all are added up
 constexpr size_t ROOM = 222 * 1024;  // shared memory of a CTA, beside the static

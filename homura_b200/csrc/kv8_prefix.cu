@@ -55,10 +55,10 @@ __host__ __device__ inline Shape shape_of(int dim, int vdim, int terms, int q_ti
     s.q_tile = (uint32_t)terms * s.katoms * TILE * 128;
     s.k_tile = (uint32_t)s.katoms * BLOCK * 128;
     s.v_tile = 2u * s.vp * 128;
-    // two blocks of values, then of keys, where they leave the ring four pages (two blocks); then as many pages as fit
+    // two blocks of values, then of keys, where they leave the ring three pages (a block and half of the next); then as many pages as fit
     const uint32_t page = 2u * s.half, room = (uint32_t)ROOM - 8192 - 1024 - q_tiles * s.q_tile;
-    s.vst = s.k_tile + 2 * s.v_tile + 4 * page <= room ? 2 : 1;
-    s.kst = 2 * s.k_tile + s.vst * s.v_tile + 4 * page <= room ? 2 : 1;
+    s.vst = s.k_tile + 2 * s.v_tile + 3 * page <= room ? 2 : 1;
+    s.kst = 2 * s.k_tile + s.vst * s.v_tile + 3 * page <= room ? 2 : 1;
     s.raw = (int)((room - s.kst * s.k_tile - s.vst * s.v_tile) / page);
     if (s.raw > MAX_RAW) s.raw = MAX_RAW;
     s.q_at = 0;
@@ -220,7 +220,7 @@ __global__ void __launch_bounds__(THREADS, 1) kv8_prefix_kernel(const Kv8AttnArg
             mb_init(&sh.pv_done[s], 1);
         }
         for (int s = 0; s < RING; ++s) mb_init(&sh.sc_full[s], CONV_WARPS);
-        mb_init(&sh.q_full, (PAIRED ? 2 : 1) * STREAM_WARPS);
+        mb_init(&sh.q_full, SOFT_WARPS);
         mb_init(&sh.done, 1);
         sh.abort_flag = 0;
         sh.longest = 0;
@@ -230,7 +230,7 @@ __global__ void __launch_bounds__(THREADS, 1) kv8_prefix_kernel(const Kv8AttnArg
     // ---- the pair of a thread of the first warps, and how far it sees; its page of the blocks ----
     const int stream = (warp >> 3) & 1, side = (warp >> 2) & 1, tile = tiles0 + (PAIRED ? stream : 0), pair = tile * TILE + (tid & (TILE - 1));
     const bool mine = warp < SOFT_WARPS && pair < pairs;
-    const int row = mine ? pair / group : 0, head = kvh * group + (mine ? pair - row * group : 0);
+    const int row = mine ? pair / group : 0;
     int len = 0;
     if (mine) {
         const int seq = __ldg(a.row_seq + row);
@@ -289,8 +289,8 @@ __global__ void __launch_bounds__(THREADS, 1) kv8_prefix_kernel(const Kv8AttnArg
             const uint32_t d_s = tmem + (uint32_t)s * BLOCK, d_o = tmem + 2 * BLOCK + (uint32_t)s * 128;
             if (j >= 2) {  // the product of task j - 2
                 const int t = j - 2, b = block_of(t);
-                const int vs = b % g.vst;
-                if ((!PAIRED || s == 0) && !(ok = wait(&sh.v_full[vs], (b / g.vst) & 1))) break;
+                const int vs = b & (g.vst - 1);  // one stage or two
+                if ((!PAIRED || s == 0) && !(ok = wait(&sh.v_full[vs], (b >> (g.vst - 1)) & 1))) break;
                 if (!(ok = wait(&sh.p_full[s], (t >> 1) & 1))) break;
                 tc_fence_after();
                 const uint32_t v = v_lo + (uint32_t)vs * (g.v_tile / 16);
@@ -307,8 +307,8 @@ __global__ void __launch_bounds__(THREADS, 1) kv8_prefix_kernel(const Kv8AttnArg
             }
             if (j < tasks) {
                 const int b = block_of(j);
-                const int ks = b % g.kst;
-                if ((!PAIRED || s == 0) && !(ok = wait(&sh.k_full[ks], (b / g.kst) & 1))) break;
+                const int ks = b & (g.kst - 1);
+                if ((!PAIRED || s == 0) && !(ok = wait(&sh.k_full[ks], (b >> (g.kst - 1)) & 1))) break;
                 if (j >= 2 && !(ok = wait(&sh.pv_done[s], ((j - 2) >> 1) & 1))) break;  // the weights stand where the scores go
                 tc_fence_after();
                 if (lead) {
@@ -343,11 +343,23 @@ __global__ void __launch_bounds__(THREADS, 1) kv8_prefix_kernel(const Kv8AttnArg
             return t * 128 + (((2 * c) ^ (t & 7)) << 4);
         };
         const int off0 = place(r0), off1 = place(r0 + 16);
+        const int more = (values ? g.vst : g.kst) - 1;  // stages but one
+        int next = 0;                                   // slot of the next page, and the parity of its wait
+        uint32_t parity = 0;
         bool ok = true;
         for (int b = 0; b < n; ++b) {
-            const int stages = values ? g.vst : g.kst, st = b % stages, slot[2] = {2 * b % g.raw, (2 * b + 1) % g.raw};
-            for (int pg = 0; pg < 2 && ok; ++pg) ok = wait(&sh.raw_full[slot[pg]], ((2 * b + pg) / g.raw) & 1);
-            if (ok && b >= stages) ok = wait(values ? &sh.v_empty[st] : &sh.k_empty[st], (b / stages - 1) & 1);
+            const int st = b & more;
+            int slot[2];
+#pragma unroll
+            for (int pg = 0; pg < 2; ++pg) {
+                slot[pg] = next;
+                ok = ok && wait(&sh.raw_full[next], parity);
+                if (++next == g.raw) {
+                    next = 0;
+                    parity ^= 1u;
+                }
+            }
+            if (ok && b > more) ok = wait(values ? &sh.v_empty[st] : &sh.k_empty[st], ((b >> more) - 1) & 1);
             if (!ok) break;
             if (!values) {
                 // scales, and what there is of the block.  What stood in their ring is four blocks old: the scores of the block two in front are done, whose place the keys take, or of
@@ -379,34 +391,49 @@ __global__ void __launch_bounds__(THREADS, 1) kv8_prefix_kernel(const Kv8AttnArg
             // a warp takes 32 elements of a half at a time: a lane 16 elements of two tokens, or 16 tokens of two elements
             const unsigned char* raw[2] = {base + g.raw_at + (size_t)slot[0] * 2 * g.half + part, base + g.raw_at + (size_t)slot[1] * 2 * g.half + part};
             unsigned char* tile = base + (values ? g.v_at + (uint32_t)st * g.v_tile : g.k_at + (uint32_t)st * g.k_tile);
-            int ph = 0, q = cw;
-            while (q >= units) {
-                q -= units;
-                ++ph;
-            }
-            while (ph < 4) {
-                const unsigned char* from = raw[ph >> 1] + (ph & 1) * g.half + q * 1024;
-                const uint4 w0 = *reinterpret_cast<const uint4*>(from), w1 = *reinterpret_cast<const uint4*>(from + 512);
-                unsigned char* to = tile + (values ? (uint32_t)(ph >> 1) * (g.v_tile / 2) + q * 4096 : (uint32_t)(q >> 1) * (BLOCK * 128) + ph * 4096);
-                const int flip = ((values ? ph : q) & 1) << 6;
+            struct Unit {
+                int ph, q;
+                uint4 w0, w1;
+            };
+            auto settle = [&](Unit& u) {
+                while (u.q >= units) {
+                    u.q -= units;
+                    ++u.ph;
+                }
+                if (u.ph >= 4) return;
+                const unsigned char* from = raw[u.ph >> 1] + (u.ph & 1) * g.half + u.q * 1024;
+                u.w0 = *reinterpret_cast<const uint4*>(from);
+                u.w1 = *reinterpret_cast<const uint4*>(from + 512);
+            };
+            auto convert = [&](const Unit& u) {
+                unsigned char* to = tile + (values ? (uint32_t)(u.ph >> 1) * (g.v_tile / 2) + u.q * 4096 : (uint32_t)(u.q >> 1) * (BLOCK * 128) + u.ph * 4096);
+                const int flip = ((values ? u.ph : u.q) & 1) << 6;
                 uint4 x, y;
-                codes_f16(w0.x, x.x, x.y);
-                codes_f16(w0.y, x.z, x.w);
-                codes_f16(w0.z, y.x, y.y);
-                codes_f16(w0.w, y.z, y.w);
+                codes_f16(u.w0.x, x.x, x.y);
+                codes_f16(u.w0.y, x.z, x.w);
+                codes_f16(u.w0.z, y.x, y.y);
+                codes_f16(u.w0.w, y.z, y.w);
                 *reinterpret_cast<uint4*>(to + (off0 ^ flip)) = x;
                 *reinterpret_cast<uint4*>(to + (off0 ^ flip ^ 16)) = y;
-                codes_f16(w1.x, x.x, x.y);
-                codes_f16(w1.y, x.z, x.w);
-                codes_f16(w1.z, y.x, y.y);
-                codes_f16(w1.w, y.z, y.w);
+                codes_f16(u.w1.x, x.x, x.y);
+                codes_f16(u.w1.y, x.z, x.w);
+                codes_f16(u.w1.z, y.x, y.y);
+                codes_f16(u.w1.w, y.z, y.w);
                 *reinterpret_cast<uint4*>(to + (off1 ^ flip)) = x;
                 *reinterpret_cast<uint4*>(to + (off1 ^ flip ^ 16)) = y;
-                q += CONV_WARPS;
-                while (q >= units) {
-                    q -= units;
-                    ++ph;
-                }
+            };
+            Unit u{0, cw}, v;
+            settle(u);
+            while (u.ph < 4) {  // one is loaded while another is converted
+                v.ph = u.ph;
+                v.q = u.q + CONV_WARPS;
+                settle(v);
+                convert(u);
+                if (v.ph >= 4) break;
+                u.ph = v.ph;
+                u.q = v.q + CONV_WARPS;
+                settle(u);
+                convert(v);
             }
             fence_async_smem();
             __syncwarp();
@@ -421,59 +448,57 @@ __global__ void __launch_bounds__(THREADS, 1) kv8_prefix_kernel(const Kv8AttnArg
         const uint32_t lanes = (uint32_t)(warp & 3) * 32 << 16, s_at = tmem + lanes + (uint32_t)stream * BLOCK, o_at = tmem + lanes + 2 * BLOCK + (uint32_t)stream * 128;
         float c = 0.f;  // what scores are multiplied with
         if (n > 0) {
-            const size_t q_at = (size_t)row * a.ldq + (size_t)head * a.pool.dim;
-            auto load8 = [&](int d, float (&x)[8]) {
+            // a warp takes pairs one by one, four elements a lane, so that a row is read by neighbours; several are on their way at once
+            constexpr int MINE = (PAIRED ? 2 : 1) * TILE / SOFT_WARPS, AHEAD = 4;
+            const int d = 4 * lane;
+            for (int r0 = warp * MINE; r0 < (warp + 1) * MINE; r0 += AHEAD) {
+                float x[AHEAD][4];
 #pragma unroll
-                for (int e = 0; e < 8; ++e) x[e] = 0.f;
-                if (!mine || d >= a.pool.dim) return;
-                if (wide & 2) {
-                    float y[4], z[4];
-                    load_row<BF16, 4>(a.q, q_at + d, y);
-                    load_row<BF16, 4>(a.q, q_at + d + 4, z);
+                for (int k = 0; k < AHEAD; ++k) {
+                    const int p = tiles0 * TILE + r0 + k, m = p / group;
+                    const size_t at = (size_t)m * a.ldq + (size_t)(kvh * group + p - m * group) * a.pool.dim + d;
 #pragma unroll
-                    for (int e = 0; e < 8; ++e) x[e] = e < 4 ? y[e & 3] : z[e & 3];
-                } else {
+                    for (int e = 0; e < 4; ++e) x[k][e] = 0.f;
+                    if (p >= pairs || d >= a.pool.dim) continue;
+                    if (wide & 2) {
+                        load_row<BF16, 4>(a.q, at, x[k]);
+                    } else {
 #pragma unroll
-                    for (int e = 0; e < 8; ++e) {
-                        float one[1] = {0.f};
-                        if (d + e < a.pool.dim) load_row<BF16, 1>(a.q, q_at + d + e, one);
-                        x[e] = one[0];
+                        for (int e = 0; e < 4; ++e) {
+                            float one[1] = {0.f};
+                            if (d + e < a.pool.dim) load_row<BF16, 1>(a.q, at + e, one);
+                            x[k][e] = one[0];
+                        }
                     }
                 }
-            };
-            uint32_t top = 0;
-#pragma unroll 2
-            for (int d = 0; d < g.dp; d += 8) {
-                float x[8];
-                load8(d, x);
 #pragma unroll
-                for (int e = 0; e < 8; ++e) top = max(top, __float_as_uint(x[e]) & 0x7FFFFFFFu);
-            }
-            const bool finite = top < 0x7F800000u;
-            const int ex = min(max((int)(top >> 23), 15), 254);
-            const float up = finite ? __uint_as_float((uint32_t)(254 + 14 - ex) << 23) * (a.scale < 0.f ? -1.f : 1.f) : 0.f;
-            c = finite ? fabsf(a.scale) * LOG2E * exp2f((float)(ex - 127 - 14)) : __uint_as_float(0x7FC00000u);
-            if (PAIRED || stream == 0) {
-                unsigned char* to = base + g.q_at + (PAIRED ? stream * g.q_tile : 0u) + (tid & (TILE - 1)) * 128;
-#pragma unroll 1
-                for (int d = side * 32; d < g.katoms * 64; d += (d & 31) == 24 ? 40 : 8) {  // every other 32 elements
-                    float x[8];
-                    load8(d, x);
-                    uint32_t hi[4], lo[4];
+                for (int k = 0; k < AHEAD; ++k) {
+                    uint32_t top = 0;
 #pragma unroll
-                    for (int e = 0; e < 4; ++e) {
-                        const float u = x[2 * e] * up, v = x[2 * e + 1] * up;
+                    for (int e = 0; e < 4; ++e) top = max(top, __float_as_uint(x[k][e]) & 0x7FFFFFFFu);
+                    top = __reduce_max_sync(0xffffffffu, top);
+                    const bool finite = top < 0x7F800000u;
+                    const int ex = min(max((int)(top >> 23), 15), 254), r = r0 + k;
+                    const float up = finite ? __uint_as_float((uint32_t)(254 + 14 - ex) << 23) * (a.scale < 0.f ? -1.f : 1.f) : 0.f;
+                    if (lane < (PAIRED ? 1 : 2)) sh.half[PAIRED ? r >> 7 : lane][1][0][r & (TILE - 1)] = finite ? fabsf(a.scale) * LOG2E * exp2f((float)(ex - 127 - 14)) : __uint_as_float(0x7FC00000u);
+                    if (d >= g.katoms * 64) continue;
+                    uint32_t hi[2], lo[2];
+#pragma unroll
+                    for (int e = 0; e < 2; ++e) {
+                        const float u = x[k][2 * e] * up, v = x[k][2 * e + 1] * up;
                         hi[e] = f16x2(u, v);
                         lo[e] = f16x2(u - f16_lo(hi[e]), v - f16_hi(hi[e]));
                     }
-                    const size_t at = (size_t)(d >> 6) * (TILE * 128) + ((((d >> 3) & 7) ^ (tid & 7)) << 4);
-                    *reinterpret_cast<uint4*>(to + at) = make_uint4(hi[0], hi[1], hi[2], hi[3]);
-                    if (TERMS == 2) *reinterpret_cast<uint4*>(to + g.q_tile / 2 + at) = make_uint4(lo[0], lo[1], lo[2], lo[3]);
+                    unsigned char* to = base + g.q_at + (uint32_t)(r >> 7) * g.q_tile + (d >> 6) * (TILE * 128) + (r & (TILE - 1)) * 128 + ((((d >> 3) & 7) ^ (r & 7)) << 4) + (d & 4) * 2;
+                    *reinterpret_cast<uint2*>(to) = make_uint2(hi[0], hi[1]);
+                    if (TERMS == 2) *reinterpret_cast<uint2*>(to + g.q_tile / 2) = make_uint2(lo[0], lo[1]);
                 }
-                fence_async_smem();
-                __syncwarp();
-                if (lane == 0) mb_arrive(&sh.q_full);
             }
+            fence_async_smem();
+            __syncwarp();
+            if (lane == 0) mb_arrive(&sh.q_full);
+            asm volatile("barrier.cta.sync.aligned 9, %0;" ::"n"(SOFT_WARPS * 32) : "memory");
+            c = sh.half[stream][1][0][tid & (TILE - 1)];  // both warps that have a pair read it in front of their first barrier, behind which the place is written again
         }
         bool ok = true;
         float ref = -INFINITY, over = -INFINITY, l = 0.f;  // the pair's largest score at the last move; the exponent that value scales are brought down from; sum of the weights of this side
