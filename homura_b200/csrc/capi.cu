@@ -1536,7 +1536,7 @@ int hm_rope(const void* x, int dtype, size_t ldx, int M, int heads, int dim, int
     a.magnitude = magnitude;
     if (!a.x || !a.y || !a.pos || (rot > 0 && !a.turns)) return sg.finish(cudaErrorMemoryAllocation);
     if (sg.elsewhere()) return gfail(HM_ERR_INVALID, "hm_rope: memory of another device than the current one");
-    return sg.finish(launch_rope(a, st));
+    return sg.finish(launch_rope(a, sm_count_of_current_device(), st));
 }
 
 // Sizes that a cache of 8 bits cannot have.

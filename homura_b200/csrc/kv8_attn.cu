@@ -785,7 +785,7 @@ __global__ void __launch_bounds__(WARPS * 32, 1) kv8_stream_kernel(const Kv8Attn
 
 // One column of CTAs per cut of the line: the item that a cut falls into, if the CTA in front of the cut holds its beginning; a CTA has JOIN_PAIRS of its pairs.  A long context has a
 // hundred parts and more: the warps share them, every lane with its elements of several parts in flight at once.  The CTAs behind those have rows that have nothing but the prefix.
-constexpr int JOIN_THREADS = 256, JOIN_PAIRS = 2;
+constexpr int JOIN_THREADS = 256, JOIN_PAIRS = 2, JOIN_HEADS = 4;
 template <bool BF16, int VS>
 __global__ void __launch_bounds__(JOIN_THREADS) kv8_join_kernel(const Kv8AttnArgs a, int ctas, int tiles, int wide) {
     constexpr int THREADS = JOIN_THREADS, JW = THREADS / 32, NI = JOIN_PAIRS * VS * 8 / 32, AHEAD = 4;  // warps; groups of four elements a lane; parts in flight
@@ -795,15 +795,56 @@ __global__ void __launch_bounds__(JOIN_THREADS) kv8_join_kernel(const Kv8AttnArg
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, items = a.pool.kv_heads * tiles, group = a.heads / a.pool.kv_heads, cut = blockIdx.x + 1, vp = kv8_pad(a.pool.vdim), quads = vp / 4;
     if (cut >= ctas) {
         pdl_wait();
-        const long all = (long)a.M * a.heads * quads, step = (long)(gridDim.x - (ctas - 1)) * gridDim.y * THREADS;
-        for (long k = ((long)(cut - ctas) * gridDim.y + blockIdx.y) * THREADS + tid; k < all; k += step) {
-            const int m = (int)(k / ((long)a.heads * quads)), r = (int)(k - (long)m * a.heads * quads), head = r / quads, d = (r - head * quads) * 4;
-            if (row_pieces(a, m) > 0 || (unsigned)__ldg(a.row_seq + m) >= (unsigned)a.pool.n_seq) continue;
-            float top = -INFINITY, sum = 0.f, v[4] = {0.f, 0.f, 0.f, 0.f};
-            add_prefix(a, vp, head / group, m * group + head % group, d, top, sum, v);
-            const float inv = sum == 0.f ? 0.f : 1.0f / sum;
-            store2<BF16>(a, m, head, d, v[0] * inv, v[1] * inv, wide & 1);
-            store2<BF16>(a, m, head, d + 2, v[2] * inv, v[3] * inv, wide & 1);
+        // a warp to JOIN_HEADS heads of all rows at a time, four elements a lane
+        const int all = a.M * a.heads, step = ((int)gridDim.x - (ctas - 1)) * (int)gridDim.y * JW * JOIN_HEADS;
+        const size_t all_pairs = (size_t)a.M * group, part = (size_t)a.pool.kv_heads * all_pairs * (vp + 4);
+        for (int k = ((((cut - ctas) * (int)gridDim.y + (int)blockIdx.y) * JW) + warp) * JOIN_HEADS; k < all; k += step) {
+            int m[JOIN_HEADS], head[JOIN_HEADS];
+            const float* at[JOIN_HEADS];
+            bool is[JOIN_HEADS];
+#pragma unroll
+            for (int j = 0; j < JOIN_HEADS; ++j) {
+                const int r = min(k + j, all - 1);
+                m[j] = r / a.heads;
+                head[j] = r - m[j] * a.heads;
+                const int kvh = head[j] / group;
+                at[j] = a.prefix + ((size_t)kvh * all_pairs + (size_t)m[j] * group + (head[j] - kvh * group)) * (vp + 4);
+                is[j] = k + j < all && row_pieces(a, m[j]) == 0 && (unsigned)__ldg(a.row_seq + m[j]) < (unsigned)a.pool.n_seq;
+            }
+            for (int d = 4 * lane; d < vp; d += 128) {
+                float top[JOIN_HEADS], sum[JOIN_HEADS];
+                float4 v[JOIN_HEADS];
+#pragma unroll
+                for (int j = 0; j < JOIN_HEADS; ++j) {
+                    top[j] = -INFINITY;
+                    sum[j] = 0.f;
+                    v[j] = make_float4(0.f, 0.f, 0.f, 0.f);
+                }
+                for (int i = 0; i < a.prefix_n; ++i) {
+                    float2 ml[JOIN_HEADS];
+                    float4 x[JOIN_HEADS];
+#pragma unroll
+                    for (int j = 0; j < JOIN_HEADS; ++j) {
+                        ml[j] = is[j] ? __ldcg(reinterpret_cast<const float2*>(at[j] + i * part)) : make_float2(-INFINITY, 0.f);
+                        x[j] = is[j] ? __ldcg(reinterpret_cast<const float4*>(at[j] + i * part + 4 + d)) : make_float4(0.f, 0.f, 0.f, 0.f);
+                    }
+#pragma unroll
+                    for (int j = 0; j < JOIN_HEADS; ++j) {
+                        if (ml[j].x == -INFINITY) continue;  // nothing seen
+                        const float now = fmaxf(top[j], ml[j].x), f0 = exp2f(top[j] - now), f1 = exp2f(ml[j].x - now);
+                        top[j] = now;
+                        sum[j] = fmaf(f1, ml[j].y, sum[j] * f0);
+                        v[j].x = fmaf(f1, x[j].x, v[j].x * f0); v[j].y = fmaf(f1, x[j].y, v[j].y * f0); v[j].z = fmaf(f1, x[j].z, v[j].z * f0); v[j].w = fmaf(f1, x[j].w, v[j].w * f0);
+                    }
+                }
+#pragma unroll
+                for (int j = 0; j < JOIN_HEADS; ++j) {
+                    if (!is[j]) continue;
+                    const float inv = sum[j] == 0.f ? 0.f : 1.0f / sum[j];
+                    store2<BF16>(a, m[j], head[j], d, v[j].x * inv, v[j].y * inv, wide & 1);
+                    store2<BF16>(a, m[j], head[j], d + 2, v[j].z * inv, v[j].w * inv, wide & 1);
+                }
+            }
         }
         return;
     }
@@ -928,7 +969,7 @@ cudaError_t launch_stream(const Kv8AttnArgs& a_in, int sm_count, cudaStream_t st
     }
     if (e != cudaSuccess) return e;
     const int columns = (std::min(group, PAIRS) + JOIN_PAIRS - 1) / JOIN_PAIRS;
-    const long rest = a.prefix_n ? std::min(((long)a.M * a.heads * kv8_pad(a.pool.vdim) / 4 + JOIN_THREADS * columns - 1) / (JOIN_THREADS * columns), 4096l) : 0;
+    const long rest = a.prefix_n ? std::min(((long)a.M * a.heads + JOIN_THREADS / 32 * JOIN_HEADS * columns - 1) / (JOIN_THREADS / 32 * JOIN_HEADS * columns), 4096l) : 0;
     return launch_behind(kv8_join_kernel<BF16, VS>, dim3((unsigned)(ctas - 1 + rest), (unsigned)columns), JOIN_THREADS, join_smem, st, a, ctas, tiles, wide);
 }
 

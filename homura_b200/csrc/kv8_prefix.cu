@@ -336,13 +336,12 @@ __global__ void __launch_bounds__(THREADS, 1) kv8_prefix_kernel(const Kv8AttnArg
         const bool values = warp >= SOFT_WARPS + CONV_WARPS;
         const int cw = (warp - SOFT_WARPS) % CONV_WARPS, units = values ? g.vp / 32 : g.dp / 32;
         auto wait = [&](uint64_t* bar, uint32_t parity) { return __all_sync(0xffffffffu, mb_wait(bar, parity, a.err_flag, &sh.abort_flag)); };
-        // a lane's place in 32 rows of 32 bytes, and where its rows go: a 16-byte piece of a row of 128 bytes has its number turned by the row's
-        const int r0 = lane >> 1, c = lane & 1, part = (values ? g.kpart : 0) + KV8_HALF * 4 + r0 * 32 + c * 16;
-        auto place = [&](int r) {
-            const int t = values ? r : ((r >> 1) & 3) * 8 + (r >> 3) * 2 + (r & 1);  // of keys: kv8_key_row(t) = r
-            return t * 128 + (((2 * c) ^ (t & 7)) << 4);
-        };
-        const int off0 = place(r0), off1 = place(r0 + 16);
+        // A lane's place in 32 rows of 32 bytes, and where it goes: a 16-byte piece of a row of 128 bytes has its number turned by the row's.  Lanes are dealt out so that eight of them read
+        // and write eight different pieces of 16 bytes of the banks: values by rows and pieces, keys (whose row r is token t, kv8_key_row(t) = r) by the bits that make the last of t.
+        const int h = (lane >> 1) & 3, y = lane >> 3;
+        const int r0 = values ? (lane & 7) + 8 * (lane >> 4) : 8 * h + 2 * ((h & 1) ^ (y & 1)) + (lane & 1), c = values ? (h >> 1) ^ (y & 1) : (h >> 1) ^ (y >> 1);
+        const int t0 = values ? r0 : ((r0 >> 1) & 3) * 8 + (r0 >> 3) * 2 + (r0 & 1), off = t0 * 128 + (((2 * c) ^ (t0 & 7)) << 4);
+        const int part = (values ? g.kpart : 0) + KV8_HALF * 4 + r0 * 32 + c * 16, second = values ? 512 : 128;  // the lane's other place, whose token (element) is 16 behind
         const int more = (values ? g.vst : g.kst) - 1;  // stages but one
         int next = 0;                                   // slot of the next page, and the parity of its wait
         uint32_t parity = 0;
@@ -403,24 +402,24 @@ __global__ void __launch_bounds__(THREADS, 1) kv8_prefix_kernel(const Kv8AttnArg
                 if (u.ph >= 4) return;
                 const unsigned char* from = raw[u.ph >> 1] + (u.ph & 1) * g.half + u.q * 1024;
                 u.w0 = *reinterpret_cast<const uint4*>(from);
-                u.w1 = *reinterpret_cast<const uint4*>(from + 512);
+                u.w1 = *reinterpret_cast<const uint4*>(from + second);
             };
             auto convert = [&](const Unit& u) {
                 unsigned char* to = tile + (values ? (uint32_t)(u.ph >> 1) * (g.v_tile / 2) + u.q * 4096 : (uint32_t)(u.q >> 1) * (BLOCK * 128) + u.ph * 4096);
-                const int flip = ((values ? u.ph : u.q) & 1) << 6;
+                const int at = off ^ (((values ? u.ph : u.q) & 1) << 6);
                 uint4 x, y;
                 codes_f16(u.w0.x, x.x, x.y);
                 codes_f16(u.w0.y, x.z, x.w);
                 codes_f16(u.w0.z, y.x, y.y);
                 codes_f16(u.w0.w, y.z, y.w);
-                *reinterpret_cast<uint4*>(to + (off0 ^ flip)) = x;
-                *reinterpret_cast<uint4*>(to + (off0 ^ flip ^ 16)) = y;
+                *reinterpret_cast<uint4*>(to + at) = x;
+                *reinterpret_cast<uint4*>(to + (at ^ 16)) = y;
                 codes_f16(u.w1.x, x.x, x.y);
                 codes_f16(u.w1.y, x.z, x.w);
                 codes_f16(u.w1.z, y.x, y.y);
                 codes_f16(u.w1.w, y.z, y.w);
-                *reinterpret_cast<uint4*>(to + (off1 ^ flip)) = x;
-                *reinterpret_cast<uint4*>(to + (off1 ^ flip ^ 16)) = y;
+                *reinterpret_cast<uint4*>(to + at + 2048) = x;
+                *reinterpret_cast<uint4*>(to + (at ^ 16) + 2048) = y;
             };
             Unit u{0, cw}, v;
             settle(u);
@@ -448,50 +447,54 @@ __global__ void __launch_bounds__(THREADS, 1) kv8_prefix_kernel(const Kv8AttnArg
         const uint32_t lanes = (uint32_t)(warp & 3) * 32 << 16, s_at = tmem + lanes + (uint32_t)stream * BLOCK, o_at = tmem + lanes + 2 * BLOCK + (uint32_t)stream * 128;
         float c = 0.f;  // what scores are multiplied with
         if (n > 0) {
-            // a warp takes pairs one by one, four elements a lane, so that a row is read by neighbours; several are on their way at once
-            constexpr int MINE = (PAIRED ? 2 : 1) * TILE / SOFT_WARPS, AHEAD = 4;
-            const int d = 4 * lane;
-            for (int r0 = warp * MINE; r0 < (warp + 1) * MINE; r0 += AHEAD) {
-                float x[AHEAD][4];
+            // eight elements a lane, 8 or 16 lanes to a pair, so that a row is read by neighbours; two groups of pairs are on their way at once
+            constexpr int MINE = (PAIRED ? 2 : 1) * TILE / SOFT_WARPS;
+            const int lanes = 8 * g.katoms, at_once = 32 / lanes, sub = lane / lanes, d = 8 * (lane - sub * lanes);
+            for (int r0 = warp * MINE + sub; r0 < (warp + 1) * MINE; r0 += 2 * at_once) {
+                float x[2][8];
 #pragma unroll
-                for (int k = 0; k < AHEAD; ++k) {
-                    const int p = tiles0 * TILE + r0 + k, m = p / group;
+                for (int k = 0; k < 2; ++k) {
+                    const int p = tiles0 * TILE + r0 + k * at_once, m = p / group, left = p < pairs ? a.pool.dim - d : 0;
                     const size_t at = (size_t)m * a.ldq + (size_t)(kvh * group + p - m * group) * a.pool.dim + d;
+                    if ((wide & 2) && left > 0) {
+                        float y[2][4];
+                        load_row<BF16, 4>(a.q, at, y[0]);
+                        load_row<BF16, 4>(a.q, at + 4, y[1]);
 #pragma unroll
-                    for (int e = 0; e < 4; ++e) x[k][e] = 0.f;
-                    if (p >= pairs || d >= a.pool.dim) continue;
-                    if (wide & 2) {
-                        load_row<BF16, 4>(a.q, at, x[k]);
+                        for (int e = 0; e < 8; ++e) x[k][e] = y[e >> 2][e & 3];
                     } else {
 #pragma unroll
-                        for (int e = 0; e < 4; ++e) {
+                        for (int e = 0; e < 8; ++e) {
                             float one[1] = {0.f};
-                            if (d + e < a.pool.dim) load_row<BF16, 1>(a.q, at + e, one);
+                            if (e < left) load_row<BF16, 1>(a.q, at + e, one);
                             x[k][e] = one[0];
                         }
                     }
                 }
 #pragma unroll
-                for (int k = 0; k < AHEAD; ++k) {
+                for (int k = 0; k < 2; ++k) {
+                    const int r = r0 + k * at_once;
                     uint32_t top = 0;
 #pragma unroll
-                    for (int e = 0; e < 4; ++e) top = max(top, __float_as_uint(x[k][e]) & 0x7FFFFFFFu);
-                    top = __reduce_max_sync(0xffffffffu, top);
+                    for (int e = 0; e < 8; ++e) top = max(top, __float_as_uint(x[k][e]) & 0x7FFFFFFFu);
+                    top = max(top, __shfl_xor_sync(0xffffffffu, top, 1));
+                    top = max(top, __shfl_xor_sync(0xffffffffu, top, 2));
+                    top = max(top, __shfl_xor_sync(0xffffffffu, top, 4));
+                    if (lanes == 16) top = max(top, __shfl_xor_sync(0xffffffffu, top, 8));
                     const bool finite = top < 0x7F800000u;
-                    const int ex = min(max((int)(top >> 23), 15), 254), r = r0 + k;
+                    const int ex = min(max((int)(top >> 23), 15), 254);
                     const float up = finite ? __uint_as_float((uint32_t)(254 + 14 - ex) << 23) * (a.scale < 0.f ? -1.f : 1.f) : 0.f;
-                    if (lane < (PAIRED ? 1 : 2)) sh.half[PAIRED ? r >> 7 : lane][1][0][r & (TILE - 1)] = finite ? fabsf(a.scale) * LOG2E * exp2f((float)(ex - 127 - 14)) : __uint_as_float(0x7FC00000u);
-                    if (d >= g.katoms * 64) continue;
-                    uint32_t hi[2], lo[2];
+                    if (d < (PAIRED ? 8 : 16)) sh.half[PAIRED ? r >> 7 : d >> 3][1][0][r & (TILE - 1)] = finite ? fabsf(a.scale) * LOG2E * exp2f((float)(ex - 127 - 14)) : __uint_as_float(0x7FC00000u);
+                    uint32_t hi[4], lo[4];
 #pragma unroll
-                    for (int e = 0; e < 2; ++e) {
+                    for (int e = 0; e < 4; ++e) {
                         const float u = x[k][2 * e] * up, v = x[k][2 * e + 1] * up;
                         hi[e] = f16x2(u, v);
-                        lo[e] = f16x2(u - f16_lo(hi[e]), v - f16_hi(hi[e]));
+                        if (TERMS == 2) lo[e] = f16x2(u - f16_lo(hi[e]), v - f16_hi(hi[e]));
                     }
-                    unsigned char* to = base + g.q_at + (uint32_t)(r >> 7) * g.q_tile + (d >> 6) * (TILE * 128) + (r & (TILE - 1)) * 128 + ((((d >> 3) & 7) ^ (r & 7)) << 4) + (d & 4) * 2;
-                    *reinterpret_cast<uint2*>(to) = make_uint2(hi[0], hi[1]);
-                    if (TERMS == 2) *reinterpret_cast<uint2*>(to + g.q_tile / 2) = make_uint2(lo[0], lo[1]);
+                    unsigned char* to = base + g.q_at + (uint32_t)(r >> 7) * g.q_tile + (d >> 6) * (TILE * 128) + (r & (TILE - 1)) * 128 + ((((d >> 3) & 7) ^ (r & 7)) << 4);
+                    *reinterpret_cast<uint4*>(to) = make_uint4(hi[0], hi[1], hi[2], hi[3]);
+                    if (TERMS == 2) *reinterpret_cast<uint4*>(to + g.q_tile / 2) = make_uint4(lo[0], lo[1], lo[2], lo[3]);
                 }
             }
             fence_async_smem();

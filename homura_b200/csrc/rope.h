@@ -19,6 +19,6 @@ struct RopeArgs {
     const double* turns;   // [rot / 2] turns per position
     float magnitude;       // the rotated elements are multiplied with this
 };
-cudaError_t launch_rope(const RopeArgs& a, cudaStream_t st);
+cudaError_t launch_rope(const RopeArgs& a, int sm_count, cudaStream_t st);
 
 }  // namespace hm
