@@ -447,14 +447,15 @@ __global__ void __launch_bounds__(THREADS, 1) kv8_prefix_kernel(const Kv8AttnArg
         const uint32_t lanes = (uint32_t)(warp & 3) * 32 << 16, s_at = tmem + lanes + (uint32_t)stream * BLOCK, o_at = tmem + lanes + 2 * BLOCK + (uint32_t)stream * 128;
         float c = 0.f;  // what scores are multiplied with
         if (n > 0) {
-            // eight elements a lane, 8 or 16 lanes to a pair, so that a row is read by neighbours; two groups of pairs are on their way at once
+            // eight elements a lane, 8 or 16 lanes to a pair, so that a row is read by neighbours; the loads of several groups of pairs are on their way at once
             constexpr int MINE = (PAIRED ? 2 : 1) * TILE / SOFT_WARPS;
+            constexpr int AHEAD = BF16 ? 4 : 2;
             const int lanes = 8 * g.katoms, at_once = 32 / lanes, sub = lane / lanes, d = 8 * (lane - sub * lanes);
-            for (int r0 = warp * MINE + sub; r0 < (warp + 1) * MINE; r0 += 2 * at_once) {
-                float x[2][8];
+            for (int r0 = warp * MINE + sub; r0 < (warp + 1) * MINE; r0 += AHEAD * at_once) {
+                float x[AHEAD][8];
 #pragma unroll
-                for (int k = 0; k < 2; ++k) {
-                    const int p = tiles0 * TILE + r0 + k * at_once, m = p / group, left = p < pairs ? a.pool.dim - d : 0;
+                for (int k = 0; k < AHEAD; ++k) {
+                    const int r = r0 + k * at_once, p = tiles0 * TILE + r, m = p / group, left = r < (warp + 1) * MINE && p < pairs ? a.pool.dim - d : 0;
                     const size_t at = (size_t)m * a.ldq + (size_t)(kvh * group + p - m * group) * a.pool.dim + d;
                     if ((wide & 2) && left > 0) {
                         float y[2][4];
@@ -472,8 +473,9 @@ __global__ void __launch_bounds__(THREADS, 1) kv8_prefix_kernel(const Kv8AttnArg
                     }
                 }
 #pragma unroll
-                for (int k = 0; k < 2; ++k) {
+                for (int k = 0; k < AHEAD; ++k) {
                     const int r = r0 + k * at_once;
+                    if (r - sub >= (warp + 1) * MINE) break;  // eight pairs may be fewer than those at once
                     uint32_t top = 0;
 #pragma unroll
                     for (int e = 0; e < 8; ++e) top = max(top, __float_as_uint(x[k][e]) & 0x7FFFFFFFu);
@@ -646,27 +648,34 @@ __global__ void __launch_bounds__(THREADS, 1) kv8_prefix_kernel(const Kv8AttnArg
     if (warp == MMA_WARP) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, 512;" ::"r"(tmem) : "memory");
     // ---- the splits of a cluster (and the two streams of a tile) joined: a warp to a pair, the CTAs take turns ----
     const int rank = cluster > 1 ? (int)cluster_ctarank() : 0, rows = PAIRED ? 2 * TILE : TILE, sources = PAIRED ? cluster : 2 * cluster;
-    for (int r = rank * (THREADS / 32) + warp; r < rows; r += cluster * (THREADS / 32)) {
-        const int p = tiles0 * TILE + r;
-        if (p >= pairs) break;
-        // source s: CTA s, or CTA s / 2 and stream s % 2
-        auto source = [&](int s) { return dsmem_addr(reinterpret_cast<const float*>(base) + (size_t)(PAIRED ? r : r + (s & 1) * TILE) * ldo, (uint32_t)(PAIRED ? s : s >> 1)); };
-        float m = -INFINITY, l = 0.f;
-        if (lane < sources) {
-            const uint32_t at = source(lane);
-            m = ld_dsmem_f32(at);
-            l = ld_dsmem_f32(at + 4);
-        }
-        const float top = warp_max(m), ref = top == -INFINITY ? 0.f : top, f = exp2f(m - ref);
-        l = warp_sum(f * l);
+    constexpr int AT_ONCE = 4;  // sources whose loads are on their way together
+    const int step = cluster * (THREADS / 32), last = min(rows, pairs - tiles0 * TILE) - 1, d = min(4 * lane, g.vp - 4);
+    for (int r = rank * (THREADS / 32) + warp; r <= last; r += step) {
+        float top = -INFINITY, l = 0.f;
         float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
-        for (int s = 0; s < sources; ++s) {
-            const float fs = __shfl_sync(0xffffffffu, f, s);
-            if (4 * lane >= g.vp) continue;
-            const float4 x = ld_dsmem_f32x4(source(s) + 16 + 16 * lane);
-            v.x = fmaf(fs, x.x, v.x); v.y = fmaf(fs, x.y, v.y); v.z = fmaf(fs, x.z, v.z); v.w = fmaf(fs, x.w, v.w);
+        for (int s0 = 0; s0 < sources; s0 += AT_ONCE) {
+            float m[AT_ONCE], lm[AT_ONCE];
+            float4 x[AT_ONCE];
+#pragma unroll
+            for (int k = 0; k < AT_ONCE; ++k) {  // source s: CTA s, or CTA s / 2 and stream s % 2
+                const int s = s0 + k;
+                m[k] = -INFINITY;
+                if (s >= sources) continue;
+                const uint32_t at = dsmem_addr(reinterpret_cast<const float*>(base) + (size_t)(PAIRED ? r : r + (s & 1) * TILE) * ldo, (uint32_t)(PAIRED ? s : s >> 1));
+                m[k] = ld_dsmem_f32(at);
+                lm[k] = ld_dsmem_f32(at + 4);
+                x[k] = ld_dsmem_f32x4(at + 16 + 4 * d);
+            }
+#pragma unroll
+            for (int k = 0; k < AT_ONCE; ++k) {
+                if (m[k] == -INFINITY) continue;  // nothing seen
+                const float now = fmaxf(top, m[k]), f0 = exp2_ftz(top - now), f1 = exp2_ftz(m[k] - now);
+                top = now;
+                l = fmaf(f1, lm[k], l * f0);
+                v.x = fmaf(f1, x[k].x, v.x * f0); v.y = fmaf(f1, x[k].y, v.y * f0); v.z = fmaf(f1, x[k].z, v.z * f0); v.w = fmaf(f1, x[k].w, v.w * f0);
+            }
         }
-        float* to = parts + (((size_t)(split / cluster) * a.pool.kv_heads + kvh) * pairs + p) * (g.vp + 4);
+        float* to = parts + (((size_t)(split / cluster) * a.pool.kv_heads + kvh) * pairs + tiles0 * TILE + r) * (g.vp + 4);
         if (lane == 0) *reinterpret_cast<float2*>(to) = make_float2(top, l);
         if (4 * lane < g.vp) *reinterpret_cast<float4*>(to + 4 + 4 * lane) = v;
     }
