@@ -212,7 +212,9 @@ __host__ __device__ inline StreamShape stream_shape(int dim, int vdim, int passe
     s.q_at = (size_t)warps * depth * (s.kpart + s.vpart);
     s.queries = s.dp / 32 * passes * 32;
     s.merge_at = s.q_at + 2 * sizeof(uint4) * s.queries;
-    s.bytes = s.merge_at + sizeof(float) * MERGE_ROWS * s.ldo;
+    // a warp's own items have their queries in the same place
+    const size_t merge = 2 * sizeof(uint4) * s.queries + sizeof(float) * MERGE_ROWS * s.ldo, own = sizeof(uint4) * s.queries * warps;
+    s.bytes = s.q_at + (merge > own ? merge : own);
     return s;
 }
 
@@ -459,11 +461,11 @@ __global__ void __launch_bounds__(WARPS * 32, 1) kv8_stream_kernel(const Kv8Attn
     };
 
     const int gid = lane >> 2, tig = lane & 3, slabs = sh.dp / 32, vslabs = sh.vp / 32;
-    int i = 0, slot = 0, rings = 1, len = 0;  // this warp's next piece, counted over the CTA (or its own item), and its slot; slots in use; tokens of the segment's row
+    int i = 0, slot = 0, len = 0;  // this warp's next piece, counted over the CTA (or its own item), and its slot; tokens of the segment's row
     bool good = true;                         // no wait has run out
     bool alone = line.solo;                   // with items of this warp's own; then with the line
     int own = warp * ctas + (int)blockIdx.x;  // those are every WARPS * ctas-th of all
-    uint4* own_queries = reinterpret_cast<uint4*>(kbuf + (size_t)(depth - 1) * sh.kpart);  // where the last slot's keys will stand
+    uint4* own_queries = queries + warp * sh.queries;  // where the line's queries and sums will stand
     float next_q[8];
     int begin = 0, turn = 0;
     bool joined = false, waited = false;  // at the line; for the prefix
@@ -487,8 +489,7 @@ __global__ void __launch_bounds__(WARPS * 32, 1) kv8_stream_kernel(const Kv8Attn
             sg = Segment{m, own - m * items, 0, n, n};
             own += WARPS * ctas;
             __syncwarp();
-            rings = depth - 1;
-            start(sg, 0, n, 1, rings);
+            start(sg, 0, n, 1, depth);
             len = row_len(a, m);
             i = begin = slot = 0;
             // lane (gid, tig): elements 8 tig .. 8 tig + 7 of every slab of pair gid
@@ -536,15 +537,13 @@ __global__ void __launch_bounds__(WARPS * 32, 1) kv8_stream_kernel(const Kv8Attn
             if (!joined) {
                 joined = true;
                 if (count == 0) break;
-                asm volatile("fence.proxy.async.shared::cta;" ::: "memory");  // queries stood where pieces are copied to
-                __syncwarp();
                 sg = line_begin;
-                rings = depth;
                 if (warp < PAIRS) fetch_query(sg, warp, next_q);  // in front of the copies, behind which they would wait
                 start(sg, warp, count, WARPS, good ? depth : 0);  // nothing into slots whose copies were given up
                 len = row_len(a, sg.m);
                 i = warp;
                 begin = slot = 0;
+                if (line.solo) __syncthreads();  // no warp has items of its own left
                 if (warp < PAIRS) {
                     const float f = put_query(next_q, warp, queries);
                     if (lane == 0) s_c[0][warp] = f;
@@ -677,7 +676,7 @@ __global__ void __launch_bounds__(WARPS * 32, 1) kv8_stream_kernel(const Kv8Attn
             }
             if (next) copy(values, next + sh.kpart, sh.vpart, &vfull[slot]);
             there = (there & ~(1u << slot)) | (next ? 1u << slot : 0u);
-            slot = slot + 1 == rings ? 0 : slot + 1;
+            slot = slot + 1 == depth ? 0 : slot + 1;
         }
 
         l += __shfl_xor_sync(0xffffffffu, l, 1);
@@ -776,7 +775,7 @@ __global__ void __launch_bounds__(WARPS * 32, 1) kv8_stream_kernel(const Kv8Attn
     if (!waited) pdl_wait();  // kv8_join_kernel waits for this launch alone
     // every copy has been waited for, unless a wait ran out: then what is still on its way has to land before this CTA's shared memory is another's
     if (!good)
-        for (int s = 0; s < rings; ++s) {
+        for (int s = 0; s < depth; ++s) {
             if (!((there >> s) & 1u)) continue;
             mb_land(&kfull[s], (phase >> s) & 1u);
             mb_land(&vfull[s], (phase >> s) & 1u);
@@ -955,8 +954,8 @@ cudaError_t launch_stream(const Kv8AttnArgs& a_in, int sm_count, cudaStream_t st
     auto bytes = [&](int depth) { return stream_shape(a.pool.dim, a.pool.vdim, BF16 ? 1 : 2, WARPS, depth).bytes; };
     int depth = MAX_DEPTH;
     while (depth > 1 && bytes(depth) > ROOM) --depth;
-    // a warp's own items need a second slot for their queries.  Where there are more items than CTAs, a CTA would take them one by one
-    a.solo = depth >= 2 && (long)a.M * a.pool.kv_heads * tiles >= 2 * sm_count ? 12 : 0;
+    // where there are more items than CTAs, a CTA would take them one by one
+    a.solo = (long)a.M * a.pool.kv_heads * tiles >= 2 * sm_count ? 12 : 0;
     const size_t smem = bytes(depth), join_smem = sizeof(float2) * JOIN_PAIRS * ctas + 16 + sizeof(float) * JOIN_THREADS * JOIN_PAIRS * VS;
     cudaError_t e = ensure_dyn_smem(kv8_stream_kernel<BF16, VS, WARPS>, smem);
     if (e == cudaSuccess) e = ensure_dyn_smem(kv8_join_kernel<BF16, VS>, join_smem);
