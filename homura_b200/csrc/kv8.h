@@ -64,6 +64,8 @@ struct Kv8AttnArgs {
     int* err_flag;
     // filled in by the launcher
     int solo;                // items of at most so many pieces are a warp's own
+    int whole;               // a CTA takes an item as a whole, and there are no more items than CTAs
+    int direct;              // kv8_prefix.cu writes the rows that have nothing but the prefix
     int own_from;            // the rows' own pieces (halves of pages) begin here: what stands in front is in `prefix`
     const float* prefix;     // [prefix_n parts][kv_heads][M * heads / kv_heads][padded vdim + 4]: reference and sum of a pair, then from the fifth on its elements
     int prefix_n;

@@ -28,9 +28,9 @@
 #include <algorithm>
 #include <type_traits>
 
+#include "kv8_rows.cuh"
 #include "launch_attrs.h"
 #include "mbarrier.cuh"
-#include "rows.cuh"
 
 namespace hm {
 namespace {
@@ -38,6 +38,8 @@ namespace {
 constexpr int PAIRS = 8;           // of an item
 constexpr int LEAST_PIECES = 12;   // of a CTA, one for each of its warps: fewer would only leave more to be joined
 constexpr int BEGIN = 20;           // pieces that take a CTA as long as the beginning and end of an item
+constexpr int WHOLE = 36;           // pieces that a CTA takes in less time than a join takes
+constexpr int SOLO = 12;            // pieces that a warp takes alone where there are many items
 constexpr int MAX_DEPTH = 4;
 constexpr int MERGE_ROWS = 32;      // pairs' results of several warps that stand in shared memory when those of all are added up
 constexpr size_t ROOM = 222 * 1024;  // shared memory of a CTA, beside the static
@@ -50,15 +52,9 @@ struct Line {
     bool solo;               // there are items of a few pieces
 };
 
-__device__ __forceinline__ int row_len(const Kv8AttnArgs& a, int m) {
-    const int seq = __ldg(a.row_seq + m);
-    return (unsigned)seq < (unsigned)a.pool.n_seq ? min(__ldg(a.row_pos + m), a.pool.max_pages * KV8_PAGE - 1) + 1 : 0;
-}
-__device__ __forceinline__ int row_pieces(const Kv8AttnArgs& a, int m) { return max(0, (row_len(a, m) + KV8_HALF - 1) / KV8_HALF - a.own_from); }
-
 // Pieces of a row's items that stand in the line.
 __device__ __forceinline__ int line_pieces(const Kv8AttnArgs& a, int m) {
-    const int n = row_pieces(a, m);
+    const int n = kv8_row_pieces(a, m);
     return n > a.solo ? n : 0;
 }
 
@@ -78,7 +74,7 @@ __device__ __forceinline__ Line make_line(const Kv8AttnArgs& a, int items, int c
     int most = 0;
     bool solo = false;
     for (int m = m0; m < m1; ++m) {
-        const int n = row_pieces(a, m);
+        const int n = kv8_row_pieces(a, m);
         if (n > a.solo) sum += (1ll << 32) + n + BEGIN;
         else solo |= n > 0;
         most = max(most, n);
@@ -251,21 +247,6 @@ __device__ __forceinline__ void put_digits(const float (&x)[8], float up, uint4*
 // What is left of an item in `work`: maximum and sum of every pair, then its elements (relative to the maximum, not divided).
 __host__ __device__ inline size_t part_floats(int vp) { return PAIRS * (size_t)(vp + 4); }
 
-// Two results of a row: elements d and d + 1 of a head.
-template <bool BF16>
-__device__ __forceinline__ void store2(const Kv8AttnArgs& a, int m, int head, int d, float x, float y, bool wide) {
-    const size_t at = (size_t)m * a.ldo + (size_t)head * a.pool.vdim + d;
-    if (wide) {  // an even number of elements, pairs aligned
-        if (d >= a.pool.vdim) return;
-        if (BF16) *reinterpret_cast<uint32_t*>(static_cast<uint16_t*>(a.out) + at) = bf16x2_rne(x, y);
-        else *reinterpret_cast<float2*>(static_cast<float*>(a.out) + at) = make_float2(x, y);
-        return;
-    }
-    const float v[2][1] = {{x}, {y}};
-    if (d < a.pool.vdim) store_row<BF16, 1>(a.out, at, v[0]);
-    if (d + 1 < a.pool.vdim) store_row<BF16, 1>(a.out, at + 1, v[1]);
-}
-
 // Parts in `work`: of CTA c its first item (0) and its last (1).
 __device__ __forceinline__ float* cta_part(const Kv8AttnArgs& a, int vp, int cta, int which) { return static_cast<float*>(a.work) + (size_t)(2 * cta + which) * part_floats(vp); }
 
@@ -351,11 +332,17 @@ __global__ void __launch_bounds__(WARPS * 32, 1) kv8_stream_kernel(const Kv8Attn
         s_abort = 0;
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
-    const Line line = make_line<THREADS>(a, items, ctas, first);
+    Line line{};
+    if (a.whole) __syncthreads();
+    else line = make_line<THREADS>(a, items, ctas, first);
     const long long u0 = min(line.total, blockIdx.x * line.chunk), u1 = min(line.total, u0 + line.chunk);
     Segment line_begin{};
     int count = 0;  // pieces of this CTA
-    if (u0 < u1) {
+    if (a.whole && (int)blockIdx.x < a.M * items) {
+        line_begin.m = (int)blockIdx.x / items;
+        line_begin.item = (int)blockIdx.x - line_begin.m * items;
+        line_begin.of = line_begin.n = count = kv8_row_pieces(a, line_begin.m);
+    } else if (u0 < u1) {
         long long begin, before, behind = (long long)items * (units_of(first[THREADS]) - rows_of(first[THREADS]) * BEGIN);
         if (u1 < line.total) unit_at<THREADS>(a, first, items, u1, begin, behind);
         line_begin = unit_at<THREADS>(a, first, items, u0, begin, before);
@@ -366,7 +353,7 @@ __global__ void __launch_bounds__(WARPS * 32, 1) kv8_stream_kernel(const Kv8Attn
 
     // ---- rows without a context (where there is a prefix, kv8_join_kernel writes them) ----
     for (int m = blockIdx.x; m < a.M && a.prefix_n == 0; m += ctas) {
-        if (row_pieces(a, m) > 0 || (unsigned)__ldg(a.row_seq + m) >= (unsigned)a.pool.n_seq) continue;
+        if (kv8_row_pieces(a, m) > 0 || (unsigned)__ldg(a.row_seq + m) >= (unsigned)a.pool.n_seq) continue;
         const float zero[1] = {0.f};
         for (int i = tid; i < a.heads * a.pool.vdim; i += THREADS) store_row<BF16, 1>(a.out, (size_t)m * a.ldo + i, zero);
     }
@@ -479,7 +466,7 @@ __global__ void __launch_bounds__(WARPS * 32, 1) kv8_stream_kernel(const Kv8Attn
             int m = 0, n = 0;
             for (; own < a.M * items; own += WARPS * ctas) {
                 m = own / items;
-                n = row_pieces(a, m);
+                n = kv8_row_pieces(a, m);
                 if (n > 0 && n <= a.solo) break;
             }
             if (own >= a.M * items || !good) {
@@ -490,7 +477,7 @@ __global__ void __launch_bounds__(WARPS * 32, 1) kv8_stream_kernel(const Kv8Attn
             own += WARPS * ctas;
             __syncwarp();
             start(sg, 0, n, 1, depth);
-            len = row_len(a, m);
+            len = kv8_row_len(a, m);
             i = begin = slot = 0;
             // lane (gid, tig): elements 8 tig .. 8 tig + 7 of every slab of pair gid
             const int kvh = sg.item / tiles, tile = sg.item - kvh * tiles;
@@ -540,7 +527,7 @@ __global__ void __launch_bounds__(WARPS * 32, 1) kv8_stream_kernel(const Kv8Attn
                 sg = line_begin;
                 if (warp < PAIRS) fetch_query(sg, warp, next_q);  // in front of the copies, behind which they would wait
                 start(sg, warp, count, WARPS, good ? depth : 0);  // nothing into slots whose copies were given up
-                len = row_len(a, sg.m);
+                len = kv8_row_len(a, sg.m);
                 i = warp;
                 begin = slot = 0;
                 if (line.solo) __syncthreads();  // no warp has items of its own left
@@ -557,7 +544,7 @@ __global__ void __launch_bounds__(WARPS * 32, 1) kv8_stream_kernel(const Kv8Attn
             behind = sg;
             if (!last) {  // the next segment's queries are fetched now
                 next_segment(a, items, behind, count - begin - sg.n);
-                len_behind = row_len(a, behind.m);
+                len_behind = kv8_row_len(a, behind.m);
                 if (warp < PAIRS) fetch_query(behind, warp, next_q);
             }
         }
@@ -688,7 +675,7 @@ __global__ void __launch_bounds__(WARPS * 32, 1) kv8_stream_kernel(const Kv8Attn
             const float inv = l == 0.f ? 0.f : 1.0f / l;
 #pragma unroll
             for (int s = 0; s < VS * 4; ++s)
-                if (s < vslabs * 4 && gid < pairs) store2<BF16>(a, sg.m, head0 + gid, 8 * s + 2 * tig, o[s][0] * inv, o[s][1] * inv, wide & 1);
+                if (s < vslabs * 4 && gid < pairs) kv8_store2<BF16>(a, sg.m, head0 + gid, 8 * s + 2 * tig, o[s][0] * inv, o[s][1] * inv, wide & 1);
             continue;
         }
         // ---- the warps' results added up: `slots` warps at a time to those of the first `slots` warps, then these ----
@@ -754,8 +741,8 @@ __global__ void __launch_bounds__(WARPS * 32, 1) kv8_stream_kernel(const Kv8Attn
                     add_prefix(a, sh.vp, kvh, sg.m * group + tile * PAIRS + pr, d, top, sum, v);
                 }
                 const float inv = sum == 0.f ? 0.f : 1.0f / sum;
-                store2<BF16>(a, sg.m, head0 + pr, d, v[0] * inv, v[1] * inv, wide & 1);
-                store2<BF16>(a, sg.m, head0 + pr, d + 2, v[2] * inv, v[3] * inv, wide & 1);
+                kv8_store2<BF16>(a, sg.m, head0 + pr, d, v[0] * inv, v[1] * inv, wide & 1);
+                kv8_store2<BF16>(a, sg.m, head0 + pr, d + 2, v[2] * inv, v[3] * inv, wide & 1);
             } else {
                 float* at = part + (size_t)pr * (sh.vp + 4);
                 *reinterpret_cast<float4*>(at + 4 + d) = make_float4(v[0], v[1], v[2], v[3]);
@@ -786,7 +773,7 @@ __global__ void __launch_bounds__(WARPS * 32, 1) kv8_stream_kernel(const Kv8Attn
 // hundred parts and more: the warps share them, every lane with its elements of several parts in flight at once.  The CTAs behind those have rows that have nothing but the prefix.
 constexpr int JOIN_THREADS = 256, JOIN_PAIRS = 2, JOIN_HEADS = 4;
 template <bool BF16, int VS>
-__global__ void __launch_bounds__(JOIN_THREADS) kv8_join_kernel(const Kv8AttnArgs a, int ctas, int tiles, int wide) {
+__global__ void __launch_bounds__(JOIN_THREADS) kv8_join_kernel(const Kv8AttnArgs a, int ctas, int tiles, int wide) {  // ctas: one more than cuts
     constexpr int THREADS = JOIN_THREADS, JW = THREADS / 32, NI = JOIN_PAIRS * VS * 8 / 32, AHEAD = 4;  // warps; groups of four elements a lane; parts in flight
     extern __shared__ __align__(128) unsigned char dyn[];                                               // factors [parts][JOIN_PAIRS], then the warps' sums
     __shared__ float s_top[JOIN_PAIRS], s_sum[JOIN_PAIRS];
@@ -808,7 +795,7 @@ __global__ void __launch_bounds__(JOIN_THREADS) kv8_join_kernel(const Kv8AttnArg
                 head[j] = r - m[j] * a.heads;
                 const int kvh = head[j] / group;
                 at[j] = a.prefix + ((size_t)kvh * all_pairs + (size_t)m[j] * group + (head[j] - kvh * group)) * (vp + 4);
-                is[j] = k + j < all && row_pieces(a, m[j]) == 0 && (unsigned)__ldg(a.row_seq + m[j]) < (unsigned)a.pool.n_seq;
+                is[j] = k + j < all && kv8_row_pieces(a, m[j]) == 0 && (unsigned)__ldg(a.row_seq + m[j]) < (unsigned)a.pool.n_seq;
             }
             for (int d = 4 * lane; d < vp; d += 128) {
                 float top[JOIN_HEADS], sum[JOIN_HEADS];
@@ -840,8 +827,8 @@ __global__ void __launch_bounds__(JOIN_THREADS) kv8_join_kernel(const Kv8AttnArg
                 for (int j = 0; j < JOIN_HEADS; ++j) {
                     if (!is[j]) continue;
                     const float inv = sum[j] == 0.f ? 0.f : 1.0f / sum[j];
-                    store2<BF16>(a, m[j], head[j], d, v[j].x * inv, v[j].y * inv, wide & 1);
-                    store2<BF16>(a, m[j], head[j], d + 2, v[j].z * inv, v[j].w * inv, wide & 1);
+                    kv8_store2<BF16>(a, m[j], head[j], d, v[j].x * inv, v[j].y * inv, wide & 1);
+                    kv8_store2<BF16>(a, m[j], head[j], d + 2, v[j].z * inv, v[j].w * inv, wide & 1);
                 }
             }
         }
@@ -925,8 +912,8 @@ __global__ void __launch_bounds__(JOIN_THREADS) kv8_join_kernel(const Kv8AttnArg
         float top = s_top[pr], sum = s_sum[pr];
         if (a.prefix_n) add_prefix(a, vp, kvh, sg.m * group + tile * PAIRS + pr0 + pr, d, top, sum, v);
         const float inv = sum == 0.f ? 0.f : 1.0f / sum;
-        store2<BF16>(a, sg.m, head0 + pr, d, v[0] * inv, v[1] * inv, wide & 1);
-        store2<BF16>(a, sg.m, head0 + pr, d + 2, v[2] * inv, v[3] * inv, wide & 1);
+        kv8_store2<BF16>(a, sg.m, head0 + pr, d, v[0] * inv, v[1] * inv, wide & 1);
+        kv8_store2<BF16>(a, sg.m, head0 + pr, d + 2, v[2] * inv, v[3] * inv, wide & 1);
     }
 }
 
@@ -948,28 +935,31 @@ cudaError_t launch_behind(void (*kern)(KArgs...), dim3 grid, int threads, size_t
 template <bool BF16, int VS, int WARPS>
 cudaError_t launch_stream(const Kv8AttnArgs& a_in, int sm_count, cudaStream_t st) {
     Kv8AttnArgs a = a_in;
-    const int group = a.heads / a.pool.kv_heads, tiles = (group + PAIRS - 1) / PAIRS, size = BF16 ? 2 : 4, ctas = sm_count;
-    // bit 0: results in pairs, bit 1: queries in groups of four
-    const int wide = (a.pool.vdim % 2 == 0 && (((uintptr_t)a.out | a.ldo * size) & (2 * size - 1)) == 0 ? 1 : 0) | (a.pool.dim % 8 == 0 && (((uintptr_t)a.q | a.ldq * size) & (4 * size - 1)) == 0 ? 2 : 0);
+    const int group = a.heads / a.pool.kv_heads, tiles = (group + PAIRS - 1) / PAIRS, ctas = sm_count;
+    const int wide = kv8_wide(a);
     auto bytes = [&](int depth) { return stream_shape(a.pool.dim, a.pool.vdim, BF16 ? 1 : 2, WARPS, depth).bytes; };
     int depth = MAX_DEPTH;
     while (depth > 1 && bytes(depth) > ROOM) --depth;
     // where there are more items than CTAs, a CTA would take them one by one
-    a.solo = (long)a.M * a.pool.kv_heads * tiles >= 2 * sm_count ? 12 : 0;
+    const long all = (long)a.M * a.pool.kv_heads * tiles, most = std::max(0l, (long)a.pool.max_pages * (KV8_PAGE / KV8_HALF) - a.own_from);  // items; pieces of one
+    a.solo = all >= 2 * sm_count ? SOLO : 0;
+    a.whole = all <= ctas && most <= WHOLE;
+    const bool own = most > 0 || a.prefix_n == 0, cut = own && !a.whole && most > a.solo, rest = a.prefix_n > 0 && !a.direct;
     const size_t smem = bytes(depth), join_smem = sizeof(float2) * JOIN_PAIRS * ctas + 16 + sizeof(float) * JOIN_THREADS * JOIN_PAIRS * VS;
     cudaError_t e = ensure_dyn_smem(kv8_stream_kernel<BF16, VS, WARPS>, smem);
     if (e == cudaSuccess) e = ensure_dyn_smem(kv8_join_kernel<BF16, VS>, join_smem);
     if (e != cudaSuccess) return e;
-    if (a.prefix_n) {
+    if (own && a.prefix_n) {
         e = launch_behind(kv8_stream_kernel<BF16, VS, WARPS>, dim3((unsigned)ctas), WARPS * 32, smem, st, a, depth, tiles, wide);
-    } else {
+    } else if (own) {
         kv8_stream_kernel<BF16, VS, WARPS><<<(unsigned)ctas, WARPS * 32, smem, st>>>(a, depth, tiles, wide);
         e = cudaGetLastError();
     }
-    if (e != cudaSuccess) return e;
-    const int columns = (std::min(group, PAIRS) + JOIN_PAIRS - 1) / JOIN_PAIRS;
-    const long rest = a.prefix_n ? std::min(((long)a.M * a.heads + JOIN_THREADS / 32 * JOIN_HEADS * columns - 1) / (JOIN_THREADS / 32 * JOIN_HEADS * columns), 4096l) : 0;
-    return launch_behind(kv8_join_kernel<BF16, VS>, dim3((unsigned)(ctas - 1 + rest), (unsigned)columns), JOIN_THREADS, join_smem, st, a, ctas, tiles, wide);
+    if (e != cudaSuccess || !(cut || rest)) return e;
+    // a column of CTAs for every cut, then those of the rows that have nothing but the prefix
+    const int columns = (std::min(group, PAIRS) + JOIN_PAIRS - 1) / JOIN_PAIRS, cuts = cut ? ctas - 1 : 0, at_once = JOIN_THREADS / 32 * JOIN_HEADS * columns;
+    const long more = rest ? std::min(((long)a.M * a.heads + at_once - 1) / at_once, 4096l) : 0;
+    return launch_behind(kv8_join_kernel<BF16, VS>, dim3((unsigned)(cuts + more), (unsigned)columns), JOIN_THREADS, join_smem, st, a, cuts + 1, tiles, wide);
 }
 
 // 12 warps (168 registers a thread) where their pieces fit, else eight.
@@ -1004,12 +994,13 @@ cudaError_t launch_kv8_attn(const Kv8AttnArgs& a_in, int sm_count, cudaStream_t 
     const Kv8Prefix p = kv8_prefix_plan(a.pool.kv_heads, a.pool.dim, a.pool.vdim, a.bf16, a.M, a.heads, a.n_shared, sm_count);
     a.own_from = 0;
     a.prefix_n = p.parts;
+    a.direct = p.parts == 1;
     if (p.parts) {
         float* parts = static_cast<float*>(a.work) + line_floats(a.pool.vdim, sm_count);
+        a.own_from = a.n_shared * (KV8_PAGE / KV8_HALF);
         const cudaError_t e = launch_kv8_prefix(a, p, parts, st);
         if (e != cudaSuccess) return e;
         a.prefix = parts;
-        a.own_from = a.n_shared * (KV8_PAGE / KV8_HALF);
     }
     return a.bf16 ? launch_typed<true>(a, sm_count, st) : launch_typed<false>(a, sm_count, st);
 }

@@ -20,9 +20,9 @@
 #include <utility>
 
 #include "kv8.h"
+#include "kv8_rows.cuh"
 #include "launch_attrs.h"
 #include "mbarrier.cuh"
-#include "rows.cuh"
 
 namespace hm {
 namespace {
@@ -233,8 +233,7 @@ __global__ void __launch_bounds__(THREADS, 1) kv8_prefix_kernel(const Kv8AttnArg
     const int row = mine ? pair / group : 0;
     int len = 0;
     if (mine) {
-        const int seq = __ldg(a.row_seq + row);
-        if ((unsigned)seq < (unsigned)a.pool.n_seq) len = max(0, min(__ldg(a.row_pos + row), a.n_shared * KV8_PAGE - 1) + 1);
+        len = max(0, min(kv8_row_len(a, row), a.n_shared * KV8_PAGE));
     }
     {
         const int most = __reduce_max_sync(0xffffffffu, len);
@@ -675,7 +674,16 @@ __global__ void __launch_bounds__(THREADS, 1) kv8_prefix_kernel(const Kv8AttnArg
                 v.x = fmaf(f1, x[k].x, v.x * f0); v.y = fmaf(f1, x[k].y, v.y * f0); v.z = fmaf(f1, x[k].z, v.z * f0); v.w = fmaf(f1, x[k].w, v.w * f0);
             }
         }
-        float* to = parts + (((size_t)(split / cluster) * a.pool.kv_heads + kvh) * pairs + tiles0 * TILE + r) * (g.vp + 4);
+        const int p = tiles0 * TILE + r, m = p / group;
+        if (a.direct && kv8_row_pieces(a, m) == 0) {  // the row has nothing else
+            if ((unsigned)__ldg(a.row_seq + m) >= (unsigned)a.pool.n_seq || 4 * lane >= g.vp) continue;
+            const int head = kvh * group + p - m * group;
+            const float inv = l == 0.f ? 0.f : 1.0f / l;
+            kv8_store2<BF16>(a, m, head, 4 * lane, v.x * inv, v.y * inv, wide & 1);
+            kv8_store2<BF16>(a, m, head, 4 * lane + 2, v.z * inv, v.w * inv, wide & 1);
+            continue;
+        }
+        float* to = parts + (((size_t)(split / cluster) * a.pool.kv_heads + kvh) * pairs + p) * (g.vp + 4);
         if (lane == 0) *reinterpret_cast<float2*>(to) = make_float2(top, l);
         if (4 * lane < g.vp) *reinterpret_cast<float4*>(to + 4 + 4 * lane) = v;
     }
@@ -685,7 +693,7 @@ __global__ void __launch_bounds__(THREADS, 1) kv8_prefix_kernel(const Kv8AttnArg
 template <bool BF16, int TERMS, bool PAIRED>
 cudaError_t launch(const Kv8AttnArgs& a, const Kv8Prefix& p, float* parts, cudaStream_t st) {
     const Shape g = shape_of(a.pool.dim, a.pool.vdim, TERMS, PAIRED ? 2 : 1);
-    const int size = BF16 ? 2 : 4, wide = a.pool.dim % 8 == 0 && (((uintptr_t)a.q | a.ldq * size) & (4 * size - 1)) == 0 ? 2 : 0;
+    const int wide = kv8_wide(a);
     const cudaError_t e = ensure_dyn_smem(kv8_prefix_kernel<BF16, TERMS, PAIRED>, g.bytes);
     if (e != cudaSuccess) return e;
     cudaLaunchConfig_t cfg = {};
