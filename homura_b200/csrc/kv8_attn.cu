@@ -38,7 +38,7 @@ namespace {
 constexpr int PAIRS = 8;           // of an item
 constexpr int LEAST_PIECES = 12;   // of a CTA, one for each of its warps: fewer would only leave more to be joined
 constexpr int BEGIN = 20;           // pieces that take a CTA as long as the beginning and end of an item
-constexpr int WHOLE = 36;           // pieces that a CTA takes in less time than a join takes
+constexpr int WHOLE = 64;           // pieces that a CTA takes in less time than a join takes
 constexpr int SOLO = 12;            // pieces that a warp takes alone where there are many items
 constexpr int MAX_DEPTH = 4;
 constexpr int MERGE_ROWS = 32;      // pairs' results of several warps that stand in shared memory when those of all are added up

@@ -32,7 +32,8 @@ constexpr int SOFT_WARPS = 16, CONV_WARPS = 3, THREADS = 768;  // those of keys,
 constexpr int COPY_WARP = SOFT_WARPS + 2 * CONV_WARPS, MMA_WARP = COPY_WARP + 1;
 constexpr int STREAM_WARPS = SOFT_WARPS / 2;
 constexpr int MAX_RAW = 8;              // pages in flight or being converted
-constexpr int RING = 4;                 // blocks whose scales are kept
+constexpr int RING = 5;                 // blocks whose scales are kept
+constexpr int MOST_BUFS = 3;            // of scores
 constexpr int MOST_PARTS = 8;           // that are left to be joined with the rows' own pages
 constexpr size_t ROOM = 226 * 1024;
 constexpr float LOG2E = 1.4426950408889634f;
@@ -43,6 +44,7 @@ constexpr float DROP = 5.f;             // weights enter as 2^(DROP - exponent o
 struct Shape {
     int dp, vp, katoms, kpart, half;  // padded sizes, pieces of 64 elements of keys, bytes of a half's keys, of a half
     int raw, kst, vst;                // pages of the ring, blocks of keys and of values as f16
+    int bufs;                         // scores of so many tasks have a place in tensor memory: three where two results of 64 elements leave one more
     uint32_t q_tile, k_tile, v_tile, q_at, k_at, v_at, raw_at, bytes;
 };
 __host__ __device__ inline Shape shape_of(int dim, int vdim, int terms, int q_tiles) {
@@ -52,11 +54,12 @@ __host__ __device__ inline Shape shape_of(int dim, int vdim, int terms, int q_ti
     s.katoms = (s.dp + 63) / 64;
     s.kpart = kv8_part_bytes(dim);
     s.half = (int)kv8_half_bytes(dim, vdim);
+    s.bufs = s.vp <= 64 ? 3 : 2;
     s.q_tile = (uint32_t)terms * s.katoms * TILE * 128;
     s.k_tile = (uint32_t)s.katoms * BLOCK * 128;
     s.v_tile = 2u * s.vp * 128;
     // two blocks of values, then of keys, where they leave the ring three pages (a block and half of the next); then as many pages as fit
-    const uint32_t page = 2u * s.half, room = (uint32_t)ROOM - 8192 - 1024 - q_tiles * s.q_tile;
+    const uint32_t page = 2u * s.half, room = (uint32_t)ROOM - 9216 - 1024 - q_tiles * s.q_tile;
     s.vst = s.k_tile + 2 * s.v_tile + 3 * page <= room ? 2 : 1;
     s.kst = 2 * s.k_tile + s.vst * s.v_tile + 3 * page <= room ? 2 : 1;
     s.raw = (int)((room - s.kst * s.k_tile - s.vst * s.v_tile) / page);
@@ -72,7 +75,7 @@ __host__ __device__ inline Shape shape_of(int dim, int vdim, int terms, int q_ti
 }
 
 struct Shared {
-    uint64_t raw_full[MAX_RAW], raw_empty[MAX_RAW], k_full[2], k_empty[2], v_full[2], v_empty[2], s_full[2], p_full[2], pv_done[2], sc_full[RING], q_full, done;
+    uint64_t raw_full[MAX_RAW], raw_empty[MAX_RAW], k_full[2], k_empty[2], v_full[2], v_empty[2], s_full[MOST_BUFS], p_full[MOST_BUFS], pv_done[MOST_BUFS], sc_full[RING], q_full, done;
     uint32_t tmem;
     volatile int abort_flag;
     int longest;
@@ -215,6 +218,8 @@ __global__ void __launch_bounds__(THREADS, 1) kv8_prefix_kernel(const Kv8AttnArg
             mb_init(&sh.k_empty[s], 1);
             mb_init(&sh.v_full[s], CONV_WARPS);
             mb_init(&sh.v_empty[s], 1);
+        }
+        for (int s = 0; s < MOST_BUFS; ++s) {
             mb_init(&sh.s_full[s], 1);
             mb_init(&sh.p_full[s], STREAM_WARPS);
             mb_init(&sh.pv_done[s], 1);
@@ -246,7 +251,7 @@ __global__ void __launch_bounds__(THREADS, 1) kv8_prefix_kernel(const Kv8AttnArg
     tc_fence_before();
     __syncthreads();
     tc_fence_after();
-    const uint32_t tmem = sh.tmem;
+    const uint32_t tmem = sh.tmem, o_at0 = tmem + (uint32_t)g.bufs * BLOCK, o_step = g.bufs == 2 ? 128u : 64u;  // the streams' results, behind the scores
     const int longest = sh.longest, nb = (longest + BLOCK - 1) / BLOCK, per = (nb + splits - 1) / splits, b0 = min(nb, split * per), n = min(nb, b0 + per) - b0;  // this CTA's blocks
     const int tasks = PAIRED ? 2 * n : n;  // task j belongs to stream j & 1
     auto block_of = [&](int j) { return PAIRED ? j >> 1 : j; };  // counted from b0
@@ -283,14 +288,16 @@ __global__ void __launch_bounds__(THREADS, 1) kv8_prefix_kernel(const Kv8AttnArg
         const uint32_t q_lo = desc_lo(s32(base + g.q_at)), k_lo = desc_lo(s32(base + g.k_at)), v_lo = desc_lo(s32(base + g.v_at));
         auto wait = [&](uint64_t* bar, uint32_t parity) { return __all_sync(0xffffffffu, mb_wait(bar, parity, a.err_flag, &sh.abort_flag)); };
         bool ok = tasks == 0 || wait(&sh.q_full, 0);
-        for (int j = 0; j < tasks + 2 && ok; ++j) {
-            const int s = j & 1;
-            const uint32_t d_s = tmem + (uint32_t)s * BLOCK, d_o = tmem + 2 * BLOCK + (uint32_t)s * 128;
-            if (j >= 2) {  // the product of task j - 2
-                const int t = j - 2, b = block_of(t);
+        int buf = 0;      // task j and the one `bufs` in front of it have the same place
+        uint32_t turn = 0;  // j / bufs
+        for (int j = 0; j < tasks + g.bufs && ok; ++j) {
+            const uint32_t d_s = tmem + (uint32_t)buf * BLOCK;
+            if (j >= g.bufs) {  // the product of that task
+                const int t = j - g.bufs, b = block_of(t), s = t & 1;
+                const uint32_t d_o = o_at0 + (uint32_t)s * o_step;
                 const int vs = b & (g.vst - 1);  // one stage or two
                 if ((!PAIRED || s == 0) && !(ok = wait(&sh.v_full[vs], (b >> (g.vst - 1)) & 1))) break;
-                if (!(ok = wait(&sh.p_full[s], (t >> 1) & 1))) break;
+                if (!(ok = wait(&sh.p_full[buf], (turn - 1) & 1))) break;
                 tc_fence_after();
                 const uint32_t v = v_lo + (uint32_t)vs * (g.v_tile / 16);
                 if (lead) {
@@ -299,16 +306,16 @@ __global__ void __launch_bounds__(THREADS, 1) kv8_prefix_kernel(const Kv8AttnArg
 #pragma unroll
                         for (int k = 0; k < BLOCK / 16; ++k)
                             mma_ts(d_o, d_s + (k >> 1) * 32 + h * 16 + (k & 1) * 8, v + (uint32_t)(k >> 2) * (g.v_tile / 32) + (k & 3) * 2, id_o, t > 1 || h > 0 || k > 0);
-                    mma_commit(&sh.pv_done[s]);
+                    mma_commit(&sh.pv_done[buf]);
                     if (!PAIRED || s == 1) mma_commit(&sh.v_empty[vs]);
                 }
                 __syncwarp();
             }
             if (j < tasks) {
-                const int b = block_of(j);
+                const int b = block_of(j), s = j & 1;
                 const int ks = b & (g.kst - 1);
                 if ((!PAIRED || s == 0) && !(ok = wait(&sh.k_full[ks], (b >> (g.kst - 1)) & 1))) break;
-                if (j >= 2 && !(ok = wait(&sh.pv_done[s], ((j - 2) >> 1) & 1))) break;  // the weights stand where the scores go
+                if (j >= g.bufs && !(ok = wait(&sh.pv_done[buf], (turn - 1) & 1))) break;  // the weights stand where the scores go
                 tc_fence_after();
                 if (lead) {
                     const uint32_t q = q_lo + (PAIRED ? (uint32_t)s * (g.q_tile / 16) : 0u), key = k_lo + (uint32_t)ks * (g.k_tile / 16);
@@ -320,10 +327,14 @@ __global__ void __launch_bounds__(THREADS, 1) kv8_prefix_kernel(const Kv8AttnArg
                             mma_ss(d_s, q + (uint32_t)h * (g.q_tile / TERMS / 16) + at, key + at, id_s, more);
                             more = true;
                         }
-                    mma_commit(&sh.s_full[s]);
+                    mma_commit(&sh.s_full[buf]);
                     if (!PAIRED || s == 1) mma_commit(&sh.k_empty[ks]);
                 }
                 __syncwarp();
+            }
+            if (++buf == g.bufs) {
+                buf = 0;
+                ++turn;
             }
         }
         // what was issued has to end before the tensor memory is given back
@@ -360,8 +371,8 @@ __global__ void __launch_bounds__(THREADS, 1) kv8_prefix_kernel(const Kv8AttnArg
             if (ok && b > more) ok = wait(values ? &sh.v_empty[st] : &sh.k_empty[st], ((b >> more) - 1) & 1);
             if (!ok) break;
             if (!values) {
-                // scales, and what there is of the block.  What stood in their ring is four blocks old: the scores of the block two in front are done, whose place the keys take, or of
-                // the one in front, and its stream's products were done before those were begun
+                // scales, and what there is of the block.  What stood in their ring is five blocks old.  The keys took the place of those of block b - 2 or b - 1, whose scores are done;
+                // the products that stood in their place were done before: with three places for scores, those of block b - 5 at least
                 const int ring = b % RING, left = longest - (b0 + b) * BLOCK;
                 uint32_t top = 0;
                 int there = 0;
@@ -443,7 +454,7 @@ __global__ void __launch_bounds__(THREADS, 1) kv8_prefix_kernel(const Kv8AttnArg
         }
     } else {
         // ---- scores to weights ----
-        const uint32_t lanes = (uint32_t)(warp & 3) * 32 << 16, s_at = tmem + lanes + (uint32_t)stream * BLOCK, o_at = tmem + lanes + 2 * BLOCK + (uint32_t)stream * 128;
+        const uint32_t lanes = (uint32_t)(warp & 3) * 32 << 16, o_at = o_at0 + lanes + (uint32_t)stream * o_step;
         float c = 0.f;  // what scores are multiplied with
         if (n > 0) {
             // eight elements a lane, 8 or 16 lanes to a pair, so that a row is read by neighbours; the loads of several groups of pairs are on their way at once
@@ -508,9 +519,12 @@ __global__ void __launch_bounds__(THREADS, 1) kv8_prefix_kernel(const Kv8AttnArg
         float ref = -INFINITY, over = -INFINITY, l = 0.f;  // the pair's largest score at the last move; the exponent that value scales are brought down from; sum of the weights of this side
         float unit = -INFINITY;                            // reference of the weights: ref + over - DROP
         const int mine_n = PAIRED ? n : (n + 1 - stream) / 2, t0 = 64 * side;
+        int buf = stream, before = 0;           // places of the scores of task 2 i + stream, and of the stream's task in front
+        uint32_t turn = 0, turn_before = 0;     // parities of the waits for them
         for (int i = 0; i < mine_n; ++i) {
+            const uint32_t s_at = tmem + lanes + (uint32_t)buf * BLOCK;
             const int b = PAIRED ? i : 2 * i + stream, ring = b % RING;
-            ok = __all_sync(0xffffffffu, mb_wait(&sh.sc_full[ring], (b / RING) & 1, a.err_flag, &sh.abort_flag) && mb_wait(&sh.s_full[stream], i & 1, a.err_flag, &sh.abort_flag));
+            ok = __all_sync(0xffffffffu, mb_wait(&sh.sc_full[ring], (b / RING) & 1, a.err_flag, &sh.abort_flag) && mb_wait(&sh.s_full[buf], turn, a.err_flag, &sh.abort_flag));
             tc_fence_after();
             const int seen = (sh.there[ring] >> side) & 1 ? len - (b0 + b) * BLOCK - t0 : 0;  // tokens of this side in front of the row's end
             const bool masked = __any_sync(0xffffffffu, seen < 64);
@@ -561,7 +575,9 @@ __global__ void __launch_bounds__(THREADS, 1) kv8_prefix_kernel(const Kv8AttnArg
             const float ve = (float)(max(sh.ve[ring], 27) - 127);
             if (ve > over) over = ve + VALUE_ROOM;
             const float now = ref + over - DROP;  // -inf while the pair has seen nothing
-            if (i > 0 && __any_sync(0xffffffffu, now != unit)) {  // O is the product of the blocks so far: complete, since its stream's scores came behind it
+            if (i > 0 && __any_sync(0xffffffffu, now != unit)) {  // O is the product of the blocks so far, when the last of them is done
+                ok = __all_sync(0xffffffffu, mb_wait(&sh.pv_done[before], turn_before, a.err_flag, &sh.abort_flag));
+                tc_fence_after();
                 const float corr = unit == -INFINITY || now == unit ? 1.f : exp2_ftz(unit - now);
                 l *= corr;
 #pragma unroll 1
@@ -619,7 +635,13 @@ __global__ void __launch_bounds__(THREADS, 1) kv8_prefix_kernel(const Kv8AttnArg
             tmem_st_wait();
             tc_fence_before();
             __syncwarp();
-            if (lane == 0) mb_arrive(&sh.p_full[stream]);
+            if (lane == 0) mb_arrive(&sh.p_full[buf]);
+            before = buf;
+            turn_before = turn;
+            if ((buf += 2) >= g.bufs) {
+                buf -= g.bufs;
+                turn ^= 1u;
+            }
         }
         // all products are done: of this stream, and those that read what stands where the results go
         ok = __all_sync(0xffffffffu, mb_wait(&sh.done, 0, a.err_flag, &sh.abort_flag)) && ok;
