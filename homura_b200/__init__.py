@@ -741,6 +741,12 @@ def qknorm_rope(x, cos_rows, sin_rows, norm_w=None, eps: float = 1e-6) -> np.nda
 # arguments integer device addresses, sizes and types given; rows may be `ld` elements apart.
 
 
+def _flat(x):
+    """[M, ...] as [M, elements]; M may be 0."""
+    x = np.asarray(x)
+    return x.reshape(len(x), int(np.prod(x.shape[1:])))
+
+
 def _rows_in(x):
     """(contiguous [rows, K] array, its DType) of f32 rows or bf16 bits."""
     x = np.atleast_2d(np.asarray(x))
@@ -1052,7 +1058,7 @@ def rope(x, heads: int, dim: int, turns, pos, rot: Optional[int] = None, neighbo
         (xa, M) = x
         _check(lib.hm_rope(_ptr(xa), int(dtype), ldx or heads * dim, M, heads, dim, rot, int(neighbours), _ptr(pos), _ptr(turns), magnitude, _ptr(y), ldy or heads * dim, _ptr(stream)))
         return None
-    xa, dtype = _rows_in(np.asarray(x).reshape(len(x), -1))
+    xa, dtype = _rows_in(_flat(x))
     M = xa.shape[0]
     turns, pos = np.ascontiguousarray(turns, dtype=np.float64), np.ascontiguousarray(pos, dtype=np.int32)
     if xa.shape[1] != heads * dim or turns.size != rot // 2 or pos.size != M:
@@ -1097,7 +1103,7 @@ class KV8Cache:
             (ka, M) = k
             _check(lib.hm_kv8_write(C.byref(c), _ptr(ka), _ptr(v), int(dtype), ldk or wk, ldv or wv, _ptr(row_seq), _ptr(row_pos), M, _ptr(stream)))
             return
-        (ka, dtype), (va, other) = _rows_in(np.asarray(k).reshape(len(k), -1)), _rows_in(np.asarray(v).reshape(len(v), -1))
+        (ka, dtype), (va, other) = _rows_in(_flat(k)), _rows_in(_flat(v))
         seq, pos = self._rows(row_seq, row_pos, len(ka))
         if dtype != other or len(ka) != len(va) or ka.shape[1] != wk or va.shape[1] != wv:
             raise HomuraError(HM_ERR_INVALID, "keys and values are rows [M, kv_heads * dim] and [M, kv_heads * vdim] of one type")
@@ -1127,7 +1133,7 @@ class KV8Cache:
             (qa, M), (sa, n) = q, shared or (None, 0)
             _check(lib.hm_kv8_attn(C.byref(c), _ptr(qa), int(dtype), ldq or wq, _ptr(row_seq), _ptr(row_pos), M, heads, scale, _ptr(sa), n, _ptr(out), ldo or wo, _ptr(work), _ptr(stream)))
             return None
-        qa, dtype = _rows_in(np.asarray(q).reshape(len(q), -1))
+        qa, dtype = _rows_in(_flat(q))
         seq, pos = self._rows(row_seq, row_pos, len(qa))
         if qa.shape[1] != wq:
             raise HomuraError(HM_ERR_INVALID, "queries are rows [M, heads * dim]")
