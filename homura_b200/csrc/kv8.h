@@ -63,7 +63,7 @@ struct Kv8AttnArgs {
     void* work;
     int* err_flag;
     // filled in by the launcher
-    int solo;                // items of at most so many pieces are a warp's own
+    int solo, team;          // items of at most so many pieces belong to so many warps
     int whole;               // a CTA takes an item as a whole, and there are no more items than CTAs
     int direct;              // kv8_prefix.cu writes the rows that have nothing but the prefix
     int own_from;            // the rows' own pieces (halves of pages) begin here: what stands in front is in `prefix`

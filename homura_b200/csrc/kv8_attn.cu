@@ -247,6 +247,13 @@ __device__ __forceinline__ void put_digits(const float (&x)[8], float up, uint4*
 // What is left of an item in `work`: maximum and sum of every pair, then its elements (relative to the maximum, not divided).
 __host__ __device__ inline size_t part_floats(int vp) { return PAIRS * (size_t)(vp + 4); }
 
+// Barrier of a team's warps, with an OR over their predicates.
+__device__ __forceinline__ bool team_any(int team, int threads, bool v) {
+    uint32_t r;
+    asm volatile("{ .reg .pred p, q; setp.ne.u32 p, %1, 0; barrier.cta.red.or.aligned.pred q, %2, %3, p; selp.u32 %0, 1, 0, q; }" : "=r"(r) : "r"((uint32_t)v), "r"(1 + team), "r"(threads) : "memory");
+    return r != 0;
+}
+
 // Parts in `work`: of CTA c its first item (0) and its last (1).
 __device__ __forceinline__ float* cta_part(const Kv8AttnArgs& a, int vp, int cta, int which) { return static_cast<float*>(a.work) + (size_t)(2 * cta + which) * part_floats(vp); }
 
@@ -450,8 +457,9 @@ __global__ void __launch_bounds__(WARPS * 32, 1) kv8_stream_kernel(const Kv8Attn
     const int gid = lane >> 2, tig = lane & 3, slabs = sh.dp / 32, vslabs = sh.vp / 32;
     int i = 0, slot = 0, len = 0;  // this warp's next piece, counted over the CTA (or its own item), and its slot; tokens of the segment's row
     bool good = true;                         // no wait has run out
-    bool alone = line.solo;                   // with items of this warp's own; then with the line
-    int own = warp * ctas + (int)blockIdx.x;  // those are every WARPS * ctas-th of all
+    bool alone = line.solo;                   // with items of this warp's team; then with the line
+    const int teams = WARPS / a.team, team = warp / a.team, in_team = warp - team * a.team;
+    int own = team * ctas + (int)blockIdx.x;  // those are every teams * ctas-th of all
     uint4* own_queries = queries + warp * sh.queries;  // where the line's queries and sums will stand
     float next_q[8];
     int begin = 0, turn = 0;
@@ -464,7 +472,7 @@ __global__ void __launch_bounds__(WARPS * 32, 1) kv8_stream_kernel(const Kv8Attn
         const uint4* qf;
         if (alone) {
             int m = 0, n = 0;
-            for (; own < a.M * items; own += WARPS * ctas) {
+            for (; own < a.M * items; own += teams * ctas) {
                 m = own / items;
                 n = kv8_row_pieces(a, m);
                 if (n > 0 && n <= a.solo) break;
@@ -474,11 +482,12 @@ __global__ void __launch_bounds__(WARPS * 32, 1) kv8_stream_kernel(const Kv8Attn
                 continue;
             }
             sg = Segment{m, own - m * items, 0, n, n};
-            own += WARPS * ctas;
+            own += teams * ctas;
             __syncwarp();
-            start(sg, 0, n, 1, depth);
+            start(sg, in_team, n, a.team, depth);
             len = kv8_row_len(a, m);
-            i = begin = slot = 0;
+            begin = slot = 0;
+            i = in_team;
             // lane (gid, tig): elements 8 tig .. 8 tig + 7 of every slab of pair gid
             const int kvh = sg.item / tiles, tile = sg.item - kvh * tiles;
             const bool is = gid < min(PAIRS, group - tile * PAIRS);
@@ -669,6 +678,36 @@ __global__ void __launch_bounds__(WARPS * 32, 1) kv8_stream_kernel(const Kv8Attn
         l += __shfl_xor_sync(0xffffffffu, l, 1);
         l += __shfl_xor_sync(0xffffffffu, l, 2);
         if (alone) {
+            if (a.team > 1) {  // the team's results to its first warp, by way of the others' first slot, which is free (32 * padded vdim bytes, and the scales' place)
+                float* mine = reinterpret_cast<float*>(vbuf);
+                if (in_team > 0) {
+                    if (tig == 0) *reinterpret_cast<float2*>(mine + PAIRS * sh.vp + 2 * gid) = make_float2(mx, l);
+#pragma unroll
+                    for (int s = 0; s < VS * 4; ++s)
+                        if (s < vslabs * 4) *reinterpret_cast<float2*>(mine + gid * sh.vp + 8 * (s ^ (gid & 3)) + 2 * tig) = make_float2(o[s][0], o[s][1]);
+                }
+                good = !team_any(team, a.team * 32, !good);
+                if (in_team == 0) {
+                    for (int w = 1; w < a.team; ++w) {
+                        const float* from = reinterpret_cast<const float*>(vbuf + (size_t)w * depth * (sh.kpart + sh.vpart));
+                        const float2 ml = *reinterpret_cast<const float2*>(from + PAIRS * sh.vp + 2 * gid);
+                        const float now = fmaxf(mx, ml.x), ref = now == -INFINITY ? 0.f : now, f0 = exp2f(mx - ref), f1 = exp2f(ml.x - ref);
+                        l = fmaf(l, f0, ml.y * f1);
+                        mx = now;
+#pragma unroll
+                        for (int s = 0; s < VS * 4; ++s) {
+                            if (s >= vslabs * 4) break;
+                            const float2 x = *reinterpret_cast<const float2*>(from + gid * sh.vp + 8 * (s ^ (gid & 3)) + 2 * tig);
+                            o[s][0] = fmaf(o[s][0], f0, x.x * f1);
+                            o[s][1] = fmaf(o[s][1], f0, x.y * f1);
+                        }
+                    }
+                }
+                team_any(team, a.team * 32, false);  // they have been read
+                asm volatile("fence.proxy.async.shared::cta;" ::: "memory");  // pieces are copied there again
+                __syncwarp();
+                if (in_team > 0) continue;
+            }
             if (!waited) pdl_wait();  // the parts of the prefix are there
             waited = true;
             if (a.prefix_n) add_prefix_to<VS>(a, sh.vp, kvh, sg.m * group + tile * PAIRS + min(gid, pairs - 1), tig, mx, l, o);
@@ -942,6 +981,9 @@ cudaError_t launch_stream(const Kv8AttnArgs& a_in, int sm_count, cudaStream_t st
     while (depth > 1 && bytes(depth) > ROOM) --depth;
     // where there are more items than CTAs, a CTA would take them one by one
     const long all = (long)a.M * a.pool.kv_heads * tiles, most = std::max(0l, (long)a.pool.max_pages * (KV8_PAGE / KV8_HALF) - a.own_from);  // items; pieces of one
+    a.team = 1;
+    for (int t = 2; t <= 4; ++t)
+        if (WARPS % t == 0 && all <= (long)ctas * (WARPS / t)) a.team = t;
     a.solo = all >= 2 * sm_count ? SOLO : 0;
     a.whole = all <= ctas && most <= WHOLE;
     const bool own = most > 0 || a.prefix_n == 0, cut = own && !a.whole && most > a.solo, rest = a.prefix_n > 0 && !a.direct;
