@@ -15,7 +15,7 @@
 namespace hm {
 namespace {
 
-constexpr int WT = 256;
+constexpr int WT = 128;
 constexpr int MOST_ROWS = 32;                   // of a CTA
 constexpr float TINY = 7.888609052210118e-31f;  // 2^-100
 constexpr int LDV = KV8_MAX_DIM + 4;            // bytes from row to row in shared memory: an odd number of words
