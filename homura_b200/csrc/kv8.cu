@@ -6,7 +6,9 @@
 //
 // A CTA takes `rows` consecutive rows of the call and one head.  LANES lanes share a vector, eight elements each, and have several vectors on their way before they look for the rows' places.
 // Codes of keys stand by token and go straight to their places; codes of values stand by element, 32 tokens side by side, so they pass through shared memory: four rows that follow one
-// another in a page (rows of a prompt) become words of four tokens, others single bytes.  What bounds both directions is bytes.
+// another in a page (rows of a prompt) become words of four tokens, others single bytes.
+// 8191 rows of 8 heads of 128 in bf16, written and read back: 27 us (102 MB, 3.8 TB/s), where bytes alone take 15.5: the write's instructions, some 85 for 256 elements, are in the way (the schedulers
+// issue in 6 of 10 cycles).  Blocks of 256 and 512 threads: 29 and 49 us; 16 rows to a block instead of 32: 44 us; four elements a lane, one vector of a group at a time: 47 us.
 #include "kv8.h"
 #include "rows.cuh"
 

@@ -4,7 +4,7 @@
 // (kv8_prefix.cu), and what follows here begins behind them and joins both.
 //
 // kv8_stream_kernel   rows' contexts, eight (row, head) pairs of one key/value head at a time; bound by the bytes of the cache
-// kv8_join_kernel     joins the parts of contexts that several CTAs share
+// kv8_join_kernel     joins the parts of contexts that several CTAs share; launched where there can be such
 //
 // Arithmetic of the first.  A warp takes a piece, 32 tokens (half of a page), for eight pairs, on m16n8k32 MMAs of 8-bit whole numbers with 32-bit sums, whose B operands are the
 // codes as they are cached:
@@ -15,13 +15,21 @@
 // codes are exact; what f32 rounds is what one would round without digits.  A token's key scale joins behind the product, its value scale goes into the weight,
 // W = 2^(s - max) * scale, so that the largest of a piece is found with it.
 // Against f16 operands (codes become f16 by two instructions for two codes, queries and weights by two terms): 981 instructions for 32 tokens x 256 elements, of which
-// a third made f16 of codes, 105 us for 64 sequences of up to 8000 tokens (366 MB).
+// a third made f16 of codes, 105 us for 64 sequences of 500 to 8000 tokens (366 MB).
 //
-// Work.  The pieces of all rows, heads and tiles of eight pairs stand in one line, which the CTAs cut into equal lengths: contexts of any lengths keep all SMs busy to the
-// end, and no length needs to be known on the host.  A CTA's warps take its pieces in turn, each with a ring of copies of its own; what they have of an item is added up in shared
-// memory.  The CTA writes the items that it has as a whole and leaves the rest (its first and its last) in `work`, for kv8_join_kernel.  Items of a few pieces are not worth a CTA's
-// attention (adding up and two barriers take some 5 us): they are no part of the line, and every warp takes some of them alone before it joins in.
-// Slower where tried, at 64 sequences of up to 8000 tokens (93 us with each of them): a range of pieces for every warp, which then has more partial items than are worth joining; whole
+// Work.  The pieces of all rows, heads and tiles of eight pairs stand in one line, which the CTAs cut into lengths of equal cost: contexts of any lengths keep all SMs busy to the
+// end, and no length needs to be known on the host.  An item's beginning (queries, sums of the warps, barriers) counts as much as BEGIN pieces: with 0, 6, 12, 20 and 28 the 64
+// sequences took 99, 91, 79, 75 and 77 us.  A CTA's warps take its pieces in turn, each with a ring of copies of its own; what they have of an item is added up in shared memory.  The
+// CTA writes the items that it has as a whole and leaves the rest (its first and its last) in `work`, for kv8_join_kernel.
+// Two kinds of items are no part of the line:
+//   short ones where there are many.  Adding up takes a CTA some 5 us, so that a team of 1 to 4 warps takes an item of up to SOLO pieces, before the CTA joins in with the line: as many
+//   warps as leave each item a team.  64 rows of up to 500 own tokens behind a prefix: teams of 3 60 us, of 2 63, single warps 67 (all in the line: 105 when single warps took 80); limits of 8 and 16 pieces instead of
+//   12 (single warps): 72 and 71 us, and 16 pieces at the 64 sequences above 97 us, as a team's items are not shared out.
+//   all of them where there are no more than CTAs and the table has room for WHOLE pieces at most: a CTA takes an item, nothing is counted or joined.  One row of 14 heads over 2 of 64
+//   elements: 64 tokens 6.6 us against 10.8, 1024 10.1 against 14.7, 2048 14.0 against 16.0, 3000 17.7 against 16.1.
+// 64 sequences of 500 to 8000 tokens, 8 heads of 128: 74 us, 4.9 TB/s, three quarters of what a copy reaches; what is left is the start (7 us to the first scores) and the uneven end.  Three rows
+// of 20000 to 32768 tokens: 22 us, of which the join takes 5.
+// Slower where tried, at the 64 sequences with an even line (93 us with each of them): a range of pieces for every warp, which then has more partial items than are worth joining; whole
 // pages for a warp, of which 12 do not fit twice; 16 warps with one piece each.
 #include "kv8.h"
 

@@ -11,8 +11,15 @@
 //
 // 24 warps: 0 .. 7 and 8 .. 15 turn scores into weights, two threads for every pair, a page each; 16 .. 18 make f16 of keys' codes, 19 .. 21 of values'; 22 copies pages; 23 issues the MMAs.  Two streams of
 // blocks take turns on the tensor cores, so that one's MMAs run beside the other's exponentials: the two halves of 256 pairs over the same blocks (a block's codes are then converted once
-// for both), or, for fewer pairs and f32 rows, whose two terms leave room for one tile of queries, the even and the odd blocks of 128 pairs.  The token axis is split where there are too few pairs for all SMs; splits form
-// clusters that join what they have over their shared memory, and what is left goes to `work`, relative to its references, to be joined with the rows' own pages.
+// for both), or, for fewer pairs and f32 rows, whose two terms leave room for one tile of queries, the even and the odd blocks of 128 pairs.  Weights stand where their scores were; where
+// two results of 64 elements leave room, a third place lets a stream's next scores come while its weights are still multiplied (256 rows of 32 heads behind 16384 tokens: 111 -> 106 us).
+// The token axis is split where there are too few pairs for all SMs; splits form clusters that join what they have over their shared memory.  A row that has nothing but the prefix is then
+// done, where that leaves one part; others, and further parts, go to `work`, relative to their references, to be joined with the rows' own pages.
+//
+// What bounds it: the instructions of the softmax.  256 rows of 32 heads over 4 of 64 elements: 4700 cycles for a block of 256 pairs, in which the schedulers issue in 7 of 10 (exponentials fill
+// 2050 of them, the tensor cores 730); 106 us in all, 325 TFLOP/s.  With 128 elements a block takes 7000, as the only place for keys is converted (4000)
+// between two blocks' scores: 1021 rows of 12 heads, 87 us.  Found slower there: two places for keys and one for values (109 us); a pass that finds no maximum and is done again where a
+// score exceeds its reference by too much, which a quarter of the blocks does with heavy-tailed scores; all six converting warps on keys, then on values (the 256 rows 117 us).
 #include <algorithm>
 #include <map>
 #include <mutex>

@@ -4,7 +4,9 @@
 //
 // Angles: turns * position in 64 bits, less its nearest quarter, leaves at most an eighth of a turn, which f32 holds to 2^-28; so a far position is as
 // exact as a near one.  A block has `rows` rows: it computes their sines and cosines once, in shared memory, and all heads take them from there; the elements that a thread
-// begins with are on their way meanwhile.  What bounds it is bytes, for few rows the chain of a position's load, its sine, a barrier and the rows' elements.
+// begins with are on their way meanwhile.  What bounds it is bytes, for few rows the chain of a position's load, its sine, a barrier and the rows'
+// elements.  8191 rows of 14 heads (and 2 beside them) of 128 in bf16: 13.0 us (4.5 TB/s) against 15.4 with one row to a block and elements loaded behind the sines.  Blocks of 128 threads:
+// 12.3 us there, but 3.5 instead of 2.8 us for 64 rows of 36 heads.
 #include "rope.h"
 
 #include "rows.cuh"
