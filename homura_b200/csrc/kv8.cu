@@ -1,7 +1,7 @@
 // Keys and values into a paged cache of 8 bits, and back.
 //
-// A row's key (or value) of one head is quantised as a whole: m = max |x|, code = rint(x * (127 / m)), scale = m / 127, every step rounded to f32, so that
-// each implementation gives the same bits; m < 2^-100 leaves zeros with the scale 0, an infinity or a NaN makes the scale NaN and with it the whole vector.
+// A row's key (or value) of one head is quantised as a whole: m = max |x|, code = rint(x * (127 * (1 / m))), scale = m * (1 / 127), every step rounded to f32, so that each implementation
+// gives the same bits (those of the elementary operations of torch on a GPU, where a quotient with a number is a product with a reciprocal); m < 2^-100 leaves zeros with the scale 0, an infinity or a NaN makes the scale NaN and with it the whole vector.
 // The maximum is taken over the bits of |x|, among which those of infinities and NaN are the largest.
 //
 // A CTA takes `rows` consecutive rows of the call and one head.  LANES lanes share a vector, eight elements each, and have several vectors on their way before they look for the rows' places.
@@ -134,14 +134,14 @@ __global__ void __launch_bounds__(WT) kv8_write_kernel(const Kv8RowsArgs a, int 
             for (int o = LANES / 2; o > 0; o >>= 1) t = max(t, __shfl_xor_sync(mask, t, o));
             if (lane == k) top = t;
         }
-        // the first lanes divide for all
+        // the first lanes find the factors for all
         const float most = __uint_as_float(top);
         const bool finite = top < 0x7F800000u, some = finite && most >= TINY;
-        const float up = some ? __fdiv_rn(127.f, most) : 0.f;
+        const float up = some ? __fmul_rn(__frcp_rn(most), 127.f) : 0.f;
         {
             const int i = base + group + lane * GROUPS, r = i >= rows ? i - rows : i;
             if (lane < AHEAD && i < 2 * rows && s.key[r])
-                reinterpret_cast<float*>(s.key[r] + (i >= rows ? kv8_part_bytes(dim) : 0))[s.token[r]] = !finite ? __uint_as_float(0x7FC00000u) : some ? __fdiv_rn(most, 127.f) : 0.f;
+                reinterpret_cast<float*>(s.key[r] + (i >= rows ? kv8_part_bytes(dim) : 0))[s.token[r]] = !finite ? __uint_as_float(0x7FC00000u) : some ? __fmul_rn(most, 1.0f / 127.0f) : 0.f;
         }
 #pragma unroll
         for (int k = 0; k < AHEAD; ++k) {

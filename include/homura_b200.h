@@ -391,7 +391,7 @@ HM_API int hm_rope_turns(double theta, int rot, int kind, double factor, double 
  * dim <= 1024; rot even.  The heads of queries and keys that stand side by side in a projection's rows are one call. */
 HM_API int hm_rope(const void* x, int dtype, size_t ldx, int M, int heads, int dim, int rot, int neighbours, const int32_t* pos, const double* turns, float magnitude, void* y, size_t ldy, void* stream);
 /* A paged cache of 8 bits: 64 tokens per page; per token and head one f32 scale for the key and one for the value.  With m the largest magnitude of a key (of a value):
- * codes rint(x * (127 / m)), scale m / 127, each step rounded to f32 (so a value is off by at most half a scale); m < 2^-100: zeros; an infinity or a NaN: the whole
+ * codes rint(x * (127 * (1 / m))), scale m * (1 / 127), each step rounded to f32 (so a value is off by at most half a scale and 2^-21 of itself); m < 2^-100: zeros; an infinity or a NaN: the whole
  * vector is NaN.  `pages` is device memory of hm_kv8_pool_bytes, 16-byte aligned, that needs no clearing; one pool holds keys and values of a layer.
  * A position whose entry of page_table [n_seq, max_pages] lies outside [0, n_pages) has no place (-1: not there, or given up again).
  * dim, vdim <= 256; kv_heads <= 1024; max_pages <= 2^24. */

@@ -18,9 +18,9 @@ def quantise(x):
         m = np.abs(x).max(-1, keepdims=True)
         bad = ~np.isfinite(x).all(-1, keepdims=True)
         some = ~bad & (m >= np.float32(2.0**-100))
-        up = np.float32(127) / np.where(some, m, np.float32(1))
+        up = np.float32(127) * (np.float32(1) / np.where(some, m, np.float32(1)))
         codes = np.where(some, np.rint(np.where(some, x, 0) * up), 0).astype(np.int32)
-        scales = np.where(bad, np.float32(np.nan), np.where(some, m / np.float32(127), np.float32(0))).astype(np.float32)
+        scales = np.where(bad, np.float32(np.nan), np.where(some, m * (np.float32(1) / np.float32(127)), np.float32(0))).astype(np.float32)
     return codes, scales
 
 
