@@ -88,8 +88,8 @@ cudaError_t launch_v(const RopeArgs& a, int sm_count, cudaStream_t st) {
     // rows until every thread has something to do, 16 at most, but no fewer blocks than four for every SM
     const int pieces = a.heads * (a.neighbours ? (V == 1 ? a.rot / 2 : a.rot / V) : a.rot / 2 / V);
     int rows = 1;
-    while (rows < 16 && rows * pieces < RT && (a.M + 2 * rows - 1) / (2 * rows) >= 4 * sm_count) rows *= 2;
-    const unsigned grid = (unsigned)((a.M + rows - 1) / rows);
+    while (rows < 16 && rows * pieces < RT && ((long)a.M + 2 * rows - 1) / (2 * rows) >= 4 * sm_count) rows *= 2;
+    const unsigned grid = (unsigned)(((long)a.M + rows - 1) / rows);
     const size_t smem = sizeof(float2) * (size_t)(a.rot / 2) * rows;
     if (a.neighbours) rope_kernel<BF16, V, true><<<grid, RT, smem, st>>>(a, rows);
     else rope_kernel<BF16, V, false><<<grid, RT, smem, st>>>(a, rows);

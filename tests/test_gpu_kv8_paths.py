@@ -371,3 +371,28 @@ def test_many_rows_of_few_heads(hm, M, heads, dim, rot, neighbours, bf16):
     got = bf16_value(got) if bf16 else got
     if rot < dim:
         np.testing.assert_array_equal(got.reshape(M, heads, dim)[..., rot:], x.reshape(M, heads, dim)[..., rot:])
+
+
+@pytest.mark.parametrize("bf16", [False, True])
+@pytest.mark.parametrize("rows,pages,dim,width", [(5, 0, 64, 4), (5, 0, 64, 90), (300, 0, 32, 90), (60, 3, 64, 9), (60, 3, 128, 9), (40, 3, 64, 3)])
+def test_queries_that_are_not_finite(hm, rows, pages, dim, width, bf16):
+    """A query with a NaN or an infinity makes its own head's result NaN, and no other's."""
+    m = Model(hm, rows + dim, 2, dim, dim, [64 * pages + (150 if width > pages else 0)] * 2, n_shared=pages, max_pages=width)
+    seq, pos = np.arange(rows) % 2, np.full(rows, m.lens[0] - 1) - np.arange(rows) % 70
+    q, clean = attend(m, seq, pos, 6, bf16, shared=pages > 0)
+    bad = (bf16_value(q) if bf16 else q).copy().reshape(rows, 6, dim)
+    bad[1, 4, 3], bad[rows - 1, 0, 0], bad[rows // 2, 5, dim - 1] = np.nan, np.inf, -np.inf
+    bad = bad.reshape(rows, -1)
+    out = m.cache.attend(bf16_bits(bad) if bf16 else bad, seq, pos, 6, dim**-0.5, shared=m.shared if pages else None)
+    hit = np.zeros((rows, 6), bool)
+    hit[[1, rows - 1, rows // 2], [4, 0, 5]] = True
+    f = (bf16_value(out) if bf16 else out).reshape(rows, 6, dim)
+    assert np.isnan(f[hit]).all()
+    np.testing.assert_array_equal(out.reshape(rows, 6, dim)[~hit], clean.reshape(rows, 6, dim)[~hit])
+
+
+@pytest.mark.parametrize("heads,kv_heads,dim,pages", [(256, 256, 8, 2), (1024, 2, 16, 2), (130, 1, 64, 5), (9, 1, 64, 2)])
+def test_many_heads(hm, heads, kv_heads, dim, pages):
+    m = Model(hm, heads, kv_heads, dim, dim, [64 * pages + 70, 64 * pages + 3], n_shared=pages)
+    for shared in (False, True):
+        attend(m, [0, 1, 0], [64 * pages + 69, 64 * pages + 2, 100], heads, False, shared=shared)

@@ -168,3 +168,11 @@ def test_python_forms_refuse_what_does_not_fit(hm):
                  lambda: c.read([0, 0], [0]), lambda: c.attend(rows(2, 255), [0, 0], [0, 1], 4, 1.0), lambda: c.attend(rows(2, 256), [0], [0, 1], 4, 1.0)]:
         with pytest.raises(hm.HomuraError):
             call()
+
+
+def test_attention_over_tables_too_wide(hm, memory):
+    """Rows times the table's width times heads has a limit, as the pieces of all items are counted."""
+    lib = hm.load_library()
+    size = lambda max_pages, M, heads: lib.hm_kv8_attn_bytes(C.byref(cache(hm, memory, max_pages=max_pages)), M, heads, 0)
+    assert size(2**24, 32, 128) > 0 and size(2**24, 33, 128) == 0
+    assert size(2**24, 1, 4096) > 0 and size(2**24, 2, 4096) == 0
