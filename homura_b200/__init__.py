@@ -222,6 +222,11 @@ def _ptr(a) -> C.c_void_p:
     return C.c_void_p(int(a))
 
 
+def _addr(a):
+    """The same for an argument that is mostly an int already."""
+    return a if a is None or type(a) is int else _ptr(a)
+
+
 def _check(rc: int, handle=None):
     if rc == HM_OK:
         return
@@ -1056,7 +1061,7 @@ def rope(x, heads: int, dim: int, turns, pos, rot: Optional[int] = None, neighbo
     rot = dim if rot is None else rot
     if isinstance(x, tuple):
         (xa, M) = x
-        _check(lib.hm_rope(_ptr(xa), int(dtype), ldx or heads * dim, M, heads, dim, rot, int(neighbours), _ptr(pos), _ptr(turns), magnitude, _ptr(y), ldy or heads * dim, _ptr(stream)))
+        _check(lib.hm_rope(_addr(xa), int(dtype), ldx or heads * dim, M, heads, dim, rot, int(neighbours), _addr(pos), _addr(turns), magnitude, _addr(y), ldy or heads * dim, _addr(stream)))
         return None
     xa, dtype = _rows_in(_flat(x))
     M = xa.shape[0]
@@ -1101,7 +1106,7 @@ class KV8Cache:
         lib, c, wk, wv = load_library(), self.c, self.c.kv_heads * self.c.dim, self.c.kv_heads * self.c.vdim
         if isinstance(k, tuple):
             (ka, M) = k
-            _check(lib.hm_kv8_write(C.byref(c), _ptr(ka), _ptr(v), int(dtype), ldk or wk, ldv or wv, _ptr(row_seq), _ptr(row_pos), M, _ptr(stream)))
+            _check(lib.hm_kv8_write(C.byref(c), _addr(ka), _addr(v), int(dtype), ldk or wk, ldv or wv, _addr(row_seq), _addr(row_pos), M, _addr(stream)))
             return
         (ka, dtype), (va, other) = _rows_in(_flat(k)), _rows_in(_flat(v))
         seq, pos = self._rows(row_seq, row_pos, len(ka))
@@ -1114,7 +1119,7 @@ class KV8Cache:
         lib, c, wk, wv = load_library(), self.c, self.c.kv_heads * self.c.dim, self.c.kv_heads * self.c.vdim
         if isinstance(row_seq, tuple):
             (sa, M) = row_seq
-            _check(lib.hm_kv8_read(C.byref(c), _ptr(sa), _ptr(row_pos), M, _ptr(k), _ptr(v), int(dtype), ldk or wk, ldv or wv, _ptr(stream)))
+            _check(lib.hm_kv8_read(C.byref(c), _addr(sa), _addr(row_pos), M, _addr(k), _addr(v), int(dtype), ldk or wk, ldv or wv, _addr(stream)))
             return None
         seq, pos = self._rows(row_seq, row_pos, np.asarray(row_seq).size)
         ko, vo = _rows_out((seq.size, wk), dtype), _rows_out((seq.size, wv), dtype)
@@ -1131,7 +1136,7 @@ class KV8Cache:
         lib, c, wq, wo = load_library(), self.c, heads * self.c.dim, heads * self.c.vdim
         if isinstance(q, tuple):
             (qa, M), (sa, n) = q, shared or (None, 0)
-            _check(lib.hm_kv8_attn(C.byref(c), _ptr(qa), int(dtype), ldq or wq, _ptr(row_seq), _ptr(row_pos), M, heads, scale, _ptr(sa), n, _ptr(out), ldo or wo, _ptr(work), _ptr(stream)))
+            _check(lib.hm_kv8_attn(C.byref(c), _addr(qa), int(dtype), ldq or wq, _addr(row_seq), _addr(row_pos), M, heads, scale, _addr(sa), n, _addr(out), ldo or wo, _addr(work), _addr(stream)))
             return None
         qa, dtype = _rows_in(_flat(q))
         seq, pos = self._rows(row_seq, row_pos, len(qa))

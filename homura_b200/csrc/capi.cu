@@ -82,6 +82,8 @@ class Staging {
         return d;
     }
     bool staged() const { return !owned_.empty(); }
+    // Device memory that a call takes as it is: asked once, as every question costs a short call a quarter of a microsecond.
+    bool on_device(const void* p) { return is_device(p); }
     // Whether a pointer was memory of another GPU than the current one.
     bool elsewhere() const { return elsewhere_; }
     bool ok(cudaError_t e) {
@@ -1558,12 +1560,11 @@ static int kv8_rows(const char* name, const hm_kv8* cache, void* k, void* v, int
         return refuse(HM_ERR_INVALID, "misaligned pointer (pages start on 16-byte boundaries)");
     if (M == 0) return HM_OK;
     NEED_DEVICE();
-    if (!is_device_ptr(cache->pages)) return refuse(HM_ERR_INVALID, "the pages must live in device memory");
     cudaStream_t st = (cudaStream_t)stream;
     Staging sg(st);
+    if (!sg.on_device(cache->pages)) return refuse(HM_ERR_INVALID, "the pages must live in device memory");
     Kv8RowsArgs a{};
     a.pool = kv8_pool(cache, sg);
-    sg.in((const uint8_t*)cache->pages, 0);  // device memory: only looked at
     const size_t nk = span_bytes(M, cache->kv_heads * cache->dim, ldk, dtype), nv = span_bytes(M, cache->kv_heads * cache->vdim, ldv, dtype);
     a.k = write ? (void*)sg.in((const uint8_t*)k, nk) : sg.out((uint8_t*)k, nk, true);
     a.v = write ? (void*)sg.in((const uint8_t*)v, nv) : sg.out((uint8_t*)v, nv, true);
@@ -1609,14 +1610,12 @@ int hm_kv8_attn(const hm_kv8* cache, const void* q, int dtype, size_t ldq, const
     if (rows_meet(q, wq, ldq, out, wo, ldo, M, dtype)) return gfail(HM_ERR_INVALID, "hm_kv8_attn: q and out overlap");
     if (M == 0) return HM_OK;
     NEED_DEVICE();
-    if (!is_device_ptr(cache->pages) || (work && !is_device_ptr(work))) return gfail(HM_ERR_INVALID, "hm_kv8_attn: the pages and the work memory must live in device memory");
     cudaStream_t st = (cudaStream_t)stream;
     Staging sg(st);
+    if (!sg.on_device(cache->pages) || (work && !sg.on_device(work))) return gfail(HM_ERR_INVALID, "hm_kv8_attn: the pages and the work memory must live in device memory");
     const int sms = sm_count_of_current_device();
     Kv8AttnArgs a{};
     a.pool = kv8_pool(cache, sg);
-    sg.in((const uint8_t*)cache->pages, 0);  // device memory: only looked at
-    sg.in((const uint8_t*)work, 0);
     a.q = sg.in((const uint8_t*)q, span_bytes(M, wq, ldq, dtype));
     a.out = sg.out((uint8_t*)out, span_bytes(M, wo, ldo, dtype), true);
     a.ldq = ldq;

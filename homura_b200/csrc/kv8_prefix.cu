@@ -19,7 +19,8 @@
 // What bounds it: the instructions of the softmax.  256 rows of 32 heads over 4 of 64 elements: 4700 cycles for a block of 256 pairs, in which the schedulers issue in 7 of 10 (exponentials fill
 // 2050 of them, the tensor cores 730); 106 us in all, 325 TFLOP/s.  With 128 elements a block takes 7000, as the only place for keys is converted (4000)
 // between two blocks' scores: 1021 rows of 12 heads, 87 us.  Found slower there: two places for keys and one for values (109 us); a pass that finds no maximum and is done again where a
-// score exceeds its reference by too much, which a quarter of the blocks does with heavy-tailed scores; all six converting warps on keys, then on values (the 256 rows 117 us).
+// score exceeds its reference by too much, which a quarter of the blocks does with heavy-tailed scores; all six converting warps on keys, then on values (the 256 rows 117 us); a fourth warp for keys,
+// which leaves 72 registers a thread (109 us there, 86 for the 1021 rows).
 #include <algorithm>
 #include <map>
 #include <mutex>
