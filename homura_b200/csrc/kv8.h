@@ -9,6 +9,7 @@ namespace hm {
 constexpr int KV8_PAGE = 64;        // tokens per page
 constexpr int KV8_MAX_DIM = 256;    // elements of a key or a value
 constexpr int KV8_MAX_ROWS = 8192;  // rows of one attention call
+constexpr int KV8_PAIRS = 8;        // (row, head) pairs of one item of kv8_attn.cu
 
 // A page holds one block per key/value head, in two halves of 32 tokens: the 32 scales of its keys (f32) and their codes, one signed byte each, then the same of its values.
 // Codes stand in the order in which the lanes of warp-level MMAs want them:

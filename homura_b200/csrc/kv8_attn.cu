@@ -1,6 +1,6 @@
 // Softmax attention over the 8-bit paged cache:
 //   out[row, head] = sum over the positions t <= row_pos whose page exists of softmax_t(scale q . k_t) v_t,   zeros where there is no such position.
-// Page i of a row is shared[i] for i < n_shared and its sequence's page table entry behind them.  Where there is more than one item of rows, the shared pages are taken on their own
+// Page i of a row is shared[i] for i < n_shared and its sequence's page table entry behind them.  Where there is enough of both rows and shared pages, these are taken on their own
 // (kv8_prefix.cu), and what follows here begins behind them and joins both.
 //
 // kv8_stream_kernel   rows' contexts, eight (row, head) pairs of one key/value head at a time; bound by the bytes of the cache
@@ -26,7 +26,8 @@
 //   warps as leave each item a team.  64 rows of up to 500 own tokens behind a prefix: teams of 3 60 us, of 2 63, single warps 67 (all in the line: 105 when single warps took 80); limits of 8 and 16 pieces instead of
 //   12 (single warps): 72 and 71 us, and 16 pieces at the 64 sequences above 97 us, as a team's items are not shared out.
 //   all of them where there are no more than CTAs and the table has room for WHOLE pieces at most: a CTA takes an item, nothing is counted or joined.  One row of 14 heads over 2 of 64
-//   elements: 64 tokens 6.6 us against 10.8, 1024 10.1 against 14.7, 2048 14.0 against 16.0, 3000 17.7 against 16.1.
+//   elements: 64 tokens 6.6 us against 10.8, 1024 10.1 against 14.7, 2048 14.0 against 16.0, 3000 (94 pieces) 17.7 against 16.1;
+//   16 rows of 3000 tokens 18.1 against 19.0.
 // 64 sequences of 500 to 8000 tokens, 8 heads of 128: 74 us, 4.9 TB/s, three quarters of what a copy reaches; what is left is the start (7 us to the first scores) and the uneven end.  Three rows
 // of 20000 to 32768 tokens: 22 us, of which the join takes 5.
 // Slower where tried, at the 64 sequences with an even line (93 us with each of them): a range of pieces for every warp, which then has more partial items than are worth joining; whole
@@ -43,10 +44,10 @@
 namespace hm {
 namespace {
 
-constexpr int PAIRS = 8;           // of an item
+constexpr int PAIRS = KV8_PAIRS;   // of an item
 constexpr int LEAST_PIECES = 12;   // of a CTA, one for each of its warps: fewer would only leave more to be joined
 constexpr int BEGIN = 20;           // pieces that take a CTA as long as the beginning and end of an item
-constexpr int WHOLE = 64;           // pieces that a CTA takes in less time than a join takes
+constexpr int WHOLE = 80;           // pieces that a CTA takes in less time than a join takes
 constexpr int SOLO = 12;            // pieces that a warp takes alone where there are many items
 constexpr int MAX_DEPTH = 4;
 constexpr int MERGE_ROWS = 32;      // pairs' results of several warps that stand in shared memory when those of all are added up

@@ -42,6 +42,11 @@ constexpr int STREAM_WARPS = SOFT_WARPS / 2;
 constexpr int MAX_RAW = 8;              // pages in flight or being converted
 constexpr int RING = 5;                 // blocks whose scales are kept
 constexpr int MOST_BUFS = 3;            // of scores
+// Pieces of the streaming kernel (32 shared tokens, eight pairs) that take it as long as this kernel and its join.  us here / there, rows of 16 heads over 2, 100 own tokens:
+//   bf16, 64 elements     64 rows behind 32, 64, 128 pages (8192, 16384, 32768 pieces): 30/26, 32/31, 36/42;  256 rows behind 4, 8, 16 pages (4096 to 16384): 28/13, 26/33, 32/39
+//   bf16, 128 elements    36/29, 40/36, 44/51;  35/16, 33/37, 40/45
+//   f32, 64 elements      24/27, 28/34, 36/47;  24/13, 25/34, 27/42
+constexpr long LEAST_SHARED = 12288;
 constexpr int MOST_PARTS = 8;           // that are left to be joined with the rows' own pages
 constexpr size_t ROOM = 226 * 1024;
 constexpr float LOG2E = 1.4426950408889634f;
@@ -774,8 +779,11 @@ int clusters_at_once(int cluster, int sm_count) {
 Kv8Prefix kv8_prefix_plan(int kv_heads, int dim, int vdim, int bf16, int M, int heads, int n_shared, int sm_count) {
     Kv8Prefix p{};
     const long pairs = (long)M * (heads / kv_heads);
-    // wider heads do not fit tensor memory (two streams of scores and results) or shared memory; few pairs are one item of the streaming kernel anyway
-    if (n_shared < 1 || dim > 128 || vdim > 128 || pairs <= 8) return p;
+    // wider heads do not fit tensor memory (two streams of scores and results) or shared memory.  Up to 16 pairs are two items of the streaming kernel at most, which reads 2.5 TB/s of a prefix
+    // twice while its codes are converted here at 2 TB/s
+    if (n_shared < 1 || dim > 128 || vdim > 128 || pairs <= 2 * KV8_PAIRS) return p;
+    const long group = heads / kv_heads, pieces = (long)M * kv_heads * ((group + KV8_PAIRS - 1) / KV8_PAIRS) * n_shared * (KV8_PAGE / KV8_HALF);
+    if (pieces < LEAST_SHARED) return p;
     const long tiles = (pairs + TILE - 1) / TILE;
     p.paired = bf16 && tiles > 1;
     const long groups = p.paired ? (tiles + 1) / 2 : tiles, items = groups * kv_heads, blocks = (n_shared + 1) / 2;

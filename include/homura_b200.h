@@ -411,7 +411,7 @@ HM_API int hm_kv8_read(const hm_kv8* cache, const int32_t* row_seq, const int32_
  * (row_pos -1).  Rows whose sequence lies outside [0, n_seq) are left as they are; a row_pos beyond the table means its last position.
  * shared_pages [n_shared] (NULL with 0): pages that stand for the first n_shared pages of every row's sequence, whatever page_table says there; the keys and values
  * of a common prefix are then read once for all rows.  Rows of one sequence that follow one another (a portion of a prompt) share its whole table.
- * q and out have one type; their rows do not overlap.  M <= 8192, M * max_pages <= 2^29 and 2^36 / heads, heads <= 4096.  work: device memory of hm_kv8_attn_bytes, 16-byte aligned, for this call alone until it has
+ * q and out have one type; their rows do not overlap.  M <= 8192, M * max_pages <= 2^29 and 2^36 / heads, heads <= 4096.  work: device memory of hm_kv8_attn_bytes (of the same sizes), 16-byte aligned, for this call alone until it has
  * ended; needs no clearing.  NULL: the call takes its own and waits. */
 HM_API size_t hm_kv8_attn_bytes(const hm_kv8* cache, int M, int heads, int n_shared);
 HM_API int hm_kv8_attn(const hm_kv8* cache, const void* q, int dtype, size_t ldq, const int32_t* row_seq, const int32_t* row_pos, int M, int heads, float scale, const int32_t* shared_pages, int n_shared, void* out, size_t ldo, void* work,

@@ -396,3 +396,51 @@ def test_many_heads(hm, heads, kv_heads, dim, pages):
     m = Model(hm, heads, kv_heads, dim, dim, [64 * pages + 70, 64 * pages + 3], n_shared=pages)
     for shared in (False, True):
         attend(m, [0, 1, 0], [64 * pages + 69, 64 * pages + 2, 100], heads, False, shared=shared)
+
+
+@pytest.mark.parametrize("bf16", [False, True])
+@pytest.mark.parametrize("own", [0, 130])
+@pytest.mark.parametrize("heads,kv_heads,dim,vdim,pages", [(h, k, d, v, 5) for h, k, d, v in SIZES if max(d, v) <= 128] + [(8, 2, 64, 64, 130), (34, 2, 33, 100, 1), (6, 1, 128, 128, 64), (16, 8, 128, 128, 33)])
+def test_prefixes_of_enough_rows(hm, heads, kv_heads, dim, vdim, pages, own, bf16):
+    """As many rows as it takes for the shared pages to be taken on their own, and some beside: rows inside the prefix, at its end, behind it, of no sequence."""
+    items = kv_heads * -(-heads // kv_heads // 8)
+    M = min(8192, -(-12288 // (items * 2 * pages)) + 3)
+    rng = np.random.default_rng(heads + dim + pages)
+    S = 64 * pages
+    m = Model(hm, heads + dim, kv_heads, dim, vdim, [S + own, S + own // 2, S], n_shared=pages)
+    seq = rng.integers(0, 3, M)
+    pos = np.where(rng.random(M) < 0.5, np.array(m.lens)[seq] - 1, rng.integers(-1, S, M))
+    seq[1::9] = -1
+    q = m.queries(M, heads, bf16)
+    out = m.cache.attend(q, seq, pos, heads, dim**-0.5, shared=m.shared)
+    at = np.unique(np.concatenate([np.arange(4), M - 1 - np.arange(4), rng.integers(0, M, 24)]))
+    m.check(out[at], q[at], seq[at], pos[at], heads, dim**-0.5, shared=True)
+    np.testing.assert_array_equal(out, m.cache.attend(q, seq, pos, heads, dim**-0.5, shared=m.shared))
+
+
+@pytest.mark.parametrize("bf16", [False, True])
+def test_missing_pages_and_bad_vectors_in_a_prefix_of_many_rows(hm, bf16):
+    M, heads, pages = 900, 8, 9
+    m = Model(hm, 20, 2, 64, 64, [64 * pages + 30] * 2, n_shared=pages)
+    m.shared = m.shared.copy()
+    m.shared[[0, 5]] = [-1, m.n_pages]
+    seq, pos = np.arange(M) % 2, np.arange(M) * 7 % (64 * pages + 30)
+    q = m.queries(M, heads, bf16)
+    out = m.cache.attend(q, seq, pos, heads, 0.125, shared=m.shared)
+    at = np.arange(0, M, 29)
+    m.check(out[at], q[at], seq[at], pos[at], heads, 0.125, shared=True, seen=lambda i: ~np.isin(np.arange(m.lens[i]) // 64, [0, 5]))
+    one = hm.KV8Cache(2, 64, 64, m.pool.ptr, m.n_pages, m.shared[None])
+    bad = m.common[1][200].copy()
+    bad[0, 3] = np.inf
+    one.write(m.common[0][200][None].reshape(1, -1), bad.reshape(1, -1), [0], [200])  # of the first key/value head alone
+    f = m.cache.attend(q, seq, pos, heads, 0.125, shared=m.shared).reshape(M, heads, 64)
+    assert np.isnan((bf16_value(f) if bf16 else f)[pos >= 200][:, :4]).all()
+    np.testing.assert_array_equal(f[pos < 200], out.reshape(M, heads, 64)[pos < 200])
+    np.testing.assert_array_equal(f[:, 4:], out.reshape(M, heads, 64)[:, 4:])
+    queries = (bf16_value(q) if bf16 else q).copy()
+    queries[10, 64 * 5 + 1] = np.nan
+    g = m.cache.attend(bf16_bits(queries) if bf16 else queries, seq, pos, heads, 0.125, shared=m.shared).reshape(M, heads, 64)
+    assert np.isnan((bf16_value(g) if bf16 else g)[10, 5]).all()
+    keep = np.ones((M, heads), bool)
+    keep[10, 5] = False
+    np.testing.assert_array_equal(g[keep], f[keep])
