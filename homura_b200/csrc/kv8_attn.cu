@@ -22,9 +22,11 @@
 // sequences took 99, 91, 79, 75 and 77 us.  A CTA's warps take its pieces in turn, each with a ring of copies of its own; what they have of an item is added up in shared memory.  The
 // CTA writes the items that it has as a whole and leaves the rest (its first and its last) in `work`, for kv8_join_kernel.
 // Two kinds of items are no part of the line:
-//   short ones where there are many.  Adding up takes a CTA some 5 us, so that a team of 1 to 4 warps takes an item of up to SOLO pieces, before the CTA joins in with the line: as many
-//   warps as leave each item a team.  64 rows of up to 500 own tokens behind a prefix: teams of 3 60 us, of 2 63, single warps 67 (all in the line: 105 when single warps took 80); limits of 8 and 16 pieces instead of
-//   12 (single warps): 72 and 71 us, and 16 pieces at the 64 sequences above 97 us, as a team's items are not shared out.
+//   short ones where there are more than CTAs.  Adding up takes a CTA some 5 us, so that a team of 1 to 4 warps takes an item, as many warps as leave each item a team.  Where the table has
+//   room for 40 pieces per warp of a team at most, 96 in all, these are all items, and there is nothing to join; with longer ones in between it is those of up to SOLO pieces, before the CTA
+//   joins in with the line, as what a team has is not shared out.  Rows of 8 pairs over 2 heads of 128, all of one length, in teams / in the line, us: 100 rows of 500 tokens 14 / 25, 200 of 1100
+//   28 / 44, 290 of 1500 46 / 60, 400 of 2500 (80 pieces, not in teams of 2: 93) 103, 800 of 500 46 / 89, 80 of 4000 (125 pieces, teams of 4) 53 / 47; with lengths from 1 to these the
+//   teams gain as much.  The rest with SOLO: 64 rows of up to 500 own tokens behind a prefix 60 us in teams of 3, 67 by single warps; at the 64 sequences 16 pieces instead of 12 took 97 us.
 //   all of them where there are no more than CTAs and the table has room for WHOLE pieces at most: a CTA takes an item, nothing is counted or joined.  One row of 14 heads over 2 of 64
 //   elements: 64 tokens 6.6 us against 10.8, 1024 10.1 against 14.7, 2048 14.0 against 16.0, 3000 (94 pieces) 17.7 against 16.1;
 //   16 rows of 3000 tokens 18.1 against 19.0.
@@ -48,7 +50,8 @@ constexpr int PAIRS = KV8_PAIRS;   // of an item
 constexpr int LEAST_PIECES = 12;   // of a CTA, one for each of its warps: fewer would only leave more to be joined
 constexpr int BEGIN = 20;           // pieces that take a CTA as long as the beginning and end of an item
 constexpr int WHOLE = 80;           // pieces that a CTA takes in less time than a join takes
-constexpr int SOLO = 12;            // pieces that a warp takes alone where there are many items
+constexpr int SOLO = 12;            // pieces that a team takes before its CTA joins in with the line
+constexpr int TEAM_PIECES = 40, MOST_TEAM_PIECES = 96;  // pieces per warp, and of an item, up to which there is no line
 constexpr int MAX_DEPTH = 4;
 constexpr int MERGE_ROWS = 32;      // pairs' results of several warps that stand in shared memory when those of all are added up
 constexpr size_t ROOM = 222 * 1024;  // shared memory of a CTA, beside the static
@@ -993,7 +996,8 @@ cudaError_t launch_stream(const Kv8AttnArgs& a_in, int sm_count, cudaStream_t st
     a.team = 1;
     for (int t = 2; t <= 4; ++t)
         if (WARPS % t == 0 && all <= (long)ctas * (WARPS / t)) a.team = t;
-    a.solo = all >= 2 * sm_count ? SOLO : 0;
+    const long no_line = std::min(TEAM_PIECES * a.team, MOST_TEAM_PIECES);
+    a.solo = all <= ctas ? 0 : most <= no_line ? (int)no_line : SOLO;
     a.whole = all <= ctas && most <= WHOLE;
     const bool own = most > 0 || a.prefix_n == 0, cut = own && !a.whole && most > a.solo, rest = a.prefix_n > 0 && !a.direct;
     const size_t smem = bytes(depth), join_smem = sizeof(float2) * JOIN_PAIRS * ctas + 16 + sizeof(float) * JOIN_THREADS * JOIN_PAIRS * VS;

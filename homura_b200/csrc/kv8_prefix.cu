@@ -42,11 +42,12 @@ constexpr int STREAM_WARPS = SOFT_WARPS / 2;
 constexpr int MAX_RAW = 8;              // pages in flight or being converted
 constexpr int RING = 5;                 // blocks whose scales are kept
 constexpr int MOST_BUFS = 3;            // of scores
-// Pieces of the streaming kernel (32 shared tokens, eight pairs) that take it as long as this kernel and its join.  us here / there, rows of 16 heads over 2, 100 own tokens:
-//   bf16, 64 elements     64 rows behind 32, 64, 128 pages (8192, 16384, 32768 pieces): 30/26, 32/31, 36/42;  256 rows behind 4, 8, 16 pages (4096 to 16384): 28/13, 26/33, 32/39
-//   bf16, 128 elements    36/29, 40/36, 44/51;  35/16, 33/37, 40/45
-//   f32, 64 elements      24/27, 28/34, 36/47;  24/13, 25/34, 27/42
-constexpr long LEAST_SHARED = 12288;
+// Pieces of the streaming kernel (32 shared tokens, eight pairs) that take it as long as this kernel and its join.  us here / there at 16384 and 32768 pieces, 100 own
+// tokens, rows of 16 heads over 2:
+//   bf16, 64 elements     64 rows 32/31 and 36/42,  128 rows 29/26 and 36/45,  256 rows 31/22 and 33/34,  512 rows 28/28 and 31/45
+//   bf16, 128 elements    40/36 and 44/51,  38/32 and 47/54,  40/28 and 43/44,  37/36 and 40/57
+//   f32, 64 elements      28/34 and 37/47,  27/29 and 35/50,  27/25 and 31/40,  28/32 and 32/52
+constexpr long LEAST_SHARED = 24576;
 constexpr int MOST_PARTS = 8;           // that are left to be joined with the rows' own pages
 constexpr size_t ROOM = 226 * 1024;
 constexpr float LOG2E = 1.4426950408889634f;

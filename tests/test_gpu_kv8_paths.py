@@ -404,7 +404,7 @@ def test_many_heads(hm, heads, kv_heads, dim, pages):
 def test_prefixes_of_enough_rows(hm, heads, kv_heads, dim, vdim, pages, own, bf16):
     """As many rows as it takes for the shared pages to be taken on their own, and some beside: rows inside the prefix, at its end, behind it, of no sequence."""
     items = kv_heads * -(-heads // kv_heads // 8)
-    M = min(8192, -(-12288 // (items * 2 * pages)) + 3)
+    M = min(8192, -(-32768 // (items * 2 * pages)) + 3)
     rng = np.random.default_rng(heads + dim + pages)
     S = 64 * pages
     m = Model(hm, heads + dim, kv_heads, dim, vdim, [S + own, S + own // 2, S], n_shared=pages)
@@ -420,7 +420,7 @@ def test_prefixes_of_enough_rows(hm, heads, kv_heads, dim, vdim, pages, own, bf1
 
 @pytest.mark.parametrize("bf16", [False, True])
 def test_missing_pages_and_bad_vectors_in_a_prefix_of_many_rows(hm, bf16):
-    M, heads, pages = 900, 8, 9
+    M, heads, pages = 1000, 8, 9
     m = Model(hm, 20, 2, 64, 64, [64 * pages + 30] * 2, n_shared=pages)
     m.shared = m.shared.copy()
     m.shared[[0, 5]] = [-1, m.n_pages]
@@ -444,3 +444,21 @@ def test_missing_pages_and_bad_vectors_in_a_prefix_of_many_rows(hm, bf16):
     keep = np.ones((M, heads), bool)
     keep[10, 5] = False
     np.testing.assert_array_equal(g[keep], f[keep])
+
+
+@pytest.mark.parametrize("bf16", [False, True])
+@pytest.mark.parametrize("rows,width,heads,kv_heads,dim", [(75, 48, 8, 2, 64), (100, 48, 12, 2, 128), (220, 40, 8, 2, 32), (400, 20, 4, 2, 64), (150, 3, 16, 2, 256), (1000, 20, 16, 2, 64), (160, 48, 6, 1, 192)])
+def test_teams_of_warps(hm, rows, width, heads, kv_heads, dim, bf16):
+    """More items than SMs in tables that leave none for the line: teams of one to four warps, some with fewer pieces than warps, several items to a team."""
+    n = 64 * width
+    m = Model(hm, rows + dim, kv_heads, dim, dim, [n, n // 2 + 5], max_pages=width)
+    rng = np.random.default_rng(rows)
+    seq = rng.integers(0, 2, rows)
+    pos = (rng.random(rows) ** 3 * np.array(m.lens)[seq]).astype(int) - (rng.random(rows) < 0.05)
+    seq[3::13] = -1
+    q = m.queries(rows, heads, bf16)
+    out = m.cache.attend(q, seq, pos, heads, dim**-0.5)
+    at = np.unique(np.concatenate([np.arange(5), rng.integers(0, rows, 50), np.argsort(pos)[-3:]]))
+    m.check(out[at], q[at], seq[at], pos[at], heads, dim**-0.5)
+    assert (out[(seq >= 0) & (pos < 0)] == 0).all()
+    np.testing.assert_array_equal(out, m.cache.attend(q, seq, pos, heads, dim**-0.5))
