@@ -5,9 +5,10 @@
 //   O [128 pairs x vdim]      += P [128 x 128 tokens] . V    P in tensor memory, where S was; V in shared memory, element by token
 // Codes are whole numbers below 128, exact in f16.  A query row enters times a power of two (largest element 2^14 .. 2^15): a bf16 row is exact in one f16 term down to 2^-30 of
 // its largest element, an f32 row takes two terms (2^-22 of a value).  A token's key scale joins the scores, its value scale the weights: P = 2^(s - ref) * scale enters as f16 in one
-// term (2^-12 of itself) for bf16 rows, in two for f32 rows.  `ref` is a pair's reference in the units of the weights: it follows its largest score and the largest value
-// scale of the blocks so far, each with some room (2^8 and 2^2), so that O in tensor memory is hardly ever multiplied; P stays below 2^15, and a weight of 2^-30
-// of the largest still has a step.
+// term (2^-12 of itself) for bf16 rows, in two for f32 rows.  `ref` is a pair's reference in the units of P: it follows the largest s + log2(scale) of the tokens that the pair sees,
+// with some room (2^8), so that O in tensor memory is hardly ever multiplied.  What other pairs see, and values whose own weights are next to nothing, have no part in it.  P stays below
+// 2^15, and its smallest step, 2^-24, is 2^-31 of the largest product or less.  Scales count as 2^-80 at least, so that the sum of the weights, which is relative to the same reference, stays
+// finite: values below 2^-73 lose bits behind others whose weights are larger, and weights below 2^-126 of the reference are zero, which values above 2^100 bring near the largest.
 //
 // 24 warps: 0 .. 7 and 8 .. 15 turn scores into weights, two threads for every pair, a page each; 16 .. 18 make f16 of keys' codes, 19 .. 21 of values'; 22 copies pages; 23 issues the MMAs.  Two streams of
 // blocks take turns on the tensor cores, so that one's MMAs run beside the other's exponentials: the two halves of 256 pairs over the same blocks (a block's codes are then converted once
@@ -50,10 +51,11 @@ constexpr int MOST_BUFS = 3;            // of scores
 constexpr long LEAST_SHARED = 24576;
 constexpr int MOST_PARTS = 8;           // that are left to be joined with the rows' own pages
 constexpr size_t ROOM = 226 * 1024;
+constexpr uint32_t STATIC = 12288;      // of which what the kernel declares
 constexpr float LOG2E = 1.4426950408889634f;
 constexpr float SLACK = 8.f;            // how far a score may exceed its reference, as an exponent
-constexpr float VALUE_ROOM = 2.f;       // how far the reference value scale is set above the largest so far, where it moves
-constexpr float DROP = 5.f;             // weights enter as 2^(DROP - exponent of the value scale) times themselves: 2^(SLACK + DROP + 1) < 2^15
+constexpr float DROP = 7.f;             // a weight times its value scale enters as 2^DROP times what it is of the reference: 2^(SLACK + DROP) = 2^15
+constexpr float LEAST_LOG = -80.f;      // of value scales, in the reference
 
 struct Shape {
     int dp, vp, katoms, kpart, half;  // padded sizes, pieces of 64 elements of keys, bytes of a half's keys, of a half
@@ -73,7 +75,7 @@ __host__ __device__ inline Shape shape_of(int dim, int vdim, int terms, int q_ti
     s.k_tile = (uint32_t)s.katoms * BLOCK * 128;
     s.v_tile = 2u * s.vp * 128;
     // two blocks of values, then of keys, where they leave the ring three pages (a block and half of the next); then as many pages as fit
-    const uint32_t page = 2u * s.half, room = (uint32_t)ROOM - 9216 - 1024 - q_tiles * s.q_tile;
+    const uint32_t page = 2u * s.half, room = (uint32_t)ROOM - STATIC - 1024 - q_tiles * s.q_tile;
     s.vst = s.k_tile + 2 * s.v_tile + 3 * page <= room ? 2 : 1;
     s.kst = 2 * s.k_tile + s.vst * s.v_tile + 3 * page <= room ? 2 : 1;
     s.raw = (int)((room - s.kst * s.k_tile - s.vst * s.v_tile) / page);
@@ -95,11 +97,12 @@ struct Shared {
     int longest;
     alignas(16) float ks[RING][BLOCK];
     alignas(16) float vs[RING][BLOCK];
-    int ve[RING];      // exponent field of the largest value scale of a block's tokens that a row sees
+    alignas(16) float lv[RING][BLOCK];  // log2 of the value scales
     int there[RING];   // bit i: page i of the block exists
     int raw_there[MAX_RAW];
     float half[2][2][2][TILE];  // [stream][turn][page of the block][pair]: what the two threads of a pair tell one another
 };
+static_assert(sizeof(Shared) <= STATIC, "");
 
 __device__ __forceinline__ uint32_t desc_lo(uint32_t addr) { return ((addr >> 4) & 0x3FFF) | (1u << 16); }
 constexpr uint32_t DESC_HI = (1024u >> 4) | (1u << 14) | (2u << 29);  // rows of 128 bytes in groups of eight, 128-byte swizzle
@@ -387,27 +390,15 @@ __global__ void __launch_bounds__(THREADS, 1) kv8_prefix_kernel(const Kv8AttnArg
             if (!values) {
                 // scales, and what there is of the block.  What stood in their ring is five blocks old.  The keys took the place of those of block b - 2 or b - 1, whose scores are done;
                 // the products that stood in their place were done before: with three places for scores, those of block b - 5 at least
-                const int ring = b % RING, left = longest - (b0 + b) * BLOCK;
-                uint32_t top = 0;
-                int there = 0;
+                const int ring = b % RING;
                 for (int ph = cw; ph < 4; ph += CONV_WARPS) {
                     const unsigned char* from = base + g.raw_at + (size_t)slot[ph >> 1] * 2 * g.half + (size_t)(ph & 1) * g.half;
+                    const float v = reinterpret_cast<const float*>(from + g.kpart)[lane];
                     sh.ks[ring][ph * 32 + lane] = reinterpret_cast<const float*>(from)[lane];
-                    sh.vs[ring][ph * 32 + lane] = reinterpret_cast<const float*>(from + g.kpart)[lane];
+                    sh.vs[ring][ph * 32 + lane] = v;
+                    sh.lv[ring][ph * 32 + lane] = fmaxf(__log2f(v), LEAST_LOG);  // of NaN: the least
                 }
-                if (cw == 0) {
-                    for (int ph = 0; ph < 4; ++ph) {
-                        if (!sh.raw_there[slot[ph >> 1]]) continue;
-                        there |= 1 << (ph >> 1);
-                        const uint32_t v = __float_as_uint(reinterpret_cast<const float*>(base + g.raw_at + (size_t)slot[ph >> 1] * 2 * g.half + (size_t)(ph & 1) * g.half + g.kpart)[lane]);
-                        if (ph * 32 + lane < left && v < 0x7F800000u) top = max(top, v);
-                    }
-                    top = __reduce_max_sync(0xffffffffu, top);
-                    if (lane == 0) {
-                        sh.ve[ring] = (int)(top >> 23);
-                        sh.there[ring] = there;
-                    }
-                }
+                if (cw == 0 && lane == 0) sh.there[ring] = (sh.raw_there[slot[0]] ? 1 : 0) | (sh.raw_there[slot[1]] ? 2 : 0);
                 __syncwarp();
                 if (lane == 0) mb_arrive(&sh.sc_full[ring]);
             }
@@ -530,8 +521,7 @@ __global__ void __launch_bounds__(THREADS, 1) kv8_prefix_kernel(const Kv8AttnArg
             c = sh.half[stream][1][0][tid & (TILE - 1)];  // both warps that have a pair read it in front of their first barrier, behind which the place is written again
         }
         bool ok = true;
-        float ref = -INFINITY, over = -INFINITY, l = 0.f;  // the pair's largest score at the last move; the exponent that value scales are brought down from; sum of the weights of this side
-        float unit = -INFINITY;                            // reference of the weights: ref + over - DROP
+        float ref = -INFINITY, unit = -INFINITY, l = 0.f;  // the pair's largest score + log2(value scale) at the last move; ref - DROP, which weights are relative to; sum of the weights of this side
         const int mine_n = PAIRED ? n : (n + 1 - stream) / 2, t0 = 64 * side;
         int buf = stream, before = 0;           // places of the scores of task 2 i + stream, and of the stream's task in front
         uint32_t turn = 0, turn_before = 0;     // parities of the waits for them
@@ -547,8 +537,9 @@ __global__ void __launch_bounds__(THREADS, 1) kv8_prefix_kernel(const Kv8AttnArg
                 const int k = seen - c0;
                 return k <= 0 ? 0u : k >= 32 ? 0xffffffffu : (1u << k) - 1u;
             };
-            const ulonglong2 *ks2 = reinterpret_cast<const ulonglong2*>(&sh.ks[ring][t0]), *vs2 = reinterpret_cast<const ulonglong2*>(&sh.vs[ring][t0]);  // two pairs of scales
-            // ---- the largest score of both sides ----
+            const ulonglong2 *ks2 = reinterpret_cast<const ulonglong2*>(&sh.ks[ring][t0]), *vs2 = reinterpret_cast<const ulonglong2*>(&sh.vs[ring][t0]), *lv2 = reinterpret_cast<const ulonglong2*>(&sh.lv[ring][t0]);  // two pairs of scales
+            const uint64_t c2 = pair_of(c, c);
+            // ---- the largest score + log2(value scale) of both sides ----
             float top = -INFINITY;
             auto find = [&](auto mask) {
 #pragma unroll 1
@@ -559,8 +550,8 @@ __global__ void __launch_bounds__(THREADS, 1) kv8_prefix_kernel(const Kv8AttnArg
                     tmem_wait(x);
 #pragma unroll
                     for (int e = 0; e < 32; e += 4) {
-                        const ulonglong2 k = ks2[(c0 + e) >> 2];
-                        const float2 y = of_pair(mul2(pair_of(x[e], x[e + 1]), k.x)), z = of_pair(mul2(pair_of(x[e + 2], x[e + 3]), k.y));
+                        const ulonglong2 k = ks2[(c0 + e) >> 2], v = lv2[(c0 + e) >> 2];
+                        const float2 y = of_pair(fma2(mul2(pair_of(x[e], x[e + 1]), k.x), c2, v.x)), z = of_pair(fma2(mul2(pair_of(x[e + 2], x[e + 3]), k.y), c2, v.y));
                         if (decltype(mask)::value) {
                             if ((vis >> e) & 1) top = fmaxf(top, y.x);
                             if ((vis >> (e + 1)) & 1) top = fmaxf(top, y.y);
@@ -581,14 +572,9 @@ __global__ void __launch_bounds__(THREADS, 1) kv8_prefix_kernel(const Kv8AttnArg
                 break;
             }
             top = fmaxf(top, sh.half[stream][i & 1][side ^ 1][tid & (TILE - 1)]);
-            // ---- the references, which move only where they have to ----
-            if (top > -INFINITY) {
-                top *= c;
-                if (!(top <= ref + SLACK)) ref = top;
-            }
-            const float ve = (float)(max(sh.ve[ring], 27) - 127);
-            if (ve > over) over = ve + VALUE_ROOM;
-            const float now = ref + over - DROP;  // -inf while the pair has seen nothing
+            // ---- the reference, which moves only where it has to ----
+            if (top > ref + SLACK) ref = top;
+            const float now = ref - DROP;  // -inf while the pair has seen nothing
             if (i > 0 && __any_sync(0xffffffffu, now != unit)) {  // O is the product of the blocks so far, when the last of them is done
                 ok = __all_sync(0xffffffffu, mb_wait(&sh.pv_done[before], turn_before, a.err_flag, &sh.abort_flag));
                 tc_fence_after();
@@ -607,7 +593,7 @@ __global__ void __launch_bounds__(THREADS, 1) kv8_prefix_kernel(const Kv8AttnArg
             unit = now;
             // ---- scores to weights ----
             const float shift = now == -INFINITY ? 0.f : now;
-            const uint64_t c2 = pair_of(c, c), shift2 = pair_of(-shift, -shift);
+            const uint64_t shift2 = pair_of(-shift, -shift);
             uint64_t sum[2] = {0, 0};
             auto weigh = [&](auto mask) {
 #pragma unroll 1
