@@ -269,7 +269,7 @@ __device__ __forceinline__ bool team_any(int team, int threads, bool v) {
 // Parts in `work`: of CTA c its first item (0) and its last (1).
 __device__ __forceinline__ float* cta_part(const Kv8AttnArgs& a, int vp, int cta, int which) { return static_cast<float*>(a.work) + (size_t)(2 * cta + which) * part_floats(vp); }
 
-// Joins four elements of a pair (relative to 2^top, with their sum) with the parts of the prefix.
+// Joins four elements of a pair (relative to 2^top, with their sum; top is -inf where nothing was seen, so that the prefix's references alone count) with the parts of the prefix.
 __device__ __forceinline__ void add_prefix(const Kv8AttnArgs& a, int vp, int kvh, int pair, int d, float& top, float& sum, float (&v)[4]) {
     const size_t pairs = (size_t)a.M * (a.heads / a.pool.kv_heads), step = (size_t)a.pool.kv_heads * pairs * (vp + 4);
     const float* at = a.prefix + ((size_t)kvh * pairs + pair) * (vp + 4);
@@ -787,10 +787,7 @@ __global__ void __launch_bounds__(WARPS * 32, 1) kv8_stream_kernel(const Kv8Attn
                 sum = fmaf(f, s_l[w * room + pr], sum);
             }
             if (whole) {
-                if (a.prefix_n) {
-                    top = ref;  // v is relative to it
-                    add_prefix(a, sh.vp, kvh, sg.m * group + tile * PAIRS + pr, d, top, sum, v);
-                }
+                if (a.prefix_n) add_prefix(a, sh.vp, kvh, sg.m * group + tile * PAIRS + pr, d, top, sum, v);
                 const float inv = sum == 0.f ? 0.f : 1.0f / sum;
                 kv8_store2<BF16>(a, sg.m, head0 + pr, d, v[0] * inv, v[1] * inv, wide & 1);
                 kv8_store2<BF16>(a, sg.m, head0 + pr, d + 2, v[2] * inv, v[3] * inv, wide & 1);
@@ -932,7 +929,7 @@ __global__ void __launch_bounds__(JOIN_THREADS) kv8_join_kernel(const Kv8AttnArg
         }
         sum = warp_sum(sum);
         if (lane == 0) {
-            s_top[warp] = ref;
+            s_top[warp] = top;
             s_sum[warp] = sum;
         }
     }

@@ -68,6 +68,27 @@ def test_values_of_very_different_sizes(hm, dim, vdim, bf16):
     attend(m, seq, pos, heads, bf16, some(M, 3, 40), q=q, what="kv8 values of different sizes")
 
 
+# ---- what is not there, and what is not finite ----------------------------------------------------------
+
+
+@pytest.mark.parametrize("bf16", [False, True])
+@pytest.mark.parametrize("M,pages,more", [(74, 84, 40), (74, 84, 90), (100, 66, 20), (100, 66, 90)])
+def test_own_pages_that_are_not_there_behind_low_scores(hm, M, pages, more, bf16):
+    """Rows whose own pages are all missing have the prefix's average, however low its scores are: items of a CTA as a whole, cut ones, and those of teams of warps."""
+    heads, rng = 8, np.random.default_rng(more)
+    S = 64 * pages
+    m = Model(hm, M + more, 2, 64, 64, [S] * 4, n_shared=pages, max_pages=pages + more)
+    for k in m.k:
+        k[:, :, 0] = -20
+    refill(m)
+    seq, pos = np.arange(M) % 4, S + rng.integers(0, 64 * more, M)
+    pos[::9] = S - 1 - np.arange(len(pos[::9]))
+    q = (m.rng.standard_normal((M, heads * 64)) * 0.1).astype(np.float32)
+    q = pointed(m, bf16_bits(q) if bf16 else q, heads, 60.0)
+    _, out = attend(m, seq, pos, heads, bf16, some(M, 5), q=q, what="kv8 low scores")
+    assert (out != 0).any(-1).all()
+
+
 def calls(hm):
     out = []
     for seed, M, heads, dim, lens, pages, bf16 in [(1, 300, 8, 64, (100, 0, 9), 22, False), (2, 66, 8, 128, (0, 0), 110, False), (3, 600, 6, 64, (64, 1), 12, True), (4, 70, 8, 128, (500, 20), 100, True), (5, 1000, 8, 64, (0,), 16, True)]:
