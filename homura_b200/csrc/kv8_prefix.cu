@@ -538,7 +538,7 @@ __global__ void __launch_bounds__(THREADS, 1) kv8_prefix_kernel(const Kv8AttnArg
                 return k <= 0 ? 0u : k >= 32 ? 0xffffffffu : (1u << k) - 1u;
             };
             const ulonglong2 *ks2 = reinterpret_cast<const ulonglong2*>(&sh.ks[ring][t0]), *vs2 = reinterpret_cast<const ulonglong2*>(&sh.vs[ring][t0]), *lv2 = reinterpret_cast<const ulonglong2*>(&sh.lv[ring][t0]);  // two pairs of scales
-            const uint64_t c2 = pair_of(c, c);
+            const uint64_t c2 = pair_of(c, c);  // joins a key's scale first: sums times either alone may leave f32
             // ---- the largest score + log2(value scale) of both sides ----
             float top = -INFINITY;
             auto find = [&](auto mask) {
@@ -551,7 +551,7 @@ __global__ void __launch_bounds__(THREADS, 1) kv8_prefix_kernel(const Kv8AttnArg
 #pragma unroll
                     for (int e = 0; e < 32; e += 4) {
                         const ulonglong2 k = ks2[(c0 + e) >> 2], v = lv2[(c0 + e) >> 2];
-                        const float2 y = of_pair(fma2(mul2(pair_of(x[e], x[e + 1]), k.x), c2, v.x)), z = of_pair(fma2(mul2(pair_of(x[e + 2], x[e + 3]), k.y), c2, v.y));
+                        const float2 y = of_pair(fma2(pair_of(x[e], x[e + 1]), mul2(k.x, c2), v.x)), z = of_pair(fma2(pair_of(x[e + 2], x[e + 3]), mul2(k.y, c2), v.y));
                         if (decltype(mask)::value) {
                             if ((vis >> e) & 1) top = fmaxf(top, y.x);
                             if ((vis >> (e + 1)) & 1) top = fmaxf(top, y.y);
@@ -607,7 +607,7 @@ __global__ void __launch_bounds__(THREADS, 1) kv8_prefix_kernel(const Kv8AttnArg
                         const ulonglong2 k = ks2[(c0 + e) >> 2], v = vs2[(c0 + e) >> 2];
 #pragma unroll
                         for (int f = 0; f < 2; ++f) {
-                            float2 t = of_pair(fma2(mul2(pair_of(x[e + 2 * f], x[e + 2 * f + 1]), f ? k.y : k.x), c2, shift2));
+                            float2 t = of_pair(fma2(pair_of(x[e + 2 * f], x[e + 2 * f + 1]), mul2(f ? k.y : k.x, c2), shift2));
                             if (decltype(mask)::value) {
                                 if (!((vis >> (e + 2 * f)) & 1)) t.x = -INFINITY;
                                 if (!((vis >> (e + 2 * f + 1)) & 1)) t.y = -INFINITY;

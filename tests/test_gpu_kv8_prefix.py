@@ -68,6 +68,19 @@ def test_values_of_very_different_sizes(hm, dim, vdim, bf16):
     attend(m, seq, pos, heads, bf16, some(M, 3, 40), q=q, what="kv8 values of different sizes")
 
 
+@pytest.mark.parametrize("bf16", [False, True])
+@pytest.mark.parametrize("small,large", [(-110, 112), (100, -95), (60, 40)])
+def test_queries_and_keys_far_apart_in_size(hm, small, large, bf16):
+    """Sizes whose products are ordinary scores: sums of digits times codes stay within f32 when a key's scale has joined them."""
+    heads, M, pages = 8, 400, 16
+    m = Model(hm, 6, 2, 64, 64, [64 * pages], n_shared=pages)
+    m.k[0] *= np.float32(2.0**large)
+    refill(m)
+    q = (m.rng.standard_normal((M, heads * 64))).astype(np.float32) * np.float32(2.0**small)
+    scale = 0.125 * 2.0 ** -(small + large)
+    attend(m, np.zeros(M, int), 64 * pages - 1 - np.arange(M), heads, bf16, some(M, 8), scale=scale, q=bf16_bits(q) if bf16 else q, what="kv8 sizes far apart")
+
+
 # ---- what is not there, and what is not finite ----------------------------------------------------------
 
 
