@@ -203,7 +203,9 @@ __device__ __forceinline__ float from_digits(const int (&c)[PASSES][4], int e) {
 }
 constexpr float Q_MOST = 32639.f;   // two signed digits: 127 * 256 + 127
 constexpr float W_PART = 65535.f / 65536.f;
-constexpr float Q_TINY = 1.262177448353619e-29f;  // 2^-96: queries whose largest element is below count as zeros
+// Queries are brought up by less than 2^128: those whose largest element is below 2^-112 (bf16) or 2^-98 have a step of 2^-127 for it.
+constexpr float Q_LEAST = 1.925929944387236e-34f;  // 2^-112
+constexpr int Q_LEAST_EX = 29;                     // exponent field of 2^-98
 constexpr int W_LEAST = 32;         // smallest exponent field that weights are brought up from
 
 struct StreamShape {
@@ -226,16 +228,16 @@ __host__ __device__ inline StreamShape stream_shape(int dim, int vdim, int passe
     return s;
 }
 
-// A query with the largest magnitude `top` (as bits): what its elements are multiplied with to be whole numbers (f32: a power of two that brings the largest to 2^29 .. 2^30; 0: the
-// query counts as zeros), and what its scores are multiplied with.
+// A query with the largest magnitude `top` (as bits): what its elements are multiplied with to be whole numbers (f32: a power of two that brings the largest to 2^29 .. 2^30; 0: it has an
+// infinity or a NaN), and what its scores are multiplied with.
 template <bool BF16>
 __device__ __forceinline__ float query_factors(float scale, uint32_t top, float& up) {
-    const float most = __uint_as_float(top);
-    const bool some = top < 0x7F800000u && most >= Q_TINY;
-    const int ex = (int)(top >> 23);
-    up = !some ? 0.f : BF16 ? Q_MOST / most : pow2_bits(127 + 29 - (ex - 127));
-    const float down = !some ? 0.f : BF16 ? most / Q_MOST : exp2f((float)(ex - 127 - 29));
-    return top < 0x7F800000u ? scale * LOG2E * down : __uint_as_float(0x7FC00000u);
+    const bool finite = top < 0x7F800000u;
+    const float most = fmaxf(__uint_as_float(top), Q_LEAST);
+    const int ex = max((int)(top >> 23), Q_LEAST_EX);
+    up = !finite ? 0.f : BF16 ? Q_MOST / most : pow2_bits(127 + 29 - (ex - 127));
+    const float down = BF16 ? most / Q_MOST : exp2f((float)(ex - 127 - 29));
+    return finite ? scale * LOG2E * down : __uint_as_float(0x7FC00000u);
 }
 // Eight elements of a query as signed digits, the upper two first, a product 32 words of 16 bytes behind the other.
 template <bool BF16>
