@@ -271,6 +271,8 @@ __device__ __forceinline__ bool team_any(int team, int threads, bool v) {
 // Parts in `work`: of CTA c its first item (0) and its last (1).
 __device__ __forceinline__ float* cta_part(const Kv8AttnArgs& a, int vp, int cta, int which) { return static_cast<float*>(a.work) + (size_t)(2 * cta + which) * part_floats(vp); }
 
+// References of the prefix's parts are those of products of weights and value scales, so that they may be more than 2^126 apart where the sums of weights that are relative to them are not: these are
+// multiplied with the root of a factor twice.
 // Joins four elements of a pair (relative to 2^top, with their sum; top is -inf where nothing was seen, so that the prefix's references alone count) with the parts of the prefix.
 __device__ __forceinline__ void add_prefix(const Kv8AttnArgs& a, int vp, int kvh, int pair, int d, float& top, float& sum, float (&v)[4]) {
     const size_t pairs = (size_t)a.M * (a.heads / a.pool.kv_heads), step = (size_t)a.pool.kv_heads * pairs * (vp + 4);
@@ -278,17 +280,17 @@ __device__ __forceinline__ void add_prefix(const Kv8AttnArgs& a, int vp, int kvh
     float most = top;
 #pragma unroll 4
     for (int i = 0; i < a.prefix_n; ++i) most = fmaxf(most, __ldcg(at + i * step));
-    const float ref = most == -INFINITY ? 0.f : most, own = exp2f(top - ref);
-    sum *= own;
+    const float ref = most == -INFINITY ? 0.f : most, root = exp2f(0.5f * (top - ref)), own = root * root;
+    sum = sum * root * root;
 #pragma unroll
     for (int e = 0; e < 4; ++e) v[e] *= own;
 #pragma unroll 4
     for (int i = 0; i < a.prefix_n; ++i) {
         const float2 ml = __ldcg(reinterpret_cast<const float2*>(at + i * step));
         if (ml.x == -INFINITY) continue;  // nothing seen
-        const float f = exp2f(ml.x - ref);
+        const float r = exp2f(0.5f * (ml.x - ref)), f = r * r;
         const float4 x = __ldcg(reinterpret_cast<const float4*>(at + i * step + 4 + d));
-        sum = fmaf(f, ml.y, sum);
+        sum = fmaf(r * ml.y, r, sum);
         v[0] = fmaf(f, x.x, v[0]); v[1] = fmaf(f, x.y, v[1]); v[2] = fmaf(f, x.z, v[2]); v[3] = fmaf(f, x.w, v[3]);
     }
     top = most;
@@ -302,8 +304,8 @@ __device__ __forceinline__ void add_prefix_to(const Kv8AttnArgs& a, int vp, int 
     float most = top;
 #pragma unroll 4
     for (int i = 0; i < a.prefix_n; ++i) most = fmaxf(most, __ldcg(at + i * step));
-    const float ref = most == -INFINITY ? 0.f : most, own = exp2f(top - ref);
-    sum *= own;
+    const float ref = most == -INFINITY ? 0.f : most, root = exp2f(0.5f * (top - ref)), own = root * root;
+    sum = sum * root * root;
 #pragma unroll
     for (int s = 0; s < VS * 4; ++s) {
         o[s][0] *= own;
@@ -312,8 +314,8 @@ __device__ __forceinline__ void add_prefix_to(const Kv8AttnArgs& a, int vp, int 
 #pragma unroll 1
     for (int i = 0; i < a.prefix_n; ++i) {
         const float2 ml = __ldcg(reinterpret_cast<const float2*>(at + i * step));
-        const float f = ml.x == -INFINITY ? 0.f : exp2f(ml.x - ref);
-        if (ml.x != -INFINITY) sum = fmaf(f, ml.y, sum);
+        const float r = ml.x == -INFINITY ? 0.f : exp2f(0.5f * (ml.x - ref)), f = r * r;
+        if (ml.x != -INFINITY) sum = fmaf(r * ml.y, r, sum);
 #pragma unroll
         for (int s = 0; s < VS * 4; ++s) {
             if (8 * s >= vp) break;
@@ -867,9 +869,9 @@ __global__ void __launch_bounds__(JOIN_THREADS) kv8_join_kernel(const Kv8AttnArg
 #pragma unroll
                     for (int j = 0; j < JOIN_HEADS; ++j) {
                         if (ml[j].x == -INFINITY) continue;  // nothing seen
-                        const float now = fmaxf(top[j], ml[j].x), f0 = exp2f(top[j] - now), f1 = exp2f(ml[j].x - now);
+                        const float now = fmaxf(top[j], ml[j].x), r0 = exp2f(0.5f * (top[j] - now)), r1 = exp2f(0.5f * (ml[j].x - now)), f0 = r0 * r0, f1 = r1 * r1;
                         top[j] = now;
-                        sum[j] = fmaf(f1, ml[j].y, sum[j] * f0);
+                        sum[j] = fmaf(r1 * ml[j].y, r1, sum[j] * r0 * r0);
                         v[j].x = fmaf(f1, x[j].x, v[j].x * f0); v[j].y = fmaf(f1, x[j].y, v[j].y * f0); v[j].z = fmaf(f1, x[j].z, v[j].z * f0); v[j].w = fmaf(f1, x[j].w, v[j].w * f0);
                     }
                 }

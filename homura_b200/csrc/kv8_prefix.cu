@@ -578,8 +578,8 @@ __global__ void __launch_bounds__(THREADS, 1) kv8_prefix_kernel(const Kv8AttnArg
             if (i > 0 && __any_sync(0xffffffffu, now != unit)) {  // O is the product of the blocks so far, when the last of them is done
                 ok = __all_sync(0xffffffffu, mb_wait(&sh.pv_done[before], turn_before, a.err_flag, &sh.abort_flag));
                 tc_fence_after();
-                const float corr = unit == -INFINITY || now == unit ? 1.f : exp2_ftz(unit - now);
-                l *= corr;
+                const float root = unit == -INFINITY || now == unit ? 1.f : exp2_ftz(0.5f * (unit - now)), corr = root * root;
+                l = l * root * root;  // stays in range where the factor does not: its weights may belong to small values
 #pragma unroll 1
                 for (int c0 = 16 * side; c0 < g.vp; c0 += 32) {
                     uint32_t x[16];
@@ -690,9 +690,9 @@ __global__ void __launch_bounds__(THREADS, 1) kv8_prefix_kernel(const Kv8AttnArg
 #pragma unroll
             for (int k = 0; k < AT_ONCE; ++k) {
                 if (m[k] == -INFINITY) continue;  // nothing seen
-                const float now = fmaxf(top, m[k]), f0 = exp2_ftz(top - now), f1 = exp2_ftz(m[k] - now);
+                const float now = fmaxf(top, m[k]), r0 = exp2_ftz(0.5f * (top - now)), r1 = exp2_ftz(0.5f * (m[k] - now)), f0 = r0 * r0, f1 = r1 * r1;
                 top = now;
-                l = fmaf(f1, lm[k], l * f0);
+                l = fmaf(r1 * lm[k], r1, l * r0 * r0);
                 v.x = fmaf(f1, x[k].x, v.x * f0); v.y = fmaf(f1, x[k].y, v.y * f0); v.z = fmaf(f1, x[k].z, v.z * f0); v.w = fmaf(f1, x[k].w, v.w * f0);
             }
         }

@@ -81,6 +81,24 @@ def test_queries_and_keys_far_apart_in_size(hm, small, large, bf16):
     attend(m, np.zeros(M, int), 64 * pages - 1 - np.arange(M), heads, bf16, some(M, 8), scale=scale, q=bf16_bits(q) if bf16 else q, what="kv8 sizes far apart")
 
 
+@pytest.mark.parametrize("bf16", [False, True])
+@pytest.mark.parametrize("M,pages,own", [(400, 16, 0), (400, 16, 200), (66, 130, 0), (66, 130, 100), (74, 84, 3000)])
+@pytest.mark.parametrize("large", ["first", "middle", "last", "own"])
+def test_weights_that_belong_to_values_of_nothing(hm, large, M, pages, own, bf16):
+    """Some tokens have all of the weight and values of zero, others have next to no weight and values of 2^110: a sum is relative to a product, and both kinds count."""
+    heads, S = 8, 64 * pages
+    m = Model(hm, pages, 2, 64, 64, [S + own] * 2, n_shared=pages)
+    for k, v in zip(m.k, m.v):
+        k[:, :, 0], v[:] = 20, 0
+        at = {"first": slice(0, 40), "middle": slice(S // 2, S // 2 + 150), "last": slice(S - 70, S), "own": slice(S, S + own)}[large]
+        k[at, :, 0], v[at] = -10, m.rng.standard_normal(v[at].shape).astype(np.float32) * np.float32(2.0**110)
+    refill(m)
+    seq, pos = np.arange(M) % 2, S + own - 1 - np.arange(M) % 20
+    q = (m.rng.standard_normal((M, heads * 64)) * 0.1).astype(np.float32)
+    q = pointed(m, bf16_bits(q) if bf16 else q, heads, 8.0)
+    attend(m, seq, pos, heads, bf16, some(M, 9, 6), q=q, what="kv8 weights of nothing")
+
+
 # ---- what is not there, and what is not finite ----------------------------------------------------------
 
 
