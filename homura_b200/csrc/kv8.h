@@ -75,10 +75,11 @@ struct Kv8AttnArgs {
 struct Kv8Prefix {
     int paired, groups, splits, cluster;
     int parts;               // splits / cluster; 0: they are taken with the rows' own
+    size_t sums;             // floats of the sums that CTAs with many blocks keep in memory
 };
 Kv8Prefix kv8_prefix_plan(int kv_heads, int dim, int vdim, int bf16, int M, int heads, int n_shared, int sm_count);
 int kv8_prefix_most_parts(int kv_heads, int M, int heads, int n_shared, int sm_count);  // of any plan
-cudaError_t launch_kv8_prefix(const Kv8AttnArgs& a, const Kv8Prefix& p, float* parts, cudaStream_t st);
+cudaError_t launch_kv8_prefix(const Kv8AttnArgs& a, const Kv8Prefix& p, float* parts, float* sums, cudaStream_t st);
 cudaError_t launch_kv8_attn(const Kv8AttnArgs& a, int sm_count, cudaStream_t st);
 size_t kv8_attn_bytes(int kv_heads, int dim, int vdim, int M, int heads, int n_shared, int sm_count);
 

@@ -1036,13 +1036,14 @@ cudaError_t launch_typed(const Kv8AttnArgs& a, int sm_count, cudaStream_t st) {
 
 }  // namespace
 
-// `work`: parts of the line's cuts, then those of the prefix.
+// `work`: parts of the line's cuts, then those of the prefix, then its sums.
 static size_t line_floats(int vdim, int sm_count) { return 2 * (size_t)sm_count * part_floats(kv8_pad(vdim)); }
+static size_t parts_floats(int kv_heads, int vdim, int M, int heads, int n_shared, int sm_count) { return (size_t)kv8_prefix_most_parts(kv_heads, M, heads, n_shared, sm_count) * M * heads * (kv8_pad(vdim) + 4); }
 
 size_t kv8_attn_bytes(int kv_heads, int dim, int vdim, int M, int heads, int n_shared, int sm_count) {
-    const bool own = kv8_prefix_plan(kv_heads, dim, vdim, 0, M, heads, n_shared, sm_count).parts == 0;
-    const int parts = own ? 0 : kv8_prefix_most_parts(kv_heads, M, heads, n_shared, sm_count);
-    return sizeof(float) * (line_floats(vdim, sm_count) + (size_t)parts * M * heads * (kv8_pad(vdim) + 4));
+    // rows of either type
+    const Kv8Prefix p = kv8_prefix_plan(kv_heads, dim, vdim, 0, M, heads, n_shared, sm_count), q = kv8_prefix_plan(kv_heads, dim, vdim, 1, M, heads, n_shared, sm_count);
+    return sizeof(float) * (line_floats(vdim, sm_count) + (p.parts ? parts_floats(kv_heads, vdim, M, heads, n_shared, sm_count) + std::max(p.sums, q.sums) : 0));
 }
 
 cudaError_t launch_kv8_attn(const Kv8AttnArgs& a_in, int sm_count, cudaStream_t st) {
@@ -1054,7 +1055,7 @@ cudaError_t launch_kv8_attn(const Kv8AttnArgs& a_in, int sm_count, cudaStream_t 
     if (p.parts) {
         float* parts = static_cast<float*>(a.work) + line_floats(a.pool.vdim, sm_count);
         a.own_from = a.n_shared * (KV8_PAGE / KV8_HALF);
-        const cudaError_t e = launch_kv8_prefix(a, p, parts, st);
+        const cudaError_t e = launch_kv8_prefix(a, p, parts, parts + parts_floats(a.pool.kv_heads, a.pool.vdim, a.M, a.heads, a.n_shared, sm_count), st);
         if (e != cudaSuccess) return e;
         a.prefix = parts;
     }

@@ -49,6 +49,10 @@ constexpr int MOST_BUFS = 3;            // of scores
 //   bf16, 128 elements    40/36 and 44/51,  38/32 and 47/54,  40/28 and 43/44,  37/36 and 40/57
 //   f32, 64 elements      28/34 and 37/47,  27/29 and 35/50,  27/25 and 31/40,  28/32 and 32/52
 constexpr long LEAST_SHARED = 24576;
+// Blocks of a stream whose products are one sum in tensor memory.  Its steps round towards zero, and values of one sign gather that: 1024 steps (64 blocks of f32 rows, whose two terms take 16
+// steps each) 5.3e-5, 4096 of them 2.1e-4.  After 64 steps of f32 rows, 512 of bf16 rows, a thread adds what its pair has to f32 sums in `work`: 1.3e-6 at any length of f32 rows, which
+// take 3 to 8 % longer for it (256 rows of 32 heads of 64 behind 16384 tokens 144 -> 150 us, 1021 rows of 32 heads of 128 there 810 -> 879).
+__host__ __device__ constexpr int chunk_of(int terms) { return terms == 2 ? 4 : 64; }
 constexpr int MOST_PARTS = 8;           // that are left to be joined with the rows' own pages
 constexpr size_t ROOM = 226 * 1024;
 constexpr uint32_t STATIC = 12288;      // of which what the kernel declares
@@ -217,7 +221,8 @@ __device__ __forceinline__ bool both_any(int id, bool v) {
 
 // TERMS: f16 terms of queries and weights; PAIRED: the streams are two tiles of pairs over the same blocks.
 template <bool BF16, int TERMS, bool PAIRED>
-__global__ void __launch_bounds__(THREADS, 1) kv8_prefix_kernel(const Kv8AttnArgs a, int splits, int cluster, float* parts, int wide) {
+__global__ void __launch_bounds__(THREADS, 1) kv8_prefix_kernel(const Kv8AttnArgs a, int splits, int cluster, float* parts, float4* sums, int wide) {
+    constexpr int CHUNK = chunk_of(TERMS);
     extern __shared__ __align__(128) unsigned char dsm[];
     __shared__ Shared sh;
     const Shape g = shape_of(a.pool.dim, a.pool.vdim, TERMS, PAIRED ? 2 : 1);
@@ -309,7 +314,7 @@ __global__ void __launch_bounds__(THREADS, 1) kv8_prefix_kernel(const Kv8AttnArg
         uint32_t turn = 0;  // j / bufs
         for (int j = 0; j < tasks + g.bufs && ok; ++j) {
             const uint32_t d_s = tmem + (uint32_t)buf * BLOCK;
-            if (j >= g.bufs) {  // the product of that task
+            if (j >= g.bufs) {  // the product of that task; the first of a chunk begins with zeros
                 const int t = j - g.bufs, b = block_of(t), s = t & 1;
                 const uint32_t d_o = o_at0 + (uint32_t)s * o_step;
                 const int vs = b & (g.vst - 1);  // one stage or two
@@ -322,7 +327,7 @@ __global__ void __launch_bounds__(THREADS, 1) kv8_prefix_kernel(const Kv8AttnArg
                     for (int h = 0; h < TERMS; ++h)
 #pragma unroll
                         for (int k = 0; k < BLOCK / 16; ++k)
-                            mma_ts(d_o, d_s + (k >> 1) * 32 + h * 16 + (k & 1) * 8, v + (uint32_t)(k >> 2) * (g.v_tile / 32) + (k & 3) * 2, id_o, t > 1 || h > 0 || k > 0);
+                            mma_ts(d_o, d_s + (k >> 1) * 32 + h * 16 + (k & 1) * 8, v + (uint32_t)(k >> 2) * (g.v_tile / 32) + (k & 3) * 2, id_o, ((t >> 1) & (CHUNK - 1)) != 0 || h > 0 || k > 0);
                     mma_commit(&sh.pv_done[buf]);
                     if (!PAIRED || s == 1) mma_commit(&sh.v_empty[vs]);
                 }
@@ -522,6 +527,8 @@ __global__ void __launch_bounds__(THREADS, 1) kv8_prefix_kernel(const Kv8AttnArg
         }
         bool ok = true;
         float ref = -INFINITY, unit = -INFINITY, l = 0.f;  // the pair's largest score + log2(value scale) at the last move; ref - DROP, which weights are relative to; sum of the weights of this side
+        float kept = -INFINITY;  // reference of the sums in memory
+        float4* const sum_at = sums + ((size_t)(blockIdx.y * gridDim.x + blockIdx.x) * 2 + stream) * (g.vp / 4) * TILE + (tid & (TILE - 1));  // those of elements 4 i .. 4 i + 3 stand TILE i behind
         const int mine_n = PAIRED ? n : (n + 1 - stream) / 2, t0 = 64 * side;
         int buf = stream, before = 0;           // places of the scores of task 2 i + stream, and of the stream's task in front
         uint32_t turn = 0, turn_before = 0;     // parities of the waits for them
@@ -575,19 +582,38 @@ __global__ void __launch_bounds__(THREADS, 1) kv8_prefix_kernel(const Kv8AttnArg
             // ---- the reference, which moves only where it has to ----
             if (top > ref + SLACK) ref = top;
             const float now = ref - DROP;  // -inf while the pair has seen nothing
-            if (i > 0 && __any_sync(0xffffffffu, now != unit)) {  // O is the product of the blocks so far, when the last of them is done
+            const bool next_chunk = i > 0 && (i & (CHUNK - 1)) == 0;
+            if (next_chunk || (i > 0 && __any_sync(0xffffffffu, now != unit))) {  // O is the product of the blocks so far, when the last of them is done
                 ok = __all_sync(0xffffffffu, mb_wait(&sh.pv_done[before], turn_before, a.err_flag, &sh.abort_flag));
                 tc_fence_after();
                 const float root = unit == -INFINITY || now == unit ? 1.f : exp2_ftz(0.5f * (unit - now)), corr = root * root;
                 l = l * root * root;  // stays in range where the factor does not: its weights may belong to small values
+                if (next_chunk) {
+                    const float down = kept == -INFINITY || now == kept ? 1.f : exp2_ftz(kept - now);
 #pragma unroll 1
-                for (int c0 = 16 * side; c0 < g.vp; c0 += 32) {
-                    uint32_t x[16];
-                    tmem_ld16(x, o_at + c0);
-                    tmem_wait16(x);
+                    for (int c0 = 16 * side; c0 < g.vp; c0 += 32) {
+                        uint32_t x[16];
+                        tmem_ld16(x, o_at + c0);
 #pragma unroll
-                    for (int e = 0; e < 16; ++e) x[e] = __float_as_uint(__uint_as_float(x[e]) * corr);
-                    tmem_st16(o_at + c0, x);
+                        for (int e = 0; e < 16; e += 4) {
+                            float4* at = sum_at + (size_t)((c0 + e) / 4) * TILE;
+                            const float4 y = i > CHUNK ? __ldcg(at) : make_float4(0.f, 0.f, 0.f, 0.f);
+                            if (e == 0) tmem_wait16(x);
+                            __stcg(at, make_float4(fmaf(y.x, down, __uint_as_float(x[e]) * corr), fmaf(y.y, down, __uint_as_float(x[e + 1]) * corr), fmaf(y.z, down, __uint_as_float(x[e + 2]) * corr),
+                                                   fmaf(y.w, down, __uint_as_float(x[e + 3]) * corr)));
+                        }
+                    }
+                    kept = now;
+                } else {
+#pragma unroll 1
+                    for (int c0 = 16 * side; c0 < g.vp; c0 += 32) {
+                        uint32_t x[16];
+                        tmem_ld16(x, o_at + c0);
+                        tmem_wait16(x);
+#pragma unroll
+                        for (int e = 0; e < 16; ++e) x[e] = __float_as_uint(__uint_as_float(x[e]) * corr);
+                        tmem_st16(o_at + c0, x);
+                    }
                 }
             }
             unit = now;
@@ -650,6 +676,7 @@ __global__ void __launch_bounds__(THREADS, 1) kv8_prefix_kernel(const Kv8AttnArg
         sh.half[stream][mine_n & 1][side][tid & (TILE - 1)] = l;
         both_any(stream * 4 + (warp & 3), false);
         l += sh.half[stream][mine_n & 1][side ^ 1][tid & (TILE - 1)];
+        const float down = kept == -INFINITY || kept == unit ? 1.f : exp2_ftz(kept - unit);
         float* to = reinterpret_cast<float*>(base) + (size_t)(stream * TILE + (tid & (TILE - 1))) * ldo;
         if (side == 0) *reinterpret_cast<float2*>(to) = make_float2(unit == -INFINITY && l != 0.f ? 0.f : unit, l);  // a sum that is NaN is not passed over
 #pragma unroll 1
@@ -659,7 +686,14 @@ __global__ void __launch_bounds__(THREADS, 1) kv8_prefix_kernel(const Kv8AttnArg
             tmem_wait16(x);
             const bool some = ok && mine_n > 0;
 #pragma unroll
-            for (int e = 0; e < 16; e += 4) *reinterpret_cast<uint4*>(to + 4 + c0 + e) = some ? make_uint4(x[e], x[e + 1], x[e + 2], x[e + 3]) : make_uint4(0u, 0u, 0u, 0u);
+            for (int e = 0; e < 16; e += 4) {
+                float4 y = some ? make_float4(__uint_as_float(x[e]), __uint_as_float(x[e + 1]), __uint_as_float(x[e + 2]), __uint_as_float(x[e + 3])) : make_float4(0.f, 0.f, 0.f, 0.f);
+                if (some && mine_n > CHUNK) {
+                    const float4 z = __ldcg(sum_at + (size_t)((c0 + e) / 4) * TILE);
+                    y = make_float4(fmaf(z.x, down, y.x), fmaf(z.y, down, y.y), fmaf(z.z, down, y.z), fmaf(z.w, down, y.w));
+                }
+                *reinterpret_cast<float4*>(to + 4 + c0 + e) = y;
+            }
         }
     }
     __syncwarp();
@@ -713,7 +747,7 @@ __global__ void __launch_bounds__(THREADS, 1) kv8_prefix_kernel(const Kv8AttnArg
 }
 
 template <bool BF16, int TERMS, bool PAIRED>
-cudaError_t launch(const Kv8AttnArgs& a, const Kv8Prefix& p, float* parts, cudaStream_t st) {
+cudaError_t launch(const Kv8AttnArgs& a, const Kv8Prefix& p, float* parts, float* sums, cudaStream_t st) {
     const Shape g = shape_of(a.pool.dim, a.pool.vdim, TERMS, PAIRED ? 2 : 1);
     const int wide = kv8_wide(a);
     const cudaError_t e = ensure_dyn_smem(kv8_prefix_kernel<BF16, TERMS, PAIRED>, g.bytes);
@@ -729,7 +763,7 @@ cudaError_t launch(const Kv8AttnArgs& a, const Kv8Prefix& p, float* parts, cudaS
     at[0].val.clusterDim.y = at[0].val.clusterDim.z = 1;
     cfg.attrs = at;
     cfg.numAttrs = p.cluster > 1 ? 1 : 0;
-    return cudaLaunchKernelEx(&cfg, kv8_prefix_kernel<BF16, TERMS, PAIRED>, a, p.splits, p.cluster, parts, wide);
+    return cudaLaunchKernelEx(&cfg, kv8_prefix_kernel<BF16, TERMS, PAIRED>, a, p.splits, p.cluster, parts, reinterpret_cast<float4*>(sums), wide);
 }
 
 // Clusters of CTAs that have an SM each which the current device holds at the same time; asked once per size.
@@ -789,6 +823,8 @@ Kv8Prefix kv8_prefix_plan(int kv_heads, int dim, int vdim, int bf16, int M, int 
         }
     p.groups = (int)groups;
     p.parts = p.splits / p.cluster;
+    const long of_cta = (blocks + p.splits - 1) / p.splits;
+    if ((p.paired ? of_cta : (of_cta + 1) / 2) > chunk_of(bf16 ? 1 : 2)) p.sums = 2 * (size_t)TILE * kv8_pad(vdim) * items * p.splits;
     return p;
 }
 
@@ -797,9 +833,9 @@ int kv8_prefix_most_parts(int kv_heads, int M, int heads, int n_shared, int sm_c
     return (int)std::min<long>({(n_shared + 1) / 2, MOST_PARTS, std::max<long>(1, (2l * sm_count + items - 1) / items)});
 }
 
-cudaError_t launch_kv8_prefix(const Kv8AttnArgs& a, const Kv8Prefix& p, float* parts, cudaStream_t st) {
-    if (!a.bf16) return launch<false, 2, false>(a, p, parts, st);
-    return p.paired ? launch<true, 1, true>(a, p, parts, st) : launch<true, 1, false>(a, p, parts, st);
+cudaError_t launch_kv8_prefix(const Kv8AttnArgs& a, const Kv8Prefix& p, float* parts, float* sums, cudaStream_t st) {
+    if (!a.bf16) return launch<false, 2, false>(a, p, parts, sums, st);
+    return p.paired ? launch<true, 1, true>(a, p, parts, sums, st) : launch<true, 1, false>(a, p, parts, sums, st);
 }
 
 }  // namespace hm

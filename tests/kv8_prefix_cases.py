@@ -16,7 +16,8 @@ def formula(q, k, v, scale, bf16, tokens):
     To the bound of pages that are not shared:  scores of shared ones have a query's f16 terms (2^-22 of a value, bf16 rows exactly; no step below 2^-38 of the row's largest) and a chain of at
     most 16 truncating sums of 2^-23: 2^-18.9 of the terms' magnitudes.  A weight times its value's scale has two f16 terms (2^-22 of itself) or, in bf16 rows, one (2^-11), and no
     step below 2^-24; what it is relative to is no more than 2^-7 times the largest of these products that the row sees, so that half a step is 2^-32 of that product (times 127, of the largest
-    weight times the largest element of its value), or of 2^-80 of the largest weight where all products are below.  2^-31.5: the reference's logarithm is approximate."""
+    weight times the largest element of its value), or of 2^-80 of the largest weight where all products are below.  2^-31.5: the reference's logarithm is approximate.  The products
+    are summed in chunks of 64 (bf16 rows: 512) steps that round towards zero, 2^-23 each: 2^-17 (2^-14)."""
     want, parts = kc.attention(q, k, v, scale)
     tol = kc.bound(want, parts, bf16)
     if tokens == 0 or len(k) == 0:
@@ -29,6 +30,7 @@ def formula(q, k, v, scale, bf16, tokens):
         p = np.exp(s - s.max())
         peak[h] = (p / p.sum() * np.abs(v[:, h // group]).max(-1)).max()
     e = 2 * (terms * 2.0**-18.9 + full * 2.0**-38)[:, None] + 2.0**-18
+    e = e + (2.0**-14 if bf16 else 2.0**-17)
     return want, tol + mag * e + (tokens * (2.0**-31.5 * peak + 2.0**-105))[:, None] + (mag * 2.0**-11 if bf16 else 0)
 
 
@@ -99,7 +101,7 @@ class OnDevice:
                           ldq=self.ldq, out=at(self.ob), ldo=self.ldo, work=(self.work if work is None else work).data_ptr(), stream=None if stream is None else stream.cuda_stream)
 
     def parts(self):
-        """How many parts of the shared pages the call has left in the work memory that was full of ones."""
+        """How many parts of the shared pages a call whose CTAs have few blocks has left in the work memory that was full of ones."""
         x = self.work.cpu().numpy()
         step = self.M * self.heads * ((self.m.vdim + 31) // 32 * 32 + 4) * 4
         assert (x[self.size :] == 255).all()

@@ -99,6 +99,22 @@ def test_weights_that_belong_to_values_of_nothing(hm, large, M, pages, own, bf16
     attend(m, seq, pos, heads, bf16, some(M, 9, 6), q=q, what="kv8 weights of nothing")
 
 
+@pytest.mark.parametrize("bf16,M,heads,dim,pages", [(False, 300, 8, 64, 256), (False, 2000, 8, 64, 256), (False, 1500, 6, 128, 200), (False, 260, 8, 96, 81), (True, 5000, 8, 64, 270), (True, 2600, 16, 128, 140)])
+def test_values_of_one_sign(hm, bf16, M, heads, dim, pages):
+    """Sums in tensor memory round towards zero at every step: long ones would lose all of that."""
+    m = Model(hm, M, 2, dim, dim, [64 * pages, 64 * pages - 70], n_shared=pages)
+    for v in m.v:
+        v *= np.float32(0.1)
+        v += 1
+    refill(m)
+    q = m.queries(M, heads, False) * np.float32(0.2)
+    seq = np.arange(M) % 2
+    pos = np.array(m.lens)[seq] - 1
+    pos[3::4] -= 1000
+    rows = np.array([0, 1, 3, M // 2, M - 2, M - 1])
+    attend(m, seq, pos, heads, bf16, rows, q=bf16_bits(q) if bf16 else q, what="kv8 values of one sign")
+
+
 # ---- what is not there, and what is not finite ----------------------------------------------------------
 
 
