@@ -74,6 +74,20 @@ class Staging {
         outs_.push_back({p, d, count * sizeof(T)});
         return static_cast<T*>(d);
     }
+    // Rows of `width` bytes, `pitch` apart: what stands between them may be another output's and is not copied back.
+    uint8_t* out_rows(uint8_t* p, int rows, size_t width, size_t pitch) {
+        if (!p || is_device(p)) return p;
+        const size_t bytes = (size_t)(rows - 1) * pitch + width;
+        void* d = nullptr;
+        if (!ok(cudaMalloc(&d, std::max<size_t>(bytes, 16)))) return nullptr;
+        owned_.push_back(d);
+        ok(cudaMemcpyAsync(d, p, bytes, cudaMemcpyHostToDevice, st_));
+        if (pitch == width || rows == 1) outs_.push_back({p, d, bytes});
+        else if (pitch < (size_t)1 << 31) outs_.push_back({p, d, width, rows, pitch});  // the longest pitch that one copy takes
+        else
+            for (int r = 0; r < rows; ++r) outs_.push_back({p + r * pitch, static_cast<uint8_t*>(d) + r * pitch, width});
+        return static_cast<uint8_t*>(d);
+    }
     void* scratch(size_t bytes, bool zero) {
         void* d = nullptr;
         if (!ok(cudaMalloc(&d, std::max<size_t>(bytes, 16)))) return nullptr;
@@ -94,7 +108,8 @@ class Staging {
     int finish(cudaError_t launch_err) {
         ok(launch_err);
         if (err_ == cudaSuccess)
-            for (auto& o : outs_) ok(cudaMemcpyAsync(o.host, o.dev, o.bytes, cudaMemcpyDeviceToHost, st_));
+            for (auto& o : outs_)
+                ok(o.rows == 1 ? cudaMemcpyAsync(o.host, o.dev, o.bytes, cudaMemcpyDeviceToHost, st_) : cudaMemcpy2DAsync(o.host, o.pitch, o.dev, o.pitch, o.bytes, o.rows, cudaMemcpyDeviceToHost, st_));
         if (!owned_.empty()) ok(cudaStreamSynchronize(st_));
         if (err_ != cudaSuccess) return gfail(HM_ERR_CUDA, std::string("CUDA error: ") + cudaGetErrorString(err_));
         return HM_OK;
@@ -104,7 +119,9 @@ class Staging {
     struct Out {
         void* host;
         void* dev;
-        size_t bytes;
+        size_t bytes;  // of a row
+        int rows = 1;
+        size_t pitch = 0;
     };
     bool is_device(const void* p) {
         cudaPointerAttributes at;
@@ -1558,6 +1575,7 @@ static int kv8_rows(const char* name, const hm_kv8* cache, void* k, void* v, int
     if (!is_row_dtype(dtype)) return refuse(HM_ERR_UNSUPPORTED, "rows are HM_F32 or HM_BF16");
     if (misaligned(cache->pages, 16) || misaligned(cache->page_table, 4) || misaligned(k, row_bytes(dtype)) || misaligned(v, row_bytes(dtype)) || misaligned(row_seq, 4) || misaligned(row_pos, 4))
         return refuse(HM_ERR_INVALID, "misaligned pointer (pages start on 16-byte boundaries)");
+    if (!write && rows_meet(k, (size_t)cache->kv_heads * cache->dim, ldk, v, (size_t)cache->kv_heads * cache->vdim, ldv, M, dtype)) return refuse(HM_ERR_INVALID, "k and v overlap");
     if (M == 0) return HM_OK;
     NEED_DEVICE();
     cudaStream_t st = (cudaStream_t)stream;
@@ -1565,9 +1583,10 @@ static int kv8_rows(const char* name, const hm_kv8* cache, void* k, void* v, int
     if (!sg.on_device(cache->pages)) return refuse(HM_ERR_INVALID, "the pages must live in device memory");
     Kv8RowsArgs a{};
     a.pool = kv8_pool(cache, sg);
-    const size_t nk = span_bytes(M, cache->kv_heads * cache->dim, ldk, dtype), nv = span_bytes(M, cache->kv_heads * cache->vdim, ldv, dtype);
-    a.k = write ? (void*)sg.in((const uint8_t*)k, nk) : sg.out((uint8_t*)k, nk, true);
-    a.v = write ? (void*)sg.in((const uint8_t*)v, nv) : sg.out((uint8_t*)v, nv, true);
+    const int wk = cache->kv_heads * cache->dim, wv = cache->kv_heads * cache->vdim;
+    const size_t size = row_bytes(dtype);
+    a.k = write ? (void*)sg.in((const uint8_t*)k, span_bytes(M, wk, ldk, dtype)) : sg.out_rows((uint8_t*)k, M, wk * size, ldk * size);
+    a.v = write ? (void*)sg.in((const uint8_t*)v, span_bytes(M, wv, ldv, dtype)) : sg.out_rows((uint8_t*)v, M, wv * size, ldv * size);
     a.ldk = ldk;
     a.ldv = ldv;
     a.bf16 = dtype == HM_BF16;

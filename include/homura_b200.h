@@ -405,7 +405,8 @@ HM_API size_t hm_kv8_pool_bytes(int kv_heads, int dim, int vdim, int n_pages);
 /* Quantises row m's keys k [M, kv_heads, dim] and values v [M, kv_heads, vdim] into position row_pos[m] of sequence row_seq[m].  Rows without a place are not written;
  * of two rows with one place either may stay, or parts of both. */
 HM_API int hm_kv8_write(const hm_kv8* cache, const void* k, const void* v, int dtype, size_t ldk, size_t ldv, const int32_t* row_seq, const int32_t* row_pos, int M, void* stream);
-/* The values that the cache holds at those places (code * scale, HM_BF16 rounded once).  Rows without a place are left as they are. */
+/* The values that the cache holds at those places (code * scale, HM_BF16 rounded once).  Rows without a place are left as they are.  Rows of k and v may
+ * stand beside one another in one buffer (ldk = ldv); those that overlap are refused. */
 HM_API int hm_kv8_read(const hm_kv8* cache, const int32_t* row_seq, const int32_t* row_pos, int M, void* k, void* v, int dtype, size_t ldk, size_t ldv, void* stream);
 /* out [M, heads, vdim] = softmax(scale q . k) v of q [M, heads, dim] over the positions 0 .. row_pos[m] of sequence row_seq[m] that have a place; zeros where there are none
  * (row_pos -1).  Rows whose sequence lies outside [0, n_seq) are left as they are; a row_pos beyond the table means its last position.

@@ -31,3 +31,34 @@ def test_queries_and_keys_far_apart_in_size(hm, rows, width, small, large, bf16)
         # beside the bound of ordinary queries: a query's elements have no step below 2^-127, and its factor, about 2^-127 too, none below 2^-149: 2^-20 of a score
         off = 2 * (scale * np.abs(k).sum(-1).max() * 2.0**-128 + parts[1] * 2.0**-20)[:, None]
         assert (np.abs(o[r].reshape(heads, 64) - want) <= kc.bound(want, parts, bf16) + parts[0] * off).all(), r
+
+
+@pytest.mark.parametrize("bf16", [False, True])
+@pytest.mark.parametrize("values_first", [False, True])
+@pytest.mark.parametrize("on_device", [False, True])
+def test_keys_and_values_read_into_one_buffer(hm, on_device, values_first, bf16):
+    """Rows of keys beside rows of values: each call brings both, and leaves what stands between and the rows without a place."""
+    import ctypes as C
+
+    import torch
+
+    kvh, dim, vdim, M = 2, 40, 24, 9
+    m = Model(hm, 3, kvh, dim, vdim, [M])
+    wk, wv, pad = kvh * dim, kvh * vdim, 3
+    ld = wk + wv + pad
+    seq, pos = np.zeros(M, np.int32), np.arange(M, dtype=np.int32)
+    seq[4] = -1
+    buf = torch.full((M, ld), 5, dtype=torch.uint16 if bf16 else torch.float32, device="cuda" if on_device else "cpu")
+    k_at, v_at = (wv, 0) if values_first else (0, wk)
+    at = lambda i: C.c_void_p(buf.data_ptr() + i * buf.element_size())
+    host = lambda x: C.c_void_p(x.ctypes.data)
+    rc = hm.load_library().hm_kv8_read(C.byref(m.cache.c), host(seq), host(pos), M, at(k_at), at(v_at), 1 if bf16 else 0, ld, ld, None)
+    torch.cuda.synchronize()
+    assert rc == 0
+    got = buf.cpu().numpy()
+    for i, w, x in ((k_at, wk, m.k[0]), (v_at, wv, m.v[0])):
+        want = kc.held(x).reshape(M, w)
+        want = bf16_bits(want) if bf16 else want
+        want[4] = 5
+        np.testing.assert_array_equal(got[:, i : i + w], want)
+    assert (got[:, wk + wv :] == 5).all()

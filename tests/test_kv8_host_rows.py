@@ -1,0 +1,22 @@
+"""Rows of the 8-bit cache's host forms and refusals that need no GPU."""
+import ctypes as C
+
+import numpy as np
+import pytest
+
+INV = 1
+
+
+def test_keys_and_values_that_overlap_are_not_read(hm):
+    raw = np.zeros(1 << 16, np.uint8)
+    base = raw.ctypes.data + -raw.ctypes.data % 16
+    c = hm.HmKv8(base, base + 4096, 4, 2, 2, 2, 64, 32)  # keys 128 wide, values 64
+    lib = hm.load_library()
+    read = lambda k, v, ldk, ldv, M=3: lib.hm_kv8_read(C.byref(c), C.c_void_p(base + 32768), C.c_void_p(base + 36864), M, C.c_void_p(k), C.c_void_p(v), 0, ldk, ldv, None)
+    at = base + 8192
+    for k, v, ldk, ldv in [(at, at, 192, 192), (at, at + 508, 192, 192), (at + 4, at, 192, 192), (at, at + 256, 128, 64), (at, at + 3 * 512 - 4, 128, 64), (at, at + 512, 192, 193)]:
+        assert read(k, v, ldk, ldv) == INV, (k - at, v - at, ldk, ldv)
+    if not hm.device_count():
+        for k, v, ldk, ldv in [(at, at + 512, 192, 192), (at + 256, at, 192, 192), (at, at + 3 * 512, 128, 64)]:
+            assert read(k, v, ldk, ldv) == hm.HM_ERR_CUDA, (k - at, v - at, ldk, ldv)
+    assert read(at, at, 192, 192, M=0) == 0
