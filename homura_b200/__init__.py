@@ -776,6 +776,15 @@ def _ids_in(ids) -> np.ndarray:
     return np.ascontiguousarray(ids)
 
 
+def _places_in(x) -> np.ndarray:
+    """Sequences, positions or pages as int32.  Those beyond 32 bits stay out of range, below or above, instead of becoming what is left of their bits."""
+    x = np.asarray(x)
+    if x.dtype != np.int32:
+        x = np.minimum(x, 2**31 - 1).astype(np.int64) if x.dtype.kind == "u" else x.astype(np.float64) if x.dtype.kind == "f" else x
+        x = np.where(x > 2**31 - 1, 2**31 - 1, np.where(x >= -(2**31), x, -1)).astype(np.int32)
+    return np.ascontiguousarray(x)
+
+
 def _rows_out(shape, dtype) -> np.ndarray:
     return np.zeros(shape, np.uint16 if dtype == DType.BF16 else np.float32)
 
@@ -1065,9 +1074,12 @@ def rope(x, heads: int, dim: int, turns, pos, rot: Optional[int] = None, neighbo
         return None
     xa, dtype = _rows_in(_flat(x))
     M = xa.shape[0]
-    turns, pos = np.ascontiguousarray(turns, dtype=np.float64), np.ascontiguousarray(pos, dtype=np.int32)
+    turns, pos = np.ascontiguousarray(turns, dtype=np.float64), np.asarray(pos)
     if xa.shape[1] != heads * dim or turns.size != rot // 2 or pos.size != M:
         raise HomuraError(HM_ERR_INVALID, "rows are heads * dim elements, turns rot / 2, positions one per row")
+    if not ((pos >= -(2**31)) & (pos <= 2**31 - 1)).all():
+        raise HomuraError(HM_ERR_INVALID, "positions are whole numbers of 32 bits")
+    pos = np.ascontiguousarray(pos, dtype=np.int32)
     o = _rows_out(xa.shape, dtype)
     _check(lib.hm_rope(_ptr(xa), int(dtype), heads * dim, M, heads, dim, rot, int(neighbours), _ptr(pos), _ptr(turns), magnitude, _ptr(o), heads * dim, None))
     return o
@@ -1089,14 +1101,14 @@ class KV8Cache:
             raise HomuraError(HM_ERR_INVALID, "a cache has 1 to 1024 heads, keys and values of 1 to 256 elements, and pages")
         self._own = DeviceBuffer(size) if pages is None else None
         if not isinstance(page_table, tuple):
-            table = np.array(page_table, dtype=np.int32, ndmin=2)  # a copy of its own
+            table = np.array(_places_in(page_table), ndmin=2)  # a copy of its own
             page_table = (table.ctypes.data, *table.shape)
             self._table = table
         at, n_seq, max_pages = page_table
         self.c = HmKv8(self._own.ptr if pages is None else int(pages), int(at), n_pages, n_seq, max_pages, kv_heads, dim, vdim)
 
     def _rows(self, row_seq, row_pos, M):
-        seq, pos = (np.ascontiguousarray(r, dtype=np.int32) for r in (row_seq, row_pos))
+        seq, pos = _places_in(row_seq), _places_in(row_pos)
         if seq.size != M or pos.size != M:
             raise HomuraError(HM_ERR_INVALID, "a sequence and a position per row")
         return seq, pos
@@ -1142,7 +1154,7 @@ class KV8Cache:
         seq, pos = self._rows(row_seq, row_pos, len(qa))
         if qa.shape[1] != wq:
             raise HomuraError(HM_ERR_INVALID, "queries are rows [M, heads * dim]")
-        sa = np.ascontiguousarray([] if shared is None else shared, dtype=np.int32)
+        sa = _places_in([] if shared is None else shared)
         o = _rows_out((len(qa), wo), dtype)
         _check(lib.hm_kv8_attn(C.byref(c), _ptr(qa), int(dtype), wq, _ptr(seq), _ptr(pos), len(qa), heads, scale, _ptr(sa) if sa.size else None, sa.size, _ptr(o), wo, None, None))
         return o

@@ -62,3 +62,19 @@ def test_keys_and_values_read_into_one_buffer(hm, on_device, values_first, bf16)
         want[4] = 5
         np.testing.assert_array_equal(got[:, i : i + w], want)
     assert (got[:, wk + wv :] == 5).all()
+
+
+def test_places_beyond_32_bits(hm):
+    """Arrays of 64 bits: sequences, positions and pages beyond 32 are nobody's, behind the table, or not there."""
+    rng = np.random.default_rng(0)
+    k, v, q = (rng.standard_normal((n, 64)).astype(np.float32) for n in (64, 64, 3))
+    cache = hm.KV8Cache(1, 64, 64, None, 2, np.array([[0], [2**32 + 1]]))
+    cache.write(k, v, np.zeros(64, np.int64), np.arange(64))
+    cache.write(k[:4] + 1, v[:4], np.array([2**32, 0, 0, 1]), np.array([5, 2**32 + 6, -(2**32) + 7, 8]))  # none of them has a place
+    got, _ = cache.read(np.zeros(64, np.int64), np.arange(64))
+    np.testing.assert_array_equal(got, kc.held(k[:, None])[:, 0])
+    assert (cache.read([2**32, 0, 1], [5, 2**32 + 6, 8])[0] == 0).all()
+    out = cache.attend(q, np.array([0, 2**32, 1]), np.array([2**40, 63, 63]), 1, 0.125)
+    np.testing.assert_array_equal(out[0], cache.attend(q[:1], [0], [63], 1, 0.125)[0])
+    assert (out[1:] == 0).all()
+    np.testing.assert_array_equal(cache.attend(q[:1], [0], [63], 1, 0.125, shared=np.array([2**32])), np.zeros((1, 64), np.float32))
