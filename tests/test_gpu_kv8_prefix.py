@@ -69,6 +69,16 @@ def test_values_of_very_different_sizes(hm, dim, vdim, bf16):
 
 
 @pytest.mark.parametrize("bf16", [False, True])
+@pytest.mark.parametrize("scale", [0.0, -0.1, -1.0, 2.0])
+def test_scales_of_either_sign(hm, scale, bf16):
+    heads, M, pages = 8, 500, 13
+    m = Model(hm, 3, 2, 64, 64, [64 * pages + 50, 64 * pages], n_shared=pages)
+    seq, pos = np.arange(M) % 2, 64 * pages - 1 - np.arange(M) % 400
+    pos[::5] = np.array(m.lens)[seq[::5]] - 1
+    attend(m, seq, pos, heads, bf16, some(M, 4), scale=scale)
+
+
+@pytest.mark.parametrize("bf16", [False, True])
 @pytest.mark.parametrize("small,large", [(-110, 112), (100, -95), (60, 40)])
 def test_queries_and_keys_far_apart_in_size(hm, small, large, bf16):
     """Sizes whose products are ordinary scores: sums of digits times codes stay within f32 when a key's scale has joined them."""
@@ -136,6 +146,86 @@ def test_own_pages_that_are_not_there_behind_low_scores(hm, M, pages, more, bf16
     assert (out != 0).any(-1).all()
 
 
+@pytest.mark.parametrize("bf16", [False, True])
+@pytest.mark.parametrize("M,pages,own", [(66, 130, 0), (66, 130, 70), (100, 200, 0), (1000, 9, 0)])
+def test_queries_that_are_not_finite(hm, M, pages, own, bf16):
+    """Their own head is NaN, whether a row has pages of its own or not, and whether the shared ones are left in one part or in several."""
+    heads, S = 8, 64 * pages
+    m = Model(hm, M, 2, 64, 64, [S + own] * 2, n_shared=pages, max_pages=pages + 2)
+    seq, pos = np.arange(M) % 2, S + own - 1 - np.arange(M) % 300
+    clean = OnDevice(m, heads, seq, pos, m.queries(M, heads, bf16), 0.125)
+    clean.run()
+    x = (bf16_value(clean.q) if bf16 else clean.q).copy().reshape(M, heads, 64)
+    hit = [(1, 4), (M - 1, 0), (M // 2, 5)]
+    for (r, h), bad in zip(hit, (np.nan, np.inf, -np.inf)):
+        x[r, h, 7 * h] = bad
+    x = x.reshape(M, -1)
+    call = OnDevice(m, heads, seq, pos, bf16_bits(x) if bf16 else x, 0.125)
+    call.run()
+    if M == 66 and not bf16:
+        assert call.parts() > 1
+    a, b = call.rows().reshape(M, heads, 64), clean.rows().reshape(M, heads, 64)
+    keep = np.ones((M, heads), bool)
+    for r, h in hit:
+        keep[r, h] = False
+    f = bf16_value(a) if bf16 else a
+    assert np.isnan(f[~keep]).all()
+    np.testing.assert_array_equal(a[keep], b[keep])
+
+
+@pytest.mark.parametrize("bf16", [False, True])
+@pytest.mark.parametrize("M,pages", [(66, 130), (300, 30)])
+def test_vectors_that_are_not_finite(hm, M, pages, bf16):
+    """All values that a row sees NaN, or one key, or one value: rows that see them are NaN, others as they were; also with scores that leave weights of nothing."""
+    heads, S = 8, 64 * pages
+    m = Model(hm, M, 2, 64, 64, [S] * 2, n_shared=pages)
+    seq, pos = np.arange(M) % 2, 63 + np.arange(M) * (S - 64) // M
+    q = m.queries(M, heads, bf16)
+    clean = m.cache.attend(q, seq, pos, heads, 0.125, shared=m.shared)
+    one = hm.KV8Cache(2, 64, 64, m.pool.ptr, m.n_pages, m.shared[None])
+    flat = lambda x: np.ascontiguousarray(x.reshape(len(x), -1))
+    for part, t in ((0, S // 2), (1, S // 2)):
+        k, v = (x[t : t + 1].copy() for x in m.common)
+        (v if part else k)[0, :, 9] = np.nan
+        one.write(flat(k), flat(v), [0], [t])
+        out = m.cache.attend(q, seq, pos, heads, 0.125, shared=m.shared)
+        f = bf16_value(out) if bf16 else out
+        assert np.isnan(f[pos >= t]).all()
+        np.testing.assert_array_equal(out[pos < t], clean[pos < t])
+        one.write(flat(m.common[0][t : t + 1]), flat(m.common[1][t : t + 1]), [0], [t])
+    # every value NaN, scores far below and far above zero
+    v = np.full_like(m.common[1], np.nan)
+    one.write(flat(m.common[0]), flat(v), np.zeros(S), np.arange(S))
+    for scale in (0.125, 30.0, -30.0):
+        f = m.cache.attend(q, seq, pos, heads, scale, shared=m.shared)
+        assert np.isnan(bf16_value(f) if bf16 else f).all()
+
+
+# ---- rows at any place ------------------------------------------------------------------------------------
+
+
+@pytest.mark.parametrize("bf16", [False, True])
+@pytest.mark.parametrize("M,pages", [(300, 22), (66, 110), (40, 180)])
+@pytest.mark.parametrize("dim,vdim,offset,pad", [(64, 64, 1, 0), (64, 64, 2, 2), (128, 128, 4, 4), (33, 31, 1, 3), (32, 48, 8, 8), (20, 6, 3, 1)])
+def test_strided_rows_at_any_address(hm, dim, vdim, offset, pad, M, pages, bf16):
+    """Results stand where they belong and nowhere else; rows of no sequence are left, rows that see nothing are zeros; work memory ends where it says."""
+    heads, kvh, S, rng = 6, 2, 64 * pages, np.random.default_rng(M + dim)
+    m = Model(hm, dim, kvh, dim, vdim, [S + 100, S + 7, S], n_shared=pages)
+    seq = rng.integers(0, 3, M)
+    pos = np.where(rng.random(M) < 0.6, np.array(m.lens)[seq] - 1, rng.integers(0, S, M))
+    seq[2::11], pos[3::13] = [-1, 3, 2**31 - 1, -(2**31)][M % 4], -1
+    call = OnDevice(m, heads, seq, pos, m.queries(M, heads, bf16), 0.2, offset, pad)
+    call.run()
+    out = call.rows()
+    call.parts()  # guard bytes
+    gone = (seq < 0) | (seq >= 3)
+    assert (out[gone] == 5).all() and (out[~gone & (pos < 0)] == 0).all()
+    call.check(some(M, 6))
+
+
+# ---- streams and graphs ---------------------------------------------------------------------------------
+
+
 def calls(hm):
     out = []
     for seed, M, heads, dim, lens, pages, bf16 in [(1, 300, 8, 64, (100, 0, 9), 22, False), (2, 66, 8, 128, (0, 0), 110, False), (3, 600, 6, 64, (64, 1), 12, True), (4, 70, 8, 128, (500, 20), 100, True), (5, 1000, 8, 64, (0,), 16, True)]:
@@ -144,3 +234,108 @@ def calls(hm):
         pos = np.array(m.lens)[seq] - 1 - (np.arange(M) % 3) * (np.arange(M) % 50)
         out.append(OnDevice(m, heads, seq, pos, m.queries(M, heads, bf16), dim**-0.5))
     return out
+
+
+def test_calls_on_two_streams(hm):
+    import torch
+
+    streams, all_ = [torch.cuda.Stream(), torch.cuda.Stream()], calls(hm)
+    for c in all_:
+        c.run()
+    torch.cuda.synchronize()
+    first = [c.ob.clone() for c in all_]
+    for c in all_:
+        c.check(some(c.M, 7, 8))
+        c.ob.fill_(5)
+        c.work.fill_(255)
+    torch.cuda.synchronize()
+    for _ in range(5):
+        for i, c in enumerate(all_):
+            c.run(streams[i % 2])
+    torch.cuda.synchronize()
+    for c, o in zip(all_, first):  # no order of arrival changes a result
+        assert torch.equal(c.ob, o)
+
+
+def test_graphs_with_one_work_memory_and_positions_that_move(hm):
+    """Captured calls, replayed one behind the other over the same work memory, with other queries and positions each time."""
+    import torch
+
+    all_ = calls(hm)
+    work = torch.empty(max(c.size for c in all_), dtype=torch.uint8, device="cuda")
+    graphs, stream = [], torch.cuda.Stream()
+    for c in all_:
+        c.run()
+    torch.cuda.synchronize()
+    for c in all_:
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g, stream=stream):
+            c.run(stream, work)
+        graphs.append(g)
+    rng = np.random.default_rng(0)
+    for turn in range(3):
+        for c in all_:
+            n = np.array(c.m.lens)[c.seq]
+            c.pos = n - 1 - (rng.random(c.M) ** 4 * (n + 1)).astype(int)
+            c.q = c.m.queries(c.M, c.heads, c.bf16)
+            c.pd.copy_(torch.from_numpy(c.pos.astype(np.int32)))
+            c.qd.copy_(torch.from_numpy(c.q))
+        work.fill_(255)
+        torch.cuda.synchronize()
+        for g in graphs:
+            g.replay()
+        torch.cuda.synchronize()
+        for c in all_:
+            c.check(some(c.M, turn, 6))
+
+
+# ---- a run of the operators together --------------------------------------------------------------------
+
+
+@pytest.mark.parametrize("bf16", [False, True])
+def test_a_prompt_in_portions(hm, bf16):
+    """Rotary positions, the write and the attention of two portions of a prompt, large enough for its pages to be taken on their own, captured once a portion; then a row behind them."""
+    import torch
+
+    heads, kvh, dim, n = 8, 2, 64, 1200
+    t, dt, size, width = (torch.uint16, hm.DType.BF16, 2, (heads + 2 * kvh) * dim) if bf16 else (torch.float32, hm.DType.F32, 4, (heads + 2 * kvh) * dim)
+    rng = np.random.default_rng(5)
+    turns, mult = hm.rope_turns(1e6, dim, "bands", factor=4.0, original=256)
+    pages = -(-(n + 1) // 64)
+    table = rng.permutation(pages).reshape(1, pages).astype(np.int32)
+    own = hm.KV8Cache(kvh, dim, dim, None, pages, table)
+    td, turns_d = torch.from_numpy(table).cuda(), torch.from_numpy(turns).cuda()
+    cache = hm.KV8Cache(kvh, dim, dim, own.c.pages, pages, (td.data_ptr(), 1, pages))
+    stream = torch.cuda.Stream()
+    x = rng.standard_normal((n + 1, width)).astype(np.float32)
+    bits = bf16_bits(x) if bf16 else x
+    x = bf16_value(bits) if bf16 else x
+    y = turned(x[:, : (heads + kvh) * dim], heads + kvh, dim, turns, np.arange(n + 1), dim, False, mult)[0].reshape(n + 1, heads + kvh, dim).astype(np.float32)
+    y = bf16_value(bf16_bits(y)) if bf16 else y
+    k, v = kc.held(y[:, heads:]).astype(np.float64), kc.held(x[:, (heads + kvh) * dim :].reshape(n + 1, kvh, dim)).astype(np.float64)
+    keep = []
+    for first, M in ((0, 700), (700, 500), (1200, 1)):
+        d, sd, pd = torch.from_numpy(bits[first : first + M]).cuda(), torch.zeros(M, dtype=torch.int32, device="cuda"), torch.arange(first, first + M, dtype=torch.int32, device="cuda")
+        out = torch.zeros(M, heads * dim, dtype=t, device="cuda")
+        work = torch.empty(cache.attend_bytes(M, heads, pages), dtype=torch.uint8, device="cuda")
+        assert M == 1 or on_their_own(cache, M, heads, pages)
+        torch.cuda.synchronize()
+        g, at = torch.cuda.CUDAGraph(), d.data_ptr()
+        with torch.cuda.graph(g, stream=stream):
+            s = stream.cuda_stream
+            hm.rope((at, M), heads + kvh, dim, turns_d.data_ptr(), pd.data_ptr(), magnitude=mult, dtype=dt, ldx=width, y=at, ldy=width, stream=s)
+            cache.write((at + heads * dim * size, M), at + (heads + kvh) * dim * size, sd.data_ptr(), pd.data_ptr(), dtype=dt, ldk=width, ldv=width, stream=s)
+            cache.attend((at, M), sd.data_ptr(), pd.data_ptr(), heads, dim**-0.5, shared=(td.data_ptr(), pages), dtype=dt, ldq=width, out=out.data_ptr(), work=work.data_ptr(), stream=s)
+        g.replay()
+        torch.cuda.synchronize()
+        keep.append((g, d, sd, pd, work))
+        o = out.cpu().numpy()
+        o = bf16_value(o) if bf16 else o
+        for r in some(M, first, 10) if M > 1 else [0]:
+            p = first + r
+            want, tol = formula(y[p, :heads].astype(np.float64), k[: p + 1], v[: p + 1], dim**-0.5, bf16, p + 1)
+            _, (mag, terms, _, _) = kc.attention(y[p, :heads].astype(np.float64), k[: p + 1], v[: p + 1], dim**-0.5)
+            # turned elements may fall on the other side of a rounding (bf16 rows: 2^-7 of a product), and codes too: a step, 1 / 127 of the largest, for every element of a key; a weight
+            # is off by twice what its score is
+            off = dim**-0.5 * np.abs(y[p, :heads]).sum(-1) * np.abs(k[: p + 1]).max() / 127 + terms * (2.0**-7 if bf16 else 2.0**-18)
+            assert (np.abs(o[r].reshape(heads, dim) - want) <= tol + mag * np.expm1(2 * off)[:, None]).all(), p
