@@ -55,11 +55,12 @@ constexpr long LEAST_SHARED = 24576;
 __host__ __device__ constexpr int chunk_of(int terms) { return terms == 2 ? 4 : 64; }
 constexpr int MOST_PARTS = 8;           // that are left to be joined with the rows' own pages
 constexpr size_t ROOM = 226 * 1024;
-constexpr uint32_t STATIC = 12288;      // of which what the kernel declares
+constexpr uint32_t STATIC = 12800;      // of which what the kernel declares
 constexpr float LOG2E = 1.4426950408889634f;
 constexpr float SLACK = 8.f;            // how far a score may exceed its reference, as an exponent
 constexpr float DROP = 7.f;             // a weight times its value scale enters as 2^DROP times what it is of the reference: 2^(SLACK + DROP) = 2^15
 constexpr float LEAST_LOG = -80.f;      // of value scales, in the reference
+constexpr float FAR = 65536.f;          // references from here on are counted from a score, as f32 would leave too little of what is added to it
 
 struct Shape {
     int dp, vp, katoms, kpart, half;  // padded sizes, pieces of 64 elements of keys, bytes of a half's keys, of a half
@@ -99,7 +100,7 @@ struct Shared {
     uint32_t tmem;
     volatile int abort_flag;
     int longest;
-    alignas(16) float ks[RING][BLOCK];
+    alignas(16) float ks[RING + 1][BLOCK];  // the last row: ones, for scores that have theirs
     alignas(16) float vs[RING][BLOCK];
     alignas(16) float lv[RING][BLOCK];  // log2 of the value scales
     int there[RING];   // bit i: page i of the block exists
@@ -230,6 +231,7 @@ __global__ void __launch_bounds__(THREADS, 1) kv8_prefix_kernel(const Kv8AttnArg
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, kvh = blockIdx.y, split = blockIdx.x % splits, tiles0 = blockIdx.x / splits * (PAIRED ? 2 : 1);
     const int group = a.heads / a.pool.kv_heads, pairs = a.M * group, ldo = g.vp + 4;
     pdl_launch_dependents();
+    if (tid < BLOCK) sh.ks[RING][tid] = 1.f;
     if (tid == 0) {
         for (int s = 0; s < g.raw; ++s) {
             mb_init(&sh.raw_full[s], 1);
@@ -528,6 +530,7 @@ __global__ void __launch_bounds__(THREADS, 1) kv8_prefix_kernel(const Kv8AttnArg
         bool ok = true;
         float ref = -INFINITY, unit = -INFINITY, l = 0.f;  // the pair's largest score + log2(value scale) at the last move; ref - DROP, which weights are relative to; sum of the weights of this side
         float kept = -INFINITY;  // reference of the sums in memory
+        float origin = 0.f;      // the score that all references are counted from
         float4* const sum_at = sums + ((size_t)(blockIdx.y * gridDim.x + blockIdx.x) * 2 + stream) * (g.vp / 4) * TILE + (tid & (TILE - 1));  // those of elements 4 i .. 4 i + 3 stand TILE i behind
         const int mine_n = PAIRED ? n : (n + 1 - stream) / 2, t0 = 64 * side;
         int buf = stream, before = 0;           // places of the scores of task 2 i + stream, and of the stream's task in front
@@ -538,17 +541,37 @@ __global__ void __launch_bounds__(THREADS, 1) kv8_prefix_kernel(const Kv8AttnArg
             ok = __all_sync(0xffffffffu, mb_wait(&sh.sc_full[ring], (b / RING) & 1, a.err_flag, &sh.abort_flag) && mb_wait(&sh.s_full[buf], turn, a.err_flag, &sh.abort_flag));
             tc_fence_after();
             const int seen = (sh.there[ring] >> side) & 1 ? len - (b0 + b) * BLOCK - t0 : 0;  // tokens of this side in front of the row's end
-            const bool masked = __any_sync(0xffffffffu, seen < 64);
+            bool special = __any_sync(0xffffffffu, seen < 64 || origin != 0.f);  // tokens to be left out, or an origin; scores are counted from theirs
             // tokens c0 .. c0 + 31 of this side that are seen, a bit for each
             auto visible = [&](int c0) -> uint32_t {
                 const int k = seen - c0;
                 return k <= 0 ? 0u : k >= 32 ? 0xffffffffu : (1u << k) - 1u;
             };
-            const ulonglong2 *ks2 = reinterpret_cast<const ulonglong2*>(&sh.ks[ring][t0]), *vs2 = reinterpret_cast<const ulonglong2*>(&sh.vs[ring][t0]), *lv2 = reinterpret_cast<const ulonglong2*>(&sh.lv[ring][t0]);  // two pairs of scales
-            const uint64_t c2 = pair_of(c, c);  // joins a key's scale first: sums times either alone may leave f32
+            const ulonglong2 *vs2 = reinterpret_cast<const ulonglong2*>(&sh.vs[ring][t0]), *lv2 = reinterpret_cast<const ulonglong2*>(&sh.lv[ring][t0]);  // two pairs of scales
+            // Where a pair of the warp has an origin, scores are put in the place of their sums, counted from there; what they are multiplied with is one from then on.
+            bool counted = false;
+            auto count = [&](float by) {
+                const float factor = counted ? 1.f : c;
+                const float* keys = &sh.ks[counted ? RING : ring][t0];
+#pragma unroll 1
+                for (int c0 = 0; c0 < 64; c0 += 16) {
+                    uint32_t x[16];
+                    tmem_ld16(x, s_at + t0 + c0);
+                    tmem_wait16(x);
+#pragma unroll
+                    for (int e = 0; e < 16; ++e) x[e] = __float_as_uint(__fsub_rn(__fmul_rn(__uint_as_float(x[e]), keys[c0 + e] * factor), by));  // rounded as scores in f32 are, so that the difference is exact
+                    tmem_st16(s_at + t0 + c0, x);
+                }
+                tmem_st_wait();
+                counted = true;
+            };
+            if (special && __any_sync(0xffffffffu, origin != 0.f)) count(origin);
             // ---- the largest score + log2(value scale) of both sides ----
-            float top = -INFINITY;
+            float top;
             auto find = [&](auto mask) {
+                const ulonglong2* ks2 = reinterpret_cast<const ulonglong2*>(&sh.ks[decltype(mask)::value && counted ? RING : ring][t0]);
+                const uint64_t c2 = decltype(mask)::value && counted ? pair_of(1.f, 1.f) : pair_of(c, c);  // joins a key's scale first: sums times either alone may leave f32
+                top = -INFINITY;
 #pragma unroll 1
                 for (int c0 = 0; c0 < 64; c0 += 32) {
                     uint32_t x[32];
@@ -558,27 +581,45 @@ __global__ void __launch_bounds__(THREADS, 1) kv8_prefix_kernel(const Kv8AttnArg
 #pragma unroll
                     for (int e = 0; e < 32; e += 4) {
                         const ulonglong2 k = ks2[(c0 + e) >> 2], v = lv2[(c0 + e) >> 2];
-                        const float2 y = of_pair(fma2(pair_of(x[e], x[e + 1]), mul2(k.x, c2), v.x)), z = of_pair(fma2(pair_of(x[e + 2], x[e + 3]), mul2(k.y, c2), v.y));
-                        if (decltype(mask)::value) {
-                            if ((vis >> e) & 1) top = fmaxf(top, y.x);
-                            if ((vis >> (e + 1)) & 1) top = fmaxf(top, y.y);
-                            if ((vis >> (e + 2)) & 1) top = fmaxf(top, z.x);
-                            if ((vis >> (e + 3)) & 1) top = fmaxf(top, z.y);
-                        } else {
-                            top = fmaxf(fmaxf(top, y.x), y.y);
-                            top = fmaxf(fmaxf(top, z.x), z.y);
+#pragma unroll
+                        for (int f = 0; f < 2; ++f) {
+                            const float2 y = of_pair(fma2(pair_of(x[e + 2 * f], x[e + 2 * f + 1]), mul2(f ? k.y : k.x, c2), f ? v.y : v.x));
+                            if (decltype(mask)::value) {
+                                if ((vis >> (e + 2 * f)) & 1) top = fmaxf(top, y.x);
+                                if ((vis >> (e + 2 * f + 1)) & 1) top = fmaxf(top, y.y);
+                            } else {
+                                top = fmaxf(fmaxf(top, y.x), y.y);
+                            }
                         }
                     }
                 }
             };
-            if (masked) find(std::true_type{});
+            auto tell = [&](int place) {  // two places in turn: the other side may be a step behind
+                sh.half[stream][place & 1][side][tid & (TILE - 1)] = top;
+                if (both_any(stream * 4 + (warp & 3), !ok)) return ok = false;
+                top = fmaxf(top, sh.half[stream][place & 1][side ^ 1][tid & (TILE - 1)]);
+                return true;
+            };
+            if (special) find(std::true_type{});
             else find(std::false_type{});
-            sh.half[stream][i & 1][side][tid & (TILE - 1)] = top;  // two places in turn: the other side may be a block behind
-            if (both_any(stream * 4 + (warp & 3), !ok)) {
-                ok = false;
-                break;
+            if (!tell(i)) break;
+            // A new reference that is far from the origin: counted from there, it is found again, twice: the second time the origin is exact, where the first sum with it was not
+            auto far = [&]() { return top > ref + SLACK && fabsf(top) >= FAR && fabsf(top) < INFINITY; };
+            if (__any_sync(0xffffffffu, far())) {
+                special = true;
+#pragma unroll 1
+                for (int again = 1; ok && again <= 2; ++again) {
+                    const float to = far() ? origin + top : origin, by = to - origin;
+                    origin = to;
+                    ref -= by;
+                    unit -= by;
+                    kept -= by;
+                    count(counted ? by : origin);
+                    find(std::true_type{});
+                    tell(i + again);
+                }
             }
-            top = fmaxf(top, sh.half[stream][i & 1][side ^ 1][tid & (TILE - 1)]);
+            if (!ok) break;
             // ---- the reference, which moves only where it has to ----
             if (top > ref + SLACK) ref = top;
             const float now = ref - DROP;  // -inf while the pair has seen nothing
@@ -622,6 +663,8 @@ __global__ void __launch_bounds__(THREADS, 1) kv8_prefix_kernel(const Kv8AttnArg
             const uint64_t shift2 = pair_of(-shift, -shift);
             uint64_t sum[2] = {0, 0};
             auto weigh = [&](auto mask) {
+                const ulonglong2* ks2 = reinterpret_cast<const ulonglong2*>(&sh.ks[decltype(mask)::value && counted ? RING : ring][t0]);
+                const uint64_t c2 = decltype(mask)::value && counted ? pair_of(1.f, 1.f) : pair_of(c, c);  // joins a key's scale first: sums times either alone may leave f32
 #pragma unroll 1
                 for (int c0 = 0; c0 < 64; c0 += 32) {
                     uint32_t x[32], p[TERMS][16];
@@ -654,7 +697,7 @@ __global__ void __launch_bounds__(THREADS, 1) kv8_prefix_kernel(const Kv8AttnArg
                     for (int h = 0; h < TERMS; ++h) tmem_st16(s_at + t0 + c0 + 16 * h, p[h]);
                 }
             };
-            if (masked) weigh(std::true_type{});
+            if (special) weigh(std::true_type{});
             else weigh(std::false_type{});
             const float2 sums = of_pair(add2(sum[0], sum[1]));
             l += sums.x + sums.y;
@@ -678,7 +721,7 @@ __global__ void __launch_bounds__(THREADS, 1) kv8_prefix_kernel(const Kv8AttnArg
         l += sh.half[stream][mine_n & 1][side ^ 1][tid & (TILE - 1)];
         const float down = kept == -INFINITY || kept == unit ? 1.f : exp2_ftz(kept - unit);
         float* to = reinterpret_cast<float*>(base) + (size_t)(stream * TILE + (tid & (TILE - 1))) * ldo;
-        if (side == 0) *reinterpret_cast<float2*>(to) = make_float2(unit == -INFINITY && l != 0.f ? 0.f : unit, l);  // a sum that is NaN is not passed over
+        if (side == 0) *reinterpret_cast<float2*>(to) = make_float2(unit == -INFINITY && l != 0.f ? 0.f : origin + unit, l);  // a sum that is NaN is not passed over
 #pragma unroll 1
         for (int c0 = 16 * side; c0 < g.vp; c0 += 32) {
             uint32_t x[16];

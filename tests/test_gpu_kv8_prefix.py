@@ -125,6 +125,37 @@ def test_values_of_one_sign(hm, bf16, M, heads, dim, pages):
     attend(m, seq, pos, heads, bf16, rows, q=bf16_bits(q) if bf16 else q, what="kv8 values of one sign")
 
 
+@pytest.mark.parametrize("bf16", [False, True])
+@pytest.mark.parametrize("size", [1e5, 1e6, 1e7, 1e8, 1e9, 1e12, 1e20])
+@pytest.mark.parametrize("M,pages,sign", [(400, 16, 1), (66, 130, 1), (400, 16, -1)])
+def test_scores_of_any_size(hm, M, pages, sign, size, bf16):
+    """Where one token's score is far above all others, by more than the scores' own roundings, the result is that token's value."""
+    heads, S = 8, 64 * pages
+    m = Model(hm, pages, 2, 64, 64, [S], n_shared=pages)
+    if sign < 0:  # all scores far below zero
+        m.k[0][:, :, 0] = -30
+    refill(m)
+    q = m.queries(M, heads, bf16)
+    q = pointed(m, q, heads, 8.0) if sign < 0 else q
+    seq, pos = np.zeros(M, int), S - 1 - np.arange(M)
+    assert on_their_own(m.cache, M, heads, pages)
+    out = m.cache.attend(q, seq, pos, heads, size, shared=m.shared)
+    x, o = (bf16_value(q), bf16_value(out)) if bf16 else (q, out)
+    k, v = kc.held(m.k[0]).astype(np.float64), kc.held(m.v[0]).astype(np.float64)
+    clear = 0
+    for r in some(M, 10):
+        for h in range(heads):
+            s = k[: pos[r] + 1, h // 4] @ x[r].astype(np.float64).reshape(heads, 64)[h]
+            terms = (np.abs(k[: pos[r] + 1, h // 4]) @ np.abs(x[r].astype(np.float64).reshape(heads, 64)[h])).max()
+            first, second = s.argmax(), np.partition(s, -2)[-2]
+            if s[first] - second < terms * 2.0**-14 + 40 / size:  # twice what a score may be off, and a weight of e^-40
+                continue
+            clear += 1
+            got, want = o[r].reshape(heads, 64)[h], v[first, h // 4]
+            assert (np.abs(got - want) <= np.abs(want) * (2.0**-7 if bf16 else 2.0**-17) + 1e-12).all(), (r, h)
+    assert clear > 50
+
+
 # ---- what is not there, and what is not finite ----------------------------------------------------------
 
 
