@@ -78,3 +78,31 @@ def test_places_beyond_32_bits(hm):
     np.testing.assert_array_equal(out[0], cache.attend(q[:1], [0], [63], 1, 0.125)[0])
     assert (out[1:] == 0).all()
     np.testing.assert_array_equal(cache.attend(q[:1], [0], [63], 1, 0.125, shared=np.array([2**32])), np.zeros((1, 64), np.float32))
+
+
+@pytest.mark.parametrize("bf16", [False, True])
+@pytest.mark.parametrize("size", [1e6, 1e9, 1e20])
+@pytest.mark.parametrize("rows,width", [(20, 8), (200, 8), (20, 100)])
+def test_scores_of_any_size(hm, rows, width, size, bf16):
+    """Where one token's score is far above all others, by more than the scores' own roundings, the result is that token's value."""
+    heads, n = 8, 500
+    m = Model(hm, rows, 2, 64, 64, [n], max_pages=width)
+    q = m.queries(rows, heads, bf16)
+    pos = n - 1 - np.arange(rows)
+    out = m.cache.attend(q, np.zeros(rows), pos, heads, size)
+    x, o = (bf16_value(q), bf16_value(out)) if bf16 else (q, out)
+    k, v = kc.held(m.k[0]).astype(np.float64), kc.held(m.v[0]).astype(np.float64)
+    clear = 0
+    for r in range(0, rows, max(1, rows // 20)):
+        for h in range(heads):
+            y = x[r].astype(np.float64).reshape(heads, 64)[h]
+            s, terms = k[: pos[r] + 1, h // 4] @ y, (np.abs(k[: pos[r] + 1, h // 4]) @ np.abs(y)).max()
+            # twice what a score may be off (bf16 queries: half of 1 / 32639 of their largest element for each), and a weight of e^-40
+            off = 2 * (terms * 2.0**-21 + (np.abs(y).max() * np.abs(k[: pos[r] + 1, h // 4]).sum(-1).max() * 2.0**-15.9 if bf16 else 0))
+            if s.max() - np.partition(s, -2)[-2] < 2 * off + 40 / size:
+                continue
+            clear += 1
+            want = v[s.argmax(), h // 4]
+            # a weight has 31 bits (bf16 rows: 16) of the largest product
+            assert (np.abs(o[r].reshape(heads, 64)[h] - want) <= np.abs(want) * (2.0**-8 + 2.0**-14 if bf16 else 2.0**-20)).all(), (r, h)
+    assert clear > 50
