@@ -5,23 +5,24 @@
 //   O [128 pairs x vdim]      += P [128 x 128 tokens] . V    P in tensor memory, where S was; V in shared memory, element by token
 // Codes are whole numbers below 128, exact in f16.  A query row enters times a power of two (largest element 2^14 .. 2^15): a bf16 row is exact in one f16 term down to 2^-30 of
 // its largest element, an f32 row takes two terms (2^-22 of a value).  A token's key scale joins the scores, its value scale the weights: P = 2^(s - ref) * scale enters as f16 in one
-// term (2^-12 of itself) for bf16 rows, in two for f32 rows.  `ref` is a pair's reference in the units of P: it follows the largest s + log2(scale) of the tokens that the pair sees,
-// with some room (2^8), so that O in tensor memory is hardly ever multiplied.  What other pairs see, and values whose own weights are next to nothing, have no part in it.  P stays below
-// 2^15, and its smallest step, 2^-24, is 2^-31 of the largest product or less.  Scales count as 2^-80 at least, so that the sum of the weights, which is relative to the same reference, stays
+// term (2^-11 of itself) for bf16 rows, in two for f32 rows.  `ref` is a pair's reference in the units of P: it follows the largest s + log2(scale) of the tokens that the pair sees,
+// with some room (2^8), so that O in tensor memory is hardly ever multiplied.  What other pairs see, and values whose own weights are next to nothing, have no part in it.  P is 2^15
+// at most, and its smallest step, 2^-24, is 2^-31 of the largest product or less.  Scales count as 2^-80 at least, so that the sum of the weights, which is relative to the same reference, stays
 // finite: values below 2^-73 lose bits behind others whose weights are larger, and weights below 2^-126 of the reference are zero, which values above 2^100 bring near the largest.
 //
 // 24 warps: 0 .. 7 and 8 .. 15 turn scores into weights, two threads for every pair, a page each; 16 .. 18 make f16 of keys' codes, 19 .. 21 of values'; 22 copies pages; 23 issues the MMAs.  Two streams of
 // blocks take turns on the tensor cores, so that one's MMAs run beside the other's exponentials: the two halves of 256 pairs over the same blocks (a block's codes are then converted once
 // for both), or, for fewer pairs and f32 rows, whose two terms leave room for one tile of queries, the even and the odd blocks of 128 pairs.  Weights stand where their scores were; where
-// two results of 64 elements leave room, a third place lets a stream's next scores come while its weights are still multiplied (256 rows of 32 heads behind 16384 tokens: 111 -> 106 us).
+// two results of 64 elements leave room, a third place lets a stream's next scores come while its weights are still multiplied (256 rows of 32 heads behind 16384 tokens: 5 us less).
 // The token axis is split where there are too few pairs for all SMs; splits form clusters that join what they have over their shared memory.  A row that has nothing but the prefix is then
 // done, where that leaves one part; others, and further parts, go to `work`, relative to their references, to be joined with the rows' own pages.
 //
-// What bounds it: the instructions of the softmax.  256 rows of 32 heads over 4 of 64 elements: 4700 cycles for a block of 256 pairs, in which the schedulers issue in 7 of 10 (exponentials fill
-// 2050 of them, the tensor cores 730); 106 us in all, 325 TFLOP/s.  With 128 elements a block takes 7000, as the only place for keys is converted (4000)
-// between two blocks' scores: 1021 rows of 12 heads, 87 us.  Found slower there: two places for keys and one for values (109 us); a pass that finds no maximum and is done again where a
-// score exceeds its reference by too much, which a quarter of the blocks does with heavy-tailed scores; all six converting warps on keys, then on values (the 256 rows 117 us); a fourth warp for keys,
-// which leaves 72 registers a thread (109 us there, 86 for the 1021 rows).
+// What bounds it: the instructions of the softmax.  256 rows of 32 heads over 4 of 64 elements: the schedulers issue in 7 of 10 cycles; exponentials fill 2050 cycles of a block of 256 pairs, the tensor
+// cores 730; 116 us in all, 296 TFLOP/s.  A block took 4700 cycles and the whole 106 us while references followed scores alone: value scales in them cost one operation for two scores and the
+// loads of their logarithms (8 us), counting from an origin a vote per block (1.5 us).  With 128 elements a block takes 7000, as the only place for keys is converted (4000)
+// between two blocks' scores: 1021 rows of 12 heads, 90 us, the schedulers issue in 6 of 10.  Found slower, against 106 and 87 us: two places for keys and one for values (109 us for the
+// 1021 rows); a pass that finds no maximum and is done again where a score exceeds its reference by too much, which a quarter of the blocks does with heavy-tailed scores; all six converting
+// warps on keys, then on values (the 256 rows 117 us); a fourth warp for keys, which leaves 72 registers a thread (109 us there, 86 for the 1021 rows).
 #include <algorithm>
 #include <map>
 #include <mutex>
@@ -43,11 +44,16 @@ constexpr int STREAM_WARPS = SOFT_WARPS / 2;
 constexpr int MAX_RAW = 8;              // pages in flight or being converted
 constexpr int RING = 5;                 // blocks whose scales are kept
 constexpr int MOST_BUFS = 3;            // of scores
-// Pieces of the streaming kernel (32 shared tokens, eight pairs) that take it as long as this kernel and its join.  us here / there at 16384 and 32768 pieces, 100 own
-// tokens, rows of 16 heads over 2:
-//   bf16, 64 elements     64 rows 32/31 and 36/42,  128 rows 29/26 and 36/45,  256 rows 31/22 and 33/34,  512 rows 28/28 and 31/45
-//   bf16, 128 elements    40/36 and 44/51,  38/32 and 47/54,  40/28 and 43/44,  37/36 and 40/57
-//   f32, 64 elements      28/34 and 37/47,  27/29 and 35/50,  27/25 and 31/40,  28/32 and 32/52
+// Pieces of the streaming kernel (32 shared tokens, eight pairs) that take it as long as this kernel and its join.  us here / there at 16384, 24576 and 32768 pieces, rows of 16 heads over 2:
+//   100 own tokens      64 rows              128 rows             256 rows             512 rows
+//   bf16,  64 elements  33/31 34/36 37/42    30/26 35/39 38/45    33/22 30/29 36/35    30/28 32/36 32/45
+//   bf16, 128 elements  41/36 42/44 45/51    40/33 45/47 49/54    42/29 40/37 45/45    39/36 42/47 42/58
+//   f32,   64 elements  29/34 34/41 38/47    29/29 31/43 36/50    28/25 30/33 32/41    29/32 31/42 33/52
+//   f32,  128 elements  38/41 43/52 49/61    38/39 42/55 47/64    36/35 39/47 43/58    37/44 40/58 43/72
+//   none
+//   bf16,  96 elements  30/34 31/41 34/48    26/29 29/39 33/50    26/24 25/32 29/40    22/28 25/39 25/49
+//   f32,   64 elements  22/33 26/40 30/47    20/28 22/38 26/49    18/23 20/31 22/39    17/27 19/37 21/47
+// One limit for all of them, where bf16 rows with tokens of their own gain but for 256 rows; f32 rows and rows without own tokens gain from fewer pieces on, at most sizes from 16384.
 constexpr long LEAST_SHARED = 24576;
 // Blocks of a stream whose products are one sum in tensor memory.  Its steps round towards zero, and values of one sign gather that: 1024 steps (64 blocks of f32 rows, whose two terms take 16
 // steps each) 5.3e-5, 4096 of them 2.1e-4.  After 64 steps of f32 rows, 512 of bf16 rows, a thread adds what its pair has to f32 sums in `work`: 1.3e-6 at any length of f32 rows, which
