@@ -206,7 +206,8 @@ constexpr float W_PART = 65535.f / 65536.f;
 // Queries are brought up by less than 2^128: those whose largest element is below 2^-112 (bf16) or 2^-98 have a step of 2^-127 for it.
 constexpr float Q_LEAST = 1.925929944387236e-34f;  // 2^-112
 constexpr int Q_LEAST_EX = 29;                     // exponent field of 2^-98
-constexpr int W_LEAST = 32;         // smallest exponent field that weights are brought up from
+// Smallest exponent field that weights are brought up from: the last digit's step stays a normal number, 2^-126 or 2^-125
+__device__ constexpr int w_least(bool bf16) { return bf16 ? 16 : 32; }
 
 struct StreamShape {
     int dp, vp, ldo, kpart, vpart, queries;  // padded sizes, row of the warps' results, bytes of a piece's keys and values, words of 16 bytes of an item's queries
@@ -648,7 +649,7 @@ __global__ void __launch_bounds__(WARPS * 32, 1) kv8_stream_kernel(const Kv8Attn
                 top = max(top, __shfl_xor_sync(0xffffffffu, top, 1));
                 top = max(top, __shfl_xor_sync(0xffffffffu, top, 2));
                 if (top >= 0x7F800000u) l = __uint_as_float(0x7FC00000u);
-                const int ex = min(max((int)(top >> 23), W_LEAST), 254);
+                const int ex = min(max((int)(top >> 23), w_least(BF16)), 254);
                 // bf16: whole numbers up to 65535, f32: below 2^31, for the largest
                 const float up = BF16 ? pow2_bits(127 + 15 - (ex - 127)) * W_PART : pow2_bits(127 + 30 - (ex - 127)), unit = exp2_ftz((float)(ex - 127 - (BF16 ? 15 : 30))) * (BF16 ? 1.f / W_PART : 1.f);
                 uint4 wa[PASSES];

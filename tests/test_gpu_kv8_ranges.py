@@ -106,3 +106,18 @@ def test_scores_of_any_size(hm, rows, width, size, bf16):
             # a weight has 31 bits (bf16 rows: 16) of the largest product
             assert (np.abs(o[r].reshape(heads, 64)[h] - want) <= np.abs(want) * (2.0**-8 + 2.0**-14 if bf16 else 2.0**-20)).all(), (r, h)
     assert clear > 50
+
+
+@pytest.mark.parametrize("bf16", [False, True])
+@pytest.mark.parametrize("small", [-60, -85, -95, -99])
+@pytest.mark.parametrize("rows,width", [(20, 8), (200, 8), (20, 100)])
+def test_values_next_to_nothing(hm, rows, width, small, bf16):
+    """The smallest values that the cache holds keep their weights' bits."""
+    heads, n = 8, 500
+    m = Model(hm, rows, 2, 64, 64, [n], max_pages=width)
+    m.v[0] = m.rng.standard_normal(m.v[0].shape).astype(np.float32) * np.float32(2.0**small)
+    m.fill()
+    q = m.queries(rows, heads, bf16)
+    pos = n - 1 - np.arange(rows)
+    out = m.cache.attend(q, np.zeros(rows), pos, heads, 0.125)
+    assert m.check(out, q, np.zeros(rows, int), pos, heads, 0.125) <= 1
