@@ -7,8 +7,8 @@
 // its largest element, an f32 row takes two terms (2^-22 of a value).  A token's key scale joins the scores, its value scale the weights: P = 2^(s - ref) * scale enters as f16 in one
 // term (2^-11 of itself) for bf16 rows, in two for f32 rows.  `ref` is a pair's reference in the units of P: it follows the largest s + log2(scale) of the tokens that the pair sees,
 // with some room (2^8), so that O in tensor memory is hardly ever multiplied.  What other pairs see, and values whose own weights are next to nothing, have no part in it.  P is 2^15
-// at most, and its smallest step, 2^-24, is 2^-31 of the largest product or less.  Scales count as 2^-80 at least, so that the sum of the weights, which is relative to the same reference, stays
-// finite: values below 2^-73 lose bits behind others whose weights are larger, and weights below 2^-126 of the reference are zero, which values above 2^100 bring near the largest.
+// at most, and its smallest step, 2^-24, is 2^-31 of the largest product or less.  Scales count as 2^-100 at least and sums of weights, which are relative to the same
+// reference, as 2^-20 of theirs, so that these stay finite.  Weights below 2^-126 of the reference are zero, which values above 2^100 bring near the largest.
 //
 // 24 warps: 0 .. 7 and 8 .. 15 turn scores into weights, two threads for every pair, a page each; 16 .. 18 make f16 of keys' codes, 19 .. 21 of values'; 22 copies pages; 23 issues the MMAs.  Two streams of
 // blocks take turns on the tensor cores, so that one's MMAs run beside the other's exponentials: the two halves of 256 pairs over the same blocks (a block's codes are then converted once
@@ -65,7 +65,9 @@ constexpr uint32_t STATIC = 12800;      // of which what the kernel declares
 constexpr float LOG2E = 1.4426950408889634f;
 constexpr float SLACK = 8.f;            // how far a score may exceed its reference, as an exponent
 constexpr float DROP = 7.f;             // a weight times its value scale enters as 2^DROP times what it is of the reference: 2^(SLACK + DROP) = 2^15
-constexpr float LEAST_LOG = -80.f;      // of value scales, in the reference
+// Of value scales, in the reference.  A weight is below 2^(100 + SLACK + DROP) then, and a sum of 64 below 2^121; those of 2^23 blocks stay finite as 2^-SUM_DROP of theirs
+constexpr float LEAST_LOG = -100.f;
+constexpr int SUM_DROP = 20;
 constexpr float FAR = 65536.f;          // references from here on are counted from a score, as f32 would leave too little of what is added to it
 
 struct Shape {
@@ -534,7 +536,7 @@ __global__ void __launch_bounds__(THREADS, 1) kv8_prefix_kernel(const Kv8AttnArg
             c = sh.half[stream][1][0][tid & (TILE - 1)];  // both warps that have a pair read it in front of their first barrier, behind which the place is written again
         }
         bool ok = true;
-        float ref = -INFINITY, unit = -INFINITY, l = 0.f;  // the pair's largest score + log2(value scale) at the last move; ref - DROP, which weights are relative to; sum of the weights of this side
+        float ref = -INFINITY, unit = -INFINITY, l = 0.f;  // the pair's largest score + log2(value scale) at the last move; ref - DROP, which weights are relative to; 2^-SUM_DROP of the sum of the weights of this side
         float kept = -INFINITY;  // reference of the sums in memory
         float origin = 0.f;      // the score that all references are counted from
         float4* const sum_at = sums + ((size_t)(blockIdx.y * gridDim.x + blockIdx.x) * 2 + stream) * (g.vp / 4) * TILE + (tid & (TILE - 1));  // those of elements 4 i .. 4 i + 3 stand TILE i behind
@@ -706,7 +708,7 @@ __global__ void __launch_bounds__(THREADS, 1) kv8_prefix_kernel(const Kv8AttnArg
             if (special) weigh(std::true_type{});
             else weigh(std::false_type{});
             const float2 sums = of_pair(add2(sum[0], sum[1]));
-            l += sums.x + sums.y;
+            l = fmaf(sums.x + sums.y, 1.f / (1 << SUM_DROP), l);
             tmem_st_wait();
             tc_fence_before();
             __syncwarp();
@@ -727,7 +729,7 @@ __global__ void __launch_bounds__(THREADS, 1) kv8_prefix_kernel(const Kv8AttnArg
         l += sh.half[stream][mine_n & 1][side ^ 1][tid & (TILE - 1)];
         const float down = kept == -INFINITY || kept == unit ? 1.f : exp2_ftz(kept - unit);
         float* to = reinterpret_cast<float*>(base) + (size_t)(stream * TILE + (tid & (TILE - 1))) * ldo;
-        if (side == 0) *reinterpret_cast<float2*>(to) = make_float2(unit == -INFINITY && l != 0.f ? 0.f : origin + unit, l);  // a sum that is NaN is not passed over
+        if (side == 0) *reinterpret_cast<float2*>(to) = make_float2(unit == -INFINITY && l != 0.f ? 0.f : origin + unit + SUM_DROP, l);  // a sum that is NaN is not passed over
 #pragma unroll 1
         for (int c0 = 16 * side; c0 < g.vp; c0 += 32) {
             uint32_t x[16];
@@ -741,7 +743,8 @@ __global__ void __launch_bounds__(THREADS, 1) kv8_prefix_kernel(const Kv8AttnArg
                     const float4 z = __ldcg(sum_at + (size_t)((c0 + e) / 4) * TILE);
                     y = make_float4(fmaf(z.x, down, y.x), fmaf(z.y, down, y.y), fmaf(z.z, down, y.z), fmaf(z.w, down, y.w));
                 }
-                *reinterpret_cast<float4*>(to + 4 + c0 + e) = y;
+                constexpr float F = 1.f / (1 << SUM_DROP);
+                *reinterpret_cast<float4*>(to + 4 + c0 + e) = make_float4(y.x * F, y.y * F, y.z * F, y.w * F);
             }
         }
     }

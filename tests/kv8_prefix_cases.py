@@ -16,7 +16,7 @@ def formula(q, k, v, scale, bf16, tokens):
     To the bound of pages that are not shared:  scores of shared ones have a query's f16 terms (2^-22 of a value, bf16 rows exactly; no step below 2^-38 of the row's largest) and a chain of at
     most 16 truncating sums of 2^-23: 2^-18.9 of the terms' magnitudes.  A weight times its value's scale has two f16 terms (2^-22 of itself) or, in bf16 rows, one (2^-11), and no
     step below 2^-24; what it is relative to is no more than 2^-7 times the largest of these products that the row sees, so that half a step is 2^-32 of that product (times 127, of the largest
-    weight times the largest element of its value), or of 2^-80 of the largest weight where all products are below.  2^-31.5: the reference's logarithm is approximate.  The products
+    weight times the largest element of its value), or of 2^-100 of the largest weight where all products are below.  2^-31.5: the reference's logarithm is approximate.  The products
     are summed in chunks of 64 (bf16 rows: 512) steps that round towards zero, 2^-23 each: 2^-17 (2^-14)."""
     want, parts = kc.attention(q, k, v, scale)
     tol = kc.bound(want, parts, bf16)
@@ -31,7 +31,7 @@ def formula(q, k, v, scale, bf16, tokens):
         peak[h] = (p / p.sum() * np.abs(v[:, h // group]).max(-1)).max()
     e = 2 * (terms * 2.0**-18.9 + full * 2.0**-38)[:, None] + 2.0**-18
     e = e + (2.0**-14 if bf16 else 2.0**-17)
-    return want, tol + mag * e + (tokens * (2.0**-31.5 * peak + 2.0**-105))[:, None] + (mag * 2.0**-11 if bf16 else 0)
+    return want, tol + mag * e + (tokens * (2.0**-31.5 * peak + 2.0**-125))[:, None] + (mag * 2.0**-11 if bf16 else 0)
 
 
 def check_rows(m, out, q, seq, pos, heads, scale, rows, seen=None):

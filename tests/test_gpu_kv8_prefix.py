@@ -156,6 +156,19 @@ def test_scores_of_any_size(hm, M, pages, sign, size, bf16):
     assert clear > 50
 
 
+@pytest.mark.parametrize("bf16", [False, True])
+@pytest.mark.parametrize("small", [-60, -80, -93, -99])
+@pytest.mark.parametrize("M,pages,own", [(400, 16, 0), (66, 130, 100)])
+def test_values_next_to_nothing(hm, M, pages, own, small, bf16):
+    """The smallest values that the cache holds keep their weights' bits."""
+    heads, S = 8, 64 * pages
+    m = Model(hm, pages, 2, 64, 64, [S + own] * 2, n_shared=pages)
+    for v in m.v:
+        v[:] = m.rng.standard_normal(v.shape).astype(np.float32) * np.float32(2.0**small)
+    refill(m)
+    attend(m, np.arange(M) % 2, S + own - 1 - np.arange(M), heads, bf16, some(M, 11), what="kv8 smallest values")
+
+
 # ---- what is not there, and what is not finite ----------------------------------------------------------
 
 
