@@ -127,7 +127,7 @@ def test_values_of_one_sign(hm, bf16, M, heads, dim, pages):
 
 @pytest.mark.parametrize("bf16", [False, True])
 @pytest.mark.parametrize("size", [1e5, 1e6, 1e7, 1e8, 1e9, 1e12, 1e20])
-@pytest.mark.parametrize("M,pages,sign", [(400, 16, 1), (66, 130, 1), (400, 16, -1)])
+@pytest.mark.parametrize("M,pages,sign", [(400, 16, 1), (66, 130, 1), (400, 16, -1), (2000, 40, 1)])
 def test_scores_of_any_size(hm, M, pages, sign, size, bf16):
     """Where one token's score is far above all others, by more than the scores' own roundings, the result is that token's value."""
     heads, S = 8, 64 * pages
