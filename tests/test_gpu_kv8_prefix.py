@@ -267,6 +267,51 @@ def test_strided_rows_at_any_address(hm, dim, vdim, offset, pad, M, pages, bf16)
     call.check(some(M, 6))
 
 
+@pytest.mark.parametrize("bf16,heads", [(False, 1024), (True, 128)])
+def test_the_most_rows(hm, bf16, heads):
+    """8192 rows, the most of a call; f32 sums behind the parts, beyond 32 bits of work memory."""
+    import torch
+
+    M, kvh, dim, pages = 8192, 2, 64, 21
+    m = Model(hm, 30, kvh, dim, dim, [64 * pages], n_shared=pages)
+    seq, pos = np.zeros(M, int), 64 * pages - 1 - np.arange(M) % 700
+    g = torch.Generator(device="cuda").manual_seed(1)
+    q = torch.randn(M, heads * dim, generator=g, device="cuda").to(torch.bfloat16 if bf16 else torch.float32)
+    q = q.view(torch.uint16).cpu().numpy() if bf16 else q.cpu().numpy()
+    call = OnDevice(m, heads, seq, pos, q, 0.125)
+    assert bf16 or call.size > 6 << 30
+    call.run()
+    torch.cuda.synchronize()
+    o = call.ob.view(M, -1)
+    at = some(M, 12, 6)
+    check_rows(m, torch.stack([o[int(r)] for r in at]).cpu().numpy(), q[at], seq[at], pos[at], heads, 0.125, np.arange(len(at)))
+    assert (call.work[-64:] == 255).all()
+
+
+@pytest.mark.parametrize("bf16", [False, True])
+def test_shared_pages_behind_four_gigabytes(hm, bf16):
+    kvh, dim, M, heads, n = 8, 128, 200, 16, 36000
+    size = hm.kv8_pool_bytes(kvh, dim, dim, n)
+    assert size > 4 << 30
+    pool = hm.DeviceBuffer(size)
+    shared = np.array([n - 1, 0, n // 2, n - 2, 35000, 1, 33333, 7], np.int32)
+    cache = hm.KV8Cache(kvh, dim, dim, pool.ptr, n, shared[None])
+    rng, S = np.random.default_rng(0), 64 * len(shared)
+    k, v = (rng.standard_normal((S, kvh * dim)).astype(np.float32) for _ in range(2))
+    cache.write(k, v, np.zeros(S), np.arange(S))
+    x = rng.standard_normal((M, heads * dim)).astype(np.float32)
+    q = bf16_bits(x) if bf16 else x
+    x = bf16_value(q) if bf16 else x
+    assert on_their_own(cache, M, heads, len(shared))
+    pos = S - 1 - np.arange(M)
+    out = cache.attend(q, np.zeros(M), pos, heads, dim**-0.5, shared=shared)
+    o = bf16_value(out) if bf16 else out
+    hk, hv = (kc.held(y.reshape(S, kvh, dim)).astype(np.float64) for y in (k, v))
+    for r in some(M, 13, 5):
+        want, tol = formula(x[r].astype(np.float64).reshape(heads, dim), hk[: pos[r] + 1], hv[: pos[r] + 1], dim**-0.5, bf16, pos[r] + 1)
+        assert (np.abs(o[r].reshape(heads, dim) - want) <= tol).all(), r
+
+
 # ---- streams and graphs ---------------------------------------------------------------------------------
 
 
