@@ -121,3 +121,36 @@ def test_values_next_to_nothing(hm, rows, width, small, bf16):
     pos = n - 1 - np.arange(rows)
     out = m.cache.attend(q, np.zeros(rows), pos, heads, 0.125)
     assert m.check(out, q, np.zeros(rows, int), pos, heads, 0.125) <= 1
+
+
+def test_calls_of_several_threads(hm):
+    """Host calls of four threads at once: writes, reads and attention of caches of their own, with and without shared pages."""
+    import threading
+
+    def work(seed, said):
+        try:
+            bf16, M, pages = seed % 2 == 1, 300, 22
+            m = Model(hm, seed, 2, 64, 64, [64 * pages + 40 * seed, 64 * pages], n_shared=pages)
+            seq, pos = np.arange(M) % 2, 64 * pages - 1 - np.arange(M)
+            pos[::2] = m.lens[0] - 1
+            q = m.queries(M, 8, bf16)
+            first = [m.cache.attend(q, seq, pos, 8, 0.125, shared=s) for s in (m.shared, None)]
+            for _ in range(6):
+                for s, want in zip((m.shared, None), first):
+                    np.testing.assert_array_equal(m.cache.attend(q, seq, pos, 8, 0.125, shared=s), want)
+                n = m.lens[0] - 64 * pages
+                if n:
+                    own = np.arange(64 * pages, m.lens[0])
+                    m.cache.write(m.k[0][own].reshape(n, -1), m.v[0][own].reshape(n, -1), np.zeros(n), own)
+                    np.testing.assert_array_equal(m.cache.read(np.zeros(n), own)[0].reshape(n, 2, 64), kc.held(m.k[0][own]))
+            said[seed] = True
+        except BaseException as e:  # told by the test's own thread
+            said[seed] = e
+
+    said = {}
+    threads = [threading.Thread(target=work, args=(i, said)) for i in range(4)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert [said[i] for i in range(4)] == [True] * 4
