@@ -18,9 +18,9 @@
 // done, where that leaves one part; others, and further parts, go to `work`, relative to their references, to be joined with the rows' own pages.
 //
 // What bounds it: the instructions of the softmax.  256 rows of 32 heads over 4 of 64 elements: the schedulers issue in 7 of 10 cycles; exponentials fill 2050 cycles of a block of 256 pairs, the tensor
-// cores 730; 116 us in all, 296 TFLOP/s.  A block took 4700 cycles and the whole 106 us while references followed scores alone: value scales in them cost one operation for two scores and the
+// cores 730; 117 us in all, 294 TFLOP/s.  A block took 4700 cycles and the whole 106 us while references followed scores alone: value scales in them cost one operation for two scores and the
 // loads of their logarithms (8 us), counting from an origin a vote per block (1.5 us).  With 128 elements a block takes 7000, as the only place for keys is converted (4000)
-// between two blocks' scores: 1021 rows of 12 heads, 90 us, the schedulers issue in 6 of 10.  Found slower, against 106 and 87 us: two places for keys and one for values (109 us for the
+// between two blocks' scores: 1021 rows of 12 heads, 91 us, the schedulers issue in 6 of 10.  Found slower, against 106 and 87 us: two places for keys and one for values (109 us for the
 // 1021 rows); a pass that finds no maximum and is done again where a score exceeds its reference by too much, which a quarter of the blocks does with heavy-tailed scores; all six converting
 // warps on keys, then on values (the 256 rows 117 us); a fourth warp for keys, which leaves 72 registers a thread (109 us there, 86 for the 1021 rows).
 #include <algorithm>
